@@ -244,6 +244,59 @@ hipError_t k_gdn_recur(const bf16_t *proj, int proj_stride, const float *conv_w,
                        float eps, int Hk, int Hv, bf16_t *y, const cujev_gdn_scratch *scratch,
                        int N, hipStream_t stream);
 
+/* ---- paged K/V cache (paged.hip, attention_paged.hip) ------------------------
+ * A pool of pages of 64 tokens that many sequences share, K and V of one layer:
+ * k [num_pages][Hkv][64][256], vt [num_pages][Hkv][256][64], bf16 or e4m3 with
+ * fp32 scales k_scale, v_scale [num_pages][Hkv][64] (a token and kv-head's row
+ * is its e4m3 values times a power of two). */
+#define CUJEV_KV_PAGE 64
+#define CUJEV_KV_BF16 0
+#define CUJEV_KV_E4M3 1
+typedef struct cujev_kv_pages {
+    void *k, *vt;
+    float *k_scale, *v_scale; /* CUJEV_KV_E4M3 only */
+    int num_pages, Hkv, type;
+} cujev_kv_pages;
+/* The sequences of one call: sequence b has rows q_start[b] .. q_start[b + 1]
+ * (its ql new tokens) and kv_len[b] keys, the new tokens' own last: row i of ql
+ * is at position kv_len[b] - ql + i, and position p in slot p % 64 of page
+ * page_table[b * max_pages + p / 64]. All device memory. The kernels cut
+ * lengths to the call's rows and the table, and skip page ids outside the
+ * pool. */
+typedef struct cujev_paged_seqs {
+    const int32_t *q_start, *kv_len, *page_table;
+    int max_pages, B;
+} cujev_paged_seqs;
+/* Whether the pool's pointers, alignment and type are usable. */
+int cujev_kv_pages_ok(const cujev_kv_pages *pages);
+
+/* k_attn_prep with K and V written into pages: rows, norms, RoPE (pos[n], cut
+ * to the table's npos positions) and q_out as there, for any Hq / Hkv; rot 8,
+ * 16, 32 or 64. Rows of no sequence are left alone. */
+hipError_t k_attn_prep_paged(const bf16_t *proj, int proj_stride, const float *q_norm_w,
+                             const float *k_norm_w, const int32_t *pos,
+                             const cujev_paged_seqs *seqs, int N, int Hq, int rot,
+                             const float *rope_table, int npos, float eps, float q_scale,
+                             bf16_t *q_out, const cujev_kv_pages *pages, hipStream_t stream);
+/* Columns [0, min(kv_len[b], max_kv)) of the caches k_cache [B][Hkv][stride][256]
+ * and vt_cache [B][Hkv][256][stride] from the sequences' pages (exact in bf16;
+ * zeros for a page id outside the pool). q_start is not read. */
+hipError_t k_kv_page_read(const cujev_kv_pages *pages, const cujev_paged_seqs *seqs, int max_kv,
+                          bf16_t *k_cache, bf16_t *vt_cache, int cache_stride,
+                          hipStream_t stream);
+/* Attention of the sequences' rows over their pages: row (n, h) at position p
+ * sees keys j <= p with window == 0 or j > p - window or j < sinks;
+ *   out[n, h*256 + d] = sigmoid(gate) * softmax2_j(q[n, h] . k_j) v_j
+ * (gate NULL: no gate; no key: 0), q bf16 [N][Hq][256] scaled as for
+ * k_attention. max_q and max_kv bound ql and kv_len. */
+hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int gate_tok_stride,
+                             int gate_head_stride, const cujev_kv_pages *pages,
+                             const cujev_paged_seqs *seqs, int N, int max_q, int max_kv, int Hq,
+                             int window, int sinks, bf16_t *out, void *ws, size_t ws_bytes,
+                             hipStream_t stream);
+size_t cujev_attention_paged_ws_bytes(int N, int B, int max_q, int max_kv, int Hq, int Hkv,
+                                      int window, int sinks, int type);
+
 /* ---- per-layer glue --------------------------------------------------------
  * x[N,H] fp32 residual = E[tokens] (bf16 table).  REF elementwise.cu:3-11. */
 hipError_t k_embed(const int32_t *tokens, const bf16_t *E, float *x, int N, int H, hipStream_t s);

@@ -295,6 +295,131 @@ EXPORT int cujev_op_attention_noalloc(const void *q, const void *gate, int gate_
                     "attention_noalloc");
 }
 
+/* ---- paged K/V cache ------------------------------------------------------ */
+static_assert(CUJEV_OPS_KV_PAGE == CUJEV_KV_PAGE && CUJEV_OPS_KV_BF16 == CUJEV_KV_BF16 &&
+                  CUJEV_OPS_KV_E4M3 == CUJEV_KV_E4M3,
+              "one definition of a page");
+
+static int paged_check(const char *what, const cujev_kv_pages *pages, const int32_t *page_table,
+                       int max_pages, const int32_t *kv_len, int B) {
+    if (!cujev_kv_pages_ok(pages))
+        return fail(1, "%s: bad page pool (type %d, %d pages, %d kv-heads; pointers set and "
+                       "16-byte aligned, scales with e4m3)",
+                    what, pages->type, pages->num_pages, pages->Hkv);
+    if (B < 0 || max_pages <= 0 || max_pages > 0x7fffffff / CUJEV_KV_PAGE ||
+        (B > 0 && (!page_table || !kv_len)))
+        return fail(1, "%s: bad page table (B=%d, max_pages=%d)", what, B, max_pages);
+    return 0;
+}
+
+/* Heads of q: a multiple of the kv-heads, at most 16 per kv-head. */
+static int paged_heads_ok(int Hq, int Hkv) {
+    return Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Hq / Hkv <= 16;
+}
+
+EXPORT int cujev_op_attn_prep_paged(const void *proj, int proj_stride, const float *q_norm_w,
+                                    const float *k_norm_w, const int32_t *pos,
+                                    const int32_t *q_start, const int32_t *kv_len,
+                                    const int32_t *page_table, int max_pages, int B, int N, int Hq,
+                                    int Hkv, int rot, const float *rope_table, int npos, float eps,
+                                    float q_scale, void *q_out, int kv_type, void *k_pages,
+                                    void *vt_pages, float *k_scale, float *v_scale, int num_pages,
+                                    void *stream) {
+    const cujev_kv_pages pages = {k_pages, vt_pages, k_scale, v_scale, num_pages, Hkv, kv_type};
+    const int st = paged_check("attn_prep_paged", &pages, page_table, max_pages, kv_len, B);
+    if (st != 0)
+        return st;
+    if (N < 0 || !paged_heads_ok(Hq, Hkv) || (rot != 8 && rot != 16 && rot != 32 && rot != 64) ||
+        npos <= 0)
+        return fail(1, "attn_prep_paged: unsupported shape N=%d Hq=%d Hkv=%d rot=%d npos=%d", N,
+                    Hq, Hkv, rot, npos);
+    if (N > 0 && B > 0 &&
+        (!proj || !q_norm_w || !k_norm_w || !pos || !q_start || !rope_table || !q_out))
+        return fail(1, "attn_prep_paged: null argument");
+    if (proj_stride < Hq * 512 + Hkv * 512 || proj_stride % 4 || ((uintptr_t)proj & 7) ||
+        ((uintptr_t)q_out & 7))
+        return fail(1, "attn_prep_paged: rows must be 8-byte aligned and hold %d values",
+                    Hq * 512 + Hkv * 512);
+    if (((uintptr_t)q_norm_w | (uintptr_t)k_norm_w | (uintptr_t)rope_table) & 15)
+        return fail(1, "attn_prep_paged: weights and RoPE table must be 16-byte aligned");
+    const cujev_paged_seqs seqs = {q_start, kv_len, page_table, max_pages, B};
+    return launched(k_attn_prep_paged((const bf16_t *)proj, proj_stride, q_norm_w, k_norm_w, pos,
+                                      &seqs, N, Hq, rot, rope_table, npos, eps, q_scale,
+                                      (bf16_t *)q_out, &pages, (hipStream_t)stream),
+                    "attn_prep_paged");
+}
+
+EXPORT int cujev_op_kv_page_read(int kv_type, const void *k_pages, const void *vt_pages,
+                                 const float *k_scale, const float *v_scale, int num_pages,
+                                 const int32_t *page_table, int max_pages, const int32_t *kv_len,
+                                 int B, int max_kv, int Hkv, void *k_cache, void *vt_cache,
+                                 int cache_stride, void *stream) {
+    const cujev_kv_pages pages = {(void *)k_pages, (void *)vt_pages, (float *)k_scale,
+                                  (float *)v_scale, num_pages, Hkv, kv_type};
+    const int st = paged_check("kv_page_read", &pages, page_table, max_pages, kv_len, B);
+    if (st != 0)
+        return st;
+    if (max_kv < 0 || max_kv > max_pages * CUJEV_KV_PAGE)
+        return fail(1, "kv_page_read: max_kv=%d is not within the table's %d tokens", max_kv,
+                    max_pages * CUJEV_KV_PAGE);
+    if (cache_stride % 64 || cache_stride < cujev_kv_stride(max_kv))
+        return fail(1, "kv_page_read: cache stride %d, need a multiple of 64 of at least %d",
+                    cache_stride, cujev_kv_stride(max_kv));
+    if (B > 0 && (!k_cache || !vt_cache || (((uintptr_t)k_cache | (uintptr_t)vt_cache) & 15)))
+        return fail(1, "kv_page_read: caches must be set and 16-byte aligned");
+    const cujev_paged_seqs seqs = {nullptr, kv_len, page_table, max_pages, B};
+    return launched(k_kv_page_read(&pages, &seqs, max_kv, (bf16_t *)k_cache, (bf16_t *)vt_cache,
+                                   cache_stride, (hipStream_t)stream),
+                    "kv_page_read");
+}
+
+EXPORT int cujev_op_attention_paged(const void *q, const void *gate, int gate_tok_stride,
+                                    int gate_head_stride, int kv_type, const void *k_pages,
+                                    const void *vt_pages, const float *k_scale,
+                                    const float *v_scale, int num_pages, const int32_t *q_start,
+                                    const int32_t *kv_len, const int32_t *page_table,
+                                    int max_pages, int B, int N, int max_q, int max_kv, int Hq,
+                                    int Hkv, int window, int sinks, void *out, void *ws,
+                                    size_t ws_bytes, void *stream) {
+    const cujev_kv_pages pages = {(void *)k_pages, (void *)vt_pages, (float *)k_scale,
+                                  (float *)v_scale, num_pages, Hkv, kv_type};
+    const int st = paged_check("attention_paged", &pages, page_table, max_pages, kv_len, B);
+    if (st != 0)
+        return st;
+    if (N < 0 || max_q < 0 || max_kv < 0 || !paged_heads_ok(Hq, Hkv))
+        return fail(1, "attention_paged: unsupported shape N=%d max_q=%d max_kv=%d Hq=%d Hkv=%d",
+                    N, max_q, max_kv, Hq, Hkv);
+    if (max_kv > max_pages * CUJEV_KV_PAGE)
+        return fail(1, "attention_paged: max_kv=%d is not within the table's %d tokens", max_kv,
+                    max_pages * CUJEV_KV_PAGE);
+    if (window < 0 || sinks < 0 || (sinks > 0 && window == 0))
+        return fail(1, "attention_paged: window=%d sinks=%d (sinks go with a window)", window,
+                    sinks);
+    if (N > 0 && B > 0 && (!q || !q_start || !out))
+        return fail(1, "attention_paged: null argument");
+    if ((((uintptr_t)q | (uintptr_t)out) & 15) || ((uintptr_t)gate & 7) ||
+        (gate && (gate_tok_stride % 4 || gate_head_stride % 4)))
+        return fail(1, "attention_paged: q and out must be 16-byte, gate rows 8-byte aligned");
+    const size_t need = cujev_attention_paged_ws_bytes(N, B, max_q, max_kv, Hq, Hkv, window, sinks,
+                                                       kv_type);
+    if (need > 0 && (!ws || ((uintptr_t)ws & 15) || ws_bytes < need))
+        return fail(6, "attention_paged: needs a 16-byte aligned workspace of %zu bytes, got %zu",
+                    need, ws ? ws_bytes : (size_t)0);
+    const cujev_paged_seqs seqs = {q_start, kv_len, page_table, max_pages, B};
+    return launched(k_attention_paged((const bf16_t *)q, (const bf16_t *)gate, gate_tok_stride,
+                                      gate_head_stride, &pages, &seqs, N, max_q, max_kv, Hq,
+                                      window, sinks, (bf16_t *)out, ws, ws_bytes,
+                                      (hipStream_t)stream),
+                    "attention_paged");
+}
+
+EXPORT size_t cujev_ops_attention_paged_ws_bytes(int N, int B, int max_q, int max_kv, int Hq,
+                                                 int Hkv, int window, int sinks, int kv_type) {
+    if (!paged_heads_ok(Hq, Hkv))
+        return 0;
+    return cujev_attention_paged_ws_bytes(N, B, max_q, max_kv, Hq, Hkv, window, sinks, kv_type);
+}
+
 EXPORT int cujev_op_gdn_conv_prep(const void *proj, int proj_stride, const float *conv_w,
                                   const float *conv_in, float *conv_out, int seg0_len,
                                   const int32_t *own_base, const float *A_neg_exp,

@@ -1,0 +1,369 @@
+/* The paged K/V cache of gfx950: new tokens into pages (norm, RoPE, e4m3
+ * quantisation), and pages back into a state's contiguous caches. The
+ * reference has one contiguous bf16 cache per state (src/engine/model.h:60-72)
+ * and neither operator. */
+#include "paged.h"
+
+namespace CUJEV_KNS {
+namespace {
+
+/* ---- new tokens into pages ---------------------------------------------------
+ * Two kinds of wave in one launch. A row wave normalises TOK tokens' rows of
+ * one q-head or K head, lane l holding dims 4l .. 4l + 3, as attn_prep does:
+ *   y = x rsqrt(mean x^2 + eps) w, RoPE (dim i with i + rot/2, lane l with
+ *   l ^ rot/8), q times q_scale.
+ * A V wave takes the tokens of one aligned group of 16 positions and one
+ * kv-head: the group's V^T rows are whole 16-byte (e4m3) or 32-byte pieces, so
+ * the transpose needs neither LDS nor another wave's data: lane l holds 16
+ * tokens of dims 4l .. 4l + 3 and stores one piece per dim. */
+constexpr int VTOK = 16;
+
+template <bool E4M3, int TOK>
+__global__ __launch_bounds__(256) void prep_paged_kernel(
+    const bf16 *__restrict__ proj, int ps, const float *__restrict__ qw,
+    const float *__restrict__ kw, const int32_t *__restrict__ pos,
+    const int32_t *__restrict__ q_start, const int32_t *__restrict__ kv_len,
+    const int32_t *__restrict__ page_table, int max_pages, int B, int N, int Hq, int Hkv, int rot,
+    const float2 *__restrict__ rope, int npos, float eps, float q_scale, bf16 *__restrict__ q_out,
+    void *__restrict__ k_pages, void *__restrict__ vt_pages, float *__restrict__ k_scale,
+    float *__restrict__ v_scale, int num_pages, int row_blocks, int groups) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if ((int)blockIdx.x < row_blocks) {
+        const int heads = Hq + Hkv, unit = blockIdx.x * 4 + wave;
+        const int head = unit % heads, n0 = unit / heads * TOK;
+        if (n0 >= N)
+            return;
+        const bool is_k = head >= Hq;
+        const float *w = is_k ? kw : qw;
+        const bf16 *src = proj + (is_k ? Hq * 512 + (head - Hq) * 256 : head * 512) + 4 * lane;
+        const int half_lanes = rot / 8;
+        const bool rotates = lane < 2 * half_lanes, first = lane < half_lanes;
+        const int fi0 = rotates ? (first ? 4 * lane : 4 * lane - rot / 2) : 0;
+        /* every load before any arithmetic, token indices clamped */
+        bf16x4 raw[TOK];
+#pragma unroll
+        for (int t = 0; t < TOK; t++)
+            raw[t] = *(const bf16x4 *)(src + (size_t)min(n0 + t, N - 1) * ps);
+        const float4 wl = *(const float4 *)(w + 4 * lane);
+        float4 rc[TOK][2];
+#pragma unroll
+        for (int t = 0; t < TOK; t++) {
+            const int p = min(max(pos[min(n0 + t, N - 1)], 0), npos - 1);
+            const float4 *r = (const float4 *)(rope + (size_t)p * (rot / 2) + fi0);
+            rc[t][0] = r[0];
+            rc[t][1] = r[1];
+        }
+#pragma unroll
+        for (int t = 0; t < TOK; t++) {
+            const int n = n0 + t;
+            if (n >= N)
+                continue;
+            float x[4], ss = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                x[e] = bf2f(raw[t][e]);
+                ss += x[e] * x[e];
+            }
+            const float rinv = rsqrtf(wave_sum(ss) * (1.f / 256.f) + eps);
+            x[0] = x[0] * rinv * wl.x;
+            x[1] = x[1] * rinv * wl.y;
+            x[2] = x[2] * rinv * wl.z;
+            x[3] = x[3] * rinv * wl.w;
+            float other[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                other[e] = __shfl_xor(x[e], half_lanes, 64);
+            if (rotates) {
+                const float cz[8] = {rc[t][0].x, rc[t][0].y, rc[t][0].z, rc[t][0].w,
+                                     rc[t][1].x, rc[t][1].y, rc[t][1].z, rc[t][1].w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float c = cz[2 * e], sn = cz[2 * e + 1];
+                    x[e] = first ? x[e] * c - other[e] * sn : x[e] * c + other[e] * sn;
+                }
+            }
+            const int b = find_seq(q_start, B, n);
+            if (b < 0) /* no sequence's row */
+                continue;
+            if (!is_k) {
+                const bf16x4 o = {f2bf(x[0] * q_scale), f2bf(x[1] * q_scale),
+                                  f2bf(x[2] * q_scale), f2bf(x[3] * q_scale)};
+                *(bf16x4 *)(q_out + ((size_t)n * Hq + head) * 256 + 4 * lane) = o;
+                continue;
+            }
+            const Seq s = load_seq(q_start, kv_len, b, N, max_pages);
+            const int p = s.p0 + (n - s.q0);
+            if ((unsigned)(n - s.q0) >= (unsigned)s.ql || p < 0 || p >= s.kv)
+                continue;
+            const int page = page_table[(size_t)b * max_pages + p / PG];
+            if (page < 0 || page >= num_pages)
+                continue;
+            const size_t row = ((size_t)page * Hkv + head - Hq) * PG + p % PG;
+            if constexpr (E4M3) {
+                const float a = wave_max(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])),
+                                               fmaxf(fabsf(x[2]), fabsf(x[3]))));
+                const int e = e4m3_exp(a);
+                const float inv = exp2_int(-e);
+                ((uint32_t *)k_pages)[row * 64 + lane] =
+                    pack_e4m3(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+                if (lane == 0)
+                    k_scale[row] = exp2_int(e);
+            } else {
+                const bf16x4 o = {f2bf(x[0]), f2bf(x[1]), f2bf(x[2]), f2bf(x[3])};
+                *(bf16x4 *)((bf16 *)k_pages + row * 256 + 4 * lane) = o;
+            }
+        }
+        return;
+    }
+
+    /* ---- V ---- */
+    const int unit = (blockIdx.x - row_blocks) * 4 + wave;
+    if (unit >= groups * Hkv)
+        return;
+    const int kh = unit % Hkv;
+    Seq s;
+    int g;
+    const int b = find_item(
+        q_start, kv_len, B, N, max_pages, unit / Hkv,
+        [](const Seq &q) {
+            const int lo = max(q.p0, 0), hi = min(q.p0 + q.ql, q.kv);
+            return hi > lo ? (hi - 1) / VTOK - lo / VTOK + 1 : 0;
+        },
+        &s, &g);
+    if (b < 0)
+        return;
+    const int base = (max(s.p0, 0) / VTOK + g) * VTOK; /* the group's first position */
+    const int page = page_table[(size_t)b * max_pages + base / PG];
+    if (page < 0 || page >= num_pages)
+        return;
+    const int lo = max(s.p0, base), hi = min(min(s.p0 + s.ql, s.kv), base + VTOK);
+    const bf16 *src = proj + Hq * 512 + Hkv * 256 + kh * 256 + 4 * lane;
+    bf16x4 v[VTOK];
+#pragma unroll
+    for (int t = 0; t < VTOK; t++) {
+        const int p = min(max(base + t, lo), hi - 1);
+        v[t] = *(const bf16x4 *)(src + (size_t)(s.q0 + p - s.p0) * ps);
+    }
+    const size_t head = (size_t)page * Hkv + kh;
+    const int col = base % PG;
+    const bool whole = hi - lo == VTOK;
+    if constexpr (E4M3) {
+        /* max of each token over the wave: lanes that meet exchange the halves
+         * they give up (16 -> 8 -> 4 -> 2 -> 1 tokens a lane), so lane l ends
+         * with token l >> 2 */
+        float m[VTOK];
+#pragma unroll
+        for (int t = 0; t < VTOK; t++)
+            m[t] = fmaxf(fmaxf(fabsf(bf2f(v[t][0])), fabsf(bf2f(v[t][1]))),
+                         fmaxf(fabsf(bf2f(v[t][2])), fabsf(bf2f(v[t][3]))));
+#pragma unroll
+        for (int half = VTOK / 2, o = 32; half >= 1; half >>= 1, o >>= 1) {
+            const bool upper = lane & o;
+#pragma unroll
+            for (int t = 0; t < half; t++) {
+                const float mine = upper ? m[t + half] : m[t], give = upper ? m[t] : m[t + half];
+                m[t] = fmaxf(mine, __shfl_xor(give, o, 64));
+            }
+        }
+        m[0] = fmaxf(m[0], __shfl_xor(m[0], 2, 64));
+        m[0] = fmaxf(m[0], __shfl_xor(m[0], 1, 64));
+        const int e = e4m3_exp(m[0]), tok = lane >> 2;
+        if ((lane & 3) == 0 && base + tok >= lo && base + tok < hi)
+            v_scale[head * PG + col + tok] = exp2_int(e);
+        float inv[VTOK];
+#pragma unroll
+        for (int t = 0; t < VTOK; t++)
+            inv[t] = exp2_int(-__builtin_amdgcn_readlane(e, 4 * t));
+        uint8_t *dst = (uint8_t *)vt_pages + head * PSLICE + (size_t)4 * lane * PG + col;
+#pragma unroll
+        for (int d = 0; d < 4; d++) {
+            u32x4 q;
+#pragma unroll
+            for (int w = 0; w < 4; w++)
+                q[w] = pack_e4m3(bf2f(v[4 * w][d]) * inv[4 * w],
+                                 bf2f(v[4 * w + 1][d]) * inv[4 * w + 1],
+                                 bf2f(v[4 * w + 2][d]) * inv[4 * w + 2],
+                                 bf2f(v[4 * w + 3][d]) * inv[4 * w + 3]);
+            if (whole) {
+                *(u32x4 *)(dst + d * PG) = q;
+            } else {
+#pragma unroll
+                for (int t = 0; t < VTOK; t++)
+                    if (base + t >= lo && base + t < hi)
+                        dst[d * PG + t] = (uint8_t)(q[t >> 2] >> (8 * (t & 3)));
+            }
+        }
+    } else {
+        bf16 *dst = (bf16 *)vt_pages + head * PSLICE + (size_t)4 * lane * PG + col;
+#pragma unroll
+        for (int d = 0; d < 4; d++) {
+            if (whole) {
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    bf16x8 q;
+#pragma unroll
+                    for (int t = 0; t < 8; t++)
+                        q[t] = v[8 * w + t][d];
+                    *(bf16x8 *)(dst + d * PG + 8 * w) = q;
+                }
+            } else {
+#pragma unroll
+                for (int t = 0; t < VTOK; t++)
+                    if (base + t >= lo && base + t < hi)
+                        dst[d * PG + t] = v[t][d];
+            }
+        }
+    }
+}
+
+/* ---- pages back into a state's caches -----------------------------------------
+ * One workgroup per (sequence, page, kv-head, K or V^T): 64 rows of 512 bytes
+ * or 256 rows of 128 out, 16 values a thread and step. A page id outside the
+ * pool reads as zeros; columns from kv_len on stay as they were. */
+template <bool E4M3>
+__global__ __launch_bounds__(256) void page_read_kernel(
+    const void *__restrict__ k_pages, const void *__restrict__ vt_pages,
+    const float *__restrict__ k_scale, const float *__restrict__ v_scale, int num_pages,
+    const int32_t *__restrict__ page_table, int max_pages, const int32_t *__restrict__ kv_len,
+    int max_kv, int Hkv, bf16 *__restrict__ kc, bf16 *__restrict__ vtc, int stride) {
+    const int j = blockIdx.x >> 1, b = blockIdx.z, kh = blockIdx.y, tid = threadIdx.x;
+    const int kv = min(kv_len[b], max_kv), left = kv - j * PG; /* tokens of this page */
+    if (left <= 0)
+        return;
+    const int page = page_table[(size_t)b * max_pages + j];
+    const bool ok = page >= 0 && page < num_pages;
+    const size_t head = (size_t)(ok ? page : 0) * Hkv + kh;
+    const size_t out = ((size_t)b * Hkv + kh) * PD * (size_t)stride;
+    if ((blockIdx.x & 1) == 0) { /* K: 16 dims a thread, 16 rows a step */
+        bf16 *dst = kc + out + (size_t)j * PG * PD;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int row = 16 * i + (tid >> 4), at = row * PD + (tid & 15) * 16;
+            bf16x8 r[2] = {};
+            if constexpr (E4M3) {
+                const u32x4 v = *(const u32x4 *)((const uint8_t *)k_pages + head * PSLICE + at);
+                const float sc = k_scale[head * PG + row];
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    const bf16x2 a = unpack_e4m3<false>(v[w], sc), c = unpack_e4m3<true>(v[w], sc);
+                    r[w >> 1][4 * (w & 1)] = a[0], r[w >> 1][4 * (w & 1) + 1] = a[1];
+                    r[w >> 1][4 * (w & 1) + 2] = c[0], r[w >> 1][4 * (w & 1) + 3] = c[1];
+                }
+            } else {
+                const bf16x8 *v = (const bf16x8 *)((const bf16 *)k_pages + head * PSLICE + at);
+                r[0] = v[0], r[1] = v[1];
+            }
+            if (!ok)
+                r[0] = r[1] = bf16x8{};
+            if (row < left) {
+                *(bf16x8 *)(dst + at) = r[0];
+                *(bf16x8 *)(dst + at + 8) = r[1];
+            }
+        }
+        return;
+    }
+    /* V^T: 16 tokens a thread, 64 rows a step */
+    const int t0 = (tid & 3) * 16;
+    float sc[16];
+    if constexpr (E4M3) {
+#pragma unroll
+        for (int t = 0; t < 16; t += 4) {
+            const float4 s4 = *(const float4 *)(v_scale + head * PG + t0 + t);
+            sc[t] = s4.x, sc[t + 1] = s4.y, sc[t + 2] = s4.z, sc[t + 3] = s4.w;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int d = 64 * i + (tid >> 2);
+        bf16x8 r[2] = {};
+        if constexpr (E4M3) {
+            const u32x4 v =
+                *(const u32x4 *)((const uint8_t *)vt_pages + head * PSLICE + d * PG + t0);
+#pragma unroll
+            for (int t = 0; t < 16; t++) {
+                const bf16x2 p = t & 2 ? unpack_e4m3<true>(v[t >> 2], 1.f)
+                                       : unpack_e4m3<false>(v[t >> 2], 1.f);
+                r[t >> 3][t & 7] = f2bf(bf2f(p[t & 1]) * sc[t]);
+            }
+        } else {
+            const bf16x8 *v = (const bf16x8 *)((const bf16 *)vt_pages + head * PSLICE + d * PG + t0);
+            r[0] = v[0], r[1] = v[1];
+        }
+        if (!ok)
+            r[0] = r[1] = bf16x8{};
+        bf16 *dst = vtc + out + (size_t)d * stride + j * PG + t0;
+        if (t0 + 16 <= left) {
+            *(bf16x8 *)dst = r[0];
+            *(bf16x8 *)(dst + 8) = r[1];
+        } else {
+#pragma unroll
+            for (int t = 0; t < 16; t++)
+                if (t0 + t < left)
+                    dst[t] = r[t >> 3][t & 7];
+        }
+    }
+}
+
+} // namespace
+} // namespace CUJEV_KNS
+using namespace CUJEV_KNS;
+
+extern "C" int cujev_kv_pages_ok(const cujev_kv_pages *p) {
+    const uintptr_t at = (uintptr_t)p->k | (uintptr_t)p->vt;
+    if (!p->k || !p->vt || (at & 15) || p->num_pages <= 0 || p->Hkv <= 0 ||
+        (p->type != CUJEV_KV_BF16 && p->type != CUJEV_KV_E4M3))
+        return 0;
+    return p->type == CUJEV_KV_BF16 ||
+           (p->k_scale && p->v_scale && !(((uintptr_t)p->k_scale | (uintptr_t)p->v_scale) & 15));
+}
+
+extern "C" hipError_t k_attn_prep_paged(const bf16_t *proj, int proj_stride, const float *q_norm_w,
+                                        const float *k_norm_w, const int32_t *pos,
+                                        const cujev_paged_seqs *seqs, int N, int Hq, int rot,
+                                        const float *rope_table, int npos, float eps,
+                                        float q_scale, bf16_t *q_out, const cujev_kv_pages *pages,
+                                        hipStream_t stream) {
+    const int Hkv = pages->Hkv, B = seqs->B;
+    if (N <= 0 || B <= 0)
+        return hipSuccess;
+    const long long units = (long long)CEIL_DIV(N, 4) * (Hq + Hkv);
+    const long long groups = N < N / VTOK + 2ll * B ? N : N / VTOK + 2ll * B;
+    const long long row_blocks = CEIL_DIV(units, 4), v_blocks = CEIL_DIV(groups * Hkv, 4);
+    if (row_blocks + v_blocks > 0x7fffffff || groups * Hkv > 0x7fffffff)
+        return hipErrorInvalidValue;
+#define LAUNCH(T)                                                                                 \
+    hipLaunchKernelGGL((prep_paged_kernel<T, 4>), dim3((unsigned)(row_blocks + v_blocks)),        \
+                       dim3(256), 0, stream, (const bf16 *)proj, proj_stride, q_norm_w, k_norm_w, \
+                       pos, seqs->q_start, seqs->kv_len, seqs->page_table, seqs->max_pages, B, N, \
+                       Hq, Hkv, rot, (const float2 *)rope_table, npos, eps, q_scale,              \
+                       (bf16 *)q_out, pages->k, pages->vt, pages->k_scale, pages->v_scale,        \
+                       pages->num_pages, (int)row_blocks, (int)groups)
+    if (pages->type == CUJEV_KV_E4M3)
+        LAUNCH(true);
+    else
+        LAUNCH(false);
+#undef LAUNCH
+    return hipGetLastError();
+}
+
+extern "C" hipError_t k_kv_page_read(const cujev_kv_pages *pages, const cujev_paged_seqs *seqs,
+                                     int max_kv, bf16_t *k_cache, bf16_t *vt_cache,
+                                     int cache_stride, hipStream_t stream) {
+    if (seqs->B <= 0 || max_kv <= 0)
+        return hipSuccess;
+    const int n = CEIL_DIV(max_kv, PG);
+    if (n > seqs->max_pages || seqs->B > 65535 || pages->Hkv > 65535)
+        return hipErrorInvalidValue;
+    const dim3 grid(2u * n, (unsigned)pages->Hkv, (unsigned)seqs->B);
+#define LAUNCH(T)                                                                                 \
+    hipLaunchKernelGGL(page_read_kernel<T>, grid, dim3(256), 0, stream, pages->k, pages->vt,      \
+                       pages->k_scale, pages->v_scale, pages->num_pages, seqs->page_table,        \
+                       seqs->max_pages, seqs->kv_len, max_kv, pages->Hkv, (bf16 *)k_cache,        \
+                       (bf16 *)vt_cache, cache_stride)
+    if (pages->type == CUJEV_KV_E4M3)
+        LAUNCH(true);
+    else
+        LAUNCH(false);
+#undef LAUNCH
+    return hipGetLastError();
+}

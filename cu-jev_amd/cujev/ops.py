@@ -42,6 +42,17 @@ _SIGS = {
     # Na, Pa, oka, ovta, oa_stride, Nb, Pb, okb, ovtb, ob_stride, stream
     "cujev_op_attention_pair": [_P, _P, _I, _I, _P, _P, _I, _P, _P, _I, _I, _I, _I, _P, _P, _I,
                                 _I, _I, _P, _P, _I, _P],
+    # proj, stride, qw, kw, pos, q_start, kv_len, page_table, max_pages, B, N, Hq, Hkv, rot, rope,
+    # npos, eps, q_scale, q_out, kv_type, k, vt, k_scale, v_scale, num_pages, stream
+    "cujev_op_attn_prep_paged": [_P, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _I,
+                                 _F, _F, _P, _I, _P, _P, _P, _P, _I, _P],
+    # kv_type, k, vt, k_scale, v_scale, num_pages, page_table, max_pages, kv_len, B, max_kv, Hkv,
+    # k_cache, vt_cache, stride, stream
+    "cujev_op_kv_page_read": [_I, _P, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _P, _P, _I, _P],
+    # q, gate, gts, ghs, kv_type, k, vt, k_scale, v_scale, num_pages, q_start, kv_len, page_table,
+    # max_pages, B, N, max_q, max_kv, Hq, Hkv, window, sinks, out, ws, ws_bytes, stream
+    "cujev_op_attention_paged": [_P, _P, _I, _I, _I, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I,
+                                 _I, _I, _I, _I, _I, _I, _P, _P, C.c_size_t, _P],
     "cujev_op_gdn_conv_prep": [_P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _P, _P, _P, _P,
                                _P, _P],
     "cujev_op_gemm_small": [_P, _I, _P, _I, _I, _I, _I, _I, _P, _I, _P, _P],
@@ -82,6 +93,8 @@ def load():
         plan.restype = _I
     lib.cujev_ops_attention_ws_bytes.argtypes = [_I, _I, _I, _I]
     lib.cujev_ops_attention_ws_bytes.restype = C.c_size_t
+    lib.cujev_ops_attention_paged_ws_bytes.argtypes = [_I] * 9
+    lib.cujev_ops_attention_paged_ws_bytes.restype = C.c_size_t
     lib.cujev_ops_blaslt_version.argtypes = []
     lib.cujev_ops_blaslt_version.restype = _I
     lib.cujev_op_gemm_tune.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, _I, _I, _I, _I,
@@ -99,7 +112,8 @@ def load():
 def exported_symbols():
     return ["cujev_ops_kv_stride", "cujev_ops_last_error", "cujev_ops_gdn_scratch_bytes",
             "cujev_ops_gemm_small_splits", "cujev_ops_gemm_plan", "cujev_ops_gemm_wide_plan",
-            "cujev_ops_attention_ws_bytes", "cujev_ops_blaslt_version", "cujev_op_gemm_tune", *_SIGS]
+            "cujev_ops_attention_ws_bytes", "cujev_ops_attention_paged_ws_bytes",
+            "cujev_ops_blaslt_version", "cujev_op_gemm_tune", *_SIGS]
 
 
 def _ptr(t):
@@ -191,6 +205,151 @@ def attention_noalloc(q, gate, gate_tok_stride, gate_head_stride, pk, pvt, P, p_
     _call("cujev_op_attention_noalloc", _ptr(q), _ptr(gate), gate_tok_stride, gate_head_stride,
           _ptr(pk), _ptr(pvt), int(P), p_stride, _ptr(ok), _ptr(ovt), o_stride, _ptr(own_base),
           N, Hq, Hkv, _ptr(out), _stream())
+
+
+KV_PAGE = 64  # tokens a page
+
+
+class KvPages:
+    """A layer's page pool: k [pages, Hkv, 64, 256] and vt [pages, Hkv, 256, 64],
+    both bf16, or both float8_e4m3fn with float32 scales k_scale, v_scale
+    [pages, Hkv, 64] (powers of two). The tensors are the caller's; kv_pages()
+    makes new ones."""
+
+    __slots__ = ("k", "vt", "k_scale", "v_scale", "num_pages", "Hkv", "e4m3", "args")
+
+    def __init__(self, k, vt, k_scale=None, v_scale=None):
+        import torch
+        self.e4m3 = k.dtype == torch.float8_e4m3fn
+        if k.dim() != 4 or k.shape[2:] != (KV_PAGE, 256):
+            raise OpsError(f"KvPages: k is {tuple(k.shape)}, not [pages, Hkv, {KV_PAGE}, 256]")
+        self.num_pages, self.Hkv = k.shape[0], k.shape[1]
+        want = (self.num_pages, self.Hkv)
+        if not self.e4m3 and k.dtype != torch.bfloat16:
+            raise OpsError(f"KvPages: pages are bfloat16 or float8_e4m3fn, not {k.dtype}")
+        _need("vt", vt, k.dtype, k.device, want + (256, KV_PAGE))
+        _need("k", k, k.dtype, k.device, want + (KV_PAGE, 256))
+        if self.e4m3:
+            _need("k_scale", k_scale, torch.float32, k.device, want + (KV_PAGE,))
+            _need("v_scale", v_scale, torch.float32, k.device, want + (KV_PAGE,))
+        elif k_scale is not None or v_scale is not None:
+            raise OpsError("KvPages: bfloat16 pages have no scales")
+        self.k, self.vt, self.k_scale, self.v_scale = k, vt, k_scale, v_scale
+        # kv_type, k, vt, k_scale, v_scale, num_pages of the C calls
+        self.args = (int(self.e4m3), k.data_ptr(), vt.data_ptr(),
+                     k_scale.data_ptr() if self.e4m3 else None,
+                     v_scale.data_ptr() if self.e4m3 else None, self.num_pages)
+
+
+def kv_pages(num_pages, Hkv, e4m3=False, device="cuda"):
+    """A zeroed KvPages pool."""
+    import torch
+    t = torch.float8_e4m3fn if e4m3 else torch.bfloat16
+    # zeros as bytes: every byte of 0 is the value 0 in both types
+    z = lambda *s: torch.zeros(*s, t.itemsize, dtype=torch.uint8, device=device).view(t)[..., 0]
+    sc = [torch.zeros(num_pages, Hkv, KV_PAGE, device=device) for _ in range(2 * bool(e4m3))]
+    return KvPages(z(num_pages, Hkv, KV_PAGE, 256).contiguous(),
+                   z(num_pages, Hkv, 256, KV_PAGE).contiguous(), *sc)
+
+
+def _need(name, t, dtype, device, shape):
+    """A contiguous tensor of this type, device and shape, or an OpsError (None in
+    a shape: any size)."""
+    if t is None or t.dtype != dtype or t.device != device or not t.is_contiguous() or \
+            len(t.shape) != len(shape) or any(b is not None and a != b
+                                              for a, b in zip(t.shape, shape)):
+        got = "None" if t is None else f"{t.dtype} {tuple(t.shape)} on {t.device}" + (
+            "" if t.is_contiguous() else ", not contiguous")
+        raise OpsError(f"{name}: need contiguous {dtype} {shape} on {device}, got {got}")
+
+
+def _paged_call(device, name, *args):
+    """_call on the device of the pages, on its current stream there."""
+    import torch
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _call(name, *args, torch.cuda.current_stream().cuda_stream)
+    return _call(name, *args, torch.cuda.current_stream().cuda_stream)
+
+
+def _paged_seqs(pages, page_table, kv_len, q_start=None):
+    import torch
+    dev, B = pages.k.device, page_table.shape[0]
+    _need("page_table", page_table, torch.int32, dev, (B, None))
+    _need("kv_len", kv_len, torch.int32, dev, (B,))
+    if q_start is not None:
+        _need("q_start", q_start, torch.int32, dev, (B + 1,))
+    return dev, B
+
+
+def attn_prep_paged(proj, q_norm_w, k_norm_w, pos, q_start, kv_len, page_table, Hq, rot, rope,
+                    eps, q_scale, q_out, pages):
+    """attn_prep with K and V written into the pages of each row's sequence:
+    sequence b's new tokens are rows q_start[b] .. q_start[b + 1], the last of
+    its kv_len[b] keys. q_out [N, Hq, 256]; rope from rope_table."""
+    import torch
+    dev, B = _paged_seqs(pages, page_table, kv_len, q_start)
+    N, Hkv = proj.shape[0], pages.Hkv
+    if proj.dtype != torch.bfloat16 or proj.device != dev or proj.dim() != 2 or \
+            proj.stride(1) != 1 or proj.shape[1] < Hq * 512 + Hkv * 512:
+        raise OpsError(f"proj: need bfloat16 rows of {Hq * 512 + Hkv * 512} values on {dev}")
+    _need("q_norm_w", q_norm_w, torch.float32, dev, (256,))
+    _need("k_norm_w", k_norm_w, torch.float32, dev, (256,))
+    _need("pos", pos, torch.int32, dev, (N,))
+    _need("rope", rope, torch.float32, dev, (None, rot // 2, 2))
+    _need("q_out", q_out, torch.bfloat16, dev, (N, Hq, 256))
+    _paged_call(dev, "cujev_op_attn_prep_paged", proj.data_ptr(), proj.stride(0),
+                q_norm_w.data_ptr(), k_norm_w.data_ptr(), pos.data_ptr(), q_start.data_ptr(),
+                kv_len.data_ptr(), page_table.data_ptr(), page_table.shape[1], B, N, Hq, Hkv, rot,
+                rope.data_ptr(), rope.shape[0], eps, q_scale, q_out.data_ptr(), *pages.args)
+
+
+def kv_page_read(pages, page_table, kv_len, max_kv, k_cache, vt_cache):
+    """Keys [0, min(kv_len[b], max_kv)) of each sequence into contiguous caches
+    k_cache [B, Hkv, stride, 256] and vt_cache [B, Hkv, 256, stride] (a state's
+    layout; stride at least kv_stride(max_kv)); the other columns stay."""
+    import torch
+    dev, B = _paged_seqs(pages, page_table, kv_len)
+    stride = k_cache.shape[-2]
+    _need("k_cache", k_cache, torch.bfloat16, dev, (B, pages.Hkv, stride, 256))
+    _need("vt_cache", vt_cache, torch.bfloat16, dev, (B, pages.Hkv, 256, stride))
+    _paged_call(dev, "cujev_op_kv_page_read", *pages.args, page_table.data_ptr(),
+                page_table.shape[1], kv_len.data_ptr(), B, max_kv, pages.Hkv, k_cache.data_ptr(),
+                vt_cache.data_ptr(), stride)
+
+
+def attention_paged_ws_bytes(N, B, max_q, max_kv, Hq, Hkv, window=0, sinks=0, e4m3=False) -> int:
+    return int(load().cujev_ops_attention_paged_ws_bytes(N, B, max_q, max_kv, Hq, Hkv, window,
+                                                         sinks, int(e4m3)))
+
+
+def attention_paged(q, gate, gate_tok_stride, gate_head_stride, pages, page_table, q_start, kv_len,
+                    max_q, max_kv, out, window=0, sinks=0, ws=None):
+    """Attention of the call's rows q [N, Hq, 256] over their sequences' pages,
+    causal; with window > 0 over the last `window` positions and the first
+    `sinks`. gate may be None. max_q and max_kv bound the sequences' new tokens
+    and keys; ws: uint8 device workspace of attention_paged_ws_bytes (None where
+    that is 0)."""
+    import torch
+    dev, B = _paged_seqs(pages, page_table, kv_len, q_start)
+    N, Hq = q.shape[0], q.shape[1]
+    _need("q", q, torch.bfloat16, dev, (N, Hq, 256))
+    _need("out", out, torch.bfloat16, dev, (N, Hq * 256))
+    if gate is not None:
+        last = (N - 1) * gate_tok_stride + (Hq - 1) * gate_head_stride + 256
+        if gate.dtype != torch.bfloat16 or gate.device != dev or min(gate_tok_stride,
+                                                                     gate_head_stride) < 0 or \
+                N > 0 and gate.untyped_storage().nbytes() < 2 * (gate.storage_offset() + last):
+            raise OpsError(f"gate: need bfloat16 on {dev}, with {N} rows and {Hq} heads at these "
+                           "strides")
+    if ws is not None:
+        _need("ws", ws, torch.uint8, dev, (None,))
+    _paged_call(dev, "cujev_op_attention_paged", q.data_ptr(),
+                None if gate is None else gate.data_ptr(), gate_tok_stride, gate_head_stride,
+                *pages.args, q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(),
+                page_table.shape[1], B, N, max_q, max_kv, Hq, pages.Hkv, window, sinks,
+                out.data_ptr(), None if ws is None else ws.data_ptr(),
+                0 if ws is None else ws.numel())
 
 
 def gdn_conv_prep(proj, conv_w, conv_in, conv_out, seg0_len, own_base, A_neg_exp, dt_bias,

@@ -187,6 +187,87 @@ int cujev_op_attention_noalloc(const void *q, const void *gate, int gate_tok_str
                                const int32_t *own_base, int N, int Hq, int Hkv, void *out,
                                void *stream);
 
+/* ---- paged K/V cache ------------------------------------------------------
+ * No counterpart in the reference, whose K/V cache is one contiguous bf16
+ * buffer per state (src/engine/model.h:60-72): a pool of pages that many
+ * sequences share, its writer, its reader and the attention over it.
+ *
+ * A page holds CUJEV_OPS_KV_PAGE = 64 tokens of every kv-head:
+ *   k_pages   [num_pages][Hkv][64][256]
+ *   vt_pages  [num_pages][Hkv][256][64]   V transposed, as in the vt cache
+ * kv_type CUJEV_OPS_KV_BF16: elements are bf16, the scales are not read (NULL).
+ * kv_type CUJEV_OPS_KV_E4M3: elements are e4m3 (OCP, no infinities), and
+ *   k_scale, v_scale  fp32 [num_pages][Hkv][64]
+ * hold one scale per token and kv-head. A row x (256 values) is stored as
+ * e4m3(x / s), nearest even, s = 2^e with e the least integer such that
+ * max |x| <= 448 * 2^e, within [-100, 120]: what a reader gets back, e4m3 *
+ * s, is exact in bf16. NaN and infinity are stored as NaN. Scales that the
+ * caller writes have to be powers of two in that range, too. Pools,
+ * 16-byte aligned, are the caller's device memory; a slot that was never
+ * written may hold anything.
+ *
+ * The sequences of one call (device int32 arrays, B sequences):
+ *   q_start [B + 1]   sequence b's new tokens are rows q_start[b] ..
+ *                     q_start[b + 1] - 1 of the call's N (rising; a sequence may
+ *                     have none; rows outside all of them are left as they were)
+ *   kv_len [B]        its keys, the new tokens' last: new token i of ql is at
+ *                     position kv_len[b] - ql + i (one at a negative position
+ *                     is not stored and sees nothing)
+ *   page_table [B][max_pages]   position p is slot p % 64 of page
+ *                     page_table[b][p / 64]
+ * Sequences may share pages that a call only reads. A page that a call writes
+ * belongs to one of its sequences: two sequences that write the same slot
+ * leave either's values. Lengths are cut to N, max_pages * 64 (and max_q,
+ * max_kv where given); a page id outside [0, num_pages) is a page that is not
+ * there: nothing is written to it, its keys are seen by no row, it reads as
+ * zeros. These arrays are read on the device, so a captured graph can be
+ * replayed with other lengths and tables within the same bounds. */
+#define CUJEV_OPS_KV_PAGE 64
+#define CUJEV_OPS_KV_BF16 0
+#define CUJEV_OPS_KV_E4M3 1
+
+/* cujev_op_attn_prep with K and V written into pages: per row n of a sequence
+ * q_out[n] bf16 [N][Hq][256] and, at the row's position, its K and V. Any Hq /
+ * Hkv up to 16; rot is 8, 16, 32 or 64; pos [N] picks the row's RoPE angles
+ * (cut to [0, npos), the table's positions); proj rows 8-byte aligned. */
+int cujev_op_attn_prep_paged(const void *proj, int proj_stride, const float *q_norm_w,
+                             const float *k_norm_w, const int32_t *pos, const int32_t *q_start,
+                             const int32_t *kv_len, const int32_t *page_table, int max_pages,
+                             int B, int N, int Hq, int Hkv, int rot, const float *rope_table,
+                             int npos, float eps, float q_scale, void *q_out, int kv_type,
+                             void *k_pages, void *vt_pages, float *k_scale, float *v_scale,
+                             int num_pages, void *stream);
+
+/* Reads sequences back: columns [0, min(kv_len[b], max_kv)) of k_cache
+ * [B][Hkv][cache_stride][256] and vt_cache [B][Hkv][256][cache_stride], the
+ * layout of a state's caches, cache_stride >= cujev_ops_kv_stride(max_kv);
+ * further columns stay as they were. max_kv <= max_pages * 64. */
+int cujev_op_kv_page_read(int kv_type, const void *k_pages, const void *vt_pages,
+                          const float *k_scale, const float *v_scale, int num_pages,
+                          const int32_t *page_table, int max_pages, const int32_t *kv_len, int B,
+                          int max_kv, int Hkv, void *k_cache, void *vt_cache, int cache_stride,
+                          void *stream);
+
+/* Attention of the call's rows over their sequences' pages. q bf16
+ * [N][Hq][256], scaled by 256^-1/2 * log2 e; gate as for cujev_op_attention,
+ * or NULL for none; out bf16 [N][Hq*256]. The row at position p sees keys j <=
+ * p and, where window > 0, of those only j > p - window and j < sinks (the
+ * first tokens of the sequence); a row that sees no key gives 0. K and V of
+ * keys that some row of the call sees have to be finite; other slots may hold
+ * anything. Any Hq / Hkv up to 16. No sequence has more than max_q new tokens
+ * or max_kv keys (what is past them is not computed, or not seen). ws: device
+ * workspace of cujev_ops_attention_paged_ws_bytes() for the same arguments
+ * (0: none needed); calls that may overlap need one each. */
+int cujev_op_attention_paged(const void *q, const void *gate, int gate_tok_stride,
+                             int gate_head_stride, int kv_type, const void *k_pages,
+                             const void *vt_pages, const float *k_scale, const float *v_scale,
+                             int num_pages, const int32_t *q_start, const int32_t *kv_len,
+                             const int32_t *page_table, int max_pages, int B, int N, int max_q,
+                             int max_kv, int Hq, int Hkv, int window, int sinks, void *out,
+                             void *ws, size_t ws_bytes, void *stream);
+size_t cujev_ops_attention_paged_ws_bytes(int N, int B, int max_q, int max_kv, int Hq, int Hkv,
+                                          int window, int sinks, int kv_type);
+
 /* Replaces reference src/kernels/kernels.h:214-215 (k_gdn_conv) and :221-223
  * (k_gdn_prep), fused. proj rows [q Hk*128 | k Hk*128 | v Hv*128 | z | b | a].
  * Conv (width 4) + SiLU with taps before a segment taken from conv_in [C][3]

@@ -1,0 +1,128 @@
+"""Refusals of the paged K/V cache's entry points, on the CPU: every call here
+is turned away by the host's checks before anything is launched."""
+import ctypes as C
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from cujev import ops  # noqa: E402
+
+FAKE = 1 << 20  # a well-aligned address that nothing may touch
+INVALID, CAPACITY = 1, 6
+
+
+def call(name, **changes):
+    args = dict(BASE[name])
+    assert set(changes) <= set(args), changes
+    args.update(changes)
+    lib = ops.load()
+    st = getattr(lib, name)(*args.values())
+    return st, lib.cujev_ops_last_error().decode()
+
+
+POOL = dict(kv_type=1, k_pages=FAKE, vt_pages=FAKE, k_scale=FAKE, v_scale=FAKE, num_pages=4)
+BASE = {
+    "cujev_op_attn_prep_paged": dict(
+        proj=FAKE, proj_stride=5120, q_norm_w=FAKE, k_norm_w=FAKE, pos=FAKE, q_start=FAKE,
+        kv_len=FAKE, page_table=FAKE, max_pages=2, B=0, N=0, Hq=8, Hkv=2, rot=64, rope_table=FAKE,
+        npos=128, eps=1e-6, q_scale=0.09, q_out=FAKE, **POOL, stream=None),
+    "cujev_op_kv_page_read": dict(
+        **POOL, page_table=FAKE, max_pages=2, kv_len=FAKE, B=0, max_kv=128, Hkv=2, k_cache=FAKE,
+        vt_cache=FAKE, cache_stride=192, stream=None),
+    "cujev_op_attention_paged": dict(
+        q=FAKE, gate=FAKE, gate_tok_stride=5120, gate_head_stride=512, **POOL, q_start=FAKE,
+        kv_len=FAKE, page_table=FAKE, max_pages=2, B=0, N=0, max_q=1, max_kv=128, Hq=8, Hkv=2,
+        window=0, sinks=0, out=FAKE, ws=None, ws_bytes=0, stream=None),
+}
+READ, PREP, ATTN = "cujev_op_kv_page_read", "cujev_op_attn_prep_paged", "cujev_op_attention_paged"
+
+
+def test_argument_order_is_the_headers():
+    for name, args in BASE.items():
+        assert len(args) == len(ops._SIGS[name])
+
+
+@pytest.mark.parametrize("name", [PREP, READ, ATTN])
+def test_an_empty_call_does_nothing(name):
+    assert call(name)[0] == 0
+
+
+BAD_POOL = [dict(kv_type=2), dict(kv_type=-1), dict(k_pages=None), dict(vt_pages=None),
+            dict(k_pages=FAKE + 8), dict(vt_pages=FAKE + 2), dict(k_scale=None),
+            dict(v_scale=None), dict(v_scale=FAKE + 4), dict(num_pages=0), dict(num_pages=-1),
+            dict(Hkv=0), dict(max_pages=0), dict(max_pages=1 << 26), dict(B=-1),
+            dict(B=1, page_table=None), dict(B=1, kv_len=None)]
+
+
+@pytest.mark.parametrize("name", [PREP, READ, ATTN])
+@pytest.mark.parametrize("bad", BAD_POOL, ids=str)
+def test_pool_and_table_are_checked(name, bad):
+    st, msg = call(name, **bad)
+    assert st == INVALID and name[9:] in msg
+
+
+@pytest.mark.parametrize("bad", [
+    dict(N=-1), dict(Hq=7), dict(Hq=0), dict(Hq=34), dict(rot=0), dict(rot=24), dict(rot=128),
+    dict(npos=0), dict(proj_stride=5119), dict(proj_stride=5121), dict(proj=FAKE + 4),
+    dict(q_out=FAKE + 4), dict(q_norm_w=FAKE + 4), dict(rope_table=FAKE + 8),
+    dict(N=1, B=1, proj=None), dict(N=1, B=1, q_start=None), dict(N=1, B=1, q_out=None),
+    dict(N=1, B=1, pos=None), dict(N=1, B=1, rope_table=None), dict(N=1, B=1, q_norm_w=None),
+    dict(N=1, B=1, k_norm_w=None)], ids=str)
+def test_prep_refuses(bad):
+    assert call(PREP, **bad)[0] == INVALID
+
+
+@pytest.mark.parametrize("bad", [
+    dict(max_kv=-1), dict(max_kv=129), dict(cache_stride=128), dict(cache_stride=200),
+    dict(B=1, k_cache=None), dict(B=1, vt_cache=FAKE + 8), dict(B=70000)], ids=str)
+def test_read_refuses(bad):
+    assert call(READ, **bad)[0] == INVALID
+
+
+@pytest.mark.parametrize("bad", [
+    dict(N=-1), dict(max_q=-1), dict(max_kv=-1), dict(max_kv=129), dict(Hq=7), dict(Hq=34),
+    dict(window=-1), dict(window=8, sinks=-1), dict(sinks=4), dict(q=FAKE + 8), dict(out=FAKE + 8),
+    dict(gate=FAKE + 2), dict(gate_tok_stride=5121), dict(gate_head_stride=2),
+    dict(N=1, B=1, q=None), dict(N=1, B=1, q_start=None), dict(N=1, B=1, out=None)], ids=str)
+def test_attention_refuses(bad):
+    assert call(ATTN, **bad)[0] == INVALID
+
+
+def test_bindings_refuse_wrong_tensors():
+    k = torch.zeros(2, 1, 64, 256, dtype=torch.bfloat16)
+    vt = torch.zeros(2, 1, 256, 64, dtype=torch.bfloat16)
+    sc = torch.zeros(2, 1, 64)
+    f8 = torch.float8_e4m3fn
+    pages = ops.KvPages(k, vt)
+    ops.KvPages(k.to(f8), vt.to(f8), sc, sc)
+    for args in [(k, vt, sc, sc), (k.half(), vt.half()), (k, vt[:1]), (k, vt.transpose(2, 3)),
+                 (k.to(f8), vt.to(f8)), (k.to(f8), vt, sc, sc), (k[..., :128], vt),
+                 (k.to(f8), vt.to(f8), sc.double(), sc)]:
+        with pytest.raises(ops.OpsError):
+            ops.KvPages(*args)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)
+    q, out = torch.zeros(1, 4, 256).bfloat16(), torch.zeros(1, 1024).bfloat16()
+    good = dict(q=q, gate=None, gate_tok_stride=0, gate_head_stride=0, pages=pages,
+                page_table=i32(0)[None], q_start=i32(0, 1), kv_len=i32(1), max_q=1, max_kv=1,
+                out=out)
+    for bad in [dict(q=q.float()), dict(q=q[..., :128]), dict(out=out[:, :512]),
+                dict(kv_len=i32(1, 2)), dict(q_start=i32(0)), dict(page_table=i32(0)),
+                dict(kv_len=torch.tensor([1])), dict(ws=torch.zeros(4)),
+                dict(gate=q.float()), dict(gate=q, gate_tok_stride=1024, gate_head_stride=512),
+                dict(gate=q, gate_tok_stride=-4)]:
+        with pytest.raises(ops.OpsError):
+            ops.attention_paged(**{**good, **bad})
+    kc, vc = torch.zeros(1, 1, 128, 256).bfloat16(), torch.zeros(1, 1, 256, 128).bfloat16()
+    for a, b in [(kc[0], vc), (kc, vc[..., :64]), (kc.float(), vc)]:
+        with pytest.raises(ops.OpsError):
+            ops.kv_page_read(pages, i32(0)[None], i32(1), 1, a, b)
+    w = torch.ones(256)
+    prep = dict(proj=torch.zeros(1, 4 * 512 + 512).bfloat16(), q_norm_w=w, k_norm_w=w, pos=i32(0),
+                q_start=i32(0, 1), kv_len=i32(1), page_table=i32(0)[None], Hq=4, rot=64,
+                rope=torch.zeros(8, 32, 2), eps=1e-6, q_scale=0.1, q_out=q, pages=pages)
+    for bad in [dict(proj=prep["proj"].float()), dict(proj=prep["proj"][:, :2048]),
+                dict(pos=i32(0, 1)), dict(rope=torch.zeros(8, 16, 2)), dict(q_out=q[:, :2]),
+                dict(q_norm_w=w.bfloat16()), dict(k_norm_w=w[:128])]:
+        with pytest.raises(ops.OpsError):
+            ops.attn_prep_paged(**{**prep, **bad})
