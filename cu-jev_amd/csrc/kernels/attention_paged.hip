@@ -2,91 +2,962 @@
  *
  * Row (n, h) of sequence b, at position p, sees the keys j <= p of b's pages
  * and, with a window W, of those only j > p - W and the first S (sinks):
- *   out = sigmoid(gate) sum_j 2^(q.k_j) v_j / sum_j 2^(q.k_j). */
+ *   out = sigmoid(gate) sum_j 2^(q.k_j) v_j / sum_j 2^(q.k_j).
+ *
+ * The rows of one sequence that share a kv-head, ql new tokens x G q-heads, are
+ * packed (row r = token r / G, head r % G), so any G fills the same tiles.
+ * Both kernels below run S^T = K Q^T and O^T += V^T P^T on matrix
+ * instructions, keys (or dims) on the M side and rows on N: a lane holds
+ * scores of one row, and feeding K's rows in the right order makes its score
+ * accumulators exactly the P operand of the next product. e4m3 pages become
+ * bf16 operands in registers, exactly: K's scale is the conversion's, V's (one
+ * per key, the summed index) multiplies p before its rounding, which a power
+ * of two does not change. */
 #include "paged.h"
+
+#include <type_traits>
 
 namespace CUJEV_KNS {
 namespace {
 
-/* One wave per (row, q-head): lane j takes key j of a page for the scores, dims
- * 4 lane .. + 3 for the output; running maximum and sum in fp32. */
+typedef __attribute__((address_space(3))) void *lds_ptr;
+typedef __attribute__((address_space(3))) const unsigned char lds_u8;
+DEV u32x4 lds_read16(lds_u8 *base, uint32_t off) {
+    return *(__attribute__((address_space(3))) const u32x4 *)(base + off);
+}
+DEV void lds_write16(unsigned char *base, uint32_t off, u32x4 v) { *(u32x4 *)(base + off) = v; }
+
+DEV __amdgpu_buffer_rsrc_t make_rsrc(const void *base, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, (int)bytes, 0x00020000);
+}
+DEV u32x4 buf_load16(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, 0));
+}
+
+/* 8 e4m3 values (two dwords) times a power of two -> 8 bf16 */
+DEV bf16x8 widen(uint32_t a, uint32_t b, float scale) {
+    const bf16x2 p = unpack_e4m3<false>(a, scale), q = unpack_e4m3<true>(a, scale);
+    const bf16x2 r = unpack_e4m3<false>(b, scale), s = unpack_e4m3<true>(b, scale);
+    return bf16x8{p[0], p[1], q[0], q[1], r[0], r[1], s[0], s[1]};
+}
+/* x, or -inf where the key is hidden. On the bits: hidden scores may be NaN. */
+DEV float hide(bool seen, float x) {
+    return __uint_as_float(seen ? __float_as_uint(x) : 0xff800000u);
+}
+
+/* What both kernels and the merge share. A tile of rows whose key tiles are
+ * shared out over several workgroups keeps, per share, unnormalised o, l and
+ * the softmax's reference mu of its RT rows in slot (tile Hkv + kh) nshare +
+ * share. */
+struct Call {
+    const bf16 *q, *gate;
+    int gts, ghs;
+    const void *k, *vt;
+    const float *ks, *vs;
+    int num_pages;
+    const int32_t *q_start, *kv_len, *page_table;
+    int max_pages, B, N, max_q, max_kv, Hq, Hkv, G, window, sinks;
+    bf16 *out;
+    float *po, *pl, *pmu;
+    int items;   /* tiles of rows, at most */
+    int share;   /* key tiles a share */
+    int nshare;  /* shares a tile, at most */
+};
+DEV pg_seq seq_of(const Call &c, int b) {
+    return load_seq(c.q_start, c.kv_len, b, c.N, c.max_q, c.max_kv);
+}
+/* Tile `item` of RT packed rows: its sequence and number within it. */
+template <int RT> DEV int find_tile(const Call &c, int item, pg_seq *s, int *local) {
+    return find_item(
+        c.q_start, c.kv_len, c.B, c.N, c.max_q, c.max_kv, item,
+        [&](const pg_seq &q) { return (int)(((long long)q.ql * c.G + RT - 1) / RT); }, s, local);
+}
+DEV int page_id(const Call &c, int b, const pg_tiles &t, int i) {
+    const int page = c.page_table[(size_t)b * c.max_pages + pg_tile_page(t, i)];
+    return page >= 0 && page < c.num_pages ? page : -1;
+}
+
+/* ---- few rows: up to 16 packed rows of a sequence and kv-head ------------------
+ * Bound by the K/V bytes. A workgroup takes one share of the key tiles; its 4
+ * waves take whole tiles in turn and work alone until they merge through LDS.
+ * K and V^T go from memory into registers as the operands of
+ * v_mfma_f32_16x16x32_bf16 (16 bytes a lane, 64 bytes of 16 rows a load): K of
+ * the next tile is in flight during the softmax and the PV products, V^T
+ * during the scores, so a wave keeps at least half a tile in flight. */
+constexpr int FEW = 16;
+
 template <bool E4M3>
-__global__ __launch_bounds__(64) void attention_paged_kernel(
-    const bf16 *__restrict__ q, const bf16 *__restrict__ gate, int gts, int ghs,
-    const void *__restrict__ kp, const void *__restrict__ vp, const float *__restrict__ ks,
-    const float *__restrict__ vs, int num_pages, const int32_t *__restrict__ q_start,
-    const int32_t *__restrict__ kv_len, const int32_t *__restrict__ page_table, int max_pages,
-    int B, int N, int Hq, int Hkv, int window, int sinks, bf16 *__restrict__ out) {
-    const int n = blockIdx.x / Hq, h = blockIdx.x % Hq, kh = h / (Hq / Hkv), lane = threadIdx.x;
-    __shared__ float qs[PD], pr[PG];
-    const int b = find_seq(q_start, B, n);
-    if (b < 0)
+__global__ __launch_bounds__(256) void attention_few_kernel(Call c) {
+    __shared__ __attribute__((aligned(16))) float so[4][FEW][PD];
+    __shared__ float sl[4][FEW], sm[4][FEW];
+    constexpr int NK = E4M3 ? 16 : 32; /* 16-byte loads of a K or V^T tile */
+    const int kh = blockIdx.x, share = blockIdx.y, b = blockIdx.z;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int m = lane & 15, g = lane >> 4;
+    const pg_seq s = seq_of(c, b);
+    const int rows = min(s.ql * c.G, FEW);
+    if (rows <= 0)
         return;
-    const Seq s = load_seq(q_start, kv_len, b, N, max_pages);
-    if ((unsigned)(n - s.q0) >= (unsigned)s.ql)
+    const pg_tiles list = pg_tile_list(s, 0, s.ql - 1, c.window, c.sinks);
+    const int nshare = pg_max(pg_div_up(list.ntl, c.share), 1);
+    if (share >= nshare)
         return;
-    const int pos = s.p0 + n - s.q0;
-    for (int e = 0; e < 4; e++)
-        qs[4 * lane + e] = bf2f(q[((size_t)n * Hq + h) * PD + 4 * lane + e]);
-    __syncthreads();
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    const int hi = min(pos, s.kv - 1), lo = window ? max(pos - window + 1, 0) : 0;
-    for (int t = 0; t <= hi / PG && hi >= 0; t++) {
-        const int j = t * PG + lane;
-        const bool seen = j <= hi && (j >= lo || j < sinks);
-        const int page = page_table[(size_t)b * max_pages + t];
-        if (!__any(seen) || page < 0 || page >= num_pages)
-            continue;
-        const size_t head = (size_t)page * Hkv + kh;
-        float x = 0.f;
-        for (int d = 0; d < PD; d++) {
-            const size_t at = head * PSLICE + (size_t)lane * PD + d;
-            float kv;
-            if constexpr (E4M3)
-                kv = bf2f(unpack_e4m3<false>(((const uint8_t *)kp)[at], 1.f)[0]);
-            else
-                kv = bf2f(((const bf16 *)kp)[at]);
-            x += qs[d] * kv;
+    const int tb = share * c.share, ntl = min(list.ntl - tb, c.share);
+
+    /* this lane's row (column of S^T and O^T) */
+    const int row = min(m, rows - 1), tok = row / c.G, head = kh * c.G + row % c.G;
+    const int pos = s.p0 + tok;
+    bf16x8 qf[8];
+    {
+        const bf16 *qp = c.q + ((size_t)(s.q0 + tok) * c.Hq + head) * PD;
+#pragma unroll
+        for (int ks = 0; ks < 8; ks++) /* dims of k-step ks: as K's loads below */
+            qf[ks] = *(const bf16x8 *)(qp + (E4M3 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1)
+                                                  : 32 * ks + 8 * g));
+    }
+    /* Row m of score block kb is key key0 + 4 kb (e4m3), or key0 + 4 (kb & 1)
+     * + 32 (kb >> 1): lane g then holds, in accumulators 4 kb .. + 3, the keys
+     * its V^T loads bring. */
+    const int key0 = (E4M3 ? 16 : 8) * (m >> 2) + (m & 3);
+    auto kkey = [&](int kb) { return E4M3 ? 4 * kb : 4 * (kb & 1) + 32 * (kb >> 1); };
+    const uint32_t kvoff = E4M3 ? key0 * PD + 16 * g : key0 * PD * 2 + 16 * g;
+    const uint32_t vvoff = E4M3 ? m * PG + 16 * g : m * PG * 2 + 16 * g;
+    constexpr uint32_t SLICE = PSLICE * (E4M3 ? 1 : 2);
+    /* key of accumulator v = 4 kb + i of this lane */
+    auto key_of = [&](int v) { return E4M3 ? 16 * g + v : 8 * g + (v & 7) + 32 * (v >> 3); };
+
+    u32x4 kr[NK], vr[NK];
+    float ksc[4];
+    auto load_k = [&](int page) {
+        const size_t at = (size_t)max(page, 0) * c.Hkv + kh;
+        const __amdgpu_buffer_rsrc_t r = make_rsrc((const char *)c.k + at * SLICE, SLICE);
+#pragma unroll
+        for (int kb = 0; kb < 4; kb++)
+#pragma unroll
+            for (int i = 0; i < NK / 4; i++)
+                kr[kb * (NK / 4) + i] = buf_load16(r, kvoff, kkey(kb) * (SLICE / PG) + 64 * i);
+        if constexpr (E4M3) {
+#pragma unroll
+            for (int kb = 0; kb < 4; kb++)
+                ksc[kb] = c.ks[at * PG + key0 + kkey(kb)];
         }
-        if constexpr (E4M3)
-            x *= ks[head * PG + lane];
-        x = seen ? x : -INFINITY;
-        const float mn = fmaxf(m, wave_max(x)), a = fast_exp2(m - mn), p = fast_exp2(x - mn);
-        m = mn;
-        l = l * a + wave_sum(p);
-        __syncthreads();
-        pr[lane] = p;
-        __syncthreads();
-        for (int e = 0; e < 4; e++) {
-            o[e] *= a;
-            for (int i = 0; i < PG; i++) {
-                const size_t at = head * PSLICE + (size_t)(4 * lane + e) * PG + i;
-                float v;
-                if constexpr (E4M3)
-                    v = bf2f(unpack_e4m3<false>(((const uint8_t *)vp)[at], 1.f)[0]) *
-                        vs[head * PG + i];
-                else
-                    v = bf2f(((const bf16 *)vp)[at]);
-                o[e] += pr[i] > 0.f ? pr[i] * v : 0.f;
+    };
+
+    floatx4 o[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+        o[i] = floatx4{};
+    float mrun = -INFINITY, lrun = 0.f;
+    int page = wave < ntl ? page_id(c, b, list, tb + wave) : -1;
+    if (wave < ntl)
+        load_k(page);
+    for (int i = wave; i < ntl; i += 4) {
+        const int cur = page, k0 = pg_tile_page(list, tb + i) * PG;
+        const size_t at = (size_t)max(cur, 0) * c.Hkv + kh;
+        const __amdgpu_buffer_rsrc_t rv = make_rsrc((const char *)c.vt + at * SLICE, SLICE);
+        floatx4 vsc[4];
+        if constexpr (E4M3) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                vsc[e] = *(const floatx4 *)(c.vs + at * PG + 16 * g + 4 * e);
+        }
+#pragma unroll
+        for (int t = 0; t < 16; t++)
+#pragma unroll
+            for (int h = 0; h < NK / 16; h++)
+                vr[t * (NK / 16) + h] = buf_load16(rv, vvoff, t * 16 * (SLICE / PD) + 64 * h);
+        if (i + 4 < ntl)
+            page = page_id(c, b, list, tb + i + 4);
+
+        floatx4 x[4];
+#pragma unroll
+        for (int kb = 0; kb < 4; kb++) {
+            x[kb] = floatx4{};
+#pragma unroll
+            for (int ks = 0; ks < 8; ks++) {
+                bf16x8 a;
+                if constexpr (E4M3) {
+                    const u32x4 w = kr[kb * 4 + (ks >> 1)];
+                    a = ks & 1 ? widen(w[2], w[3], ksc[kb]) : widen(w[0], w[1], ksc[kb]);
+                } else {
+                    a = __builtin_bit_cast(bf16x8, kr[kb * 8 + ks]);
+                }
+                x[kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[ks], x[kb], 0, 0, 0);
             }
         }
+        if (i + 4 < ntl)
+            load_k(page);
+
+        const bool foreign = cur < 0 || pg_tile_foreign(k0, s.p0, s.kv, c.window, c.sinks);
+        if (foreign) { /* values and scales of no key of this call meet p = 0: make them 0 */
+            auto own = [&](int j) {
+                return cur >= 0 && pg_key_own(k0 + j, s.p0, s.kv, c.window, c.sinks);
+            };
+            u32x4 keep[2];
+#pragma unroll
+            for (int h = 0; h < NK / 16; h++)
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    uint32_t k = 0;
+#pragma unroll
+                    for (int e = 0; e < (E4M3 ? 4 : 2); e++) {
+                        const bool is =
+                            own(E4M3 ? 16 * g + 4 * w + e : 32 * h + 8 * g + 2 * w + e);
+                        k |= is ? (E4M3 ? 0xffu << (8 * e) : 0xffffu << (16 * e)) : 0u;
+                        if constexpr (E4M3)
+                            vsc[w][e] = is ? vsc[w][e] : 0.f;
+                    }
+                    keep[h][w] = k;
+                }
+#pragma unroll
+            for (int t = 0; t < NK; t++)
+                vr[t] &= keep[t % (NK / 16)];
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < 16; v++) {
+            const bool seen =
+                cur >= 0 && pg_key_seen(k0 + key_of(v), pos, s.kv, c.window, c.sinks);
+            x[v >> 2][v & 3] = hide(seen, x[v >> 2][v & 3]);
+            mx = fmaxf(mx, x[v >> 2][v & 3]);
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float mnew = fmaxf(mrun, mx);
+        const float ref = mnew == -INFINITY ? 0.f : mnew; /* no key yet: p = 2^-inf = 0 */
+        if (__any(mnew != mrun)) {
+            const float a = fast_exp2(mrun - ref);
+            lrun *= a;
+#pragma unroll
+            for (int t = 0; t < 16; t++)
+                o[t] *= a;
+        }
+        mrun = mnew;
+        bf16x8 p[2];
+#pragma unroll
+        for (int v = 0; v < 16; v++) {
+            float pv = fast_exp2(x[v >> 2][v & 3] - ref);
+            lrun += pv;
+            if constexpr (E4M3)
+                pv *= vsc[v >> 2][v & 3];
+            p[v >> 3][v & 7] = f2bf(pv);
+        }
+#pragma unroll
+        for (int t = 0; t < 16; t++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                bf16x8 a;
+                if constexpr (E4M3)
+                    a = h ? widen(vr[t][2], vr[t][3], 1.f) : widen(vr[t][0], vr[t][1], 1.f);
+                else
+                    a = __builtin_bit_cast(bf16x8, vr[2 * t + h]);
+                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, p[h], o[t], 0, 0, 0);
+            }
     }
+    lrun += __shfl_xor(lrun, 16, 64);
+    lrun += __shfl_xor(lrun, 32, 64);
+
+    /* merge the waves; lane (m, g) holds dims 16 t + 4 g .. + 3 of row m */
+#pragma unroll
+    for (int t = 0; t < 16; t++)
+        *(floatx4 *)&so[wave][m][16 * t + 4 * g] = o[t];
+    if (g == 0)
+        sl[wave][m] = lrun, sm[wave][m] = mrun;
+    __syncthreads();
+    const size_t slot = ((size_t)b * c.Hkv + kh) * c.nshare + share;
+    for (int r = wave; r < rows; r += 4) {
+        float ref = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; w++)
+            ref = fmaxf(ref, sm[w][r]);
+        const float mu = ref == -INFINITY ? 0.f : ref;
+        floatx4 acc = {};
+        float l = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float a = fast_exp2(sm[w][r] - mu);
+            acc += *(const floatx4 *)&so[w][r][4 * lane] * a;
+            l += sl[w][r] * a;
+        }
+        if (nshare > 1) {
+            *(floatx4 *)(c.po + (slot * FEW + r) * PD + 4 * lane) = acc;
+            if (lane == 0)
+                c.pl[slot * FEW + r] = l, c.pmu[slot * FEW + r] = mu;
+            continue;
+        }
+        const int n = s.q0 + r / c.G, hd = kh * c.G + r % c.G;
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        bf16x4 gv = {}, res;
+        if (c.gate)
+            gv = *(const bf16x4 *)(c.gate + (size_t)n * c.gts + (size_t)hd * c.ghs + 4 * lane);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            res[e] = f2bf(acc[e] * inv * (c.gate ? sigmoid_f(bf2f(gv[e])) : 1.f));
+        *(bf16x4 *)(c.out + ((size_t)n * c.Hq + hd) * PD + 4 * lane) = res;
+    }
+}
+
+/* ---- many rows: tiles of 128 packed rows -----------------------------------------
+ * One workgroup, 4 waves. Wave (i, j) computes the scores of 64 rows (half i)
+ * against 32 keys of a tile (half j), and then O^T of the same rows for 128
+ * dims (half j): each K and V^T operand it reads from LDS feeds two
+ * v_mfma_f32_32x32x16_bf16, and what the pair (i, 0), (i, 1) has to exchange
+ * is its P, 4 KiB each way per tile through LDS. One wave per 32 rows instead
+ * reads every operand once per MFMA, 256 KiB of LDS a tile, as long as its
+ * MFMAs take; here it is 160 (bf16).
+ *
+ * Per tile one barrier. Before it a wave runs the S^T MFMAs of tile i + 1 with
+ * the softmax of tile i, and leaves P of tile i in LDS; after it the PV MFMAs of
+ * tile i, its own keys' first, while K of tile i + 3 and V^T of tile i + 1 go
+ * to the buffers that were last read before the barrier.
+ *
+ * The softmax's reference mu of a row stays 0 while the scores are within 2^+-64
+ * of it (mu cancels in o / l). A wave that leaves that range takes an integer
+ * mu of its own for the tile and tells the other of its pair through the signs
+ * of its P, which are otherwise 0: lane h = 0 sends the low and h = 1 the high
+ * half of the float. Both then agree on the larger one and rescale. */
+constexpr int RT = 128;
+constexpr float SHIFT_RANGE = 64.f;
+
+template <bool E4M3> struct Lay {
+    static constexpr int T = PSLICE * (E4M3 ? 1 : 2); /* bytes of a K or V^T tile */
+    static constexpr int V = 0, K = 2 * T, P = 4 * T, PBUF = 16384, SC = P + 2 * PBUF;
+    /* e4m3: K scales of two tiles, V scales of four (read a tile later) */
+    static constexpr int TILES = SC + (E4M3 ? 2 * 256 + 4 * 256 : 0);
+    static constexpr int STAT = RT * PD * 4; /* l, mu behind the staged O */
+    static constexpr int BYTES = TILES > STAT + RT * 16 ? TILES : STAT + RT * 16;
+};
+static_assert(Lay<false>::BYTES <= 163840 && Lay<true>::BYTES <= 163840, "LDS of a CU");
+
+/* 16-byte pieces of the tiles are XOR-swizzled so that the 16 lanes of a
+ * ds_read_b128 phase hit 16 distinct bank groups. bf16: K rows of 512 bytes,
+ * V^T rows of 128; e4m3: 256 and 64. */
+template <bool E4M3> DEV int swz_k(int key) {
+    return E4M3 ? (key & 3) | ((key >> 4) & 1) << 2 | ((key >> 2) & 1) << 3
+                : ((key & 4) << 1) | ((key & 8) >> 1) | (key & 3);
+}
+template <bool E4M3> DEV int swz_v(int d) {
+    return E4M3 ? (d >> 2) & 3 : (d & 7) ^ ((d >> 3) & 1);
+}
+/* key of MFMA row m of a 32-key block: score accumulator r of lane half h is
+ * then key 16 (r >> 3) + 8 h + (r & 7) (bf16), 16 h + r (e4m3) */
+template <bool E4M3> DEV int perm_row(int m) {
+    return E4M3 ? 16 * ((m >> 2) & 1) + (m & 3) + 4 * (m >> 3)
+                : (m & ~12) | ((m & 4) << 1) | ((m & 8) >> 1);
+}
+
+template <bool E4M3>
+__global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
+    typedef Lay<E4M3> L;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[L::BYTES];
+    /* XCD-aware: where the kv-heads divide the 8 XCDs, an XCD's workgroups read
+     * the same kv-head. The longest (last) tiles of a sequence start first. */
+    int kh, item;
+    if (8 % c.Hkv == 0) {
+        const int per = 8 / c.Hkv, xcd = blockIdx.x & 7;
+        kh = xcd / per;
+        item = (blockIdx.x >> 3) * per + xcd % per;
+    } else {
+        kh = blockIdx.x % c.Hkv;
+        item = blockIdx.x / c.Hkv;
+    }
+    if (item >= c.items)
+        return;
+    item = c.items - 1 - item;
+    pg_seq s;
+    int local;
+    const int b = find_tile<RT>(c, item, &s, &local);
+    if (b < 0)
+        return;
+    const int r0 = local * RT, nrows = min(s.ql * c.G - r0, RT);
+    const int i0 = r0 / c.G, i1 = (r0 + nrows - 1) / c.G;
+    const pg_tiles list = pg_tile_list(s, i0, i1, c.window, c.sinks);
+    const int nshare = pg_max(pg_div_up(list.ntl, c.share), 1), share = blockIdx.y;
+    if (share >= nshare)
+        return;
+    const int tb = share * c.share, ntl = min(list.ntl - tb, c.share);
+    const size_t slot = ((size_t)item * c.Hkv + kh) * c.nshare + share;
+
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int wi = wave >> 1, wj = wave & 1, h = lane >> 5, col = lane & 31;
+
+    /* Q^T operands of this wave's 64 rows; rows past the last repeat it */
+    bf16x8 qf[2][16];
+    int pos[2];
+#pragma unroll
+    for (int rb = 0; rb < 2; rb++) {
+        const int r = r0 + min(64 * wi + 32 * rb + col, nrows - 1);
+        const int tok = r / c.G, head = kh * c.G + r % c.G;
+        pos[rb] = s.p0 + tok;
+        const bf16 *qp = c.q + ((size_t)(s.q0 + tok) * c.Hq + head) * PD;
+#pragma unroll
+        for (int ks = 0; ks < 16; ks++)
+            qf[rb][ks] = *(const bf16x8 *)(qp + (E4M3 ? 32 * (ks >> 1) + 16 * h + 8 * (ks & 1)
+                                                      : 16 * ks + 8 * h));
+    }
+    const int pmin = s.p0 + i0, pmax = s.p0 + i1;
+
+    /* ---- tile loads: memory -> LDS (buffer_load ... lds: lane l's 16 bytes land
+     * at base + 16 l, so the swizzle is applied to the address) ---- */
+    uint32_t kvoff[2], vvoff;
+    if constexpr (E4M3) { /* a load is 4 K rows or 16 V^T rows */
+#pragma unroll
+        for (int par = 0; par < 2; par++) {
+            const int row = 16 * par + 4 * wave + (lane >> 4);
+            kvoff[par] = (lane >> 4) * 256 + (((lane & 15) ^ swz_k<true>(row)) << 4);
+        }
+        vvoff = (lane >> 2) * 64 + (((lane & 3) ^ swz_v<true>(lane >> 2)) << 4);
+    } else { /* 2 K rows or 8 V^T rows */
+#pragma unroll
+        for (int par = 0; par < 2; par++) {
+            const int row = 8 * par + 2 * wave + (lane >> 5);
+            kvoff[par] = (lane >> 5) * 512 + (((lane & 31) ^ swz_k<false>(row)) << 4);
+        }
+        vvoff = (lane >> 3) * 128 + (((lane & 7) ^ swz_v<false>(8 * wave + (lane >> 3))) << 4);
+    }
+    constexpr int NL = E4M3 ? 4 : 8; /* loads of a wave, tile and operand */
+    auto slice = [&](int page) { return (size_t)max(page, 0) * c.Hkv + kh; };
+    auto k_rsrc = [&](int page) {
+        return make_rsrc((const char *)c.k + slice(page) * L::T, L::T);
+    };
+    auto v_rsrc = [&](int page) {
+        return make_rsrc((const char *)c.vt + slice(page) * L::T, L::T);
+    };
+    auto issue_k = [&](__amdgpu_buffer_rsrc_t r, int buf, int n) {
+        const int at = (E4M3 ? 4096 : 4096) * n + 1024 * wave;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(smem + L::K + buf * L::T + at), 16,
+                                                 kvoff[n & 1], at, 0, 0);
+    };
+    auto issue_v = [&](__amdgpu_buffer_rsrc_t r, int buf, int n) {
+        const int at = 4096 * n + 1024 * wave;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(smem + L::V + buf * L::T + at), 16,
+                                                 vvoff, at, 0, 0);
+    };
+    /* scales of tile t: wave 0 K's, wave 1 V's */
+    auto issue_scales = [&](int page, int t) {
+        if constexpr (E4M3) {
+            if (wave < 2) {
+                const float *src = (wave ? c.vs : c.ks) + slice(page) * PG;
+                const int at = L::SC + (wave ? 512 + (t & 3) * 256 : (t & 1) * 256);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(make_rsrc(src, 256),
+                                                         (lds_ptr)(smem + at), 4, lane * 4, 0, 0,
+                                                         0);
+            }
+        }
+    };
+
+    /* ---- per-lane LDS read addresses ---- */
+    lds_u8 *lds = (lds_u8 *)smem;
+    const int arow = perm_row<E4M3>(col);
+    uint32_t ka[8];
+#pragma unroll
+    for (int p = 0; p < 8; p++)
+        ka[p] = L::K + (32 * wj + arow) * (L::T / PG) +
+                (((2 * p + h) ^ swz_k<E4M3>(32 * wj + arow)) << 4);
+    /* V^T pieces of key half kb (0: this wave's own keys, 1: the other's) */
+    uint32_t va[2][2];
+#pragma unroll
+    for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+        for (int st = 0; st < 2; st++) {
+            const int half = wj ^ kb;
+            const int piece = E4M3 ? 2 * half + h : 4 * half + 2 * st + h;
+            va[kb][st] = L::V + (128 * wj + col) * (L::T / PD) +
+                         ((piece ^ swz_v<E4M3>(col)) << 4);
+        }
+    const uint32_t psend = L::P + wave * 4096 + lane * 16;
+    const uint32_t precv = L::P + (wave ^ 1) * 4096 + lane * 16;
+
+    /* page ids of the list, 64 entries in a lane each */
+    int ids = 0;
+    auto page_of = [&](int t) { /* called with t = 0, 1, 2, ... < ntl */
+        if ((t & 63) == 0)
+            ids = page_id(c, b, list, min(tb + t + lane, list.ntl - 1));
+        return __builtin_amdgcn_readlane(ids, t & 63);
+    };
+
+    floatx16 o[4][2];
+#pragma unroll
+    for (int d = 0; d < 4; d++)
+#pragma unroll
+        for (int rb = 0; rb < 2; rb++)
+            o[d][rb] = floatx16{};
+    float mrun[2] = {-INFINITY, -INFINITY}, lrun[2] = {0.f, 0.f}, mus[2] = {0.f, 0.f};
+
+    /* One k-step pair or step of S^T: operand reads QD ahead */
+    constexpr int QD = E4M3 ? 2 : 4;
+    constexpr int NKR = E4M3 ? 8 : 16; /* K reads a tile */
+    auto kaddr = [&](int n, int buf) {
+        return (E4M3 ? ka[n] : ka[n & 7] + (n >> 3) * 256) + buf * L::T;
+    };
+    auto kscale = [&](int buf) {
+        return E4M3 ? *(__attribute__((address_space(3))) const float *)(lds + L::SC + buf * 256 +
+                                                                         (32 * wj + arow) * 4)
+                    : 1.f;
+    };
+
+    int pg[4]; /* pages of tiles i .. i + 3 */
+    auto step = [&](auto has_next, int i, auto parity, floatx16 (&x)[2], floatx16 (&y)[2]) {
+        constexpr bool NEXT = decltype(has_next)::value;
+        constexpr int PAR = decltype(parity)::value; /* i & 1 */
+        const int k0 = pg_tile_page(list, tb + i) * PG;
+        const bool there = pg[0] >= 0;
+        floatx4 vsc[4];
+        if constexpr (E4M3) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                vsc[e] = __builtin_bit_cast(
+                    floatx4, lds_read16(lds, L::SC + 512 + (i & 3) * 256 +
+                                                 (32 * wj + 16 * h + 4 * e) * 4));
+        }
+        if (!there || !pg_tile_whole(k0, pmin, pmax, s.kv, c.window, c.sinks)) {
+            const int kb = k0 + 32 * wj + (E4M3 ? 16 : 8) * h;
+#pragma unroll
+            for (int rb = 0; rb < 2; rb++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int j = kb + (E4M3 ? r : 16 * (r >> 3) + (r & 7));
+                    x[rb][r] = hide(
+                        there && pg_key_seen(j, pos[rb], s.kv, c.window, c.sinks), x[rb][r]);
+                    if constexpr (E4M3) /* a scale of no key of this call: any bits */
+                        if (!there || !pg_key_own(j, pmin, s.kv, c.window, c.sinks))
+                            vsc[r >> 2][r & 3] = 0.f;
+                }
+        }
+        /* ---- S^T of tile i + 1 with the softmax of tile i ---- */
+        u32x4 ring[QD];
+        float ksc = 1.f;
+        if constexpr (NEXT) {
+            ksc = kscale(PAR ^ 1);
+#pragma unroll
+            for (int n = 0; n < QD; n++)
+                ring[n] = lds_read16(lds, kaddr(n, PAR ^ 1));
+        }
+        float mx[2] = {-INFINITY, -INFINITY}, ls[2] = {0.f, 0.f};
+        bf16x8 pf[2][2];
+        auto pair = [&](int rb, int v, float shift) { /* p of accumulators v, v + 1 */
+            float a = fast_exp2(x[rb][v] - shift), e = fast_exp2(x[rb][v + 1] - shift);
+            ls[rb] += a + e;
+            if constexpr (E4M3) {
+                a *= vsc[v >> 2][v & 3];
+                e *= vsc[v >> 2][(v & 3) + 1];
+            }
+            pf[rb][v >> 3][v & 7] = f2bf(a);
+            pf[rb][v >> 3][(v & 7) + 1] = f2bf(e);
+        };
+        __builtin_amdgcn_sched_barrier(0);
+        bf16x8 odd = {};
+#pragma unroll
+        for (int ks = 0; ks < 16; ks++) {
+            if constexpr (NEXT) {
+                bf16x8 a;
+                if constexpr (E4M3) {
+                    if (ks & 1) {
+                        a = odd;
+                    } else {
+                        const u32x4 w = ring[(ks >> 1) % QD];
+                        if ((ks >> 1) + QD < NKR)
+                            ring[(ks >> 1) % QD] = lds_read16(lds, kaddr((ks >> 1) + QD, PAR ^ 1));
+                        a = widen(w[0], w[1], ksc);
+                        odd = widen(w[2], w[3], ksc);
+                    }
+                } else {
+                    a = __builtin_bit_cast(bf16x8, ring[ks % QD]);
+                    if (ks + QD < NKR)
+                        ring[ks % QD] = lds_read16(lds, kaddr(ks + QD, PAR ^ 1));
+                }
+#pragma unroll
+                for (int rb = 0; rb < 2; rb++)
+                    y[rb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                        a, qf[rb][ks], ks == 0 ? floatx16{} : y[rb], 0, 0, 0);
+            }
+            mx[ks >> 3] = fmaxf(mx[ks >> 3], fmaxf(x[ks >> 3][2 * (ks & 7)],
+                                                   x[ks >> 3][2 * (ks & 7) + 1]));
+            pair(ks >> 3, 2 * (ks & 7), 0.f);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        float mul[2];
+        bool moved = false;
+#pragma unroll
+        for (int rb = 0; rb < 2; rb++) {
+            const auto sw = __builtin_amdgcn_permlane32_swap(
+                __float_as_uint(mx[rb]), __float_as_uint(mx[rb]), false, false);
+            mrun[rb] = fmaxf(mrun[rb], fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])));
+            /* a row without a key yet leaves the choice to the other wave */
+            mul[rb] = mrun[rb] == -INFINITY                        ? -INFINITY
+                      : fabsf(mrun[rb] - mus[rb]) > SHIFT_RANGE ? ceilf(mrun[rb])
+                                                                   : mus[rb];
+            moved |= mul[rb] != 0.f;
+        }
+        moved = __any(moved);
+        if (__builtin_expect(moved, 0)) {
+#pragma unroll
+            for (int rb = 0; rb < 2; rb++) {
+                const float shift = mul[rb] == -INFINITY ? 0.f : mul[rb];
+                ls[rb] = 0.f;
+#pragma unroll
+                for (int v = 0; v < 16; v += 2)
+                    pair(rb, v, shift);
+            }
+        }
+#pragma unroll
+        for (int rb = 0; rb < 2; rb++)
+#pragma unroll
+            for (int st = 0; st < 2; st++) {
+                u32x4 w = __builtin_bit_cast(u32x4, pf[rb][st]);
+                if (__builtin_expect(moved, 0)) {
+                    const uint32_t u = __float_as_uint(mul[rb]) >> (16 * h + 8 * st);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        w[e] |= ((u >> (2 * e)) & 1) << 15 | ((u >> (2 * e + 1)) & 1) << 31;
+                }
+                lds_write16(smem, psend + PAR * L::PBUF + (2 * rb + st) * 1024, w);
+            }
+        /* P is in LDS, this wave's reads of K are done, its tile loads have landed */
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+
+        if (!there || pg_tile_foreign(k0, pmin, s.kv, c.window, c.sinks)) {
+            /* values of no key of these rows meet p = 0: make them 0 */
+#pragma unroll 4
+            for (int n = 0; n < L::T / 4096; n++) {
+                const int at = (n * 256 + (int)threadIdx.x) * 16, d = at / (L::T / PD);
+                const int piece = ((at >> 4) & (L::T / PD / 16 - 1)) ^ swz_v<E4M3>(d);
+                u32x4 w = lds_read16(lds, L::V + PAR * L::T + at);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    uint32_t keep = 0;
+#pragma unroll
+                    for (int f = 0; f < (E4M3 ? 4 : 2); f++) {
+                        const int j =
+                            k0 + (E4M3 ? 16 * piece + 4 * e + f : 8 * piece + 2 * e + f);
+                        const bool own =
+                            there && pg_key_own(j, pmin, s.kv, c.window, c.sinks);
+                        keep |= own ? (E4M3 ? 0xffu << (8 * f) : 0xffffu << (16 * f)) : 0u;
+                    }
+                    w[e] &= keep;
+                }
+                lds_write16(smem, L::V + PAR * L::T + at, w);
+            }
+            lds_barrier();
+        }
+
+        u32x4 pw[2][2];
+#pragma unroll
+        for (int rb = 0; rb < 2; rb++)
+#pragma unroll
+            for (int st = 0; st < 2; st++)
+                pw[rb][st] = lds_read16(lds, precv + PAR * L::PBUF + (2 * rb + st) * 1024);
+        /* Both waves' references of a row are known: take the larger one */
+        auto agree = [&]() {
+#pragma unroll
+            for (int rb = 0; rb < 2; rb++) {
+                uint32_t u = 0;
+#pragma unroll
+                for (int st = 0; st < 2; st++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        u |= ((pw[rb][st][e] >> 15) & 1) << (8 * st + 2 * e);
+                        u |= (pw[rb][st][e] >> 31) << (8 * st + 2 * e + 1);
+                    }
+                const uint32_t v = __shfl_xor(u, 32, 64);
+                const float mup = __uint_as_float(h ? u << 16 | v : v << 16 | u);
+                float ref = fmaxf(mul[rb], mup);
+                ref = ref == -INFINITY ? mus[rb] : ref;
+                /* it only falls while no key has counted, with o = l = 0 */
+                const float fo = fast_exp2(fminf(mus[rb] - ref, 0.f));
+                const float fm = fast_exp2(mul[rb] - ref), fp = fast_exp2(mup - ref);
+#pragma unroll
+                for (int d = 0; d < 4; d++)
+                    o[d][rb] *= fo;
+                lrun[rb] *= fo;
+                ls[rb] *= fm;
+                mus[rb] = ref;
+#pragma unroll
+                for (int st = 0; st < 2; st++) {
+                    pw[rb][st] &= 0x7fff7fffu;
+                    bf16x8 t = __builtin_bit_cast(bf16x8, pw[rb][st]);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        t[e] = f2bf(bf2f(t[e]) * fp);
+                        pf[rb][st][e] = f2bf(bf2f(pf[rb][st][e]) * fm);
+                    }
+                    pw[rb][st] = __builtin_bit_cast(u32x4, t);
+                }
+            }
+        };
+        /* ---- O^T += V^T P^T: own keys, then the other wave's ---- */
+        const __amdgpu_buffer_rsrc_t rk = k_rsrc(pg[3]), rv = v_rsrc(pg[1]);
+        if (__builtin_expect(moved, 0))
+            agree();
+        constexpr int NVR = E4M3 ? 4 : 8; /* V^T reads of a key half */
+        constexpr int VD = E4M3 ? 2 : 4;
+        auto vaddr = [&](int n, int kb) { /* bf16: step-major, e4m3: both steps a read */
+            return (E4M3 ? va[kb][0] + n * 32 * (L::T / PD)
+                         : va[kb][n >> 2] + (n & 3) * 32 * (L::T / PD)) +
+                   PAR * L::T;
+        };
+        u32x4 vring[VD];
+#pragma unroll
+        for (int n = 0; n < VD; n++)
+            vring[n] = lds_read16(lds, vaddr(n, 0));
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++) {
+            if (kb == 1 && !moved) {
+                uint32_t any = 0;
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+                    any |= pw[t >> 1][t & 1][0] | pw[t >> 1][t & 1][1] | pw[t >> 1][t & 1][2] |
+                           pw[t >> 1][t & 1][3];
+                if (__builtin_expect(__any((any & 0x80008000u) != 0), 0))
+                    agree();
+            }
+#pragma unroll
+            for (int n = 0; n < NVR; n++) {
+                const u32x4 w = vring[n % VD];
+                const int nn = kb * NVR + n + VD;
+                if (nn < 2 * NVR)
+                    vring[n % VD] = lds_read16(lds, vaddr(nn % NVR, nn / NVR));
+#pragma unroll
+                for (int half = 0; half < (E4M3 ? 2 : 1); half++) {
+                    bf16x8 a;
+                    if constexpr (E4M3)
+                        a = half ? widen(w[2], w[3], 1.f) : widen(w[0], w[1], 1.f);
+                    else
+                        a = __builtin_bit_cast(bf16x8, w);
+                    const int d = E4M3 ? n : n & 3, st = E4M3 ? half : n >> 2;
+#pragma unroll
+                    for (int rb = 0; rb < 2; rb++) {
+                        const bf16x8 p = kb ? __builtin_bit_cast(bf16x8, pw[rb][st]) : pf[rb][st];
+                        o[d][rb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, p, o[d][rb], 0, 0, 0);
+                    }
+                    if constexpr (NEXT) { /* one tile load beside each pair of MFMAs */
+                        const int at = E4M3 ? (kb * NVR + n) * 2 + half : kb * NVR + n;
+                        if (E4M3 ? !(at & 1) : true) {
+                            const int q = E4M3 ? at >> 1 : at;
+                            if (q < NL)
+                                issue_v(rv, PAR ^ 1, q);
+                            else
+                                issue_k(rk, PAR ^ 1, q - NL);
+                        }
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        if constexpr (NEXT)
+            issue_scales(pg[3], i + 3);
+#pragma unroll
+        for (int rb = 0; rb < 2; rb++)
+            lrun[rb] += ls[rb];
+        pg[0] = pg[1], pg[1] = pg[2], pg[2] = pg[3];
+        if (i + 4 < ntl)
+            pg[3] = page_of(i + 4);
+    };
+
+    if (ntl > 0) {
+        floatx16 xa[2], xb[2];
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+            pg[t] = t < ntl ? page_of(t) : pg[t - 1];
+        const __amdgpu_buffer_rsrc_t k_0 = k_rsrc(pg[0]), v_0 = v_rsrc(pg[0]), k_1 = k_rsrc(pg[1]);
+#pragma unroll
+        for (int n = 0; n < NL; n++) {
+            issue_k(k_0, 0, n);
+            issue_v(v_0, 0, n);
+            issue_k(k_1, 1, n);
+        }
+        issue_scales(pg[0], 0);
+        issue_scales(pg[1], 1);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        {
+            const float ksc = kscale(0);
+#pragma unroll
+            for (int n = 0; n < NKR; n++) {
+                const u32x4 w = lds_read16(lds, kaddr(n, 0));
+#pragma unroll
+                for (int half = 0; half < (E4M3 ? 2 : 1); half++) {
+                    bf16x8 a;
+                    if constexpr (E4M3)
+                        a = half ? widen(w[2], w[3], ksc) : widen(w[0], w[1], ksc);
+                    else
+                        a = __builtin_bit_cast(bf16x8, w);
+                    const int ks = E4M3 ? 2 * n + half : n;
+#pragma unroll
+                    for (int rb = 0; rb < 2; rb++)
+                        xa[rb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                            a, qf[rb][ks], ks == 0 ? floatx16{} : xa[rb], 0, 0, 0);
+                }
+            }
+        }
+        __syncthreads(); /* K buffer 0 is free */
+        {
+            const __amdgpu_buffer_rsrc_t k_2 = k_rsrc(pg[2]);
+#pragma unroll
+            for (int n = 0; n < NL; n++)
+                issue_k(k_2, 0, n);
+            issue_scales(pg[2], 2);
+        }
+        const std::true_type more{};
+        const std::false_type last{};
+        const std::integral_constant<int, 0> even{};
+        const std::integral_constant<int, 1> odd{};
+        int i = 0;
+        for (; i + 2 < ntl; i += 2) {
+            step(more, i, even, xa, xb);
+            step(more, i + 1, odd, xb, xa);
+        }
+        if (ntl - i == 2) {
+            step(more, i, even, xa, xb);
+            step(last, i + 1, odd, xb, xa);
+        } else {
+            step(last, i, even, xa, xb);
+        }
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    }
+    __syncthreads(); /* the tile buffers are idle: O and the rows' l go there */
+
+    /* ---- epilogue: O as fp32 rows of 1 KiB through LDS (piece p of row r in slot
+     * p ^ (r & 31)), l of a row from the pair's two halves ---- */
+    float *stat = (float *)(smem + L::STAT); /* [row][l of wave 0, of wave 1, mu] */
+#pragma unroll
+    for (int rb = 0; rb < 2; rb++) {
+        const int r = 64 * wi + 32 * rb + col;
+        const float l = lrun[rb] + __shfl_xor(lrun[rb], 32, 64);
+        if (h == 0) {
+            stat[r * 4 + wj] = l;
+            if (wj == 0)
+                stat[r * 4 + 2] = mus[rb];
+        }
+#pragma unroll
+        for (int d = 0; d < 4; d++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const floatx4 v = {o[d][rb][4 * q], o[d][rb][4 * q + 1], o[d][rb][4 * q + 2],
+                                   o[d][rb][4 * q + 3]};
+                const int piece = 32 * wj + 8 * d + 2 * q + h;
+                *(floatx4 *)(smem + r * 1024 + ((piece ^ col) << 4)) = v;
+            }
+    }
+    __syncthreads();
+    for (int t = wave; t < nrows; t += 4) {
+        const floatx4 v = *(const floatx4 *)(smem + t * 1024 + ((lane ^ (t & 31)) << 4));
+        const float l = stat[t * 4] + stat[t * 4 + 1];
+        if (nshare > 1) {
+            *(floatx4 *)(c.po + (slot * RT + t) * PD + 4 * lane) = v;
+            if (lane == 0)
+                c.pl[slot * RT + t] = l, c.pmu[slot * RT + t] = stat[t * 4 + 2];
+            continue;
+        }
+        const int r = r0 + t, n = s.q0 + r / c.G, head = kh * c.G + r % c.G;
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        bf16x4 gv = {}, res;
+        if (c.gate)
+            gv = *(const bf16x4 *)(c.gate + (size_t)n * c.gts + (size_t)head * c.ghs + 4 * lane);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            res[e] = f2bf(v[e] * inv * (c.gate ? sigmoid_f(bf2f(gv[e])) : 1.f));
+        *(bf16x4 *)(c.out + ((size_t)n * c.Hq + head) * PD + 4 * lane) = res;
+    }
+}
+
+/* ---- merge of a tile's shares ----------------------------------------------------
+ * One wave per row: o = sum_s 2^(mu_s - mu) o_s over the shares that saw keys,
+ * l likewise, mu the largest of theirs; then / l and the gate. */
+template <int ROWS>
+__global__ __launch_bounds__(256) void merge_kernel(Call c) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int unit = blockIdx.x / (ROWS / 4), t = blockIdx.x % (ROWS / 4) * 4 + wave;
+    const int kh = unit % c.Hkv, item = unit / c.Hkv;
+    pg_seq s;
+    int local = 0;
+    if (ROWS == FEW)
+        s = seq_of(c, item);
+    else if (find_tile<ROWS>(c, item, &s, &local) < 0)
+        return;
+    const int r0 = local * ROWS, nrows = min(s.ql * c.G - r0, ROWS);
+    if (t >= nrows)
+        return;
+    const int i0 = r0 / c.G, i1 = (r0 + nrows - 1) / c.G;
+    const pg_tiles list = pg_tile_list(s, i0, i1, c.window, c.sinks);
+    const int nshare = pg_div_up(list.ntl, c.share);
+    if (nshare <= 1)
+        return;
+    const size_t first = ((size_t)item * c.Hkv + kh) * c.nshare * ROWS + t;
+    float mu = -INFINITY;
+    for (int i = 0; i < nshare; i++)
+        if (c.pl[first + (size_t)i * ROWS] > 0.f)
+            mu = fmaxf(mu, c.pmu[first + (size_t)i * ROWS]);
+    floatx4 acc = {};
+    float l = 0.f;
+    for (int i = 0; i < nshare; i++) {
+        const size_t at = first + (size_t)i * ROWS;
+        if (c.pl[at] > 0.f) {
+            const float w = fast_exp2(c.pmu[at] - mu);
+            acc += *(const floatx4 *)(c.po + at * PD + 4 * lane) * w;
+            l += c.pl[at] * w;
+        }
+    }
+    const int r = r0 + t, n = s.q0 + r / c.G, head = kh * c.G + r % c.G;
     const float inv = l > 0.f ? 1.f / l : 0.f;
-    for (int e = 0; e < 4; e++) {
-        float g = 1.f;
-        if (gate)
-            g = sigmoid_f(bf2f(gate[(size_t)n * gts + (size_t)h * ghs + 4 * lane + e]));
-        out[((size_t)n * Hq + h) * PD + 4 * lane + e] = f2bf(o[e] * inv * g);
-    }
+    bf16x4 gv = {}, res;
+    if (c.gate)
+        gv = *(const bf16x4 *)(c.gate + (size_t)n * c.gts + (size_t)head * c.ghs + 4 * lane);
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        res[e] = f2bf(acc[e] * inv * (c.gate ? sigmoid_f(bf2f(gv[e])) : 1.f));
+    *(bf16x4 *)(c.out + ((size_t)n * c.Hq + head) * PD + 4 * lane) = res;
 }
 
 } // namespace
 } // namespace CUJEV_KNS
 using namespace CUJEV_KNS;
 
+/* How a call is run: rows a tile, tiles at most, key tiles a share, shares. */
+struct paged_plan {
+    int rt, items, share, nshare;
+};
+static paged_plan plan_of(int N, int B, int max_q, int max_kv, int G, int Hkv, int window,
+                          int sinks) {
+    paged_plan p = {0, 0, 1, 1};
+    if (N <= 0 || B <= 0 || max_q <= 0)
+        return p;
+    const long long mq = max_q < N ? max_q : N;
+    p.rt = mq * G <= FEW ? FEW : RT;
+    long long items = B;
+    if (p.rt == RT) {
+        const long long by_rows = (long long)N * G / RT + B, by_len = B * ((mq * G + RT - 1) / RT);
+        items = by_rows < by_len ? by_rows : by_len;
+    }
+    if (items * Hkv > 1 << 22) {
+        p.items = -1;
+        return p;
+    }
+    p.items = (int)items;
+    const int tok = p.rt == FEW ? (int)mq : RT / G + 2;
+    const int most = pg_max(pg_max_tiles(tok, max_kv, window, sinks), 1);
+    const int units = p.items * Hkv;
+    int n = p.rt == FEW ? 1024 / units : 512 / units;
+    n = n < 1 ? 1 : n;
+    p.share = pg_div_up(most, n);
+    if (p.share < 4)
+        p.share = 4;
+    p.nshare = pg_div_up(most, p.share);
+    return p;
+}
+static size_t plan_rows(const paged_plan &p, int Hkv) {
+    return p.nshare > 1 ? (size_t)p.items * Hkv * p.nshare * p.rt : 0;
+}
+
 extern "C" size_t cujev_attention_paged_ws_bytes(int N, int B, int max_q, int max_kv, int Hq,
                                                  int Hkv, int window, int sinks, int type) {
-    return 0;
+    (void)type;
+    if (window >= max_kv)
+        window = sinks = 0;
+    const paged_plan p = plan_of(N, B, max_q, max_kv, Hq / Hkv, Hkv, window, sinks);
+    return plan_rows(p, Hkv) * (PD + 2) * sizeof(float);
 }
 
 extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int gate_tok_stride,
@@ -94,20 +965,43 @@ extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int
                                         const cujev_paged_seqs *seqs, int N, int max_q, int max_kv,
                                         int Hq, int window, int sinks, bf16_t *out, void *ws,
                                         size_t ws_bytes, hipStream_t stream) {
-    if (N <= 0 || seqs->B <= 0)
+    const int Hkv = pages->Hkv, B = seqs->B;
+    if (window >= max_kv) /* no row's window ends before its first key */
+        window = sinks = 0;
+    const paged_plan p = plan_of(N, B, max_q, max_kv, Hq / Hkv, Hkv, window, sinks);
+    if (p.items == 0)
         return hipSuccess;
-    if ((long long)N * Hq > 0x7fffffff)
+    if (p.items < 0 || Hkv > 65535 || p.nshare > 65535 || (p.rt == FEW && B > 65535))
         return hipErrorInvalidValue;
-#define LAUNCH(T)                                                                                 \
-    hipLaunchKernelGGL(attention_paged_kernel<T>, dim3((unsigned)(N * Hq)), dim3(64), 0, stream,  \
-                       (const bf16 *)q, (const bf16 *)gate, gate_tok_stride, gate_head_stride,    \
-                       pages->k, pages->vt, pages->k_scale, pages->v_scale, pages->num_pages,     \
-                       seqs->q_start, seqs->kv_len, seqs->page_table, seqs->max_pages, seqs->B,   \
-                       N, Hq, pages->Hkv, window, sinks, (bf16 *)out)
-    if (pages->type == CUJEV_KV_E4M3)
-        LAUNCH(true);
-    else
-        LAUNCH(false);
-#undef LAUNCH
+    const size_t rows = plan_rows(p, Hkv);
+    if (rows * (PD + 2) * sizeof(float) > ws_bytes)
+        return hipErrorInvalidValue;
+    const Call c = {(const bf16 *)q, (const bf16 *)gate, gate_tok_stride, gate_head_stride,
+                    pages->k, pages->vt, pages->k_scale, pages->v_scale, pages->num_pages,
+                    seqs->q_start, seqs->kv_len, seqs->page_table, seqs->max_pages, B, N,
+                    max_q, max_kv, Hq, Hkv, Hq / Hkv, window, sinks, (bf16 *)out,
+                    (float *)ws, (float *)ws + rows * PD, (float *)ws + rows * (PD + 1),
+                    p.items, p.share, p.nshare};
+    const bool e4m3 = pages->type == CUJEV_KV_E4M3;
+    if (p.rt == FEW) {
+        const dim3 grid((unsigned)Hkv, (unsigned)p.nshare, (unsigned)B);
+        if (e4m3)
+            hipLaunchKernelGGL(attention_few_kernel<true>, grid, dim3(256), 0, stream, c);
+        else
+            hipLaunchKernelGGL(attention_few_kernel<false>, grid, dim3(256), 0, stream, c);
+        if (p.nshare > 1)
+            hipLaunchKernelGGL(merge_kernel<FEW>, dim3((unsigned)(p.items * Hkv * (FEW / 4))),
+                               dim3(256), 0, stream, c);
+    } else {
+        const int per = 8 % Hkv == 0 ? 8 / Hkv : 1;
+        const dim3 grid((unsigned)(pg_div_up(p.items, per) * per * Hkv), (unsigned)p.nshare);
+        if (e4m3)
+            hipLaunchKernelGGL(attention_many_kernel<true>, grid, dim3(256), 0, stream, c);
+        else
+            hipLaunchKernelGGL(attention_many_kernel<false>, grid, dim3(256), 0, stream, c);
+        if (p.nshare > 1)
+            hipLaunchKernelGGL(merge_kernel<RT>, dim3((unsigned)(p.items * Hkv * (RT / 4))),
+                               dim3(256), 0, stream, c);
+    }
     return hipGetLastError();
 }

@@ -2,6 +2,7 @@
  * argument checks around the launchers of kernels.h. */
 #include "../../../include/cujev_ops.h"
 #include "kernels.h"
+#include "paged_index.h"
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdarg.h>
@@ -306,7 +307,7 @@ static int paged_check(const char *what, const cujev_kv_pages *pages, const int3
         return fail(1, "%s: bad page pool (type %d, %d pages, %d kv-heads; pointers set and "
                        "16-byte aligned, scales with e4m3)",
                     what, pages->type, pages->num_pages, pages->Hkv);
-    if (B < 0 || max_pages <= 0 || max_pages > 0x7fffffff / CUJEV_KV_PAGE ||
+    if (B < 0 || B > PG_MOST || max_pages <= 0 || max_pages > PG_MOST / CUJEV_KV_PAGE ||
         (B > 0 && (!page_table || !kv_len)))
         return fail(1, "%s: bad page table (B=%d, max_pages=%d)", what, B, max_pages);
     return 0;
@@ -329,7 +330,7 @@ EXPORT int cujev_op_attn_prep_paged(const void *proj, int proj_stride, const flo
     const int st = paged_check("attn_prep_paged", &pages, page_table, max_pages, kv_len, B);
     if (st != 0)
         return st;
-    if (N < 0 || !paged_heads_ok(Hq, Hkv) || (rot != 8 && rot != 16 && rot != 32 && rot != 64) ||
+    if (N < 0 || N > PG_MOST || !paged_heads_ok(Hq, Hkv) || (rot != 8 && rot != 16 && rot != 32 && rot != 64) ||
         npos <= 0)
         return fail(1, "attn_prep_paged: unsupported shape N=%d Hq=%d Hkv=%d rot=%d npos=%d", N,
                     Hq, Hkv, rot, npos);
@@ -386,7 +387,7 @@ EXPORT int cujev_op_attention_paged(const void *q, const void *gate, int gate_to
     const int st = paged_check("attention_paged", &pages, page_table, max_pages, kv_len, B);
     if (st != 0)
         return st;
-    if (N < 0 || max_q < 0 || max_kv < 0 || !paged_heads_ok(Hq, Hkv))
+    if (N < 0 || N > PG_MOST || max_q < 0 || max_kv < 0 || !paged_heads_ok(Hq, Hkv))
         return fail(1, "attention_paged: unsupported shape N=%d max_q=%d max_kv=%d Hq=%d Hkv=%d",
                     N, max_q, max_kv, Hq, Hkv);
     if (max_kv > max_pages * CUJEV_KV_PAGE)

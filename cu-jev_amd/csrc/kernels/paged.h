@@ -7,33 +7,19 @@
 #pragma once
 #include "common.h"
 #include "kernels.h"
+#include "paged_index.h"
 
 namespace CUJEV_KNS {
 namespace {
 
+static_assert(PG == CUJEV_KV_PAGE, "one definition of a page");
+
 constexpr int PD = 256;                /* head dim */
-constexpr int PG = CUJEV_KV_PAGE;      /* tokens a page */
 constexpr int PSLICE = PG * PD;        /* elements of one head's K or V^T in a page */
 
-/* Sequence b as one call sees it: rows q0 .. q0 + ql - 1, the first of which
- * has position p0 (negative where kv_len < ql: such rows have no slot). Lengths
- * outside the call's rows or the table are cut to them, so no value in
- * q_start, kv_len or page_table leads out of a buffer. */
-struct Seq {
-    int q0, ql, kv, p0;
-};
-DEV Seq clean_seq(int q0, int q1, int kv, int N, int max_pages) {
-    Seq s;
-    s.q0 = min(max(q0, 0), N);
-    s.ql = min(max(q1, s.q0), N) - s.q0;
-    s.p0 = (int)((unsigned)kv - (unsigned)s.ql);
-    s.kv = min(max(kv, 0), max_pages * PG);
-    if (kv < 0)
-        s.p0 = -s.ql;
-    return s;
-}
-DEV Seq load_seq(const int32_t *q_start, const int32_t *kv_len, int b, int N, int max_pages) {
-    return clean_seq(q_start[b], q_start[b + 1], kv_len[b], N, max_pages);
+DEV pg_seq load_seq(const int32_t *q_start, const int32_t *kv_len, int b, int N, int max_q,
+                    int max_kv) {
+    return pg_clean_seq(q_start[b], q_start[b + 1], kv_len[b], N, max_q, max_kv);
 }
 
 /* The sequence of row n: the last b with q_start[b] <= n, -1 for a row before
@@ -53,13 +39,13 @@ DEV int find_seq(const int32_t *q_start, int B, int n) {
 /* Work item `item` of a launch whose sequence b has count(b, s) of them, in
  * order: the sequence, and the item's number in it (-1: no such item). */
 template <typename F>
-DEV int find_item(const int32_t *q_start, const int32_t *kv_len, int B, int N, int max_pages,
-                  int item, F count, Seq *s, int *local) {
+DEV int find_item(const int32_t *q_start, const int32_t *kv_len, int B, int N, int max_q,
+                  int max_kv, int item, F count, pg_seq *s, int *local) {
     const int lane = threadIdx.x & 63;
     int before = 0;
     for (int b0 = 0; b0 < B; b0 += 64) {
         const int b = min(b0 + lane, B - 1);
-        const Seq mine = load_seq(q_start, kv_len, b, N, max_pages);
+        const pg_seq mine = load_seq(q_start, kv_len, b, N, max_q, max_kv);
         const int own = b0 + lane < B ? count(mine) : 0;
         int sum = own; /* inclusive sum over the lanes */
 #pragma unroll

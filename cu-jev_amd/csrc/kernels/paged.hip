@@ -16,8 +16,6 @@ namespace {
  * kv-head: the group's V^T rows are whole 16-byte (e4m3) or 32-byte pieces, so
  * the transpose needs neither LDS nor another wave's data: lane l holds 16
  * tokens of dims 4l .. 4l + 3 and stores one piece per dim. */
-constexpr int VTOK = 16;
-
 template <bool E4M3, int TOK>
 __global__ __launch_bounds__(256) void prep_paged_kernel(
     const bf16 *__restrict__ proj, int ps, const float *__restrict__ qw,
@@ -91,7 +89,7 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(
                 *(bf16x4 *)(q_out + ((size_t)n * Hq + head) * 256 + 4 * lane) = o;
                 continue;
             }
-            const Seq s = load_seq(q_start, kv_len, b, N, max_pages);
+            const pg_seq s = load_seq(q_start, kv_len, b, N, N, max_pages * PG);
             const int p = s.p0 + (n - s.q0);
             if ((unsigned)(n - s.q0) >= (unsigned)s.ql || p < 0 || p >= s.kv)
                 continue;
@@ -121,22 +119,18 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(
     if (unit >= groups * Hkv)
         return;
     const int kh = unit % Hkv;
-    Seq s;
+    pg_seq s;
     int g;
     const int b = find_item(
-        q_start, kv_len, B, N, max_pages, unit / Hkv,
-        [](const Seq &q) {
-            const int lo = max(q.p0, 0), hi = min(q.p0 + q.ql, q.kv);
-            return hi > lo ? (hi - 1) / VTOK - lo / VTOK + 1 : 0;
-        },
-        &s, &g);
+        q_start, kv_len, B, N, N, max_pages * PG, unit / Hkv,
+        [](const pg_seq &q) { return pg_v_groups(q); }, &s, &g);
     if (b < 0)
         return;
-    const int base = (max(s.p0, 0) / VTOK + g) * VTOK; /* the group's first position */
+    const int base = (pg_new_lo(s) / VTOK + g) * VTOK; /* the group's first position */
     const int page = page_table[(size_t)b * max_pages + base / PG];
     if (page < 0 || page >= num_pages)
         return;
-    const int lo = max(s.p0, base), hi = min(min(s.p0 + s.ql, s.kv), base + VTOK);
+    const int lo = max(pg_new_lo(s), base), hi = min(pg_new_hi(s), base + VTOK);
     const bf16 *src = proj + Hq * 512 + Hkv * 256 + kh * 256 + 4 * lane;
     bf16x4 v[VTOK];
 #pragma unroll

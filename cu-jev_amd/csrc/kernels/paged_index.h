@@ -1,0 +1,88 @@
+/* Where the paged operators read and write: how a sequence's lengths are cut,
+ * which pages a tile of rows visits, how the visits are shared out. No HIP in
+ * here: the kernels and the launchers use these functions, and a host program
+ * can check every index against the buffers. */
+#ifndef CUJEV_PAGED_INDEX_H
+#define CUJEV_PAGED_INDEX_H
+
+constexpr int PG = 64;   /* tokens a page, keys a tile */
+constexpr int VTOK = 16; /* positions of a V group of the prep */
+
+constexpr int pg_min(int a, int b) { return a < b ? a : b; }
+constexpr int pg_max(int a, int b) { return a > b ? a : b; }
+constexpr int pg_div_up(int a, int b) { return a / b + (a % b != 0); } /* a >= 0, b > 0 */
+
+/* Sequence b as one call sees it: rows q0 .. q0 + ql - 1, the first at position
+ * p0 (negative where it has fewer keys than rows: those rows have no slot),
+ * keys 0 .. kv - 1. Lengths outside the call's N rows, max_q and max_kv are
+ * cut, so no value in q_start or kv_len leads out of a buffer. N, max_kv and
+ * windows are at most 2^30: sums and differences of two fit an int. */
+constexpr int PG_MOST = 1 << 30;
+struct pg_seq {
+    int q0, ql, kv, p0;
+};
+constexpr pg_seq pg_clean_seq(int q0, int q1, int kv, int N, int max_q, int max_kv) {
+    pg_seq s{};
+    s.q0 = pg_min(pg_max(q0, 0), N);
+    const int ql = pg_min(pg_max(q1, s.q0), N) - s.q0;
+    s.p0 = pg_max(kv, 0) - ql;
+    s.ql = pg_min(ql, max_q);
+    s.kv = pg_min(pg_max(kv, 0), max_kv);
+    return s;
+}
+
+/* The positions [lo, hi) of the new tokens that have a slot */
+constexpr int pg_new_lo(const pg_seq &s) { return pg_max(s.p0, 0); }
+constexpr int pg_new_hi(const pg_seq &s) { return pg_min(s.p0 + s.ql, s.kv); }
+/* Aligned groups of VTOK positions that the new tokens touch; a call has at
+ * most min(N, N / VTOK + 2 B) of them. */
+constexpr int pg_v_groups(const pg_seq &s) {
+    const int lo = pg_new_lo(s), hi = pg_new_hi(s);
+    return hi > lo ? (hi - 1) / VTOK - lo / VTOK + 1 : 0;
+}
+
+/* Key tiles that the new tokens i0 .. i1 of a sequence visit, in order: the
+ * sinks' first (nsk of them, tiles 0 .. nsk - 1), then from tile t0 on. */
+struct pg_tiles {
+    int nsk, t0, ntl;
+};
+constexpr pg_tiles pg_tile_list(const pg_seq &s, int i0, int i1, int window, int sinks) {
+    pg_tiles t{};
+    const int hi = pg_min(s.p0 + i1, s.kv - 1); /* last key of the last row */
+    if (hi < 0)
+        return t;
+    const int lo = window > 0 ? pg_max(s.p0 + i0 - window + 1, 0) : 0; /* first of the first */
+    t.t0 = pg_min(lo, hi) / PG;
+    t.nsk = pg_min(pg_div_up(pg_min(sinks, hi + 1), PG), t.t0);
+    t.ntl = t.nsk + hi / PG - t.t0 + 1;
+    return t;
+}
+/* the page-table column of entry i of the list */
+constexpr int pg_tile_page(const pg_tiles &t, int i) { return i < t.nsk ? i : i - t.nsk + t.t0; }
+
+/* Most entries a list of a tile of `tok` tokens can have */
+constexpr int pg_max_tiles(int tok, int max_kv, int window, int sinks) {
+    const int all = pg_div_up(max_kv, PG);
+    if (window <= 0 || window > max_kv || tok > max_kv)
+        return all;
+    return pg_min(all, (window + tok) / PG + 2 + pg_div_up(pg_min(sinks, max_kv), PG));
+}
+
+/* Whether every row at positions pmin .. pmax sees all PG keys from k0 on */
+constexpr bool pg_tile_whole(int k0, int pmin, int pmax, int kv, int window, int sinks) {
+    return k0 + PG - 1 <= pg_min(pmin, kv - 1) &&
+           (window <= 0 || k0 > pmax - window || k0 + PG <= sinks);
+}
+/* Whether keys of the tile are no key of the call (behind the last one, or
+ * before every window and no sink): whatever is there may not reach a product. */
+constexpr bool pg_tile_foreign(int k0, int pmin, int kv, int window, int sinks) {
+    return k0 + PG > kv || (window > 0 && k0 <= pmin - window && k0 + PG > sinks);
+}
+constexpr bool pg_key_own(int j, int pmin, int kv, int window, int sinks) {
+    return j < kv && (window <= 0 || j > pmin - window || j < sinks);
+}
+constexpr bool pg_key_seen(int j, int p, int kv, int window, int sinks) {
+    return j <= p && j < kv && (window <= 0 || j > p - window || j < sinks);
+}
+
+#endif

@@ -1,0 +1,115 @@
+"""Where the paged operators read and write, on the CPU: paged_index.h, which
+the kernels index with, compiled for the host and checked against brute force
+over random and extreme lengths, and over lengths no caller should pass."""
+import pathlib
+import subprocess
+
+KERNELS = pathlib.Path(__file__).resolve().parent.parent / "cu-jev_amd" / "csrc" / "kernels"
+
+CHECK = r"""
+#include "paged_index.h"
+#include <cstdio>
+#include <cstdlib>
+#include <set>
+#include <vector>
+
+static int bad;
+#define NEED(c) do { if (!(c) && bad++ < 10) printf("line %d: %s\n", __LINE__, #c); } while (0)
+static unsigned rs = 12345;
+static int rnd(int lo, int hi) { rs = rs * 1664525u + 1013904223u; return lo + (int)((rs >> 4) % (unsigned)(hi - lo + 1)); }
+
+int main() {
+    /* any lengths at all stay inside the call */
+    const int odd[] = {0, 1, -1, 5, 63, 64, 65, 200, 4096, PG_MOST, -PG_MOST, 0x7fffffff, (int)0x80000000};
+    for (int q0 : odd) for (int q1 : odd) for (int kv : odd) for (int N : {0, 1, 64, 200, PG_MOST})
+        for (int mq : {0, 1, 100, PG_MOST}) for (int mk : {0, 1, 64, 1000, PG_MOST}) {
+            const pg_seq s = pg_clean_seq(q0, q1, kv, N, mq, mk);
+            NEED(s.q0 >= 0 && s.ql >= 0 && s.ql <= mq && (long long)s.q0 + s.ql <= N);
+            NEED(s.kv >= 0 && s.kv <= mk && s.p0 >= -N);
+            NEED(pg_new_lo(s) >= 0 && (pg_new_hi(s) <= s.kv));
+            for (int w : {0, 1, 100, PG_MOST}) for (int S : {0, 1, 64, 65, PG_MOST}) {
+                if (s.ql == 0) continue;
+                const pg_tiles t = pg_tile_list(s, 0, s.ql - 1, w, w ? S : 0);
+                NEED(t.ntl >= 0 && t.nsk >= 0 && t.nsk <= t.ntl);
+                if (t.ntl > 0) {
+                    NEED(pg_tile_page(t, 0) >= 0);
+                    NEED((long long)pg_tile_page(t, t.ntl - 1) * PG < s.kv);
+                }
+            }
+        }
+    /* lists, masks and bounds against brute force */
+    for (int it = 0; it < 60000; it++) {
+        const int ql = rnd(1, it % 3 ? 6 : 150), kvl = rnd(0, it % 5 ? 700 : 70), N = ql + rnd(0, 5), q0 = rnd(0, N - ql);
+        const int max_kv = kvl + rnd(-20, 200) > 0 ? kvl + rnd(-20, 200) : 1, mk = max_kv < 1 ? 1 : max_kv;
+        const int w = rnd(0, 2) ? rnd(1, 300) : 0, S = w && rnd(0, 1) ? rnd(0, 200) : 0;
+        const pg_seq s = pg_clean_seq(q0, q0 + ql, kvl, N, N, mk);
+        NEED(s.ql == ql && s.q0 == q0 && s.p0 == kvl - ql);
+        const int i0 = rnd(0, ql - 1), i1 = rnd(i0, ql - 1 < i0 + 40 ? ql - 1 : i0 + 40);
+        const pg_tiles t = pg_tile_list(s, i0, i1, w, S);
+        const int pmin = s.p0 + i0, pmax = s.p0 + i1;
+        std::set<int> visited;
+        for (int i = 0; i < t.ntl; i++) {
+            const int pg = pg_tile_page(t, i);
+            NEED(pg >= 0 && pg * PG < s.kv && visited.insert(pg).second);
+            NEED(i == 0 || pg > pg_tile_page(t, i - 1));
+            bool whole = true, foreign = false;
+            for (int j = pg * PG; j < pg * PG + PG; j++) {
+                bool own = false;
+                for (int p = pmin; p <= pmax; p++) {
+                    const bool sees = j <= p && j < s.kv && (!w || j > p - w || j < S);
+                    NEED(sees == pg_key_seen(j, p, s.kv, w, S));
+                    whole &= sees, own |= sees;
+                }
+                NEED(!own || pg_key_own(j, pmin, s.kv, w, S));
+                foreign |= !pg_key_own(j, pmin, s.kv, w, S);
+            }
+            NEED(!pg_tile_whole(pg * PG, pmin, pmax, s.kv, w, S) || whole);
+            NEED(!foreign || pg_tile_foreign(pg * PG, pmin, s.kv, w, S));
+            /* a tile with a scale or value to hide also takes the masked path */
+            NEED(!pg_tile_foreign(pg * PG, pmin, s.kv, w, S) || !pg_tile_whole(pg * PG, pmin, pmax, s.kv, w, S));
+        }
+        for (int p = pmin; p <= pmax; p++) for (int j = 0; j < s.kv; j++)
+            NEED(!pg_key_seen(j, p, s.kv, w, S) || visited.count(j / PG));
+        NEED(t.ntl <= pg_max_tiles(i1 - i0 + 1, mk, w, S));
+        NEED(t.ntl <= pg_max_tiles(i1 - i0 + 1 + rnd(0, 50), mk, w, S));
+    }
+    /* V groups: each new position in exactly one; the launch has enough */
+    for (int it = 0; it < 20000; it++) {
+        const int B = rnd(1, 8);
+        int N = 0, groups = 0;
+        std::vector<int> q, kv;
+        for (int b = 0; b < B; b++) { q.push_back(rnd(0, it % 2 ? 3 : 90)); kv.push_back(rnd(0, 200)); N += q[b]; }
+        int at = 0;
+        for (int b = 0; b < B; b++) {
+            const pg_seq s = pg_clean_seq(at, at + q[b], kv[b], N, N, 160);
+            at += q[b];
+            const int n = pg_v_groups(s);
+            groups += n;
+            std::set<int> seen;
+            for (int g = 0; g < n; g++) {
+                const int base = (pg_new_lo(s) / VTOK + g) * VTOK;
+                const int lo = pg_max(pg_new_lo(s), base), hi = pg_min(pg_new_hi(s), base + VTOK);
+                NEED(lo < hi && base % PG + VTOK <= PG && base < s.kv);
+                for (int p = lo; p < hi; p++) {
+                    NEED(seen.insert(p).second && p >= 0 && p < s.kv);
+                    const int row = s.q0 + p - s.p0;
+                    NEED(row >= s.q0 && row < s.q0 + s.ql && row < N);
+                }
+            }
+            NEED((int)seen.size() == pg_max(pg_new_hi(s) - pg_new_lo(s), 0));
+        }
+        NEED(groups <= (N < N / VTOK + 2 * B ? N : N / VTOK + 2 * B));
+    }
+    printf("bad %d\n", bad);
+    return bad != 0;
+}
+"""
+
+
+def test_every_index_stays_inside(tmp_path):
+    src, exe = tmp_path / "check.cpp", tmp_path / "check"
+    src.write_text(CHECK)
+    subprocess.run(["g++", "-O2", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover",
+                    "-I", str(KERNELS), str(src), "-o", str(exe)], check=True)
+    run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stdout + run.stderr
