@@ -40,10 +40,56 @@ DEV bf16x8 widen(uint32_t a, uint32_t b, float scale) {
     const bf16x2 r = unpack_e4m3<false>(b, scale), s = unpack_e4m3<true>(b, scale);
     return bf16x8{p[0], p[1], q[0], q[1], r[0], r[1], s[0], s[1]};
 }
+/* x of lane i of this lane's 16 (DPP row broadcast) */
+template <int i> DEV float row_lane(float x) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(
+        0, (int)__float_as_uint(x), 0x150 + i, 0xf, 0xf, false));
+}
+template <int n, typename F> DEV void unroll_for(F f) {
+    if constexpr (n > 0) {
+        unroll_for<n - 1>(f);
+        f(std::integral_constant<int, n - 1>{});
+    }
+}
 /* x, or -inf where the key is hidden. On the bits: hidden scores may be NaN. */
 DEV float hide(bool seen, float x) {
     return __uint_as_float(seen ? __float_as_uint(x) : 0xff800000u);
 }
+
+/* v_mfma_f32_32x32x16_bf16 by hand, so that O and Q stay in accumulation
+ * registers and the scores in ordinary ones; with the builtin the compiler
+ * moved Q's operands over before each MFMA (and spilled 64 registers). What
+ * it leaves to the code around it: two wait states between a VALU write of an
+ * operand and the MFMA (NOP), and 18 between an MFMA and a read of its result
+ * by anything but the next MFMA on it (settle()). Operands from LDS are waited
+ * for as for any instruction. */
+template <bool NOP> DEV void mfma_first(floatx16 &s, bf16x8 a, bf16x8 q) {
+    if constexpr (NOP)
+        asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(a), "a"(q));
+    else
+        asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(a), "a"(q));
+}
+template <bool NOP> DEV void mfma_score(floatx16 &s, bf16x8 a, bf16x8 q) {
+    if constexpr (NOP)
+        asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(a), "a"(q));
+    else
+        asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(a), "a"(q));
+}
+template <bool NOP> DEV void mfma_out(floatx16 &o, bf16x8 a, bf16x8 p) {
+    if constexpr (NOP)
+        asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(p));
+    else
+        asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(p));
+}
+/* before O is read or written by anything but mfma_out, and after */
+DEV void settle(floatx16 (&o)[4][2]) {
+    asm volatile("s_nop 15\n\ts_nop 7"
+                 : "+a"(o[0][0]), "+a"(o[0][1]), "+a"(o[1][0]), "+a"(o[1][1]), "+a"(o[2][0]),
+                   "+a"(o[2][1]), "+a"(o[3][0]), "+a"(o[3][1]));
+}
+
+/* keys hi at most, and past lo or a sink (without branches) */
+DEV bool key_seen(int j, int hi, int lo, int sinks) { return (j <= hi) & ((j > lo) | (j < sinks)); }
 
 /* What both kernels and the merge share. A tile of rows whose key tiles are
  * shared out over several workgroups keeps, per share, unnormalised o, l and
@@ -79,18 +125,23 @@ DEV int page_id(const Call &c, int b, const pg_tiles &t, int i) {
 
 /* ---- few rows: up to 16 packed rows of a sequence and kv-head ------------------
  * Bound by the K/V bytes. A workgroup takes one share of the key tiles; its 4
- * waves take whole tiles in turn and work alone until they merge through LDS.
- * K and V^T go from memory into registers as the operands of
- * v_mfma_f32_16x16x32_bf16 (16 bytes a lane, 64 bytes of 16 rows a load): K of
- * the next tile is in flight during the softmax and the PV products, V^T
- * during the scores, so a wave keeps at least half a tile in flight. */
-constexpr int FEW = 16;
+ * waves take steps (32 keys of bf16, a tile of e4m3) in turn and work alone
+ * until they merge through LDS. K and V^T go from memory into registers as
+ * the operands of v_mfma_f32_16x16x32_bf16, 16 loads each of 16 bytes a lane
+ * (64 bytes of 16 rows): K of the next step is in flight during the softmax and
+ * the PV products, V^T during the scores. All loads are unconditional (past
+ * the end the last step's again), so a wait for one operand's counts the other's
+ * in flight and not more; with 256 registers two waves share a SIMD. */
+constexpr int FEW = 16, FEW_TILES = 64; /* rows; key tiles a share, at most */
 
 template <bool E4M3>
-__global__ __launch_bounds__(256) void attention_few_kernel(Call c) {
+__global__ __launch_bounds__(256, 2) void attention_few_kernel(Call c) {
     __shared__ __attribute__((aligned(16))) float so[4][FEW][PD];
     __shared__ float sl[4][FEW], sm[4][FEW];
-    constexpr int NK = E4M3 ? 16 : 32; /* 16-byte loads of a K or V^T tile */
+    constexpr int KS = E4M3 ? 64 : 32;        /* keys a step */
+    constexpr int SPT = PG / KS;              /* steps a tile */
+    constexpr int NKB = KS / 16;              /* score blocks */
+    constexpr uint32_t EB = E4M3 ? 1 : 2, SLICE = PSLICE * EB;
     const int kh = blockIdx.x, share = blockIdx.y, b = blockIdx.z;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int m = lane & 15, g = lane >> 4;
@@ -102,44 +153,52 @@ __global__ __launch_bounds__(256) void attention_few_kernel(Call c) {
     const int nshare = pg_max(pg_div_up(list.ntl, c.share), 1);
     if (share >= nshare)
         return;
-    const int tb = share * c.share, ntl = min(list.ntl - tb, c.share);
+    const int tb = share * c.share, steps = min(list.ntl - tb, c.share) * SPT;
 
     /* this lane's row (column of S^T and O^T) */
     const int row = min(m, rows - 1), tok = row / c.G, head = kh * c.G + row % c.G;
-    const int pos = s.p0 + tok;
-    bf16x8 qf[8];
-    {
-        const bf16 *qp = c.q + ((size_t)(s.q0 + tok) * c.Hq + head) * PD;
+    const int hi = min(s.p0 + tok, s.kv - 1), lo = pg_low(s.p0 + tok, c.window);
+    const int own_lo = pg_low(s.p0, c.window); /* of the first row: below, no row's key */
+    /* Q's operands wait in LDS (where the merge comes later): read again each
+     * step, they leave the registers to loads in flight */
+    bf16x8 *const qf = (bf16x8 *)&so[0][0][0] + lane;
 #pragma unroll
-        for (int ks = 0; ks < 8; ks++) /* dims of k-step ks: as K's loads below */
-            qf[ks] = *(const bf16x8 *)(qp + (E4M3 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1)
-                                                  : 32 * ks + 8 * g));
+    for (int i = 0; i < 2; i++) {
+        const int ks = 2 * wave + i; /* its dims: as K's loads below */
+        qf[64 * ks] = *(const bf16x8 *)(c.q + ((size_t)(s.q0 + tok) * c.Hq + head) * PD +
+                                        (E4M3 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1)
+                                              : 32 * ks + 8 * g));
     }
-    /* Row m of score block kb is key key0 + 4 kb (e4m3), or key0 + 4 (kb & 1)
-     * + 32 (kb >> 1): lane g then holds, in accumulators 4 kb .. + 3, the keys
-     * its V^T loads bring. */
-    const int key0 = (E4M3 ? 16 : 8) * (m >> 2) + (m & 3);
-    auto kkey = [&](int kb) { return E4M3 ? 4 * kb : 4 * (kb & 1) + 32 * (kb >> 1); };
-    const uint32_t kvoff = E4M3 ? key0 * PD + 16 * g : key0 * PD * 2 + 16 * g;
-    const uint32_t vvoff = E4M3 ? m * PG + 16 * g : m * PG * 2 + 16 * g;
-    constexpr uint32_t SLICE = PSLICE * (E4M3 ? 1 : 2);
-    /* key of accumulator v = 4 kb + i of this lane */
-    auto key_of = [&](int v) { return E4M3 ? 16 * g + v : 8 * g + (v & 7) + 32 * (v >> 3); };
+    /* Row m of score block kb is key key0 + 4 kb of the step: lane g then holds,
+     * in accumulators 4 kb .. + 3, the keys (KS / 4) g .. that its V^T loads
+     * bring. */
+    const int key0 = KS / 4 * (m >> 2) + (m & 3), keyg = KS / 4 * g;
+    const uint32_t kvoff = key0 * PD * EB + 16 * g, vvoff = m * PG * EB + 16 * g;
 
-    u32x4 kr[NK], vr[NK];
+    u32x4 kr[16], vr[16];
     float ksc[4];
-    auto load_k = [&](int page) {
+    /* step t (past the last: it again): its page (-1: not there) and first key;
+     * the ids of the share's tiles, FEW_TILES at most, are in a lane each */
+    const int ids = steps > 0 ? page_id(c, b, list, tb + min(lane, steps / SPT - 1)) : -1;
+    auto locate = [&](int t, int *page, int *k0) {
+        t = min(t, steps - 1);
+        *page = __builtin_amdgcn_readlane(ids, t / SPT);
+        *k0 = pg_tile_page(list, tb + t / SPT) * PG + t % SPT * KS;
+    };
+    auto load_k = [&](int page, int k0) {
         const size_t at = (size_t)max(page, 0) * c.Hkv + kh;
         const __amdgpu_buffer_rsrc_t r = make_rsrc((const char *)c.k + at * SLICE, SLICE);
+        const uint32_t half = k0 % PG * PD * EB;
 #pragma unroll
-        for (int kb = 0; kb < 4; kb++)
+        for (int kb = 0; kb < NKB; kb++)
 #pragma unroll
-            for (int i = 0; i < NK / 4; i++)
-                kr[kb * (NK / 4) + i] = buf_load16(r, kvoff, kkey(kb) * (SLICE / PG) + 64 * i);
+            for (int i = 0; i < 16 / NKB; i++)
+                kr[kb * (16 / NKB) + i] =
+                    buf_load16(r, kvoff, half + 4 * kb * PD * EB + 64 * i);
         if constexpr (E4M3) {
 #pragma unroll
             for (int kb = 0; kb < 4; kb++)
-                ksc[kb] = c.ks[at * PG + key0 + kkey(kb)];
+                ksc[kb] = c.ks[at * PG + key0 + 4 * kb];
         }
     };
 
@@ -148,30 +207,31 @@ __global__ __launch_bounds__(256) void attention_few_kernel(Call c) {
     for (int i = 0; i < 16; i++)
         o[i] = floatx4{};
     float mrun = -INFINITY, lrun = 0.f;
-    int page = wave < ntl ? page_id(c, b, list, tb + wave) : -1;
-    if (wave < ntl)
-        load_k(page);
-    for (int i = wave; i < ntl; i += 4) {
-        const int cur = page, k0 = pg_tile_page(list, tb + i) * PG;
-        const size_t at = (size_t)max(cur, 0) * c.Hkv + kh;
+    int page = -1, k0 = 0;
+    if (wave < steps) {
+        locate(wave, &page, &k0);
+        load_k(page, k0);
+    }
+    lds_barrier();
+    for (int i = wave; i < steps; i += 4) {
+        const bool there = page >= 0;
+        const size_t at = (size_t)max(page, 0) * c.Hkv + kh;
         const __amdgpu_buffer_rsrc_t rv = make_rsrc((const char *)c.vt + at * SLICE, SLICE);
-        floatx4 vsc[4];
-        if constexpr (E4M3) {
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                vsc[e] = *(const floatx4 *)(c.vs + at * PG + 16 * g + 4 * e);
-        }
+        const int kc = k0;
 #pragma unroll
         for (int t = 0; t < 16; t++)
-#pragma unroll
-            for (int h = 0; h < NK / 16; h++)
-                vr[t * (NK / 16) + h] = buf_load16(rv, vvoff, t * 16 * (SLICE / PD) + 64 * h);
-        if (i + 4 < ntl)
-            page = page_id(c, b, list, tb + i + 4);
+            vr[t] = buf_load16(rv, vvoff + (t & 1) * 16 * PG * EB,
+                               (t >> 1) * 32 * PG * EB + kc % PG * EB);
+        /* V's scale of key keyg + m, in lane m of the 16 that need all 16 of them */
+        float vsc = 1.f;
+        if constexpr (E4M3)
+            vsc = c.vs[at * PG + keyg + m];
+        locate(i + 4, &page, &k0);
 
-        floatx4 x[4];
+        asm volatile("" ::: "memory"); /* Q is read here, not kept */
+        floatx4 x[NKB];
 #pragma unroll
-        for (int kb = 0; kb < 4; kb++) {
+        for (int kb = 0; kb < NKB; kb++) {
             x[kb] = floatx4{};
 #pragma unroll
             for (int ks = 0; ks < 8; ks++) {
@@ -182,45 +242,42 @@ __global__ __launch_bounds__(256) void attention_few_kernel(Call c) {
                 } else {
                     a = __builtin_bit_cast(bf16x8, kr[kb * 8 + ks]);
                 }
-                x[kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[ks], x[kb], 0, 0, 0);
+                x[kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[64 * ks], x[kb], 0, 0, 0);
             }
         }
-        if (i + 4 < ntl)
-            load_k(page);
+        load_k(page, k0);
 
-        const bool foreign = cur < 0 || pg_tile_foreign(k0, s.p0, s.kv, c.window, c.sinks);
-        if (foreign) { /* values and scales of no key of this call meet p = 0: make them 0 */
-            auto own = [&](int j) {
-                return cur >= 0 && pg_key_own(k0 + j, s.p0, s.kv, c.window, c.sinks);
-            };
-            u32x4 keep[2];
+        if (!there || kc + KS - 1 > min(s.p0, s.kv - 1) || c.window > 0) { /* some key hidden */
+            const int top = there ? s.kv - 1 : -1;
 #pragma unroll
-            for (int h = 0; h < NK / 16; h++)
+            for (int v = 0; v < KS / 4; v++)
+                x[v >> 2][v & 3] =
+                    hide(key_seen(kc + keyg + v, min(hi, top), lo, c.sinks), x[v >> 2][v & 3]);
+            if (!there || kc + KS > s.kv || kc <= own_lo) {
+                /* values and scales of no key of this call meet p = 0: make them 0 */
+                u32x4 keep;
 #pragma unroll
                 for (int w = 0; w < 4; w++) {
                     uint32_t k = 0;
 #pragma unroll
                     for (int e = 0; e < (E4M3 ? 4 : 2); e++) {
-                        const bool is =
-                            own(E4M3 ? 16 * g + 4 * w + e : 32 * h + 8 * g + 2 * w + e);
+                        const int j = (E4M3 ? 4 : 2) * w + e;
+                        const bool is = key_seen(kc + keyg + j, top, own_lo, c.sinks);
                         k |= is ? (E4M3 ? 0xffu << (8 * e) : 0xffffu << (16 * e)) : 0u;
-                        if constexpr (E4M3)
-                            vsc[w][e] = is ? vsc[w][e] : 0.f;
                     }
-                    keep[h][w] = k;
+                    keep[w] = k;
                 }
+                vsc = __uint_as_float(
+                    key_seen(kc + keyg + m, top, own_lo, c.sinks) ? __float_as_uint(vsc) : 0u);
 #pragma unroll
-            for (int t = 0; t < NK; t++)
-                vr[t] &= keep[t % (NK / 16)];
+                for (int t = 0; t < 16; t++)
+                    vr[t] &= keep;
+            }
         }
         float mx = -INFINITY;
 #pragma unroll
-        for (int v = 0; v < 16; v++) {
-            const bool seen =
-                cur >= 0 && pg_key_seen(k0 + key_of(v), pos, s.kv, c.window, c.sinks);
-            x[v >> 2][v & 3] = hide(seen, x[v >> 2][v & 3]);
+        for (int v = 0; v < KS / 4; v++)
             mx = fmaxf(mx, x[v >> 2][v & 3]);
-        }
         mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
         const float mnew = fmaxf(mrun, mx);
@@ -233,30 +290,32 @@ __global__ __launch_bounds__(256) void attention_few_kernel(Call c) {
                 o[t] *= a;
         }
         mrun = mnew;
-        bf16x8 p[2];
-#pragma unroll
-        for (int v = 0; v < 16; v++) {
+        bf16x8 p[NKB / 2];
+        unroll_for<KS / 4>([&](auto iv) {
+            constexpr int v = decltype(iv)::value;
             float pv = fast_exp2(x[v >> 2][v & 3] - ref);
             lrun += pv;
             if constexpr (E4M3)
-                pv *= vsc[v >> 2][v & 3];
+                pv *= row_lane<v>(vsc);
             p[v >> 3][v & 7] = f2bf(pv);
-        }
+        });
 #pragma unroll
-        for (int t = 0; t < 16; t++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                bf16x8 a;
-                if constexpr (E4M3)
-                    a = h ? widen(vr[t][2], vr[t][3], 1.f) : widen(vr[t][0], vr[t][1], 1.f);
-                else
-                    a = __builtin_bit_cast(bf16x8, vr[2 * t + h]);
-                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, p[h], o[t], 0, 0, 0);
+        for (int t = 0; t < 16; t++) {
+            if constexpr (E4M3) {
+                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(vr[t][0], vr[t][1], 1.f),
+                                                               p[0], o[t], 0, 0, 0);
+                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(vr[t][2], vr[t][3], 1.f),
+                                                               p[1], o[t], 0, 0, 0);
+            } else {
+                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vr[t]),
+                                                               p[0], o[t], 0, 0, 0);
             }
+        }
     }
     lrun += __shfl_xor(lrun, 16, 64);
     lrun += __shfl_xor(lrun, 32, 64);
 
+    __syncthreads(); /* Q is read */
     /* merge the waves; lane (m, g) holds dims 16 t + 4 g .. + 3 of row m */
 #pragma unroll
     for (int t = 0; t < 16; t++)
@@ -383,12 +442,13 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
 
     /* Q^T operands of this wave's 64 rows; rows past the last repeat it */
     bf16x8 qf[2][16];
-    int pos[2];
+    int hi[2], lo[2];
 #pragma unroll
     for (int rb = 0; rb < 2; rb++) {
         const int r = r0 + min(64 * wi + 32 * rb + col, nrows - 1);
         const int tok = r / c.G, head = kh * c.G + r % c.G;
-        pos[rb] = s.p0 + tok;
+        hi[rb] = min(s.p0 + tok, s.kv - 1);
+        lo[rb] = pg_low(s.p0 + tok, c.window);
         const bf16 *qp = c.q + ((size_t)(s.q0 + tok) * c.Hq + head) * PD;
 #pragma unroll
         for (int ks = 0; ks < 16; ks++)
@@ -496,6 +556,16 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
                     : 1.f;
     };
 
+    auto score = [&](floatx16 (&y)[2], bf16x8 a, int ks) { /* k-step ks of S^T */
+        if (ks == 0) {
+            mfma_first<E4M3>(y[0], a, qf[0][0]);
+            mfma_first<false>(y[1], a, qf[1][0]);
+        } else {
+            mfma_score<E4M3>(y[0], a, qf[0][ks]);
+            mfma_score<false>(y[1], a, qf[1][ks]);
+        }
+    };
+
     int pg[4]; /* pages of tiles i .. i + 3 */
     auto step = [&](auto has_next, int i, auto parity, floatx16 (&x)[2], floatx16 (&y)[2]) {
         constexpr bool NEXT = decltype(has_next)::value;
@@ -512,17 +582,17 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
         }
         if (!there || !pg_tile_whole(k0, pmin, pmax, s.kv, c.window, c.sinks)) {
             const int kb = k0 + 32 * wj + (E4M3 ? 16 : 8) * h;
+            const int top = there ? s.kv - 1 : -1, low = pg_low(pmin, c.window);
 #pragma unroll
-            for (int rb = 0; rb < 2; rb++)
+            for (int r = 0; r < 16; r++) {
+                const int j = kb + (E4M3 ? r : 16 * (r >> 3) + (r & 7));
 #pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int j = kb + (E4M3 ? r : 16 * (r >> 3) + (r & 7));
-                    x[rb][r] = hide(
-                        there && pg_key_seen(j, pos[rb], s.kv, c.window, c.sinks), x[rb][r]);
-                    if constexpr (E4M3) /* a scale of no key of this call: any bits */
-                        if (!there || !pg_key_own(j, pmin, s.kv, c.window, c.sinks))
-                            vsc[r >> 2][r & 3] = 0.f;
-                }
+                for (int rb = 0; rb < 2; rb++)
+                    x[rb][r] = hide(key_seen(j, min(hi[rb], top), lo[rb], c.sinks), x[rb][r]);
+                if constexpr (E4M3) /* a scale of no key of this call: any bits */
+                    vsc[r >> 2][r & 3] = __uint_as_float(
+                        key_seen(j, top, low, c.sinks) ? __float_as_uint(vsc[r >> 2][r & 3]) : 0u);
+            }
         }
         /* ---- S^T of tile i + 1 with the softmax of tile i ---- */
         u32x4 ring[QD];
@@ -542,8 +612,11 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
                 a *= vsc[v >> 2][v & 3];
                 e *= vsc[v >> 2][(v & 3) + 1];
             }
-            pf[rb][v >> 3][v & 7] = f2bf(a);
-            pf[rb][v >> 3][(v & 7) + 1] = f2bf(e);
+            /* the empty asm keeps the pair in its place among the MFMAs */
+            bf16x2 pk = {f2bf(a), f2bf(e)};
+            asm volatile("" : "+v"(pk), "+v"(ls[rb]));
+            pf[rb][v >> 3][v & 7] = pk[0];
+            pf[rb][v >> 3][(v & 7) + 1] = pk[1];
         };
         __builtin_amdgcn_sched_barrier(0);
         bf16x8 odd = {};
@@ -566,10 +639,7 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
                     if (ks + QD < NKR)
                         ring[ks % QD] = lds_read16(lds, kaddr(ks + QD, PAR ^ 1));
                 }
-#pragma unroll
-                for (int rb = 0; rb < 2; rb++)
-                    y[rb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                        a, qf[rb][ks], ks == 0 ? floatx16{} : y[rb], 0, 0, 0);
+                score(y, a, ks);
             }
             mx[ks >> 3] = fmaxf(mx[ks >> 3], fmaxf(x[ks >> 3][2 * (ks & 7)],
                                                    x[ks >> 3][2 * (ks & 7) + 1]));
@@ -598,21 +668,23 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
 #pragma unroll
                 for (int v = 0; v < 16; v += 2)
                     pair(rb, v, shift);
+#pragma unroll
+                for (int st = 0; st < 2; st++) {
+                    u32x4 w = __builtin_bit_cast(u32x4, pf[rb][st]);
+                    const uint32_t u = __float_as_uint(mul[rb]) >> (16 * h + 8 * st);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        w[e] |= ((u >> (2 * e)) & 1) << 15 | ((u >> (2 * e + 1)) & 1) << 31;
+                    pf[rb][st] = __builtin_bit_cast(bf16x8, w);
+                }
             }
         }
 #pragma unroll
         for (int rb = 0; rb < 2; rb++)
 #pragma unroll
-            for (int st = 0; st < 2; st++) {
-                u32x4 w = __builtin_bit_cast(u32x4, pf[rb][st]);
-                if (__builtin_expect(moved, 0)) {
-                    const uint32_t u = __float_as_uint(mul[rb]) >> (16 * h + 8 * st);
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        w[e] |= ((u >> (2 * e)) & 1) << 15 | ((u >> (2 * e + 1)) & 1) << 31;
-                }
-                lds_write16(smem, psend + PAR * L::PBUF + (2 * rb + st) * 1024, w);
-            }
+            for (int st = 0; st < 2; st++)
+                lds_write16(smem, psend + PAR * L::PBUF + (2 * rb + st) * 1024,
+                            __builtin_bit_cast(u32x4, pf[rb][st]));
         /* P is in LDS, this wave's reads of K are done, its tile loads have landed */
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
@@ -633,7 +705,7 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
                         const int j =
                             k0 + (E4M3 ? 16 * piece + 4 * e + f : 8 * piece + 2 * e + f);
                         const bool own =
-                            there && pg_key_own(j, pmin, s.kv, c.window, c.sinks);
+                            there && key_seen(j, s.kv - 1, pg_low(pmin, c.window), c.sinks);
                         keep |= own ? (E4M3 ? 0xffu << (8 * f) : 0xffffu << (16 * f)) : 0u;
                     }
                     w[e] &= keep;
@@ -651,6 +723,7 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
                 pw[rb][st] = lds_read16(lds, precv + PAR * L::PBUF + (2 * rb + st) * 1024);
         /* Both waves' references of a row are known: take the larger one */
         auto agree = [&]() {
+            settle(o);
 #pragma unroll
             for (int rb = 0; rb < 2; rb++) {
                 uint32_t u = 0;
@@ -676,16 +749,20 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
                 mus[rb] = ref;
 #pragma unroll
                 for (int st = 0; st < 2; st++) {
-                    pw[rb][st] &= 0x7fff7fffu;
-                    bf16x8 t = __builtin_bit_cast(bf16x8, pw[rb][st]);
+                    bf16x8 t = __builtin_bit_cast(bf16x8, pw[rb][st] & 0x7fff7fffu);
+                    bf16x8 w = __builtin_bit_cast(
+                        bf16x8, __builtin_bit_cast(u32x4, pf[rb][st]) & 0x7fff7fffu);
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
                         t[e] = f2bf(bf2f(t[e]) * fp);
-                        pf[rb][st][e] = f2bf(bf2f(pf[rb][st][e]) * fm);
+                        w[e] = f2bf(bf2f(w[e]) * fm);
                     }
                     pw[rb][st] = __builtin_bit_cast(u32x4, t);
+                    pf[rb][st] = w;
+                    asm volatile("s_nop 1" : "+v"(pw[rb][st]), "+v"(pf[rb][st]));
                 }
             }
+            settle(o);
         };
         /* ---- O^T += V^T P^T: own keys, then the other wave's ---- */
         const __amdgpu_buffer_rsrc_t rk = k_rsrc(pg[3]), rv = v_rsrc(pg[1]);
@@ -727,11 +804,11 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
                     else
                         a = __builtin_bit_cast(bf16x8, w);
                     const int d = E4M3 ? n : n & 3, st = E4M3 ? half : n >> 2;
-#pragma unroll
-                    for (int rb = 0; rb < 2; rb++) {
-                        const bf16x8 p = kb ? __builtin_bit_cast(bf16x8, pw[rb][st]) : pf[rb][st];
-                        o[d][rb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, p, o[d][rb], 0, 0, 0);
-                    }
+                    auto p = [&](int rb) {
+                        return kb ? __builtin_bit_cast(bf16x8, pw[rb][st]) : pf[rb][st];
+                    };
+                    mfma_out<E4M3>(o[d][0], a, p(0));
+                    mfma_out<false>(o[d][1], a, p(1));
                     if constexpr (NEXT) { /* one tile load beside each pair of MFMAs */
                         const int at = E4M3 ? (kb * NVR + n) * 2 + half : kb * NVR + n;
                         if (E4M3 ? !(at & 1) : true) {
@@ -785,12 +862,10 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
                     else
                         a = __builtin_bit_cast(bf16x8, w);
                     const int ks = E4M3 ? 2 * n + half : n;
-#pragma unroll
-                    for (int rb = 0; rb < 2; rb++)
-                        xa[rb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                            a, qf[rb][ks], ks == 0 ? floatx16{} : xa[rb], 0, 0, 0);
+                    score(xa, a, ks);
                 }
             }
+            asm volatile("s_nop 15\n\ts_nop 7" : "+v"(xa[0]), "+v"(xa[1]));
         }
         __syncthreads(); /* K buffer 0 is free */
         {
@@ -817,6 +892,7 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
         }
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     }
+    settle(o);
     __syncthreads(); /* the tile buffers are idle: O and the rows' l go there */
 
     /* ---- epilogue: O as fp32 rows of 1 KiB through LDS (piece p of row r in slot
@@ -944,6 +1020,8 @@ static paged_plan plan_of(int N, int B, int max_q, int max_kv, int G, int Hkv, i
     p.share = pg_div_up(most, n);
     if (p.share < 4)
         p.share = 4;
+    if (p.rt == FEW && p.share > FEW_TILES)
+        p.share = FEW_TILES;
     p.nshare = pg_div_up(most, p.share);
     return p;
 }

@@ -22,18 +22,28 @@ DEV pg_seq load_seq(const int32_t *q_start, const int32_t *kv_len, int b, int N,
     return pg_clean_seq(q_start[b], q_start[b + 1], kv_len[b], N, max_q, max_kv);
 }
 
-/* The sequence of row n: the last b with q_start[b] <= n, -1 for a row before
- * the first or behind the last sequence. One load of 64 starts a step. */
-DEV int find_seq(const int32_t *q_start, int B, int n) {
+/* The sequences of rows n0 .. n0 + TOK - 1, row n0 + t in lane t: the last b
+ * with q_start[b] <= n, -1 for a row before the first or behind the last
+ * sequence. One load of 64 starts a step. */
+template <int TOK> DEV int find_seqs(const int32_t *q_start, int B, int n0) {
     const int lane = threadIdx.x & 63;
-    int before = 0; /* starts <= n among q_start[0 .. B] */
+    int before[TOK] = {}; /* starts <= n among q_start[0 .. B] */
     for (int b0 = 0; b0 <= B; b0 += 64) {
-        const int c = __popcll(__ballot(b0 + lane <= B && q_start[min(b0 + lane, B)] <= n));
-        before += c;
+        const int v = q_start[min(b0 + lane, B)];
+        int c = 0;
+#pragma unroll
+        for (int t = 0; t < TOK; t++) {
+            c = __popcll(__ballot(b0 + lane <= B && v <= n0 + t));
+            before[t] += c;
+        }
         if (c < 64)
             break;
     }
-    return before == 0 || before > B ? -1 : before - 1;
+    int b = before[0];
+#pragma unroll
+    for (int t = 1; t < TOK; t++)
+        b = lane == t ? before[t] : b;
+    return b == 0 || b > B ? -1 : b - 1;
 }
 
 /* Work item `item` of a launch whose sequence b has count(b, s) of them, in

@@ -43,71 +43,90 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(
         for (int t = 0; t < TOK; t++)
             raw[t] = *(const bf16x4 *)(src + (size_t)min(n0 + t, N - 1) * ps);
         const float4 wl = *(const float4 *)(w + 4 * lane);
+        const int pos_lane = min(max(pos[min(n0 + (lane & (TOK - 1)), N - 1)], 0), npos - 1);
+        /* The tokens' sequences, then (K) their slots, token t in lane t: one
+         * chain of loads for all of them. at: the K row in the pool, -1: none */
+        int b = find_seqs<TOK>(q_start, B, n0);
         float4 rc[TOK][2];
 #pragma unroll
         for (int t = 0; t < TOK; t++) {
-            const int p = min(max(pos[min(n0 + t, N - 1)], 0), npos - 1);
-            const float4 *r = (const float4 *)(rope + (size_t)p * (rot / 2) + fi0);
+            const float4 *r = (const float4 *)(
+                rope + (size_t)__builtin_amdgcn_readlane(pos_lane, t) * (rot / 2) + fi0);
             rc[t][0] = r[0];
             rc[t][1] = r[1];
         }
+        if (n0 + lane >= N)
+            b = -1;
+        long long at = b;
+        if (is_k) {
+            const pg_seq s = load_seq(q_start, kv_len, max(b, 0), N, N, max_pages * PG);
+            const int p = s.p0 + (n0 + lane - s.q0);
+            const bool in = b >= 0 && (unsigned)(n0 + lane - s.q0) < (unsigned)s.ql && p >= 0 &&
+                            p < s.kv;
+            const int page = page_table[(size_t)max(b, 0) * max_pages + (in ? p / PG : 0)];
+            at = in && page >= 0 && page < num_pages
+                     ? ((long long)page * Hkv + head - Hq) * PG + p % PG
+                     : -1;
+        }
+        float x[TOK][4], ss[TOK];
 #pragma unroll
         for (int t = 0; t < TOK; t++) {
-            const int n = n0 + t;
-            if (n >= N)
-                continue;
-            float x[4], ss = 0.f;
+            ss[t] = 0.f;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                x[e] = bf2f(raw[t][e]);
-                ss += x[e] * x[e];
+                x[t][e] = bf2f(raw[t][e]);
+                ss[t] += x[t][e] * x[t][e];
             }
-            const float rinv = rsqrtf(wave_sum(ss) * (1.f / 256.f) + eps);
-            x[0] = x[0] * rinv * wl.x;
-            x[1] = x[1] * rinv * wl.y;
-            x[2] = x[2] * rinv * wl.z;
-            x[3] = x[3] * rinv * wl.w;
-            float other[4];
+        }
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                other[e] = __shfl_xor(x[e], half_lanes, 64);
-            if (rotates) {
-                const float cz[8] = {rc[t][0].x, rc[t][0].y, rc[t][0].z, rc[t][0].w,
-                                     rc[t][1].x, rc[t][1].y, rc[t][1].z, rc[t][1].w};
+        for (int o = 32; o > 0; o >>= 1)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float c = cz[2 * e], sn = cz[2 * e + 1];
-                    x[e] = first ? x[e] * c - other[e] * sn : x[e] * c + other[e] * sn;
-                }
+            for (int t = 0; t < TOK; t++)
+                ss[t] += __shfl_xor(ss[t], o, 64);
+        const float we[4] = {wl.x, wl.y, wl.z, wl.w};
+        float amax[TOK];
+#pragma unroll
+        for (int t = 0; t < TOK; t++) {
+            const float rinv = rsqrtf(ss[t] * (1.f / 256.f) + eps);
+            const float cz[8] = {rc[t][0].x, rc[t][0].y, rc[t][0].z, rc[t][0].w,
+                                 rc[t][1].x, rc[t][1].y, rc[t][1].z, rc[t][1].w};
+            amax[t] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float y = x[t][e] * rinv * we[e];
+                /* rounded as attn_prep rounds: the same bits reach both caches */
+                const float o = __shfl_xor(y, half_lanes, 64) * cz[2 * e + 1];
+                x[t][e] = rotates ? __builtin_fmaf(y, cz[2 * e], first ? -o : o) : y;
+                amax[t] = fmaxf(amax[t], fabsf(x[t][e]));
             }
-            const int b = find_seq(q_start, B, n);
-            if (b < 0) /* no sequence's row */
+        }
+        if (E4M3 && is_k) {
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1)
+#pragma unroll
+                for (int t = 0; t < TOK; t++)
+                    amax[t] = fmaxf(amax[t], __shfl_xor(amax[t], o, 64));
+        }
+#pragma unroll
+        for (int t = 0; t < TOK; t++) {
+            const long long row =
+                (long long)(uint32_t)__builtin_amdgcn_readlane((int)at, t) |
+                (long long)__builtin_amdgcn_readlane((int)(at >> 32), t) << 32;
+            if (row < 0) /* no sequence's row, or no slot */
                 continue;
+            const float f = is_k ? 1.f : q_scale;
+            const bf16x4 o = {f2bf(x[t][0] * f), f2bf(x[t][1] * f), f2bf(x[t][2] * f),
+                              f2bf(x[t][3] * f)};
             if (!is_k) {
-                const bf16x4 o = {f2bf(x[0] * q_scale), f2bf(x[1] * q_scale),
-                                  f2bf(x[2] * q_scale), f2bf(x[3] * q_scale)};
-                *(bf16x4 *)(q_out + ((size_t)n * Hq + head) * 256 + 4 * lane) = o;
-                continue;
-            }
-            const pg_seq s = load_seq(q_start, kv_len, b, N, N, max_pages * PG);
-            const int p = s.p0 + (n - s.q0);
-            if ((unsigned)(n - s.q0) >= (unsigned)s.ql || p < 0 || p >= s.kv)
-                continue;
-            const int page = page_table[(size_t)b * max_pages + p / PG];
-            if (page < 0 || page >= num_pages)
-                continue;
-            const size_t row = ((size_t)page * Hkv + head - Hq) * PG + p % PG;
-            if constexpr (E4M3) {
-                const float a = wave_max(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])),
-                                               fmaxf(fabsf(x[2]), fabsf(x[3]))));
-                const int e = e4m3_exp(a);
+                *(bf16x4 *)(q_out + ((size_t)(n0 + t) * Hq + head) * 256 + 4 * lane) = o;
+            } else if constexpr (E4M3) {
+                const int e = e4m3_exp(amax[t]);
                 const float inv = exp2_int(-e);
-                ((uint32_t *)k_pages)[row * 64 + lane] =
-                    pack_e4m3(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+                ((uint32_t *)k_pages)[row * 64 + lane] = pack_e4m3(
+                    x[t][0] * inv, x[t][1] * inv, x[t][2] * inv, x[t][3] * inv);
                 if (lane == 0)
                     k_scale[row] = exp2_int(e);
             } else {
-                const bf16x4 o = {f2bf(x[0]), f2bf(x[1]), f2bf(x[2]), f2bf(x[3])};
                 *(bf16x4 *)((bf16 *)k_pages + row * 256 + 4 * lane) = o;
             }
         }
@@ -128,8 +147,6 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(
         return;
     const int base = (pg_new_lo(s) / VTOK + g) * VTOK; /* the group's first position */
     const int page = page_table[(size_t)b * max_pages + base / PG];
-    if (page < 0 || page >= num_pages)
-        return;
     const int lo = max(pg_new_lo(s), base), hi = min(pg_new_hi(s), base + VTOK);
     const bf16 *src = proj + Hq * 512 + Hkv * 256 + kh * 256 + 4 * lane;
     bf16x4 v[VTOK];
@@ -138,6 +155,8 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(
         const int p = min(max(base + t, lo), hi - 1);
         v[t] = *(const bf16x4 *)(src + (size_t)(s.q0 + p - s.p0) * ps);
     }
+    if (page < 0 || page >= num_pages)
+        return;
     const size_t head = (size_t)page * Hkv + kh;
     const int col = base % PG;
     const bool whole = hi - lo == VTOK;
@@ -221,10 +240,10 @@ __global__ __launch_bounds__(256) void page_read_kernel(
     const int32_t *__restrict__ page_table, int max_pages, const int32_t *__restrict__ kv_len,
     int max_kv, int Hkv, bf16 *__restrict__ kc, bf16 *__restrict__ vtc, int stride) {
     const int j = blockIdx.x >> 1, b = blockIdx.z, kh = blockIdx.y, tid = threadIdx.x;
+    const int page = page_table[(size_t)b * max_pages + j]; /* beside kv_len's load */
     const int kv = min(kv_len[b], max_kv), left = kv - j * PG; /* tokens of this page */
     if (left <= 0)
         return;
-    const int page = page_table[(size_t)b * max_pages + j];
     const bool ok = page >= 0 && page < num_pages;
     const size_t head = (size_t)(ok ? page : 0) * Hkv + kh;
     const size_t out = ((size_t)b * Hkv + kh) * PD * (size_t)stride;

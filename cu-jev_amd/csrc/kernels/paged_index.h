@@ -78,11 +78,9 @@ constexpr bool pg_tile_whole(int k0, int pmin, int pmax, int kv, int window, int
 constexpr bool pg_tile_foreign(int k0, int pmin, int kv, int window, int sinks) {
     return k0 + PG > kv || (window > 0 && k0 <= pmin - window && k0 + PG > sinks);
 }
-constexpr bool pg_key_own(int j, int pmin, int kv, int window, int sinks) {
-    return j < kv && (window <= 0 || j > pmin - window || j < sinks);
-}
-constexpr bool pg_key_seen(int j, int p, int kv, int window, int sinks) {
-    return j <= p && j < kv && (window <= 0 || j > p - window || j < sinks);
-}
+/* The row at position p sees the keys j <= min(p, kv - 1) with j > pg_low or j <
+ * sinks; a key is some row's from pmin on where it is before kv and past
+ * pg_low(pmin) or a sink. */
+constexpr int pg_low(int p, int window) { return window > 0 ? p - window : -1; }
 
 #endif

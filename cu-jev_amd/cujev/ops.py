@@ -216,29 +216,28 @@ class KvPages:
     [pages, Hkv, 64] (powers of two). The tensors are the caller's; kv_pages()
     makes new ones."""
 
-    __slots__ = ("k", "vt", "k_scale", "v_scale", "num_pages", "Hkv", "e4m3", "args")
+    __slots__ = ("k", "vt", "k_scale", "v_scale", "num_pages", "Hkv", "e4m3", "device", "args")
 
     def __init__(self, k, vt, k_scale=None, v_scale=None):
         import torch
-        self.e4m3 = k.dtype == torch.float8_e4m3fn
-        if k.dim() != 4 or k.shape[2:] != (KV_PAGE, 256):
-            raise OpsError(f"KvPages: k is {tuple(k.shape)}, not [pages, Hkv, {KV_PAGE}, 256]")
-        self.num_pages, self.Hkv = k.shape[0], k.shape[1]
-        want = (self.num_pages, self.Hkv)
-        if not self.e4m3 and k.dtype != torch.bfloat16:
-            raise OpsError(f"KvPages: pages are bfloat16 or float8_e4m3fn, not {k.dtype}")
-        _need("vt", vt, k.dtype, k.device, want + (256, KV_PAGE))
-        _need("k", k, k.dtype, k.device, want + (KV_PAGE, 256))
+        t, dev, shape = k.dtype, k.get_device(), k.shape
+        if len(shape) != 4 or t is not torch.bfloat16 and t is not torch.float8_e4m3fn:
+            raise OpsError(f"KvPages: k is {t} {tuple(shape)}, not bfloat16 or float8_e4m3fn "
+                           f"[pages, Hkv, {KV_PAGE}, 256]")
+        n, Hkv = self.num_pages, self.Hkv = shape[0], shape[1]
+        self.e4m3 = t is torch.float8_e4m3fn
+        _need("k", k, t, dev, (n, Hkv, KV_PAGE, 256))
+        _need("vt", vt, t, dev, (n, Hkv, 256, KV_PAGE))
+        ks = vs = None
         if self.e4m3:
-            _need("k_scale", k_scale, torch.float32, k.device, want + (KV_PAGE,))
-            _need("v_scale", v_scale, torch.float32, k.device, want + (KV_PAGE,))
+            _need("k_scale", k_scale, torch.float32, dev, (n, Hkv, KV_PAGE))
+            _need("v_scale", v_scale, torch.float32, dev, (n, Hkv, KV_PAGE))
+            ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
         elif k_scale is not None or v_scale is not None:
             raise OpsError("KvPages: bfloat16 pages have no scales")
-        self.k, self.vt, self.k_scale, self.v_scale = k, vt, k_scale, v_scale
+        self.k, self.vt, self.k_scale, self.v_scale, self.device = k, vt, k_scale, v_scale, dev
         # kv_type, k, vt, k_scale, v_scale, num_pages of the C calls
-        self.args = (int(self.e4m3), k.data_ptr(), vt.data_ptr(),
-                     k_scale.data_ptr() if self.e4m3 else None,
-                     v_scale.data_ptr() if self.e4m3 else None, self.num_pages)
+        self.args = (1 if self.e4m3 else 0, k.data_ptr(), vt.data_ptr(), ks, vs, n)
 
 
 def kv_pages(num_pages, Hkv, e4m3=False, device="cuda"):
@@ -252,33 +251,39 @@ def kv_pages(num_pages, Hkv, e4m3=False, device="cuda"):
                    z(num_pages, Hkv, 256, KV_PAGE).contiguous(), *sc)
 
 
-def _need(name, t, dtype, device, shape):
-    """A contiguous tensor of this type, device and shape, or an OpsError (None in
-    a shape: any size)."""
-    if t is None or t.dtype != dtype or t.device != device or not t.is_contiguous() or \
-            len(t.shape) != len(shape) or any(b is not None and a != b
-                                              for a, b in zip(t.shape, shape)):
+def _need(name, t, dtype, dev, shape):
+    """A contiguous tensor of this type, device index (-1: CPU) and shape, or an
+    OpsError. Cheap: a call on a few tokens takes the device 5 us."""
+    if t is None or t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or \
+            t.get_device() != dev:
         got = "None" if t is None else f"{t.dtype} {tuple(t.shape)} on {t.device}" + (
             "" if t.is_contiguous() else ", not contiguous")
-        raise OpsError(f"{name}: need contiguous {dtype} {shape} on {device}, got {got}")
+        raise OpsError(f"{name}: need contiguous {dtype} {shape} on device {dev}, got {got}")
 
 
-def _paged_call(device, name, *args):
-    """_call on the device of the pages, on its current stream there."""
+def _paged_call(dev, name, *args):
+    """A call on the device of the pages, on that device's current stream."""
     import torch
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _call(name, *args, torch.cuda.current_stream().cuda_stream)
-    return _call(name, *args, torch.cuda.current_stream().cuda_stream)
+    fn = getattr(_lib or load(), name)
+    if dev == torch.cuda.current_device():
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            st = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if st != 0:
+        raise OpsError(f"{name}: status {st}: {_lib.cujev_ops_last_error().decode()}")
 
 
 def _paged_seqs(pages, page_table, kv_len, q_start=None):
     import torch
-    dev, B = pages.k.device, page_table.shape[0]
-    _need("page_table", page_table, torch.int32, dev, (B, None))
-    _need("kv_len", kv_len, torch.int32, dev, (B,))
+    dev, i32, shape = pages.device, torch.int32, page_table.shape
+    if len(shape) != 2:
+        raise OpsError(f"page_table: need [B, max_pages], got {tuple(shape)}")
+    B = shape[0]
+    _need("page_table", page_table, i32, dev, shape)
+    _need("kv_len", kv_len, i32, dev, (B,))
     if q_start is not None:
-        _need("q_start", q_start, torch.int32, dev, (B + 1,))
+        _need("q_start", q_start, i32, dev, (B + 1,))
     return dev, B
 
 
@@ -290,13 +295,13 @@ def attn_prep_paged(proj, q_norm_w, k_norm_w, pos, q_start, kv_len, page_table, 
     import torch
     dev, B = _paged_seqs(pages, page_table, kv_len, q_start)
     N, Hkv = proj.shape[0], pages.Hkv
-    if proj.dtype != torch.bfloat16 or proj.device != dev or proj.dim() != 2 or \
+    if proj.dtype is not torch.bfloat16 or proj.get_device() != dev or proj.dim() != 2 or \
             proj.stride(1) != 1 or proj.shape[1] < Hq * 512 + Hkv * 512:
-        raise OpsError(f"proj: need bfloat16 rows of {Hq * 512 + Hkv * 512} values on {dev}")
+        raise OpsError(f"proj: need bfloat16 rows of {Hq * 512 + Hkv * 512} values on device {dev}")
     _need("q_norm_w", q_norm_w, torch.float32, dev, (256,))
     _need("k_norm_w", k_norm_w, torch.float32, dev, (256,))
     _need("pos", pos, torch.int32, dev, (N,))
-    _need("rope", rope, torch.float32, dev, (None, rot // 2, 2))
+    _need("rope", rope, torch.float32, dev, (rope.shape[0], rot // 2, 2))
     _need("q_out", q_out, torch.bfloat16, dev, (N, Hq, 256))
     _paged_call(dev, "cujev_op_attn_prep_paged", proj.data_ptr(), proj.stride(0),
                 q_norm_w.data_ptr(), k_norm_w.data_ptr(), pos.data_ptr(), q_start.data_ptr(),
@@ -337,13 +342,13 @@ def attention_paged(q, gate, gate_tok_stride, gate_head_stride, pages, page_tabl
     _need("out", out, torch.bfloat16, dev, (N, Hq * 256))
     if gate is not None:
         last = (N - 1) * gate_tok_stride + (Hq - 1) * gate_head_stride + 256
-        if gate.dtype != torch.bfloat16 or gate.device != dev or min(gate_tok_stride,
-                                                                     gate_head_stride) < 0 or \
-                N > 0 and gate.untyped_storage().nbytes() < 2 * (gate.storage_offset() + last):
-            raise OpsError(f"gate: need bfloat16 on {dev}, with {N} rows and {Hq} heads at these "
-                           "strides")
+        if gate.dtype is not torch.bfloat16 or gate.get_device() != dev or gate_tok_stride < 0 or \
+                gate_head_stride < 0 or N > 0 and \
+                gate.untyped_storage().nbytes() < 2 * (gate.storage_offset() + last):
+            raise OpsError(f"gate: need bfloat16 on device {dev}, with {N} rows and {Hq} heads at "
+                           "these strides")
     if ws is not None:
-        _need("ws", ws, torch.uint8, dev, (None,))
+        _need("ws", ws, torch.uint8, dev, (ws.numel(),))
     _paged_call(dev, "cujev_op_attention_paged", q.data_ptr(),
                 None if gate is None else gate.data_ptr(), gate_tok_stride, gate_head_stride,
                 *pages.args, q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(),

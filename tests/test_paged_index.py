@@ -18,6 +18,8 @@ static int bad;
 static unsigned rs = 12345;
 static int rnd(int lo, int hi) { rs = rs * 1664525u + 1013904223u; return lo + (int)((rs >> 4) % (unsigned)(hi - lo + 1)); }
 
+static bool seen(int j, int hi, int lo, int S) { return j <= hi && (j > lo || j < S); }
+
 int main() {
     /* any lengths at all stay inside the call */
     const int odd[] = {0, 1, -1, 5, 63, 64, 65, 200, 4096, PG_MOST, -PG_MOST, 0x7fffffff, (int)0x80000000};
@@ -57,11 +59,11 @@ int main() {
                 bool own = false;
                 for (int p = pmin; p <= pmax; p++) {
                     const bool sees = j <= p && j < s.kv && (!w || j > p - w || j < S);
-                    NEED(sees == pg_key_seen(j, p, s.kv, w, S));
+                    NEED(sees == seen(j, pg_min(p, s.kv - 1), pg_low(p, w), S));
                     whole &= sees, own |= sees;
                 }
-                NEED(!own || pg_key_own(j, pmin, s.kv, w, S));
-                foreign |= !pg_key_own(j, pmin, s.kv, w, S);
+                NEED(!own || seen(j, s.kv - 1, pg_low(pmin, w), S));
+                foreign |= !seen(j, s.kv - 1, pg_low(pmin, w), S);
             }
             NEED(!pg_tile_whole(pg * PG, pmin, pmax, s.kv, w, S) || whole);
             NEED(!foreign || pg_tile_foreign(pg * PG, pmin, s.kv, w, S));
@@ -69,7 +71,7 @@ int main() {
             NEED(!pg_tile_foreign(pg * PG, pmin, s.kv, w, S) || !pg_tile_whole(pg * PG, pmin, pmax, s.kv, w, S));
         }
         for (int p = pmin; p <= pmax; p++) for (int j = 0; j < s.kv; j++)
-            NEED(!pg_key_seen(j, p, s.kv, w, S) || visited.count(j / PG));
+            NEED(!seen(j, pg_min(p, s.kv - 1), pg_low(p, w), S) || visited.count(j / PG));
         NEED(t.ntl <= pg_max_tiles(i1 - i0 + 1, mk, w, S));
         NEED(t.ntl <= pg_max_tiles(i1 - i0 + 1 + rnd(0, 50), mk, w, S));
     }
