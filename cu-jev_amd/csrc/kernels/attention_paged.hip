@@ -65,13 +65,17 @@ DEV float hide(bool seen, float x) {
  * for as for any instruction. */
 template <bool NOP> DEV void mfma_first(floatx16 &s, bf16x8 a, bf16x8 q) {
     if constexpr (NOP)
-        asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(a), "a"(q));
+        asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(a), "v"(q));
     else
-        asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(a), "a"(q));
+        asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(a), "v"(q));
 }
-template <bool NOP> DEV void mfma_score(floatx16 &s, bf16x8 a, bf16x8 q) {
-    if constexpr (NOP)
+template <bool NOP, bool QV> DEV void mfma_score(floatx16 &s, bf16x8 a, bf16x8 q) {
+    if constexpr (NOP && QV)
+        asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(a), "v"(q));
+    else if constexpr (NOP)
         asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(a), "a"(q));
+    else if constexpr (QV)
+        asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(a), "v"(q));
     else
         asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(a), "a"(q));
 }
@@ -542,10 +546,15 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
 #pragma unroll
         for (int rb = 0; rb < 2; rb++)
             o[d][rb] = floatx16{};
+    /* per row: running maximum, l, the reference agreed on; of the current tile:
+     * its p, their sum, the reference this wave wants */
     float mrun[2] = {-INFINITY, -INFINITY}, lrun[2] = {0.f, 0.f}, mus[2] = {0.f, 0.f};
+    float mx[2], ls[2], mul[2];
+    bf16x8 pf[2][2], pn[2];
+    floatx4 vsc[4];
+    bool moved = false;
 
-    /* One k-step pair or step of S^T: operand reads QD ahead */
-    constexpr int QD = E4M3 ? 2 : 4;
+    constexpr int QD = E4M3 ? 2 : 4;   /* K operand reads ahead */
     constexpr int NKR = E4M3 ? 8 : 16; /* K reads a tile */
     auto kaddr = [&](int n, int buf) {
         return (E4M3 ? ka[n] : ka[n & 7] + (n >> 3) * 256) + buf * L::T;
@@ -555,99 +564,66 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
                                                                          (32 * wj + arow) * 4)
                     : 1.f;
     };
-
+    constexpr int QV = 4; /* k-steps whose Q is in ordinary registers */
     auto score = [&](floatx16 (&y)[2], bf16x8 a, int ks) { /* k-step ks of S^T */
         if (ks == 0) {
             mfma_first<E4M3>(y[0], a, qf[0][0]);
             mfma_first<false>(y[1], a, qf[1][0]);
+        } else if (ks < QV) {
+            mfma_score<E4M3, true>(y[0], a, qf[0][ks]);
+            mfma_score<false, true>(y[1], a, qf[1][ks]);
         } else {
-            mfma_score<E4M3>(y[0], a, qf[0][ks]);
-            mfma_score<false>(y[1], a, qf[1][ks]);
+            mfma_score<E4M3, false>(y[0], a, qf[0][ks]);
+            mfma_score<false, false>(y[1], a, qf[1][ks]);
         }
     };
-
-    int pg[4]; /* pages of tiles i .. i + 3 */
-    auto step = [&](auto has_next, int i, auto parity, floatx16 (&x)[2], floatx16 (&y)[2]) {
-        constexpr bool NEXT = decltype(has_next)::value;
-        constexpr int PAR = decltype(parity)::value; /* i & 1 */
-        const int k0 = pg_tile_page(list, tb + i) * PG;
-        const bool there = pg[0] >= 0;
-        floatx4 vsc[4];
+    /* V's scales of this lane's keys of tile t */
+    auto load_vsc = [&](int t) {
         if constexpr (E4M3) {
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                vsc[e] = __builtin_bit_cast(
-                    floatx4, lds_read16(lds, L::SC + 512 + (i & 3) * 256 +
-                                                 (32 * wj + 16 * h + 4 * e) * 4));
+                vsc[e] = __builtin_bit_cast(floatx4, lds_read16(lds, L::SC + 512 + (t & 3) * 256 +
+                                                                         (32 * wj + 16 * h + 4 * e) * 4));
         }
-        if (!there || !pg_tile_whole(k0, pmin, pmax, s.kv, c.window, c.sinks)) {
-            const int kb = k0 + 32 * wj + (E4M3 ? 16 : 8) * h;
-            const int top = there ? s.kv - 1 : -1, low = pg_low(pmin, c.window);
+    };
+    /* hides what the rows of tile t's scores do not see */
+    auto mask = [&](floatx16 (&x)[2], int t, bool there) {
+        const int k0 = pg_tile_page(list, tb + t) * PG;
+        if (there && pg_tile_whole(k0, pmin, pmax, s.kv, c.window, c.sinks))
+            return;
+        const int kb = k0 + 32 * wj + (E4M3 ? 16 : 8) * h;
+        const int top = there ? s.kv - 1 : -1, low = pg_low(pmin, c.window);
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int j = kb + (E4M3 ? r : 16 * (r >> 3) + (r & 7));
+        for (int r = 0; r < 16; r++) {
+            const int j = kb + (E4M3 ? r : 16 * (r >> 3) + (r & 7));
 #pragma unroll
-                for (int rb = 0; rb < 2; rb++)
-                    x[rb][r] = hide(key_seen(j, min(hi[rb], top), lo[rb], c.sinks), x[rb][r]);
-                if constexpr (E4M3) /* a scale of no key of this call: any bits */
-                    vsc[r >> 2][r & 3] = __uint_as_float(
-                        key_seen(j, top, low, c.sinks) ? __float_as_uint(vsc[r >> 2][r & 3]) : 0u);
-            }
+            for (int rb = 0; rb < 2; rb++)
+                x[rb][r] = hide(key_seen(j, min(hi[rb], top), lo[rb], c.sinks), x[rb][r]);
+            if constexpr (E4M3) /* a scale of no key of this call: any bits */
+                vsc[r >> 2][r & 3] = __uint_as_float(
+                    key_seen(j, top, low, c.sinks) ? __float_as_uint(vsc[r >> 2][r & 3]) : 0u);
         }
-        /* ---- S^T of tile i + 1 with the softmax of tile i ---- */
-        u32x4 ring[QD];
-        float ksc = 1.f;
-        if constexpr (NEXT) {
-            ksc = kscale(PAR ^ 1);
-#pragma unroll
-            for (int n = 0; n < QD; n++)
-                ring[n] = lds_read16(lds, kaddr(n, PAR ^ 1));
+    };
+    /* p of accumulators v, v + 1 of a row block into operand f[v >> 3] */
+    auto pair = [&](const floatx16 (&x)[2], bf16x8 (&f)[2], int rb, int v, float shift) {
+        float a = fast_exp2(x[rb][v] - shift), e = fast_exp2(x[rb][v + 1] - shift);
+        ls[rb] += a + e;
+        if constexpr (E4M3) {
+            a *= vsc[v >> 2][v & 3];
+            e *= vsc[v >> 2][(v & 3) + 1];
         }
-        float mx[2] = {-INFINITY, -INFINITY}, ls[2] = {0.f, 0.f};
-        bf16x8 pf[2][2];
-        auto pair = [&](int rb, int v, float shift) { /* p of accumulators v, v + 1 */
-            float a = fast_exp2(x[rb][v] - shift), e = fast_exp2(x[rb][v + 1] - shift);
-            ls[rb] += a + e;
-            if constexpr (E4M3) {
-                a *= vsc[v >> 2][v & 3];
-                e *= vsc[v >> 2][(v & 3) + 1];
-            }
-            /* the empty asm keeps the pair in its place among the MFMAs */
-            bf16x2 pk = {f2bf(a), f2bf(e)};
-            asm volatile("" : "+v"(pk), "+v"(ls[rb]));
-            pf[rb][v >> 3][v & 7] = pk[0];
-            pf[rb][v >> 3][(v & 7) + 1] = pk[1];
-        };
-        __builtin_amdgcn_sched_barrier(0);
-        bf16x8 odd = {};
-#pragma unroll
-        for (int ks = 0; ks < 16; ks++) {
-            if constexpr (NEXT) {
-                bf16x8 a;
-                if constexpr (E4M3) {
-                    if (ks & 1) {
-                        a = odd;
-                    } else {
-                        const u32x4 w = ring[(ks >> 1) % QD];
-                        if ((ks >> 1) + QD < NKR)
-                            ring[(ks >> 1) % QD] = lds_read16(lds, kaddr((ks >> 1) + QD, PAR ^ 1));
-                        a = widen(w[0], w[1], ksc);
-                        odd = widen(w[2], w[3], ksc);
-                    }
-                } else {
-                    a = __builtin_bit_cast(bf16x8, ring[ks % QD]);
-                    if (ks + QD < NKR)
-                        ring[ks % QD] = lds_read16(lds, kaddr(ks + QD, PAR ^ 1));
-                }
-                score(y, a, ks);
-            }
-            mx[ks >> 3] = fmaxf(mx[ks >> 3], fmaxf(x[ks >> 3][2 * (ks & 7)],
-                                                   x[ks >> 3][2 * (ks & 7) + 1]));
-            pair(ks >> 3, 2 * (ks & 7), 0.f);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        float mul[2];
-        bool moved = false;
+        /* the empty asm keeps the pair in its place among the MFMAs */
+        bf16x2 pk = {f2bf(a), f2bf(e)};
+        asm volatile("" : "+v"(pk), "+v"(ls[rb]));
+        f[v >> 3][v & 7] = pk[0];
+        f[v >> 3][(v & 7) + 1] = pk[1];
+    };
+    auto max2 = [&](const floatx16 (&x)[2], int rb, int v) {
+        mx[rb] = v == 0 ? fmaxf(x[rb][0], x[rb][1]) : fmaxf(mx[rb], fmaxf(x[rb][v], x[rb][v + 1]));
+    };
+    /* the references this wave wants for a tile whose maxima are known */
+    auto want = [&]() {
+        bool any = false;
 #pragma unroll
         for (int rb = 0; rb < 2; rb++) {
             const auto sw = __builtin_amdgcn_permlane32_swap(
@@ -657,9 +633,47 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
             mul[rb] = mrun[rb] == -INFINITY                        ? -INFINITY
                       : fabsf(mrun[rb] - mus[rb]) > SHIFT_RANGE ? ceilf(mrun[rb])
                                                                    : mus[rb];
-            moved |= mul[rb] != 0.f;
+            any |= mul[rb] != 0.f;
         }
-        moved = __any(moved);
+        moved = __any(any);
+    };
+
+    int pg[4]; /* pages of tiles i .. i + 3 */
+    u32x4 ring[QD];
+    float ksc = 1.f;
+    /* One tile. On entry x holds its masked scores, pn the p of row block 0 for
+     * the reference 0, and ring the first K operands of tile i + 1. The last tile
+     * runs the same code: what it does for a next one (from stale buffers, and
+     * loads of the last page again) reaches no result. A variant without it cost
+     * the registers of a second set of accumulators where the two meet. */
+    auto step = [&](int i, auto parity, floatx16 (&x)[2], floatx16 (&y)[2]) {
+        constexpr int PAR = decltype(parity)::value; /* i & 1 */
+        const bool there = pg[0] >= 0;
+        /* ---- S^T of tile i + 1 with the p of row block 1; its last two k-steps
+         * wait for the barrier, to work while the reads behind it come back ---- */
+        bf16x8 held[2] = {};
+#pragma unroll
+        for (int ks = 0; ks < 16; ks++) {
+            if constexpr (E4M3) {
+                if ((ks & 1) == 0) {
+                    const u32x4 w = ring[(ks >> 1) % QD];
+                    if ((ks >> 1) + QD < NKR)
+                        ring[(ks >> 1) % QD] = lds_read16(lds, kaddr((ks >> 1) + QD, PAR ^ 1));
+                    held[0] = widen(w[0], w[1], ksc);
+                    held[1] = widen(w[2], w[3], ksc);
+                }
+            } else {
+                held[ks & 1] = __builtin_bit_cast(bf16x8, ring[ks % QD]);
+                if (ks + QD < NKR)
+                    ring[ks % QD] = lds_read16(lds, kaddr(ks + QD, PAR ^ 1));
+            }
+            if (ks < 14)
+                score(y, held[ks & 1], ks);
+            if (ks < 14 && ks % 7 < 4) /* 8 pairs among 14 k-steps */
+                pair(x, pf[1], 1, 2 * (ks / 7 * 4 + ks % 7), 0.f);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        pf[0][0] = pn[0], pf[0][1] = pn[1];
         if (__builtin_expect(moved, 0)) {
 #pragma unroll
             for (int rb = 0; rb < 2; rb++) {
@@ -667,7 +681,7 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
                 ls[rb] = 0.f;
 #pragma unroll
                 for (int v = 0; v < 16; v += 2)
-                    pair(rb, v, shift);
+                    pair(x, pf[rb], rb, v, shift);
 #pragma unroll
                 for (int st = 0; st < 2; st++) {
                     u32x4 w = __builtin_bit_cast(u32x4, pf[rb][st]);
@@ -690,9 +704,10 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
 
+        const int k0 = pg_tile_page(list, tb + i) * PG;
         if (!there || pg_tile_foreign(k0, pmin, s.kv, c.window, c.sinks)) {
             /* values of no key of these rows meet p = 0: make them 0 */
-#pragma unroll 4
+#pragma unroll 1
             for (int n = 0; n < L::T / 4096; n++) {
                 const int at = (n * 256 + (int)threadIdx.x) * 16, d = at / (L::T / PD);
                 const int piece = ((at >> 4) & (L::T / PD / 16 - 1)) ^ swz_v<E4M3>(d);
@@ -715,14 +730,36 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
             lds_barrier();
         }
 
-        u32x4 pw[2][2];
+        /* ---- O^T += V^T P^T: own keys, then the other wave's; beside it the tile
+         * loads, and the mask, maximum and first half of p of tile i + 1 ---- */
+        constexpr int NVR = E4M3 ? 4 : 8; /* V^T reads of a key half */
+        constexpr int VD = E4M3 ? 2 : 4;
+        auto vaddr = [&](int n, int kb) { /* bf16: step-major, e4m3: both steps a read */
+            return (E4M3 ? va[kb][0] + n * 32 * (L::T / PD)
+                         : va[kb][n >> 2] + (n & 3) * 32 * (L::T / PD)) +
+                   PAR * L::T;
+        };
+        u32x4 vring[VD], pw[2][2];
 #pragma unroll
         for (int rb = 0; rb < 2; rb++)
 #pragma unroll
             for (int st = 0; st < 2; st++)
                 pw[rb][st] = lds_read16(lds, precv + PAR * L::PBUF + (2 * rb + st) * 1024);
-        /* Both waves' references of a row are known: take the larger one */
-        auto agree = [&]() {
+#pragma unroll
+        for (int n = 0; n < VD; n++)
+            vring[n] = lds_read16(lds, vaddr(n, 0));
+        __builtin_amdgcn_sched_barrier(0);
+        score(y, held[0], 14);
+        score(y, held[1], 15);
+        __builtin_amdgcn_sched_barrier(0);
+        uint32_t signs = 0;
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+            signs |= pw[t >> 1][t & 1][0] | pw[t >> 1][t & 1][1] | pw[t >> 1][t & 1][2] |
+                     pw[t >> 1][t & 1][3];
+        if (__builtin_expect(moved || __any((signs & 0x80008000u) != 0), 0)) {
+            /* Both waves' references of a row are known: take the larger one. The
+             * accumulators of y are not touched in here. */
             settle(o);
 #pragma unroll
             for (int rb = 0; rb < 2; rb++) {
@@ -742,8 +779,11 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
                 const float fo = fast_exp2(fminf(mus[rb] - ref, 0.f));
                 const float fm = fast_exp2(mul[rb] - ref), fp = fast_exp2(mup - ref);
 #pragma unroll
-                for (int d = 0; d < 4; d++)
+                for (int d = 0; d < 4; d++) { /* one at a time: 16 registers in passing */
                     o[d][rb] *= fo;
+                    asm volatile("" : "+a"(o[d][rb]));
+                    __builtin_amdgcn_sched_barrier(0);
+                }
                 lrun[rb] *= fo;
                 ls[rb] *= fm;
                 mus[rb] = ref;
@@ -763,71 +803,56 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
                 }
             }
             settle(o);
-        };
-        /* ---- O^T += V^T P^T: own keys, then the other wave's ---- */
-        const __amdgpu_buffer_rsrc_t rk = k_rsrc(pg[3]), rv = v_rsrc(pg[1]);
-        if (__builtin_expect(moved, 0))
-            agree();
-        constexpr int NVR = E4M3 ? 4 : 8; /* V^T reads of a key half */
-        constexpr int VD = E4M3 ? 2 : 4;
-        auto vaddr = [&](int n, int kb) { /* bf16: step-major, e4m3: both steps a read */
-            return (E4M3 ? va[kb][0] + n * 32 * (L::T / PD)
-                         : va[kb][n >> 2] + (n & 3) * 32 * (L::T / PD)) +
-                   PAR * L::T;
-        };
-        u32x4 vring[VD];
-#pragma unroll
-        for (int n = 0; n < VD; n++)
-            vring[n] = lds_read16(lds, vaddr(n, 0));
-#pragma unroll
-        for (int kb = 0; kb < 2; kb++) {
-            if (kb == 1 && !moved) {
-                uint32_t any = 0;
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-                    any |= pw[t >> 1][t & 1][0] | pw[t >> 1][t & 1][1] | pw[t >> 1][t & 1][2] |
-                           pw[t >> 1][t & 1][3];
-                if (__builtin_expect(__any((any & 0x80008000u) != 0), 0))
-                    agree();
-            }
-#pragma unroll
-            for (int n = 0; n < NVR; n++) {
-                const u32x4 w = vring[n % VD];
-                const int nn = kb * NVR + n + VD;
-                if (nn < 2 * NVR)
-                    vring[n % VD] = lds_read16(lds, vaddr(nn % NVR, nn / NVR));
-#pragma unroll
-                for (int half = 0; half < (E4M3 ? 2 : 1); half++) {
-                    bf16x8 a;
-                    if constexpr (E4M3)
-                        a = half ? widen(w[2], w[3], 1.f) : widen(w[0], w[1], 1.f);
-                    else
-                        a = __builtin_bit_cast(bf16x8, w);
-                    const int d = E4M3 ? n : n & 3, st = E4M3 ? half : n >> 2;
-                    auto p = [&](int rb) {
-                        return kb ? __builtin_bit_cast(bf16x8, pw[rb][st]) : pf[rb][st];
-                    };
-                    mfma_out<E4M3>(o[d][0], a, p(0));
-                    mfma_out<false>(o[d][1], a, p(1));
-                    if constexpr (NEXT) { /* one tile load beside each pair of MFMAs */
-                        const int at = E4M3 ? (kb * NVR + n) * 2 + half : kb * NVR + n;
-                        if (E4M3 ? !(at & 1) : true) {
-                            const int q = E4M3 ? at >> 1 : at;
-                            if (q < NL)
-                                issue_v(rv, PAR ^ 1, q);
-                            else
-                                issue_k(rk, PAR ^ 1, q - NL);
-                        }
-                    }
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
         }
-        if constexpr (NEXT)
-            issue_scales(pg[3], i + 3);
 #pragma unroll
         for (int rb = 0; rb < 2; rb++)
             lrun[rb] += ls[rb];
+        const __amdgpu_buffer_rsrc_t rk = k_rsrc(pg[3]), rv = v_rsrc(pg[1]);
+#pragma unroll
+        for (int g = 0; g < 16; g++) { /* pairs of MFMAs */
+            constexpr int PER = E4M3 ? 2 : 1; /* pairs a V^T read feeds */
+            const int n = g / PER, kb = n / NVR, half = g % PER;
+            const u32x4 w = vring[n % VD];
+            if (half == PER - 1 && n + VD < 2 * NVR)
+                vring[n % VD] = lds_read16(lds, vaddr((n + VD) % NVR, (n + VD) / NVR));
+            bf16x8 a;
+            if constexpr (E4M3)
+                a = half ? widen(w[2], w[3], 1.f) : widen(w[0], w[1], 1.f);
+            else
+                a = __builtin_bit_cast(bf16x8, w);
+            const int d = E4M3 ? n % NVR : n & 3, st = E4M3 ? half : n % NVR >> 2;
+            auto p = [&](int rb) {
+                return kb ? __builtin_bit_cast(bf16x8, pw[rb][st]) : pf[rb][st];
+            };
+            mfma_out<E4M3>(o[d][0], a, p(0));
+            mfma_out<false>(o[d][1], a, p(1));
+            if (g < 2 * NL) { /* tile loads, one beside a pair */
+                if (g < NL)
+                    issue_v(rv, PAR ^ 1, g);
+                else
+                    issue_k(rk, PAR ^ 1, g - NL);
+            }
+            if (g == 0)
+                load_vsc(i + 1);
+            if (g == 1) { /* y's last MFMAs are four behind */
+                asm volatile("" : "+v"(y[0]), "+v"(y[1]));
+                mask(y, i + 1, pg[1] >= 0);
+                ls[0] = ls[1] = 0.f;
+            }
+            if (g >= 2 && g < 10) {
+                max2(y, 0, 2 * (g - 2));
+                max2(y, 1, 2 * (g - 2));
+                pair(y, pn, 0, 2 * (g - 2), 0.f);
+            }
+            if (g == 11)
+                want();
+            if (g >= 16 - QD) /* K of tile i + 2 is there since the barrier */
+                ring[g - 16 + QD] = lds_read16(lds, kaddr(g - 16 + QD, PAR));
+            if (g == 15)
+                ksc = kscale(PAR);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        issue_scales(pg[3], i + 3);
         pg[0] = pg[1], pg[1] = pg[2], pg[2] = pg[3];
         if (i + 4 < ntl)
             pg[3] = page_of(i + 4);
@@ -849,54 +874,76 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
         issue_scales(pg[1], 1);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        {
-            const float ksc = kscale(0);
+        ksc = kscale(0);
 #pragma unroll
-            for (int n = 0; n < NKR; n++) {
-                const u32x4 w = lds_read16(lds, kaddr(n, 0));
+        for (int n = 0; n < NKR; n++) {
+            const u32x4 w = lds_read16(lds, kaddr(n, 0));
 #pragma unroll
-                for (int half = 0; half < (E4M3 ? 2 : 1); half++) {
-                    bf16x8 a;
-                    if constexpr (E4M3)
-                        a = half ? widen(w[2], w[3], ksc) : widen(w[0], w[1], ksc);
-                    else
-                        a = __builtin_bit_cast(bf16x8, w);
-                    const int ks = E4M3 ? 2 * n + half : n;
-                    score(xa, a, ks);
-                }
+            for (int half = 0; half < (E4M3 ? 2 : 1); half++) {
+                bf16x8 a;
+                if constexpr (E4M3)
+                    a = half ? widen(w[2], w[3], ksc) : widen(w[0], w[1], ksc);
+                else
+                    a = __builtin_bit_cast(bf16x8, w);
+                score(xa, a, E4M3 ? 2 * n + half : n);
             }
-            asm volatile("s_nop 15\n\ts_nop 7" : "+v"(xa[0]), "+v"(xa[1]));
         }
-        __syncthreads(); /* K buffer 0 is free */
-        {
-            const __amdgpu_buffer_rsrc_t k_2 = k_rsrc(pg[2]);
+        asm volatile("s_nop 15\n\ts_nop 7" : "+v"(xa[0]), "+v"(xa[1]));
+        load_vsc(0);
+        mask(xa, 0, pg[0] >= 0);
+        ls[0] = ls[1] = 0.f;
 #pragma unroll
-            for (int n = 0; n < NL; n++)
-                issue_k(k_2, 0, n);
-            issue_scales(pg[2], 2);
+        for (int v = 0; v < 16; v += 2) {
+            max2(xa, 0, v);
+            max2(xa, 1, v);
+            pair(xa, pn, 0, v, 0.f);
         }
-        const std::true_type more{};
-        const std::false_type last{};
+        want();
+        ksc = kscale(1);
+#pragma unroll
+        for (int n = 0; n < QD; n++)
+            ring[n] = lds_read16(lds, kaddr(n, 1));
+        __syncthreads(); /* K buffer 0 is free */
+        const __amdgpu_buffer_rsrc_t k_2 = k_rsrc(pg[2]);
+#pragma unroll
+        for (int n = 0; n < NL; n++)
+            issue_k(k_2, 0, n);
+        issue_scales(pg[2], 2);
         const std::integral_constant<int, 0> even{};
         const std::integral_constant<int, 1> odd{};
-        int i = 0;
-        for (; i + 2 < ntl; i += 2) {
-            step(more, i, even, xa, xb);
-            step(more, i + 1, odd, xb, xa);
-        }
-        if (ntl - i == 2) {
-            step(more, i, even, xa, xb);
-            step(last, i + 1, odd, xb, xa);
-        } else {
-            step(last, i, even, xa, xb);
+        for (int i = 0;;) {
+            step(i, even, xa, xb);
+            if (++i == ntl)
+                break;
+            step(i, odd, xb, xa);
+            if (++i == ntl)
+                break;
         }
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     }
-    settle(o);
-    __syncthreads(); /* the tile buffers are idle: O and the rows' l go there */
 
     /* ---- epilogue: O as fp32 rows of 1 KiB through LDS (piece p of row r in slot
-     * p ^ (r & 31)), l of a row from the pair's two halves ---- */
+     * p ^ (r & 31)), l of a row from the pair's two halves. A wave finishes 32
+     * rows, 16 at a time, their gates all on their way before O is staged. ---- */
+    settle(o);
+    const bool whole = nshare == 1;
+    const int t0 = 32 * wave;
+    int tok = (r0 + t0) / c.G, hd = (r0 + t0) % c.G;
+    const int tok0 = tok, hd0 = hd;
+    auto next_row = [&]() { /* rows past the last: the last again */
+        if (r0 + nrows - 1 > tok * c.G + hd && ++hd == c.G)
+            hd = 0, tok++;
+    };
+    bf16x4 gv[2][16];
+    if (whole && c.gate && t0 < nrows) {
+        const bf16 *gp = c.gate + (size_t)s.q0 * c.gts + (size_t)kh * c.G * c.ghs + 4 * lane;
+#pragma unroll
+        for (int t = 0; t < 32; t++) {
+            gv[t >> 4][t & 15] = *(const bf16x4 *)(gp + (size_t)tok * c.gts + (size_t)hd * c.ghs);
+            next_row();
+        }
+    }
+    __syncthreads(); /* the tile buffers are idle */
     float *stat = (float *)(smem + L::STAT); /* [row][l of wave 0, of wave 1, mu] */
 #pragma unroll
     for (int rb = 0; rb < 2; rb++) {
@@ -918,24 +965,27 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
             }
     }
     __syncthreads();
-    for (int t = wave; t < nrows; t += 4) {
-        const floatx4 v = *(const floatx4 *)(smem + t * 1024 + ((lane ^ (t & 31)) << 4));
-        const float l = stat[t * 4] + stat[t * 4 + 1];
-        if (nshare > 1) {
-            *(floatx4 *)(c.po + (slot * RT + t) * PD + 4 * lane) = v;
+    tok = tok0, hd = hd0;
+#pragma unroll
+    for (int t = 0; t < 32; t++) {
+        if (t0 + t >= nrows)
+            break;
+        const int r = t0 + t;
+        const floatx4 v = *(const floatx4 *)(smem + r * 1024 + ((lane ^ (r & 31)) << 4));
+        const float l = stat[r * 4] + stat[r * 4 + 1];
+        if (!whole) {
+            *(floatx4 *)(c.po + (slot * RT + r) * PD + 4 * lane) = v;
             if (lane == 0)
-                c.pl[slot * RT + t] = l, c.pmu[slot * RT + t] = stat[t * 4 + 2];
+                c.pl[slot * RT + r] = l, c.pmu[slot * RT + r] = stat[r * 4 + 2];
             continue;
         }
-        const int r = r0 + t, n = s.q0 + r / c.G, head = kh * c.G + r % c.G;
         const float inv = l > 0.f ? 1.f / l : 0.f;
-        bf16x4 gv = {}, res;
-        if (c.gate)
-            gv = *(const bf16x4 *)(c.gate + (size_t)n * c.gts + (size_t)head * c.ghs + 4 * lane);
+        bf16x4 res;
 #pragma unroll
         for (int e = 0; e < 4; e++)
-            res[e] = f2bf(v[e] * inv * (c.gate ? sigmoid_f(bf2f(gv[e])) : 1.f));
-        *(bf16x4 *)(c.out + ((size_t)n * c.Hq + head) * PD + 4 * lane) = res;
+            res[e] = f2bf(v[e] * inv * (c.gate ? sigmoid_f(bf2f(gv[t >> 4][t & 15][e])) : 1.f));
+        *(bf16x4 *)(c.out + ((size_t)(s.q0 + tok) * c.Hq + kh * c.G + hd) * PD + 4 * lane) = res;
+        next_row();
     }
 }
 
