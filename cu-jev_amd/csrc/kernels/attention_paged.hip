@@ -45,10 +45,11 @@ template <int i> DEV float row_lane(float x) {
     return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(
         0, (int)__float_as_uint(x), 0x150 + i, 0xf, 0xf, false));
 }
+template <int n> using template_int = std::integral_constant<int, n>;
 template <int n, typename F> DEV void unroll_for(F f) {
     if constexpr (n > 0) {
         unroll_for<n - 1>(f);
-        f(std::integral_constant<int, n - 1>{});
+        f(template_int<n - 1>{});
     }
 }
 /* x, or -inf where the key is hidden. On the bits: hidden scores may be NaN. */
@@ -65,17 +66,13 @@ DEV float hide(bool seen, float x) {
  * for as for any instruction. */
 template <bool NOP> DEV void mfma_first(floatx16 &s, bf16x8 a, bf16x8 q) {
     if constexpr (NOP)
-        asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(a), "v"(q));
+        asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(a), "a"(q));
     else
-        asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(a), "v"(q));
+        asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(a), "a"(q));
 }
-template <bool NOP, bool QV> DEV void mfma_score(floatx16 &s, bf16x8 a, bf16x8 q) {
-    if constexpr (NOP && QV)
-        asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(a), "v"(q));
-    else if constexpr (NOP)
+template <bool NOP> DEV void mfma_score(floatx16 &s, bf16x8 a, bf16x8 q) {
+    if constexpr (NOP)
         asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(a), "a"(q));
-    else if constexpr (QV)
-        asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(a), "v"(q));
     else
         asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(a), "a"(q));
 }
@@ -86,10 +83,8 @@ template <bool NOP> DEV void mfma_out(floatx16 &o, bf16x8 a, bf16x8 p) {
         asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(p));
 }
 /* before O is read or written by anything but mfma_out, and after */
-DEV void settle(floatx16 (&o)[4][2]) {
-    asm volatile("s_nop 15\n\ts_nop 7"
-                 : "+a"(o[0][0]), "+a"(o[0][1]), "+a"(o[1][0]), "+a"(o[1][1]), "+a"(o[2][0]),
-                   "+a"(o[2][1]), "+a"(o[3][0]), "+a"(o[3][1]));
+DEV void settle(floatx16 (&o)[4]) {
+    asm volatile("s_nop 15\n\ts_nop 7" : "+a"(o[0]), "+a"(o[1]), "+a"(o[2]), "+a"(o[3]));
 }
 
 /* keys hi at most, and past lo or a sink (without branches) */
@@ -361,18 +356,19 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(Call c) {
 }
 
 /* ---- many rows: tiles of 128 packed rows -----------------------------------------
- * One workgroup, 4 waves. Wave (i, j) computes the scores of 64 rows (half i)
- * against 32 keys of a tile (half j), and then O^T of the same rows for 128
- * dims (half j): each K and V^T operand it reads from LDS feeds two
- * v_mfma_f32_32x32x16_bf16, and what the pair (i, 0), (i, 1) has to exchange
- * is its P, 4 KiB each way per tile through LDS. One wave per 32 rows instead
- * reads every operand once per MFMA, 256 KiB of LDS a tile, as long as its
- * MFMAs take; here it is 160 (bf16).
+ * One workgroup, 8 waves, two on each SIMD. Wave (i, j) computes the scores of
+ * 32 rows (quarter i) against 32 keys of a tile (half j), and then O^T of the same
+ * rows for 128 dims (half j); the pair (i, 0), (i, 1) exchanges its P, 2 KiB each
+ * way per tile, through LDS. Half of a row's scores and half of its O per wave fit
+ * 256 registers (O 64, Q 64), so that one wave's softmax, conversions and waits
+ * run beside the other's MFMAs; one wave a SIMD (64 rows of it, half the operand
+ * reads) issued a VALU instruction only every other slot.
  *
- * Per tile one barrier. Before it a wave runs the S^T MFMAs of tile i + 1 with
- * the softmax of tile i, and leaves P of tile i in LDS; after it the PV MFMAs of
- * tile i, its own keys' first, while K of tile i + 3 and V^T of tile i + 1 go
- * to the buffers that were last read before the barrier.
+ * Per tile one barrier. Before it a wave runs the S^T MFMAs of tile i + 1 with the
+ * second half of p of tile i, and leaves P of tile i in LDS; after it the PV MFMAs
+ * of tile i, its own keys' first, with the mask, maximum and first half of p of
+ * tile i + 1, while K of tile i + 3 and V^T of tile i + 1 go to the buffers that
+ * were last read before the barrier.
  *
  * The softmax's reference mu of a row stays 0 while the scores are within 2^+-64
  * of it (mu cancels in o / l). A wave that leaves that range takes an integer
@@ -387,8 +383,8 @@ template <bool E4M3> struct Lay {
     static constexpr int V = 0, K = 2 * T, P = 4 * T, PBUF = 16384, SC = P + 2 * PBUF;
     /* e4m3: K scales of two tiles, V scales of four (read a tile later) */
     static constexpr int TILES = SC + (E4M3 ? 2 * 256 + 4 * 256 : 0);
-    static constexpr int STAT = RT * PD * 4; /* l, mu behind the staged O */
-    static constexpr int BYTES = TILES > STAT + RT * 16 ? TILES : STAT + RT * 16;
+    static constexpr int STAT = RT * PD * 4; /* l behind the staged O */
+    static constexpr int BYTES = TILES > STAT + RT * 8 ? TILES : STAT + RT * 8;
 };
 static_assert(Lay<false>::BYTES <= 163840 && Lay<true>::BYTES <= 163840, "LDS of a CU");
 
@@ -410,7 +406,7 @@ template <bool E4M3> DEV int perm_row(int m) {
 }
 
 template <bool E4M3>
-__global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
+__global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
     typedef Lay<E4M3> L;
     __shared__ __attribute__((aligned(1024))) unsigned char smem[L::BYTES];
     /* XCD-aware: where the kv-heads divide the 8 XCDs, an XCD's workgroups read
@@ -442,44 +438,36 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
     const size_t slot = ((size_t)item * c.Hkv + kh) * c.nshare + share;
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int wi = wave >> 1, wj = wave & 1, h = lane >> 5, col = lane & 31;
+    const int wi = wave & 3, wj = wave >> 2, h = lane >> 5, col = lane & 31;
 
-    /* Q^T operands of this wave's 64 rows; rows past the last repeat it */
-    bf16x8 qf[2][16];
-    int hi[2], lo[2];
-#pragma unroll
-    for (int rb = 0; rb < 2; rb++) {
-        const int r = r0 + min(64 * wi + 32 * rb + col, nrows - 1);
+    /* Q^T operands of this wave's 32 rows; rows past the last repeat it */
+    bf16x8 qf[16];
+    int hi, lo;
+    {
+        const int r = r0 + min(32 * wi + col, nrows - 1);
         const int tok = r / c.G, head = kh * c.G + r % c.G;
-        hi[rb] = min(s.p0 + tok, s.kv - 1);
-        lo[rb] = pg_low(s.p0 + tok, c.window);
+        hi = min(s.p0 + tok, s.kv - 1);
+        lo = pg_low(s.p0 + tok, c.window);
         const bf16 *qp = c.q + ((size_t)(s.q0 + tok) * c.Hq + head) * PD;
 #pragma unroll
         for (int ks = 0; ks < 16; ks++)
-            qf[rb][ks] = *(const bf16x8 *)(qp + (E4M3 ? 32 * (ks >> 1) + 16 * h + 8 * (ks & 1)
-                                                      : 16 * ks + 8 * h));
+            qf[ks] = *(const bf16x8 *)(qp + (E4M3 ? 32 * (ks >> 1) + 16 * h + 8 * (ks & 1)
+                                                  : 16 * ks + 8 * h));
     }
     const int pmin = s.p0 + i0, pmax = s.p0 + i1;
 
     /* ---- tile loads: memory -> LDS (buffer_load ... lds: lane l's 16 bytes land
-     * at base + 16 l, so the swizzle is applied to the address) ---- */
-    uint32_t kvoff[2], vvoff;
-    if constexpr (E4M3) { /* a load is 4 K rows or 16 V^T rows */
-#pragma unroll
-        for (int par = 0; par < 2; par++) {
-            const int row = 16 * par + 4 * wave + (lane >> 4);
-            kvoff[par] = (lane >> 4) * 256 + (((lane & 15) ^ swz_k<true>(row)) << 4);
-        }
+     * at base + 16 l, so the swizzle is applied to the address). Load n of a wave is
+     * KiB 8 n + wave of the tile: 2 K rows or 8 V^T rows (e4m3 4 and 16). ---- */
+    constexpr int NL = L::T / 8192; /* loads of a wave, tile and operand */
+    uint32_t kvoff, vvoff;
+    if constexpr (E4M3) {
+        kvoff = (lane >> 4) * 256 + (((lane & 15) ^ swz_k<true>(4 * wave + (lane >> 4))) << 4);
         vvoff = (lane >> 2) * 64 + (((lane & 3) ^ swz_v<true>(lane >> 2)) << 4);
-    } else { /* 2 K rows or 8 V^T rows */
-#pragma unroll
-        for (int par = 0; par < 2; par++) {
-            const int row = 8 * par + 2 * wave + (lane >> 5);
-            kvoff[par] = (lane >> 5) * 512 + (((lane & 31) ^ swz_k<false>(row)) << 4);
-        }
+    } else {
+        kvoff = (lane >> 5) * 512 + (((lane & 31) ^ swz_k<false>(2 * wave + (lane >> 5))) << 4);
         vvoff = (lane >> 3) * 128 + (((lane & 7) ^ swz_v<false>(8 * wave + (lane >> 3))) << 4);
     }
-    constexpr int NL = E4M3 ? 4 : 8; /* loads of a wave, tile and operand */
     auto slice = [&](int page) { return (size_t)max(page, 0) * c.Hkv + kh; };
     auto k_rsrc = [&](int page) {
         return make_rsrc((const char *)c.k + slice(page) * L::T, L::T);
@@ -488,12 +476,12 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
         return make_rsrc((const char *)c.vt + slice(page) * L::T, L::T);
     };
     auto issue_k = [&](__amdgpu_buffer_rsrc_t r, int buf, int n) {
-        const int at = (E4M3 ? 4096 : 4096) * n + 1024 * wave;
+        const int at = 8192 * n + 1024 * wave;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(smem + L::K + buf * L::T + at), 16,
-                                                 kvoff[n & 1], at, 0, 0);
+                                                 kvoff, at, 0, 0);
     };
     auto issue_v = [&](__amdgpu_buffer_rsrc_t r, int buf, int n) {
-        const int at = 4096 * n + 1024 * wave;
+        const int at = 8192 * n + 1024 * wave;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(smem + L::V + buf * L::T + at), 16,
                                                  vvoff, at, 0, 0);
     };
@@ -529,8 +517,8 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
             va[kb][st] = L::V + (128 * wj + col) * (L::T / PD) +
                          ((piece ^ swz_v<E4M3>(col)) << 4);
         }
-    const uint32_t psend = L::P + wave * 4096 + lane * 16;
-    const uint32_t precv = L::P + (wave ^ 1) * 4096 + lane * 16;
+    const uint32_t psend = L::P + wave * 2048 + lane * 16;
+    const uint32_t precv = L::P + (wave ^ 4) * 2048 + lane * 16;
 
     /* page ids of the list, 64 entries in a lane each */
     int ids = 0;
@@ -540,165 +528,139 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
         return __builtin_amdgcn_readlane(ids, t & 63);
     };
 
-    floatx16 o[4][2];
+    floatx16 o[4];
 #pragma unroll
     for (int d = 0; d < 4; d++)
-#pragma unroll
-        for (int rb = 0; rb < 2; rb++)
-            o[d][rb] = floatx16{};
-    /* per row: running maximum, l, the reference agreed on; of the current tile:
-     * its p, their sum, the reference this wave wants */
-    float mrun[2] = {-INFINITY, -INFINITY}, lrun[2] = {0.f, 0.f}, mus[2] = {0.f, 0.f};
-    float mx[2], ls[2], mul[2];
-    bf16x8 pf[2][2], pn[2];
-    floatx4 vsc[4];
+        o[d] = floatx16{};
+    /* of this lane's row: running maximum, l, the reference agreed on; of the
+     * current tile: its p, their sum, the reference this wave wants */
+    float mrun = -INFINITY, lrun = 0.f, mus = 0.f, mx = 0.f, ls = 0.f, mul = 0.f;
+    bf16x8 pf[2], pn;
+    float vsc = 1.f; /* e4m3: V's scale of key (lane & 15) of this half's 16 */
     bool moved = false;
 
-    constexpr int QD = E4M3 ? 2 : 4;   /* K operand reads ahead */
+    constexpr int QD = E4M3 ? 2 : 3;   /* K operand reads ahead */
     constexpr int NKR = E4M3 ? 8 : 16; /* K reads a tile */
     auto kaddr = [&](int n, int buf) {
         return (E4M3 ? ka[n] : ka[n & 7] + (n >> 3) * 256) + buf * L::T;
     };
+    typedef __attribute__((address_space(3))) const float *lds_f32;
     auto kscale = [&](int buf) {
-        return E4M3 ? *(__attribute__((address_space(3))) const float *)(lds + L::SC + buf * 256 +
-                                                                         (32 * wj + arow) * 4)
-                    : 1.f;
+        return E4M3 ? *(lds_f32)(lds + L::SC + buf * 256 + (32 * wj + arow) * 4) : 1.f;
     };
-    constexpr int QV = 4; /* k-steps whose Q is in ordinary registers */
-    auto score = [&](floatx16 (&y)[2], bf16x8 a, int ks) { /* k-step ks of S^T */
-        if (ks == 0) {
-            mfma_first<E4M3>(y[0], a, qf[0][0]);
-            mfma_first<false>(y[1], a, qf[1][0]);
-        } else if (ks < QV) {
-            mfma_score<E4M3, true>(y[0], a, qf[0][ks]);
-            mfma_score<false, true>(y[1], a, qf[1][ks]);
-        } else {
-            mfma_score<E4M3, false>(y[0], a, qf[0][ks]);
-            mfma_score<false, false>(y[1], a, qf[1][ks]);
-        }
+    auto score = [&](floatx16 &y, bf16x8 a, int ks) { /* k-step ks of S^T */
+        if (ks == 0)
+            mfma_first<E4M3>(y, a, qf[0]);
+        else
+            mfma_score<E4M3>(y, a, qf[ks]);
     };
-    /* V's scales of this lane's keys of tile t */
     auto load_vsc = [&](int t) {
-        if constexpr (E4M3) {
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                vsc[e] = __builtin_bit_cast(floatx4, lds_read16(lds, L::SC + 512 + (t & 3) * 256 +
-                                                                         (32 * wj + 16 * h + 4 * e) * 4));
-        }
+        if constexpr (E4M3)
+            vsc = *(lds_f32)(lds + L::SC + 512 + (t & 3) * 256 +
+                             (32 * wj + 16 * h + (lane & 15)) * 4);
     };
     /* hides what the rows of tile t's scores do not see */
-    auto mask = [&](floatx16 (&x)[2], int t, bool there) {
+    auto mask = [&](floatx16 &x, int t, bool there) {
         const int k0 = pg_tile_page(list, tb + t) * PG;
         if (there && pg_tile_whole(k0, pmin, pmax, s.kv, c.window, c.sinks))
             return;
         const int kb = k0 + 32 * wj + (E4M3 ? 16 : 8) * h;
-        const int top = there ? s.kv - 1 : -1, low = pg_low(pmin, c.window);
+        const int top = there ? s.kv - 1 : -1;
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-            const int j = kb + (E4M3 ? r : 16 * (r >> 3) + (r & 7));
-#pragma unroll
-            for (int rb = 0; rb < 2; rb++)
-                x[rb][r] = hide(key_seen(j, min(hi[rb], top), lo[rb], c.sinks), x[rb][r]);
-            if constexpr (E4M3) /* a scale of no key of this call: any bits */
-                vsc[r >> 2][r & 3] = __uint_as_float(
-                    key_seen(j, top, low, c.sinks) ? __float_as_uint(vsc[r >> 2][r & 3]) : 0u);
-        }
+        for (int r = 0; r < 16; r++)
+            x[r] = hide(key_seen(kb + (E4M3 ? r : 16 * (r >> 3) + (r & 7)), min(hi, top), lo,
+                                 c.sinks),
+                        x[r]);
+        if constexpr (E4M3) /* a scale of no key of this call: any bits */
+            vsc = __uint_as_float(
+                key_seen(kb + (lane & 15), top, pg_low(pmin, c.window), c.sinks)
+                    ? __float_as_uint(vsc)
+                    : 0u);
     };
-    /* p of accumulators v, v + 1 of a row block into operand f[v >> 3] */
-    auto pair = [&](const floatx16 (&x)[2], bf16x8 (&f)[2], int rb, int v, float shift) {
-        float a = fast_exp2(x[rb][v] - shift), e = fast_exp2(x[rb][v + 1] - shift);
-        ls[rb] += a + e;
+    /* p of accumulators v, v + 1 into operand f */
+    auto pair = [&](const floatx16 &x, bf16x8 &f, auto iv, float shift) {
+        constexpr int v = decltype(iv)::value;
+        float a = fast_exp2(x[v] - shift), e = fast_exp2(x[v + 1] - shift);
+        ls += a + e;
         if constexpr (E4M3) {
-            a *= vsc[v >> 2][v & 3];
-            e *= vsc[v >> 2][(v & 3) + 1];
+            a *= row_lane<v>(vsc);
+            e *= row_lane<v + 1>(vsc);
         }
         /* the empty asm keeps the pair in its place among the MFMAs */
         bf16x2 pk = {f2bf(a), f2bf(e)};
-        asm volatile("" : "+v"(pk), "+v"(ls[rb]));
-        f[v >> 3][v & 7] = pk[0];
-        f[v >> 3][(v & 7) + 1] = pk[1];
+        asm volatile("" : "+v"(pk), "+v"(ls));
+        f[v & 7] = pk[0];
+        f[(v & 7) + 1] = pk[1];
     };
-    auto max2 = [&](const floatx16 (&x)[2], int rb, int v) {
-        mx[rb] = v == 0 ? fmaxf(x[rb][0], x[rb][1]) : fmaxf(mx[rb], fmaxf(x[rb][v], x[rb][v + 1]));
-    };
-    /* the references this wave wants for a tile whose maxima are known */
+    /* the reference this wave wants for a tile whose maximum is known */
     auto want = [&]() {
-        bool any = false;
-#pragma unroll
-        for (int rb = 0; rb < 2; rb++) {
-            const auto sw = __builtin_amdgcn_permlane32_swap(
-                __float_as_uint(mx[rb]), __float_as_uint(mx[rb]), false, false);
-            mrun[rb] = fmaxf(mrun[rb], fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])));
-            /* a row without a key yet leaves the choice to the other wave */
-            mul[rb] = mrun[rb] == -INFINITY                        ? -INFINITY
-                      : fabsf(mrun[rb] - mus[rb]) > SHIFT_RANGE ? ceilf(mrun[rb])
-                                                                   : mus[rb];
-            any |= mul[rb] != 0.f;
-        }
-        moved = __any(any);
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx),
+                                                         false, false);
+        mrun = fmaxf(mrun, fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])));
+        /* a row without a key yet leaves the choice to the other wave */
+        mul = mrun == -INFINITY                    ? -INFINITY
+              : fabsf(mrun - mus) > SHIFT_RANGE ? ceilf(mrun)
+                                                   : mus;
+        moved = __any(mul != 0.f);
     };
 
     int pg[4]; /* pages of tiles i .. i + 3 */
     u32x4 ring[QD];
     float ksc = 1.f;
-    /* One tile. On entry x holds its masked scores, pn the p of row block 0 for
-     * the reference 0, and ring the first K operands of tile i + 1. The last tile
+    /* One tile. On entry x holds its masked scores, pn the first half of p for the
+     * reference 0, and ring the first K operands of tile i + 1. The last tile
      * runs the same code: what it does for a next one (from stale buffers, and
      * loads of the last page again) reaches no result. A variant without it cost
      * the registers of a second set of accumulators where the two meet. */
-    auto step = [&](int i, auto parity, floatx16 (&x)[2], floatx16 (&y)[2]) {
+    auto step = [&](int i, auto parity, floatx16 &x, floatx16 &y) {
         constexpr int PAR = decltype(parity)::value; /* i & 1 */
         const bool there = pg[0] >= 0;
-        /* ---- S^T of tile i + 1 with the p of row block 1; its last two k-steps
-         * wait for the barrier, to work while the reads behind it come back ---- */
+        /* ---- S^T of tile i + 1 with the second half of p; its last two k-steps wait
+         * for the barrier, to work while the reads behind it come back ---- */
         bf16x8 held[2] = {};
-#pragma unroll
-        for (int ks = 0; ks < 16; ks++) {
+        unroll_for<16>([&](auto iks) {
+            constexpr int ks = decltype(iks)::value;
             if constexpr (E4M3) {
-                if ((ks & 1) == 0) {
+                if constexpr ((ks & 1) == 0) {
                     const u32x4 w = ring[(ks >> 1) % QD];
-                    if ((ks >> 1) + QD < NKR)
+                    if constexpr ((ks >> 1) + QD < NKR)
                         ring[(ks >> 1) % QD] = lds_read16(lds, kaddr((ks >> 1) + QD, PAR ^ 1));
                     held[0] = widen(w[0], w[1], ksc);
                     held[1] = widen(w[2], w[3], ksc);
                 }
             } else {
                 held[ks & 1] = __builtin_bit_cast(bf16x8, ring[ks % QD]);
-                if (ks + QD < NKR)
+                if constexpr (ks + QD < NKR)
                     ring[ks % QD] = lds_read16(lds, kaddr(ks + QD, PAR ^ 1));
             }
-            if (ks < 14)
+            if constexpr (ks < 14)
                 score(y, held[ks & 1], ks);
-            if (ks < 14 && ks % 7 < 4) /* 8 pairs among 14 k-steps */
-                pair(x, pf[1], 1, 2 * (ks / 7 * 4 + ks % 7), 0.f);
+            if constexpr (ks < 12 && ks % 3 == 1)
+                pair(x, pf[1], template_int<8 + ks / 3 * 2>{}, 0.f);
             __builtin_amdgcn_sched_barrier(0);
-        }
-        pf[0][0] = pn[0], pf[0][1] = pn[1];
+        });
+        pf[0] = pn;
         if (__builtin_expect(moved, 0)) {
+            const float shift = mul == -INFINITY ? 0.f : mul;
+            ls = 0.f;
+            unroll_for<8>([&](auto iv) {
+                constexpr int v = 2 * decltype(iv)::value;
+                pair(x, pf[v >> 3], template_int<v>{}, shift);
+            });
 #pragma unroll
-            for (int rb = 0; rb < 2; rb++) {
-                const float shift = mul[rb] == -INFINITY ? 0.f : mul[rb];
-                ls[rb] = 0.f;
+            for (int st = 0; st < 2; st++) {
+                u32x4 w = __builtin_bit_cast(u32x4, pf[st]);
+                const uint32_t u = __float_as_uint(mul) >> (16 * h + 8 * st);
 #pragma unroll
-                for (int v = 0; v < 16; v += 2)
-                    pair(x, pf[rb], rb, v, shift);
-#pragma unroll
-                for (int st = 0; st < 2; st++) {
-                    u32x4 w = __builtin_bit_cast(u32x4, pf[rb][st]);
-                    const uint32_t u = __float_as_uint(mul[rb]) >> (16 * h + 8 * st);
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        w[e] |= ((u >> (2 * e)) & 1) << 15 | ((u >> (2 * e + 1)) & 1) << 31;
-                    pf[rb][st] = __builtin_bit_cast(bf16x8, w);
-                }
+                for (int e = 0; e < 4; e++)
+                    w[e] |= ((u >> (2 * e)) & 1) << 15 | ((u >> (2 * e + 1)) & 1) << 31;
+                pf[st] = __builtin_bit_cast(bf16x8, w);
             }
         }
 #pragma unroll
-        for (int rb = 0; rb < 2; rb++)
-#pragma unroll
-            for (int st = 0; st < 2; st++)
-                lds_write16(smem, psend + PAR * L::PBUF + (2 * rb + st) * 1024,
-                            __builtin_bit_cast(u32x4, pf[rb][st]));
+        for (int st = 0; st < 2; st++)
+            lds_write16(smem, psend + PAR * L::PBUF + st * 1024,
+                        __builtin_bit_cast(u32x4, pf[st]));
         /* P is in LDS, this wave's reads of K are done, its tile loads have landed */
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
@@ -708,8 +670,8 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
         if (!there || pg_tile_foreign(k0, pmin, s.kv, c.window, c.sinks)) {
             /* values of no key of these rows meet p = 0: make them 0 */
 #pragma unroll 1
-            for (int n = 0; n < L::T / 4096; n++) {
-                const int at = (n * 256 + (int)threadIdx.x) * 16, d = at / (L::T / PD);
+            for (int n = 0; n < L::T / 8192; n++) {
+                const int at = (n * 512 + (int)threadIdx.x) * 16, d = at / (L::T / PD);
                 const int piece = ((at >> 4) & (L::T / PD / 16 - 1)) ^ swz_v<E4M3>(d);
                 u32x4 w = lds_read16(lds, L::V + PAR * L::T + at);
 #pragma unroll
@@ -733,18 +695,16 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
         /* ---- O^T += V^T P^T: own keys, then the other wave's; beside it the tile
          * loads, and the mask, maximum and first half of p of tile i + 1 ---- */
         constexpr int NVR = E4M3 ? 4 : 8; /* V^T reads of a key half */
-        constexpr int VD = E4M3 ? 2 : 4;
+        constexpr int VD = E4M3 ? 2 : 3;
         auto vaddr = [&](int n, int kb) { /* bf16: step-major, e4m3: both steps a read */
             return (E4M3 ? va[kb][0] + n * 32 * (L::T / PD)
                          : va[kb][n >> 2] + (n & 3) * 32 * (L::T / PD)) +
                    PAR * L::T;
         };
-        u32x4 vring[VD], pw[2][2];
+        u32x4 vring[VD], pw[2];
 #pragma unroll
-        for (int rb = 0; rb < 2; rb++)
-#pragma unroll
-            for (int st = 0; st < 2; st++)
-                pw[rb][st] = lds_read16(lds, precv + PAR * L::PBUF + (2 * rb + st) * 1024);
+        for (int st = 0; st < 2; st++)
+            pw[st] = lds_read16(lds, precv + PAR * L::PBUF + st * 1024);
 #pragma unroll
         for (int n = 0; n < VD; n++)
             vring[n] = lds_read16(lds, vaddr(n, 0));
@@ -752,106 +712,94 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
         score(y, held[0], 14);
         score(y, held[1], 15);
         __builtin_amdgcn_sched_barrier(0);
-        uint32_t signs = 0;
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-            signs |= pw[t >> 1][t & 1][0] | pw[t >> 1][t & 1][1] | pw[t >> 1][t & 1][2] |
-                     pw[t >> 1][t & 1][3];
+        const uint32_t signs = pw[0][0] | pw[0][1] | pw[0][2] | pw[0][3] | pw[1][0] | pw[1][1] |
+                               pw[1][2] | pw[1][3];
         if (__builtin_expect(moved || __any((signs & 0x80008000u) != 0), 0)) {
             /* Both waves' references of a row are known: take the larger one. The
              * accumulators of y are not touched in here. */
+            uint32_t u = 0;
+#pragma unroll
+            for (int st = 0; st < 2; st++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    u |= ((pw[st][e] >> 15) & 1) << (8 * st + 2 * e);
+                    u |= (pw[st][e] >> 31) << (8 * st + 2 * e + 1);
+                }
+            const uint32_t v = __shfl_xor(u, 32, 64);
+            const float mup = __uint_as_float(h ? u << 16 | v : v << 16 | u);
+            float ref = fmaxf(mul, mup);
+            ref = ref == -INFINITY ? mus : ref;
+            /* it only falls while no key has counted, with o = l = 0 */
+            const float fo = fast_exp2(fminf(mus - ref, 0.f));
+            const float fm = fast_exp2(mul - ref), fp = fast_exp2(mup - ref);
             settle(o);
 #pragma unroll
-            for (int rb = 0; rb < 2; rb++) {
-                uint32_t u = 0;
+            for (int d = 0; d < 4; d++) { /* one at a time: 16 registers in passing */
+                o[d] *= fo;
+                asm volatile("" : "+a"(o[d]));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            lrun *= fo;
+            ls *= fm;
+            mus = ref;
 #pragma unroll
-                for (int st = 0; st < 2; st++)
+            for (int st = 0; st < 2; st++) {
+                bf16x8 t = __builtin_bit_cast(bf16x8, pw[st] & 0x7fff7fffu);
+                bf16x8 w = __builtin_bit_cast(
+                    bf16x8, __builtin_bit_cast(u32x4, pf[st]) & 0x7fff7fffu);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        u |= ((pw[rb][st][e] >> 15) & 1) << (8 * st + 2 * e);
-                        u |= (pw[rb][st][e] >> 31) << (8 * st + 2 * e + 1);
-                    }
-                const uint32_t v = __shfl_xor(u, 32, 64);
-                const float mup = __uint_as_float(h ? u << 16 | v : v << 16 | u);
-                float ref = fmaxf(mul[rb], mup);
-                ref = ref == -INFINITY ? mus[rb] : ref;
-                /* it only falls while no key has counted, with o = l = 0 */
-                const float fo = fast_exp2(fminf(mus[rb] - ref, 0.f));
-                const float fm = fast_exp2(mul[rb] - ref), fp = fast_exp2(mup - ref);
-#pragma unroll
-                for (int d = 0; d < 4; d++) { /* one at a time: 16 registers in passing */
-                    o[d][rb] *= fo;
-                    asm volatile("" : "+a"(o[d][rb]));
-                    __builtin_amdgcn_sched_barrier(0);
+                for (int e = 0; e < 8; e++) {
+                    t[e] = f2bf(bf2f(t[e]) * fp);
+                    w[e] = f2bf(bf2f(w[e]) * fm);
                 }
-                lrun[rb] *= fo;
-                ls[rb] *= fm;
-                mus[rb] = ref;
-#pragma unroll
-                for (int st = 0; st < 2; st++) {
-                    bf16x8 t = __builtin_bit_cast(bf16x8, pw[rb][st] & 0x7fff7fffu);
-                    bf16x8 w = __builtin_bit_cast(
-                        bf16x8, __builtin_bit_cast(u32x4, pf[rb][st]) & 0x7fff7fffu);
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        t[e] = f2bf(bf2f(t[e]) * fp);
-                        w[e] = f2bf(bf2f(w[e]) * fm);
-                    }
-                    pw[rb][st] = __builtin_bit_cast(u32x4, t);
-                    pf[rb][st] = w;
-                    asm volatile("s_nop 1" : "+v"(pw[rb][st]), "+v"(pf[rb][st]));
-                }
+                pw[st] = __builtin_bit_cast(u32x4, t);
+                pf[st] = w;
+                asm volatile("s_nop 1" : "+v"(pw[st]), "+v"(pf[st]));
             }
             settle(o);
         }
-#pragma unroll
-        for (int rb = 0; rb < 2; rb++)
-            lrun[rb] += ls[rb];
+        lrun += ls;
         const __amdgpu_buffer_rsrc_t rk = k_rsrc(pg[3]), rv = v_rsrc(pg[1]);
-#pragma unroll
-        for (int g = 0; g < 16; g++) { /* pairs of MFMAs */
-            constexpr int PER = E4M3 ? 2 : 1; /* pairs a V^T read feeds */
-            const int n = g / PER, kb = n / NVR, half = g % PER;
+        unroll_for<16>([&](auto ig) {
+            constexpr int g = decltype(ig)::value;
+            constexpr int PER = E4M3 ? 2 : 1; /* MFMAs a V^T read feeds */
+            constexpr int n = g / PER, kb = n / NVR, half = g % PER;
             const u32x4 w = vring[n % VD];
-            if (half == PER - 1 && n + VD < 2 * NVR)
+            if constexpr (half == PER - 1 && n + VD < 2 * NVR)
                 vring[n % VD] = lds_read16(lds, vaddr((n + VD) % NVR, (n + VD) / NVR));
             bf16x8 a;
             if constexpr (E4M3)
                 a = half ? widen(w[2], w[3], 1.f) : widen(w[0], w[1], 1.f);
             else
                 a = __builtin_bit_cast(bf16x8, w);
-            const int d = E4M3 ? n % NVR : n & 3, st = E4M3 ? half : n % NVR >> 2;
-            auto p = [&](int rb) {
-                return kb ? __builtin_bit_cast(bf16x8, pw[rb][st]) : pf[rb][st];
-            };
-            mfma_out<E4M3>(o[d][0], a, p(0));
-            mfma_out<false>(o[d][1], a, p(1));
-            if (g < 2 * NL) { /* tile loads, one beside a pair */
-                if (g < NL)
-                    issue_v(rv, PAR ^ 1, g);
-                else
-                    issue_k(rk, PAR ^ 1, g - NL);
-            }
-            if (g == 0)
+            constexpr int d = E4M3 ? n % NVR : n & 3, st = E4M3 ? half : n % NVR >> 2;
+            mfma_out<E4M3>(o[d], a, kb ? __builtin_bit_cast(bf16x8, pw[st]) : pf[st]);
+            if constexpr (g < NL) /* a tile load beside an MFMA */
+                issue_v(rv, PAR ^ 1, g);
+            else if constexpr (g < 2 * NL)
+                issue_k(rk, PAR ^ 1, g - NL);
+            if constexpr (g == 0)
                 load_vsc(i + 1);
-            if (g == 1) { /* y's last MFMAs are four behind */
-                asm volatile("" : "+v"(y[0]), "+v"(y[1]));
+            if constexpr (g == 3) { /* y's last MFMA is four behind */
+                asm volatile("" : "+v"(y));
                 mask(y, i + 1, pg[1] >= 0);
-                ls[0] = ls[1] = 0.f;
+                ls = 0.f;
+                mx = fmaxf(y[0], y[1]);
             }
-            if (g >= 2 && g < 10) {
-                max2(y, 0, 2 * (g - 2));
-                max2(y, 1, 2 * (g - 2));
-                pair(y, pn, 0, 2 * (g - 2), 0.f);
+            if constexpr (g >= 4 && g < 11) {
+                constexpr int v = 2 * (g - 3);
+                mx = fmaxf(mx, fmaxf(y[v], y[v + 1]));
             }
-            if (g == 11)
+            if constexpr (g >= 4 && g < 12 && (g & 1) == 1)
+                pair(y, pn, template_int<g - 5>{}, 0.f);
+            if constexpr (g == 12)
                 want();
-            if (g >= 16 - QD) /* K of tile i + 2 is there since the barrier */
+            if constexpr (g >= 16 - QD) /* K of tile i + 2 is there since the barrier */
                 ring[g - 16 + QD] = lds_read16(lds, kaddr(g - 16 + QD, PAR));
-            if (g == 15)
+            if constexpr (g == 15)
                 ksc = kscale(PAR);
             __builtin_amdgcn_sched_barrier(0);
-        }
+        });
         issue_scales(pg[3], i + 3);
         pg[0] = pg[1], pg[1] = pg[2], pg[2] = pg[3];
         if (i + 4 < ntl)
@@ -859,45 +807,49 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
     };
 
     if (ntl > 0) {
-        floatx16 xa[2], xb[2];
+        floatx16 xa, xb;
 #pragma unroll
         for (int t = 0; t < 4; t++)
             pg[t] = t < ntl ? page_of(t) : pg[t - 1];
         const __amdgpu_buffer_rsrc_t k_0 = k_rsrc(pg[0]), v_0 = v_rsrc(pg[0]), k_1 = k_rsrc(pg[1]);
 #pragma unroll
-        for (int n = 0; n < NL; n++) {
+        for (int n = 0; n < NL; n++)
             issue_k(k_0, 0, n);
-            issue_v(v_0, 0, n);
-            issue_k(k_1, 1, n);
-        }
         issue_scales(pg[0], 0);
+#pragma unroll
+        for (int n = 0; n < NL; n++) {
+            issue_k(k_1, 1, n);
+            issue_v(v_0, 0, n);
+        }
         issue_scales(pg[1], 1);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         ksc = kscale(0);
+        unroll_for<2>([&](auto ib) { /* operands of 8 k-steps at a time */
+            constexpr int part = decltype(ib)::value;
+            u32x4 w[NKR / 2];
 #pragma unroll
-        for (int n = 0; n < NKR; n++) {
-            const u32x4 w = lds_read16(lds, kaddr(n, 0));
-#pragma unroll
-            for (int half = 0; half < (E4M3 ? 2 : 1); half++) {
-                bf16x8 a;
+            for (int n = 0; n < NKR / 2; n++)
+                w[n] = lds_read16(lds, kaddr(part * (NKR / 2) + n, 0));
+            __builtin_amdgcn_sched_barrier(0);
+            unroll_for<8>([&](auto ik) {
+                constexpr int k = decltype(ik)::value;
                 if constexpr (E4M3)
-                    a = half ? widen(w[2], w[3], ksc) : widen(w[0], w[1], ksc);
+                    score(xa, k & 1 ? widen(w[k >> 1][2], w[k >> 1][3], ksc)
+                                    : widen(w[k >> 1][0], w[k >> 1][1], ksc),
+                          8 * part + k);
                 else
-                    a = __builtin_bit_cast(bf16x8, w);
-                score(xa, a, E4M3 ? 2 * n + half : n);
-            }
-        }
-        asm volatile("s_nop 15\n\ts_nop 7" : "+v"(xa[0]), "+v"(xa[1]));
+                    score(xa, __builtin_bit_cast(bf16x8, w[k]), 8 * part + k);
+            });
+        });
+        asm volatile("s_nop 15\n\ts_nop 7" : "+v"(xa));
         load_vsc(0);
         mask(xa, 0, pg[0] >= 0);
-        ls[0] = ls[1] = 0.f;
+        mx = -INFINITY;
 #pragma unroll
-        for (int v = 0; v < 16; v += 2) {
-            max2(xa, 0, v);
-            max2(xa, 1, v);
-            pair(xa, pn, 0, v, 0.f);
-        }
+        for (int v = 0; v < 16; v++)
+            mx = fmaxf(mx, xa[v]);
+        unroll_for<4>([&](auto iv) { pair(xa, pn, template_int<2 * decltype(iv)::value>{}, 0.f); });
         want();
         ksc = kscale(1);
 #pragma unroll
@@ -909,83 +861,80 @@ __global__ __launch_bounds__(256) void attention_many_kernel(Call c) {
         for (int n = 0; n < NL; n++)
             issue_k(k_2, 0, n);
         issue_scales(pg[2], 2);
-        const std::integral_constant<int, 0> even{};
-        const std::integral_constant<int, 1> odd{};
         for (int i = 0;;) {
-            step(i, even, xa, xb);
+            step(i, template_int<0>{}, xa, xb);
             if (++i == ntl)
                 break;
-            step(i, odd, xb, xa);
+            step(i, template_int<1>{}, xb, xa);
             if (++i == ntl)
                 break;
         }
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     }
 
-    /* ---- epilogue: O as fp32 rows of 1 KiB through LDS (piece p of row r in slot
-     * p ^ (r & 31)), l of a row from the pair's two halves. A wave finishes 32
-     * rows, 16 at a time, their gates all on their way before O is staged. ---- */
+    /* ---- epilogue: l of a row from the pair's two halves; O / l (a share: O) as fp32
+     * rows of 1 KiB through LDS, piece p of row r in slot p ^ (r & 31); then a wave
+     * finishes 16 rows, their gates on the way since before O was staged. Where row
+     * t's gate and output lie is worked out by lane t. ---- */
     settle(o);
-    const bool whole = nshare == 1;
-    const int t0 = 32 * wave;
-    int tok = (r0 + t0) / c.G, hd = (r0 + t0) % c.G;
-    const int tok0 = tok, hd0 = hd;
-    auto next_row = [&]() { /* rows past the last: the last again */
-        if (r0 + nrows - 1 > tok * c.G + hd && ++hd == c.G)
-            hd = 0, tok++;
+    const bool whole = nshare == 1, gated = whole && c.gate;
+    const int t0 = 16 * wave;
+    size_t gat, oat;
+    {
+        const int r = r0 + min(t0 + (lane & 15), nrows - 1), tok = r / c.G, hd = r % c.G;
+        gat = (size_t)(s.q0 + tok) * c.gts + (size_t)(kh * c.G + hd) * c.ghs;
+        oat = whole ? ((size_t)(s.q0 + tok) * c.Hq + kh * c.G + hd) * PD
+                    : (slot * RT + t0 + (lane & 15)) * PD;
+    }
+    auto of_row = [&](size_t x, int t) {
+        return (size_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, t) |
+               (size_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), t) << 32;
     };
-    bf16x4 gv[2][16];
-    if (whole && c.gate && t0 < nrows) {
-        const bf16 *gp = c.gate + (size_t)s.q0 * c.gts + (size_t)kh * c.G * c.ghs + 4 * lane;
+    bf16x4 gv[16];
+    if (gated) {
 #pragma unroll
-        for (int t = 0; t < 32; t++) {
-            gv[t >> 4][t & 15] = *(const bf16x4 *)(gp + (size_t)tok * c.gts + (size_t)hd * c.ghs);
-            next_row();
-        }
+        for (int t = 0; t < 16; t++)
+            gv[t] = *(const bf16x4 *)(c.gate + of_row(gat, t) + 4 * lane);
     }
     __syncthreads(); /* the tile buffers are idle */
-    float *stat = (float *)(smem + L::STAT); /* [row][l of wave 0, of wave 1, mu] */
+    float *stat = (float *)(smem + L::STAT); /* [2][row] */
+    const float lw = lrun + __shfl_xor(lrun, 32, 64);
+    if (h == 0)
+        stat[wj * RT + 32 * wi + col] = lw;
+    __syncthreads();
+    const float l = stat[32 * wi + col] + stat[RT + 32 * wi + col];
+    const float inv = !whole ? 1.f : l > 0.f ? 1.f / l : 0.f;
+    if (!whole && wj == 0 && h == 0) {
+        c.pl[slot * RT + 32 * wi + col] = l;
+        c.pmu[slot * RT + 32 * wi + col] = mus;
+    }
 #pragma unroll
-    for (int rb = 0; rb < 2; rb++) {
-        const int r = 64 * wi + 32 * rb + col;
-        const float l = lrun[rb] + __shfl_xor(lrun[rb], 32, 64);
-        if (h == 0) {
-            stat[r * 4 + wj] = l;
-            if (wj == 0)
-                stat[r * 4 + 2] = mus[rb];
+    for (int d = 0; d < 4; d++) {
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const floatx4 v = {o[d][4 * q] * inv, o[d][4 * q + 1] * inv, o[d][4 * q + 2] * inv,
+                               o[d][4 * q + 3] * inv};
+            const int piece = 32 * wj + 8 * d + 2 * q + h;
+            *(floatx4 *)(smem + (32 * wi + col) * 1024 + ((piece ^ col) << 4)) = v;
         }
-#pragma unroll
-        for (int d = 0; d < 4; d++)
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const floatx4 v = {o[d][rb][4 * q], o[d][rb][4 * q + 1], o[d][rb][4 * q + 2],
-                                   o[d][rb][4 * q + 3]};
-                const int piece = 32 * wj + 8 * d + 2 * q + h;
-                *(floatx4 *)(smem + r * 1024 + ((piece ^ col) << 4)) = v;
-            }
+        __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
-    tok = tok0, hd = hd0;
 #pragma unroll
-    for (int t = 0; t < 32; t++) {
+    for (int t = 0; t < 16; t++) {
         if (t0 + t >= nrows)
             break;
-        const int r = t0 + t;
-        const floatx4 v = *(const floatx4 *)(smem + r * 1024 + ((lane ^ (r & 31)) << 4));
-        const float l = stat[r * 4] + stat[r * 4 + 1];
+        const floatx4 v = *(const floatx4 *)(smem + (t0 + t) * 1024 +
+                                             ((lane ^ ((t0 + t) & 31)) << 4));
         if (!whole) {
-            *(floatx4 *)(c.po + (slot * RT + r) * PD + 4 * lane) = v;
-            if (lane == 0)
-                c.pl[slot * RT + r] = l, c.pmu[slot * RT + r] = stat[r * 4 + 2];
+            *(floatx4 *)(c.po + of_row(oat, t) + 4 * lane) = v;
             continue;
         }
-        const float inv = l > 0.f ? 1.f / l : 0.f;
         bf16x4 res;
 #pragma unroll
         for (int e = 0; e < 4; e++)
-            res[e] = f2bf(v[e] * inv * (c.gate ? sigmoid_f(bf2f(gv[t >> 4][t & 15][e])) : 1.f));
-        *(bf16x4 *)(c.out + ((size_t)(s.q0 + tok) * c.Hq + kh * c.G + hd) * PD + 4 * lane) = res;
-        next_row();
+            res[e] = f2bf(gated ? v[e] * sigmoid_f(bf2f(gv[t][e])) : v[e]);
+        *(bf16x4 *)(c.out + of_row(oat, t) + 4 * lane) = res;
     }
 }
 
@@ -1124,9 +1073,9 @@ extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int
         const int per = 8 % Hkv == 0 ? 8 / Hkv : 1;
         const dim3 grid((unsigned)(pg_div_up(p.items, per) * per * Hkv), (unsigned)p.nshare);
         if (e4m3)
-            hipLaunchKernelGGL(attention_many_kernel<true>, grid, dim3(256), 0, stream, c);
+            hipLaunchKernelGGL(attention_many_kernel<true>, grid, dim3(512), 0, stream, c);
         else
-            hipLaunchKernelGGL(attention_many_kernel<false>, grid, dim3(256), 0, stream, c);
+            hipLaunchKernelGGL(attention_many_kernel<false>, grid, dim3(512), 0, stream, c);
         if (p.nshare > 1)
             hipLaunchKernelGGL(merge_kernel<RT>, dim3((unsigned)(p.items * Hkv * (RT / 4))),
                                dim3(256), 0, stream, c);
