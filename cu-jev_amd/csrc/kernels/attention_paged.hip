@@ -90,10 +90,16 @@ DEV void settle(floatx16 (&o)[4]) {
 /* keys hi at most, and past lo or a sink (without branches) */
 DEV bool key_seen(int j, int hi, int lo, int sinks) { return (j <= hi) & ((j > lo) | (j < sinks)); }
 
-/* What both kernels and the merge share. A tile of rows whose key tiles are
- * shared out over several workgroups keeps, per share, unnormalised o, l and
- * the softmax's reference mu of its RT rows in slot (tile Hkv + kh) nshare +
- * share. */
+/* What both kernels and the merge share.
+ *
+ * The work of a kv-head is its units, tiles of RT packed rows of a sequence. So
+ * that the workgroups of a call finish together however uneven its sequences,
+ * each of them works out the same plan from q_start and kv_len: the key tiles of
+ * all units (a sequence's units counted with its longest list) over the
+ * workgroups that the chip holds at once give the tiles a share should have,
+ * and a sequence's units are cut into as many even shares as that asks for. A
+ * unit of several shares keeps, per share, unnormalised o, l and the softmax's
+ * reference mu of its rows in a slot each, for the merge. */
 struct Call {
     const bf16 *q, *gate;
     int gts, ghs;
@@ -104,23 +110,91 @@ struct Call {
     int max_pages, B, N, max_q, max_kv, Hq, Hkv, G, window, sinks;
     bf16 *out;
     float *po, *pl, *pmu;
-    int items;   /* tiles of rows, at most */
-    int share;   /* key tiles a share */
-    int nshare;  /* shares a tile, at most */
+    pg_plan plan;
 };
 DEV pg_seq seq_of(const Call &c, int b) {
     return load_seq(c.q_start, c.kv_len, b, c.N, c.max_q, c.max_kv);
-}
-/* Tile `item` of RT packed rows: its sequence and number within it. */
-template <int RT> DEV int find_tile(const Call &c, int item, pg_seq *s, int *local) {
-    return find_item(
-        c.q_start, c.kv_len, c.B, c.N, c.max_q, c.max_kv, item,
-        [&](const pg_seq &q) { return (int)(((long long)q.ql * c.G + RT - 1) / RT); }, s, local);
 }
 DEV int page_id(const Call &c, int b, const pg_tiles &t, int i) {
     const int page = c.page_table[(size_t)b * c.max_pages + pg_tile_page(t, i)];
     return page >= 0 && page < c.num_pages ? page : -1;
 }
+
+DEV int wave_sum_i(int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        v += __shfl_xor(v, o, 64);
+    return v;
+}
+/* Where a workgroup (BY_SHARE: share `target` of a kv-head) or a merging wave
+ * (unit `target`) works: the sequence (-1: no such share or unit), the number of
+ * its unit in it, the share, the unit's shares and the slot of its first. */
+struct Where {
+    pg_seq s;
+    int b, unit, share, nshare, slot0;
+};
+template <bool BY_SHARE> DEV Where locate(const Call &c, int target) {
+    const int lane = threadIdx.x & 63;
+    Where w;
+    w.b = -1;
+    if (c.B == 1) { /* no scan for one sequence */
+        const pg_seq s = seq_of(c, 0);
+        const int units = pg_units(s, c.G, c.plan.rt);
+        const int tiles = pg_longest(s, c.G, c.plan.rt, c.window, c.sinks);
+        const int n = pg_nshare(tiles, pg_share(c.plan, units, (unsigned)units * (unsigned)tiles));
+        if (target >= units * (BY_SHARE ? n : 1))
+            return w;
+        w.s = s, w.b = 0, w.nshare = n;
+        w.unit = BY_SHARE ? target / n : target;
+        w.share = BY_SHARE ? target % n : 0;
+        w.slot0 = w.unit * n;
+        return w;
+    }
+    int U = 0;
+    unsigned T = 0;
+    for (int b0 = 0; b0 < c.B; b0 += 64) {
+        const bool in = b0 + lane < c.B;
+        const pg_seq s = seq_of(c, min(b0 + lane, c.B - 1));
+        const int units = in ? pg_units(s, c.G, c.plan.rt) : 0;
+        U += units;
+        T += (unsigned)units * (unsigned)pg_longest(s, c.G, c.plan.rt, c.window, c.sinks);
+    }
+    const int share = pg_share(c.plan, wave_sum_i(U), (unsigned)wave_sum_i((int)T));
+    int before_u = 0, before_s = 0;
+    for (int b0 = 0; b0 < c.B; b0 += 64) {
+        const bool in = b0 + lane < c.B;
+        const pg_seq s = seq_of(c, min(b0 + lane, c.B - 1));
+        const int n = pg_nshare(pg_longest(s, c.G, c.plan.rt, c.window, c.sinks), share);
+        const int units = in ? pg_units(s, c.G, c.plan.rt) : 0, shares = units * n;
+        int su = units, ss = shares; /* inclusive sums over the lanes */
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int x = __shfl_up(su, o, 64), y = __shfl_up(ss, o, 64);
+            su += lane >= o ? x : 0;
+            ss += lane >= o ? y : 0;
+        }
+        const uint64_t past =
+            __ballot(BY_SHARE ? before_s + ss > target : before_u + su > target);
+        if (past) {
+            const int l = __ffsll((unsigned long long)past) - 1;
+            auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+            w.s.q0 = of(s.q0), w.s.ql = of(s.ql), w.s.kv = of(s.kv), w.s.p0 = of(s.p0);
+            w.b = b0 + l;
+            w.nshare = of(n);
+            const int local = target - (BY_SHARE ? before_s + of(ss - shares)
+                                                 : before_u + of(su - units));
+            w.unit = BY_SHARE ? local / w.nshare : local;
+            w.share = BY_SHARE ? local % w.nshare : 0;
+            w.slot0 = before_s + of(ss - shares) + w.unit * w.nshare;
+            return w;
+        }
+        before_u += __builtin_amdgcn_readlane(su, 63);
+        before_s += __builtin_amdgcn_readlane(ss, 63);
+    }
+    return w;
+}
+/* The slot of share `at` of a kv-head */
+DEV size_t slot_of(const Call &c, int kh, int at) { return (size_t)kh * c.plan.slots + at; }
 
 /* ---- few rows: up to 16 packed rows of a sequence and kv-head ------------------
  * Bound by the K/V bytes. A workgroup takes one share of the key tiles; its 4
@@ -131,7 +205,7 @@ DEV int page_id(const Call &c, int b, const pg_tiles &t, int i) {
  * the PV products, V^T during the scores. All loads are unconditional (past
  * the end the last step's again), so a wait for one operand's counts the other's
  * in flight and not more; with 256 registers two waves share a SIMD. */
-constexpr int FEW = 16, FEW_TILES = 64; /* rows; key tiles a share, at most */
+constexpr int FEW = PG_FEW;
 
 template <bool E4M3>
 __global__ __launch_bounds__(256, 2) void attention_few_kernel(Call c) {
@@ -141,18 +215,17 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(Call c) {
     constexpr int SPT = PG / KS;              /* steps a tile */
     constexpr int NKB = KS / 16;              /* score blocks */
     constexpr uint32_t EB = E4M3 ? 1 : 2, SLICE = PSLICE * EB;
-    const int kh = blockIdx.x, share = blockIdx.y, b = blockIdx.z;
+    const int kh = blockIdx.x % c.Hkv;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int m = lane & 15, g = lane >> 4;
-    const pg_seq s = seq_of(c, b);
-    const int rows = min(s.ql * c.G, FEW);
-    if (rows <= 0)
+    const Where w = locate<true>(c, blockIdx.x / c.Hkv);
+    if (w.b < 0)
         return;
+    const pg_seq s = w.s;
+    const int b = w.b, nshare = w.nshare, rows = min(s.ql * c.G, FEW);
     const pg_tiles list = pg_tile_list(s, 0, s.ql - 1, c.window, c.sinks);
-    const int nshare = pg_max(pg_div_up(list.ntl, c.share), 1);
-    if (share >= nshare)
-        return;
-    const int tb = share * c.share, steps = min(list.ntl - tb, c.share) * SPT;
+    const int tb = pg_share_begin(list.ntl, w.share, nshare);
+    const int steps = (pg_share_begin(list.ntl, w.share + 1, nshare) - tb) * SPT;
 
     /* this lane's row (column of S^T and O^T) */
     const int row = min(m, rows - 1), tok = row / c.G, head = kh * c.G + row % c.G;
@@ -177,7 +250,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(Call c) {
     u32x4 kr[16], vr[16];
     float ksc[4];
     /* step t (past the last: it again): its page (-1: not there) and first key;
-     * the ids of the share's tiles, FEW_TILES at most, are in a lane each */
+     * the ids of the share's tiles, 64 at most, are in a lane each */
     const int ids = steps > 0 ? page_id(c, b, list, tb + min(lane, steps / SPT - 1)) : -1;
     auto locate = [&](int t, int *page, int *k0) {
         t = min(t, steps - 1);
@@ -189,11 +262,10 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(Call c) {
         const __amdgpu_buffer_rsrc_t r = make_rsrc((const char *)c.k + at * SLICE, SLICE);
         const uint32_t half = k0 % PG * PD * EB;
 #pragma unroll
-        for (int kb = 0; kb < NKB; kb++)
+        for (int i = 0; i < 16 / NKB; i++)
 #pragma unroll
-            for (int i = 0; i < 16 / NKB; i++)
-                kr[kb * (16 / NKB) + i] =
-                    buf_load16(r, kvoff, half + 4 * kb * PD * EB + 64 * i);
+            for (int kb = 0; kb < NKB; kb++)
+                kr[i * NKB + kb] = buf_load16(r, kvoff, half + 4 * kb * PD * EB + 64 * i);
         if constexpr (E4M3) {
 #pragma unroll
             for (int kb = 0; kb < 4; kb++)
@@ -230,18 +302,22 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(Call c) {
         asm volatile("" ::: "memory"); /* Q is read here, not kept */
         floatx4 x[NKB];
 #pragma unroll
-        for (int kb = 0; kb < NKB; kb++) {
-            x[kb] = floatx4{};
+        for (int i2 = 0; i2 < 16 / NKB; i2++) { /* a K load a block, one or two k-steps */
 #pragma unroll
-            for (int ks = 0; ks < 8; ks++) {
-                bf16x8 a;
-                if constexpr (E4M3) {
-                    const u32x4 w = kr[kb * 4 + (ks >> 1)];
-                    a = ks & 1 ? widen(w[2], w[3], ksc[kb]) : widen(w[0], w[1], ksc[kb]);
-                } else {
-                    a = __builtin_bit_cast(bf16x8, kr[kb * 8 + ks]);
+            for (int st = 0; st < (E4M3 ? 2 : 1); st++) {
+                const int ks = E4M3 ? 2 * i2 + st : i2;
+                const bf16x8 q = qf[64 * ks];
+#pragma unroll
+                for (int kb = 0; kb < NKB; kb++) {
+                    const u32x4 w = kr[i2 * NKB + kb];
+                    bf16x8 a;
+                    if constexpr (E4M3)
+                        a = st ? widen(w[2], w[3], ksc[kb]) : widen(w[0], w[1], ksc[kb]);
+                    else
+                        a = __builtin_bit_cast(bf16x8, w);
+                    x[kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        a, q, ks == 0 ? floatx4{} : x[kb], 0, 0, 0);
                 }
-                x[kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[64 * ks], x[kb], 0, 0, 0);
             }
         }
         load_k(page, k0);
@@ -311,33 +387,48 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(Call c) {
             }
         }
     }
+    /* the gates of the rows this wave finishes (wave, wave + 4, ..) are on their way
+     * while the waves merge */
+    const bool whole = nshare == 1, gated = whole && c.gate;
+    bf16x4 gv[FEW / 4];
+#pragma unroll
+    for (int i = 0; i < FEW / 4; i++) {
+        const int r = min(wave + 4 * i, rows - 1);
+        if (gated && wave + 4 * i < rows)
+            gv[i] = *(const bf16x4 *)(c.gate + (size_t)(s.q0 + r / c.G) * c.gts +
+                                      (size_t)(kh * c.G + r % c.G) * c.ghs + 4 * lane);
+    }
     lrun += __shfl_xor(lrun, 16, 64);
     lrun += __shfl_xor(lrun, 32, 64);
 
-    __syncthreads(); /* Q is read */
+    lds_barrier(); /* Q is read */
     /* merge the waves; lane (m, g) holds dims 16 t + 4 g .. + 3 of row m */
 #pragma unroll
     for (int t = 0; t < 16; t++)
         *(floatx4 *)&so[wave][m][16 * t + 4 * g] = o[t];
     if (g == 0)
         sl[wave][m] = lrun, sm[wave][m] = mrun;
-    __syncthreads();
-    const size_t slot = ((size_t)b * c.Hkv + kh) * c.nshare + share;
-    for (int r = wave; r < rows; r += 4) {
+    lds_barrier();
+    const size_t slot = slot_of(c, kh, w.slot0 + w.share);
+#pragma unroll
+    for (int i = 0; i < FEW / 4; i++) {
+        const int r = wave + 4 * i;
+        if (r >= rows)
+            break;
         float ref = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 4; w++)
-            ref = fmaxf(ref, sm[w][r]);
+        for (int v = 0; v < 4; v++)
+            ref = fmaxf(ref, sm[v][r]);
         const float mu = ref == -INFINITY ? 0.f : ref;
         floatx4 acc = {};
         float l = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
-            const float a = fast_exp2(sm[w][r] - mu);
-            acc += *(const floatx4 *)&so[w][r][4 * lane] * a;
-            l += sl[w][r] * a;
+        for (int v = 0; v < 4; v++) {
+            const float a = fast_exp2(sm[v][r] - mu);
+            acc += *(const floatx4 *)&so[v][r][4 * lane] * a;
+            l += sl[v][r] * a;
         }
-        if (nshare > 1) {
+        if (!whole) {
             *(floatx4 *)(c.po + (slot * FEW + r) * PD + 4 * lane) = acc;
             if (lane == 0)
                 c.pl[slot * FEW + r] = l, c.pmu[slot * FEW + r] = mu;
@@ -345,12 +436,10 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(Call c) {
         }
         const int n = s.q0 + r / c.G, hd = kh * c.G + r % c.G;
         const float inv = l > 0.f ? 1.f / l : 0.f;
-        bf16x4 gv = {}, res;
-        if (c.gate)
-            gv = *(const bf16x4 *)(c.gate + (size_t)n * c.gts + (size_t)hd * c.ghs + 4 * lane);
+        bf16x4 res;
 #pragma unroll
         for (int e = 0; e < 4; e++)
-            res[e] = f2bf(acc[e] * inv * (c.gate ? sigmoid_f(bf2f(gv[e])) : 1.f));
+            res[e] = f2bf(acc[e] * inv * (gated ? sigmoid_f(bf2f(gv[i][e])) : 1.f));
         *(bf16x4 *)(c.out + ((size_t)n * c.Hq + hd) * PD + 4 * lane) = res;
     }
 }
@@ -375,7 +464,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(Call c) {
  * mu of its own for the tile and tells the other of its pair through the signs
  * of its P, which are otherwise 0: lane h = 0 sends the low and h = 1 the high
  * half of the float. Both then agree on the larger one and rescale. */
-constexpr int RT = 128;
+constexpr int RT = PG_MANY;
 constexpr float SHIFT_RANGE = 64.f;
 
 template <bool E4M3> struct Lay {
@@ -411,31 +500,28 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
     __shared__ __attribute__((aligned(1024))) unsigned char smem[L::BYTES];
     /* XCD-aware: where the kv-heads divide the 8 XCDs, an XCD's workgroups read
      * the same kv-head. The longest (last) tiles of a sequence start first. */
-    int kh, item;
+    int kh, at;
     if (8 % c.Hkv == 0) {
         const int per = 8 / c.Hkv, xcd = blockIdx.x & 7;
         kh = xcd / per;
-        item = (blockIdx.x >> 3) * per + xcd % per;
+        at = (blockIdx.x >> 3) * per + xcd % per;
     } else {
         kh = blockIdx.x % c.Hkv;
-        item = blockIdx.x / c.Hkv;
+        at = blockIdx.x / c.Hkv;
     }
-    if (item >= c.items)
+    if (at >= c.plan.shares)
         return;
-    item = c.items - 1 - item;
-    pg_seq s;
-    int local;
-    const int b = find_tile<RT>(c, item, &s, &local);
-    if (b < 0)
+    const Where w = locate<true>(c, c.plan.shares - 1 - at);
+    if (w.b < 0)
         return;
-    const int r0 = local * RT, nrows = min(s.ql * c.G - r0, RT);
+    const pg_seq s = w.s;
+    const int b = w.b, nshare = w.nshare;
+    const int r0 = w.unit * RT, nrows = min(s.ql * c.G - r0, RT);
     const int i0 = r0 / c.G, i1 = (r0 + nrows - 1) / c.G;
     const pg_tiles list = pg_tile_list(s, i0, i1, c.window, c.sinks);
-    const int nshare = pg_max(pg_div_up(list.ntl, c.share), 1), share = blockIdx.y;
-    if (share >= nshare)
-        return;
-    const int tb = share * c.share, ntl = min(list.ntl - tb, c.share);
-    const size_t slot = ((size_t)item * c.Hkv + kh) * c.nshare + share;
+    const int tb = pg_share_begin(list.ntl, w.share, nshare);
+    const int ntl = pg_share_begin(list.ntl, w.share + 1, nshare) - tb;
+    const size_t slot = slot_of(c, kh, w.slot0 + w.share);
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int wi = wave & 3, wj = wave >> 2, h = lane >> 5, col = lane & 31;
@@ -938,48 +1024,57 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
     }
 }
 
-/* ---- merge of a tile's shares ----------------------------------------------------
+/* ---- merge of a unit's shares ----------------------------------------------------
  * One wave per row: o = sum_s 2^(mu_s - mu) o_s over the shares that saw keys,
- * l likewise, mu the largest of theirs; then / l and the gate. */
+ * l likewise, mu the largest of theirs; then / l and the gate. l and mu of all
+ * shares come in one load (lane i: share i), o eight shares at a time. */
 template <int ROWS>
-__global__ __launch_bounds__(256) void merge_kernel(Call c) {
+__global__ __launch_bounds__(256) void merge_kernel(Call c, int groups) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int unit = blockIdx.x / (ROWS / 4), t = blockIdx.x % (ROWS / 4) * 4 + wave;
-    const int kh = unit % c.Hkv, item = unit / c.Hkv;
-    pg_seq s;
-    int local = 0;
-    if (ROWS == FEW)
-        s = seq_of(c, item);
-    else if (find_tile<ROWS>(c, item, &s, &local) < 0)
+    const int t = blockIdx.x % groups * 4 + wave, kh = blockIdx.x / groups % c.Hkv;
+    const Where w = locate<false>(c, blockIdx.x / groups / c.Hkv);
+    if (w.b < 0 || w.nshare <= 1)
         return;
-    const int r0 = local * ROWS, nrows = min(s.ql * c.G - r0, ROWS);
-    if (t >= nrows)
+    const int r = w.unit * ROWS + t;
+    if (t >= ROWS || r >= w.s.ql * c.G)
         return;
-    const int i0 = r0 / c.G, i1 = (r0 + nrows - 1) / c.G;
-    const pg_tiles list = pg_tile_list(s, i0, i1, c.window, c.sinks);
-    const int nshare = pg_div_up(list.ntl, c.share);
-    if (nshare <= 1)
-        return;
-    const size_t first = ((size_t)item * c.Hkv + kh) * c.nshare * ROWS + t;
-    float mu = -INFINITY;
-    for (int i = 0; i < nshare; i++)
-        if (c.pl[first + (size_t)i * ROWS] > 0.f)
-            mu = fmaxf(mu, c.pmu[first + (size_t)i * ROWS]);
-    floatx4 acc = {};
-    float l = 0.f;
-    for (int i = 0; i < nshare; i++) {
-        const size_t at = first + (size_t)i * ROWS;
-        if (c.pl[at] > 0.f) {
-            const float w = fast_exp2(c.pmu[at] - mu);
-            acc += *(const floatx4 *)(c.po + at * PD + 4 * lane) * w;
-            l += c.pl[at] * w;
-        }
-    }
-    const int r = r0 + t, n = s.q0 + r / c.G, head = kh * c.G + r % c.G;
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    bf16x4 gv = {}, res;
+    const size_t first = slot_of(c, kh, w.slot0) * ROWS + t;
+    const int n = w.s.q0 + r / c.G, head = kh * c.G + r % c.G;
+    bf16x4 gv = {};
     if (c.gate)
         gv = *(const bf16x4 *)(c.gate + (size_t)n * c.gts + (size_t)head * c.ghs + 4 * lane);
+    float mu = -INFINITY, l = 0.f;
+    floatx4 acc = {};
+    for (int i0 = 0; i0 < w.nshare; i0 += 64) { /* more than 64 shares: in turns */
+        const int cnt = min(w.nshare - i0, 64);
+        const size_t mine = first + (size_t)(i0 + min(lane, cnt - 1)) * ROWS;
+        const float li = lane < cnt ? c.pl[mine] : 0.f;
+        const float mi = li > 0.f ? c.pmu[mine] : -INFINITY;
+        const float next = fmaxf(mu, wave_max(mi));
+        const float ref = next == -INFINITY ? 0.f : next, old = fast_exp2(mu - ref);
+        const float wi = li > 0.f ? fast_exp2(mi - ref) : 0.f;
+        mu = next;
+        l = l * old + wave_sum(wi * li);
+        acc *= old;
+        for (int j0 = 0; j0 < cnt; j0 += 8) {
+            floatx4 v[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                v[j] = *(const floatx4 *)(c.po +
+                                          (first + (size_t)(i0 + min(j0 + j, cnt - 1)) * ROWS) * PD +
+                                          4 * lane);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float f = __uint_as_float((uint32_t)__builtin_amdgcn_readlane(
+                    (int)__float_as_uint(wi), min(j0 + j, 63)));
+                /* a share without keys wrote no o */
+                if (j0 + j < cnt && f > 0.f)
+                    acc += v[j] * f;
+            }
+        }
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    bf16x4 res;
 #pragma unroll
     for (int e = 0; e < 4; e++)
         res[e] = f2bf(acc[e] * inv * (c.gate ? sigmoid_f(bf2f(gv[e])) : 1.f));
@@ -990,51 +1085,11 @@ __global__ __launch_bounds__(256) void merge_kernel(Call c) {
 } // namespace CUJEV_KNS
 using namespace CUJEV_KNS;
 
-/* How a call is run: rows a tile, tiles at most, key tiles a share, shares. */
-struct paged_plan {
-    int rt, items, share, nshare;
-};
-static paged_plan plan_of(int N, int B, int max_q, int max_kv, int G, int Hkv, int window,
-                          int sinks) {
-    paged_plan p = {0, 0, 1, 1};
-    if (N <= 0 || B <= 0 || max_q <= 0)
-        return p;
-    const long long mq = max_q < N ? max_q : N;
-    p.rt = mq * G <= FEW ? FEW : RT;
-    long long items = B;
-    if (p.rt == RT) {
-        const long long by_rows = (long long)N * G / RT + B, by_len = B * ((mq * G + RT - 1) / RT);
-        items = by_rows < by_len ? by_rows : by_len;
-    }
-    if (items * Hkv > 1 << 22) {
-        p.items = -1;
-        return p;
-    }
-    p.items = (int)items;
-    const int tok = p.rt == FEW ? (int)mq : RT / G + 2;
-    const int most = pg_max(pg_max_tiles(tok, max_kv, window, sinks), 1);
-    const int units = p.items * Hkv;
-    int n = p.rt == FEW ? 1024 / units : 512 / units;
-    n = n < 1 ? 1 : n;
-    p.share = pg_div_up(most, n);
-    if (p.share < 4)
-        p.share = 4;
-    if (p.rt == FEW && p.share > FEW_TILES)
-        p.share = FEW_TILES;
-    p.nshare = pg_div_up(most, p.share);
-    return p;
-}
-static size_t plan_rows(const paged_plan &p, int Hkv) {
-    return p.nshare > 1 ? (size_t)p.items * Hkv * p.nshare * p.rt : 0;
-}
-
 extern "C" size_t cujev_attention_paged_ws_bytes(int N, int B, int max_q, int max_kv, int Hq,
                                                  int Hkv, int window, int sinks, int type) {
-    (void)type;
-    if (window >= max_kv)
-        window = sinks = 0;
-    const paged_plan p = plan_of(N, B, max_q, max_kv, Hq / Hkv, Hkv, window, sinks);
-    return plan_rows(p, Hkv) * (PD + 2) * sizeof(float);
+    const pg_plan p = pg_make_plan(N, B, max_q, max_kv, Hq / Hkv, Hkv, window, sinks,
+                                   type == CUJEV_KV_E4M3);
+    return (size_t)p.slots * Hkv * p.rt * (PD + 2) * sizeof(float);
 }
 
 extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int gate_tok_stride,
@@ -1042,43 +1097,42 @@ extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int
                                         const cujev_paged_seqs *seqs, int N, int max_q, int max_kv,
                                         int Hq, int window, int sinks, bf16_t *out, void *ws,
                                         size_t ws_bytes, hipStream_t stream) {
-    const int Hkv = pages->Hkv, B = seqs->B;
-    if (window >= max_kv) /* no row's window ends before its first key */
-        window = sinks = 0;
-    const paged_plan p = plan_of(N, B, max_q, max_kv, Hq / Hkv, Hkv, window, sinks);
-    if (p.items == 0)
+    const int Hkv = pages->Hkv, B = seqs->B, G = Hq / Hkv;
+    const bool e4m3 = pages->type == CUJEV_KV_E4M3;
+    const pg_plan p = pg_make_plan(N, B, max_q, max_kv, G, Hkv, window, sinks, e4m3);
+    if (p.shares == 0)
         return hipSuccess;
-    if (p.items < 0 || Hkv > 65535 || p.nshare > 65535 || (p.rt == FEW && B > 65535))
+    if (p.shares < 0)
         return hipErrorInvalidValue;
-    const size_t rows = plan_rows(p, Hkv);
+    const size_t rows = (size_t)p.slots * Hkv * p.rt;
     if (rows * (PD + 2) * sizeof(float) > ws_bytes)
         return hipErrorInvalidValue;
+    if (window >= max_kv) /* no row's window ends before its first key */
+        window = sinks = 0;
     const Call c = {(const bf16 *)q, (const bf16 *)gate, gate_tok_stride, gate_head_stride,
                     pages->k, pages->vt, pages->k_scale, pages->v_scale, pages->num_pages,
                     seqs->q_start, seqs->kv_len, seqs->page_table, seqs->max_pages, B, N,
-                    max_q, max_kv, Hq, Hkv, Hq / Hkv, window, sinks, (bf16 *)out,
-                    (float *)ws, (float *)ws + rows * PD, (float *)ws + rows * (PD + 1),
-                    p.items, p.share, p.nshare};
-    const bool e4m3 = pages->type == CUJEV_KV_E4M3;
-    if (p.rt == FEW) {
-        const dim3 grid((unsigned)Hkv, (unsigned)p.nshare, (unsigned)B);
-        if (e4m3)
-            hipLaunchKernelGGL(attention_few_kernel<true>, grid, dim3(256), 0, stream, c);
+                    max_q, max_kv, Hq, Hkv, G, window, sinks, (bf16 *)out,
+                    (float *)ws, (float *)ws + rows * PD, (float *)ws + rows * (PD + 1), p};
+    const bool few = p.rt == FEW;
+    const int per = !few && 8 % Hkv == 0 ? 8 / Hkv : 1;
+    const dim3 grid((unsigned)(pg_div_up(p.shares, per) * per * Hkv));
+    if (few && e4m3)
+        hipLaunchKernelGGL(attention_few_kernel<true>, grid, dim3(256), 0, stream, c);
+    else if (few)
+        hipLaunchKernelGGL(attention_few_kernel<false>, grid, dim3(256), 0, stream, c);
+    else if (e4m3)
+        hipLaunchKernelGGL(attention_many_kernel<true>, grid, dim3(512), 0, stream, c);
+    else
+        hipLaunchKernelGGL(attention_many_kernel<false>, grid, dim3(512), 0, stream, c);
+    if (p.slots > 0) {
+        const long long rows_most = (long long)pg_min(max_q, N) * G;
+        const int groups = pg_div_up(rows_most < p.rt ? (int)rows_most : p.rt, 4);
+        const dim3 mgrid((unsigned)(p.units * Hkv * groups));
+        if (few)
+            hipLaunchKernelGGL(merge_kernel<FEW>, mgrid, dim3(256), 0, stream, c, groups);
         else
-            hipLaunchKernelGGL(attention_few_kernel<false>, grid, dim3(256), 0, stream, c);
-        if (p.nshare > 1)
-            hipLaunchKernelGGL(merge_kernel<FEW>, dim3((unsigned)(p.items * Hkv * (FEW / 4))),
-                               dim3(256), 0, stream, c);
-    } else {
-        const int per = 8 % Hkv == 0 ? 8 / Hkv : 1;
-        const dim3 grid((unsigned)(pg_div_up(p.items, per) * per * Hkv), (unsigned)p.nshare);
-        if (e4m3)
-            hipLaunchKernelGGL(attention_many_kernel<true>, grid, dim3(512), 0, stream, c);
-        else
-            hipLaunchKernelGGL(attention_many_kernel<false>, grid, dim3(512), 0, stream, c);
-        if (p.nshare > 1)
-            hipLaunchKernelGGL(merge_kernel<RT>, dim3((unsigned)(p.items * Hkv * (RT / 4))),
-                               dim3(256), 0, stream, c);
+            hipLaunchKernelGGL(merge_kernel<RT>, mgrid, dim3(256), 0, stream, c, groups);
     }
     return hipGetLastError();
 }

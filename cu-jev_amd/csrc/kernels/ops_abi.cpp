@@ -307,7 +307,7 @@ static int paged_check(const char *what, const cujev_kv_pages *pages, const int3
         return fail(1, "%s: bad page pool (type %d, %d pages, %d kv-heads; pointers set and "
                        "16-byte aligned, scales with e4m3)",
                     what, pages->type, pages->num_pages, pages->Hkv);
-    if (B < 0 || B > PG_MOST || max_pages <= 0 || max_pages > PG_MOST / CUJEV_KV_PAGE ||
+    if (B < 0 || B > PG_MOST || max_pages <= 0 || max_pages > PG_MOST_KEYS / CUJEV_KV_PAGE ||
         (B > 0 && (!page_table || !kv_len)))
         return fail(1, "%s: bad page table (B=%d, max_pages=%d)", what, B, max_pages);
     return 0;

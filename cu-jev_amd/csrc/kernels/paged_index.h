@@ -15,9 +15,10 @@ constexpr int pg_div_up(int a, int b) { return a / b + (a % b != 0); } /* a >= 0
 /* Sequence b as one call sees it: rows q0 .. q0 + ql - 1, the first at position
  * p0 (negative where it has fewer keys than rows: those rows have no slot),
  * keys 0 .. kv - 1. Lengths outside the call's N rows, max_q and max_kv are
- * cut, so no value in q_start or kv_len leads out of a buffer. N, max_kv and
- * windows are at most 2^30: sums and differences of two fit an int. */
-constexpr int PG_MOST = 1 << 30;
+ * cut, so no value in q_start or kv_len leads out of a buffer. N and B are at most
+ * PG_MOST, max_kv and windows PG_MOST_KEYS: sums and differences of two fit an
+ * int, and the key tiles of fewer than 512 units 32 bits. */
+constexpr int PG_MOST = 1 << 30, PG_MOST_KEYS = 1 << 28;
 struct pg_seq {
     int q0, ql, kv, p0;
 };
@@ -66,6 +67,92 @@ constexpr int pg_max_tiles(int tok, int max_kv, int window, int sinks) {
     if (window <= 0 || window > max_kv || tok > max_kv)
         return all;
     return pg_min(all, (window + tok) / PG + 2 + pg_div_up(pg_min(sinks, max_kv), PG));
+}
+
+/* ---- how the attention's work is shared out ----------------------------------
+ * A unit is a tile of rt packed rows (token, q-head of the group) of a sequence and
+ * kv-head; a share is a part of a unit's key tiles. rt is PG_FEW where no sequence
+ * of the call has more rows than that (one unit each), PG_MANY otherwise. */
+constexpr int PG_FEW = 16, PG_MANY = 128;
+constexpr int PG_FEW_SHARE = 64; /* key tiles a share of PG_FEW rows, at most */
+
+struct pg_plan {
+    int rt;
+    int units;  /* units of a kv-head, at most */
+    int shares; /* shares of a kv-head, at most (workgroups; 0: no work, -1: too many) */
+    int slots;  /* of those, at most, with partial results to merge (0: no merge) */
+    int goal;   /* workgroups of a kv-head that the chip runs at once; 0: do not share out */
+    int least;  /* key tiles a share, at least */
+};
+
+constexpr int pg_units(const pg_seq &s, int G, int rt) {
+    return (int)(((long long)s.ql * G + rt - 1) / rt);
+}
+/* Key tiles of a sequence's longest unit, 1 at least: the last one's (with a window
+ * a full one before it may have a tile or two more) */
+constexpr int pg_longest(const pg_seq &s, int G, int rt, int window, int sinks) {
+    if (s.ql <= 0)
+        return 0;
+    const int units = pg_units(s, G, rt);
+    const pg_tiles t =
+        pg_tile_list(s, (int)((long long)(units - 1) * rt / G), s.ql - 1, window, sinks);
+    return pg_max(t.ntl, 1);
+}
+/* Key tiles a share should have, for U units of a kv-head with T tiles in all. A
+ * sequence's last share is half empty on average: as many workgroups fewer to
+ * count on. */
+constexpr int pg_share(const pg_plan &p, int U, unsigned T) {
+    const int cap = p.rt == PG_FEW ? PG_FEW_SHARE : PG_MOST;
+    if (p.goal == 0 || U >= p.goal)
+        return cap;
+    const unsigned n = (unsigned)pg_max(p.goal - U / 2, U);
+    return pg_min(pg_max((int)(T / n + (T % n != 0)), p.least), cap);
+}
+constexpr int pg_nshare(int tiles, int share) { return pg_max(pg_div_up(tiles, share), 1); }
+/* First list entry of share i of n even ones */
+constexpr int pg_share_begin(int ntl, int i, int n) { return (int)((long long)ntl * i / n); }
+
+constexpr pg_plan pg_make_plan(int N, int B, int max_q, int max_kv, int G, int Hkv, int window,
+                               int sinks, bool e4m3) {
+    pg_plan p{};
+    const long long mq = pg_min(max_q, N);
+    p.rt = mq * G <= PG_FEW ? PG_FEW : PG_MANY;
+    if (mq <= 0 || B <= 0)
+        return p;
+    long long units = B;
+    if (p.rt == PG_MANY) {
+        const long long by_rows = (long long)N * G / PG_MANY + B;
+        const long long by_len = B * ((mq * G + PG_MANY - 1) / PG_MANY);
+        units = by_rows < by_len ? by_rows : by_len;
+    }
+    if (window >= max_kv)
+        window = sinks = 0;
+    const int tok = p.rt == PG_FEW ? (int)mq : PG_MANY / G + 2;
+    const int most = pg_max(pg_max_tiles(tok, max_kv, window, sinks), 1);
+    const bool few = p.rt == PG_FEW;
+    p.goal = pg_max((few ? 512 : 256) / Hkv, 1);
+    p.least = few ? (e4m3 ? 4 : 2) : 8;
+    /* the rows that the caller brings fill the chip: whole units */
+    if (few ? units >= p.goal : (long long)N * G / PG_MANY >= p.goal)
+        p.goal = 0;
+    /* sum over units of max(ceil(t / share), 1), with share = ceil(T / n) at least: n
+     * + units, n <= max(goal, units) */
+    long long shares = units;
+    if (p.goal > 0 && most > p.least)
+        shares = units < p.goal ? p.goal + units : units < 2ll * p.goal ? 2ll * p.goal : units;
+    if (few && most > PG_FEW_SHARE) {
+        const long long capped = units * pg_div_up(most, PG_FEW_SHARE);
+        shares = shares < capped ? capped : shares;
+    }
+    if (units * Hkv > 1 << 22 || shares * Hkv > 1 << 22) {
+        p.shares = -1;
+        return p;
+    }
+    p.units = (int)units;
+    p.shares = (int)shares;
+    const bool split = p.goal > 0 ? most > p.least : few && most > PG_FEW_SHARE;
+    p.slots = split ? (int)shares : 0;
+    return p;
 }
 
 /* Whether every row at positions pmin .. pmax sees all PG keys from k0 on */

@@ -51,7 +51,7 @@ def test_an_empty_call_does_nothing(name):
 BAD_POOL = [dict(kv_type=2), dict(kv_type=-1), dict(k_pages=None), dict(vt_pages=None),
             dict(k_pages=FAKE + 8), dict(vt_pages=FAKE + 2), dict(k_scale=None),
             dict(v_scale=None), dict(v_scale=FAKE + 4), dict(num_pages=0), dict(num_pages=-1),
-            dict(Hkv=0), dict(max_pages=0), dict(max_pages=1 << 26), dict(B=-1),
+            dict(Hkv=0), dict(max_pages=0), dict(max_pages=(1 << 22) + 1), dict(B=-1),
             dict(B=1, page_table=None), dict(B=1, kv_len=None)]
 
 

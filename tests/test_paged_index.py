@@ -24,12 +24,12 @@ int main() {
     /* any lengths at all stay inside the call */
     const int odd[] = {0, 1, -1, 5, 63, 64, 65, 200, 4096, PG_MOST, -PG_MOST, 0x7fffffff, (int)0x80000000};
     for (int q0 : odd) for (int q1 : odd) for (int kv : odd) for (int N : {0, 1, 64, 200, PG_MOST})
-        for (int mq : {0, 1, 100, PG_MOST}) for (int mk : {0, 1, 64, 1000, PG_MOST}) {
+        for (int mq : {0, 1, 100, PG_MOST}) for (int mk : {0, 1, 64, 1000, PG_MOST_KEYS}) {
             const pg_seq s = pg_clean_seq(q0, q1, kv, N, mq, mk);
             NEED(s.q0 >= 0 && s.ql >= 0 && s.ql <= mq && (long long)s.q0 + s.ql <= N);
             NEED(s.kv >= 0 && s.kv <= mk && s.p0 >= -N);
             NEED(pg_new_lo(s) >= 0 && (pg_new_hi(s) <= s.kv));
-            for (int w : {0, 1, 100, PG_MOST}) for (int S : {0, 1, 64, 65, PG_MOST}) {
+            for (int w : {0, 1, 100, PG_MOST_KEYS}) for (int S : {0, 1, 64, 65, PG_MOST}) {
                 if (s.ql == 0) continue;
                 const pg_tiles t = pg_tile_list(s, 0, s.ql - 1, w, w ? S : 0);
                 NEED(t.ntl >= 0 && t.nsk >= 0 && t.nsk <= t.ntl);
@@ -101,6 +101,58 @@ int main() {
             NEED((int)seen.size() == pg_max(pg_new_hi(s) - pg_new_lo(s), 0));
         }
         NEED(groups <= (N < N / VTOK + 2 * B ? N : N / VTOK + 2 * B));
+    }
+    /* the plan: shares tile each unit's list, and the launch and slots hold them */
+    for (int it = 0; it < 30000; it++) {
+        const int G = 1 << rnd(0, 4), Hkv = 1 << rnd(0, 3), e4m3 = rnd(0, 1);
+        const int B = it % 7 ? rnd(1, 12) : rnd(1, 600), top = it % 3 ? 1 << rnd(0, 13) : 20000;
+        const int mq = it % 2 ? rnd(1, 3) : rnd(1, 300), w = rnd(0, 2) ? 0 : rnd(1, 2000), S = w ? rnd(0, 100) : 0;
+        std::vector<int> q, kv;
+        int N = rnd(0, 3), max_q = 0, max_kv = 1;
+        for (int b = 0; b < B; b++) {
+            q.push_back(rnd(0, 3) ? rnd(0, mq) : mq), kv.push_back(rnd(0, top));
+            N += q[b], max_q = pg_max(max_q, q[b]), max_kv = pg_max(max_kv, kv[b]);
+        }
+        if (rnd(0, 1)) max_kv += rnd(0, 500);
+        const pg_plan p = pg_make_plan(N, B, max_q, max_kv, G, Hkv, w, S, e4m3);
+        const int W = w >= max_kv ? 0 : w, SS = W ? S : 0;
+        long long U = 0, T = 0, C = 0;
+        int at = 0;
+        std::vector<pg_seq> seqs;
+        for (int b = 0; b < B; b++) {
+            seqs.push_back(pg_clean_seq(at, at + q[b], kv[b], N, max_q, max_kv));
+            at += q[b];
+            const int u = max_q ? pg_units(seqs[b], G, p.rt) : 0;
+            U += u, T += (long long)u * pg_longest(seqs[b], G, p.rt, W, SS);
+        }
+        if (max_q == 0) { NEED(p.shares == 0); continue; }
+        NEED(p.rt == (max_q * G <= 16 ? 16 : 128) && U <= p.units);
+        const int share = pg_share(p, (int)U, (unsigned)T);
+        NEED(p.rt == 128 || share <= 64);
+        for (int b = 0; b < B; b++) {
+            const int u = pg_units(seqs[b], G, p.rt), n = pg_nshare(pg_longest(seqs[b], G, p.rt, W, SS), share);
+            C += (long long)u * n;
+            NEED(u == 0 || n == 1 || p.slots > 0);
+            for (int k = 0; k < u; k++) {
+                const int r0 = k * p.rt, rows = pg_min(seqs[b].ql * G - r0, p.rt);
+                NEED(rows > 0);
+                const pg_tiles t = pg_tile_list(seqs[b], r0 / G, (r0 + rows - 1) / G, W, SS);
+                NEED(pg_share_begin(t.ntl, 0, n) == 0 && pg_share_begin(t.ntl, n, n) == t.ntl);
+                for (int i = 0; i < n && i < 70; i++) {
+                    const int len = pg_share_begin(t.ntl, i + 1, n) - pg_share_begin(t.ntl, i, n);
+                    NEED(len >= 0 && (p.rt == 128 || len <= 64));
+                }
+            }
+        }
+        NEED(C <= p.shares && (p.slots == 0 || p.slots >= C));
+    }
+    {   /* the largest call: nothing overflows */
+        const pg_plan p = pg_make_plan(PG_MOST, 1, PG_MOST, PG_MOST_KEYS, 16, 1, 0, 0, true);
+        NEED(p.shares == -1);
+        const pg_plan f = pg_make_plan(60, 60, 1, PG_MOST_KEYS, 16, 1, 0, 0, true);
+        const pg_seq s = pg_clean_seq(0, 1, PG_MOST_KEYS, 60, 1, PG_MOST_KEYS);
+        const int share = pg_share(f, 60, 60u * (unsigned)pg_longest(s, 16, 16, 0, 0));
+        NEED(share == 64 && 60ll * pg_nshare(pg_longest(s, 16, 16, 0, 0), share) <= f.shares);
     }
     printf("bad %d\n", bad);
     return bad != 0;
