@@ -90,16 +90,14 @@ DEV void settle(floatx16 (&o)[4]) {
 /* keys hi at most, and past lo or a sink (without branches) */
 DEV bool key_seen(int j, int hi, int lo, int sinks) { return (j <= hi) & ((j > lo) | (j < sinks)); }
 
-/* What both kernels and the merge share.
+/* What the kernels and the merge share.
  *
- * The work of a kv-head is its units, tiles of RT packed rows of a sequence. So
- * that the workgroups of a call finish together however uneven its sequences,
- * each of them works out the same plan from q_start and kv_len: the key tiles of
- * all units (a sequence's units counted with its longest list) over the
- * workgroups that the chip holds at once give the tiles a share should have,
- * and a sequence's units are cut into as many even shares as that asks for. A
- * unit of several shares keeps, per share, unnormalised o, l and the softmax's
- * reference mu of its rows in a slot each, for the merge. */
+ * The work of a kv-head is its units, tiles of packed rows of a sequence. So that
+ * all parts of a call finish together however uneven its sequences are, each
+ * workgroup works out the same plan from q_start and kv_len: what all units have
+ * to do, over what the chip runs at once, gives the size of a share
+ * (paged_index.h). A unit that several shares work on keeps, in a slot for each,
+ * unnormalised o, l and the softmax's reference mu of its rows, for the merge. */
 struct Call {
     const bf16 *q, *gate;
     int gts, ghs;
@@ -124,138 +122,180 @@ DEV int wave_sum_i(int v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1)
         v += __shfl_xor(v, o, 64);
-    return v;
+    return __builtin_amdgcn_readfirstlane(v); /* uniform, for the compiler too */
 }
-/* Where a workgroup (BY_SHARE: share `target` of a kv-head) or a merging wave
- * (unit `target`) works: the sequence (-1: no such share or unit), the number of
- * its unit in it, the share, the unit's shares and the slot of its first. */
+/* The unit that part `target` of a kv-head belongs to (BY_PART), or unit `target`:
+ * its sequence (b -1: there is none), its number in it, its parts, the first
+ * one's number, which of them `target` is. With few rows the parts are those of
+ * the pieces of the line (numbered by pg_few_slot), and begin .. begin + own the
+ * unit's steps on it, with many rows the unit's shares. */
 struct Where {
     pg_seq s;
-    int b, unit, share, nshare, slot0;
+    int b, unit, parts, first, part;
+    int begin, own, size; /* few rows: the unit on the line, steps a piece */
 };
-template <bool BY_SHARE> DEV Where locate(const Call &c, int target) {
+template <int RT_, int KS, bool BY_PART> DEV Where locate(const Call &c, int target) {
+    constexpr bool FEWR = RT_ == PG_FEW;
     const int lane = threadIdx.x & 63;
     Where w;
-    w.b = -1;
+    w.b = -1, w.begin = w.own = w.size = 0;
+    /* a sequence's units, and what each has: steps of KS keys, or key tiles */
+    auto units_of = [&](const pg_seq &s) { return pg_units(s, c.G, RT_); };
+    auto each = [&](const pg_seq &s) {
+        const int tiles = pg_longest(s, c.G, RT_, c.window, c.sinks);
+        return FEWR ? tiles * (PG / KS) : tiles;
+    };
     if (c.B == 1) { /* no scan for one sequence */
-        const pg_seq s = seq_of(c, 0);
-        const int units = pg_units(s, c.G, c.plan.rt);
-        const int tiles = pg_longest(s, c.G, c.plan.rt, c.window, c.sinks);
-        const int n = pg_nshare(tiles, pg_share(c.plan, units, (unsigned)units * (unsigned)tiles));
-        if (target >= units * (BY_SHARE ? n : 1))
+        w.s = seq_of(c, 0);
+        const int units = units_of(w.s), n = each(w.s);
+        if (units == 0)
             return w;
-        w.s = s, w.b = 0, w.nshare = n;
-        w.unit = BY_SHARE ? target / n : target;
-        w.share = BY_SHARE ? target % n : 0;
-        w.slot0 = w.unit * n;
+        if constexpr (FEWR) {
+            w.size = pg_few_share(c.plan, (unsigned)n, n);
+            w.own = n;
+            w.parts = (n - 1) / w.size + 1;
+        } else {
+            w.parts = pg_nshare(n, pg_share(c.plan, units, (unsigned)units * (unsigned)n));
+        }
+        w.unit = BY_PART ? target / w.parts : target;
+        w.first = w.unit * w.parts;
+        w.part = BY_PART ? target - w.first : 0;
+        w.b = w.unit < units ? 0 : -1;
         return w;
     }
-    int U = 0;
+    int U = 0, most = 0;
     unsigned T = 0;
     for (int b0 = 0; b0 < c.B; b0 += 64) {
-        const bool in = b0 + lane < c.B;
         const pg_seq s = seq_of(c, min(b0 + lane, c.B - 1));
-        const int units = in ? pg_units(s, c.G, c.plan.rt) : 0;
+        const int units = b0 + lane < c.B ? units_of(s) : 0, n = units ? each(s) : 0;
         U += units;
-        T += (unsigned)units * (unsigned)pg_longest(s, c.G, c.plan.rt, c.window, c.sinks);
+        T += (unsigned)units * (unsigned)n;
+        most = max(most, n);
     }
-    const int share = pg_share(c.plan, wave_sum_i(U), (unsigned)wave_sum_i((int)T));
-    int before_u = 0, before_s = 0;
+    T = (unsigned)wave_sum_i((int)T);
+    int size;
+    if constexpr (FEWR) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1)
+            most = max(most, __shfl_xor(most, o, 64));
+        size = pg_few_share(c.plan, T, __builtin_amdgcn_readfirstlane(most));
+    } else {
+        size = pg_share(c.plan, wave_sum_i(U), T);
+    }
+    int before_u = 0, before_n = 0;
     for (int b0 = 0; b0 < c.B; b0 += 64) {
-        const bool in = b0 + lane < c.B;
         const pg_seq s = seq_of(c, min(b0 + lane, c.B - 1));
-        const int n = pg_nshare(pg_longest(s, c.G, c.plan.rt, c.window, c.sinks), share);
-        const int units = in ? pg_units(s, c.G, c.plan.rt) : 0, shares = units * n;
-        int su = units, ss = shares; /* inclusive sums over the lanes */
+        const int units = b0 + lane < c.B ? units_of(s) : 0, n = each(s);
+        const int parts = FEWR ? 0 : pg_nshare(n, size);
+        const int all = units * (FEWR ? n : parts);
+        int su = units, sn = all; /* inclusive sums over the lanes */
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
-            const int x = __shfl_up(su, o, 64), y = __shfl_up(ss, o, 64);
+            const int x = __shfl_up(su, o, 64), y = __shfl_up(sn, o, 64);
             su += lane >= o ? x : 0;
-            ss += lane >= o ? y : 0;
+            sn += lane >= o ? y : 0;
         }
-        const uint64_t past =
-            __ballot(BY_SHARE ? before_s + ss > target : before_u + su > target);
+        su += before_u, sn += before_n;
+        const int u = su - units, a = sn - all; /* before this lane's sequence */
+        /* few rows: one unit, its parts are pieces p0 .. p1 */
+        const int p0 = FEWR ? a / size : 0, p1 = FEWR ? (sn - 1) / size : 0;
+        const bool mine = !BY_PART ? su > target
+                          : FEWR   ? units > 0 && pg_few_slot(p1, u) >= target
+                                   : sn > target;
+        const uint64_t past = __ballot(mine);
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
             auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
             w.s.q0 = of(s.q0), w.s.ql = of(s.ql), w.s.kv = of(s.kv), w.s.p0 = of(s.p0);
             w.b = b0 + l;
-            w.nshare = of(n);
-            const int local = target - (BY_SHARE ? before_s + of(ss - shares)
-                                                 : before_u + of(su - units));
-            w.unit = BY_SHARE ? local / w.nshare : local;
-            w.share = BY_SHARE ? local % w.nshare : 0;
-            w.slot0 = before_s + of(ss - shares) + w.unit * w.nshare;
+            if constexpr (FEWR) {
+                w.unit = 0, w.begin = of(a), w.own = of(n), w.size = size;
+                w.first = pg_few_slot(of(p0), of(u));
+                w.parts = of(p1) - of(p0) + 1;
+                w.part = BY_PART ? target - w.first : 0;
+                if (w.part < 0) /* a number between two units' */
+                    w.b = -1;
+            } else {
+                w.parts = of(parts);
+                w.unit = BY_PART ? (target - of(a)) / w.parts : target - of(u);
+                w.first = of(a) + w.unit * w.parts;
+                w.part = BY_PART ? target - w.first : 0;
+            }
             return w;
         }
-        before_u += __builtin_amdgcn_readlane(su, 63);
-        before_s += __builtin_amdgcn_readlane(ss, 63);
+        before_u = __builtin_amdgcn_readlane(su, 63);
+        before_n = __builtin_amdgcn_readlane(sn, 63);
     }
     return w;
 }
-/* The slot of share `at` of a kv-head */
+/* The slot of part `at` of a kv-head */
 DEV size_t slot_of(const Call &c, int kh, int at) { return (size_t)kh * c.plan.slots + at; }
 
 /* ---- few rows: up to 16 packed rows of a sequence and kv-head ------------------
- * Bound by the K/V bytes. A workgroup takes one share of the key tiles; its 4
- * waves take steps (32 keys of bf16, a tile of e4m3) in turn and work alone
- * until they merge through LDS. K and V^T go from memory into registers as
- * the operands of v_mfma_f32_16x16x32_bf16, 16 loads each of 16 bytes a lane
- * (64 bytes of 16 rows): K of the next step is in flight during the softmax and
- * the PV products, V^T during the scores. All loads are unconditional (past
- * the end the last step's again), so a wait for one operand's counts the other's
- * in flight and not more; with 256 registers two waves share a SIMD. */
+ * Bound by the K/V bytes, so that what counts is that every wave of the chip
+ * streams all the time. The steps of all units of a kv-head (32 keys of bf16, a
+ * tile of 64 of e4m3: 32 KiB of K and V) are one line, cut into equal pieces; a wave
+ * takes a piece, or the part of it that lies in one unit, and waits for no other. K and V^T go from memory into registers as the operands of
+ * v_mfma_f32_16x16x32_bf16, 16 loads each of 16 bytes a lane (64 bytes of 16
+ * rows): K of the next step is in flight during the softmax and the PV products,
+ * V^T during the scores. All loads are unconditional (past the end the last
+ * step's again), so a wait for one operand's counts the other's in flight and not
+ * more; in 256 registers two waves share a SIMD. Q waits in LDS: read again each
+ * step, it leaves the registers to loads. */
 constexpr int FEW = PG_FEW;
 
 template <bool E4M3>
-__global__ __launch_bounds__(256, 2) void attention_few_kernel(Call c) {
-    __shared__ __attribute__((aligned(16))) float so[4][FEW][PD];
-    __shared__ float sl[4][FEW], sm[4][FEW];
+__global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
     constexpr int KS = E4M3 ? 64 : 32;        /* keys a step */
     constexpr int SPT = PG / KS;              /* steps a tile */
     constexpr int NKB = KS / 16;              /* score blocks */
     constexpr uint32_t EB = E4M3 ? 1 : 2, SLICE = PSLICE * EB;
+    __shared__ bf16x8 sq[8 * 64];
     const int kh = blockIdx.x % c.Hkv;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int m = lane & 15, g = lane >> 4;
-    const Where w = locate<true>(c, blockIdx.x / c.Hkv);
+    const int lane = threadIdx.x, m = lane & 15, g = lane >> 4;
+    const Where w = locate<FEW, KS, true>(c, blockIdx.x / c.Hkv);
     if (w.b < 0)
         return;
     const pg_seq s = w.s;
-    const int b = w.b, nshare = w.nshare, rows = min(s.ql * c.G, FEW);
+    const int b = w.b, rows = min(s.ql * c.G, FEW);
     const pg_tiles list = pg_tile_list(s, 0, s.ql - 1, c.window, c.sinks);
-    const int tb = pg_share_begin(list.ntl, w.share, nshare);
-    const int steps = (pg_share_begin(list.ntl, w.share + 1, nshare) - tb) * SPT;
-
-    /* this lane's row (column of S^T and O^T) */
-    const int row = min(m, rows - 1), tok = row / c.G, head = kh * c.G + row % c.G;
-    const int hi = min(s.p0 + tok, s.kv - 1), lo = pg_low(s.p0 + tok, c.window);
-    const int own_lo = pg_low(s.p0, c.window); /* of the first row: below, no row's key */
-    /* Q's operands wait in LDS (where the merge comes later): read again each
-     * step, they leave the registers to loads in flight */
-    bf16x8 *const qf = (bf16x8 *)&so[0][0][0] + lane;
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int ks = 2 * wave + i; /* its dims: as K's loads below */
-        qf[64 * ks] = *(const bf16x8 *)(c.q + ((size_t)(s.q0 + tok) * c.Hq + head) * PD +
-                                        (E4M3 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1)
-                                              : 32 * ks + 8 * g));
-    }
+    /* steps [i0, i1) of the unit; a unit without a key has some that see none */
+    const int cut = (w.begin / w.size + w.part) * w.size - w.begin;
+    const int i0 = max(cut, 0), i1 = min(cut + w.size, w.own);
+    const int steps = min(i1, list.ntl * SPT);
+    bf16x8 *const qf = sq + lane;
     /* Row m of score block kb is key key0 + 4 kb of the step: lane g then holds,
      * in accumulators 4 kb .. + 3, the keys (KS / 4) g .. that its V^T loads
      * bring. */
     const int key0 = KS / 4 * (m >> 2) + (m & 3), keyg = KS / 4 * g;
     const uint32_t kvoff = key0 * PD * EB + 16 * g, vvoff = m * PG * EB + 16 * g;
 
+    /* this lane's row (column of S^T and O^T) */
+    const int row = min(m, rows - 1), tok = row / c.G, head = kh * c.G + row % c.G;
+    const int hi = min(s.p0 + tok, s.kv - 1), lo = pg_low(s.p0 + tok, c.window);
+    const int own_lo = pg_low(s.p0, c.window); /* of the first row: below, no row's key */
+    {
+        const bf16 *qp = c.q + ((size_t)(s.q0 + tok) * c.Hq + head) * PD;
+#pragma unroll
+        for (int ks = 0; ks < 8; ks++) /* dims as K's loads below */
+            qf[64 * ks] = *(const bf16x8 *)(qp + (E4M3 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1)
+                                                       : 32 * ks + 8 * g));
+    }
+
     u32x4 kr[16], vr[16];
     float ksc[4];
     /* step t (past the last: it again): its page (-1: not there) and first key;
-     * the ids of the share's tiles, 64 at most, are in a lane each */
-    const int ids = steps > 0 ? page_id(c, b, list, tb + min(lane, steps / SPT - 1)) : -1;
-    auto locate = [&](int t, int *page, int *k0) {
+     * the ids of 64 tiles of the list are in a lane each */
+    int ids = -1, ids0 = -64;
+    auto locate_step = [&](int t, int *page, int *k0) {
         t = min(t, steps - 1);
-        *page = __builtin_amdgcn_readlane(ids, t / SPT);
-        *k0 = pg_tile_page(list, tb + t / SPT) * PG + t % SPT * KS;
+        const int i = t / SPT;
+        if (i - ids0 >= 64) {
+            ids0 = i;
+            ids = page_id(c, b, list, min(i + lane, list.ntl - 1));
+        }
+        *page = __builtin_amdgcn_readlane(ids, i - ids0);
+        *k0 = pg_tile_page(list, i) * PG + t % SPT * KS;
     };
     auto load_k = [&](int page, int k0) {
         const size_t at = (size_t)max(page, 0) * c.Hkv + kh;
@@ -279,12 +319,11 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(Call c) {
         o[i] = floatx4{};
     float mrun = -INFINITY, lrun = 0.f;
     int page = -1, k0 = 0;
-    if (wave < steps) {
-        locate(wave, &page, &k0);
+    if (i0 < steps) {
+        locate_step(i0, &page, &k0);
         load_k(page, k0);
     }
-    lds_barrier();
-    for (int i = wave; i < steps; i += 4) {
+    for (int i = i0; i < steps; i++) {
         const bool there = page >= 0;
         const size_t at = (size_t)max(page, 0) * c.Hkv + kh;
         const __amdgpu_buffer_rsrc_t rv = make_rsrc((const char *)c.vt + at * SLICE, SLICE);
@@ -297,7 +336,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(Call c) {
         float vsc = 1.f;
         if constexpr (E4M3)
             vsc = c.vs[at * PG + keyg + m];
-        locate(i + 4, &page, &k0);
+        locate_step(i + 1, &page, &k0);
 
         asm volatile("" ::: "memory"); /* Q is read here, not kept */
         floatx4 x[NKB];
@@ -387,60 +426,42 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(Call c) {
             }
         }
     }
-    /* the gates of the rows this wave finishes (wave, wave + 4, ..) are on their way
-     * while the waves merge */
-    const bool whole = nshare == 1, gated = whole && c.gate;
-    bf16x4 gv[FEW / 4];
-#pragma unroll
-    for (int i = 0; i < FEW / 4; i++) {
-        const int r = min(wave + 4 * i, rows - 1);
-        if (gated && wave + 4 * i < rows)
-            gv[i] = *(const bf16x4 *)(c.gate + (size_t)(s.q0 + r / c.G) * c.gts +
-                                      (size_t)(kh * c.G + r % c.G) * c.ghs + 4 * lane);
-    }
     lrun += __shfl_xor(lrun, 16, 64);
     lrun += __shfl_xor(lrun, 32, 64);
 
-    lds_barrier(); /* Q is read */
-    /* merge the waves; lane (m, g) holds dims 16 t + 4 g .. + 3 of row m */
+    /* lane (m, g) holds dims 16 t + 4 g .. + 3 of row m. Where that goes is
+     * worked out again: kept over the loop it cost registers. */
+    int r = m;
+    asm volatile("" : "+v"(r));
+    if (w.parts > 1) {
+        const size_t slot = slot_of(c, kh, w.first + w.part);
+        if (r < rows) {
 #pragma unroll
-    for (int t = 0; t < 16; t++)
-        *(floatx4 *)&so[wave][m][16 * t + 4 * g] = o[t];
-    if (g == 0)
-        sl[wave][m] = lrun, sm[wave][m] = mrun;
-    lds_barrier();
-    const size_t slot = slot_of(c, kh, w.slot0 + w.share);
-#pragma unroll
-    for (int i = 0; i < FEW / 4; i++) {
-        const int r = wave + 4 * i;
-        if (r >= rows)
-            break;
-        float ref = -INFINITY;
-#pragma unroll
-        for (int v = 0; v < 4; v++)
-            ref = fmaxf(ref, sm[v][r]);
-        const float mu = ref == -INFINITY ? 0.f : ref;
-        floatx4 acc = {};
-        float l = 0.f;
-#pragma unroll
-        for (int v = 0; v < 4; v++) {
-            const float a = fast_exp2(sm[v][r] - mu);
-            acc += *(const floatx4 *)&so[v][r][4 * lane] * a;
-            l += sl[v][r] * a;
+            for (int t = 0; t < 16; t++)
+                *(floatx4 *)(c.po + (slot * FEW + r) * PD + 16 * t + 4 * g) = o[t];
+            if (g == 0) {
+                c.pl[slot * FEW + r] = lrun;
+                c.pmu[slot * FEW + r] = mrun == -INFINITY ? 0.f : mrun;
+            }
         }
-        if (!whole) {
-            *(floatx4 *)(c.po + (slot * FEW + r) * PD + 4 * lane) = acc;
-            if (lane == 0)
-                c.pl[slot * FEW + r] = l, c.pmu[slot * FEW + r] = mu;
-            continue;
-        }
+    } else if (r < rows) {
+        const float inv = lrun > 0.f ? 1.f / lrun : 0.f;
         const int n = s.q0 + r / c.G, hd = kh * c.G + r % c.G;
-        const float inv = l > 0.f ? 1.f / l : 0.f;
-        bf16x4 res;
+        bf16x4 gv[16];
+        if (c.gate) {
+            const bf16 *gp = c.gate + (size_t)n * c.gts + (size_t)hd * c.ghs + 4 * g;
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            res[e] = f2bf(acc[e] * inv * (gated ? sigmoid_f(bf2f(gv[i][e])) : 1.f));
-        *(bf16x4 *)(c.out + ((size_t)n * c.Hq + hd) * PD + 4 * lane) = res;
+            for (int t = 0; t < 16; t++)
+                gv[t] = *(const bf16x4 *)(gp + 16 * t);
+        }
+#pragma unroll
+        for (int t = 0; t < 16; t++) {
+            bf16x4 res;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                res[e] = f2bf(o[t][e] * inv * (c.gate ? sigmoid_f(bf2f(gv[t][e])) : 1.f));
+            *(bf16x4 *)(c.out + ((size_t)n * c.Hq + hd) * PD + 16 * t + 4 * g) = res;
+        }
     }
 }
 
@@ -511,17 +532,17 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
     }
     if (at >= c.plan.shares)
         return;
-    const Where w = locate<true>(c, c.plan.shares - 1 - at);
+    const Where w = locate<RT, PG, true>(c, c.plan.shares - 1 - at);
     if (w.b < 0)
         return;
     const pg_seq s = w.s;
-    const int b = w.b, nshare = w.nshare;
+    const int b = w.b, nshare = w.parts, share = w.part;
     const int r0 = w.unit * RT, nrows = min(s.ql * c.G - r0, RT);
     const int i0 = r0 / c.G, i1 = (r0 + nrows - 1) / c.G;
     const pg_tiles list = pg_tile_list(s, i0, i1, c.window, c.sinks);
-    const int tb = pg_share_begin(list.ntl, w.share, nshare);
-    const int ntl = pg_share_begin(list.ntl, w.share + 1, nshare) - tb;
-    const size_t slot = slot_of(c, kh, w.slot0 + w.share);
+    const int tb = pg_share_begin(list.ntl, share, nshare);
+    const int ntl = pg_share_begin(list.ntl, share + 1, nshare) - tb;
+    const size_t slot = slot_of(c, kh, w.first + share);
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int wi = wave & 3, wj = wave >> 2, h = lane >> 5, col = lane & 31;
@@ -1024,61 +1045,89 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
     }
 }
 
-/* ---- merge of a unit's shares ----------------------------------------------------
- * One wave per row: o = sum_s 2^(mu_s - mu) o_s over the shares that saw keys,
- * l likewise, mu the largest of theirs; then / l and the gate. l and mu of all
- * shares come in one load (lane i: share i), o eight shares at a time. */
-template <int ROWS>
+/* ---- merge of a unit's parts -----------------------------------------------------
+ * One workgroup per row of few rows (its 4 waves a quarter of the parts each, joined
+ * through LDS), or per 16 rows of many (4 of a wave in turn): o = sum 2^(mu_i - mu)
+ * o_i over the parts that saw keys, l likewise, mu the largest of theirs; then / l
+ * and the gate. l and mu come in one load (lane i: part i), o eight parts at a
+ * time. */
+template <int ROWS, int KS>
 __global__ __launch_bounds__(256) void merge_kernel(Call c, int groups) {
+    constexpr bool FEWR = ROWS == FEW;
+    __shared__ __attribute__((aligned(16))) float so[FEWR ? 4 : 1][PD];
+    __shared__ float sl[4], sm[4];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int t = blockIdx.x % groups * 4 + wave, kh = blockIdx.x / groups % c.Hkv;
-    const Where w = locate<false>(c, blockIdx.x / groups / c.Hkv);
-    if (w.b < 0 || w.nshare <= 1)
+    const int group = blockIdx.x % groups, kh = blockIdx.x / groups % c.Hkv;
+    const Where w = locate<ROWS, KS, false>(c, blockIdx.x / groups / c.Hkv);
+    if (w.b < 0 || w.parts <= 1)
         return;
-    const int r = w.unit * ROWS + t;
-    if (t >= ROWS || r >= w.s.ql * c.G)
-        return;
-    const size_t first = slot_of(c, kh, w.slot0) * ROWS + t;
-    const int n = w.s.q0 + r / c.G, head = kh * c.G + r % c.G;
-    bf16x4 gv = {};
-    if (c.gate)
-        gv = *(const bf16x4 *)(c.gate + (size_t)n * c.gts + (size_t)head * c.ghs + 4 * lane);
-    float mu = -INFINITY, l = 0.f;
-    floatx4 acc = {};
-    for (int i0 = 0; i0 < w.nshare; i0 += 64) { /* more than 64 shares: in turns */
-        const int cnt = min(w.nshare - i0, 64);
-        const size_t mine = first + (size_t)(i0 + min(lane, cnt - 1)) * ROWS;
-        const float li = lane < cnt ? c.pl[mine] : 0.f;
-        const float mi = li > 0.f ? c.pmu[mine] : -INFINITY;
-        const float next = fmaxf(mu, wave_max(mi));
-        const float ref = next == -INFINITY ? 0.f : next, old = fast_exp2(mu - ref);
-        const float wi = li > 0.f ? fast_exp2(mi - ref) : 0.f;
-        mu = next;
-        l = l * old + wave_sum(wi * li);
-        acc *= old;
-        for (int j0 = 0; j0 < cnt; j0 += 8) {
-            floatx4 v[8];
+    const int parts = w.parts;
+    const size_t slot = slot_of(c, kh, w.first);
+    const int nrows = min(w.s.ql * c.G - w.unit * ROWS, ROWS);
+    for (int i = 0; i < (FEWR ? 1 : 4); i++) {
+        const int t = FEWR ? group : 16 * group + 4 * wave + i;
+        if (t >= nrows)
+            return;
+        const int r = w.unit * ROWS + t, n = w.s.q0 + r / c.G, head = kh * c.G + r % c.G;
+        bf16x4 gv = {};
+        if (c.gate)
+            gv = *(const bf16x4 *)(c.gate + (size_t)n * c.gts + (size_t)head * c.ghs + 4 * lane);
+        const size_t first = slot * ROWS + t;
+        const int q0 = FEWR ? parts * wave / 4 : 0, q1 = FEWR ? parts * (wave + 1) / 4 : parts;
+        float mu = -INFINITY, l = 0.f;
+        floatx4 acc = {};
+        for (int j0 = q0; j0 < q1; j0 += 64) { /* more than 64 parts: in turns */
+            const int cnt = min(q1 - j0, 64);
+            const size_t mine = first + (size_t)(j0 + min(lane, cnt - 1)) * ROWS;
+            const float pl = c.pl[mine], pm = c.pmu[mine];
+            const float li = lane < cnt ? pl : 0.f, mi = li > 0.f ? pm : -INFINITY;
+            const float next = fmaxf(mu, wave_max(mi));
+            const float ref = next == -INFINITY ? 0.f : next, old = fast_exp2(mu - ref);
+            const float wi = li > 0.f ? fast_exp2(mi - ref) : 0.f;
+            mu = next;
+            l = l * old + wave_sum(wi * li);
+            acc *= old;
+            for (int k0 = 0; k0 < cnt; k0 += 8) {
+                floatx4 v[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                v[j] = *(const floatx4 *)(c.po +
-                                          (first + (size_t)(i0 + min(j0 + j, cnt - 1)) * ROWS) * PD +
-                                          4 * lane);
+                for (int k = 0; k < 8; k++)
+                    v[k] = *(const floatx4 *)(c.po +
+                                              (first + (size_t)(j0 + min(k0 + k, cnt - 1)) * ROWS) *
+                                                  PD +
+                                              4 * lane);
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float f = __uint_as_float((uint32_t)__builtin_amdgcn_readlane(
-                    (int)__float_as_uint(wi), min(j0 + j, 63)));
-                /* a share without keys wrote no o */
-                if (j0 + j < cnt && f > 0.f)
-                    acc += v[j] * f;
+                for (int k = 0; k < 8; k++) {
+                    const float f = __uint_as_float((uint32_t)__builtin_amdgcn_readlane(
+                        (int)__float_as_uint(wi), min(k0 + k, 63)));
+                    if (k0 + k < cnt && f > 0.f)
+                        acc += v[k] * f;
+                }
             }
         }
-    }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    bf16x4 res;
+        if constexpr (FEWR) {
+            *(floatx4 *)&so[wave][4 * lane] = acc;
+            if (lane == 0)
+                sl[wave] = l, sm[wave] = mu;
+            lds_barrier();
+            if (wave > 0)
+                return;
+            const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+            const float ref = top == -INFINITY ? 0.f : top;
+            acc = floatx4{}, l = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; e++)
-        res[e] = f2bf(acc[e] * inv * (c.gate ? sigmoid_f(bf2f(gv[e])) : 1.f));
-    *(bf16x4 *)(c.out + ((size_t)n * c.Hq + head) * PD + 4 * lane) = res;
+            for (int v = 0; v < 4; v++) {
+                const float f = fast_exp2(sm[v] - ref);
+                acc += *(const floatx4 *)&so[v][4 * lane] * f;
+                l += sl[v] * f;
+            }
+        }
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        bf16x4 res;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            res[e] = f2bf(acc[e] * inv * (c.gate ? sigmoid_f(bf2f(gv[e])) : 1.f));
+        *(bf16x4 *)(c.out + ((size_t)n * c.Hq + head) * PD + 4 * lane) = res;
+    }
 }
 
 } // namespace
@@ -1116,23 +1165,24 @@ extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int
                     (float *)ws, (float *)ws + rows * PD, (float *)ws + rows * (PD + 1), p};
     const bool few = p.rt == FEW;
     const int per = !few && 8 % Hkv == 0 ? 8 / Hkv : 1;
-    const dim3 grid((unsigned)(pg_div_up(p.shares, per) * per * Hkv));
+    const dim3 grid((unsigned)(pg_div_up(p.shares, per) * per * Hkv)); /* all parts */
     if (few && e4m3)
-        hipLaunchKernelGGL(attention_few_kernel<true>, grid, dim3(256), 0, stream, c);
+        hipLaunchKernelGGL(attention_few_kernel<true>, grid, dim3(64), 0, stream, c);
     else if (few)
-        hipLaunchKernelGGL(attention_few_kernel<false>, grid, dim3(256), 0, stream, c);
+        hipLaunchKernelGGL(attention_few_kernel<false>, grid, dim3(64), 0, stream, c);
     else if (e4m3)
         hipLaunchKernelGGL(attention_many_kernel<true>, grid, dim3(512), 0, stream, c);
     else
         hipLaunchKernelGGL(attention_many_kernel<false>, grid, dim3(512), 0, stream, c);
     if (p.slots > 0) {
-        const long long rows_most = (long long)pg_min(max_q, N) * G;
-        const int groups = pg_div_up(rows_most < p.rt ? (int)rows_most : p.rt, 4);
+        const int groups = few ? pg_min(max_q, N) * G : RT / 16;
         const dim3 mgrid((unsigned)(p.units * Hkv * groups));
-        if (few)
-            hipLaunchKernelGGL(merge_kernel<FEW>, mgrid, dim3(256), 0, stream, c, groups);
+        if (few && e4m3)
+            hipLaunchKernelGGL((merge_kernel<FEW, 64>), mgrid, dim3(256), 0, stream, c, groups);
+        else if (few)
+            hipLaunchKernelGGL((merge_kernel<FEW, 32>), mgrid, dim3(256), 0, stream, c, groups);
         else
-            hipLaunchKernelGGL(merge_kernel<RT>, mgrid, dim3(256), 0, stream, c, groups);
+            hipLaunchKernelGGL((merge_kernel<RT, PG>), mgrid, dim3(256), 0, stream, c, groups);
     }
     return hipGetLastError();
 }

@@ -71,18 +71,23 @@ constexpr int pg_max_tiles(int tok, int max_kv, int window, int sinks) {
 
 /* ---- how the attention's work is shared out ----------------------------------
  * A unit is a tile of rt packed rows (token, q-head of the group) of a sequence and
- * kv-head; a share is a part of a unit's key tiles. rt is PG_FEW where no sequence
- * of the call has more rows than that (one unit each), PG_MANY otherwise. */
+ * kv-head. rt is PG_FEW where no sequence of the call has more rows than that (one
+ * unit each), PG_MANY otherwise.
+ *
+ * PG_FEW: the units' steps, one after the other, are a line that pieces of equal
+ * size cut; what lies in one piece of one unit is a part, a wave's work.
+ * PG_MANY: a unit's key tiles are cut into as many even shares as the plan asks
+ * for, a workgroup each. Parts of a unit of several leave theirs in slots. */
 constexpr int PG_FEW = 16, PG_MANY = 128;
-constexpr int PG_FEW_SHARE = 64; /* key tiles a share of PG_FEW rows, at most */
+constexpr int PG_FEW_PARTS = 128; /* parts of a unit of few rows, about, at most */
 
 struct pg_plan {
     int rt;
     int units;  /* units of a kv-head, at most */
-    int shares; /* shares of a kv-head, at most (workgroups; 0: no work, -1: too many) */
-    int slots;  /* of those, at most, with partial results to merge (0: no merge) */
-    int goal;   /* workgroups of a kv-head that the chip runs at once; 0: do not share out */
-    int least;  /* key tiles a share, at least */
+    int shares; /* parts of a kv-head's units, at most (0: no work, -1: too many) */
+    int slots;  /* of these, at most, with something to merge (0: no merge) */
+    int goal;   /* waves (PG_FEW) or workgroups of a kv-head that the chip runs at
+                 * once; 0 (PG_MANY): whole units fill it */
 };
 
 constexpr int pg_units(const pg_seq &s, int G, int rt) {
@@ -98,15 +103,24 @@ constexpr int pg_longest(const pg_seq &s, int G, int rt, int window, int sinks) 
         pg_tile_list(s, (int)((long long)(units - 1) * rt / G), s.ql - 1, window, sinks);
     return pg_max(t.ntl, 1);
 }
-/* Key tiles a share should have, for U units of a kv-head with T tiles in all. A
+/* PG_FEW: steps a piece, for a line of T with `most` in its longest unit */
+constexpr int pg_few_share(const pg_plan &p, unsigned T, int most) {
+    const unsigned n = (unsigned)p.goal;
+    return pg_max(pg_max((int)(T / n + (T % n != 0)), pg_div_up(most, PG_FEW_PARTS)), 1);
+}
+/* PG_FEW: number of the part of unit u (counted over the kv-head) in a piece: rises
+ * along the line, and a unit's parts have consecutive ones */
+constexpr int pg_few_slot(int piece, int u) { return piece + u; }
+
+/* PG_MANY: key tiles a share should have, for U units with T tiles in all. A
  * sequence's last share is half empty on average: as many workgroups fewer to
  * count on. */
+constexpr int PG_MANY_LEAST = 16;
 constexpr int pg_share(const pg_plan &p, int U, unsigned T) {
-    const int cap = p.rt == PG_FEW ? PG_FEW_SHARE : PG_MOST;
     if (p.goal == 0 || U >= p.goal)
-        return cap;
+        return PG_MOST;
     const unsigned n = (unsigned)pg_max(p.goal - U / 2, U);
-    return pg_min(pg_max((int)(T / n + (T % n != 0)), p.least), cap);
+    return pg_max((int)(T / n + (T % n != 0)), PG_MANY_LEAST);
 }
 constexpr int pg_nshare(int tiles, int share) { return pg_max(pg_div_up(tiles, share), 1); }
 /* First list entry of share i of n even ones */
@@ -119,30 +133,32 @@ constexpr pg_plan pg_make_plan(int N, int B, int max_q, int max_kv, int G, int H
     p.rt = mq * G <= PG_FEW ? PG_FEW : PG_MANY;
     if (mq <= 0 || B <= 0)
         return p;
-    long long units = B;
-    if (p.rt == PG_MANY) {
-        const long long by_rows = (long long)N * G / PG_MANY + B;
-        const long long by_len = B * ((mq * G + PG_MANY - 1) / PG_MANY);
-        units = by_rows < by_len ? by_rows : by_len;
-    }
     if (window >= max_kv)
         window = sinks = 0;
     const int tok = p.rt == PG_FEW ? (int)mq : PG_MANY / G + 2;
-    const int most = pg_max(pg_max_tiles(tok, max_kv, window, sinks), 1);
-    const bool few = p.rt == PG_FEW;
-    p.goal = pg_max((few ? 512 : 256) / Hkv, 1);
-    p.least = few ? (e4m3 ? 4 : 2) : 8;
-    /* the rows that the caller brings fill the chip: whole units */
-    if (few ? units >= p.goal : (long long)N * G / PG_MANY >= p.goal)
-        p.goal = 0;
-    /* sum over units of max(ceil(t / share), 1), with share = ceil(T / n) at least: n
-     * + units, n <= max(goal, units) */
-    long long shares = units;
-    if (p.goal > 0 && most > p.least)
-        shares = units < p.goal ? p.goal + units : units < 2ll * p.goal ? 2ll * p.goal : units;
-    if (few && most > PG_FEW_SHARE) {
-        const long long capped = units * pg_div_up(most, PG_FEW_SHARE);
-        shares = shares < capped ? capped : shares;
+    const long long most = pg_max(pg_max_tiles(tok, max_kv, window, sinks), 1);
+    long long units = B, shares = 0, slots = 0;
+    if (p.rt == PG_FEW) {
+        const long long steps = most * (e4m3 ? 1 : 2);
+        p.goal = pg_max(2048 / Hkv, 1);
+        /* a line of at most units * steps, which are ints, in pieces of at least a
+         * step; the last part's number is below pieces + units */
+        const long long line = units * steps;
+        shares = line > 0x7fffffff ? PG_MOST : (line < p.goal ? line : p.goal) + units;
+        slots = steps > 1 ? shares : 0;
+    } else {
+        const long long by_rows = (long long)N * G / PG_MANY + B;
+        const long long by_len = B * ((mq * G + PG_MANY - 1) / PG_MANY);
+        units = by_rows < by_len ? by_rows : by_len;
+        /* the rows that the caller brings fill the chip: whole units */
+        p.goal = pg_max(256 / Hkv, 1);
+        if ((long long)N * G / PG_MANY >= p.goal)
+            p.goal = 0;
+        /* sum over units of max(ceil(t / share), 1), share at least T / n, n <= goal,
+         * fewer than goal units: below goal + units; goal units or more: whole */
+        const bool split = p.goal > 0 && most > PG_MANY_LEAST;
+        shares = !split ? units : units < p.goal ? p.goal + units : units < 2ll * p.goal ? 2ll * p.goal : units;
+        slots = split ? shares : 0;
     }
     if (units * Hkv > 1 << 22 || shares * Hkv > 1 << 22) {
         p.shares = -1;
@@ -150,8 +166,7 @@ constexpr pg_plan pg_make_plan(int N, int B, int max_q, int max_kv, int G, int H
     }
     p.units = (int)units;
     p.shares = (int)shares;
-    const bool split = p.goal > 0 ? most > p.least : few && most > PG_FEW_SHARE;
-    p.slots = split ? (int)shares : 0;
+    p.slots = (int)slots;
     return p;
 }
 

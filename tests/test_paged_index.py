@@ -117,18 +117,37 @@ int main() {
         const pg_plan p = pg_make_plan(N, B, max_q, max_kv, G, Hkv, w, S, e4m3);
         const int W = w >= max_kv ? 0 : w, SS = W ? S : 0;
         long long U = 0, T = 0, C = 0;
-        int at = 0;
+        int at = 0, most = 0, KS = e4m3 ? 64 : 32;
         std::vector<pg_seq> seqs;
         for (int b = 0; b < B; b++) {
             seqs.push_back(pg_clean_seq(at, at + q[b], kv[b], N, max_q, max_kv));
             at += q[b];
             const int u = max_q ? pg_units(seqs[b], G, p.rt) : 0;
-            U += u, T += (long long)u * pg_longest(seqs[b], G, p.rt, W, SS);
+            const int n = pg_longest(seqs[b], G, p.rt, W, SS) * (p.rt == 16 ? PG / KS : 1);
+            U += u, T += (long long)u * n, most = pg_max(most, u ? n : 0);
         }
         if (max_q == 0) { NEED(p.shares == 0); continue; }
         NEED(p.rt == (max_q * G <= 16 ? 16 : 128) && U <= p.units);
+        if (p.rt == 16) {
+            if (U == 0) continue;
+            const int size = pg_few_share(p, (unsigned)T, most);
+            int line = 0, u = 0, last = -1;
+            for (int b = 0; b < B; b++) {
+                if (pg_units(seqs[b], G, 16) == 0) continue;
+                NEED(pg_units(seqs[b], G, 16) == 1);
+                const int n = pg_longest(seqs[b], G, 16, W, SS) * (PG / KS);
+                const pg_tiles t = pg_tile_list(seqs[b], 0, seqs[b].ql - 1, W, SS);
+                NEED(t.ntl * (PG / KS) == n || t.ntl == 0);
+                const int p0 = line / size, p1 = (line + n - 1) / size;
+                NEED(p1 - p0 + 1 <= PG_FEW_PARTS + 1);
+                NEED(pg_few_slot(p0, u) > last && pg_few_slot(p1, u) < p.shares);
+                NEED(p0 == p1 || pg_few_slot(p1, u) < p.slots);
+                last = pg_few_slot(p1, u);
+                line += n, u++;
+            }
+            continue;
+        }
         const int share = pg_share(p, (int)U, (unsigned)T);
-        NEED(p.rt == 128 || share <= 64);
         for (int b = 0; b < B; b++) {
             const int u = pg_units(seqs[b], G, p.rt), n = pg_nshare(pg_longest(seqs[b], G, p.rt, W, SS), share);
             C += (long long)u * n;
@@ -138,21 +157,23 @@ int main() {
                 NEED(rows > 0);
                 const pg_tiles t = pg_tile_list(seqs[b], r0 / G, (r0 + rows - 1) / G, W, SS);
                 NEED(pg_share_begin(t.ntl, 0, n) == 0 && pg_share_begin(t.ntl, n, n) == t.ntl);
-                for (int i = 0; i < n && i < 70; i++) {
-                    const int len = pg_share_begin(t.ntl, i + 1, n) - pg_share_begin(t.ntl, i, n);
-                    NEED(len >= 0 && (p.rt == 128 || len <= 64));
-                }
+                for (int i = 0; i < n && i < 70; i++)
+                    NEED(pg_share_begin(t.ntl, i + 1, n) >= pg_share_begin(t.ntl, i, n));
             }
         }
         NEED(C <= p.shares && (p.slots == 0 || p.slots >= C));
     }
-    {   /* the largest call: nothing overflows */
-        const pg_plan p = pg_make_plan(PG_MOST, 1, PG_MOST, PG_MOST_KEYS, 16, 1, 0, 0, true);
-        NEED(p.shares == -1);
-        const pg_plan f = pg_make_plan(60, 60, 1, PG_MOST_KEYS, 16, 1, 0, 0, true);
-        const pg_seq s = pg_clean_seq(0, 1, PG_MOST_KEYS, 60, 1, PG_MOST_KEYS);
-        const int share = pg_share(f, 60, 60u * (unsigned)pg_longest(s, 16, 16, 0, 0));
-        NEED(share == 64 && 60ll * pg_nshare(pg_longest(s, 16, 16, 0, 0), share) <= f.shares);
+    {   /* the largest calls: nothing overflows */
+        NEED(pg_make_plan(PG_MOST, 1, PG_MOST, PG_MOST_KEYS, 16, 1, 0, 0, true).shares == -1);
+        NEED(pg_make_plan(PG_MOST, PG_MOST, 1, PG_MOST_KEYS, 16, 1, 0, 0, true).shares == -1);
+        for (int e = 0; e < 2; e++) {
+            const pg_plan f = pg_make_plan(60, 60, 1, PG_MOST_KEYS, 16, 1, 0, 0, e);
+            const pg_seq s = pg_clean_seq(0, 1, PG_MOST_KEYS, 60, 1, PG_MOST_KEYS);
+            const int n = pg_longest(s, 16, 16, 0, 0) * (e ? 1 : 2);
+            const int size = pg_few_share(f, 60u * (unsigned)n, n);
+            NEED(f.shares > 0 && pg_few_slot((int)((60ll * n - 1) / size), 59) < f.shares);
+            NEED((f.shares + 1ll) * size < 0x7fffffff); /* where a piece ends */
+        }
     }
     printf("bad %d\n", bad);
     return bad != 0;
