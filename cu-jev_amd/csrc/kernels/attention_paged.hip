@@ -106,6 +106,7 @@ struct Call {
     int num_pages;
     const int32_t *q_start, *kv_len, *page_table;
     int max_pages, B, N, max_q, max_kv, Hq, Hkv, G, window, sinks;
+    int rG; /* r / G = r * rG >> 8 for r < 16: a division kept a register and more */
     bf16 *out;
     float *po, *pl, *pmu;
     pg_plan plan;
@@ -118,40 +119,53 @@ DEV int page_id(const Call &c, int b, const pg_tiles &t, int i) {
     return page >= 0 && page < c.num_pages ? page : -1;
 }
 
-DEV int wave_sum_i(int v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
-        v += __shfl_xor(v, o, 64);
-    return __builtin_amdgcn_readfirstlane(v); /* uniform, for the compiler too */
+/* f over the lanes with the same number in each of the wave's four rows of 16 */
+template <class F> DEV float fold_rows(float x, F f) {
+    const uint32_t u = __float_as_uint(x);
+    auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t v = __float_as_uint(f(__uint_as_float(a[0]), __uint_as_float(a[1])));
+    a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return f(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
+/* Inclusive sum over the lanes below: 6 DPP adds (through LDS they took 6 trips) */
+template <int ctrl, int rows> DEV int dpp_or_0(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, ctrl, rows, 0xf, true);
+}
+DEV int wave_scan(int v) {
+    v += dpp_or_0<0x111, 0xf>(v); /* row_shr 1, 2, 4, 8 */
+    v += dpp_or_0<0x112, 0xf>(v);
+    v += dpp_or_0<0x114, 0xf>(v);
+    v += dpp_or_0<0x118, 0xf>(v);
+    v += dpp_or_0<0x142, 0xa>(v); /* row_bcast 15, 31 */
+    v += dpp_or_0<0x143, 0xc>(v);
+    return v;
+}
+DEV int last_lane(int v) { return __builtin_amdgcn_readlane(v, 63); }
+
 /* The unit that part `target` of a kv-head belongs to (BY_PART), or unit `target`:
  * its sequence (b -1: there is none), its number in it, its parts, the first
  * one's number, which of them `target` is. With few rows the parts are those of
  * the pieces of the line (numbered by pg_few_slot), and begin .. begin + own the
- * unit's steps on it, with many rows the unit's shares. */
+ * unit's tiles on it, with many rows the unit's shares. */
 struct Where {
     pg_seq s;
     int b, unit, parts, first, part;
-    int begin, own, size; /* few rows: the unit on the line, steps a piece */
+    int begin, own, size; /* few rows: the unit on the line, tiles a piece */
 };
-template <int RT_, int KS, bool BY_PART> DEV Where locate(const Call &c, int target) {
+template <int RT_, bool BY_PART> DEV Where locate(const Call &c, int target) {
     constexpr bool FEWR = RT_ == PG_FEW;
     const int lane = threadIdx.x & 63;
     Where w;
     w.b = -1, w.begin = w.own = w.size = 0;
-    /* a sequence's units, and what each has: steps of KS keys, or key tiles */
     auto units_of = [&](const pg_seq &s) { return pg_units(s, c.G, RT_); };
-    auto each = [&](const pg_seq &s) {
-        const int tiles = pg_longest(s, c.G, RT_, c.window, c.sinks);
-        return FEWR ? tiles * (PG / KS) : tiles;
-    };
+    auto each = [&](const pg_seq &s) { return pg_longest(s, c.G, RT_, c.window, c.sinks); };
     if (c.B == 1) { /* no scan for one sequence */
         w.s = seq_of(c, 0);
         const int units = units_of(w.s), n = each(w.s);
         if (units == 0)
             return w;
         if constexpr (FEWR) {
-            w.size = pg_few_share(c.plan, (unsigned)n, n);
+            w.size = pg_few_share(c.plan, (unsigned)n);
             w.own = n;
             w.parts = (n - 1) / w.size + 1;
         } else {
@@ -163,46 +177,37 @@ template <int RT_, int KS, bool BY_PART> DEV Where locate(const Call &c, int tar
         w.b = w.unit < units ? 0 : -1;
         return w;
     }
-    int U = 0, most = 0;
+    /* 64 sequences at a time, one a lane: what all have, then where target lies.
+     * Up to 64 are read once. */
+    pg_seq s;
+    int units = 0, n = 0;
+    auto read = [&](int b0) {
+        s = seq_of(c, min(b0 + lane, c.B - 1));
+        units = b0 + lane < c.B ? units_of(s) : 0;
+        n = units ? each(s) : 0;
+    };
+    int U = 0;
     unsigned T = 0;
     for (int b0 = 0; b0 < c.B; b0 += 64) {
-        const pg_seq s = seq_of(c, min(b0 + lane, c.B - 1));
-        const int units = b0 + lane < c.B ? units_of(s) : 0, n = units ? each(s) : 0;
-        U += units;
-        T += (unsigned)units * (unsigned)n;
-        most = max(most, n);
+        read(b0);
+        T += (unsigned)last_lane(wave_scan((int)((unsigned)units * (unsigned)n)));
+        if constexpr (!FEWR)
+            U += last_lane(wave_scan(units));
     }
-    T = (unsigned)wave_sum_i((int)T);
-    int size;
-    if constexpr (FEWR) {
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1)
-            most = max(most, __shfl_xor(most, o, 64));
-        size = pg_few_share(c.plan, T, __builtin_amdgcn_readfirstlane(most));
-    } else {
-        size = pg_share(c.plan, wave_sum_i(U), T);
-    }
+    const int size = FEWR ? pg_few_share(c.plan, T) : pg_share(c.plan, U, T);
     int before_u = 0, before_n = 0;
     for (int b0 = 0; b0 < c.B; b0 += 64) {
-        const pg_seq s = seq_of(c, min(b0 + lane, c.B - 1));
-        const int units = b0 + lane < c.B ? units_of(s) : 0, n = each(s);
+        if (c.B > 64)
+            read(b0);
         const int parts = FEWR ? 0 : pg_nshare(n, size);
-        const int all = units * (FEWR ? n : parts);
-        int su = units, sn = all; /* inclusive sums over the lanes */
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int x = __shfl_up(su, o, 64), y = __shfl_up(sn, o, 64);
-            su += lane >= o ? x : 0;
-            sn += lane >= o ? y : 0;
-        }
-        su += before_u, sn += before_n;
-        const int u = su - units, a = sn - all; /* before this lane's sequence */
+        const int su = before_u + wave_scan(units);
+        const int sn = before_n + wave_scan(units * (FEWR ? n : parts));
+        const int u = su - units, a = sn - units * (FEWR ? n : parts); /* before the lane's */
         /* few rows: one unit, its parts are pieces p0 .. p1 */
         const int p0 = FEWR ? a / size : 0, p1 = FEWR ? (sn - 1) / size : 0;
-        const bool mine = !BY_PART ? su > target
-                          : FEWR   ? units > 0 && pg_few_slot(p1, u) >= target
-                                   : sn > target;
-        const uint64_t past = __ballot(mine);
+        const uint64_t past = __ballot(!BY_PART ? su > target
+                                       : FEWR   ? units > 0 && pg_few_slot(p1, u) >= target
+                                                : sn > target);
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
             auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
@@ -223,8 +228,8 @@ template <int RT_, int KS, bool BY_PART> DEV Where locate(const Call &c, int tar
             }
             return w;
         }
-        before_u = __builtin_amdgcn_readlane(su, 63);
-        before_n = __builtin_amdgcn_readlane(sn, 63);
+        before_u = last_lane(su);
+        before_n = last_lane(sn);
     }
     return w;
 }
@@ -233,47 +238,45 @@ DEV size_t slot_of(const Call &c, int kh, int at) { return (size_t)kh * c.plan.s
 
 /* ---- few rows: up to 16 packed rows of a sequence and kv-head ------------------
  * Bound by the K/V bytes, so that what counts is that every wave of the chip
- * streams all the time. The steps of all units of a kv-head (32 keys of bf16, a
- * tile of 64 of e4m3: 32 KiB of K and V) are one line, cut into equal pieces; a wave
- * takes a piece, or the part of it that lies in one unit, and waits for no other. K and V^T go from memory into registers as the operands of
- * v_mfma_f32_16x16x32_bf16, 16 loads each of 16 bytes a lane (64 bytes of 16
- * rows): K of the next step is in flight during the softmax and the PV products,
- * V^T during the scores. All loads are unconditional (past the end the last
- * step's again), so a wait for one operand's counts the other's in flight and not
- * more; in 256 registers two waves share a SIMD. Q waits in LDS: read again each
- * step, it leaves the registers to loads. */
+ * streams all the time. The key tiles of all units of a kv-head are one line, cut
+ * into equal pieces; a wave takes a piece, or the part of it that lies in one unit,
+ * and waits for no other. K and V^T go from memory into registers as the operands
+ * of v_mfma_f32_16x16x32_bf16, 16 bytes a lane and whole 128-byte lines within 16
+ * loads (half a line of V^T at a time, 32 keys of bf16, read each line twice: 157 us
+ * against 126 for 64 sequences of 2560 keys), in two sets of 16 registers' worth:
+ *   e4m3  K of tile i + 1 is in flight during the softmax and the products with
+ *         V^T, V^T during the scores
+ *   bf16  a set holds 32 keys of K, then 128 dims of V^T; each goes out when the
+ *         other's products begin
+ * All loads are unconditional (past the end the last tile's again), so a wait for
+ * one set's counts the other's in flight and not more; in 256 registers two waves
+ * share a SIMD. Q waits in LDS: read again each tile, it leaves the registers to
+ * loads. */
 constexpr int FEW = PG_FEW;
 
 template <bool E4M3>
 __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
-    constexpr int KS = E4M3 ? 64 : 32;        /* keys a step */
-    constexpr int SPT = PG / KS;              /* steps a tile */
-    constexpr int NKB = KS / 16;              /* score blocks */
     constexpr uint32_t EB = E4M3 ? 1 : 2, SLICE = PSLICE * EB;
     __shared__ bf16x8 sq[8 * 64];
     const int kh = blockIdx.x % c.Hkv;
     const int lane = threadIdx.x, m = lane & 15, g = lane >> 4;
-    const Where w = locate<FEW, KS, true>(c, blockIdx.x / c.Hkv);
+    const Where w = locate<FEW, true>(c, blockIdx.x / c.Hkv);
     if (w.b < 0)
         return;
     const pg_seq s = w.s;
     const int b = w.b, rows = min(s.ql * c.G, FEW);
     const pg_tiles list = pg_tile_list(s, 0, s.ql - 1, c.window, c.sinks);
-    /* steps [i0, i1) of the unit; a unit without a key has some that see none */
+    /* tiles [i0, i1) of the unit's; a unit without a key has one that is not there */
     const int cut = (w.begin / w.size + w.part) * w.size - w.begin;
-    const int i0 = max(cut, 0), i1 = min(cut + w.size, w.own);
-    const int steps = min(i1, list.ntl * SPT);
-    bf16x8 *const qf = sq + lane;
-    /* Row m of score block kb is key key0 + 4 kb of the step: lane g then holds,
-     * in accumulators 4 kb .. + 3, the keys (KS / 4) g .. that its V^T loads
-     * bring. */
-    const int key0 = KS / 4 * (m >> 2) + (m & 3), keyg = KS / 4 * g;
-    const uint32_t kvoff = key0 * PD * EB + 16 * g, vvoff = m * PG * EB + 16 * g;
+    const int i0 = max(cut, 0), i1 = min(min(cut + w.size, w.own), list.ntl);
+    /* the ids of 64 tiles of the list are in a lane each */
+    int ids = i0 < i1 ? page_id(c, b, list, min(i0 + lane, list.ntl - 1)) : -1, ids0 = i0;
 
     /* this lane's row (column of S^T and O^T) */
-    const int row = min(m, rows - 1), tok = row / c.G, head = kh * c.G + row % c.G;
+    const int row = min(m, rows - 1), tok = row * c.rG >> 8, head = kh * c.G + row - tok * c.G;
     const int hi = min(s.p0 + tok, s.kv - 1), lo = pg_low(s.p0 + tok, c.window);
     const int own_lo = pg_low(s.p0, c.window); /* of the first row: below, no row's key */
+    bf16x8 *const qf = sq + lane;
     {
         const bf16 *qp = c.q + ((size_t)(s.q0 + tok) * c.Hq + head) * PD;
 #pragma unroll
@@ -282,118 +285,145 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
                                                        : 32 * ks + 8 * g));
     }
 
-    u32x4 kr[16], vr[16];
-    float ksc[4];
-    /* step t (past the last: it again): its page (-1: not there) and first key;
-     * the ids of 64 tiles of the list are in a lane each */
-    int ids = -1, ids0 = -64;
-    auto locate_step = [&](int t, int *page, int *k0) {
-        t = min(t, steps - 1);
-        const int i = t / SPT;
-        if (i - ids0 >= 64) {
-            ids0 = i;
-            ids = page_id(c, b, list, min(i + lane, list.ntl - 1));
-        }
-        *page = __builtin_amdgcn_readlane(ids, i - ids0);
-        *k0 = pg_tile_page(list, i) * PG + t % SPT * KS;
+    /* Row m of score block kb is key key0 + kkey(kb): lane g then holds, in
+     * accumulators v = 4 kb .. + 3, the keys key_of(v) that its V^T loads bring. */
+    const int key0 = (E4M3 ? 16 : 8) * (m >> 2) + (m & 3), keyg = (E4M3 ? 16 : 8) * g;
+    auto kkey = [](int kb) { return E4M3 ? 4 * kb : 4 * (kb & 1) + 32 * (kb >> 1); };
+    auto key_of = [&](int v) { return keyg + (E4M3 ? v : (v & 7) + 32 * (v >> 3)); };
+    const uint32_t kvoff = key0 * PD * EB + 16 * g, vvoff = m * PG * EB + 16 * g;
+
+    u32x4 ra[16], rb[16]; /* e4m3: K, V^T; bf16: the first half of each, the second */
+    float ksc[4], vsc = 1.f;
+    auto rsrc = [&](const void *p, int page) {
+        return make_rsrc((const char *)p + ((size_t)max(page, 0) * c.Hkv + kh) * SLICE, SLICE);
     };
-    auto load_k = [&](int page, int k0) {
-        const size_t at = (size_t)max(page, 0) * c.Hkv + kh;
-        const __amdgpu_buffer_rsrc_t r = make_rsrc((const char *)c.k + at * SLICE, SLICE);
-        const uint32_t half = k0 % PG * PD * EB;
+    auto scale = [&](const float *p, int page, int key) { /* without a 64-bit address a lane */
+        const __amdgpu_buffer_rsrc_t src =
+            make_rsrc(p + ((size_t)max(page, 0) * c.Hkv + kh) * PG, PG * 4);
+        return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(src, key * 4, 0, 0));
+    };
+    /* K: e4m3 all score blocks, bf16 blocks 2 part and 2 part + 1 */
+    auto load_k = [&](u32x4 (&r)[16], int page, int part) {
+        const __amdgpu_buffer_rsrc_t src = rsrc(c.k, page);
 #pragma unroll
-        for (int i = 0; i < 16 / NKB; i++)
+        for (int i = 0; i < (E4M3 ? 4 : 8); i++)
 #pragma unroll
-            for (int kb = 0; kb < NKB; kb++)
-                kr[i * NKB + kb] = buf_load16(r, kvoff, half + 4 * kb * PD * EB + 64 * i);
+            for (int k = 0; k < (E4M3 ? 4 : 2); k++)
+                r[i * (E4M3 ? 4 : 2) + k] =
+                    buf_load16(src, kvoff, kkey((E4M3 ? 0 : 2 * part) + k) * PD * EB + 64 * i);
         if constexpr (E4M3) {
 #pragma unroll
             for (int kb = 0; kb < 4; kb++)
-                ksc[kb] = c.ks[at * PG + key0 + 4 * kb];
+                ksc[kb] = scale(c.ks, page, key0 + 4 * kb);
         }
+    };
+    /* V^T: e4m3 all 16 rows of 16 dims, bf16 8 of them, two halves of 32 keys each */
+    auto load_v = [&](u32x4 (&r)[16], int page, int part) {
+        const __amdgpu_buffer_rsrc_t src = rsrc(c.vt, page);
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            r[i] = E4M3 ? buf_load16(src, vvoff + (i & 1) * 1024, (i >> 1) * 2048)
+                        : buf_load16(src, vvoff + (i & 1) * 64, (8 * part + (i >> 1)) * 2048);
+        if constexpr (E4M3) /* the scale of key keyg + m, in lane m of the 16 that need all 16 */
+            vsc = scale(c.vs, page, keyg + m);
+    };
+    /* tile t (past the last: it again): its page, -1 if it is not there */
+    auto page_of = [&](int t) {
+        t = min(t, i1 - 1);
+        if (t - ids0 >= 64) {
+            ids0 = t;
+            ids = page_id(c, b, list, min(t + lane, list.ntl - 1));
+        }
+        return __builtin_amdgcn_readlane(ids, t - ids0);
     };
 
     floatx4 o[16];
 #pragma unroll
-    for (int i = 0; i < 16; i++)
-        o[i] = floatx4{};
+    for (int t = 0; t < 16; t++)
+        o[t] = floatx4{};
     float mrun = -INFINITY, lrun = 0.f;
-    int page = -1, k0 = 0;
-    if (i0 < steps) {
-        locate_step(i0, &page, &k0);
-        load_k(page, k0);
+    int next = -1;
+    if (i0 < i1) {
+        next = page_of(i0);
+        load_k(ra, next, 0);
+        if constexpr (!E4M3)
+            load_k(rb, next, 1);
     }
-    for (int i = i0; i < steps; i++) {
+    for (int i = i0; i < i1; i++) {
+        const int page = next, k0 = pg_tile_page(list, i) * PG;
         const bool there = page >= 0;
-        const size_t at = (size_t)max(page, 0) * c.Hkv + kh;
-        const __amdgpu_buffer_rsrc_t rv = make_rsrc((const char *)c.vt + at * SLICE, SLICE);
-        const int kc = k0;
-#pragma unroll
-        for (int t = 0; t < 16; t++)
-            vr[t] = buf_load16(rv, vvoff + (t & 1) * 16 * PG * EB,
-                               (t >> 1) * 32 * PG * EB + kc % PG * EB);
-        /* V's scale of key keyg + m, in lane m of the 16 that need all 16 of them */
-        float vsc = 1.f;
         if constexpr (E4M3)
-            vsc = c.vs[at * PG + keyg + m];
-        locate_step(i + 1, &page, &k0);
+            load_v(rb, page, 0);
+        next = page_of(i + 1);
 
         asm volatile("" ::: "memory"); /* Q is read here, not kept */
-        floatx4 x[NKB];
+        floatx4 x[4];
+        if constexpr (E4M3) {
 #pragma unroll
-        for (int i2 = 0; i2 < 16 / NKB; i2++) { /* a K load a block, one or two k-steps */
-#pragma unroll
-            for (int st = 0; st < (E4M3 ? 2 : 1); st++) {
-                const int ks = E4M3 ? 2 * i2 + st : i2;
+            for (int ks = 0; ks < 8; ks++) {
                 const bf16x8 q = qf[64 * ks];
 #pragma unroll
-                for (int kb = 0; kb < NKB; kb++) {
-                    const u32x4 w = kr[i2 * NKB + kb];
-                    bf16x8 a;
-                    if constexpr (E4M3)
-                        a = st ? widen(w[2], w[3], ksc[kb]) : widen(w[0], w[1], ksc[kb]);
-                    else
-                        a = __builtin_bit_cast(bf16x8, w);
+                for (int kb = 0; kb < 4; kb++) {
+                    const u32x4 v = ra[(ks >> 1) * 4 + kb];
                     x[kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                        a, q, ks == 0 ? floatx4{} : x[kb], 0, 0, 0);
+                        ks & 1 ? widen(v[2], v[3], ksc[kb]) : widen(v[0], v[1], ksc[kb]), q,
+                        ks == 0 ? floatx4{} : x[kb], 0, 0, 0);
                 }
             }
+            load_k(ra, next, 0);
+        } else {
+            auto scores = [&](u32x4 (&r)[16], int part) {
+#pragma unroll
+                for (int ks = 0; ks < 8; ks++) {
+                    const bf16x8 q = qf[64 * ks];
+#pragma unroll
+                    for (int k = 0; k < 2; k++)
+                        x[2 * part + k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            __builtin_bit_cast(bf16x8, r[2 * ks + k]), q,
+                            ks == 0 ? floatx4{} : x[2 * part + k], 0, 0, 0);
+                }
+            };
+            scores(ra, 0);
+            load_v(ra, page, 0);
+            scores(rb, 1);
+            load_v(rb, page, 1);
         }
-        load_k(page, k0);
 
-        if (!there || kc + KS - 1 > min(s.p0, s.kv - 1) || c.window > 0) { /* some key hidden */
+        /* bits to keep of V^T values: those of no key of this call, whatever they
+         * are, meet p = 0 */
+        u32x4 keep[E4M3 ? 1 : 2];
+        bool foreign = false;
+        if (!there || k0 + PG - 1 > min(s.p0, s.kv - 1) || c.window > 0) { /* some key hidden */
             const int top = there ? s.kv - 1 : -1;
 #pragma unroll
-            for (int v = 0; v < KS / 4; v++)
+            for (int v = 0; v < 16; v++)
                 x[v >> 2][v & 3] =
-                    hide(key_seen(kc + keyg + v, min(hi, top), lo, c.sinks), x[v >> 2][v & 3]);
-            if (!there || kc + KS > s.kv || kc <= own_lo) {
-                /* values and scales of no key of this call meet p = 0: make them 0 */
-                u32x4 keep;
+                    hide(key_seen(k0 + key_of(v), min(hi, top), lo, c.sinks), x[v >> 2][v & 3]);
+            foreign = !there || pg_tile_foreign(k0, s.p0, s.kv, c.window, c.sinks);
+            if (foreign) {
 #pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    uint32_t k = 0;
+                for (int h = 0; h < (E4M3 ? 1 : 2); h++)
 #pragma unroll
-                    for (int e = 0; e < (E4M3 ? 4 : 2); e++) {
-                        const int j = (E4M3 ? 4 : 2) * w + e;
-                        const bool is = key_seen(kc + keyg + j, top, own_lo, c.sinks);
-                        k |= is ? (E4M3 ? 0xffu << (8 * e) : 0xffffu << (16 * e)) : 0u;
+                    for (int d = 0; d < 4; d++) {
+                        uint32_t k = 0;
+#pragma unroll
+                        for (int e = 0; e < (E4M3 ? 4 : 2); e++) {
+                            const int j = k0 + key_of(E4M3 ? 4 * d + e : 8 * h + 2 * d + e);
+                            k |= key_seen(j, top, own_lo, c.sinks)
+                                     ? (E4M3 ? 0xffu << (8 * e) : 0xffffu << (16 * e))
+                                     : 0u;
+                        }
+                        keep[h][d] = k;
                     }
-                    keep[w] = k;
-                }
                 vsc = __uint_as_float(
-                    key_seen(kc + keyg + m, top, own_lo, c.sinks) ? __float_as_uint(vsc) : 0u);
-#pragma unroll
-                for (int t = 0; t < 16; t++)
-                    vr[t] &= keep;
+                    key_seen(k0 + keyg + m, top, own_lo, c.sinks) ? __float_as_uint(vsc) : 0u);
             }
         }
         float mx = -INFINITY;
 #pragma unroll
-        for (int v = 0; v < KS / 4; v++)
+        for (int v = 0; v < 16; v++)
             mx = fmaxf(mx, x[v >> 2][v & 3]);
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        mx = fold_rows(mx, [](float a, float b) { return fmaxf(a, b); });
         const float mnew = fmaxf(mrun, mx);
         const float ref = mnew == -INFINITY ? 0.f : mnew; /* no key yet: p = 2^-inf = 0 */
         if (__any(mnew != mrun)) {
@@ -404,8 +434,8 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
                 o[t] *= a;
         }
         mrun = mnew;
-        bf16x8 p[NKB / 2];
-        unroll_for<KS / 4>([&](auto iv) {
+        bf16x8 p[2];
+        unroll_for<16>([&](auto iv) {
             constexpr int v = decltype(iv)::value;
             float pv = fast_exp2(x[v >> 2][v & 3] - ref);
             lrun += pv;
@@ -413,43 +443,63 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
                 pv *= row_lane<v>(vsc);
             p[v >> 3][v & 7] = f2bf(pv);
         });
+        if constexpr (E4M3) {
+            if (foreign) {
 #pragma unroll
-        for (int t = 0; t < 16; t++) {
-            if constexpr (E4M3) {
-                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(vr[t][0], vr[t][1], 1.f),
-                                                               p[0], o[t], 0, 0, 0);
-                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(vr[t][2], vr[t][3], 1.f),
-                                                               p[1], o[t], 0, 0, 0);
-            } else {
-                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vr[t]),
-                                                               p[0], o[t], 0, 0, 0);
+                for (int t = 0; t < 16; t++)
+                    rb[t] &= keep[0];
             }
+#pragma unroll
+            for (int t = 0; t < 16; t++) {
+                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(rb[t][0], rb[t][1], 1.f),
+                                                               p[0], o[t], 0, 0, 0);
+                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(rb[t][2], rb[t][3], 1.f),
+                                                               p[1], o[t], 0, 0, 0);
+            }
+        } else {
+            auto values = [&](u32x4 (&r)[16], int part) {
+                if (foreign) {
+#pragma unroll
+                    for (int j = 0; j < 16; j++)
+                        r[j] &= keep[j & 1];
+                }
+#pragma unroll
+                for (int j = 0; j < 16; j++)
+                    o[8 * part + (j >> 1)] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        __builtin_bit_cast(bf16x8, r[j]), p[j & 1], o[8 * part + (j >> 1)], 0, 0,
+                        0);
+            };
+            values(ra, 0);
+            load_k(ra, next, 0);
+            values(rb, 1);
+            load_k(rb, next, 1);
         }
     }
-    lrun += __shfl_xor(lrun, 16, 64);
-    lrun += __shfl_xor(lrun, 32, 64);
+    lrun = fold_rows(lrun, [](float a, float b) { return a + b; });
 
-    /* lane (m, g) holds dims 16 t + 4 g .. + 3 of row m. Where that goes is
-     * worked out again: kept over the loop it cost registers. */
-    int r = m;
-    asm volatile("" : "+v"(r));
+    /* lane (m, g) holds dims 16 t + 4 g .. + 3 of row m. Both are worked out again:
+     * kept over the loop they went to scratch memory. */
+    int none = 0;
+    asm volatile("" : "+v"(none));
+    const int id = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none));
+    const int r = id & 15, d0 = id >> 4 << 2;
     if (w.parts > 1) {
         const size_t slot = slot_of(c, kh, w.first + w.part);
         if (r < rows) {
 #pragma unroll
             for (int t = 0; t < 16; t++)
-                *(floatx4 *)(c.po + (slot * FEW + r) * PD + 16 * t + 4 * g) = o[t];
-            if (g == 0) {
+                *(floatx4 *)(c.po + (slot * FEW + r) * PD + 16 * t + d0) = o[t];
+            if (d0 == 0) {
                 c.pl[slot * FEW + r] = lrun;
                 c.pmu[slot * FEW + r] = mrun == -INFINITY ? 0.f : mrun;
             }
         }
     } else if (r < rows) {
         const float inv = lrun > 0.f ? 1.f / lrun : 0.f;
-        const int n = s.q0 + r / c.G, hd = kh * c.G + r % c.G;
+        const int tk = r * c.rG >> 8, n = s.q0 + tk, hd = kh * c.G + r - tk * c.G;
         bf16x4 gv[16];
         if (c.gate) {
-            const bf16 *gp = c.gate + (size_t)n * c.gts + (size_t)hd * c.ghs + 4 * g;
+            const bf16 *gp = c.gate + (size_t)n * c.gts + (size_t)hd * c.ghs + d0;
 #pragma unroll
             for (int t = 0; t < 16; t++)
                 gv[t] = *(const bf16x4 *)(gp + 16 * t);
@@ -460,7 +510,7 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
 #pragma unroll
             for (int e = 0; e < 4; e++)
                 res[e] = f2bf(o[t][e] * inv * (c.gate ? sigmoid_f(bf2f(gv[t][e])) : 1.f));
-            *(bf16x4 *)(c.out + ((size_t)n * c.Hq + hd) * PD + 16 * t + 4 * g) = res;
+            *(bf16x4 *)(c.out + ((size_t)n * c.Hq + hd) * PD + 16 * t + d0) = res;
         }
     }
 }
@@ -532,7 +582,7 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
     }
     if (at >= c.plan.shares)
         return;
-    const Where w = locate<RT, PG, true>(c, c.plan.shares - 1 - at);
+    const Where w = locate<RT, true>(c, c.plan.shares - 1 - at);
     if (w.b < 0)
         return;
     const pg_seq s = w.s;
@@ -1046,26 +1096,22 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
 }
 
 /* ---- merge of a unit's parts -----------------------------------------------------
- * One workgroup per row of few rows (its 4 waves a quarter of the parts each, joined
- * through LDS), or per 16 rows of many (4 of a wave in turn): o = sum 2^(mu_i - mu)
- * o_i over the parts that saw keys, l likewise, mu the largest of theirs; then / l
- * and the gate. l and mu come in one load (lane i: part i), o eight parts at a
- * time. */
-template <int ROWS, int KS>
+ * A wave per row (4 rows in turn of many): o = sum 2^(mu_i - mu) o_i over the parts
+ * that saw keys, l likewise, mu the largest of theirs; then / l and the gate. l and
+ * mu come in one load (lane i: part i), o 16 parts at a time. */
+template <int ROWS>
 __global__ __launch_bounds__(256) void merge_kernel(Call c, int groups) {
-    constexpr bool FEWR = ROWS == FEW;
-    __shared__ __attribute__((aligned(16))) float so[FEWR ? 4 : 1][PD];
-    __shared__ float sl[4], sm[4];
+    constexpr int EACH = ROWS == FEW ? 1 : 4; /* rows a wave */
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int group = blockIdx.x % groups, kh = blockIdx.x / groups % c.Hkv;
-    const Where w = locate<ROWS, KS, false>(c, blockIdx.x / groups / c.Hkv);
+    const Where w = locate<ROWS, false>(c, blockIdx.x / groups / c.Hkv);
     if (w.b < 0 || w.parts <= 1)
         return;
-    const int parts = w.parts;
     const size_t slot = slot_of(c, kh, w.first);
     const int nrows = min(w.s.ql * c.G - w.unit * ROWS, ROWS);
-    for (int i = 0; i < (FEWR ? 1 : 4); i++) {
-        const int t = FEWR ? group : 16 * group + 4 * wave + i;
+#pragma unroll 1
+    for (int i = 0; i < EACH; i++) {
+        const int t = (group * 4 + wave) * EACH + i;
         if (t >= nrows)
             return;
         const int r = w.unit * ROWS + t, n = w.s.q0 + r / c.G, head = kh * c.G + r % c.G;
@@ -1073,52 +1119,38 @@ __global__ __launch_bounds__(256) void merge_kernel(Call c, int groups) {
         if (c.gate)
             gv = *(const bf16x4 *)(c.gate + (size_t)n * c.gts + (size_t)head * c.ghs + 4 * lane);
         const size_t first = slot * ROWS + t;
-        const int q0 = FEWR ? parts * wave / 4 : 0, q1 = FEWR ? parts * (wave + 1) / 4 : parts;
         float mu = -INFINITY, l = 0.f;
         floatx4 acc = {};
-        for (int j0 = q0; j0 < q1; j0 += 64) { /* more than 64 parts: in turns */
-            const int cnt = min(q1 - j0, 64);
+        for (int j0 = 0; j0 < w.parts; j0 += 64) { /* more than 64 parts: in turns */
+            const int cnt = min(w.parts - j0, 64);
             const size_t mine = first + (size_t)(j0 + min(lane, cnt - 1)) * ROWS;
             const float pl = c.pl[mine], pm = c.pmu[mine];
             const float li = lane < cnt ? pl : 0.f, mi = li > 0.f ? pm : -INFINITY;
-            const float next = fmaxf(mu, wave_max(mi));
-            const float ref = next == -INFINITY ? 0.f : next, old = fast_exp2(mu - ref);
-            const float wi = li > 0.f ? fast_exp2(mi - ref) : 0.f;
-            mu = next;
-            l = l * old + wave_sum(wi * li);
-            acc *= old;
-            for (int k0 = 0; k0 < cnt; k0 += 8) {
-                floatx4 v[8];
+            float wi = 0.f;
+            for (int k0 = 0; k0 < cnt; k0 += 16) {
+                floatx4 v[16];
 #pragma unroll
-                for (int k = 0; k < 8; k++)
-                    v[k] = *(const floatx4 *)(c.po +
-                                              (first + (size_t)(j0 + min(k0 + k, cnt - 1)) * ROWS) *
-                                                  PD +
-                                              4 * lane);
+                for (int k = 0; k < 16; k++)
+                    if (k0 + k < cnt) /* uniform */
+                        v[k] = *(const floatx4 *)(c.po + (first + (size_t)(j0 + k0 + k) * ROWS) * PD +
+                                                  4 * lane);
+                if (k0 == 0) { /* with the first o on their way */
+                    const float next = fmaxf(mu, wave_max(mi));
+                    const float ref = next == -INFINITY ? 0.f : next, old = fast_exp2(mu - ref);
+                    wi = li > 0.f ? fast_exp2(mi - ref) : 0.f;
+                    mu = next;
+                    l = l * old + wave_sum(wi * li);
+                    acc *= old;
+                }
 #pragma unroll
-                for (int k = 0; k < 8; k++) {
+                for (int k = 0; k < 16; k++) {
+                    if (k0 + k >= cnt)
+                        break;
                     const float f = __uint_as_float((uint32_t)__builtin_amdgcn_readlane(
-                        (int)__float_as_uint(wi), min(k0 + k, 63)));
-                    if (k0 + k < cnt && f > 0.f)
+                        (int)__float_as_uint(wi), k0 + k));
+                    if (f > 0.f)
                         acc += v[k] * f;
                 }
-            }
-        }
-        if constexpr (FEWR) {
-            *(floatx4 *)&so[wave][4 * lane] = acc;
-            if (lane == 0)
-                sl[wave] = l, sm[wave] = mu;
-            lds_barrier();
-            if (wave > 0)
-                return;
-            const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-            const float ref = top == -INFINITY ? 0.f : top;
-            acc = floatx4{}, l = 0.f;
-#pragma unroll
-            for (int v = 0; v < 4; v++) {
-                const float f = fast_exp2(sm[v] - ref);
-                acc += *(const floatx4 *)&so[v][4 * lane] * f;
-                l += sl[v] * f;
             }
         }
         const float inv = l > 0.f ? 1.f / l : 0.f;
@@ -1136,8 +1168,8 @@ using namespace CUJEV_KNS;
 
 extern "C" size_t cujev_attention_paged_ws_bytes(int N, int B, int max_q, int max_kv, int Hq,
                                                  int Hkv, int window, int sinks, int type) {
-    const pg_plan p = pg_make_plan(N, B, max_q, max_kv, Hq / Hkv, Hkv, window, sinks,
-                                   type == CUJEV_KV_E4M3);
+    (void)type; /* the plan goes by key tiles */
+    const pg_plan p = pg_make_plan(N, B, max_q, max_kv, Hq / Hkv, Hkv, window, sinks);
     return (size_t)p.slots * Hkv * p.rt * (PD + 2) * sizeof(float);
 }
 
@@ -1148,7 +1180,7 @@ extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int
                                         size_t ws_bytes, hipStream_t stream) {
     const int Hkv = pages->Hkv, B = seqs->B, G = Hq / Hkv;
     const bool e4m3 = pages->type == CUJEV_KV_E4M3;
-    const pg_plan p = pg_make_plan(N, B, max_q, max_kv, G, Hkv, window, sinks, e4m3);
+    const pg_plan p = pg_make_plan(N, B, max_q, max_kv, G, Hkv, window, sinks);
     if (p.shares == 0)
         return hipSuccess;
     if (p.shares < 0)
@@ -1161,7 +1193,8 @@ extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int
     const Call c = {(const bf16 *)q, (const bf16 *)gate, gate_tok_stride, gate_head_stride,
                     pages->k, pages->vt, pages->k_scale, pages->v_scale, pages->num_pages,
                     seqs->q_start, seqs->kv_len, seqs->page_table, seqs->max_pages, B, N,
-                    max_q, max_kv, Hq, Hkv, G, window, sinks, (bf16 *)out,
+                    max_q, max_kv, Hq, Hkv, G, window, sinks,
+                    pg_div_up(256, G), (bf16 *)out,
                     (float *)ws, (float *)ws + rows * PD, (float *)ws + rows * (PD + 1), p};
     const bool few = p.rt == FEW;
     const int per = !few && 8 % Hkv == 0 ? 8 / Hkv : 1;
@@ -1175,14 +1208,12 @@ extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int
     else
         hipLaunchKernelGGL(attention_many_kernel<false>, grid, dim3(512), 0, stream, c);
     if (p.slots > 0) {
-        const int groups = few ? pg_min(max_q, N) * G : RT / 16;
+        const int groups = few ? pg_div_up(pg_min(max_q, N) * G, 4) : RT / 16;
         const dim3 mgrid((unsigned)(p.units * Hkv * groups));
-        if (few && e4m3)
-            hipLaunchKernelGGL((merge_kernel<FEW, 64>), mgrid, dim3(256), 0, stream, c, groups);
-        else if (few)
-            hipLaunchKernelGGL((merge_kernel<FEW, 32>), mgrid, dim3(256), 0, stream, c, groups);
+        if (few)
+            hipLaunchKernelGGL(merge_kernel<FEW>, mgrid, dim3(256), 0, stream, c, groups);
         else
-            hipLaunchKernelGGL((merge_kernel<RT, PG>), mgrid, dim3(256), 0, stream, c, groups);
+            hipLaunchKernelGGL(merge_kernel<RT>, mgrid, dim3(256), 0, stream, c, groups);
     }
     return hipGetLastError();
 }

@@ -74,12 +74,11 @@ constexpr int pg_max_tiles(int tok, int max_kv, int window, int sinks) {
  * kv-head. rt is PG_FEW where no sequence of the call has more rows than that (one
  * unit each), PG_MANY otherwise.
  *
- * PG_FEW: the units' steps, one after the other, are a line that pieces of equal
+ * PG_FEW: the units' key tiles, one after the other, are a line that pieces of equal
  * size cut; what lies in one piece of one unit is a part, a wave's work.
  * PG_MANY: a unit's key tiles are cut into as many even shares as the plan asks
  * for, a workgroup each. Parts of a unit of several leave theirs in slots. */
 constexpr int PG_FEW = 16, PG_MANY = 128;
-constexpr int PG_FEW_PARTS = 128; /* parts of a unit of few rows, about, at most */
 
 struct pg_plan {
     int rt;
@@ -103,10 +102,10 @@ constexpr int pg_longest(const pg_seq &s, int G, int rt, int window, int sinks) 
         pg_tile_list(s, (int)((long long)(units - 1) * rt / G), s.ql - 1, window, sinks);
     return pg_max(t.ntl, 1);
 }
-/* PG_FEW: steps a piece, for a line of T with `most` in its longest unit */
-constexpr int pg_few_share(const pg_plan &p, unsigned T, int most) {
+/* PG_FEW: tiles a piece of a line of T */
+constexpr int pg_few_share(const pg_plan &p, unsigned T) {
     const unsigned n = (unsigned)p.goal;
-    return pg_max(pg_max((int)(T / n + (T % n != 0)), pg_div_up(most, PG_FEW_PARTS)), 1);
+    return pg_max((int)(T / n + (T % n != 0)), 1);
 }
 /* PG_FEW: number of the part of unit u (counted over the kv-head) in a piece: rises
  * along the line, and a unit's parts have consecutive ones */
@@ -127,7 +126,7 @@ constexpr int pg_nshare(int tiles, int share) { return pg_max(pg_div_up(tiles, s
 constexpr int pg_share_begin(int ntl, int i, int n) { return (int)((long long)ntl * i / n); }
 
 constexpr pg_plan pg_make_plan(int N, int B, int max_q, int max_kv, int G, int Hkv, int window,
-                               int sinks, bool e4m3) {
+                               int sinks) {
     pg_plan p{};
     const long long mq = pg_min(max_q, N);
     p.rt = mq * G <= PG_FEW ? PG_FEW : PG_MANY;
@@ -139,13 +138,15 @@ constexpr pg_plan pg_make_plan(int N, int B, int max_q, int max_kv, int G, int H
     const long long most = pg_max(pg_max_tiles(tok, max_kv, window, sinks), 1);
     long long units = B, shares = 0, slots = 0;
     if (p.rt == PG_FEW) {
-        const long long steps = most * (e4m3 ? 1 : 2);
+        /* 2 waves a SIMD; few units: no more parts each than a merge takes in one
+         * go, 64 */
         p.goal = pg_max(2048 / Hkv, 1);
-        /* a line of at most units * steps, which are ints, in pieces of at least a
-         * step; the last part's number is below pieces + units */
-        const long long line = units * steps;
+        p.goal = 64 * units < p.goal ? (int)(64 * units) : p.goal;
+        /* a line of at most units * most tiles, which are ints, in pieces of at
+         * least a tile; the last part's number is below pieces + units */
+        const long long line = units * most;
         shares = line > 0x7fffffff ? PG_MOST : (line < p.goal ? line : p.goal) + units;
-        slots = steps > 1 ? shares : 0;
+        slots = most > 1 ? shares : 0;
     } else {
         const long long by_rows = (long long)N * G / PG_MANY + B;
         const long long by_len = B * ((mq * G + PG_MANY - 1) / PG_MANY);

@@ -104,7 +104,7 @@ int main() {
     }
     /* the plan: shares tile each unit's list, and the launch and slots hold them */
     for (int it = 0; it < 30000; it++) {
-        const int G = 1 << rnd(0, 4), Hkv = 1 << rnd(0, 3), e4m3 = rnd(0, 1);
+        const int G = 1 << rnd(0, 4), Hkv = 1 << rnd(0, 3);
         const int B = it % 7 ? rnd(1, 12) : rnd(1, 600), top = it % 3 ? 1 << rnd(0, 13) : 20000;
         const int mq = it % 2 ? rnd(1, 3) : rnd(1, 300), w = rnd(0, 2) ? 0 : rnd(1, 2000), S = w ? rnd(0, 100) : 0;
         std::vector<int> q, kv;
@@ -114,32 +114,31 @@ int main() {
             N += q[b], max_q = pg_max(max_q, q[b]), max_kv = pg_max(max_kv, kv[b]);
         }
         if (rnd(0, 1)) max_kv += rnd(0, 500);
-        const pg_plan p = pg_make_plan(N, B, max_q, max_kv, G, Hkv, w, S, e4m3);
+        const pg_plan p = pg_make_plan(N, B, max_q, max_kv, G, Hkv, w, S);
         const int W = w >= max_kv ? 0 : w, SS = W ? S : 0;
         long long U = 0, T = 0, C = 0;
-        int at = 0, most = 0, KS = e4m3 ? 64 : 32;
+        int at = 0;
         std::vector<pg_seq> seqs;
         for (int b = 0; b < B; b++) {
             seqs.push_back(pg_clean_seq(at, at + q[b], kv[b], N, max_q, max_kv));
             at += q[b];
             const int u = max_q ? pg_units(seqs[b], G, p.rt) : 0;
-            const int n = pg_longest(seqs[b], G, p.rt, W, SS) * (p.rt == 16 ? PG / KS : 1);
-            U += u, T += (long long)u * n, most = pg_max(most, u ? n : 0);
+            U += u, T += (long long)u * pg_longest(seqs[b], G, p.rt, W, SS);
         }
         if (max_q == 0) { NEED(p.shares == 0); continue; }
         NEED(p.rt == (max_q * G <= 16 ? 16 : 128) && U <= p.units);
         if (p.rt == 16) {
             if (U == 0) continue;
-            const int size = pg_few_share(p, (unsigned)T, most);
+            const int size = pg_few_share(p, (unsigned)T);
             int line = 0, u = 0, last = -1;
             for (int b = 0; b < B; b++) {
                 if (pg_units(seqs[b], G, 16) == 0) continue;
                 NEED(pg_units(seqs[b], G, 16) == 1);
-                const int n = pg_longest(seqs[b], G, 16, W, SS) * (PG / KS);
+                const int n = pg_longest(seqs[b], G, 16, W, SS);
                 const pg_tiles t = pg_tile_list(seqs[b], 0, seqs[b].ql - 1, W, SS);
-                NEED(t.ntl * (PG / KS) == n || t.ntl == 0);
+                NEED(t.ntl == n || t.ntl == 0);
                 const int p0 = line / size, p1 = (line + n - 1) / size;
-                NEED(p1 - p0 + 1 <= PG_FEW_PARTS + 1);
+                NEED(B > 1 || p1 - p0 < 64);
                 NEED(pg_few_slot(p0, u) > last && pg_few_slot(p1, u) < p.shares);
                 NEED(p0 == p1 || pg_few_slot(p1, u) < p.slots);
                 last = pg_few_slot(p1, u);
@@ -164,16 +163,14 @@ int main() {
         NEED(C <= p.shares && (p.slots == 0 || p.slots >= C));
     }
     {   /* the largest calls: nothing overflows */
-        NEED(pg_make_plan(PG_MOST, 1, PG_MOST, PG_MOST_KEYS, 16, 1, 0, 0, true).shares == -1);
-        NEED(pg_make_plan(PG_MOST, PG_MOST, 1, PG_MOST_KEYS, 16, 1, 0, 0, true).shares == -1);
-        for (int e = 0; e < 2; e++) {
-            const pg_plan f = pg_make_plan(60, 60, 1, PG_MOST_KEYS, 16, 1, 0, 0, e);
-            const pg_seq s = pg_clean_seq(0, 1, PG_MOST_KEYS, 60, 1, PG_MOST_KEYS);
-            const int n = pg_longest(s, 16, 16, 0, 0) * (e ? 1 : 2);
-            const int size = pg_few_share(f, 60u * (unsigned)n, n);
-            NEED(f.shares > 0 && pg_few_slot((int)((60ll * n - 1) / size), 59) < f.shares);
-            NEED((f.shares + 1ll) * size < 0x7fffffff); /* where a piece ends */
-        }
+        NEED(pg_make_plan(PG_MOST, 1, PG_MOST, PG_MOST_KEYS, 16, 1, 0, 0).shares == -1);
+        NEED(pg_make_plan(PG_MOST, PG_MOST, 1, PG_MOST_KEYS, 16, 1, 0, 0).shares == -1);
+        const pg_plan f = pg_make_plan(60, 60, 1, PG_MOST_KEYS, 16, 1, 0, 0);
+        const pg_seq s = pg_clean_seq(0, 1, PG_MOST_KEYS, 60, 1, PG_MOST_KEYS);
+        const int n = pg_longest(s, 16, 16, 0, 0);
+        const int size = pg_few_share(f, 60u * (unsigned)n);
+        NEED(f.shares > 0 && pg_few_slot((int)((60ll * n - 1) / size), 59) < f.shares);
+        NEED((f.shares + 1ll) * size < 0x7fffffff); /* where a piece ends */
     }
     printf("bad %d\n", bad);
     return bad != 0;
