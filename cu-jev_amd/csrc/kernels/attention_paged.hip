@@ -114,11 +114,21 @@ struct Call {
 DEV pg_seq seq_of(const Call &c, int b) {
     return load_seq(c.q_start, c.kv_len, b, c.N, c.max_q, c.max_kv);
 }
+DEV pg_seq seq_at(const pg_seq &s, int l) { /* lane l's */
+    auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+    return {of(s.q0), of(s.ql), of(s.kv), of(s.p0)};
+}
 DEV int page_id(const Call &c, int b, const pg_tiles &t, int i) {
     const int page = c.page_table[(size_t)b * c.max_pages + pg_tile_page(t, i)];
     return page >= 0 && page < c.num_pages ? page : -1;
 }
 
+/* The lane's number, worked out where it stands: kept, it may go to scratch memory */
+DEV int lane_again() {
+    int none = 0;
+    asm volatile("" : "+v"(none));
+    return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none));
+}
 /* f over the lanes with the same number in each of the wave's four rows of 16 */
 template <class F> DEV float fold_rows(float x, F f) {
     const uint32_t u = __float_as_uint(x);
@@ -142,11 +152,10 @@ DEV int wave_scan(int v) {
 }
 DEV int last_lane(int v) { return __builtin_amdgcn_readlane(v, 63); }
 
-/* The unit that part `target` of a kv-head belongs to (BY_PART), or unit `target`:
- * its sequence (b -1: there is none), its number in it, its parts, the first
- * one's number, which of them `target` is. With few rows the parts are those of
- * the pieces of the line (numbered by pg_few_slot), and begin .. begin + own the
- * unit's tiles on it, with many rows the unit's shares. */
+/* The unit that share `target` of a kv-head belongs to (BY_PART; few rows: the one
+ * that piece `target` begins in), or unit `target`: its sequence (b -1: there is
+ * none), its number in it, its parts, the first one's number (few rows: its
+ * piece's), which of them `target` is. */
 struct Where {
     pg_seq s;
     int b, unit, parts, first, part;
@@ -200,26 +209,24 @@ template <int RT_, bool BY_PART> DEV Where locate(const Call &c, int target) {
         if (c.B > 64)
             read(b0);
         const int parts = FEWR ? 0 : pg_nshare(n, size);
-        const int su = before_u + wave_scan(units);
+        const int su = FEWR && BY_PART ? 0 : before_u + wave_scan(units);
         const int sn = before_n + wave_scan(units * (FEWR ? n : parts));
         const int u = su - units, a = sn - units * (FEWR ? n : parts); /* before the lane's */
         /* few rows: one unit, its parts are pieces p0 .. p1 */
         const int p0 = FEWR ? a / size : 0, p1 = FEWR ? (sn - 1) / size : 0;
         const uint64_t past = __ballot(!BY_PART ? su > target
-                                       : FEWR   ? units > 0 && pg_few_slot(p1, u) >= target
+                                       : FEWR   ? units > 0 && p1 >= target
                                                 : sn > target);
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
             auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-            w.s.q0 = of(s.q0), w.s.ql = of(s.ql), w.s.kv = of(s.kv), w.s.p0 = of(s.p0);
+            w.s = seq_at(s, l);
             w.b = b0 + l;
             if constexpr (FEWR) {
                 w.unit = 0, w.begin = of(a), w.own = of(n), w.size = size;
-                w.first = pg_few_slot(of(p0), of(u));
+                w.first = of(p0);
                 w.parts = of(p1) - of(p0) + 1;
                 w.part = BY_PART ? target - w.first : 0;
-                if (w.part < 0) /* a number between two units' */
-                    w.b = -1;
             } else {
                 w.parts = of(parts);
                 w.unit = BY_PART ? (target - of(a)) / w.parts : target - of(u);
@@ -259,15 +266,15 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
     constexpr uint32_t EB = E4M3 ? 1 : 2, SLICE = PSLICE * EB;
     __shared__ bf16x8 sq[8 * 64];
     const int kh = blockIdx.x % c.Hkv;
-    const int lane = threadIdx.x, m = lane & 15, g = lane >> 4;
-    const Where w = locate<FEW, true>(c, blockIdx.x / c.Hkv);
-    if (w.b < 0)
-        return;
+    Where w = locate<FEW, true>(c, blockIdx.x / c.Hkv);
+    /* the units that the piece lies in */
+    while (w.b >= 0) {
+    const int lane = lane_again(), m = lane & 15, g = lane >> 4;
     const pg_seq s = w.s;
     const int b = w.b, rows = min(s.ql * c.G, FEW);
     const pg_tiles list = pg_tile_list(s, 0, s.ql - 1, c.window, c.sinks);
     /* tiles [i0, i1) of the unit's; a unit without a key has one that is not there */
-    const int cut = (w.begin / w.size + w.part) * w.size - w.begin;
+    const int cut = (w.first + w.part) * w.size - w.begin;
     const int i0 = max(cut, 0), i1 = min(min(cut + w.size, w.own), list.ntl);
     /* the ids of 64 tiles of the list are in a lane each */
     int ids = i0 < i1 ? page_id(c, b, list, min(i0 + lane, list.ntl - 1)) : -1, ids0 = i0;
@@ -292,8 +299,8 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
     auto key_of = [&](int v) { return keyg + (E4M3 ? v : (v & 7) + 32 * (v >> 3)); };
     const uint32_t kvoff = key0 * PD * EB + 16 * g, vvoff = m * PG * EB + 16 * g;
 
-    u32x4 ra[16], rb[16]; /* e4m3: K, V^T; bf16: the first half of each, the second */
-    float ksc[4], vsc = 1.f;
+    u32x4 ra[16] = {}, rb[16] = {}; /* e4m3: K, V^T; bf16: the first half of each, the second */
+    float ksc[4] = {}, vsc = 1.f;
     auto rsrc = [&](const void *p, int page) {
         return make_rsrc((const char *)p + ((size_t)max(page, 0) * c.Hkv + kh) * SLICE, SLICE);
     };
@@ -306,9 +313,9 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
     auto load_k = [&](u32x4 (&r)[16], int page, int part) {
         const __amdgpu_buffer_rsrc_t src = rsrc(c.k, page);
 #pragma unroll
-        for (int i = 0; i < (E4M3 ? 4 : 8); i++)
+        for (int k = 0; k < (E4M3 ? 4 : 2); k++)
 #pragma unroll
-            for (int k = 0; k < (E4M3 ? 4 : 2); k++)
+            for (int i = 0; i < (E4M3 ? 4 : 8); i++) /* the halves of a line in turn */
                 r[i * (E4M3 ? 4 : 2) + k] =
                     buf_load16(src, kvoff, kkey((E4M3 ? 0 : 2 * part) + k) * PD * EB + 64 * i);
         if constexpr (E4M3) {
@@ -479,12 +486,9 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
 
     /* lane (m, g) holds dims 16 t + 4 g .. + 3 of row m. Both are worked out again:
      * kept over the loop they went to scratch memory. */
-    int none = 0;
-    asm volatile("" : "+v"(none));
-    const int id = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none));
-    const int r = id & 15, d0 = id >> 4 << 2;
+    const int id = lane_again(), r = id & 15, d0 = id >> 4 << 2;
     if (w.parts > 1) {
-        const size_t slot = slot_of(c, kh, w.first + w.part);
+        const size_t slot = slot_of(c, kh, pg_few_slot(w.first, w.part));
         if (r < rows) {
 #pragma unroll
             for (int t = 0; t < 16; t++)
@@ -497,7 +501,7 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
     } else if (r < rows) {
         const float inv = lrun > 0.f ? 1.f / lrun : 0.f;
         const int tk = r * c.rG >> 8, n = s.q0 + tk, hd = kh * c.G + r - tk * c.G;
-        bf16x4 gv[16];
+        bf16x4 gv[16] = {};
         if (c.gate) {
             const bf16 *gp = c.gate + (size_t)n * c.gts + (size_t)hd * c.ghs + d0;
 #pragma unroll
@@ -512,6 +516,23 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
                 res[e] = f2bf(o[t][e] * inv * (c.gate ? sigmoid_f(bf2f(gv[t][e])) : 1.f));
             *(bf16x4 *)(c.out + ((size_t)n * c.Hq + hd) * PD + 16 * t + d0) = res;
         }
+    }
+    /* on to the next unit, if the piece goes on after this one */
+    w.begin += w.own, w.first = w.begin / w.size, w.part = 0;
+    w.b = -1;
+    for (int b0 = cut + w.size <= w.own ? c.B : b + 1; b0 < c.B; b0 += 64) {
+        const int at = lane_again();
+        const pg_seq t = seq_of(c, min(b0 + at, c.B - 1));
+        const uint64_t any = __ballot(b0 + at < c.B && pg_units(t, c.G, FEW) > 0);
+        if (any) {
+            const int l = __ffsll((unsigned long long)any) - 1;
+            w.s = seq_at(t, l);
+            w.b = b0 + l;
+            w.own = pg_longest(w.s, c.G, FEW, c.window, c.sinks);
+            w.parts = (w.begin + w.own - 1) / w.size - w.first + 1;
+            break;
+        }
+    }
     }
 }
 
@@ -1107,7 +1128,8 @@ __global__ __launch_bounds__(256) void merge_kernel(Call c, int groups) {
     const Where w = locate<ROWS, false>(c, blockIdx.x / groups / c.Hkv);
     if (w.b < 0 || w.parts <= 1)
         return;
-    const size_t slot = slot_of(c, kh, w.first);
+    const size_t slot0 = slot_of(c, kh, ROWS == FEW ? 0 : w.first);
+    auto slot = [&](int j) { return slot0 + (ROWS == FEW ? pg_few_slot(w.first, j) : j); };
     const int nrows = min(w.s.ql * c.G - w.unit * ROWS, ROWS);
 #pragma unroll 1
     for (int i = 0; i < EACH; i++) {
@@ -1118,12 +1140,11 @@ __global__ __launch_bounds__(256) void merge_kernel(Call c, int groups) {
         bf16x4 gv = {};
         if (c.gate)
             gv = *(const bf16x4 *)(c.gate + (size_t)n * c.gts + (size_t)head * c.ghs + 4 * lane);
-        const size_t first = slot * ROWS + t;
         float mu = -INFINITY, l = 0.f;
         floatx4 acc = {};
         for (int j0 = 0; j0 < w.parts; j0 += 64) { /* more than 64 parts: in turns */
             const int cnt = min(w.parts - j0, 64);
-            const size_t mine = first + (size_t)(j0 + min(lane, cnt - 1)) * ROWS;
+            const size_t mine = slot(j0 + min(lane, cnt - 1)) * ROWS + t;
             const float pl = c.pl[mine], pm = c.pmu[mine];
             const float li = lane < cnt ? pl : 0.f, mi = li > 0.f ? pm : -INFINITY;
             float wi = 0.f;
@@ -1132,8 +1153,7 @@ __global__ __launch_bounds__(256) void merge_kernel(Call c, int groups) {
 #pragma unroll
                 for (int k = 0; k < 16; k++)
                     if (k0 + k < cnt) /* uniform */
-                        v[k] = *(const floatx4 *)(c.po + (first + (size_t)(j0 + k0 + k) * ROWS) * PD +
-                                                  4 * lane);
+                        v[k] = *(const floatx4 *)(c.po + (slot(j0 + k0 + k) * ROWS + t) * PD + 4 * lane);
                 if (k0 == 0) { /* with the first o on their way */
                     const float next = fmaxf(mu, wave_max(mi));
                     const float ref = next == -INFINITY ? 0.f : next, old = fast_exp2(mu - ref);

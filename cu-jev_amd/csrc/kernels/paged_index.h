@@ -75,7 +75,7 @@ constexpr int pg_max_tiles(int tok, int max_kv, int window, int sinks) {
  * unit each), PG_MANY otherwise.
  *
  * PG_FEW: the units' key tiles, one after the other, are a line that pieces of equal
- * size cut; what lies in one piece of one unit is a part, a wave's work.
+ * size cut, a wave's work each; what lies in one piece of one unit is a part.
  * PG_MANY: a unit's key tiles are cut into as many even shares as the plan asks
  * for, a workgroup each. Parts of a unit of several leave theirs in slots. */
 constexpr int PG_FEW = 16, PG_MANY = 128;
@@ -83,8 +83,9 @@ constexpr int PG_FEW = 16, PG_MANY = 128;
 struct pg_plan {
     int rt;
     int units;  /* units of a kv-head, at most */
-    int shares; /* parts of a kv-head's units, at most (0: no work, -1: too many) */
-    int slots;  /* of these, at most, with something to merge (0: no merge) */
+    int shares; /* pieces (PG_FEW) or parts of a kv-head's units, at most (0: no
+                 * work, -1: too many) */
+    int slots;  /* of parts with something to merge, at most (0: no merge) */
     int goal;   /* waves (PG_FEW) or workgroups of a kv-head that the chip runs at
                  * once; 0 (PG_MANY): whole units fill it */
 };
@@ -102,14 +103,18 @@ constexpr int pg_longest(const pg_seq &s, int G, int rt, int window, int sinks) 
         pg_tile_list(s, (int)((long long)(units - 1) * rt / G), s.ql - 1, window, sinks);
     return pg_max(t.ntl, 1);
 }
-/* PG_FEW: tiles a piece of a line of T */
+/* PG_FEW: tiles a piece of a line of T. Pieces of one tile instead of two gain
+ * nothing, since a wave's first loads take longer than a tile (16 sequences of 1024
+ * e4m3 keys 17.4 us with one, 15.0 with two). */
+constexpr int PG_FEW_LEAST = 2;
 constexpr int pg_few_share(const pg_plan &p, unsigned T) {
     const unsigned n = (unsigned)p.goal;
-    return pg_max((int)(T / n + (T % n != 0)), 1);
+    return pg_max((int)(T / n + (T % n != 0)), PG_FEW_LEAST);
 }
-/* PG_FEW: number of the part of unit u (counted over the kv-head) in a piece: rises
- * along the line, and a unit's parts have consecutive ones */
-constexpr int pg_few_slot(int piece, int u) { return piece + u; }
+/* PG_FEW: the slot of part j of a unit that begins in piece p0 and goes on after it.
+ * A piece has at most two such parts: of a unit that came in from the piece before,
+ * and of one that begins here and goes on. */
+constexpr int pg_few_slot(int p0, int j) { return 2 * (p0 + j) + (j == 0); }
 
 /* PG_MANY: key tiles a share should have, for U units with T tiles in all. A
  * sequence's last share is half empty on average: as many workgroups fewer to
@@ -138,15 +143,17 @@ constexpr pg_plan pg_make_plan(int N, int B, int max_q, int max_kv, int G, int H
     const long long most = pg_max(pg_max_tiles(tok, max_kv, window, sinks), 1);
     long long units = B, shares = 0, slots = 0;
     if (p.rt == PG_FEW) {
-        /* 2 waves a SIMD; few units: no more parts each than a merge takes in one
-         * go, 64 */
-        p.goal = pg_max(2048 / Hkv, 1);
+        /* A wave a SIMD: 64 sequences of 1024 bf16 keys take 53 us so, 61 with two
+         * a SIMD, and half as many as SIMDs leave 24 of 5000 at 58 instead of 52.
+         * Few units: no more parts each than a merge takes in one go, 64 (one of
+         * 65536 keys 42 us; 43 with 128 parts, 60 with 32). */
+        p.goal = pg_max(1024 / Hkv, 1);
         p.goal = 64 * units < p.goal ? (int)(64 * units) : p.goal;
         /* a line of at most units * most tiles, which are ints, in pieces of at
-         * least a tile; the last part's number is below pieces + units */
-        const long long line = units * most;
-        shares = line > 0x7fffffff ? PG_MOST : (line < p.goal ? line : p.goal) + units;
-        slots = most > 1 ? shares : 0;
+         * least PG_FEW_LEAST */
+        const long long line = units * most, pieces = (line + PG_FEW_LEAST - 1) / PG_FEW_LEAST;
+        shares = line > 0x7fffffff ? PG_MOST : pieces < p.goal ? pieces : p.goal;
+        slots = most > 1 ? 2 * shares : 0;
     } else {
         const long long by_rows = (long long)N * G / PG_MANY + B;
         const long long by_len = B * ((mq * G + PG_MANY - 1) / PG_MANY);

@@ -130,7 +130,8 @@ int main() {
         if (p.rt == 16) {
             if (U == 0) continue;
             const int size = pg_few_share(p, (unsigned)T);
-            int line = 0, u = 0, last = -1;
+            int line = 0;
+            std::vector<char> used(p.slots);
             for (int b = 0; b < B; b++) {
                 if (pg_units(seqs[b], G, 16) == 0) continue;
                 NEED(pg_units(seqs[b], G, 16) == 1);
@@ -139,10 +140,13 @@ int main() {
                 NEED(t.ntl == n || t.ntl == 0);
                 const int p0 = line / size, p1 = (line + n - 1) / size;
                 NEED(B > 1 || p1 - p0 < 64);
-                NEED(pg_few_slot(p0, u) > last && pg_few_slot(p1, u) < p.shares);
-                NEED(p0 == p1 || pg_few_slot(p1, u) < p.slots);
-                last = pg_few_slot(p1, u);
-                line += n, u++;
+                NEED(p1 < p.shares);
+                for (int j = 0; p1 > p0 && j <= p1 - p0; j++) {
+                    const int slot = pg_few_slot(p0, j);
+                    NEED(slot < p.slots && !used[slot]);
+                    if (slot < p.slots) used[slot] = 1;
+                }
+                line += n;
             }
             continue;
         }
@@ -169,8 +173,8 @@ int main() {
         const pg_seq s = pg_clean_seq(0, 1, PG_MOST_KEYS, 60, 1, PG_MOST_KEYS);
         const int n = pg_longest(s, 16, 16, 0, 0);
         const int size = pg_few_share(f, 60u * (unsigned)n);
-        NEED(f.shares > 0 && pg_few_slot((int)((60ll * n - 1) / size), 59) < f.shares);
-        NEED((f.shares + 1ll) * size < 0x7fffffff); /* where a piece ends */
+        NEED(f.shares > 0 && (60ll * n - 1) / size < f.shares);
+        NEED((f.goal + 1ll) * size < 0x7fffffff); /* where a piece ends */
     }
     printf("bad %d\n", bad);
     return bad != 0;
