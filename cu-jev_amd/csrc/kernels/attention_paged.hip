@@ -174,7 +174,7 @@ template <int RT_, bool BY_PART> DEV Where locate(const Call &c, int target) {
         if (units == 0)
             return w;
         if constexpr (FEWR) {
-            w.size = pg_few_share(c.plan, (unsigned)n);
+            w.size = pg_few_share(c.plan, 1, (unsigned)n);
             w.own = n;
             w.parts = (n - 1) / w.size + 1;
         } else {
@@ -200,10 +200,9 @@ template <int RT_, bool BY_PART> DEV Where locate(const Call &c, int target) {
     for (int b0 = 0; b0 < c.B; b0 += 64) {
         read(b0);
         T += (unsigned)last_lane(wave_scan((int)((unsigned)units * (unsigned)n)));
-        if constexpr (!FEWR)
-            U += last_lane(wave_scan(units));
+        U += FEWR ? __popcll(__ballot(units > 0)) : last_lane(wave_scan(units));
     }
-    const int size = FEWR ? pg_few_share(c.plan, T) : pg_share(c.plan, U, T);
+    const int size = FEWR ? pg_few_share(c.plan, U, T) : pg_share(c.plan, U, T);
     int before_u = 0, before_n = 0;
     for (int b0 = 0; b0 < c.B; b0 += 64) {
         if (c.B > 64)
@@ -1117,12 +1116,17 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
 }
 
 /* ---- merge of a unit's parts -----------------------------------------------------
- * A wave per row (4 rows in turn of many): o = sum 2^(mu_i - mu) o_i over the parts
- * that saw keys, l likewise, mu the largest of theirs; then / l and the gate. l and
- * mu come in one load (lane i: part i), o 16 parts at a time. */
-template <int ROWS>
+ * o = sum 2^(mu_i - mu) o_i over the parts that saw keys, l likewise, mu the largest
+ * of theirs; then / l and the gate. l and mu come in one load, lane i: part i.
+ * A wave per row (4 rows in turn of many), o 16 parts at a time; or, ROW, a
+ * workgroup: a wave 64 dims, o 64 parts at a time, 4 a load. That is for
+ * few rows after many keys (4 rows of 64 parts: 5.4 us, and 8.8 a wave per row); the
+ * starts of many workgroups cost more than it gains (1024 rows of 4 parts: 5.6 and
+ * 4.8, 4096 of them 22 and 8). */
+template <int ROWS, bool ROW>
 __global__ __launch_bounds__(256) void merge_kernel(Call c, int groups) {
     constexpr int EACH = ROWS == FEW ? 1 : 4; /* rows a wave */
+    constexpr int STEP = ROW ? 64 : 16, PER = STEP / 16;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int group = blockIdx.x % groups, kh = blockIdx.x / groups % c.Hkv;
     const Where w = locate<ROWS, false>(c, blockIdx.x / groups / c.Hkv);
@@ -1131,15 +1135,16 @@ __global__ __launch_bounds__(256) void merge_kernel(Call c, int groups) {
     const size_t slot0 = slot_of(c, kh, ROWS == FEW ? 0 : w.first);
     auto slot = [&](int j) { return slot0 + (ROWS == FEW ? pg_few_slot(w.first, j) : j); };
     const int nrows = min(w.s.ql * c.G - w.unit * ROWS, ROWS);
+    const int dim = ROW ? 64 * wave + 4 * (lane & 15) : 4 * lane, own = ROW ? lane >> 4 : 0;
 #pragma unroll 1
     for (int i = 0; i < EACH; i++) {
-        const int t = (group * 4 + wave) * EACH + i;
+        const int t = ROW ? group : (group * 4 + wave) * EACH + i;
         if (t >= nrows)
             return;
         const int r = w.unit * ROWS + t, n = w.s.q0 + r / c.G, head = kh * c.G + r % c.G;
         bf16x4 gv = {};
         if (c.gate)
-            gv = *(const bf16x4 *)(c.gate + (size_t)n * c.gts + (size_t)head * c.ghs + 4 * lane);
+            gv = *(const bf16x4 *)(c.gate + (size_t)n * c.gts + (size_t)head * c.ghs + dim);
         float mu = -INFINITY, l = 0.f;
         floatx4 acc = {};
         for (int j0 = 0; j0 < w.parts; j0 += 64) { /* more than 64 parts: in turns */
@@ -1148,12 +1153,14 @@ __global__ __launch_bounds__(256) void merge_kernel(Call c, int groups) {
             const float pl = c.pl[mine], pm = c.pmu[mine];
             const float li = lane < cnt ? pl : 0.f, mi = li > 0.f ? pm : -INFINITY;
             float wi = 0.f;
-            for (int k0 = 0; k0 < cnt; k0 += 16) {
+            for (int k0 = 0; k0 < cnt; k0 += STEP) {
                 floatx4 v[16];
 #pragma unroll
                 for (int k = 0; k < 16; k++)
-                    if (k0 + k < cnt) /* uniform */
-                        v[k] = *(const floatx4 *)(c.po + (slot(j0 + k0 + k) * ROWS + t) * PD + 4 * lane);
+                    if (k0 + k * PER < cnt) { /* uniform */
+                        const int j = j0 + min(k0 + k * PER + own, cnt - 1);
+                        v[k] = *(const floatx4 *)(c.po + (slot(j) * ROWS + t) * PD + dim);
+                    }
                 if (k0 == 0) { /* with the first o on their way */
                     const float next = fmaxf(mu, wave_max(mi));
                     const float ref = next == -INFINITY ? 0.f : next, old = fast_exp2(mu - ref);
@@ -1164,21 +1171,29 @@ __global__ __launch_bounds__(256) void merge_kernel(Call c, int groups) {
                 }
 #pragma unroll
                 for (int k = 0; k < 16; k++) {
-                    if (k0 + k >= cnt)
+                    if (k0 + k * PER >= cnt)
                         break;
-                    const float f = __uint_as_float((uint32_t)__builtin_amdgcn_readlane(
-                        (int)__float_as_uint(wi), k0 + k));
+                    /* lanes from cnt on have weight 0 */
+                    const float f = ROW ? __shfl(wi, k * PER + own, 64)
+                                        : __uint_as_float((uint32_t)__builtin_amdgcn_readlane(
+                                              (int)__float_as_uint(wi), k0 + k));
                     if (f > 0.f)
                         acc += v[k] * f;
                 }
             }
+        }
+        if constexpr (ROW) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                acc[e] = fold_rows(acc[e], [](float x, float y) { return x + y; });
         }
         const float inv = l > 0.f ? 1.f / l : 0.f;
         bf16x4 res;
 #pragma unroll
         for (int e = 0; e < 4; e++)
             res[e] = f2bf(acc[e] * inv * (c.gate ? sigmoid_f(bf2f(gv[e])) : 1.f));
-        *(bf16x4 *)(c.out + ((size_t)n * c.Hq + head) * PD + 4 * lane) = res;
+        if (!ROW || lane < 16)
+            *(bf16x4 *)(c.out + ((size_t)n * c.Hq + head) * PD + dim) = res;
     }
 }
 
@@ -1228,12 +1243,16 @@ extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int
     else
         hipLaunchKernelGGL(attention_many_kernel<false>, grid, dim3(512), 0, stream, c);
     if (p.slots > 0) {
-        const int groups = few ? pg_div_up(pg_min(max_q, N) * G, 4) : RT / 16;
+        const int rows = pg_min(max_q, N) * G;
+        const bool row = few && (long long)p.units * rows * Hkv <= 512;
+        const int groups = !few ? RT / 16 : row ? rows : pg_div_up(rows, 4);
         const dim3 mgrid((unsigned)(p.units * Hkv * groups));
-        if (few)
-            hipLaunchKernelGGL(merge_kernel<FEW>, mgrid, dim3(256), 0, stream, c, groups);
+        if (row)
+            hipLaunchKernelGGL((merge_kernel<FEW, true>), mgrid, dim3(256), 0, stream, c, groups);
+        else if (few)
+            hipLaunchKernelGGL((merge_kernel<FEW, false>), mgrid, dim3(256), 0, stream, c, groups);
         else
-            hipLaunchKernelGGL(merge_kernel<RT>, mgrid, dim3(256), 0, stream, c, groups);
+            hipLaunchKernelGGL((merge_kernel<RT, false>), mgrid, dim3(256), 0, stream, c, groups);
     }
     return hipGetLastError();
 }

@@ -103,13 +103,15 @@ constexpr int pg_longest(const pg_seq &s, int G, int rt, int window, int sinks) 
         pg_tile_list(s, (int)((long long)(units - 1) * rt / G), s.ql - 1, window, sinks);
     return pg_max(t.ntl, 1);
 }
-/* PG_FEW: tiles a piece of a line of T. Pieces of one tile instead of two gain
- * nothing, since a wave's first loads take longer than a tile (16 sequences of 1024
- * e4m3 keys 17.4 us with one, 15.0 with two). */
-constexpr int PG_FEW_LEAST = 2;
-constexpr int pg_few_share(const pg_plan &p, unsigned T) {
+/* PG_FEW: tiles a piece of a line of U units with T tiles. Pieces of one tile instead
+ * of two gain nothing where there are many, since a wave's first loads take longer
+ * than a tile (16 sequences of 1024 e4m3 keys 17.4 us with one, 15.4 with two); but
+ * a short line has waves enough for its tiles (530 bf16 keys 9.9 and 12.2), and
+ * units of a tile each stay apart (256 of 64 keys 16 and 21). */
+constexpr int PG_FEW_SHORT = 16;
+constexpr int pg_few_share(const pg_plan &p, int U, unsigned T) {
     const unsigned n = (unsigned)p.goal;
-    return pg_max((int)(T / n + (T % n != 0)), PG_FEW_LEAST);
+    return pg_max((int)(T / n + (T % n != 0)), T > PG_FEW_SHORT && T / 2 >= (unsigned)U ? 2 : 1);
 }
 /* PG_FEW: the slot of part j of a unit that begins in piece p0 and goes on after it.
  * A piece has at most two such parts: of a unit that came in from the piece before,
@@ -149,10 +151,12 @@ constexpr pg_plan pg_make_plan(int N, int B, int max_q, int max_kv, int G, int H
          * 65536 keys 42 us; 43 with 128 parts, 60 with 32). */
         p.goal = pg_max(1024 / Hkv, 1);
         p.goal = 64 * units < p.goal ? (int)(64 * units) : p.goal;
-        /* a line of at most units * most tiles, which are ints, in pieces of at
-         * least PG_FEW_LEAST */
-        const long long line = units * most, pieces = (line + PG_FEW_LEAST - 1) / PG_FEW_LEAST;
-        shares = line > 0x7fffffff ? PG_MOST : pieces < p.goal ? pieces : p.goal;
+        /* a line of at most units * most tiles, which are ints: pieces of two, or of
+         * one if there are no more than this of them */
+        const long long line = units * most, two = (line + 1) / 2;
+        const long long one = units > PG_FEW_SHORT / 2 ? 2 * units : PG_FEW_SHORT;
+        shares = two > one ? two : line < one ? line : one;
+        shares = line > 0x7fffffff ? PG_MOST : shares < p.goal ? shares : p.goal;
         slots = most > 1 ? 2 * shares : 0;
     } else {
         const long long by_rows = (long long)N * G / PG_MANY + B;

@@ -129,7 +129,7 @@ int main() {
         NEED(p.rt == (max_q * G <= 16 ? 16 : 128) && U <= p.units);
         if (p.rt == 16) {
             if (U == 0) continue;
-            const int size = pg_few_share(p, (unsigned)T);
+            const int size = pg_few_share(p, (int)U, (unsigned)T);
             int line = 0;
             std::vector<char> used(p.slots);
             for (int b = 0; b < B; b++) {
@@ -172,7 +172,7 @@ int main() {
         const pg_plan f = pg_make_plan(60, 60, 1, PG_MOST_KEYS, 16, 1, 0, 0);
         const pg_seq s = pg_clean_seq(0, 1, PG_MOST_KEYS, 60, 1, PG_MOST_KEYS);
         const int n = pg_longest(s, 16, 16, 0, 0);
-        const int size = pg_few_share(f, 60u * (unsigned)n);
+        const int size = pg_few_share(f, 60, 60u * (unsigned)n);
         NEED(f.shares > 0 && (60ll * n - 1) / size < f.shares);
         NEED((f.goal + 1ll) * size < 0x7fffffff); /* where a piece ends */
     }
