@@ -114,10 +114,6 @@ struct Call {
 DEV pg_seq seq_of(const Call &c, int b) {
     return load_seq(c.q_start, c.kv_len, b, c.N, c.max_q, c.max_kv);
 }
-DEV pg_seq seq_at(const pg_seq &s, int l) { /* lane l's */
-    auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-    return {of(s.q0), of(s.ql), of(s.kv), of(s.p0)};
-}
 DEV int page_id(const Call &c, int b, const pg_tiles &t, int i) {
     const int page = c.page_table[(size_t)b * c.max_pages + pg_tile_page(t, i)];
     return page >= 0 && page < c.num_pages ? page : -1;
@@ -129,29 +125,6 @@ DEV int lane_again() {
     asm volatile("" : "+v"(none));
     return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none));
 }
-/* f over the lanes with the same number in each of the wave's four rows of 16 */
-template <class F> DEV float fold_rows(float x, F f) {
-    const uint32_t u = __float_as_uint(x);
-    auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const uint32_t v = __float_as_uint(f(__uint_as_float(a[0]), __uint_as_float(a[1])));
-    a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return f(__uint_as_float(a[0]), __uint_as_float(a[1]));
-}
-/* Inclusive sum over the lanes below: 6 DPP adds (through LDS they took 6 trips) */
-template <int ctrl, int rows> DEV int dpp_or_0(int v) {
-    return __builtin_amdgcn_update_dpp(0, v, ctrl, rows, 0xf, true);
-}
-DEV int wave_scan(int v) {
-    v += dpp_or_0<0x111, 0xf>(v); /* row_shr 1, 2, 4, 8 */
-    v += dpp_or_0<0x112, 0xf>(v);
-    v += dpp_or_0<0x114, 0xf>(v);
-    v += dpp_or_0<0x118, 0xf>(v);
-    v += dpp_or_0<0x142, 0xa>(v); /* row_bcast 15, 31 */
-    v += dpp_or_0<0x143, 0xc>(v);
-    return v;
-}
-DEV int last_lane(int v) { return __builtin_amdgcn_readlane(v, 63); }
-
 /* The unit that share `target` of a kv-head belongs to (BY_PART; few rows: the one
  * that piece `target` begins in), or unit `target`: its sequence (b -1: there is
  * none), its number in it, its parts, the first one's number (few rows: its

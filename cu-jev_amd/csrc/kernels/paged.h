@@ -22,12 +22,62 @@ DEV pg_seq load_seq(const int32_t *q_start, const int32_t *kv_len, int b, int N,
     return pg_clean_seq(q_start[b], q_start[b + 1], kv_len[b], N, max_q, max_kv);
 }
 
+DEV pg_seq seq_at(const pg_seq &s, int l) { /* lane l's */
+    auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+    return {of(s.q0), of(s.ql), of(s.kv), of(s.p0)};
+}
+
+/* f over the lanes with the same number in each of the wave's four rows of 16 */
+template <class F> DEV float fold_rows(float x, F f) {
+    const uint32_t u = __float_as_uint(x);
+    auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t v = __float_as_uint(f(__uint_as_float(a[0]), __uint_as_float(a[1])));
+    a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+/* Inclusive sum over the lanes below: 6 DPP adds (through LDS they took 6 trips) */
+template <int ctrl, int rows> DEV int dpp_or_0(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, ctrl, rows, 0xf, true);
+}
+DEV int wave_scan(int v) {
+    v += dpp_or_0<0x111, 0xf>(v); /* row_shr 1, 2, 4, 8 */
+    v += dpp_or_0<0x112, 0xf>(v);
+    v += dpp_or_0<0x114, 0xf>(v);
+    v += dpp_or_0<0x118, 0xf>(v);
+    v += dpp_or_0<0x142, 0xa>(v); /* row_bcast 15, 31 */
+    v += dpp_or_0<0x143, 0xc>(v);
+    return v;
+}
+DEV int last_lane(int v) { return __builtin_amdgcn_readlane(v, 63); }
+/* f over the lanes of each row of 16, then of the wave, in the order of a butterfly
+ * from 32 down to 1 (a rotation by o meets what lane ^ o has, once the rows' larger
+ * strides are done) */
+template <int ctrl> DEV float dpp(float x) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(
+        0, (int)__float_as_uint(x), ctrl, 0xf, 0xf, true));
+}
+template <class F> DEV float fold_wave(float x, F f) {
+    const uint32_t u = __float_as_uint(x);
+    auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t v = __float_as_uint(f(__uint_as_float(a[0]), __uint_as_float(a[1])));
+    a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    x = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    x = f(x, dpp<0x128>(x)); /* row_ror 8, 4, 2, 1 */
+    x = f(x, dpp<0x124>(x));
+    x = f(x, dpp<0x122>(x));
+    return f(x, dpp<0x121>(x));
+}
+
 /* The sequences of rows n0 .. n0 + TOK - 1, row n0 + t in lane t: the last b
  * with q_start[b] <= n, -1 for a row before the first or behind the last
- * sequence. One load of 64 starts a step. */
-template <int TOK> DEV int find_seqs(const int32_t *q_start, int B, int n0) {
+ * sequence. One load of 64 starts a step; up to 64 sequences' lengths come
+ * beside them and not after. */
+template <int TOK>
+DEV int find_seqs(const int32_t *q_start, const int32_t *kv_len, int B, int N, int max_kv, int n0,
+                  pg_seq *s) {
     const int lane = threadIdx.x & 63;
     int before[TOK] = {}; /* starts <= n among q_start[0 .. B] */
+    const pg_seq mine = load_seq(q_start, kv_len, min(lane, B - 1), N, N, max_kv);
     for (int b0 = 0; b0 <= B; b0 += 64) {
         const int v = q_start[min(b0 + lane, B)];
         int c = 0;
@@ -43,7 +93,13 @@ template <int TOK> DEV int find_seqs(const int32_t *q_start, int B, int n0) {
 #pragma unroll
     for (int t = 1; t < TOK; t++)
         b = lane == t ? before[t] : b;
-    return b == 0 || b > B ? -1 : b - 1;
+    b = b > B ? -1 : b - 1;
+    const int l = max(b, 0) & 63; /* outside a branch: its loads stay with the starts' */
+    *s = {__shfl(mine.q0, l, 64), __shfl(mine.ql, l, 64), __shfl(mine.kv, l, 64),
+          __shfl(mine.p0, l, 64)};
+    if (B > 64)
+        *s = load_seq(q_start, kv_len, max(b, 0), N, N, max_kv);
+    return b;
 }
 
 /* Work item `item` of a launch whose sequence b has count(b, s) of them, in
@@ -54,26 +110,18 @@ DEV int find_item(const int32_t *q_start, const int32_t *kv_len, int B, int N, i
     const int lane = threadIdx.x & 63;
     int before = 0;
     for (int b0 = 0; b0 < B; b0 += 64) {
-        const int b = min(b0 + lane, B - 1);
-        const pg_seq mine = load_seq(q_start, kv_len, b, N, max_q, max_kv);
+        const pg_seq mine =
+            load_seq(q_start, kv_len, min(b0 + lane, B - 1), N, max_q, max_kv);
         const int own = b0 + lane < B ? count(mine) : 0;
-        int sum = own; /* inclusive sum over the lanes */
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(sum, o, 64);
-            sum += lane >= o ? v : 0;
-        }
-        const uint64_t past = __ballot(before + sum > item);
+        const int sum = before + wave_scan(own);
+        const uint64_t past = __ballot(sum > item);
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
-            s->q0 = __builtin_amdgcn_readlane(mine.q0, l);
-            s->ql = __builtin_amdgcn_readlane(mine.ql, l);
-            s->kv = __builtin_amdgcn_readlane(mine.kv, l);
-            s->p0 = __builtin_amdgcn_readlane(mine.p0, l);
-            *local = item - before - __builtin_amdgcn_readlane(sum - own, l);
+            *s = seq_at(mine, l);
+            *local = item - __builtin_amdgcn_readlane(sum - own, l);
             return b0 + l;
         }
-        before += __builtin_amdgcn_readlane(sum, 63);
+        before = last_lane(sum);
     }
     return -1;
 }

@@ -15,7 +15,8 @@ namespace {
  * A V wave takes the tokens of one aligned group of 16 positions and one
  * kv-head: the group's V^T rows are whole 16-byte (e4m3) or 32-byte pieces, so
  * the transpose needs neither LDS nor another wave's data: lane l holds 16
- * tokens of dims 4l .. 4l + 3 and stores one piece per dim. */
+ * tokens of dims 4l .. 4l + 3 and stores one piece per dim. A workgroup's four
+ * are a page's, whose lines of V^T they fill together in one L2. */
 template <bool E4M3, int TOK>
 __global__ __launch_bounds__(256) void prep_paged_kernel(
     const bf16 *__restrict__ proj, int ps, const float *__restrict__ qw,
@@ -24,7 +25,7 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(
     const int32_t *__restrict__ page_table, int max_pages, int B, int N, int Hq, int Hkv, int rot,
     const float2 *__restrict__ rope, int npos, float eps, float q_scale, bf16 *__restrict__ q_out,
     void *__restrict__ k_pages, void *__restrict__ vt_pages, float *__restrict__ k_scale,
-    float *__restrict__ v_scale, int num_pages, int row_blocks, int groups) {
+    float *__restrict__ v_scale, int num_pages, int row_blocks) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     if ((int)blockIdx.x < row_blocks) {
         const int heads = Hq + Hkv, unit = blockIdx.x * 4 + wave;
@@ -46,20 +47,22 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(
         const int pos_lane = min(max(pos[min(n0 + (lane & (TOK - 1)), N - 1)], 0), npos - 1);
         /* The tokens' sequences, then (K) their slots, token t in lane t: one
          * chain of loads for all of them. at: the K row in the pool, -1: none */
-        int b = find_seqs<TOK>(q_start, B, n0);
-        float4 rc[TOK][2];
+        pg_seq s;
+        int b = find_seqs<TOK>(q_start, kv_len, B, N, max_pages * PG, n0, &s);
+        float4 rc[TOK][2] = {};
+        if (rotates) { /* 16 lanes' loads or fewer: by all 64 they cost more than x's */
 #pragma unroll
-        for (int t = 0; t < TOK; t++) {
-            const float4 *r = (const float4 *)(
-                rope + (size_t)__builtin_amdgcn_readlane(pos_lane, t) * (rot / 2) + fi0);
-            rc[t][0] = r[0];
-            rc[t][1] = r[1];
+            for (int t = 0; t < TOK; t++) {
+                const float4 *r = (const float4 *)(
+                    rope + (size_t)__builtin_amdgcn_readlane(pos_lane, t) * (rot / 2) + fi0);
+                rc[t][0] = r[0];
+                rc[t][1] = r[1];
+            }
         }
         if (n0 + lane >= N)
             b = -1;
         long long at = b;
         if (is_k) {
-            const pg_seq s = load_seq(q_start, kv_len, max(b, 0), N, N, max_pages * PG);
             const int p = s.p0 + (n0 + lane - s.q0);
             const bool in = b >= 0 && (unsigned)(n0 + lane - s.q0) < (unsigned)s.ql && p >= 0 &&
                             p < s.kv;
@@ -79,10 +82,8 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(
             }
         }
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1)
-#pragma unroll
-            for (int t = 0; t < TOK; t++)
-                ss[t] += __shfl_xor(ss[t], o, 64);
+        for (int t = 0; t < TOK; t++)
+            ss[t] = fold_wave(ss[t], [](float p, float q) { return p + q; });
         const float we[4] = {wl.x, wl.y, wl.z, wl.w};
         float amax[TOK];
 #pragma unroll
@@ -102,10 +103,8 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(
         }
         if (E4M3 && is_k) {
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1)
-#pragma unroll
-                for (int t = 0; t < TOK; t++)
-                    amax[t] = fmaxf(amax[t], __shfl_xor(amax[t], o, 64));
+            for (int t = 0; t < TOK; t++)
+                amax[t] = fold_wave(amax[t], [](float p, float q) { return fmaxf(p, q); });
         }
 #pragma unroll
         for (int t = 0; t < TOK; t++) {
@@ -134,19 +133,19 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(
     }
 
     /* ---- V ---- */
-    const int unit = (blockIdx.x - row_blocks) * 4 + wave;
-    if (unit >= groups * Hkv)
-        return;
-    const int kh = unit % Hkv;
+    const int unit = blockIdx.x - row_blocks, kh = unit % Hkv;
     pg_seq s;
-    int g;
+    int i;
     const int b = find_item(
         q_start, kv_len, B, N, N, max_pages * PG, unit / Hkv,
-        [](const pg_seq &q) { return pg_v_groups(q); }, &s, &g);
+        [](const pg_seq &q) { return pg_v_pages(q); }, &s, &i);
     if (b < 0)
         return;
-    const int base = (pg_new_lo(s) / VTOK + g) * VTOK; /* the group's first position */
-    const int page = page_table[(size_t)b * max_pages + base / PG];
+    const int at = pg_new_lo(s) / PG + i;          /* the page's number in the sequence */
+    const int base = at * PG + wave * VTOK; /* the group's first position */
+    if (base + VTOK <= pg_new_lo(s) || base >= pg_new_hi(s))
+        return;
+    const int page = page_table[(size_t)b * max_pages + at];
     const int lo = max(pg_new_lo(s), base), hi = min(pg_new_hi(s), base + VTOK);
     const bf16 *src = proj + Hq * 512 + Hkv * 256 + kh * 256 + 4 * lane;
     bf16x4 v[VTOK];
@@ -169,17 +168,26 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(
         for (int t = 0; t < VTOK; t++)
             m[t] = fmaxf(fmaxf(fabsf(bf2f(v[t][0])), fabsf(bf2f(v[t][1]))),
                          fmaxf(fabsf(bf2f(v[t][2])), fabsf(bf2f(v[t][3]))));
+        auto meet = [](float p, float q, bool rows32) {
+            const auto a = rows32 ? __builtin_amdgcn_permlane32_swap(__float_as_uint(p),
+                                                                     __float_as_uint(q), false, false)
+                                  : __builtin_amdgcn_permlane16_swap(__float_as_uint(p),
+                                                                     __float_as_uint(q), false, false);
+            return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+        };
 #pragma unroll
-        for (int half = VTOK / 2, o = 32; half >= 1; half >>= 1, o >>= 1) {
-            const bool upper = lane & o;
+        for (int t = 0; t < 8; t++)
+            m[t] = meet(m[t], m[t + 8], true);
 #pragma unroll
-            for (int t = 0; t < half; t++) {
-                const float mine = upper ? m[t + half] : m[t], give = upper ? m[t] : m[t + half];
-                m[t] = fmaxf(mine, __shfl_xor(give, o, 64));
-            }
-        }
-        m[0] = fmaxf(m[0], __shfl_xor(m[0], 2, 64));
-        m[0] = fmaxf(m[0], __shfl_xor(m[0], 1, 64));
+        for (int t = 0; t < 4; t++)
+            m[t] = meet(m[t], m[t + 4], false);
+#pragma unroll
+        for (int t = 0; t < 2; t++) /* row_ror 8 */
+            m[t] = fmaxf(lane & 8 ? m[t + 2] : m[t], dpp<0x128>(lane & 8 ? m[t] : m[t + 2]));
+        /* row_half_mirror: lane ^ 7, in the other four as lane ^ 4 is */
+        m[0] = fmaxf(lane & 4 ? m[1] : m[0], dpp<0x141>(lane & 4 ? m[0] : m[1]));
+        m[0] = fmaxf(m[0], dpp<0x4e>(m[0])); /* quad_perm, lane ^ 2, lane ^ 1 */
+        m[0] = fmaxf(m[0], dpp<0xb1>(m[0]));
         const int e = e4m3_exp(m[0]), tok = lane >> 2;
         if ((lane & 3) == 0 && base + tok >= lo && base + tok < hi)
             v_scale[head * PG + col + tok] = exp2_int(e);
@@ -340,9 +348,9 @@ extern "C" hipError_t k_attn_prep_paged(const bf16_t *proj, int proj_stride, con
     if (N <= 0 || B <= 0)
         return hipSuccess;
     const long long units = (long long)CEIL_DIV(N, 4) * (Hq + Hkv);
-    const long long groups = N < N / VTOK + 2ll * B ? N : N / VTOK + 2ll * B;
-    const long long row_blocks = CEIL_DIV(units, 4), v_blocks = CEIL_DIV(groups * Hkv, 4);
-    if (row_blocks + v_blocks > 0x7fffffff || groups * Hkv > 0x7fffffff)
+    const long long v_pages = N < N / PG + 2ll * B ? N : N / PG + 2ll * B;
+    const long long row_blocks = CEIL_DIV(units, 4), v_blocks = v_pages * Hkv;
+    if (row_blocks + v_blocks > 0x7fffffff)
         return hipErrorInvalidValue;
 #define LAUNCH(T)                                                                                 \
     hipLaunchKernelGGL((prep_paged_kernel<T, 4>), dim3((unsigned)(row_blocks + v_blocks)),        \
@@ -350,7 +358,7 @@ extern "C" hipError_t k_attn_prep_paged(const bf16_t *proj, int proj_stride, con
                        pos, seqs->q_start, seqs->kv_len, seqs->page_table, seqs->max_pages, B, N, \
                        Hq, Hkv, rot, (const float2 *)rope_table, npos, eps, q_scale,              \
                        (bf16 *)q_out, pages->k, pages->vt, pages->k_scale, pages->v_scale,        \
-                       pages->num_pages, (int)row_blocks, (int)groups)
+                       pages->num_pages, (int)row_blocks)
     if (pages->type == CUJEV_KV_E4M3)
         LAUNCH(true);
     else

@@ -35,11 +35,10 @@ constexpr pg_seq pg_clean_seq(int q0, int q1, int kv, int N, int max_q, int max_
 /* The positions [lo, hi) of the new tokens that have a slot */
 constexpr int pg_new_lo(const pg_seq &s) { return pg_max(s.p0, 0); }
 constexpr int pg_new_hi(const pg_seq &s) { return pg_min(s.p0 + s.ql, s.kv); }
-/* Aligned groups of VTOK positions that the new tokens touch; a call has at
- * most min(N, N / VTOK + 2 B) of them. */
-constexpr int pg_v_groups(const pg_seq &s) {
+/* Pages that the new tokens touch; a call has at most min(N, N / PG + 2 B) of them. */
+constexpr int pg_v_pages(const pg_seq &s) {
     const int lo = pg_new_lo(s), hi = pg_new_hi(s);
-    return hi > lo ? (hi - 1) / VTOK - lo / VTOK + 1 : 0;
+    return hi > lo ? (hi - 1) / PG - lo / PG + 1 : 0;
 }
 
 /* Key tiles that the new tokens i0 .. i1 of a sequence visit, in order: the

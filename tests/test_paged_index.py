@@ -85,11 +85,12 @@ int main() {
         for (int b = 0; b < B; b++) {
             const pg_seq s = pg_clean_seq(at, at + q[b], kv[b], N, N, 160);
             at += q[b];
-            const int n = pg_v_groups(s);
+            const int n = pg_v_pages(s);
             groups += n;
             std::set<int> seen;
-            for (int g = 0; g < n; g++) {
-                const int base = (pg_new_lo(s) / VTOK + g) * VTOK;
+            for (int i = 0; i < 4 * n; i++) { /* a page's four groups of positions */
+                const int base = (pg_new_lo(s) / PG + i / 4) * PG + i % 4 * VTOK;
+                if (base + VTOK <= pg_new_lo(s) || base >= pg_new_hi(s)) continue;
                 const int lo = pg_max(pg_new_lo(s), base), hi = pg_min(pg_new_hi(s), base + VTOK);
                 NEED(lo < hi && base % PG + VTOK <= PG && base < s.kv);
                 for (int p = lo; p < hi; p++) {
@@ -100,7 +101,7 @@ int main() {
             }
             NEED((int)seen.size() == pg_max(pg_new_hi(s) - pg_new_lo(s), 0));
         }
-        NEED(groups <= (N < N / VTOK + 2 * B ? N : N / VTOK + 2 * B));
+        NEED(groups <= (N < N / PG + 2 * B ? N : N / PG + 2 * B));
     }
     /* the plan: shares tile each unit's list, and the launch and slots hold them */
     for (int it = 0; it < 30000; it++) {
