@@ -106,7 +106,7 @@ struct Call {
     int num_pages;
     const int32_t *q_start, *kv_len, *page_table;
     int max_pages, B, N, max_q, max_kv, Hq, Hkv, G, window, sinks;
-    int rG; /* r / G = r * rG >> 8 for r < 16: a division kept a register and more */
+    int rG; /* r / G = r * rG >> 16 for r < 4096 (an integer division is 30 instructions) */
     bf16 *out;
     float *po, *pl, *pmu;
     pg_plan plan;
@@ -252,7 +252,7 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
     int ids = i0 < i1 ? page_id(c, b, list, min(i0 + lane, list.ntl - 1)) : -1, ids0 = i0;
 
     /* this lane's row (column of S^T and O^T) */
-    const int row = min(m, rows - 1), tok = row * c.rG >> 8, head = kh * c.G + row - tok * c.G;
+    const int row = min(m, rows - 1), tok = row * c.rG >> 16, head = kh * c.G + row - tok * c.G;
     const int hi = min(s.p0 + tok, s.kv - 1), lo = pg_low(s.p0 + tok, c.window);
     const int own_lo = pg_low(s.p0, c.window); /* of the first row: below, no row's key */
     bf16x8 *const qf = sq + lane;
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
         }
     } else if (r < rows) {
         const float inv = lrun > 0.f ? 1.f / lrun : 0.f;
-        const int tk = r * c.rG >> 8, n = s.q0 + tk, hd = kh * c.G + r - tk * c.G;
+        const int tk = r * c.rG >> 16, n = s.q0 + tk, hd = kh * c.G + r - tk * c.G;
         bf16x4 gv[16] = {};
         if (c.gate) {
             const bf16 *gp = c.gate + (size_t)n * c.gts + (size_t)hd * c.ghs + d0;
@@ -536,8 +536,12 @@ template <bool E4M3> struct Lay {
     static constexpr int V = 0, K = 2 * T, P = 4 * T, PBUF = 16384, SC = P + 2 * PBUF;
     /* e4m3: K scales of two tiles, V scales of four (read a tile later) */
     static constexpr int TILES = SC + (E4M3 ? 2 * 256 + 4 * 256 : 0);
+    /* Q on its way to registers, 64 rows each: in P, and in V^T's second buffer (e4m3:
+     * behind the scales) */
+    static constexpr int Q0 = P, Q1 = E4M3 ? TILES : V + T, QEND = Q1 + RT / 2 * PD * 2;
     static constexpr int STAT = RT * PD * 4; /* l behind the staged O */
-    static constexpr int BYTES = TILES > STAT + RT * 8 ? TILES : STAT + RT * 8;
+    static constexpr int ALL = TILES > QEND ? TILES : QEND;
+    static constexpr int BYTES = ALL > STAT + RT * 8 ? ALL : STAT + RT * 8;
 };
 static_assert(Lay<false>::BYTES <= 163840 && Lay<true>::BYTES <= 163840, "LDS of a CU");
 
@@ -581,7 +585,7 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
     const pg_seq s = w.s;
     const int b = w.b, nshare = w.parts, share = w.part;
     const int r0 = w.unit * RT, nrows = min(s.ql * c.G - r0, RT);
-    const int i0 = r0 / c.G, i1 = (r0 + nrows - 1) / c.G;
+    const int i0 = r0 / c.G, rest = r0 - i0 * c.G, i1 = i0 + ((rest + nrows - 1) * c.rG >> 16);
     const pg_tiles list = pg_tile_list(s, i0, i1, c.window, c.sinks);
     const int tb = pg_share_begin(list.ntl, share, nshare);
     const int ntl = pg_share_begin(list.ntl, share + 1, nshare) - tb;
@@ -590,19 +594,17 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int wi = wave & 3, wj = wave >> 2, h = lane >> 5, col = lane & 31;
 
-    /* Q^T operands of this wave's 32 rows; rows past the last repeat it */
-    bf16x8 qf[16];
-    int hi, lo;
+    /* page ids of the list, 64 entries in a lane each; the first ahead of Q's loads,
+     * which a wait for them would wait for too */
+    int ids = 0;
+    if (ntl > 0)
+        ids = page_id(c, b, list, min(tb + lane, list.ntl - 1));
+
+    int hi, lo; /* of this lane's row; rows past the last repeat it */
     {
-        const int r = r0 + min(32 * wi + col, nrows - 1);
-        const int tok = r / c.G, head = kh * c.G + r % c.G;
+        const int tok = i0 + ((rest + min(32 * wi + col, nrows - 1)) * c.rG >> 16);
         hi = min(s.p0 + tok, s.kv - 1);
         lo = pg_low(s.p0 + tok, c.window);
-        const bf16 *qp = c.q + ((size_t)(s.q0 + tok) * c.Hq + head) * PD;
-#pragma unroll
-        for (int ks = 0; ks < 16; ks++)
-            qf[ks] = *(const bf16x8 *)(qp + (E4M3 ? 32 * (ks >> 1) + 16 * h + 8 * (ks & 1)
-                                                  : 16 * ks + 8 * h));
     }
     const int pmin = s.p0 + i0, pmax = s.p0 + i1;
 
@@ -648,8 +650,27 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
         }
     };
 
-    /* ---- per-lane LDS read addresses ---- */
+    /* Q through LDS, as whole rows: lane by lane each load touched 32 lines, which
+     * took 3 us. Wave (i, j) brings half j of the rows of quarter i, two a load;
+     * piece p of row r lies in slot p ^ (r & 15). */
     lds_u8 *lds = (lds_u8 *)smem;
+    const uint32_t qat = (wi & 2 ? L::Q1 : L::Q0) + (wi & 1) * 16384;
+    auto issue_q = [&]() {
+        const __amdgpu_buffer_rsrc_t r =
+            make_rsrc(c.q + ((size_t)(s.q0 + i0) * c.Hq + kh * c.G) * PD, 0x7fffffff);
+#pragma unroll
+        for (int n = 0; n < 8; n++) {
+            const int at = 16 * wj + 2 * n + h, row = rest + min(32 * wi + at, nrows - 1);
+            const int tok = row * c.rG >> 16; /* after i0 */
+            const uint32_t off = (tok * c.Hq + row - tok * c.G) * PD * 2;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                r, (lds_ptr)(smem + qat + (16 * wj + 2 * n) * 512), 16,
+                off + ((col ^ (at & 15)) << 4), 0, 0, 0);
+        }
+    };
+    bf16x8 qf[16]; /* Q^T operands of this wave's 32 rows */
+
+    /* ---- per-lane LDS read addresses ---- */
     const int arow = perm_row<E4M3>(col);
     uint32_t ka[8];
 #pragma unroll
@@ -670,10 +691,8 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
     const uint32_t psend = L::P + wave * 2048 + lane * 16;
     const uint32_t precv = L::P + (wave ^ 4) * 2048 + lane * 16;
 
-    /* page ids of the list, 64 entries in a lane each */
-    int ids = 0;
     auto page_of = [&](int t) { /* called with t = 0, 1, 2, ... < ntl */
-        if ((t & 63) == 0)
+        if ((t & 63) == 0 && t > 0)
             ids = page_id(c, b, list, min(tb + t + lane, list.ntl - 1));
         return __builtin_amdgcn_readlane(ids, t & 63);
     };
@@ -966,14 +985,23 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
         for (int n = 0; n < NL; n++)
             issue_k(k_0, 0, n);
         issue_scales(pg[0], 0);
+        issue_q();
 #pragma unroll
         for (int n = 0; n < NL; n++) {
             issue_k(k_1, 1, n);
             issue_v(v_0, 0, n);
         }
         issue_scales(pg[1], 1);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
+        /* Q and K of tile 0; what was issued after them is at least 2 NL loads */
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NL) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int ks = 0; ks < 16; ks++) {
+            const int piece = E4M3 ? 4 * (ks >> 1) + 2 * h + (ks & 1) : 2 * ks + h;
+            qf[ks] = __builtin_bit_cast(
+                bf16x8, lds_read16(lds, qat + col * 512 + ((piece ^ (col & 15)) << 4)));
+        }
         ksc = kscale(0);
         unroll_for<2>([&](auto ib) { /* operands of 8 k-steps at a time */
             constexpr int part = decltype(ib)::value;
@@ -1001,11 +1029,14 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
             mx = fmaxf(mx, xa[v]);
         unroll_for<4>([&](auto iv) { pair(xa, pn, template_int<2 * decltype(iv)::value>{}, 0.f); });
         want();
+        /* K of tile 1 is there, and K buffer 0 free */
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
         ksc = kscale(1);
 #pragma unroll
         for (int n = 0; n < QD; n++)
             ring[n] = lds_read16(lds, kaddr(n, 1));
-        __syncthreads(); /* K buffer 0 is free */
         const __amdgpu_buffer_rsrc_t k_2 = k_rsrc(pg[2]);
 #pragma unroll
         for (int n = 0; n < NL; n++)
@@ -1031,7 +1062,8 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
     const int t0 = 16 * wave;
     size_t gat, oat;
     {
-        const int r = r0 + min(t0 + (lane & 15), nrows - 1), tok = r / c.G, hd = r % c.G;
+        const int r = rest + min(t0 + (lane & 15), nrows - 1), after = r * c.rG >> 16;
+        const int tok = i0 + after, hd = r - after * c.G;
         gat = (size_t)(s.q0 + tok) * c.gts + (size_t)(kh * c.G + hd) * c.ghs;
         oat = whole ? ((size_t)(s.q0 + tok) * c.Hq + kh * c.G + hd) * PD
                     : (slot * RT + t0 + (lane & 15)) * PD;
@@ -1071,20 +1103,28 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
     }
     __syncthreads();
 #pragma unroll
-    for (int t = 0; t < 16; t++) {
-        if (t0 + t >= nrows)
-            break;
-        const floatx4 v = *(const floatx4 *)(smem + (t0 + t) * 1024 +
-                                             ((lane ^ ((t0 + t) & 31)) << 4));
-        if (!whole) {
-            *(floatx4 *)(c.po + of_row(oat, t) + 4 * lane) = v;
-            continue;
-        }
-        bf16x4 res;
+    for (int half = 0; half < 2; half++) { /* no branch between the reads */
+        floatx4 v[8];
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            res[e] = f2bf(gated ? v[e] * sigmoid_f(bf2f(gv[t][e])) : v[e]);
-        *(bf16x4 *)(c.out + of_row(oat, t) + 4 * lane) = res;
+        for (int i = 0; i < 8; i++) {
+            const int row = t0 + 8 * half + i;
+            v[i] = *(const floatx4 *)(smem + row * 1024 + ((lane ^ (row & 31)) << 4));
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int t = 8 * half + i;
+            if (!whole) {
+                if (t0 + t < nrows)
+                    *(floatx4 *)(c.po + of_row(oat, t) + 4 * lane) = v[i];
+                continue;
+            }
+            bf16x4 res;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                res[e] = f2bf(gated ? v[i][e] * sigmoid_f(bf2f(gv[t][e])) : v[i][e]);
+            if (t0 + t < nrows)
+                *(bf16x4 *)(c.out + of_row(oat, t) + 4 * lane) = res;
+        }
     }
 }
 
@@ -1202,7 +1242,7 @@ extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int
                     pages->k, pages->vt, pages->k_scale, pages->v_scale, pages->num_pages,
                     seqs->q_start, seqs->kv_len, seqs->page_table, seqs->max_pages, B, N,
                     max_q, max_kv, Hq, Hkv, G, window, sinks,
-                    pg_div_up(256, G), (bf16 *)out,
+                    pg_div_up(65536, G), (bf16 *)out,
                     (float *)ws, (float *)ws + rows * PD, (float *)ws + rows * (PD + 1), p};
     const bool few = p.rt == FEW;
     const int per = !few && 8 % Hkv == 0 ? 8 / Hkv : 1;

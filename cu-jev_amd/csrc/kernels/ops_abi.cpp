@@ -387,7 +387,7 @@ EXPORT int cujev_op_attention_paged(const void *q, const void *gate, int gate_to
     const int st = paged_check("attention_paged", &pages, page_table, max_pages, kv_len, B);
     if (st != 0)
         return st;
-    if (N < 0 || N > PG_MOST || max_q < 0 || max_kv < 0 || !paged_heads_ok(Hq, Hkv))
+    if (N < 0 || N > PG_MOST || max_q < 0 || max_kv < 0 || !paged_heads_ok(Hq, Hkv) || Hq > 8192)
         return fail(1, "attention_paged: unsupported shape N=%d max_q=%d max_kv=%d Hq=%d Hkv=%d",
                     N, max_q, max_kv, Hq, Hkv);
     if (max_kv > max_pages * CUJEV_KV_PAGE)
