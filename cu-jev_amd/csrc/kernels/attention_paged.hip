@@ -1130,83 +1130,153 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
 
 /* ---- merge of a unit's parts -----------------------------------------------------
  * o = sum 2^(mu_i - mu) o_i over the parts that saw keys, l likewise, mu the largest
- * of theirs; then / l and the gate. l and mu come in one load, lane i: part i.
- * A wave per row (4 rows in turn of many), o 16 parts at a time; or, ROW, a
- * workgroup: a wave 64 dims, o 64 parts at a time, 4 a load. That is for
- * few rows after many keys (4 rows of 64 parts: 5.4 us, and 8.8 a wave per row); the
- * starts of many workgroups cost more than it gains (1024 rows of 4 parts: 5.6 and
- * 4.8, 4096 of them 22 and 8). */
-template <int ROWS, bool ROW>
-__global__ __launch_bounds__(256) void merge_kernel(Call c, int groups) {
-    constexpr int EACH = ROWS == FEW ? 1 : 4; /* rows a wave */
+ * of theirs; then / l and the gate. The loads of l and mu, a part a lane, and of the
+ * first o go out together. */
+
+/* Of few rows: a wave per row, o 16 parts at a time; or, ROW, a workgroup: a wave 64
+ * dims, o 64 parts at a time, 4 a load. That is for few rows after many keys (4 rows
+ * of 64 parts: 5.4 us, and 8.8 a wave per row); the starts of many workgroups cost
+ * more than it gains (1024 rows of 4 parts: 5.6 and 4.8, 4096 of them 22 and 8). */
+template <bool ROW> __global__ __launch_bounds__(256) void merge_few_kernel(Call c, int groups) {
     constexpr int STEP = ROW ? 64 : 16, PER = STEP / 16;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int group = blockIdx.x % groups, kh = blockIdx.x / groups % c.Hkv;
-    const Where w = locate<ROWS, false>(c, blockIdx.x / groups / c.Hkv);
-    if (w.b < 0 || w.parts <= 1)
+    const Where w = locate<FEW, false>(c, blockIdx.x / groups / c.Hkv);
+    const int r = ROW ? group : group * 4 + wave;
+    if (w.b < 0 || w.parts <= 1 || r >= w.s.ql * c.G)
         return;
-    const size_t slot0 = slot_of(c, kh, ROWS == FEW ? 0 : w.first);
-    auto slot = [&](int j) { return slot0 + (ROWS == FEW ? pg_few_slot(w.first, j) : j); };
-    const int nrows = min(w.s.ql * c.G - w.unit * ROWS, ROWS);
+    const size_t slot0 = slot_of(c, kh, 0);
+    auto at = [&](int j) { return (slot0 + pg_few_slot(w.first, j)) * FEW + r; };
     const int dim = ROW ? 64 * wave + 4 * (lane & 15) : 4 * lane, own = ROW ? lane >> 4 : 0;
-#pragma unroll 1
-    for (int i = 0; i < EACH; i++) {
-        const int t = ROW ? group : (group * 4 + wave) * EACH + i;
-        if (t >= nrows)
-            return;
-        const int r = w.unit * ROWS + t, n = w.s.q0 + r / c.G, head = kh * c.G + r % c.G;
-        bf16x4 gv = {};
-        if (c.gate)
-            gv = *(const bf16x4 *)(c.gate + (size_t)n * c.gts + (size_t)head * c.ghs + dim);
-        float mu = -INFINITY, l = 0.f;
-        floatx4 acc = {};
-        for (int j0 = 0; j0 < w.parts; j0 += 64) { /* more than 64 parts: in turns */
-            const int cnt = min(w.parts - j0, 64);
-            const size_t mine = slot(j0 + min(lane, cnt - 1)) * ROWS + t;
-            const float pl = c.pl[mine], pm = c.pmu[mine];
-            const float li = lane < cnt ? pl : 0.f, mi = li > 0.f ? pm : -INFINITY;
-            float wi = 0.f;
-            for (int k0 = 0; k0 < cnt; k0 += STEP) {
-                floatx4 v[16];
+    const int tok = r * c.rG >> 16, n = w.s.q0 + tok, head = kh * c.G + r - tok * c.G;
+    bf16x4 gv = {};
+    if (c.gate)
+        gv = *(const bf16x4 *)(c.gate + (size_t)n * c.gts + (size_t)head * c.ghs + dim);
+    float mu = -INFINITY, l = 0.f;
+    floatx4 acc = {};
+    for (int j0 = 0; j0 < w.parts; j0 += 64) { /* more than 64 parts: in turns */
+        const int cnt = min(w.parts - j0, 64);
+        const size_t mine = at(j0 + min(lane, cnt - 1));
+        const float pl = c.pl[mine], pm = c.pmu[mine];
+        const float li = lane < cnt ? pl : 0.f, mi = li > 0.f ? pm : -INFINITY;
+        float wi = 0.f;
+        for (int k0 = 0; k0 < cnt; k0 += STEP) {
+            floatx4 v[16];
 #pragma unroll
-                for (int k = 0; k < 16; k++)
-                    if (k0 + k * PER < cnt) { /* uniform */
-                        const int j = j0 + min(k0 + k * PER + own, cnt - 1);
-                        v[k] = *(const floatx4 *)(c.po + (slot(j) * ROWS + t) * PD + dim);
-                    }
-                if (k0 == 0) { /* with the first o on their way */
-                    const float next = fmaxf(mu, wave_max(mi));
-                    const float ref = next == -INFINITY ? 0.f : next, old = fast_exp2(mu - ref);
-                    wi = li > 0.f ? fast_exp2(mi - ref) : 0.f;
-                    mu = next;
-                    l = l * old + wave_sum(wi * li);
-                    acc *= old;
-                }
+            for (int k = 0; k < 16; k++)
+                if (k0 + k * PER < cnt) /* uniform */
+                    v[k] = *(const floatx4 *)(c.po + at(j0 + min(k0 + k * PER + own, cnt - 1)) * PD +
+                                              dim);
+            if (k0 == 0) {
+                const float next = fmaxf(mu, wave_max(mi));
+                const float ref = next == -INFINITY ? 0.f : next, old = fast_exp2(mu - ref);
+                wi = li > 0.f ? fast_exp2(mi - ref) : 0.f;
+                mu = next;
+                l = l * old + wave_sum(wi * li);
+                acc *= old;
+            }
 #pragma unroll
-                for (int k = 0; k < 16; k++) {
-                    if (k0 + k * PER >= cnt)
-                        break;
-                    /* lanes from cnt on have weight 0 */
-                    const float f = ROW ? __shfl(wi, k * PER + own, 64)
-                                        : __uint_as_float((uint32_t)__builtin_amdgcn_readlane(
-                                              (int)__float_as_uint(wi), k0 + k));
-                    if (f > 0.f)
-                        acc += v[k] * f;
-                }
+            for (int k = 0; k < 16; k++) {
+                if (k0 + k * PER >= cnt)
+                    break;
+                /* lanes from cnt on have weight 0 */
+                const float f = ROW ? __shfl(wi, k * PER + own, 64)
+                                    : __uint_as_float((uint32_t)__builtin_amdgcn_readlane(
+                                          (int)__float_as_uint(wi), k0 + k));
+                if (f > 0.f)
+                    acc += v[k] * f;
             }
         }
-        if constexpr (ROW) {
+    }
+    if constexpr (ROW) {
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                acc[e] = fold_rows(acc[e], [](float x, float y) { return x + y; });
+        for (int e = 0; e < 4; e++)
+            acc[e] = fold_rows(acc[e], [](float x, float y) { return x + y; });
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    bf16x4 res;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        res[e] = f2bf(acc[e] * inv * (c.gate ? sigmoid_f(bf2f(gv[e])) : 1.f));
+    if (!ROW || lane < 16)
+        *(bf16x4 *)(c.out + ((size_t)n * c.Hq + head) * PD + dim) = res;
+}
+
+/* Of many rows: a wave 4 rows, all at once (one after the other took 11.2 us instead
+ * of 9.6 for 16 sequences' 40 tokens in 2 or 3 parts). l and mu: lane 16 i + j has row
+ * i's of part j, 16 parts in turn; o 4 parts at a time. */
+__global__ __launch_bounds__(256) void merge_many_kernel(Call c) {
+    constexpr int R = 4, GROUPS = RT / (4 * R);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int group = blockIdx.x % GROUPS, kh = blockIdx.x / GROUPS % c.Hkv;
+    const Where w = locate<RT, false>(c, blockIdx.x / GROUPS / c.Hkv);
+    const int r0 = w.unit * RT, t0 = (group * 4 + wave) * R;
+    if (w.b < 0 || w.parts <= 1 || t0 >= min(w.s.ql * c.G - r0, RT))
+        return;
+    const int last = min(w.s.ql * c.G - r0, RT) - 1;
+    const float *po[R]; /* part 0 of a row's o; past the last row it again */
+    bf16 *out[R];
+    bf16x4 gv[R] = {};
+    const size_t slot = slot_of(c, kh, w.first);
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        const int t = min(t0 + i, last), r = r0 + t, tok = r / c.G, head = kh * c.G + r % c.G;
+        const size_t n = w.s.q0 + tok;
+        po[i] = c.po + (slot * RT + t) * PD + 4 * lane;
+        out[i] = c.out + (n * c.Hq + head) * PD + 4 * lane;
+        if (c.gate)
+            gv[i] = *(const bf16x4 *)(c.gate + n * c.gts + (size_t)head * c.ghs + 4 * lane);
+    }
+    const int own = min(t0 + (lane >> 4), last);
+    float mu = -INFINITY, l = 0.f; /* of row lane >> 4 */
+    floatx4 acc[R] = {};
+    auto of = [&](float x, int at) {
+        return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), at));
+    };
+    for (int j0 = 0; j0 < w.parts; j0 += 16) {
+        const int cnt = min(w.parts - j0, 16);
+        const size_t mine = (slot + j0 + min(lane & 15, cnt - 1)) * RT + own;
+        const float pl = c.pl[mine], pm = c.pmu[mine];
+        const float li = (lane & 15) < cnt ? pl : 0.f, mi = li > 0.f ? pm : -INFINITY;
+        float wi = 0.f;
+        for (int k0 = 0; k0 < cnt; k0 += 4) {
+            floatx4 v[4][R];
+#pragma unroll
+            for (int k = 0; k < 4; k++) /* past the last part it again, with weight 0 */
+#pragma unroll
+                for (int i = 0; i < R; i++)
+                    v[k][i] = *(const floatx4 *)(po[i] + (size_t)(j0 + min(k0 + k, cnt - 1)) *
+                                                             (RT * PD));
+            if (k0 == 0) {
+                const float next =
+                    fmaxf(mu, fold_row(mi, [](float x, float y) { return fmaxf(x, y); }));
+                const float ref = next == -INFINITY ? 0.f : next, old = fast_exp2(mu - ref);
+                wi = li > 0.f ? fast_exp2(mi - ref) : 0.f;
+                mu = next;
+                l = l * old + fold_row(wi * li, [](float x, float y) { return x + y; });
+#pragma unroll
+                for (int i = 0; i < R; i++)
+                    acc[i] *= of(old, 16 * i);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+#pragma unroll
+                for (int i = 0; i < R; i++) {
+                    const float f = of(wi, 16 * i + k0 + k);
+                    if (f > 0.f)
+                        acc[i] += v[k][i] * f;
+                }
         }
-        const float inv = l > 0.f ? 1.f / l : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        const float li = of(l, 16 * i), inv = li > 0.f ? 1.f / li : 0.f;
         bf16x4 res;
 #pragma unroll
         for (int e = 0; e < 4; e++)
-            res[e] = f2bf(acc[e] * inv * (c.gate ? sigmoid_f(bf2f(gv[e])) : 1.f));
-        if (!ROW || lane < 16)
-            *(bf16x4 *)(c.out + ((size_t)n * c.Hq + head) * PD + dim) = res;
+            res[e] = f2bf(acc[i][e] * inv * (c.gate ? sigmoid_f(bf2f(gv[i][e])) : 1.f));
+        if (t0 + i <= last)
+            *(bf16x4 *)out[i] = res;
     }
 }
 
@@ -1261,11 +1331,11 @@ extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int
         const int groups = !few ? RT / 16 : row ? rows : pg_div_up(rows, 4);
         const dim3 mgrid((unsigned)(p.units * Hkv * groups));
         if (row)
-            hipLaunchKernelGGL((merge_kernel<FEW, true>), mgrid, dim3(256), 0, stream, c, groups);
+            hipLaunchKernelGGL(merge_few_kernel<true>, mgrid, dim3(256), 0, stream, c, groups);
         else if (few)
-            hipLaunchKernelGGL((merge_kernel<FEW, false>), mgrid, dim3(256), 0, stream, c, groups);
+            hipLaunchKernelGGL(merge_few_kernel<false>, mgrid, dim3(256), 0, stream, c, groups);
         else
-            hipLaunchKernelGGL((merge_kernel<RT, false>), mgrid, dim3(256), 0, stream, c, groups);
+            hipLaunchKernelGGL(merge_many_kernel, mgrid, dim3(256), 0, stream, c);
     }
     return hipGetLastError();
 }

@@ -49,23 +49,25 @@ DEV int wave_scan(int v) {
     return v;
 }
 DEV int last_lane(int v) { return __builtin_amdgcn_readlane(v, 63); }
-/* f over the lanes of each row of 16, then of the wave, in the order of a butterfly
- * from 32 down to 1 (a rotation by o meets what lane ^ o has, once the rows' larger
- * strides are done) */
+/* f over the 16 lanes of each row of the wave, as a butterfly from 8 down to 1 (a
+ * rotation by o meets what lane ^ o has, once the larger strides are done), and over
+ * the wave, from 32 down */
 template <int ctrl> DEV float dpp(float x) {
     return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(
         0, (int)__float_as_uint(x), ctrl, 0xf, 0xf, true));
+}
+template <class F> DEV float fold_row(float x, F f) {
+    x = f(x, dpp<0x128>(x)); /* row_ror 8, 4, 2, 1 */
+    x = f(x, dpp<0x124>(x));
+    x = f(x, dpp<0x122>(x));
+    return f(x, dpp<0x121>(x));
 }
 template <class F> DEV float fold_wave(float x, F f) {
     const uint32_t u = __float_as_uint(x);
     auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
     const uint32_t v = __float_as_uint(f(__uint_as_float(a[0]), __uint_as_float(a[1])));
     a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    x = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    x = f(x, dpp<0x128>(x)); /* row_ror 8, 4, 2, 1 */
-    x = f(x, dpp<0x124>(x));
-    x = f(x, dpp<0x122>(x));
-    return f(x, dpp<0x121>(x));
+    return fold_row(f(__uint_as_float(a[0]), __uint_as_float(a[1])), f);
 }
 
 /* The sequences of rows n0 .. n0 + TOK - 1, row n0 + t in lane t: the last b
