@@ -1211,7 +1211,8 @@ __global__ __launch_bounds__(256) void merge_many_kernel(Call c) {
     const int group = blockIdx.x % GROUPS, kh = blockIdx.x / GROUPS % c.Hkv;
     const Where w = locate<RT, false>(c, blockIdx.x / GROUPS / c.Hkv);
     const int r0 = w.unit * RT, t0 = (group * 4 + wave) * R;
-    if (w.b < 0 || w.parts <= 1 || t0 >= min(w.s.ql * c.G - r0, RT))
+    if (w.b < 0 || w.parts <= 1 || t0 >= min(w.s.ql * c.G - r0, RT) ||
+        w.first + w.parts > c.plan.slots) /* more than any rising q_start has */
         return;
     const int last = min(w.s.ql * c.G - r0, RT) - 1;
     const float *po[R]; /* part 0 of a row's o; past the last row it again */

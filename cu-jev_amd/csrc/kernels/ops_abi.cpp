@@ -313,9 +313,10 @@ static int paged_check(const char *what, const cujev_kv_pages *pages, const int3
     return 0;
 }
 
-/* Heads of q: a multiple of the kv-heads, at most 16 per kv-head. */
+/* Heads of q: a multiple of the kv-heads, at most 16 per kv-head; 128 tokens' q
+ * within 2 GiB. */
 static int paged_heads_ok(int Hq, int Hkv) {
-    return Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Hq / Hkv <= 16;
+    return Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Hq / Hkv <= 16 && Hq <= 8192;
 }
 
 EXPORT int cujev_op_attn_prep_paged(const void *proj, int proj_stride, const float *q_norm_w,
@@ -330,8 +331,8 @@ EXPORT int cujev_op_attn_prep_paged(const void *proj, int proj_stride, const flo
     const int st = paged_check("attn_prep_paged", &pages, page_table, max_pages, kv_len, B);
     if (st != 0)
         return st;
-    if (N < 0 || N > PG_MOST || !paged_heads_ok(Hq, Hkv) || (rot != 8 && rot != 16 && rot != 32 && rot != 64) ||
-        npos <= 0)
+    if (N < 0 || N > PG_MOST || !paged_heads_ok(Hq, Hkv) ||
+        (rot != 8 && rot != 16 && rot != 32 && rot != 64) || npos <= 0)
         return fail(1, "attn_prep_paged: unsupported shape N=%d Hq=%d Hkv=%d rot=%d npos=%d", N,
                     Hq, Hkv, rot, npos);
     if (N > 0 && B > 0 &&
@@ -387,7 +388,7 @@ EXPORT int cujev_op_attention_paged(const void *q, const void *gate, int gate_to
     const int st = paged_check("attention_paged", &pages, page_table, max_pages, kv_len, B);
     if (st != 0)
         return st;
-    if (N < 0 || N > PG_MOST || max_q < 0 || max_kv < 0 || !paged_heads_ok(Hq, Hkv) || Hq > 8192)
+    if (N < 0 || N > PG_MOST || max_q < 0 || max_kv < 0 || !paged_heads_ok(Hq, Hkv))
         return fail(1, "attention_paged: unsupported shape N=%d max_q=%d max_kv=%d Hq=%d Hkv=%d",
                     N, max_q, max_kv, Hq, Hkv);
     if (max_kv > max_pages * CUJEV_KV_PAGE)

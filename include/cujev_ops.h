@@ -228,7 +228,7 @@ int cujev_op_attention_noalloc(const void *q, const void *gate, int gate_tok_str
 
 /* cujev_op_attn_prep with K and V written into pages: per row n of a sequence
  * q_out[n] bf16 [N][Hq][256] and, at the row's position, its K and V. Any Hq /
- * Hkv up to 16; rot is 8, 16, 32 or 64; pos [N] picks the row's RoPE angles
+ * Hkv up to 16, Hq up to 8192; rot is 8, 16, 32 or 64; pos [N] picks the row's RoPE angles
  * (cut to [0, npos), the table's positions); proj rows 8-byte aligned. */
 int cujev_op_attn_prep_paged(const void *proj, int proj_stride, const float *q_norm_w,
                              const float *k_norm_w, const int32_t *pos, const int32_t *q_start,
@@ -241,7 +241,8 @@ int cujev_op_attn_prep_paged(const void *proj, int proj_stride, const float *q_n
 /* Reads sequences back: columns [0, min(kv_len[b], max_kv)) of k_cache
  * [B][Hkv][cache_stride][256] and vt_cache [B][Hkv][256][cache_stride], the
  * layout of a state's caches, cache_stride >= cujev_ops_kv_stride(max_kv);
- * further columns stay as they were. max_kv <= max_pages * 64. */
+ * further columns stay as they were. max_kv <= max_pages * 64; at most 65535
+ * sequences and kv-heads a call. */
 int cujev_op_kv_page_read(int kv_type, const void *k_pages, const void *vt_pages,
                           const float *k_scale, const float *v_scale, int num_pages,
                           const int32_t *page_table, int max_pages, const int32_t *kv_len, int B,
@@ -254,7 +255,7 @@ int cujev_op_kv_page_read(int kv_type, const void *k_pages, const void *vt_pages
  * p and, where window > 0, of those only j > p - window and j < sinks (the
  * first tokens of the sequence); a row that sees no key gives 0. K and V of
  * keys that some row of the call sees have to be finite; other slots may hold
- * anything. Any Hq / Hkv up to 16. No sequence has more than max_q new tokens
+ * anything. Any Hq / Hkv up to 16, Hq up to 8192. No sequence has more than max_q new tokens
  * or max_kv keys (what is past them is not computed, or not seen). ws: device
  * workspace of cujev_ops_attention_paged_ws_bytes() for the same arguments
  * (0: none needed); calls that may overlap need one each. */

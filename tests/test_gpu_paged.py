@@ -558,3 +558,151 @@ def test_calls_run_on_the_current_stream_and_repeat_bit_for_bit():
     with torch.cuda.stream(s):
         again = run_attention(c)
     assert torch.equal(first, again)
+
+
+def _lens_over_pieces(seed):
+    """Sequences of every length up to 11 pages, and many in a row without a token."""
+    g = torch.Generator().manual_seed(seed)
+    kv = torch.randint(1, 700, (150,), generator=g).tolist()
+    return [(0 if 20 <= i < 100 or i % 7 == 3 else 1, k) for i, k in enumerate(kv)]
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 4)])
+def test_attention_of_one_token_over_many_uneven_sequences(window, sinks, e4m3):
+    c = attention_case(121, 16, 4, e4m3, _lens_over_pieces(122))
+    check_attention(c, window, sinks)
+    # of bounds far above the lengths, the work is shared out otherwise
+    check_attention(c, window, sinks, max_q=3, max_kv=700)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("Hq,lens", [
+    (4, [(0, 0)] * 15 + [(1, 9000)]),  # one sequence has all of the work of 16
+    (16, [(1, 9000)]),
+    (4, [(33, 17000)]),                # units of more than 16 shares
+    (1, [(130, 2500), (1, 3)]),
+])
+def test_attention_in_many_parts(Hq, lens, e4m3):
+    check_attention(attention_case(131, Hq, 1, e4m3, lens))
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(5, 1), (10, 2), (7, 1), (13, 1), (22, 2), (15, 1)])
+@pytest.mark.parametrize("lens", [[(1, 300), (1, 64)], [(30, 300), (11, 11)]])
+def test_attention_of_odd_head_groups(Hq, Hkv, lens):
+    check_attention(attention_case(141, Hq, Hkv, True, lens))
+
+
+def test_calls_on_two_streams_at_once():
+    """Calls with workspaces of their own, in flight together, give what each
+    gives alone."""
+    o = ops()
+    cases = [attention_case(151, 16, 4, True, [(1, 3000)] * 6),
+             attention_case(152, 8, 2, False, [(40, 2000), (3, 700)])]
+    alone = [run_attention(c) for c in cases]
+    calls, streams = [], [torch.cuda.Stream() for _ in cases]
+    for c in cases:
+        N, Hq = c["N"], c["Hq"]
+        qg = torch.zeros(N, Hq, 2 * D, dtype=torch.bfloat16, device="cuda")
+        qg[..., D:] = c["gate"].cuda()
+        nb = o.attention_paged_ws_bytes(N, len(c["kv_len"]), c["max_q"], c["max_kv"], Hq, c["Hkv"],
+                                        e4m3=c["e4m3"])
+        assert nb > 0
+        outs = [torch.full((N, Hq * D), 7.0, dtype=torch.bfloat16, device="cuda")
+                for _ in range(8)]
+        calls.append((c["q"].cuda(), qg[..., D:], Hq * 2 * D, 2 * D, c["pages"], i32(c["tab"]),
+                      i32(c["qs"]), i32(c["kv_len"]), c["max_q"], c["max_kv"], outs,
+                      torch.empty(nb, dtype=torch.uint8, device="cuda")))
+    torch.cuda.synchronize()
+    for i in range(8):
+        for s, a in zip(streams, calls):
+            with torch.cuda.stream(s):
+                o.attention_paged(*a[:-2], a[-2][i], ws=a[-1])
+    torch.cuda.synchronize()
+    for a, ref, c in zip(calls, alone, cases):
+        for out in a[-2]:
+            assert torch.equal(out.cpu().double().view(c["N"], c["Hq"], D), ref)
+
+
+def test_a_captured_prefill_replays_with_other_lengths():
+    """prep + attention of many tokens a sequence, in shares that are merged:
+    every replay equals the eager calls, rows of no sequence stay."""
+    o = ops()
+    Hq, Hkv, B, N, max_q, max_kv = 8, 2, 3, 90, 40, 2600
+    g = torch.Generator().manual_seed(161)
+    width = Hq * 512 + Hkv * 512
+    w, rope = torch.ones(D, device="cuda"), o.rope_table(1e7, ROT, max_kv)
+    tab = i32(table(162, [max_kv] * B, 130))
+    steps = [([40, 40, 10], [2600, 40, 1000]), ([1, 0, 40], [2000, 0, 64]),
+             ([40, 30, 20], [40, 2599, 2600]), ([0, 0, 1], [0, 5, 1])]
+    nb = o.attention_paged_ws_bytes(N, B, max_q, max_kv, Hq, Hkv)
+    assert nb > 0
+
+    def state():
+        return dict(pages=pool(163, 130, Hkv, False), kv=i32([1] * B), pos=i32([0] * N),
+                    qs=i32([0] * (B + 1)),
+                    proj=torch.zeros(N, width, dtype=torch.bfloat16, device="cuda"),
+                    q=torch.zeros(N, Hq, D, dtype=torch.bfloat16, device="cuda"),
+                    out=torch.zeros(N, Hq * D, dtype=torch.bfloat16, device="cuda"),
+                    ws=torch.empty(nb, dtype=torch.uint8, device="cuda"))
+
+    def step(s):
+        o.attn_prep_paged(s["proj"], w, w, s["pos"], s["qs"], s["kv"], tab, Hq, ROT, rope, EPS,
+                          Q_SCALE, s["q"], s["pages"])
+        o.attention_paged(s["q"], s["proj"][:, D:], width, 512, s["pages"], tab, s["qs"], s["kv"],
+                          max_q, max_kv, s["out"], ws=s["ws"])
+
+    a, b = state(), state()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(b)
+    for q_lens, kv in steps:
+        proj = torch.randn(N, width, generator=g).bfloat16().cuda()
+        pos = [p for n, k in zip(q_lens, kv) for p in range(k - n, k)]
+        for s in (a, b):
+            s["proj"].copy_(proj)
+            s["kv"].copy_(i32(kv))
+            s["qs"].copy_(i32(starts(q_lens)))
+            s["pos"].copy_(i32(pos + [0] * (N - len(pos))))
+            s["out"].fill_(7.0)
+        step(a)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a["out"], b["out"]), q_lens
+        assert torch.equal(a["pages"].k, b["pages"].k) and torch.equal(a["pages"].vt, b["pages"].vt)
+        assert (a["out"][sum(q_lens):] == 7.0).all()
+
+
+def test_pages_past_32_bits_of_a_pool():
+    """The last pages of a pool of more than 2^32 bytes (and 2^31 values) give
+    what the same pages give in a small one."""
+    o = ops()
+    Hq, Hkv, lens, n = 8, 8, [(1, 300), (20, 150), (1, 64)], 16600
+    c = attention_case(171, Hq, Hkv, False, lens)
+    used = c["pages"].num_pages
+    big = o.KvPages(torch.empty(n, Hkv, PAGE, D, dtype=torch.bfloat16, device="cuda"),
+                    torch.empty(n, Hkv, D, PAGE, dtype=torch.bfloat16, device="cuda"))
+    assert big.k.numel() > 2 ** 31
+    big.k[n - used:].copy_(c["pages"].k)
+    big.vt[n - used:].copy_(c["pages"].vt)
+    high = [[p + n - used for p in row] for row in c["tab"]]
+    N = c["qs"][-1]
+    proj = torch.randn(N, Hq * 512 + Hkv * 512, device="cuda").bfloat16()
+    w, rope = torch.ones(D, device="cuda"), o.rope_table(1e7, ROT, 512)
+    pos = i32([p for q, k in lens for p in range(k - q, k)])
+    got = []
+    for pages, tab in ((c["pages"], c["tab"]), (big, high)):
+        q = torch.empty(N, Hq, D, dtype=torch.bfloat16, device="cuda")
+        out = torch.empty(N, Hq * D, dtype=torch.bfloat16, device="cuda")
+        kc, vc = (torch.zeros(s, dtype=torch.bfloat16, device="cuda")
+                  for s in ((3, Hkv, o.kv_stride(300), D), (3, Hkv, D, o.kv_stride(300))))
+        nb = o.attention_paged_ws_bytes(N, 3, 20, 300, Hq, Hkv)
+        ws = torch.empty(nb, dtype=torch.uint8, device="cuda") if nb else None
+        t, qs, kv = i32(tab), i32(c["qs"]), i32(c["kv_len"])
+        o.attn_prep_paged(proj, w, w, pos, qs, kv, t, Hq, ROT, rope, EPS, Q_SCALE, q, pages)
+        o.attention_paged(q, None, 0, 0, pages, t, qs, kv, 20, 300, out, ws=ws)
+        o.kv_page_read(pages, t, kv, 300, kc, vc)
+        got.append((q, out, kc, vc))
+    torch.cuda.synchronize()
+    for a, b in zip(*got):
+        assert torch.equal(a, b)

@@ -63,7 +63,7 @@ def test_pool_and_table_are_checked(name, bad):
 
 
 @pytest.mark.parametrize("bad", [
-    dict(N=-1), dict(Hq=7), dict(Hq=0), dict(Hq=34), dict(rot=0), dict(rot=24), dict(rot=128),
+    dict(N=-1), dict(Hq=7), dict(Hq=0), dict(Hq=34), dict(Hq=1 << 30, Hkv=1 << 29), dict(rot=0), dict(rot=24), dict(rot=128),
     dict(npos=0), dict(proj_stride=5119), dict(proj_stride=5121), dict(proj=FAKE + 4),
     dict(q_out=FAKE + 4), dict(q_norm_w=FAKE + 4), dict(rope_table=FAKE + 8),
     dict(N=1, B=1, proj=None), dict(N=1, B=1, q_start=None), dict(N=1, B=1, q_out=None),
@@ -82,6 +82,7 @@ def test_read_refuses(bad):
 
 @pytest.mark.parametrize("bad", [
     dict(N=-1), dict(max_q=-1), dict(max_kv=-1), dict(max_kv=129), dict(Hq=7), dict(Hq=34),
+    dict(Hq=8200, Hkv=4100),
     dict(window=-1), dict(window=8, sinks=-1), dict(sinks=4), dict(q=FAKE + 8), dict(out=FAKE + 8),
     dict(gate=FAKE + 2), dict(gate_tok_stride=5121), dict(gate_head_stride=2),
     dict(N=1, B=1, q=None), dict(N=1, B=1, q_start=None), dict(N=1, B=1, out=None)], ids=str)
