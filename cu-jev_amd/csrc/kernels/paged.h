@@ -5,6 +5,8 @@
  * tokens are one key tile of the attention, so a tile has one page id, one
  * base address (64-bit) and offsets that fit 15 bits however long the pool. */
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 #include "kernels.h"
 #include "paged_index.h"
@@ -68,6 +70,49 @@ template <class F> DEV float fold_wave(float x, F f) {
     const uint32_t v = __float_as_uint(f(__uint_as_float(a[0]), __uint_as_float(a[1])));
     a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
     return fold_row(f(__uint_as_float(a[0]), __uint_as_float(a[1])), f);
+}
+
+/* fold_wave of doubles, dword by dword */
+template <class F> DEV double fold_wave(double x, F f) {
+    union Two {
+        double d;
+        uint32_t u[2];
+    };
+    auto swap = [&](auto swapped) {
+        Two p, q, v{x};
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const auto a = swapped(v.u[i]);
+            p.u[i] = a[0], q.u[i] = a[1];
+        }
+        x = f(p.d, q.d);
+    };
+    auto turn = [&](auto ctrl) {
+        Two p, v{x};
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            p.u[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v.u[i], decltype(ctrl)::value,
+                                                           0xf, 0xf, true);
+        x = f(x, p.d);
+    };
+    swap([](uint32_t v) { return __builtin_amdgcn_permlane32_swap(v, v, false, false); });
+    swap([](uint32_t v) { return __builtin_amdgcn_permlane16_swap(v, v, false, false); });
+    turn(std::integral_constant<int, 0x128>{});
+    turn(std::integral_constant<int, 0x124>{});
+    turn(std::integral_constant<int, 0x122>{});
+    turn(std::integral_constant<int, 0x121>{});
+    return x;
+}
+/* d towards zero, the last bit set where that lost something: rounding this again
+ * to fewer bits rounds d once */
+DEV float to_odd(double d) {
+    const float f = (float)d;
+    uint32_t u = __float_as_uint(f);
+    if ((double)f != d) {
+        u -= fabs((double)f) > fabs(d);
+        u |= 1;
+    }
+    return d != d ? f : __uint_as_float(u);
 }
 
 /* The sequences of rows n0 .. n0 + TOK - 1, row n0 + t in lane t: the last b
@@ -139,6 +184,11 @@ DEV int e4m3_exp(float a) {
     const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffff) > 0x600000 ? 1 : 0);
     return min(max(e, -100), 120);
 }
+DEV int e4m3_exp(double a) { /* the same from a double */
+    const uint64_t u = __builtin_bit_cast(uint64_t, a), low = (1ull << 52) - 1;
+    const int e = (int)(u >> 52) - 1023 - 8 + ((u & low) > (3ull << 50) ? 1 : 0);
+    return min(max(e, -100), 120);
+}
 DEV float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 /* Four values, already divided by their scales, to four e4m3 bytes (nearest
@@ -146,6 +196,11 @@ DEV float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 DEV uint32_t pack_e4m3(float a, float b, float c, float d) {
     int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+}
+/* Value i of four e4m3 bytes */
+DEV float e4m3_of(uint32_t v, int i) {
+    return i < 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(v, false)[i & 1]
+                 : __builtin_amdgcn_cvt_pk_f32_fp8(v, true)[i & 1];
 }
 /* Two e4m3 bytes (of the low or high half) times 2^k, exact in bf16. */
 template <bool HIGH> DEV bf16x2 unpack_e4m3(uint32_t v, float scale) {

@@ -17,6 +17,39 @@ namespace {
  * the transpose needs neither LDS nor another wave's data: lane l holds 16
  * tokens of dims 4l .. 4l + 3 and stores one piece per dim. A workgroup's four
  * are a page's, whose lines of V^T they fill together in one L2. */
+constexpr int PREP_TOK = 4;
+/* A K row's lane in doubles, rounded to e4m3 once: the bytes, and the scale 2^*e */
+DEV uint32_t k_row_exact(const bf16 *src, const float2 *rope, const float *w, bool rotates,
+                         bool first, int half_lanes, float eps, int *e) {
+    const bf16x4 raw = *(const bf16x4 *)src;
+    double y[4], ss = 0., most = 0.;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        y[i] = bf2f(raw[i]);
+        ss = __builtin_fma(y[i], y[i], ss);
+    }
+    ss = fold_wave(ss, [](double p, double q) { return p + q; });
+    const double a = ss * (1. / 256.) + (double)eps;
+    double rinv = __builtin_amdgcn_rsq(a); /* about 2^-26 off: Newton twice */
+    if (a > 0. && a < (double)INFINITY) {
+        rinv *= __builtin_fma(-.5 * a * rinv, rinv, 1.5);
+        rinv *= __builtin_fma(-.5 * a * rinv, rinv, 1.5);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        y[i] *= rinv * w[i];
+        const float2 cs = rope[rotates ? i : 0];
+        const double o = __shfl_xor(y[i], half_lanes, 64) * cs.y;
+        y[i] = rotates ? __builtin_fma(y[i], (double)cs.x, first ? -o : o) : y[i];
+        most = fmax(most, fabs(y[i]));
+    }
+    most = fold_wave(most, [](double p, double q) { return fmax(p, q); });
+    *e = e4m3_exp(most);
+    const double inv = exp2_int(-*e);
+    return pack_e4m3(to_odd(y[0] * inv), to_odd(y[1] * inv), to_odd(y[2] * inv),
+                     to_odd(y[3] * inv));
+}
+
 template <bool E4M3, int TOK>
 __global__ __launch_bounds__(256) void prep_paged_kernel(
     const bf16 *__restrict__ proj, int ps, const float *__restrict__ qw,
@@ -85,49 +118,81 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(
         for (int t = 0; t < TOK; t++)
             ss[t] = fold_wave(ss[t], [](float p, float q) { return p + q; });
         const float we[4] = {wl.x, wl.y, wl.z, wl.w};
-        float amax[TOK];
 #pragma unroll
         for (int t = 0; t < TOK; t++) {
             const float rinv = rsqrtf(ss[t] * (1.f / 256.f) + eps);
             const float cz[8] = {rc[t][0].x, rc[t][0].y, rc[t][0].z, rc[t][0].w,
                                  rc[t][1].x, rc[t][1].y, rc[t][1].z, rc[t][1].w};
-            amax[t] = 0.f;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const float y = x[t][e] * rinv * we[e];
                 /* rounded as attn_prep rounds: the same bits reach both caches */
                 const float o = __shfl_xor(y, half_lanes, 64) * cz[2 * e + 1];
                 x[t][e] = rotates ? __builtin_fmaf(y, cz[2 * e], first ? -o : o) : y;
-                amax[t] = fmaxf(amax[t], fabsf(x[t][e]));
             }
         }
-        if (E4M3 && is_k) {
-#pragma unroll
-            for (int t = 0; t < TOK; t++)
-                amax[t] = fold_wave(amax[t], [](float p, float q) { return fmaxf(p, q); });
-        }
+        auto row_of = [&](int t) {
+            return (long long)(uint32_t)__builtin_amdgcn_readlane((int)at, t) |
+                   (long long)__builtin_amdgcn_readlane((int)(at >> 32), t) << 32;
+        };
+        uint32_t again = 0; /* tokens */
 #pragma unroll
         for (int t = 0; t < TOK; t++) {
-            const long long row =
-                (long long)(uint32_t)__builtin_amdgcn_readlane((int)at, t) |
-                (long long)__builtin_amdgcn_readlane((int)(at >> 32), t) << 32;
+            const long long row = row_of(t);
             if (row < 0) /* no sequence's row, or no slot */
                 continue;
+            if (E4M3 && is_k) {
+                float amax = 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    amax = fmaxf(amax, fabsf(x[t][e]));
+                amax = fold_wave(amax, [](float p, float q) { return fmaxf(p, q); });
+                const int e = e4m3_exp(amax);
+                const float inv = exp2_int(-e);
+                const uint32_t out =
+                    pack_e4m3(x[t][0] * inv, x[t][1] * inv, x[t][2] * inv, x[t][3] * inv);
+                /* Close to a tie, or to the next scale, float's errors (about ten
+                 * roundings, of values up to amax sqrt 2 where they rotate) can lead a
+                 * value to the other side, a whole step of 2^-3; one or two of 5
+                 * million did. Such a row, one of 30 or so, again in doubles. */
+                constexpr float NEAR = 0x1p-20f;
+                const float top = amax * inv;
+                bool close = top > 448.f * (1.f - NEAR) || top < 224.f * (1.f + NEAR);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float v = fabsf(x[t][i] * inv), r = fabsf(e4m3_of(out, i));
+                    const float step = __uint_as_float(
+                        max(__float_as_uint(v) & 0x7f800000u, (127u - 6) << 23) - (3u << 23));
+                    close |= .5f * step - fabsf(v - r) < NEAR * (rotates ? 2.f * top : v);
+                }
+                again |= __any(close) ? 1u << t : 0u;
+                ((uint32_t *)k_pages)[row * 64 + lane] = out;
+                if (lane == 0)
+                    k_scale[row] = exp2_int(e);
+                continue;
+            }
             const float f = is_k ? 1.f : q_scale;
             const bf16x4 o = {f2bf(x[t][0] * f), f2bf(x[t][1] * f), f2bf(x[t][2] * f),
                               f2bf(x[t][3] * f)};
             if (!is_k) {
                 *(bf16x4 *)(q_out + ((size_t)(n0 + t) * Hq + head) * 256 + 4 * lane) = o;
-            } else if constexpr (E4M3) {
-                const int e = e4m3_exp(amax[t]);
-                const float inv = exp2_int(-e);
-                ((uint32_t *)k_pages)[row * 64 + lane] = pack_e4m3(
-                    x[t][0] * inv, x[t][1] * inv, x[t][2] * inv, x[t][3] * inv);
-                if (lane == 0)
-                    k_scale[row] = exp2_int(e);
             } else {
                 *(bf16x4 *)((bf16 *)k_pages + row * 256 + 4 * lane) = o;
             }
+        }
+#pragma unroll 1
+        while (E4M3 && again) { /* a loop: unrolled, it took registers from the others */
+            const int t = __ffs(again) - 1;
+            again &= again - 1;
+            const long long row = row_of(t);
+            int e;
+            const uint32_t out = k_row_exact(
+                src + (size_t)(n0 + t) * ps,
+                rope + (size_t)__builtin_amdgcn_readlane(pos_lane, t) * (rot / 2) + fi0,
+                w + 4 * lane, rotates, first, half_lanes, eps, &e);
+            ((uint32_t *)k_pages)[row * 64 + lane] = out;
+            if (lane == 0)
+                k_scale[row] = exp2_int(e);
         }
         return;
     }
@@ -347,15 +412,16 @@ extern "C" hipError_t k_attn_prep_paged(const bf16_t *proj, int proj_stride, con
     const int Hkv = pages->Hkv, B = seqs->B;
     if (N <= 0 || B <= 0)
         return hipSuccess;
-    const long long units = (long long)CEIL_DIV(N, 4) * (Hq + Hkv);
+    const long long units = (long long)CEIL_DIV(N, PREP_TOK) * (Hq + Hkv);
     const long long v_pages = N < N / PG + 2ll * B ? N : N / PG + 2ll * B;
     const long long row_blocks = CEIL_DIV(units, 4), v_blocks = v_pages * Hkv;
     if (row_blocks + v_blocks > 0x7fffffff)
         return hipErrorInvalidValue;
 #define LAUNCH(T)                                                                                 \
-    hipLaunchKernelGGL((prep_paged_kernel<T, 4>), dim3((unsigned)(row_blocks + v_blocks)),        \
-                       dim3(256), 0, stream, (const bf16 *)proj, proj_stride, q_norm_w, k_norm_w, \
-                       pos, seqs->q_start, seqs->kv_len, seqs->page_table, seqs->max_pages, B, N, \
+    hipLaunchKernelGGL((prep_paged_kernel<T, PREP_TOK>),                                          \
+                       dim3((unsigned)(row_blocks + v_blocks)), dim3(256), 0, stream,             \
+                       (const bf16 *)proj, proj_stride, q_norm_w, k_norm_w, pos, seqs->q_start,   \
+                       seqs->kv_len, seqs->page_table, seqs->max_pages, B, N,                     \
                        Hq, Hkv, rot, (const float2 *)rope_table, npos, eps, q_scale,              \
                        (bf16 *)q_out, pages->k, pages->vt, pages->k_scale, pages->v_scale,        \
                        pages->num_pages, (int)row_blocks)

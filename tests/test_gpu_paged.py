@@ -156,6 +156,35 @@ def test_prep_writes_pages(Hq, Hkv, e4m3, lens):
     assert (same | ~keep.transpose(2, 3)).all(), "a V slot of no new token changed"
 
 
+def test_prep_rounds_e4m3_keys_once():
+    """K of e4m3 pages is the 64-bit value rounded once: every byte and scale of
+    4 million values, some of tokens of zeros and of tiny and large ones."""
+    o = ops()
+    Hq, Hkv, N = 4, 4, 4000
+    g = torch.Generator().manual_seed(181)
+    width = Hq * 512 + Hkv * 512
+    proj = torch.randn(N, width, generator=g).bfloat16()
+    proj[7] = 0
+    proj[8:12] *= torch.tensor([1e-3, 1e-12, 1e4, 1e12])[:, None].bfloat16()
+    kw = 1 + 0.1 * torch.randn(D, generator=g)
+    pos = torch.randint(0, 500, (N,), generator=g, dtype=torch.int32)
+    rope = o.rope_table(1e7, ROT, 500)
+    pages, tab = pool(182, 64, Hkv, True), table(183, [N], 64)
+    q_out = torch.empty(N, Hq, D, dtype=torch.bfloat16, device="cuda")
+    o.attn_prep_paged(proj.cuda(), kw.cuda(), kw.cuda(), pos.cuda(), i32([0, N]), i32([N]),
+                      i32(tab), Hq, ROT, rope, EPS, Q_SCALE, q_out, pages)
+    torch.cuda.synchronize()
+    cs = rope.cpu().double()[pos.long()][:, None]
+    k = po.norm_rope(proj.double()[:, Hq * 512:Hq * 512 + Hkv * 256].view(-1, Hkv, D), kw.double(),
+                     cs[..., 0], cs[..., 1], ROT, EPS)
+    kq, ks = po.quantise(k, 2)
+    at = torch.tensor(tab[0])[:-(-N // PAGE)]
+    gk = pages.k.cpu().float().double()[at].transpose(1, 2).reshape(-1, Hkv, D)[:N]
+    gs = pages.k_scale.cpu().double()[at].transpose(1, 2).reshape(-1, Hkv)[:N]
+    assert torch.equal(gs, ks)
+    assert torch.equal(gk, kq)
+
+
 def test_prep_skips_pages_that_are_not_there():
     """Ids outside the pool, lengths past the table: nothing is written there."""
     o = ops()
