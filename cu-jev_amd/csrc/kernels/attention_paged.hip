@@ -151,7 +151,11 @@ template <int RT_, bool BY_PART> DEV Where locate(const Call &c, int target) {
             w.own = n;
             w.parts = (n - 1) / w.size + 1;
         } else {
-            w.parts = pg_nshare(n, pg_share(c.plan, units, (unsigned)units * (unsigned)n));
+            int share = PG_MOST;
+            if (pg_splits(c.plan, units)) /* as many for each unit as there are */
+                share = pg_share_last(
+                    pg_max((n - 1) / (c.plan.goal / units) + 1, PG_MANY_LEAST), n);
+            w.parts = pg_nshare(n, share);
         }
         w.unit = BY_PART ? target / w.parts : target;
         w.first = w.unit * w.parts;
@@ -168,14 +172,25 @@ template <int RT_, bool BY_PART> DEV Where locate(const Call &c, int target) {
         units = b0 + lane < c.B ? units_of(s) : 0;
         n = units ? each(s) : 0;
     };
-    int U = 0;
+    int U = 0, longest = 0;
     unsigned T = 0;
     for (int b0 = 0; b0 < c.B; b0 += 64) {
         read(b0);
         T += (unsigned)last_lane(wave_scan((int)((unsigned)units * (unsigned)n)));
         U += FEWR ? __popcll(__ballot(units > 0)) : last_lane(wave_scan(units));
+        if constexpr (!FEWR)
+            longest = max(longest, (int)fold_wave((float)n, [](float p, float q) {
+                              return fmaxf(p, q); /* below 2^24 tiles: exact */
+                          }));
     }
-    const int size = FEWR ? pg_few_share(c.plan, U, T) : pg_share(c.plan, U, T);
+    int size = FEWR ? pg_few_share(c.plan, U, T) : PG_MOST;
+    if (!FEWR && pg_splits(c.plan, U)) {
+        size = pg_share_first(c.plan, U, T, c.B > 64);
+        if (c.B <= 64)
+            while (last_lane(wave_scan(units * pg_nshare(n, size))) > c.plan.goal)
+                size = pg_share_next(size);
+        size = pg_share_last(size, __builtin_amdgcn_readfirstlane(longest));
+    }
     int before_u = 0, before_n = 0;
     for (int b0 = 0; b0 < c.B; b0 += 64) {
         if (c.B > 64)

@@ -117,15 +117,24 @@ constexpr int pg_few_share(const pg_plan &p, int U, unsigned T) {
  * and of one that begins here and goes on. */
 constexpr int pg_few_slot(int p0, int j) { return 2 * (p0 + j) + (j == 0); }
 
-/* PG_MANY: key tiles a share should have, for U units with T tiles in all. A
- * sequence's last share is half empty on average: as many workgroups fewer to
- * count on. */
-constexpr int PG_MANY_LEAST = 16;
-constexpr int pg_share(const pg_plan &p, int U, unsigned T) {
-    if (p.goal == 0 || U >= p.goal)
-        return PG_MOST;
-    const unsigned n = (unsigned)pg_max(p.goal - U / 2, U);
+/* PG_MANY: key tiles a share has at most, of U units with T tiles in all and
+ * `longest` the most that one has: about the least for which the parts do not
+ * outnumber the workgroups that run at once. Try pg_share_first, then pg_share_next
+ * of it until they fit; `sure` fits without trying. Where a share is then not
+ * shorter by what a merge takes, some 6 tiles (10 us), all stay whole: 8 sequences'
+ * 200 tokens on up to 1500 keys take 61 us so, 67 in 71 parts for 64 workgroups.
+ * Shares have 8 tiles at least: 2 x 64 tokens on 2048 keys take 27 us, 37 with 16;
+ * with 4 it is 25, and no less where there is more to do. */
+constexpr int PG_MANY_LEAST = 8, PG_MANY_MERGE = 6;
+constexpr bool pg_splits(const pg_plan &p, int U) { return p.goal > 0 && U < p.goal; }
+constexpr int pg_share_first(const pg_plan &p, int U, unsigned T, bool sure) {
+    /* a unit's last share is half full on average */
+    const unsigned n = (unsigned)(p.goal - (sure ? U : U / 2));
     return pg_max((int)(T / n + (T % n != 0)), PG_MANY_LEAST);
+}
+constexpr int pg_share_next(int share) { return share + pg_max(share / 16, 1); }
+constexpr int pg_share_last(int share, int longest) {
+    return share + PG_MANY_MERGE >= longest ? PG_MOST : share;
 }
 constexpr int pg_nshare(int tiles, int share) { return pg_max(pg_div_up(tiles, share), 1); }
 /* First list entry of share i of n even ones */
@@ -165,11 +174,11 @@ constexpr pg_plan pg_make_plan(int N, int B, int max_q, int max_kv, int G, int H
         p.goal = pg_max(256 / Hkv, 1);
         if ((long long)N * G / PG_MANY >= p.goal)
             p.goal = 0;
-        /* sum over units of max(ceil(t / share), 1), share at least T / n, n <= goal,
-         * fewer than goal units: below goal + units; goal units or more: whole */
-        const bool split = p.goal > 0 && most > PG_MANY_LEAST;
-        shares = !split ? units : units < p.goal ? p.goal + units : units < 2ll * p.goal ? 2ll * p.goal : units;
-        slots = split ? shares : 0;
+        const bool split = p.goal > 0 && most > PG_MANY_LEAST + PG_MANY_MERGE;
+        if (!split)
+            p.goal = 0;
+        shares = units > p.goal ? units : p.goal;
+        slots = split ? p.goal : 0;
     }
     if (units * Hkv > 1 << 22 || shares * Hkv > 1 << 22) {
         p.shares = -1;

@@ -151,11 +151,36 @@ int main() {
             }
             continue;
         }
-        const int share = pg_share(p, (int)U, (unsigned)T);
+        auto parts = [&](int share) {
+            long long n = 0;
+            for (int b = 0; b < B; b++) {
+                const int u = pg_units(seqs[b], G, p.rt);
+                n += u ? (long long)u * pg_nshare(pg_longest(seqs[b], G, p.rt, W, SS), share) : 0;
+            }
+            return n;
+        };
+        int share = PG_MOST, longest = 0;
+        for (int b = 0; b < B; b++)
+            longest = pg_max(longest, pg_longest(seqs[b], G, p.rt, W, SS));
+        if (pg_splits(p, (int)U) && U > 0) {
+            const int sure = pg_share_first(p, (int)U, (unsigned)T, true);
+            NEED(parts(sure) <= p.goal);
+            share = pg_share_first(p, (int)U, (unsigned)T, B > 64);
+            NEED(share <= sure);
+            if (B == 1)
+                share = pg_max((longest - 1) / (p.goal / (int)U) + 1, PG_MANY_LEAST);
+            else if (B <= 64)
+                for (int tries = 0; parts(share) > p.goal; tries++) {
+                    NEED(tries < 100);
+                    share = pg_share_next(share);
+                }
+            share = pg_share_last(share, longest);
+        }
+        bool split = false;
         for (int b = 0; b < B; b++) {
             const int u = pg_units(seqs[b], G, p.rt), n = pg_nshare(pg_longest(seqs[b], G, p.rt, W, SS), share);
             C += (long long)u * n;
-            NEED(u == 0 || n == 1 || p.slots > 0);
+            split |= u > 0 && n > 1;
             for (int k = 0; k < u; k++) {
                 const int r0 = k * p.rt, rows = pg_min(seqs[b].ql * G - r0, p.rt);
                 NEED(rows > 0);
@@ -165,7 +190,7 @@ int main() {
                     NEED(pg_share_begin(t.ntl, i + 1, n) >= pg_share_begin(t.ntl, i, n));
             }
         }
-        NEED(C <= p.shares && (p.slots == 0 || p.slots >= C));
+        NEED(C <= p.shares && (!split || p.slots >= C));
     }
     {   /* the largest calls: nothing overflows */
         NEED(pg_make_plan(PG_MOST, 1, PG_MOST, PG_MOST_KEYS, 16, 1, 0, 0).shares == -1);
