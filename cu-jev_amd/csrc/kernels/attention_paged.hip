@@ -59,8 +59,7 @@ DEV float hide(bool seen, float x) {
 
 /* v_mfma_f32_32x32x16_bf16 by hand, so that O and Q stay in accumulation
  * registers and the scores in ordinary ones; with the builtin the compiler
- * moved Q's operands over before each MFMA (and spilled 64 registers). What
- * it leaves to the code around it: two wait states between a VALU write of an
+ * moved Q's operands over before each MFMA. What it leaves to the code around it: two wait states between a VALU write of an
  * operand and the MFMA (NOP), and 18 between an MFMA and a read of its result
  * by anything but the next MFMA on it (settle()). Operands from LDS are waited
  * for as for any instruction. */
@@ -245,7 +244,11 @@ DEV size_t slot_of(const Call &c, int kh, int at) { return (size_t)kh * c.plan.s
  * All loads are unconditional (past the end the last tile's again), so a wait for
  * one set's counts the other's in flight and not more; in 256 registers two waves
  * share a SIMD. Q waits in LDS: read again each tile, it leaves the registers to
- * loads. */
+ * loads.
+ *
+ * 64 sequences' tokens on up to 4096 keys, e4m3: 62 us for 320 MB (5.2 TB/s), and 5
+ * for the merge. A call of one tile takes 7.5 us, a chain of loads: arguments,
+ * lengths, page ids, K, gates. */
 constexpr int FEW = PG_FEW;
 
 template <bool E4M3>
@@ -542,7 +545,12 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
  * of it (mu cancels in o / l). A wave that leaves that range takes an integer
  * mu of its own for the tile and tells the other of its pair through the signs
  * of its P, which are otherwise 0: lane h = 0 sends the low and h = 1 the high
- * half of the float. Both then agree on the larger one and rescale. */
+ * half of the float. Both then agree on the larger one and rescale.
+ *
+ * 4096 tokens on 8192 keys: 367-378 us, 1.1 PFLOP/s, within 7 % of a large library
+ * product (bf16); e4m3 388-400, where the conversions to bf16 fill the VALU beside the
+ * MFMAs. A workgroup spends 12 us outside its tiles: 3.5 on lengths, page ids and
+ * the first K, 5 on the epilogue (the gates' 32768 sigmoids are 2 of them). */
 constexpr int RT = PG_MANY;
 constexpr float SHIFT_RANGE = 64.f;
 

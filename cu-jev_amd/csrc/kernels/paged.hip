@@ -16,7 +16,12 @@ namespace {
  * kv-head: the group's V^T rows are whole 16-byte (e4m3) or 32-byte pieces, so
  * the transpose needs neither LDS nor another wave's data: lane l holds 16
  * tokens of dims 4l .. 4l + 3 and stores one piece per dim. A workgroup's four
- * are a page's, whose lines of V^T they fill together in one L2. */
+ * are a page's, whose lines of V^T they fill together in one L2.
+ *
+ * 8 sequences of up to 700 tokens, e4m3: 17.6 us for 62 MB, 3.5 TB/s (25 with one
+ * group a workgroup, reductions through LDS and rope loads by all lanes). 64 of one
+ * token: 7 us, a chain of loads: arguments, lengths, page ids, stores. Four tokens a
+ * wave; two (half the registers, twice the waves) took the same. */
 constexpr int PREP_TOK = 4;
 /* A K row's lane in doubles, rounded to e4m3 once: the bytes, and the scale 2^*e */
 DEV uint32_t k_row_exact(const bf16 *src, const float2 *rope, const float *w, bool rotates,
@@ -305,7 +310,8 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(
 /* ---- pages back into a state's caches -----------------------------------------
  * One workgroup per (sequence, page, kv-head, K or V^T): 64 rows of 512 bytes
  * or 256 rows of 128 out, 16 values a thread and step. A page id outside the
- * pool reads as zeros; columns from kv_len on stay as they were. */
+ * pool reads as zeros; columns from kv_len on stay as they were. 8192 keys of 4
+ * kv-heads from e4m3: 10.4 us for 50 MB, 4.8 TB/s. */
 template <bool E4M3>
 __global__ __launch_bounds__(256) void page_read_kernel(
     const void *__restrict__ k_pages, const void *__restrict__ vt_pages,
