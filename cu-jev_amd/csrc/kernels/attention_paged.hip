@@ -108,6 +108,7 @@ struct Call {
     int rG; /* r / G = r * rG >> 16 for r < 4096 (an integer division is 30 instructions) */
     bf16 *out;
     float *po, *pl, *pmu;
+    int2 *info; /* few rows: a sequence's first piece and parts, for the merge */
     pg_plan plan;
 };
 DEV pg_seq seq_of(const Call &c, int b) {
@@ -124,106 +125,134 @@ DEV int lane_again() {
     asm volatile("" : "+v"(none));
     return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none));
 }
-/* The unit that share `target` of a kv-head belongs to (BY_PART; few rows: the one
- * that piece `target` begins in), or unit `target`: its sequence (b -1: there is
- * none), its number in it, its parts, the first one's number (few rows: its
- * piece's), which of them `target` is. */
+/* The unit that share `target` of a kv-head belongs to (few rows: the one that piece
+ * `target` begins in): its sequence (b -1: there is none), its number in it, its parts,
+ * the first one's number (few rows: its piece's), which of them `target` is. */
 struct Where {
     pg_seq s;
     int b, unit, parts, first, part;
     int begin, own, size; /* few rows: the unit on the line, tiles a piece */
 };
-template <int RT_, bool BY_PART> DEV Where locate(const Call &c, int target) {
+/* J sequences a lane, 64 J a step: what all have, then where target lies */
+template <int RT_, int J> DEV Where locate_among(const Call &c, int target) {
     constexpr bool FEWR = RT_ == PG_FEW;
     const int lane = threadIdx.x & 63;
-    Where w;
-    w.b = -1, w.begin = w.own = w.size = 0;
-    auto units_of = [&](const pg_seq &s) { return pg_units(s, c.G, RT_); };
-    auto each = [&](const pg_seq &s) { return pg_longest(s, c.G, RT_, c.window, c.sinks); };
-    if (c.B == 1) { /* no scan for one sequence */
-        w.s = seq_of(c, 0);
-        const int units = units_of(w.s), n = each(w.s);
-        if (units == 0)
-            return w;
-        if constexpr (FEWR) {
-            w.size = pg_few_share(c.plan, 1, (unsigned)n);
-            w.own = n;
-            w.parts = (n - 1) / w.size + 1;
-        } else {
-            int share = PG_MOST;
-            if (pg_splits(c.plan, units)) /* as many for each unit as there are */
-                share = pg_share_last(
-                    pg_max((n - 1) / (c.plan.goal / units) + 1, PG_MANY_LEAST), n);
-            w.parts = pg_nshare(n, share);
-        }
-        w.unit = BY_PART ? target / w.parts : target;
-        w.first = w.unit * w.parts;
-        w.part = BY_PART ? target - w.first : 0;
-        w.b = w.unit < units ? 0 : -1;
-        return w;
-    }
-    /* 64 sequences at a time, one a lane: what all have, then where target lies.
-     * Up to 64 are read once. */
-    pg_seq s;
-    int units = 0, n = 0;
+    pg_seq s[J];
+    int units[J], n[J];
     auto read = [&](int b0) {
-        s = seq_of(c, min(b0 + lane, c.B - 1));
-        units = b0 + lane < c.B ? units_of(s) : 0;
-        n = units ? each(s) : 0;
+#pragma unroll
+        for (int j = 0; j < J; j++)
+            s[j] = seq_of(c, min(b0 + J * lane + j, c.B - 1));
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            units[j] = b0 + J * lane + j < c.B ? pg_units(s[j], c.G, RT_) : 0;
+            n[j] = units[j] ? pg_longest(s[j], c.G, RT_, c.window, c.sinks) : 0;
+        }
     };
-    int U = 0, longest = 0;
-    unsigned T = 0;
-    for (int b0 = 0; b0 < c.B; b0 += 64) {
-        read(b0);
-        T += (unsigned)last_lane(wave_scan((int)((unsigned)units * (unsigned)n)));
-        U += FEWR ? __popcll(__ballot(units > 0)) : last_lane(wave_scan(units));
-        if constexpr (!FEWR)
-            longest = max(longest, (int)fold_wave((float)n, [](float p, float q) {
-                              return fmaxf(p, q); /* below 2^24 tiles: exact */
-                          }));
+    if constexpr (J == 1) /* the only step */
+        read(0);
+    int size = PG_MOST;
+    if (FEWR || c.plan.goal > 0) {
+        int U = 0, longest = 0;
+        unsigned T = 0;
+        for (int b0 = 0; b0 < c.B; b0 += 64 * J) {
+            if constexpr (J > 1)
+                read(b0);
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+                T += (unsigned)units[j] * (unsigned)n[j];
+                U += units[j];
+                longest = max(longest, n[j]);
+            }
+        }
+        T = (unsigned)last_lane(wave_scan((int)T));
+        U = last_lane(wave_scan(U));
+        if constexpr (FEWR) {
+            size = pg_few_share(c.plan, U, T);
+        } else if (pg_splits(c.plan, U)) {
+            size = pg_share_first(c.plan, U, T, J > 1);
+            if constexpr (J == 1)
+                while (last_lane(wave_scan(units[0] * pg_nshare(n[0], size))) > c.plan.goal)
+                    size = pg_share_next(size);
+            longest = (int)fold_wave((float)longest, [](float p, float q) {
+                return fmaxf(p, q); /* below 2^24 tiles: exact */
+            });
+            size = pg_share_last(size, __builtin_amdgcn_readfirstlane(longest));
+        }
     }
-    int size = FEWR ? pg_few_share(c.plan, U, T) : PG_MOST;
-    if (!FEWR && pg_splits(c.plan, U)) {
-        size = pg_share_first(c.plan, U, T, c.B > 64);
-        if (c.B <= 64)
-            while (last_lane(wave_scan(units * pg_nshare(n, size))) > c.plan.goal)
-                size = pg_share_next(size);
-        size = pg_share_last(size, __builtin_amdgcn_readfirstlane(longest));
-    }
-    int before_u = 0, before_n = 0;
-    for (int b0 = 0; b0 < c.B; b0 += 64) {
-        if (c.B > 64)
+    Where w;
+    w.b = -1;
+    const int item = FEWR ? target * size : target; /* a tile of the line, or a part */
+    int before = 0;
+    for (int b0 = 0; b0 < c.B; b0 += 64 * J) {
+        if constexpr (J > 1)
             read(b0);
-        const int parts = FEWR ? 0 : pg_nshare(n, size);
-        const int su = FEWR && BY_PART ? 0 : before_u + wave_scan(units);
-        const int sn = before_n + wave_scan(units * (FEWR ? n : parts));
-        const int u = su - units, a = sn - units * (FEWR ? n : parts); /* before the lane's */
-        /* few rows: one unit, its parts are pieces p0 .. p1 */
-        const int p0 = FEWR ? a / size : 0, p1 = FEWR ? (sn - 1) / size : 0;
-        const uint64_t past = __ballot(!BY_PART ? su > target
-                                       : FEWR   ? units > 0 && p1 >= target
-                                                : sn > target);
+        int own[J], sum = 0;
+#pragma unroll
+        for (int j = 0; j < J; j++)
+            sum += own[j] = units[j] * (FEWR ? n[j] : pg_nshare(n[j], size));
+        const int to = before + wave_scan(sum);
+        const uint64_t past = __ballot(to > item);
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
-            auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-            w.s = seq_at(s, l);
-            w.b = b0 + l;
-            if constexpr (FEWR) {
-                w.unit = 0, w.begin = of(a), w.own = of(n), w.size = size;
-                w.first = of(p0);
-                w.parts = of(p1) - of(p0) + 1;
-                w.part = BY_PART ? target - w.first : 0;
-            } else {
-                w.parts = of(parts);
-                w.unit = BY_PART ? (target - of(a)) / w.parts : target - of(u);
-                w.first = of(a) + w.unit * w.parts;
-                w.part = BY_PART ? target - w.first : 0;
+            int at = __builtin_amdgcn_readlane(to - sum, l), have = 0;
+            w.b = 0;
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+                const int here = __builtin_amdgcn_readlane(own[j], l);
+                if (item >= at && item < at + here) {
+                    w.s = seq_at(s[j], l);
+                    w.b = b0 + J * l + j;
+                    w.own = __builtin_amdgcn_readlane(n[j], l);
+                    have = at;
+                }
+                at += here;
             }
+            if constexpr (FEWR) {
+                w.unit = 0, w.begin = have, w.size = size;
+                w.first = have / size;
+                w.parts = (have + w.own - 1) / size - w.first + 1;
+            } else {
+                w.parts = pg_nshare(w.own, size);
+                w.unit = (target - have) / w.parts;
+                w.first = have + w.unit * w.parts;
+            }
+            w.part = target - w.first;
             return w;
         }
-        before_u = last_lane(su);
-        before_n = last_lane(sn);
+        before = last_lane(to);
     }
+    return w;
+}
+template <int RT_> DEV Where locate(const Call &c, int target) {
+    constexpr bool FEWR = RT_ == PG_FEW;
+    if (c.B > 64)
+        return locate_among<RT_, 4>(c, target);
+    if (c.B > 1)
+        return locate_among<RT_, 1>(c, target);
+    /* one sequence: no scan */
+    Where w;
+    w.b = -1, w.begin = 0;
+    w.s = seq_of(c, 0);
+    const int units = pg_units(w.s, c.G, RT_);
+    const int n = pg_longest(w.s, c.G, RT_, c.window, c.sinks);
+    if (units == 0)
+        return w;
+    if constexpr (FEWR) {
+        w.size = pg_few_share(c.plan, 1, (unsigned)n);
+        w.own = n;
+        w.parts = (n - 1) / w.size + 1;
+    } else {
+        int share = PG_MOST;
+        if (pg_splits(c.plan, units)) /* as many for each unit as there are */
+            share =
+                pg_share_last(pg_max((n - 1) / (c.plan.goal / units) + 1, PG_MANY_LEAST), n);
+        w.parts = pg_nshare(n, share);
+    }
+    w.unit = target / w.parts;
+    w.first = w.unit * w.parts;
+    w.part = target - w.first;
+    w.b = w.unit < units ? 0 : -1;
     return w;
 }
 /* The slot of part `at` of a kv-head */
@@ -256,7 +285,7 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
     constexpr uint32_t EB = E4M3 ? 1 : 2, SLICE = PSLICE * EB;
     __shared__ bf16x8 sq[8 * 64];
     const int kh = blockIdx.x % c.Hkv;
-    Where w = locate<FEW, true>(c, blockIdx.x / c.Hkv);
+    Where w = locate<FEW>(c, blockIdx.x / c.Hkv);
     /* the units that the piece lies in */
     while (w.b >= 0) {
     const int lane = lane_again(), m = lane & 15, g = lane >> 4;
@@ -473,6 +502,8 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
         }
     }
     lrun = fold_rows(lrun, [](float a, float b) { return a + b; });
+    if (w.part == 0 && kh == 0 && c.plan.slots > 0 && lane_again() == 0)
+        c.info[b] = int2{w.first, w.parts};
 
     /* lane (m, g) holds dims 16 t + 4 g .. + 3 of row m. Both are worked out again:
      * kept over the loop they went to scratch memory. */
@@ -602,7 +633,7 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
     }
     if (at >= c.plan.shares)
         return;
-    const Where w = locate<RT, true>(c, c.plan.shares - 1 - at);
+    const Where w = locate<RT>(c, c.plan.shares - 1 - at);
     if (w.b < 0)
         return;
     const pg_seq s = w.s;
@@ -1164,21 +1195,23 @@ template <bool ROW> __global__ __launch_bounds__(256) void merge_few_kernel(Call
     constexpr int STEP = ROW ? 64 : 16, PER = STEP / 16;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int group = blockIdx.x % groups, kh = blockIdx.x / groups % c.Hkv;
-    const Where w = locate<FEW, false>(c, blockIdx.x / groups / c.Hkv);
-    const int r = ROW ? group : group * 4 + wave;
-    if (w.b < 0 || w.parts <= 1 || r >= w.s.ql * c.G)
+    const int b = blockIdx.x / groups / c.Hkv, r = ROW ? group : group * 4 + wave;
+    const pg_seq s = seq_of(c, b);
+    const int2 info = c.info[b]; /* of a sequence with rows */
+    if (r >= s.ql * c.G || info.y <= 1)
         return;
+    const int first = info.x, parts = info.y;
     const size_t slot0 = slot_of(c, kh, 0);
-    auto at = [&](int j) { return (slot0 + pg_few_slot(w.first, j)) * FEW + r; };
+    auto at = [&](int j) { return (slot0 + pg_few_slot(first, j)) * FEW + r; };
     const int dim = ROW ? 64 * wave + 4 * (lane & 15) : 4 * lane, own = ROW ? lane >> 4 : 0;
-    const int tok = r * c.rG >> 16, n = w.s.q0 + tok, head = kh * c.G + r - tok * c.G;
+    const int tok = r * c.rG >> 16, n = s.q0 + tok, head = kh * c.G + r - tok * c.G;
     bf16x4 gv = {};
     if (c.gate)
         gv = *(const bf16x4 *)(c.gate + (size_t)n * c.gts + (size_t)head * c.ghs + dim);
     float mu = -INFINITY, l = 0.f;
     floatx4 acc = {};
-    for (int j0 = 0; j0 < w.parts; j0 += 64) { /* more than 64 parts: in turns */
-        const int cnt = min(w.parts - j0, 64);
+    for (int j0 = 0; j0 < parts; j0 += 64) { /* more than 64 parts: in turns */
+        const int cnt = min(parts - j0, 64);
         const size_t mine = at(j0 + min(lane, cnt - 1));
         const float pl = c.pl[mine], pm = c.pmu[mine];
         const float li = lane < cnt ? pl : 0.f, mi = li > 0.f ? pm : -INFINITY;
@@ -1232,9 +1265,10 @@ __global__ __launch_bounds__(256) void merge_many_kernel(Call c) {
     constexpr int R = 4, GROUPS = RT / (4 * R);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int group = blockIdx.x % GROUPS, kh = blockIdx.x / GROUPS % c.Hkv;
-    const Where w = locate<RT, false>(c, blockIdx.x / GROUPS / c.Hkv);
+    const Where w = locate<RT>(c, blockIdx.x / GROUPS / c.Hkv);
     const int r0 = w.unit * RT, t0 = (group * 4 + wave) * R;
-    if (w.b < 0 || w.parts <= 1 || t0 >= min(w.s.ql * c.G - r0, RT) ||
+    /* the first part's workgroups do it */
+    if (w.b < 0 || w.parts <= 1 || w.part > 0 || t0 >= min(w.s.ql * c.G - r0, RT) ||
         w.first + w.parts > c.plan.slots) /* more than any rising q_start has */
         return;
     const int last = min(w.s.ql * c.G - r0, RT) - 1;
@@ -1308,11 +1342,19 @@ __global__ __launch_bounds__(256) void merge_many_kernel(Call c) {
 } // namespace CUJEV_KNS
 using namespace CUJEV_KNS;
 
+/* o, l and mu of the slots' rows, then info */
+static size_t ws_bytes_of(const pg_plan &p, int Hkv) {
+    if (p.slots <= 0)
+        return 0;
+    return (size_t)p.slots * Hkv * p.rt * (PD + 2) * sizeof(float) +
+           (p.rt == FEW ? (size_t)p.units * sizeof(int2) : 0);
+}
+
 extern "C" size_t cujev_attention_paged_ws_bytes(int N, int B, int max_q, int max_kv, int Hq,
                                                  int Hkv, int window, int sinks, int type) {
     (void)type; /* the plan goes by key tiles */
     const pg_plan p = pg_make_plan(N, B, max_q, max_kv, Hq / Hkv, Hkv, window, sinks);
-    return (size_t)p.slots * Hkv * p.rt * (PD + 2) * sizeof(float);
+    return ws_bytes_of(p, Hkv);
 }
 
 extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int gate_tok_stride,
@@ -1328,7 +1370,7 @@ extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int
     if (p.shares < 0)
         return hipErrorInvalidValue;
     const size_t rows = (size_t)p.slots * Hkv * p.rt;
-    if (rows * (PD + 2) * sizeof(float) > ws_bytes)
+    if (ws_bytes_of(p, Hkv) > ws_bytes)
         return hipErrorInvalidValue;
     if (window >= max_kv) /* no row's window ends before its first key */
         window = sinks = 0;
@@ -1337,7 +1379,8 @@ extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int
                     seqs->q_start, seqs->kv_len, seqs->page_table, seqs->max_pages, B, N,
                     max_q, max_kv, Hq, Hkv, G, window, sinks,
                     pg_div_up(65536, G), (bf16 *)out,
-                    (float *)ws, (float *)ws + rows * PD, (float *)ws + rows * (PD + 1), p};
+                    (float *)ws, (float *)ws + rows * PD, (float *)ws + rows * (PD + 1),
+                    (int2 *)((float *)ws + rows * (PD + 2)), p};
     const bool few = p.rt == FEW;
     const int per = !few && 8 % Hkv == 0 ? 8 / Hkv : 1;
     const dim3 grid((unsigned)(pg_div_up(p.shares, per) * per * Hkv)); /* all parts */
@@ -1353,7 +1396,7 @@ extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int
         const int rows = pg_min(max_q, N) * G;
         const bool row = few && (long long)p.units * rows * Hkv <= 512;
         const int groups = !few ? RT / 16 : row ? rows : pg_div_up(rows, 4);
-        const dim3 mgrid((unsigned)(p.units * Hkv * groups));
+        const dim3 mgrid((unsigned)((few ? p.units : p.slots) * Hkv * groups));
         if (row)
             hipLaunchKernelGGL(merge_few_kernel<true>, mgrid, dim3(256), 0, stream, c, groups);
         else if (few)

@@ -117,15 +117,26 @@ DEV float to_odd(double d) {
 
 /* The sequences of rows n0 .. n0 + TOK - 1, row n0 + t in lane t: the last b
  * with q_start[b] <= n, -1 for a row before the first or behind the last
- * sequence. One load of 64 starts a step; up to 64 sequences' lengths come
- * beside them and not after. */
+ * sequence. Up to 64 sequences' starts and lengths come in one go; of more, 64
+ * starts spread over those that are left narrow them down to 64 first. */
 template <int TOK>
 DEV int find_seqs(const int32_t *q_start, const int32_t *kv_len, int B, int N, int max_kv, int n0,
                   pg_seq *s) {
     const int lane = threadIdx.x & 63;
-    int before[TOK] = {}; /* starts <= n among q_start[0 .. B] */
     const pg_seq mine = load_seq(q_start, kv_len, min(lane, B - 1), N, N, max_kv);
-    for (int b0 = 0; b0 <= B; b0 += 64) {
+    int from = 0; /* starts before it are <= n0 */
+    for (int len = B + 1; len > 64;) {
+        const int stride = (len + 63) / 64;
+        const int v = q_start[min(from + lane * stride, B)];
+        const int c = __popcll(__ballot(lane * stride < len && v <= n0));
+        from += max(c - 1, 0) * stride;
+        len = min(len - max(c - 1, 0) * stride, stride);
+    }
+    int before[TOK]; /* starts <= n among q_start[0 .. B] */
+#pragma unroll
+    for (int t = 0; t < TOK; t++)
+        before[t] = from;
+    for (int b0 = from; b0 <= B; b0 += 64) {
         const int v = q_start[min(b0 + lane, B)];
         int c = 0;
 #pragma unroll
@@ -150,27 +161,48 @@ DEV int find_seqs(const int32_t *q_start, const int32_t *kv_len, int B, int N, i
 }
 
 /* Work item `item` of a launch whose sequence b has count(b, s) of them, in
- * order: the sequence, and the item's number in it (-1: no such item). */
+ * order: the sequence, and the item's number in it (-1: no such item). J
+ * sequences a lane, 64 J a step. */
+template <int J, typename F>
+DEV int find_item_among(const int32_t *q_start, const int32_t *kv_len, int B, int N, int max_q,
+                        int max_kv, int item, F count, pg_seq *s, int *local) {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int b0 = 0; b0 < B; b0 += 64 * J) {
+        pg_seq mine[J];
+        int own[J], sum = 0;
+#pragma unroll
+        for (int j = 0; j < J; j++)
+            mine[j] = load_seq(q_start, kv_len, min(b0 + J * lane + j, B - 1), N, max_q, max_kv);
+#pragma unroll
+        for (int j = 0; j < J; j++)
+            sum += own[j] = b0 + J * lane + j < B ? count(mine[j]) : 0;
+        const int to = before + wave_scan(sum);
+        const uint64_t past = __ballot(to > item);
+        if (past) {
+            const int l = __ffsll((unsigned long long)past) - 1;
+            int at = __builtin_amdgcn_readlane(to - sum, l), b = 0;
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+                const int here = __builtin_amdgcn_readlane(own[j], l);
+                if (item >= at && item < at + here) {
+                    *s = seq_at(mine[j], l);
+                    *local = item - at;
+                    b = b0 + J * l + j;
+                }
+                at += here;
+            }
+            return b;
+        }
+        before = last_lane(to);
+    }
+    return -1;
+}
 template <typename F>
 DEV int find_item(const int32_t *q_start, const int32_t *kv_len, int B, int N, int max_q,
                   int max_kv, int item, F count, pg_seq *s, int *local) {
-    const int lane = threadIdx.x & 63;
-    int before = 0;
-    for (int b0 = 0; b0 < B; b0 += 64) {
-        const pg_seq mine =
-            load_seq(q_start, kv_len, min(b0 + lane, B - 1), N, max_q, max_kv);
-        const int own = b0 + lane < B ? count(mine) : 0;
-        const int sum = before + wave_scan(own);
-        const uint64_t past = __ballot(sum > item);
-        if (past) {
-            const int l = __ffsll((unsigned long long)past) - 1;
-            *s = seq_at(mine, l);
-            *local = item - __builtin_amdgcn_readlane(sum - own, l);
-            return b0 + l;
-        }
-        before = last_lane(sum);
-    }
-    return -1;
+    return B > 64 ? find_item_among<4>(q_start, kv_len, B, N, max_q, max_kv, item, count, s, local)
+                  : find_item_among<1>(q_start, kv_len, B, N, max_q, max_kv, item, count, s, local);
 }
 
 /* Scale of a row whose largest magnitude is a: 2^e, e the least integer with

@@ -93,6 +93,7 @@ PREP = [
     (6, 1, True, [(5, 3), (64, 128), (3, 66)]),     # the first has fewer keys than tokens
     (16, 2, False, [(3, 66)] * 3 + [(0, 5)] * 70 + [(2, 63)] * 70),  # more than 64 sequences
     (4, 4, True, [(2, 63)] * 70 + [(33, 90)]),
+    (4, 1, False, [(1, 3), (0, 5), (2, 66)] * 1500),  # past 64 x 64 of them
 ]
 
 
@@ -603,6 +604,17 @@ def test_attention_of_one_token_over_many_uneven_sequences(window, sinks, e4m3):
     check_attention(c, window, sinks)
     # of bounds far above the lengths, the work is shared out otherwise
     check_attention(c, window, sinks, max_q=3, max_kv=700)
+
+
+@pytest.mark.parametrize("q", [1, 40])
+def test_attention_of_hundreds_of_sequences(q):
+    """More than the 256 that a step of the plan takes, with and without shares."""
+    g = torch.Generator().manual_seed(191)
+    lens = [(min(int(n), q), int(k)) for n, k in zip(torch.randint(0, q + 1, (700,), generator=g),
+                                                     torch.randint(40, 150, (700,), generator=g))]
+    check_attention(attention_case(192, 4, 1, False, lens), max_kv=150)
+    lens = [(0, 9)] * 600 + [(q, 1400), (1, 70)] + [(0, 9)] * 100
+    check_attention(attention_case(193, 4, 1, True, lens))
 
 
 @pytest.mark.parametrize("e4m3", [False, True])
