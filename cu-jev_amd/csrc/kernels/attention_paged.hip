@@ -57,30 +57,32 @@ DEV float hide(bool seen, float x) {
     return __uint_as_float(seen ? __float_as_uint(x) : 0xff800000u);
 }
 
-/* v_mfma_f32_32x32x16_bf16 by hand, so that O and Q stay in accumulation
- * registers and the scores in ordinary ones; with the builtin the compiler
- * moved Q's operands over before each MFMA. What it leaves to the code around it: two wait states between a VALU write of an
- * operand and the MFMA (NOP), and 18 between an MFMA and a read of its result
- * by anything but the next MFMA on it (settle()). Operands from LDS are waited
- * for as for any instruction. */
+/* v_mfma_f32_32x32x16_bf16 by hand, so that O and Q stay in accumulation registers
+ * and the scores in ordinary ones; with the builtin the compiler moved Q's operands
+ * over before each MFMA. What it leaves to the code around it: two wait states
+ * between a VALU write of an operand and the MFMA (NOP), and 18 between an MFMA and
+ * a read of its result by anything but the next MFMA on it (settle()). Operands from
+ * LDS are waited for as for any instruction. */
+#define MFMA "v_mfma_f32_32x32x16_bf16 "
 template <bool NOP> DEV void mfma_first(floatx16 &s, bf16x8 a, bf16x8 q) {
     if constexpr (NOP)
-        asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(a), "a"(q));
+        asm volatile("s_nop 1\n\t" MFMA "%0, %1, %2, 0" : "=&v"(s) : "v"(a), "a"(q));
     else
-        asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(a), "a"(q));
+        asm volatile(MFMA "%0, %1, %2, 0" : "=&v"(s) : "v"(a), "a"(q));
 }
 template <bool NOP> DEV void mfma_score(floatx16 &s, bf16x8 a, bf16x8 q) {
     if constexpr (NOP)
-        asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(a), "a"(q));
+        asm volatile("s_nop 1\n\t" MFMA "%0, %1, %2, %0" : "+v"(s) : "v"(a), "a"(q));
     else
-        asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(a), "a"(q));
+        asm volatile(MFMA "%0, %1, %2, %0" : "+v"(s) : "v"(a), "a"(q));
 }
 template <bool NOP> DEV void mfma_out(floatx16 &o, bf16x8 a, bf16x8 p) {
     if constexpr (NOP)
-        asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(p));
+        asm volatile("s_nop 1\n\t" MFMA "%0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(p));
     else
-        asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(p));
+        asm volatile(MFMA "%0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(p));
 }
+#undef MFMA
 /* before O is read or written by anything but mfma_out, and after */
 DEV void settle(floatx16 (&o)[4]) {
     asm volatile("s_nop 15\n\ts_nop 7" : "+a"(o[0]), "+a"(o[1]), "+a"(o[2]), "+a"(o[3]));
@@ -288,272 +290,272 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
     Where w = locate<FEW>(c, blockIdx.x / c.Hkv);
     /* the units that the piece lies in */
     while (w.b >= 0) {
-    const int lane = lane_again(), m = lane & 15, g = lane >> 4;
-    const pg_seq s = w.s;
-    const int b = w.b, rows = min(s.ql * c.G, FEW);
-    const pg_tiles list = pg_tile_list(s, 0, s.ql - 1, c.window, c.sinks);
-    /* tiles [i0, i1) of the unit's; a unit without a key has one that is not there */
-    const int cut = (w.first + w.part) * w.size - w.begin;
-    const int i0 = max(cut, 0), i1 = min(min(cut + w.size, w.own), list.ntl);
-    /* the ids of 64 tiles of the list are in a lane each */
-    int ids = i0 < i1 ? page_id(c, b, list, min(i0 + lane, list.ntl - 1)) : -1, ids0 = i0;
+        const int lane = lane_again(), m = lane & 15, g = lane >> 4;
+        const pg_seq s = w.s;
+        const int b = w.b, rows = min(s.ql * c.G, FEW);
+        const pg_tiles list = pg_tile_list(s, 0, s.ql - 1, c.window, c.sinks);
+        /* tiles [i0, i1) of the unit's; a unit without a key has one that is not there */
+        const int cut = (w.first + w.part) * w.size - w.begin;
+        const int i0 = max(cut, 0), i1 = min(min(cut + w.size, w.own), list.ntl);
+        /* the ids of 64 tiles of the list are in a lane each */
+        int ids = i0 < i1 ? page_id(c, b, list, min(i0 + lane, list.ntl - 1)) : -1, ids0 = i0;
 
-    /* this lane's row (column of S^T and O^T) */
-    const int row = min(m, rows - 1), tok = row * c.rG >> 16, head = kh * c.G + row - tok * c.G;
-    const int hi = min(s.p0 + tok, s.kv - 1), lo = pg_low(s.p0 + tok, c.window);
-    const int own_lo = pg_low(s.p0, c.window); /* of the first row: below, no row's key */
-    bf16x8 *const qf = sq + lane;
-    {
-        const bf16 *qp = c.q + ((size_t)(s.q0 + tok) * c.Hq + head) * PD;
+        /* this lane's row (column of S^T and O^T) */
+        const int row = min(m, rows - 1), tok = row * c.rG >> 16, head = kh * c.G + row - tok * c.G;
+        const int hi = min(s.p0 + tok, s.kv - 1), lo = pg_low(s.p0 + tok, c.window);
+        const int own_lo = pg_low(s.p0, c.window); /* of the first row: below, no row's key */
+        bf16x8 *const qf = sq + lane;
+        {
+            const bf16 *qp = c.q + ((size_t)(s.q0 + tok) * c.Hq + head) * PD;
 #pragma unroll
-        for (int ks = 0; ks < 8; ks++) /* dims as K's loads below */
-            qf[64 * ks] = *(const bf16x8 *)(qp + (E4M3 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1)
-                                                       : 32 * ks + 8 * g));
-    }
-
-    /* Row m of score block kb is key key0 + kkey(kb): lane g then holds, in
-     * accumulators v = 4 kb .. + 3, the keys key_of(v) that its V^T loads bring. */
-    const int key0 = (E4M3 ? 16 : 8) * (m >> 2) + (m & 3), keyg = (E4M3 ? 16 : 8) * g;
-    auto kkey = [](int kb) { return E4M3 ? 4 * kb : 4 * (kb & 1) + 32 * (kb >> 1); };
-    auto key_of = [&](int v) { return keyg + (E4M3 ? v : (v & 7) + 32 * (v >> 3)); };
-    const uint32_t kvoff = key0 * PD * EB + 16 * g, vvoff = m * PG * EB + 16 * g;
-
-    u32x4 ra[16] = {}, rb[16] = {}; /* e4m3: K, V^T; bf16: the first half of each, the second */
-    float ksc[4] = {}, vsc = 1.f;
-    auto rsrc = [&](const void *p, int page) {
-        return make_rsrc((const char *)p + ((size_t)max(page, 0) * c.Hkv + kh) * SLICE, SLICE);
-    };
-    auto scale = [&](const float *p, int page, int key) { /* without a 64-bit address a lane */
-        const __amdgpu_buffer_rsrc_t src =
-            make_rsrc(p + ((size_t)max(page, 0) * c.Hkv + kh) * PG, PG * 4);
-        return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(src, key * 4, 0, 0));
-    };
-    /* K: e4m3 all score blocks, bf16 blocks 2 part and 2 part + 1 */
-    auto load_k = [&](u32x4 (&r)[16], int page, int part) {
-        const __amdgpu_buffer_rsrc_t src = rsrc(c.k, page);
-#pragma unroll
-        for (int k = 0; k < (E4M3 ? 4 : 2); k++)
-#pragma unroll
-            for (int i = 0; i < (E4M3 ? 4 : 8); i++) /* the halves of a line in turn */
-                r[i * (E4M3 ? 4 : 2) + k] =
-                    buf_load16(src, kvoff, kkey((E4M3 ? 0 : 2 * part) + k) * PD * EB + 64 * i);
-        if constexpr (E4M3) {
-#pragma unroll
-            for (int kb = 0; kb < 4; kb++)
-                ksc[kb] = scale(c.ks, page, key0 + 4 * kb);
+            for (int ks = 0; ks < 8; ks++) /* dims as K's loads below */
+                qf[64 * ks] = *(const bf16x8 *)(qp + (E4M3 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1)
+                                                           : 32 * ks + 8 * g));
         }
-    };
-    /* V^T: e4m3 all 16 rows of 16 dims, bf16 8 of them, two halves of 32 keys each */
-    auto load_v = [&](u32x4 (&r)[16], int page, int part) {
-        const __amdgpu_buffer_rsrc_t src = rsrc(c.vt, page);
-#pragma unroll
-        for (int i = 0; i < 16; i++)
-            r[i] = E4M3 ? buf_load16(src, vvoff + (i & 1) * 1024, (i >> 1) * 2048)
-                        : buf_load16(src, vvoff + (i & 1) * 64, (8 * part + (i >> 1)) * 2048);
-        if constexpr (E4M3) /* the scale of key keyg + m, in lane m of the 16 that need all 16 */
-            vsc = scale(c.vs, page, keyg + m);
-    };
-    /* tile t (past the last: it again): its page, -1 if it is not there */
-    auto page_of = [&](int t) {
-        t = min(t, i1 - 1);
-        if (t - ids0 >= 64) {
-            ids0 = t;
-            ids = page_id(c, b, list, min(t + lane, list.ntl - 1));
-        }
-        return __builtin_amdgcn_readlane(ids, t - ids0);
-    };
 
-    floatx4 o[16];
-#pragma unroll
-    for (int t = 0; t < 16; t++)
-        o[t] = floatx4{};
-    float mrun = -INFINITY, lrun = 0.f;
-    int next = -1;
-    if (i0 < i1) {
-        next = page_of(i0);
-        load_k(ra, next, 0);
-        if constexpr (!E4M3)
-            load_k(rb, next, 1);
-    }
-    for (int i = i0; i < i1; i++) {
-        const int page = next, k0 = pg_tile_page(list, i) * PG;
-        const bool there = page >= 0;
-        if constexpr (E4M3)
-            load_v(rb, page, 0);
-        next = page_of(i + 1);
+        /* Row m of score block kb is key key0 + kkey(kb): lane g then holds, in
+         * accumulators v = 4 kb .. + 3, the keys key_of(v) that its V^T loads bring. */
+        const int key0 = (E4M3 ? 16 : 8) * (m >> 2) + (m & 3), keyg = (E4M3 ? 16 : 8) * g;
+        auto kkey = [](int kb) { return E4M3 ? 4 * kb : 4 * (kb & 1) + 32 * (kb >> 1); };
+        auto key_of = [&](int v) { return keyg + (E4M3 ? v : (v & 7) + 32 * (v >> 3)); };
+        const uint32_t kvoff = key0 * PD * EB + 16 * g, vvoff = m * PG * EB + 16 * g;
 
-        asm volatile("" ::: "memory"); /* Q is read here, not kept */
-        floatx4 x[4];
-        if constexpr (E4M3) {
+        u32x4 ra[16] = {}, rb[16] = {}; /* e4m3: K, V^T; bf16: the first half of each, the second */
+        float ksc[4] = {}, vsc = 1.f;
+        auto rsrc = [&](const void *p, int page) {
+            return make_rsrc((const char *)p + ((size_t)max(page, 0) * c.Hkv + kh) * SLICE, SLICE);
+        };
+        auto scale = [&](const float *p, int page, int key) { /* without a 64-bit address a lane */
+            const __amdgpu_buffer_rsrc_t src =
+                make_rsrc(p + ((size_t)max(page, 0) * c.Hkv + kh) * PG, PG * 4);
+            return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(src, key * 4, 0, 0));
+        };
+        /* K: e4m3 all score blocks, bf16 blocks 2 part and 2 part + 1 */
+        auto load_k = [&](u32x4 (&r)[16], int page, int part) {
+            const __amdgpu_buffer_rsrc_t src = rsrc(c.k, page);
 #pragma unroll
-            for (int ks = 0; ks < 8; ks++) {
-                const bf16x8 q = qf[64 * ks];
+            for (int k = 0; k < (E4M3 ? 4 : 2); k++)
 #pragma unroll
-                for (int kb = 0; kb < 4; kb++) {
-                    const u32x4 v = ra[(ks >> 1) * 4 + kb];
-                    x[kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                        ks & 1 ? widen(v[2], v[3], ksc[kb]) : widen(v[0], v[1], ksc[kb]), q,
-                        ks == 0 ? floatx4{} : x[kb], 0, 0, 0);
-                }
+                for (int i = 0; i < (E4M3 ? 4 : 8); i++) /* the halves of a line in turn */
+                    r[i * (E4M3 ? 4 : 2) + k] =
+                        buf_load16(src, kvoff, kkey((E4M3 ? 0 : 2 * part) + k) * PD * EB + 64 * i);
+            if constexpr (E4M3) {
+#pragma unroll
+                for (int kb = 0; kb < 4; kb++)
+                    ksc[kb] = scale(c.ks, page, key0 + 4 * kb);
             }
+        };
+        /* V^T: e4m3 all 16 rows of 16 dims, bf16 8 of them, two halves of 32 keys each */
+        auto load_v = [&](u32x4 (&r)[16], int page, int part) {
+            const __amdgpu_buffer_rsrc_t src = rsrc(c.vt, page);
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                r[i] = E4M3 ? buf_load16(src, vvoff + (i & 1) * 1024, (i >> 1) * 2048)
+                            : buf_load16(src, vvoff + (i & 1) * 64, (8 * part + (i >> 1)) * 2048);
+            if constexpr (E4M3) /* of key keyg + m, in lane m of the 16 that need all 16 */
+                vsc = scale(c.vs, page, keyg + m);
+        };
+        /* tile t (past the last: it again): its page, -1 if it is not there */
+        auto page_of = [&](int t) {
+            t = min(t, i1 - 1);
+            if (t - ids0 >= 64) {
+                ids0 = t;
+                ids = page_id(c, b, list, min(t + lane, list.ntl - 1));
+            }
+            return __builtin_amdgcn_readlane(ids, t - ids0);
+        };
+
+        floatx4 o[16];
+#pragma unroll
+        for (int t = 0; t < 16; t++)
+            o[t] = floatx4{};
+        float mrun = -INFINITY, lrun = 0.f;
+        int next = -1;
+        if (i0 < i1) {
+            next = page_of(i0);
             load_k(ra, next, 0);
-        } else {
-            auto scores = [&](u32x4 (&r)[16], int part) {
+            if constexpr (!E4M3)
+                load_k(rb, next, 1);
+        }
+        for (int i = i0; i < i1; i++) {
+            const int page = next, k0 = pg_tile_page(list, i) * PG;
+            const bool there = page >= 0;
+            if constexpr (E4M3)
+                load_v(rb, page, 0);
+            next = page_of(i + 1);
+
+            asm volatile("" ::: "memory"); /* Q is read here, not kept */
+            floatx4 x[4];
+            if constexpr (E4M3) {
 #pragma unroll
                 for (int ks = 0; ks < 8; ks++) {
                     const bf16x8 q = qf[64 * ks];
 #pragma unroll
-                    for (int k = 0; k < 2; k++)
-                        x[2 * part + k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                            __builtin_bit_cast(bf16x8, r[2 * ks + k]), q,
-                            ks == 0 ? floatx4{} : x[2 * part + k], 0, 0, 0);
+                    for (int kb = 0; kb < 4; kb++) {
+                        const u32x4 v = ra[(ks >> 1) * 4 + kb];
+                        x[kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            ks & 1 ? widen(v[2], v[3], ksc[kb]) : widen(v[0], v[1], ksc[kb]), q,
+                            ks == 0 ? floatx4{} : x[kb], 0, 0, 0);
+                    }
                 }
-            };
-            scores(ra, 0);
-            load_v(ra, page, 0);
-            scores(rb, 1);
-            load_v(rb, page, 1);
-        }
+                load_k(ra, next, 0);
+            } else {
+                auto scores = [&](u32x4 (&r)[16], int part) {
+#pragma unroll
+                    for (int ks = 0; ks < 8; ks++) {
+                        const bf16x8 q = qf[64 * ks];
+#pragma unroll
+                        for (int k = 0; k < 2; k++)
+                            x[2 * part + k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                __builtin_bit_cast(bf16x8, r[2 * ks + k]), q,
+                                ks == 0 ? floatx4{} : x[2 * part + k], 0, 0, 0);
+                    }
+                };
+                scores(ra, 0);
+                load_v(ra, page, 0);
+                scores(rb, 1);
+                load_v(rb, page, 1);
+            }
 
-        /* bits to keep of V^T values: those of no key of this call, whatever they
-         * are, meet p = 0 */
-        u32x4 keep[E4M3 ? 1 : 2];
-        bool foreign = false;
-        if (!there || k0 + PG - 1 > min(s.p0, s.kv - 1) || c.window > 0) { /* some key hidden */
-            const int top = there ? s.kv - 1 : -1;
+            /* bits to keep of V^T values: those of no key of this call, whatever they
+             * are, meet p = 0 */
+            u32x4 keep[E4M3 ? 1 : 2];
+            bool foreign = false;
+            if (!there || k0 + PG - 1 > min(s.p0, s.kv - 1) || c.window > 0) { /* some key hidden */
+                const int top = there ? s.kv - 1 : -1;
+#pragma unroll
+                for (int v = 0; v < 16; v++)
+                    x[v >> 2][v & 3] =
+                        hide(key_seen(k0 + key_of(v), min(hi, top), lo, c.sinks), x[v >> 2][v & 3]);
+                foreign = !there || pg_tile_foreign(k0, s.p0, s.kv, c.window, c.sinks);
+                if (foreign) {
+#pragma unroll
+                    for (int h = 0; h < (E4M3 ? 1 : 2); h++)
+#pragma unroll
+                        for (int d = 0; d < 4; d++) {
+                            uint32_t k = 0;
+#pragma unroll
+                            for (int e = 0; e < (E4M3 ? 4 : 2); e++) {
+                                const int j = k0 + key_of(E4M3 ? 4 * d + e : 8 * h + 2 * d + e);
+                                k |= key_seen(j, top, own_lo, c.sinks)
+                                         ? (E4M3 ? 0xffu << (8 * e) : 0xffffu << (16 * e))
+                                         : 0u;
+                            }
+                            keep[h][d] = k;
+                        }
+                    vsc = __uint_as_float(
+                        key_seen(k0 + keyg + m, top, own_lo, c.sinks) ? __float_as_uint(vsc) : 0u);
+                }
+            }
+            float mx = -INFINITY;
 #pragma unroll
             for (int v = 0; v < 16; v++)
-                x[v >> 2][v & 3] =
-                    hide(key_seen(k0 + key_of(v), min(hi, top), lo, c.sinks), x[v >> 2][v & 3]);
-            foreign = !there || pg_tile_foreign(k0, s.p0, s.kv, c.window, c.sinks);
-            if (foreign) {
-#pragma unroll
-                for (int h = 0; h < (E4M3 ? 1 : 2); h++)
-#pragma unroll
-                    for (int d = 0; d < 4; d++) {
-                        uint32_t k = 0;
-#pragma unroll
-                        for (int e = 0; e < (E4M3 ? 4 : 2); e++) {
-                            const int j = k0 + key_of(E4M3 ? 4 * d + e : 8 * h + 2 * d + e);
-                            k |= key_seen(j, top, own_lo, c.sinks)
-                                     ? (E4M3 ? 0xffu << (8 * e) : 0xffffu << (16 * e))
-                                     : 0u;
-                        }
-                        keep[h][d] = k;
-                    }
-                vsc = __uint_as_float(
-                    key_seen(k0 + keyg + m, top, own_lo, c.sinks) ? __float_as_uint(vsc) : 0u);
-            }
-        }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int v = 0; v < 16; v++)
-            mx = fmaxf(mx, x[v >> 2][v & 3]);
-        mx = fold_rows(mx, [](float a, float b) { return fmaxf(a, b); });
-        const float mnew = fmaxf(mrun, mx);
-        const float ref = mnew == -INFINITY ? 0.f : mnew; /* no key yet: p = 2^-inf = 0 */
-        if (__any(mnew != mrun)) {
-            const float a = fast_exp2(mrun - ref);
-            lrun *= a;
-#pragma unroll
-            for (int t = 0; t < 16; t++)
-                o[t] *= a;
-        }
-        mrun = mnew;
-        bf16x8 p[2];
-        unroll_for<16>([&](auto iv) {
-            constexpr int v = decltype(iv)::value;
-            float pv = fast_exp2(x[v >> 2][v & 3] - ref);
-            lrun += pv;
-            if constexpr (E4M3)
-                pv *= row_lane<v>(vsc);
-            p[v >> 3][v & 7] = f2bf(pv);
-        });
-        if constexpr (E4M3) {
-            if (foreign) {
+                mx = fmaxf(mx, x[v >> 2][v & 3]);
+            mx = fold_rows(mx, [](float a, float b) { return fmaxf(a, b); });
+            const float mnew = fmaxf(mrun, mx);
+            const float ref = mnew == -INFINITY ? 0.f : mnew; /* no key yet: p = 2^-inf = 0 */
+            if (__any(mnew != mrun)) {
+                const float a = fast_exp2(mrun - ref);
+                lrun *= a;
 #pragma unroll
                 for (int t = 0; t < 16; t++)
-                    rb[t] &= keep[0];
+                    o[t] *= a;
+            }
+            mrun = mnew;
+            bf16x8 p[2];
+            unroll_for<16>([&](auto iv) {
+                constexpr int v = decltype(iv)::value;
+                float pv = fast_exp2(x[v >> 2][v & 3] - ref);
+                lrun += pv;
+                if constexpr (E4M3)
+                    pv *= row_lane<v>(vsc);
+                p[v >> 3][v & 7] = f2bf(pv);
+            });
+            if constexpr (E4M3) {
+                if (foreign) {
+#pragma unroll
+                    for (int t = 0; t < 16; t++)
+                        rb[t] &= keep[0];
+                }
+#pragma unroll
+                for (int t = 0; t < 16; t++) {
+                    o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(rb[t][0], rb[t][1], 1.f),
+                                                                   p[0], o[t], 0, 0, 0);
+                    o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(rb[t][2], rb[t][3], 1.f),
+                                                                   p[1], o[t], 0, 0, 0);
+                }
+            } else {
+                auto values = [&](u32x4 (&r)[16], int part) {
+                    if (foreign) {
+#pragma unroll
+                        for (int j = 0; j < 16; j++)
+                            r[j] &= keep[j & 1];
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; j++)
+                        o[8 * part + (j >> 1)] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            __builtin_bit_cast(bf16x8, r[j]), p[j & 1],
+                            o[8 * part + (j >> 1)], 0, 0, 0);
+                };
+                values(ra, 0);
+                load_k(ra, next, 0);
+                values(rb, 1);
+                load_k(rb, next, 1);
+            }
+        }
+        lrun = fold_rows(lrun, [](float a, float b) { return a + b; });
+        if (w.part == 0 && kh == 0 && c.plan.slots > 0 && lane_again() == 0)
+            c.info[b] = int2{w.first, w.parts};
+
+        /* lane (m, g) holds dims 16 t + 4 g .. + 3 of row m. Both are worked out again:
+         * kept over the loop they went to scratch memory. */
+        const int id = lane_again(), r = id & 15, d0 = id >> 4 << 2;
+        if (w.parts > 1) {
+            const size_t slot = slot_of(c, kh, pg_few_slot(w.first, w.part));
+            if (r < rows) {
+#pragma unroll
+                for (int t = 0; t < 16; t++)
+                    *(floatx4 *)(c.po + (slot * FEW + r) * PD + 16 * t + d0) = o[t];
+                if (d0 == 0) {
+                    c.pl[slot * FEW + r] = lrun;
+                    c.pmu[slot * FEW + r] = mrun == -INFINITY ? 0.f : mrun;
+                }
+            }
+        } else if (r < rows) {
+            const float inv = lrun > 0.f ? 1.f / lrun : 0.f;
+            const int tk = r * c.rG >> 16, n = s.q0 + tk, hd = kh * c.G + r - tk * c.G;
+            bf16x4 gv[16] = {};
+            if (c.gate) {
+                const bf16 *gp = c.gate + (size_t)n * c.gts + (size_t)hd * c.ghs + d0;
+#pragma unroll
+                for (int t = 0; t < 16; t++)
+                    gv[t] = *(const bf16x4 *)(gp + 16 * t);
             }
 #pragma unroll
             for (int t = 0; t < 16; t++) {
-                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(rb[t][0], rb[t][1], 1.f),
-                                                               p[0], o[t], 0, 0, 0);
-                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(rb[t][2], rb[t][3], 1.f),
-                                                               p[1], o[t], 0, 0, 0);
-            }
-        } else {
-            auto values = [&](u32x4 (&r)[16], int part) {
-                if (foreign) {
+                bf16x4 res;
 #pragma unroll
-                    for (int j = 0; j < 16; j++)
-                        r[j] &= keep[j & 1];
-                }
-#pragma unroll
-                for (int j = 0; j < 16; j++)
-                    o[8 * part + (j >> 1)] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                        __builtin_bit_cast(bf16x8, r[j]), p[j & 1], o[8 * part + (j >> 1)], 0, 0,
-                        0);
-            };
-            values(ra, 0);
-            load_k(ra, next, 0);
-            values(rb, 1);
-            load_k(rb, next, 1);
-        }
-    }
-    lrun = fold_rows(lrun, [](float a, float b) { return a + b; });
-    if (w.part == 0 && kh == 0 && c.plan.slots > 0 && lane_again() == 0)
-        c.info[b] = int2{w.first, w.parts};
-
-    /* lane (m, g) holds dims 16 t + 4 g .. + 3 of row m. Both are worked out again:
-     * kept over the loop they went to scratch memory. */
-    const int id = lane_again(), r = id & 15, d0 = id >> 4 << 2;
-    if (w.parts > 1) {
-        const size_t slot = slot_of(c, kh, pg_few_slot(w.first, w.part));
-        if (r < rows) {
-#pragma unroll
-            for (int t = 0; t < 16; t++)
-                *(floatx4 *)(c.po + (slot * FEW + r) * PD + 16 * t + d0) = o[t];
-            if (d0 == 0) {
-                c.pl[slot * FEW + r] = lrun;
-                c.pmu[slot * FEW + r] = mrun == -INFINITY ? 0.f : mrun;
+                for (int e = 0; e < 4; e++)
+                    res[e] = f2bf(o[t][e] * inv * (c.gate ? sigmoid_f(bf2f(gv[t][e])) : 1.f));
+                *(bf16x4 *)(c.out + ((size_t)n * c.Hq + hd) * PD + 16 * t + d0) = res;
             }
         }
-    } else if (r < rows) {
-        const float inv = lrun > 0.f ? 1.f / lrun : 0.f;
-        const int tk = r * c.rG >> 16, n = s.q0 + tk, hd = kh * c.G + r - tk * c.G;
-        bf16x4 gv[16] = {};
-        if (c.gate) {
-            const bf16 *gp = c.gate + (size_t)n * c.gts + (size_t)hd * c.ghs + d0;
-#pragma unroll
-            for (int t = 0; t < 16; t++)
-                gv[t] = *(const bf16x4 *)(gp + 16 * t);
+        /* on to the next unit, if the piece goes on after this one */
+        w.begin += w.own, w.first = w.begin / w.size, w.part = 0;
+        w.b = -1;
+        for (int b0 = cut + w.size <= w.own ? c.B : b + 1; b0 < c.B; b0 += 64) {
+            const int at = lane_again();
+            const pg_seq t = seq_of(c, min(b0 + at, c.B - 1));
+            const uint64_t any = __ballot(b0 + at < c.B && pg_units(t, c.G, FEW) > 0);
+            if (any) {
+                const int l = __ffsll((unsigned long long)any) - 1;
+                w.s = seq_at(t, l);
+                w.b = b0 + l;
+                w.own = pg_longest(w.s, c.G, FEW, c.window, c.sinks);
+                w.parts = (w.begin + w.own - 1) / w.size - w.first + 1;
+                break;
+            }
         }
-#pragma unroll
-        for (int t = 0; t < 16; t++) {
-            bf16x4 res;
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                res[e] = f2bf(o[t][e] * inv * (c.gate ? sigmoid_f(bf2f(gv[t][e])) : 1.f));
-            *(bf16x4 *)(c.out + ((size_t)n * c.Hq + hd) * PD + 16 * t + d0) = res;
-        }
-    }
-    /* on to the next unit, if the piece goes on after this one */
-    w.begin += w.own, w.first = w.begin / w.size, w.part = 0;
-    w.b = -1;
-    for (int b0 = cut + w.size <= w.own ? c.B : b + 1; b0 < c.B; b0 += 64) {
-        const int at = lane_again();
-        const pg_seq t = seq_of(c, min(b0 + at, c.B - 1));
-        const uint64_t any = __ballot(b0 + at < c.B && pg_units(t, c.G, FEW) > 0);
-        if (any) {
-            const int l = __ffsll((unsigned long long)any) - 1;
-            w.s = seq_at(t, l);
-            w.b = b0 + l;
-            w.own = pg_longest(w.s, c.G, FEW, c.window, c.sinks);
-            w.parts = (w.begin + w.own - 1) / w.size - w.first + 1;
-            break;
-        }
-    }
     }
 }
 
@@ -1221,8 +1223,8 @@ template <bool ROW> __global__ __launch_bounds__(256) void merge_few_kernel(Call
 #pragma unroll
             for (int k = 0; k < 16; k++)
                 if (k0 + k * PER < cnt) /* uniform */
-                    v[k] = *(const floatx4 *)(c.po + at(j0 + min(k0 + k * PER + own, cnt - 1)) * PD +
-                                              dim);
+                    v[k] = *(const floatx4 *)(
+                        c.po + at(j0 + min(k0 + k * PER + own, cnt - 1)) * PD + dim);
             if (k0 == 0) {
                 const float next = fmaxf(mu, wave_max(mi));
                 const float ref = next == -INFINITY ? 0.f : next, old = fast_exp2(mu - ref);

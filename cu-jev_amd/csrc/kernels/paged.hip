@@ -17,12 +17,18 @@ namespace {
  * the transpose needs neither LDS nor another wave's data: lane l holds 16
  * tokens of dims 4l .. 4l + 3 and stores one piece per dim. A workgroup's four
  * are a page's, whose lines of V^T they fill together in one L2.
+ * With V_ROWS (below) V's tokens are row waves, too, and store single elements.
  *
  * 8 sequences of up to 700 tokens, e4m3: 17.6 us for 62 MB, 3.5 TB/s (25 with one
  * group a workgroup, reductions through LDS and rope loads by all lanes). 64 of one
  * token: 7 us, a chain of loads: arguments, lengths, page ids, stores. Four tokens a
  * wave; two (half the registers, twice the waves) took the same. */
 constexpr int PREP_TOK = 4;
+/* V by rows as well, a token's 256 values as single elements, where there are many
+ * sequences of a token or so each: 1024 x 1 e4m3 26 us, 38 by groups, each of which
+ * has to find its sequence among all; 1024 x 3 bf16 63 and 84; but 256 x 4 20.0 and
+ * 18.7, and 64 x 1 bf16 6.6 and 5.5. */
+constexpr int PREP_V_ROWS = 3, PREP_V_SEQS = 64;
 /* A K row's lane in doubles, rounded to e4m3 once: the bytes, and the scale 2^*e */
 DEV uint32_t k_row_exact(const bf16 *src, const float2 *rope, const float *w, bool rotates,
                          bool first, int half_lanes, float eps, int *e) {
@@ -55,7 +61,7 @@ DEV uint32_t k_row_exact(const bf16 *src, const float2 *rope, const float *w, bo
                      to_odd(y[3] * inv));
 }
 
-template <bool E4M3, int TOK>
+template <bool E4M3, int TOK, bool V_ROWS>
 __global__ __launch_bounds__(256) void prep_paged_kernel(
     const bf16 *__restrict__ proj, int ps, const float *__restrict__ qw,
     const float *__restrict__ kw, const int32_t *__restrict__ pos,
@@ -65,14 +71,16 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(
     void *__restrict__ k_pages, void *__restrict__ vt_pages, float *__restrict__ k_scale,
     float *__restrict__ v_scale, int num_pages, int row_blocks) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if ((int)blockIdx.x < row_blocks) {
-        const int heads = Hq + Hkv, unit = blockIdx.x * 4 + wave;
+    if (V_ROWS || (int)blockIdx.x < row_blocks) {
+        const int heads = Hq + Hkv + (V_ROWS ? Hkv : 0), unit = blockIdx.x * 4 + wave;
         const int head = unit % heads, n0 = unit / heads * TOK;
         if (n0 >= N)
             return;
-        const bool is_k = head >= Hq;
+        const bool is_v = V_ROWS && head >= Hq + Hkv, is_k = head >= Hq && !is_v;
         const float *w = is_k ? kw : qw;
-        const bf16 *src = proj + (is_k ? Hq * 512 + (head - Hq) * 256 : head * 512) + 4 * lane;
+        /* K's heads, then V's, follow q's and the gates' */
+        const int kv = head - Hq, kh = is_v ? kv - Hkv : kv;
+        const bf16 *src = proj + (kv >= 0 ? Hq * 512 + kv * 256 : head * 512) + 4 * lane;
         const int half_lanes = rot / 8;
         const bool rotates = lane < 2 * half_lanes, first = lane < half_lanes;
         const int fi0 = rotates ? (first ? 4 * lane : 4 * lane - rot / 2) : 0;
@@ -100,14 +108,50 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(
         if (n0 + lane >= N)
             b = -1;
         long long at = b;
-        if (is_k) {
+        if (is_k || is_v) {
             const int p = s.p0 + (n0 + lane - s.q0);
             const bool in = b >= 0 && (unsigned)(n0 + lane - s.q0) < (unsigned)s.ql && p >= 0 &&
                             p < s.kv;
             const int page = page_table[(size_t)max(b, 0) * max_pages + (in ? p / PG : 0)];
             at = in && page >= 0 && page < num_pages
-                     ? ((long long)page * Hkv + head - Hq) * PG + p % PG
+                     ? ((long long)page * Hkv + kh) * PG + p % PG
                      : -1;
+        }
+        auto row_of = [&](int t) {
+            return (long long)(uint32_t)__builtin_amdgcn_readlane((int)at, t) |
+                   (long long)__builtin_amdgcn_readlane((int)(at >> 32), t) << 32;
+        };
+        if (is_v) {
+#pragma unroll
+            for (int t = 0; t < TOK; t++) {
+                const long long row = row_of(t);
+                if (row < 0)
+                    continue;
+                const size_t to = (size_t)(row / PG) * PSLICE + (size_t)4 * lane * PG + row % PG;
+                if constexpr (E4M3) {
+                    float v[4], amax = 0.f;
+#pragma unroll
+                    for (int d = 0; d < 4; d++) {
+                        v[d] = bf2f(raw[t][d]);
+                        amax = fmaxf(amax, fabsf(v[d]));
+                    }
+                    amax = fold_wave(amax, [](float p, float q) { return fmaxf(p, q); });
+                    const int e = e4m3_exp(amax);
+                    const float inv = exp2_int(-e);
+                    const uint32_t out =
+                        pack_e4m3(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+#pragma unroll
+                    for (int d = 0; d < 4; d++)
+                        ((uint8_t *)vt_pages)[to + d * PG] = (uint8_t)(out >> (8 * d));
+                    if (lane == 0)
+                        v_scale[row] = exp2_int(e);
+                } else {
+#pragma unroll
+                    for (int d = 0; d < 4; d++)
+                        ((bf16 *)vt_pages)[to + d * PG] = raw[t][d];
+                }
+            }
+            return;
         }
         float x[TOK][4], ss[TOK];
 #pragma unroll
@@ -136,10 +180,6 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(
                 x[t][e] = rotates ? __builtin_fmaf(y, cz[2 * e], first ? -o : o) : y;
             }
         }
-        auto row_of = [&](int t) {
-            return (long long)(uint32_t)__builtin_amdgcn_readlane((int)at, t) |
-                   (long long)__builtin_amdgcn_readlane((int)(at >> 32), t) << 32;
-        };
         uint32_t again = 0; /* tokens */
 #pragma unroll
         for (int t = 0; t < TOK; t++) {
@@ -238,11 +278,10 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(
         for (int t = 0; t < VTOK; t++)
             m[t] = fmaxf(fmaxf(fabsf(bf2f(v[t][0])), fabsf(bf2f(v[t][1]))),
                          fmaxf(fabsf(bf2f(v[t][2])), fabsf(bf2f(v[t][3]))));
-        auto meet = [](float p, float q, bool rows32) {
-            const auto a = rows32 ? __builtin_amdgcn_permlane32_swap(__float_as_uint(p),
-                                                                     __float_as_uint(q), false, false)
-                                  : __builtin_amdgcn_permlane16_swap(__float_as_uint(p),
-                                                                     __float_as_uint(q), false, false);
+        auto meet = [](float p, float q, bool by32) {
+            const uint32_t u = __float_as_uint(p), v = __float_as_uint(q);
+            const auto a = by32 ? __builtin_amdgcn_permlane32_swap(u, v, false, false)
+                                : __builtin_amdgcn_permlane16_swap(u, v, false, false);
             return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
         };
 #pragma unroll
@@ -378,7 +417,8 @@ __global__ __launch_bounds__(256) void page_read_kernel(
                 r[t >> 3][t & 7] = f2bf(bf2f(p[t & 1]) * sc[t]);
             }
         } else {
-            const bf16x8 *v = (const bf16x8 *)((const bf16 *)vt_pages + head * PSLICE + d * PG + t0);
+            const bf16 *at = (const bf16 *)vt_pages + head * PSLICE + d * PG + t0;
+            const bf16x8 *v = (const bf16x8 *)at;
             r[0] = v[0], r[1] = v[1];
         }
         if (!ok)
@@ -418,23 +458,30 @@ extern "C" hipError_t k_attn_prep_paged(const bf16_t *proj, int proj_stride, con
     const int Hkv = pages->Hkv, B = seqs->B;
     if (N <= 0 || B <= 0)
         return hipSuccess;
-    const long long units = (long long)CEIL_DIV(N, PREP_TOK) * (Hq + Hkv);
+    const bool v_rows = B > PREP_V_SEQS && N <= PREP_V_ROWS * (long long)B;
+    const long long units =
+        (long long)CEIL_DIV(N, PREP_TOK) * (Hq + Hkv + (v_rows ? Hkv : 0));
     const long long v_pages = N < N / PG + 2ll * B ? N : N / PG + 2ll * B;
-    const long long row_blocks = CEIL_DIV(units, 4), v_blocks = v_pages * Hkv;
+    const long long row_blocks = CEIL_DIV(units, 4), v_blocks = v_rows ? 0 : v_pages * Hkv;
     if (row_blocks + v_blocks > 0x7fffffff)
         return hipErrorInvalidValue;
-#define LAUNCH(T)                                                                                 \
-    hipLaunchKernelGGL((prep_paged_kernel<T, PREP_TOK>),                                          \
+#define LAUNCH(T, V)                                                                              \
+    hipLaunchKernelGGL((prep_paged_kernel<T, PREP_TOK, V>),                                       \
                        dim3((unsigned)(row_blocks + v_blocks)), dim3(256), 0, stream,             \
                        (const bf16 *)proj, proj_stride, q_norm_w, k_norm_w, pos, seqs->q_start,   \
                        seqs->kv_len, seqs->page_table, seqs->max_pages, B, N,                     \
                        Hq, Hkv, rot, (const float2 *)rope_table, npos, eps, q_scale,              \
                        (bf16 *)q_out, pages->k, pages->vt, pages->k_scale, pages->v_scale,        \
                        pages->num_pages, (int)row_blocks)
-    if (pages->type == CUJEV_KV_E4M3)
-        LAUNCH(true);
+    const bool e4m3 = pages->type == CUJEV_KV_E4M3;
+    if (e4m3 && v_rows)
+        LAUNCH(true, true);
+    else if (e4m3)
+        LAUNCH(true, false);
+    else if (v_rows)
+        LAUNCH(false, true);
     else
-        LAUNCH(false);
+        LAUNCH(false, false);
 #undef LAUNCH
     return hipGetLastError();
 }
