@@ -261,6 +261,13 @@ def _need(name, t, dtype, dev, shape):
         raise OpsError(f"{name}: need contiguous {dtype} {shape} on device {dev}, got {got}")
 
 
+def _need_ints(name, *values):
+    """Sizes that a C int holds as they are (ctypes cuts larger ones)."""
+    for v in values:
+        if v >> 31:
+            raise OpsError(f"{name}: {v} is not a size from 0 to 2^31 - 1")
+
+
 def _paged_call(dev, name, *args):
     """A call on the device of the pages, on that device's current stream."""
     import torch
@@ -294,8 +301,10 @@ def attn_prep_paged(proj, q_norm_w, k_norm_w, pos, q_start, kv_len, page_table, 
     its kv_len[b] keys. q_out [N, Hq, 256]; rope from rope_table."""
     import torch
     dev, B = _paged_seqs(pages, page_table, kv_len, q_start)
+    if proj.dim() != 2:
+        raise OpsError(f"proj: need rows, got {tuple(proj.shape)}")
     N, Hkv = proj.shape[0], pages.Hkv
-    if proj.dtype is not torch.bfloat16 or proj.get_device() != dev or proj.dim() != 2 or \
+    if proj.dtype is not torch.bfloat16 or proj.get_device() != dev or \
             proj.stride(1) != 1 or proj.shape[1] < Hq * 512 + Hkv * 512:
         raise OpsError(f"proj: need bfloat16 rows of {Hq * 512 + Hkv * 512} values on device {dev}")
     _need("q_norm_w", q_norm_w, torch.float32, dev, (256,))
@@ -315,7 +324,8 @@ def kv_page_read(pages, page_table, kv_len, max_kv, k_cache, vt_cache):
     layout; stride at least kv_stride(max_kv)); the other columns stay."""
     import torch
     dev, B = _paged_seqs(pages, page_table, kv_len)
-    stride = k_cache.shape[-2]
+    _need_ints("kv_page_read", max_kv)
+    stride = k_cache.shape[-2] if k_cache.dim() == 4 else 0
     _need("k_cache", k_cache, torch.bfloat16, dev, (B, pages.Hkv, stride, 256))
     _need("vt_cache", vt_cache, torch.bfloat16, dev, (B, pages.Hkv, 256, stride))
     _paged_call(dev, "cujev_op_kv_page_read", *pages.args, page_table.data_ptr(),
@@ -324,6 +334,7 @@ def kv_page_read(pages, page_table, kv_len, max_kv, k_cache, vt_cache):
 
 
 def attention_paged_ws_bytes(N, B, max_q, max_kv, Hq, Hkv, window=0, sinks=0, e4m3=False) -> int:
+    _need_ints("attention_paged_ws_bytes", N, B, max_q, max_kv, Hq, Hkv, window, sinks)
     return int(load().cujev_ops_attention_paged_ws_bytes(N, B, max_q, max_kv, Hq, Hkv, window,
                                                          sinks, int(e4m3)))
 
@@ -337,6 +348,9 @@ def attention_paged(q, gate, gate_tok_stride, gate_head_stride, pages, page_tabl
     that is 0)."""
     import torch
     dev, B = _paged_seqs(pages, page_table, kv_len, q_start)
+    _need_ints("attention_paged", max_q, max_kv, window, sinks, gate_tok_stride, gate_head_stride)
+    if q.dim() != 3:
+        raise OpsError(f"q: need [N, Hq, 256], got {tuple(q.shape)}")
     N, Hq = q.shape[0], q.shape[1]
     _need("q", q, torch.bfloat16, dev, (N, Hq, 256))
     _need("out", out, torch.bfloat16, dev, (N, Hq * 256))

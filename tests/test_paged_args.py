@@ -111,18 +111,25 @@ def test_bindings_refuse_wrong_tensors():
                 dict(kv_len=i32(1, 2)), dict(q_start=i32(0)), dict(page_table=i32(0)),
                 dict(kv_len=torch.tensor([1])), dict(ws=torch.zeros(4)),
                 dict(gate=q.float()), dict(gate=q, gate_tok_stride=1024, gate_head_stride=512),
-                dict(gate=q, gate_tok_stride=-4)]:
+                dict(gate=q, gate_tok_stride=-4), dict(q=q[0]), dict(max_kv=2 ** 32 + 1),
+                dict(max_q=-1), dict(window=2 ** 31)]:
         with pytest.raises(ops.OpsError):
             ops.attention_paged(**{**good, **bad})
     kc, vc = torch.zeros(1, 1, 128, 256).bfloat16(), torch.zeros(1, 1, 256, 128).bfloat16()
-    for a, b in [(kc[0], vc), (kc, vc[..., :64]), (kc.float(), vc)]:
+    for a, b in [(kc[0], vc), (kc.flatten(), vc), (kc, vc[..., :64]), (kc.float(), vc)]:
         with pytest.raises(ops.OpsError):
             ops.kv_page_read(pages, i32(0)[None], i32(1), 1, a, b)
+    for max_kv in (2 ** 32 + 1, -1):
+        with pytest.raises(ops.OpsError):
+            ops.kv_page_read(pages, i32(0)[None], i32(1), max_kv, kc, vc)
+        with pytest.raises(ops.OpsError):
+            ops.attention_paged_ws_bytes(1, 1, 1, max_kv, 4, 1)
     w = torch.ones(256)
     prep = dict(proj=torch.zeros(1, 4 * 512 + 512).bfloat16(), q_norm_w=w, k_norm_w=w, pos=i32(0),
                 q_start=i32(0, 1), kv_len=i32(1), page_table=i32(0)[None], Hq=4, rot=64,
                 rope=torch.zeros(8, 32, 2), eps=1e-6, q_scale=0.1, q_out=q, pages=pages)
     for bad in [dict(proj=prep["proj"].float()), dict(proj=prep["proj"][:, :2048]),
+                dict(proj=prep["proj"][0]),
                 dict(pos=i32(0, 1)), dict(rope=torch.zeros(8, 16, 2)), dict(q_out=q[:, :2]),
                 dict(q_norm_w=w.bfloat16()), dict(k_norm_w=w[:128])]:
         with pytest.raises(ops.OpsError):
