@@ -8,21 +8,21 @@ namespace CUJEV_KNS {
 namespace {
 
 /* ---- new tokens into pages ---------------------------------------------------
- * Two kinds of wave in one launch. A row wave normalises TOK tokens' rows of
- * one q-head or K head, lane l holding dims 4l .. 4l + 3, as attn_prep does:
+ * Three kinds of wave in one launch. A row wave normalises TOK tokens' rows of one
+ * q-head or K head, lane l holding dims 4l .. 4l + 3, as attn_prep does:
  *   y = x rsqrt(mean x^2 + eps) w, RoPE (dim i with i + rot/2, lane l with
  *   l ^ rot/8), q times q_scale.
  * A V wave takes the tokens of one aligned group of 16 positions and one
  * kv-head: the group's V^T rows are whole 16-byte (e4m3) or 32-byte pieces, so
  * the transpose needs neither LDS nor another wave's data: lane l holds 16
  * tokens of dims 4l .. 4l + 3 and stores one piece per dim. A workgroup's four
- * are a page's, whose lines of V^T they fill together in one L2.
- * With V_ROWS (below) V's tokens are row waves, too, and store single elements.
+ * are a page's, whose lines of V^T they fill together in one L2. With V_ROWS V's
+ * tokens are row waves, too, and store single elements.
  *
- * 8 sequences of up to 700 tokens, e4m3: 17.6 us for 62 MB, 3.5 TB/s (25 with one
+ * 8 sequences of up to 700 tokens, e4m3: 15.5 us for 62 MB, 4 TB/s (25 with one
  * group a workgroup, reductions through LDS and rope loads by all lanes). 64 of one
- * token: 7 us, a chain of loads: arguments, lengths, page ids, stores. Four tokens a
- * wave; two (half the registers, twice the waves) took the same. */
+ * token: 6.4 us, a chain of loads: arguments, lengths, page ids, stores. Four tokens
+ * a wave, two of e4m3 keys: their rounding needs the registers. */
 constexpr int PREP_TOK = 4;
 /* V by rows as well, a token's 256 values as single elements, where there are many
  * sequences of a token or so each: 1024 x 1 e4m3 26 us, 38 by groups, each of which
@@ -61,193 +61,198 @@ DEV uint32_t k_row_exact(const bf16 *src, const float2 *rope, const float *w, bo
                      to_odd(y[3] * inv));
 }
 
-template <bool E4M3, int TOK, bool V_ROWS>
-__global__ __launch_bounds__(256) void prep_paged_kernel(
-    const bf16 *__restrict__ proj, int ps, const float *__restrict__ qw,
-    const float *__restrict__ kw, const int32_t *__restrict__ pos,
-    const int32_t *__restrict__ q_start, const int32_t *__restrict__ kv_len,
-    const int32_t *__restrict__ page_table, int max_pages, int B, int N, int Hq, int Hkv, int rot,
-    const float2 *__restrict__ rope, int npos, float eps, float q_scale, bf16 *__restrict__ q_out,
-    void *__restrict__ k_pages, void *__restrict__ vt_pages, float *__restrict__ k_scale,
-    float *__restrict__ v_scale, int num_pages, int row_blocks) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (V_ROWS || (int)blockIdx.x < row_blocks) {
-        const int heads = Hq + Hkv + (V_ROWS ? Hkv : 0), unit = blockIdx.x * 4 + wave;
-        const int head = unit % heads, n0 = unit / heads * TOK;
-        if (n0 >= N)
-            return;
-        const bool is_v = V_ROWS && head >= Hq + Hkv, is_k = head >= Hq && !is_v;
-        const float *w = is_k ? kw : qw;
-        /* K's heads, then V's, follow q's and the gates' */
-        const int kv = head - Hq, kh = is_v ? kv - Hkv : kv;
-        const bf16 *src = proj + (kv >= 0 ? Hq * 512 + kv * 256 : head * 512) + 4 * lane;
-        const int half_lanes = rot / 8;
-        const bool rotates = lane < 2 * half_lanes, first = lane < half_lanes;
-        const int fi0 = rotates ? (first ? 4 * lane : 4 * lane - rot / 2) : 0;
-        /* every load before any arithmetic, token indices clamped */
-        bf16x4 raw[TOK];
+struct Prep {
+    const bf16 *proj;
+    int ps;
+    const float *qw, *kw;
+    const int32_t *pos, *q_start, *kv_len, *page_table;
+    int max_pages, B, N, Hq, Hkv, rot;
+    const float2 *rope;
+    int npos;
+    float eps, q_scale;
+    bf16 *q_out;
+    void *k_pages, *vt_pages;
+    float *k_scale, *v_scale;
+    int num_pages, k_blocks, v_blocks;
+};
+enum { ROW_Q, ROW_K, ROW_V };
+
+/* A wave for tokens n0 .. n0 + TOK - 1 of one head */
+template <int KIND, int TOK, bool E4M3> DEV void row_wave(const Prep &c, int head, int n0) {
+    constexpr bool is_k = KIND == ROW_K;
+    const int lane = threadIdx.x & 63, N = c.N, rot = c.rot;
+    const float *w = is_k ? c.kw : c.qw;
+    /* K's heads, then V's, follow q's and the gates' */
+    const int at0 = KIND == ROW_Q ? head * 512 : c.Hq * 512 + (is_k ? head : c.Hkv + head) * 256;
+    const bf16 *src = c.proj + at0 + 4 * lane;
+    const int half_lanes = rot / 8;
+    const bool rotates = lane < 2 * half_lanes, first = lane < half_lanes;
+    const int fi0 = rotates ? (first ? 4 * lane : 4 * lane - rot / 2) : 0;
+    /* every load before any arithmetic, token indices clamped */
+    bf16x4 raw[TOK];
 #pragma unroll
-        for (int t = 0; t < TOK; t++)
-            raw[t] = *(const bf16x4 *)(src + (size_t)min(n0 + t, N - 1) * ps);
-        const float4 wl = *(const float4 *)(w + 4 * lane);
-        const int pos_lane = min(max(pos[min(n0 + (lane & (TOK - 1)), N - 1)], 0), npos - 1);
-        /* The tokens' sequences, then (K) their slots, token t in lane t: one
-         * chain of loads for all of them. at: the K row in the pool, -1: none */
-        pg_seq s;
-        int b = find_seqs<TOK>(q_start, kv_len, B, N, max_pages * PG, n0, &s);
-        float4 rc[TOK][2] = {};
-        if (rotates) { /* 16 lanes' loads or fewer: by all 64 they cost more than x's */
-#pragma unroll
-            for (int t = 0; t < TOK; t++) {
-                const float4 *r = (const float4 *)(
-                    rope + (size_t)__builtin_amdgcn_readlane(pos_lane, t) * (rot / 2) + fi0);
-                rc[t][0] = r[0];
-                rc[t][1] = r[1];
-            }
-        }
-        if (n0 + lane >= N)
-            b = -1;
-        long long at = b;
-        if (is_k || is_v) {
-            const int p = s.p0 + (n0 + lane - s.q0);
-            const bool in = b >= 0 && (unsigned)(n0 + lane - s.q0) < (unsigned)s.ql && p >= 0 &&
-                            p < s.kv;
-            const int page = page_table[(size_t)max(b, 0) * max_pages + (in ? p / PG : 0)];
-            at = in && page >= 0 && page < num_pages
-                     ? ((long long)page * Hkv + kh) * PG + p % PG
-                     : -1;
-        }
-        auto row_of = [&](int t) {
-            return (long long)(uint32_t)__builtin_amdgcn_readlane((int)at, t) |
-                   (long long)__builtin_amdgcn_readlane((int)(at >> 32), t) << 32;
-        };
-        if (is_v) {
-#pragma unroll
-            for (int t = 0; t < TOK; t++) {
-                const long long row = row_of(t);
-                if (row < 0)
-                    continue;
-                const size_t to = (size_t)(row / PG) * PSLICE + (size_t)4 * lane * PG + row % PG;
-                if constexpr (E4M3) {
-                    float v[4], amax = 0.f;
-#pragma unroll
-                    for (int d = 0; d < 4; d++) {
-                        v[d] = bf2f(raw[t][d]);
-                        amax = fmaxf(amax, fabsf(v[d]));
-                    }
-                    amax = fold_wave(amax, [](float p, float q) { return fmaxf(p, q); });
-                    const int e = e4m3_exp(amax);
-                    const float inv = exp2_int(-e);
-                    const uint32_t out =
-                        pack_e4m3(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-#pragma unroll
-                    for (int d = 0; d < 4; d++)
-                        ((uint8_t *)vt_pages)[to + d * PG] = (uint8_t)(out >> (8 * d));
-                    if (lane == 0)
-                        v_scale[row] = exp2_int(e);
-                } else {
-#pragma unroll
-                    for (int d = 0; d < 4; d++)
-                        ((bf16 *)vt_pages)[to + d * PG] = raw[t][d];
-                }
-            }
-            return;
-        }
-        float x[TOK][4], ss[TOK];
+    for (int t = 0; t < TOK; t++)
+        raw[t] = *(const bf16x4 *)(src + (size_t)min(n0 + t, N - 1) * c.ps);
+    const float4 wl = *(const float4 *)(w + 4 * lane);
+    const int pos_lane = min(max(c.pos[min(n0 + (lane & (TOK - 1)), N - 1)], 0), c.npos - 1);
+    /* The tokens' sequences, then (K) their slots, token t in lane t: one
+     * chain of loads for all of them. at: the K row in the pool, -1: none */
+    pg_seq s;
+    int b = find_seqs<TOK>(c.q_start, c.kv_len, c.B, N, c.max_pages * PG, n0, &s);
+    float4 rc[TOK][2] = {};
+    if (rotates) { /* 16 lanes' loads or fewer: by all 64 they cost more than x's */
 #pragma unroll
         for (int t = 0; t < TOK; t++) {
-            ss[t] = 0.f;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                x[t][e] = bf2f(raw[t][e]);
-                ss[t] += x[t][e] * x[t][e];
-            }
+            const float4 *r = (const float4 *)(
+                c.rope + (size_t)__builtin_amdgcn_readlane(pos_lane, t) * (rot / 2) + fi0);
+            rc[t][0] = r[0];
+            rc[t][1] = r[1];
         }
-#pragma unroll
-        for (int t = 0; t < TOK; t++)
-            ss[t] = fold_wave(ss[t], [](float p, float q) { return p + q; });
-        const float we[4] = {wl.x, wl.y, wl.z, wl.w};
-#pragma unroll
-        for (int t = 0; t < TOK; t++) {
-            const float rinv = rsqrtf(ss[t] * (1.f / 256.f) + eps);
-            const float cz[8] = {rc[t][0].x, rc[t][0].y, rc[t][0].z, rc[t][0].w,
-                                 rc[t][1].x, rc[t][1].y, rc[t][1].z, rc[t][1].w};
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float y = x[t][e] * rinv * we[e];
-                /* rounded as attn_prep rounds: the same bits reach both caches */
-                const float o = __shfl_xor(y, half_lanes, 64) * cz[2 * e + 1];
-                x[t][e] = rotates ? __builtin_fmaf(y, cz[2 * e], first ? -o : o) : y;
-            }
-        }
-        uint32_t again = 0; /* tokens */
+    }
+    if (n0 + lane >= N)
+        b = -1;
+    long long at = b;
+    if (KIND != ROW_Q) {
+        const int p = s.p0 + (n0 + lane - s.q0);
+        const bool in = b >= 0 && (unsigned)(n0 + lane - s.q0) < (unsigned)s.ql && p >= 0 &&
+                        p < s.kv;
+        const int page = c.page_table[(size_t)max(b, 0) * c.max_pages + (in ? p / PG : 0)];
+        at = in && page >= 0 && page < c.num_pages
+                 ? ((long long)page * c.Hkv + head) * PG + p % PG
+                 : -1;
+    }
+    auto row_of = [&](int t) {
+        return (long long)(uint32_t)__builtin_amdgcn_readlane((int)at, t) |
+               (long long)__builtin_amdgcn_readlane((int)(at >> 32), t) << 32;
+    };
+    if constexpr (KIND == ROW_V) {
 #pragma unroll
         for (int t = 0; t < TOK; t++) {
             const long long row = row_of(t);
-            if (row < 0) /* no sequence's row, or no slot */
+            if (row < 0)
                 continue;
-            if (E4M3 && is_k) {
-                float amax = 0.f;
+            const size_t to = (size_t)(row / PG) * PSLICE + (size_t)4 * lane * PG + row % PG;
+            if constexpr (E4M3) {
+                float v[4], amax = 0.f;
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    amax = fmaxf(amax, fabsf(x[t][e]));
+                for (int d = 0; d < 4; d++) {
+                    v[d] = bf2f(raw[t][d]);
+                    amax = fmaxf(amax, fabsf(v[d]));
+                }
                 amax = fold_wave(amax, [](float p, float q) { return fmaxf(p, q); });
                 const int e = e4m3_exp(amax);
                 const float inv = exp2_int(-e);
                 const uint32_t out =
-                    pack_e4m3(x[t][0] * inv, x[t][1] * inv, x[t][2] * inv, x[t][3] * inv);
-                /* Close to a tie, or to the next scale, float's errors (about ten
-                 * roundings, of values up to amax sqrt 2 where they rotate) can lead a
-                 * value to the other side, a whole step of 2^-3; one or two of 5
-                 * million did. Such a row, one of 30 or so, again in doubles. */
-                constexpr float NEAR = 0x1p-20f;
-                const float top = amax * inv;
-                bool close = top > 448.f * (1.f - NEAR) || top < 224.f * (1.f + NEAR);
+                    pack_e4m3(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float v = fabsf(x[t][i] * inv), r = fabsf(e4m3_of(out, i));
-                    const float step = __uint_as_float(
-                        max(__float_as_uint(v) & 0x7f800000u, (127u - 6) << 23) - (3u << 23));
-                    close |= .5f * step - fabsf(v - r) < NEAR * (rotates ? 2.f * top : v);
-                }
-                again |= __any(close) ? 1u << t : 0u;
-                ((uint32_t *)k_pages)[row * 64 + lane] = out;
+                for (int d = 0; d < 4; d++)
+                    ((uint8_t *)c.vt_pages)[to + d * PG] = (uint8_t)(out >> (8 * d));
                 if (lane == 0)
-                    k_scale[row] = exp2_int(e);
-                continue;
-            }
-            const float f = is_k ? 1.f : q_scale;
-            const bf16x4 o = {f2bf(x[t][0] * f), f2bf(x[t][1] * f), f2bf(x[t][2] * f),
-                              f2bf(x[t][3] * f)};
-            if (!is_k) {
-                *(bf16x4 *)(q_out + ((size_t)(n0 + t) * Hq + head) * 256 + 4 * lane) = o;
+                    c.v_scale[row] = exp2_int(e);
             } else {
-                *(bf16x4 *)((bf16 *)k_pages + row * 256 + 4 * lane) = o;
+#pragma unroll
+                for (int d = 0; d < 4; d++)
+                    ((bf16 *)c.vt_pages)[to + d * PG] = raw[t][d];
             }
-        }
-#pragma unroll 1
-        while (E4M3 && again) { /* a loop: unrolled, it took registers from the others */
-            const int t = __ffs(again) - 1;
-            again &= again - 1;
-            const long long row = row_of(t);
-            int e;
-            const uint32_t out = k_row_exact(
-                src + (size_t)(n0 + t) * ps,
-                rope + (size_t)__builtin_amdgcn_readlane(pos_lane, t) * (rot / 2) + fi0,
-                w + 4 * lane, rotates, first, half_lanes, eps, &e);
-            ((uint32_t *)k_pages)[row * 64 + lane] = out;
-            if (lane == 0)
-                k_scale[row] = exp2_int(e);
         }
         return;
     }
+    float x[TOK][4], ss[TOK];
+#pragma unroll
+    for (int t = 0; t < TOK; t++) {
+        ss[t] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            x[t][e] = bf2f(raw[t][e]);
+            ss[t] += x[t][e] * x[t][e];
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < TOK; t++)
+        ss[t] = fold_wave(ss[t], [](float p, float q) { return p + q; });
+    const float we[4] = {wl.x, wl.y, wl.z, wl.w};
+#pragma unroll
+    for (int t = 0; t < TOK; t++) {
+        const float rinv = rsqrtf(ss[t] * (1.f / 256.f) + c.eps);
+        const float cz[8] = {rc[t][0].x, rc[t][0].y, rc[t][0].z, rc[t][0].w,
+                             rc[t][1].x, rc[t][1].y, rc[t][1].z, rc[t][1].w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float y = x[t][e] * rinv * we[e];
+            /* rounded as attn_prep rounds: the same bits reach both caches */
+            const float o = __shfl_xor(y, half_lanes, 64) * cz[2 * e + 1];
+            x[t][e] = rotates ? __builtin_fmaf(y, cz[2 * e], first ? -o : o) : y;
+        }
+    }
+    uint32_t again = 0; /* tokens */
+#pragma unroll
+    for (int t = 0; t < TOK; t++) {
+        const long long row = row_of(t);
+        if (row < 0) /* no sequence's row, or no slot */
+            continue;
+        if constexpr (E4M3 && is_k) {
+            float amax = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                amax = fmaxf(amax, fabsf(x[t][e]));
+            amax = fold_wave(amax, [](float p, float q) { return fmaxf(p, q); });
+            const int e = e4m3_exp(amax);
+            const float inv = exp2_int(-e);
+            const uint32_t out =
+                pack_e4m3(x[t][0] * inv, x[t][1] * inv, x[t][2] * inv, x[t][3] * inv);
+            /* Close to a tie, or to the next scale, float's errors (about ten
+             * roundings, of values up to amax sqrt 2 where they rotate) can lead a
+             * value to the other side, a whole step of 2^-3; one or two of 5
+             * million did. Such a row, one of 30 or so, again in doubles. */
+            constexpr float NEAR = 0x1p-20f;
+            const float top = amax * inv;
+            bool close = top > 448.f * (1.f - NEAR) || top < 224.f * (1.f + NEAR);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float v = fabsf(x[t][i] * inv), r = fabsf(e4m3_of(out, i));
+                const float step = __uint_as_float(
+                    max(__float_as_uint(v) & 0x7f800000u, (127u - 6) << 23) - (3u << 23));
+                close |= .5f * step - fabsf(v - r) < NEAR * (rotates ? 2.f * top : v);
+            }
+            again |= __any(close) ? 1u << t : 0u;
+            ((uint32_t *)c.k_pages)[row * 64 + lane] = out;
+            if (lane == 0)
+                c.k_scale[row] = exp2_int(e);
+            continue;
+        }
+        const float f = is_k ? 1.f : c.q_scale;
+        const bf16x4 o = {f2bf(x[t][0] * f), f2bf(x[t][1] * f), f2bf(x[t][2] * f),
+                          f2bf(x[t][3] * f)};
+        if constexpr (!is_k) {
+            *(bf16x4 *)(c.q_out + ((size_t)(n0 + t) * c.Hq + head) * 256 + 4 * lane) = o;
+        } else {
+            *(bf16x4 *)((bf16 *)c.k_pages + row * 256 + 4 * lane) = o;
+        }
+    }
+#pragma unroll 1
+    while (E4M3 && is_k && again) { /* a loop: unrolled, it took registers from the others */
+        const int t = __ffs(again) - 1;
+        again &= again - 1;
+        const long long row = row_of(t);
+        int e;
+        const uint32_t out = k_row_exact(
+            src + (size_t)(n0 + t) * c.ps,
+            c.rope + (size_t)__builtin_amdgcn_readlane(pos_lane, t) * (rot / 2) + fi0,
+            w + 4 * lane, rotates, first, half_lanes, c.eps, &e);
+        ((uint32_t *)c.k_pages)[row * 64 + lane] = out;
+        if (lane == 0)
+            c.k_scale[row] = exp2_int(e);
+    }
+}
 
-    /* ---- V ---- */
-    const int unit = blockIdx.x - row_blocks, kh = unit % Hkv;
+/* A workgroup for page `unit` / Hkv of those that the new tokens touch */
+template <bool E4M3> DEV void v_page(const Prep &c, int unit) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int kh = unit % c.Hkv;
     pg_seq s;
     int i;
     const int b = find_item(
-        q_start, kv_len, B, N, N, max_pages * PG, unit / Hkv,
+        c.q_start, c.kv_len, c.B, c.N, c.N, c.max_pages * PG, unit / c.Hkv,
         [](const pg_seq &q) { return pg_v_pages(q); }, &s, &i);
     if (b < 0)
         return;
@@ -255,18 +260,18 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(
     const int base = at * PG + wave * VTOK; /* the group's first position */
     if (base + VTOK <= pg_new_lo(s) || base >= pg_new_hi(s))
         return;
-    const int page = page_table[(size_t)b * max_pages + at];
+    const int page = c.page_table[(size_t)b * c.max_pages + at];
     const int lo = max(pg_new_lo(s), base), hi = min(pg_new_hi(s), base + VTOK);
-    const bf16 *src = proj + Hq * 512 + Hkv * 256 + kh * 256 + 4 * lane;
+    const bf16 *src = c.proj + c.Hq * 512 + c.Hkv * 256 + kh * 256 + 4 * lane;
     bf16x4 v[VTOK];
 #pragma unroll
     for (int t = 0; t < VTOK; t++) {
         const int p = min(max(base + t, lo), hi - 1);
-        v[t] = *(const bf16x4 *)(src + (size_t)(s.q0 + p - s.p0) * ps);
+        v[t] = *(const bf16x4 *)(src + (size_t)(s.q0 + p - s.p0) * c.ps);
     }
-    if (page < 0 || page >= num_pages)
+    if (page < 0 || page >= c.num_pages)
         return;
-    const size_t head = (size_t)page * Hkv + kh;
+    const size_t head = (size_t)page * c.Hkv + kh;
     const int col = base % PG;
     const bool whole = hi - lo == VTOK;
     if constexpr (E4M3) {
@@ -299,12 +304,12 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(
         m[0] = fmaxf(m[0], dpp<0xb1>(m[0]));
         const int e = e4m3_exp(m[0]), tok = lane >> 2;
         if ((lane & 3) == 0 && base + tok >= lo && base + tok < hi)
-            v_scale[head * PG + col + tok] = exp2_int(e);
+            c.v_scale[head * PG + col + tok] = exp2_int(e);
         float inv[VTOK];
 #pragma unroll
         for (int t = 0; t < VTOK; t++)
             inv[t] = exp2_int(-__builtin_amdgcn_readlane(e, 4 * t));
-        uint8_t *dst = (uint8_t *)vt_pages + head * PSLICE + (size_t)4 * lane * PG + col;
+        uint8_t *dst = (uint8_t *)c.vt_pages + head * PSLICE + (size_t)4 * lane * PG + col;
 #pragma unroll
         for (int d = 0; d < 4; d++) {
             u32x4 q;
@@ -324,7 +329,7 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(
             }
         }
     } else {
-        bf16 *dst = (bf16 *)vt_pages + head * PSLICE + (size_t)4 * lane * PG + col;
+        bf16 *dst = (bf16 *)c.vt_pages + head * PSLICE + (size_t)4 * lane * PG + col;
 #pragma unroll
         for (int d = 0; d < 4; d++) {
             if (whole) {
@@ -344,6 +349,31 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(
             }
         }
     }
+}
+
+template <int n> using is = std::integral_constant<int, n>;
+template <bool E4M3, bool V_ROWS>
+__global__ __launch_bounds__(256) void prep_paged_kernel(Prep c) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int block = blockIdx.x;
+    auto rows = [&](auto kind, auto tok, int heads) {
+        const int unit = block * 4 + wave, n0 = unit / heads * decltype(tok)::value;
+        if (n0 < c.N)
+            row_wave<decltype(kind)::value, decltype(tok)::value, E4M3>(c, unit % heads, n0);
+    };
+    /* The longest first: 8 x 700 e4m3 takes 17.6 us so, 19.3 with q's rows first (1024
+     * bf16, one round of workgroups, 10.6 and 9.8). */
+    if (block < c.v_blocks) {
+        if constexpr (V_ROWS)
+            return rows(is<ROW_V>{}, is<PREP_TOK>{}, c.Hkv);
+        else
+            return v_page<E4M3>(c, block);
+    }
+    block -= c.v_blocks;
+    if (block < c.k_blocks)
+        return rows(is<ROW_K>{}, is<E4M3 ? PREP_TOK / 2 : PREP_TOK>{}, c.Hkv);
+    block -= c.k_blocks;
+    rows(is<ROW_Q>{}, is<PREP_TOK>{}, c.Hq);
 }
 
 /* ---- pages back into a state's caches -----------------------------------------
@@ -459,21 +489,23 @@ extern "C" hipError_t k_attn_prep_paged(const bf16_t *proj, int proj_stride, con
     if (N <= 0 || B <= 0)
         return hipSuccess;
     const bool v_rows = B > PREP_V_SEQS && N <= PREP_V_ROWS * (long long)B;
-    const long long units =
-        (long long)CEIL_DIV(N, PREP_TOK) * (Hq + Hkv + (v_rows ? Hkv : 0));
-    const long long v_pages = N < N / PG + 2ll * B ? N : N / PG + 2ll * B;
-    const long long row_blocks = CEIL_DIV(units, 4), v_blocks = v_rows ? 0 : v_pages * Hkv;
-    if (row_blocks + v_blocks > 0x7fffffff)
-        return hipErrorInvalidValue;
-#define LAUNCH(T, V)                                                                              \
-    hipLaunchKernelGGL((prep_paged_kernel<T, PREP_TOK, V>),                                       \
-                       dim3((unsigned)(row_blocks + v_blocks)), dim3(256), 0, stream,             \
-                       (const bf16 *)proj, proj_stride, q_norm_w, k_norm_w, pos, seqs->q_start,   \
-                       seqs->kv_len, seqs->page_table, seqs->max_pages, B, N,                     \
-                       Hq, Hkv, rot, (const float2 *)rope_table, npos, eps, q_scale,              \
-                       (bf16 *)q_out, pages->k, pages->vt, pages->k_scale, pages->v_scale,        \
-                       pages->num_pages, (int)row_blocks)
     const bool e4m3 = pages->type == CUJEV_KV_E4M3;
+    auto row_blocks = [&](int tok, int heads) {
+        return CEIL_DIV((long long)CEIL_DIV(N, tok) * heads, 4);
+    };
+    const long long v_pages = N < N / PG + 2ll * B ? N : N / PG + 2ll * B;
+    const long long k_blocks = row_blocks(e4m3 ? PREP_TOK / 2 : PREP_TOK, Hkv);
+    const long long v_blocks = v_rows ? row_blocks(PREP_TOK, Hkv) : v_pages * Hkv;
+    const long long blocks = k_blocks + v_blocks + row_blocks(PREP_TOK, Hq);
+    if (blocks > 0x7fffffff)
+        return hipErrorInvalidValue;
+    const Prep c = {(const bf16 *)proj, proj_stride, q_norm_w, k_norm_w, pos, seqs->q_start,
+                    seqs->kv_len, seqs->page_table, seqs->max_pages, B, N, Hq, Hkv, rot,
+                    (const float2 *)rope_table, npos, eps, q_scale, (bf16 *)q_out, pages->k,
+                    pages->vt, pages->k_scale, pages->v_scale, pages->num_pages, (int)k_blocks,
+                    (int)v_blocks};
+#define LAUNCH(T, V)                                                                              \
+    hipLaunchKernelGGL((prep_paged_kernel<T, V>), dim3((unsigned)blocks), dim3(256), 0, stream, c)
     if (e4m3 && v_rows)
         LAUNCH(true, true);
     else if (e4m3)
