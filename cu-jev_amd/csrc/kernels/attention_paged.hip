@@ -110,7 +110,9 @@ struct Call {
     int rG; /* r / G = r * rG >> 16 for r < 4096 (an integer division is 30 instructions) */
     bf16 *out;
     float *po, *pl, *pmu;
-    int2 *info; /* few rows: a sequence's first piece and parts, for the merge */
+    /* for the merge: few rows {first piece, parts} of each sequence, many rows
+     * {sequence, unit, parts (0: not a unit's first), 0} of each part */
+    int32_t *info;
     pg_plan plan;
 };
 DEV pg_seq seq_of(const Call &c, int b) {
@@ -505,7 +507,7 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
         }
         lrun = fold_rows(lrun, [](float a, float b) { return a + b; });
         if (w.part == 0 && kh == 0 && c.plan.slots > 0 && lane_again() == 0)
-            c.info[b] = int2{w.first, w.parts};
+            ((int2 *)c.info)[b] = int2{w.first, w.parts};
 
         /* lane (m, g) holds dims 16 t + 4 g .. + 3 of row m. Both are worked out again:
          * kept over the loop they went to scratch memory. */
@@ -635,7 +637,11 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
     }
     if (at >= c.plan.shares)
         return;
-    const Where w = locate<RT>(c, c.plan.shares - 1 - at);
+    const int target = c.plan.shares - 1 - at;
+    const Where w = locate<RT>(c, target);
+    if (kh == 0 && target < c.plan.slots && threadIdx.x == 0)
+        ((int4 *)c.info)[target] =
+            int4{w.b, w.unit, w.b >= 0 && w.part == 0 ? w.parts : 0, 0};
     if (w.b < 0)
         return;
     const pg_seq s = w.s;
@@ -1199,7 +1205,7 @@ template <bool ROW> __global__ __launch_bounds__(256) void merge_few_kernel(Call
     const int group = blockIdx.x % groups, kh = blockIdx.x / groups % c.Hkv;
     const int b = blockIdx.x / groups / c.Hkv, r = ROW ? group : group * 4 + wave;
     const pg_seq s = seq_of(c, b);
-    const int2 info = c.info[b]; /* of a sequence with rows */
+    const int2 info = ((const int2 *)c.info)[b]; /* of a sequence with rows */
     if (r >= s.ql * c.G || info.y <= 1)
         return;
     const int first = info.x, parts = info.y;
@@ -1267,21 +1273,23 @@ __global__ __launch_bounds__(256) void merge_many_kernel(Call c) {
     constexpr int R = 4, GROUPS = RT / (4 * R);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int group = blockIdx.x % GROUPS, kh = blockIdx.x / GROUPS % c.Hkv;
-    const Where w = locate<RT>(c, blockIdx.x / GROUPS / c.Hkv);
-    const int r0 = w.unit * RT, t0 = (group * 4 + wave) * R;
-    /* the first part's workgroups do it */
-    if (w.b < 0 || w.parts <= 1 || w.part > 0 || t0 >= min(w.s.ql * c.G - r0, RT) ||
-        w.first + w.parts > c.plan.slots) /* more than any rising q_start has */
+    const int part = blockIdx.x / GROUPS / c.Hkv; /* a unit's first: its merge */
+    const int4 info = ((const int4 *)c.info)[part];
+    const int parts = info.z, r0 = info.y * RT, t0 = (group * 4 + wave) * R;
+    if (parts <= 1 || part + parts > c.plan.slots) /* more than any rising q_start has */
         return;
-    const int last = min(w.s.ql * c.G - r0, RT) - 1;
+    const pg_seq s = seq_of(c, info.x);
+    const int last = min(s.ql * c.G - r0, RT) - 1;
+    if (t0 > last)
+        return;
     const float *po[R]; /* part 0 of a row's o; past the last row it again */
     bf16 *out[R];
     bf16x4 gv[R] = {};
-    const size_t slot = slot_of(c, kh, w.first);
+    const size_t slot = slot_of(c, kh, part);
 #pragma unroll
     for (int i = 0; i < R; i++) {
         const int t = min(t0 + i, last), r = r0 + t, tok = r / c.G, head = kh * c.G + r % c.G;
-        const size_t n = w.s.q0 + tok;
+        const size_t n = s.q0 + tok;
         po[i] = c.po + (slot * RT + t) * PD + 4 * lane;
         out[i] = c.out + (n * c.Hq + head) * PD + 4 * lane;
         if (c.gate)
@@ -1293,8 +1301,8 @@ __global__ __launch_bounds__(256) void merge_many_kernel(Call c) {
     auto of = [&](float x, int at) {
         return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), at));
     };
-    for (int j0 = 0; j0 < w.parts; j0 += 16) {
-        const int cnt = min(w.parts - j0, 16);
+    for (int j0 = 0; j0 < parts; j0 += 16) {
+        const int cnt = min(parts - j0, 16);
         const size_t mine = (slot + j0 + min(lane & 15, cnt - 1)) * RT + own;
         const float pl = c.pl[mine], pm = c.pmu[mine];
         const float li = (lane & 15) < cnt ? pl : 0.f, mi = li > 0.f ? pm : -INFINITY;
@@ -1349,7 +1357,7 @@ static size_t ws_bytes_of(const pg_plan &p, int Hkv) {
     if (p.slots <= 0)
         return 0;
     return (size_t)p.slots * Hkv * p.rt * (PD + 2) * sizeof(float) +
-           (p.rt == FEW ? (size_t)p.units * sizeof(int2) : 0);
+           (p.rt == FEW ? (size_t)p.units * sizeof(int2) : (size_t)p.slots * sizeof(int4));
 }
 
 extern "C" size_t cujev_attention_paged_ws_bytes(int N, int B, int max_q, int max_kv, int Hq,
@@ -1382,7 +1390,7 @@ extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int
                     max_q, max_kv, Hq, Hkv, G, window, sinks,
                     pg_div_up(65536, G), (bf16 *)out,
                     (float *)ws, (float *)ws + rows * PD, (float *)ws + rows * (PD + 1),
-                    (int2 *)((float *)ws + rows * (PD + 2)), p};
+                    (int32_t *)((float *)ws + rows * (PD + 2)), p};
     const bool few = p.rt == FEW;
     const int per = !few && 8 % Hkv == 0 ? 8 / Hkv : 1;
     const dim3 grid((unsigned)(pg_div_up(p.shares, per) * per * Hkv)); /* all parts */
