@@ -15,20 +15,25 @@ namespace {
  * A V wave takes the tokens of one aligned group of 16 positions and one
  * kv-head: the group's V^T rows are whole 16-byte (e4m3) or 32-byte pieces, so
  * the transpose needs neither LDS nor another wave's data: lane l holds 16
- * tokens of dims 4l .. 4l + 3 and stores one piece per dim. A workgroup's four
- * are a page's, whose lines of V^T they fill together in one L2. With V_ROWS V's
- * tokens are row waves, too, and store single elements.
+ * tokens of dims 4l .. 4l + 3 and stores one piece per dim. A page's four groups
+ * are a wave's, or waves' on one XCD, whose L2 gathers their lines of V^T. With
+ * V_ROWS V's tokens are row waves, too, and store single elements.
  *
- * 8 sequences of up to 700 tokens, e4m3: 15.5 us for 62 MB, 4 TB/s (25 with one
- * group a workgroup, reductions through LDS and rope loads by all lanes). 64 of one
- * token: 6.4 us, a chain of loads: arguments, lengths, page ids, stores. Four tokens
- * a wave, two of e4m3 keys: their rounding needs the registers. */
+ * 8 sequences of up to 700 tokens, e4m3: 15 us for 62 MB, 4.1 TB/s (25 with a page's
+ * groups apart, reductions through LDS and rope loads by all lanes). 64 of one token:
+ * 6.3 us, a chain of loads: arguments, lengths, page ids, stores. Four tokens a wave,
+ * two of e4m3 keys: their rounding needs the registers. A wave a workgroup: 1024
+ * tokens bf16 take 9.0 us so, 10.6 with four. */
 constexpr int PREP_TOK = 4;
 /* V by rows as well, a token's 256 values as single elements, where there are many
  * sequences of a token or so each: 1024 x 1 e4m3 26 us, 38 by groups, each of which
  * has to find its sequence among all; 1024 x 3 bf16 63 and 84; but 256 x 4 20.0 and
  * 18.7, and 64 x 1 bf16 6.6 and 5.5. */
 constexpr int PREP_V_ROWS = 3, PREP_V_SEQS = 64;
+/* V by groups, a wave each where they are few or most of a page's are there (16 x 48
+ * e4m3 9.5 us, 13.9 with a wave a page; 8 x 700 17.0 and 18.4), a wave a page
+ * otherwise, which starts fewer that have nothing to do (64 x 48 22 and 27). */
+constexpr int PREP_V_FEW = 1024, PREP_V_WHOLE = 128;
 /* A K row's lane in doubles, rounded to e4m3 once: the bytes, and the scale 2^*e */
 DEV uint32_t k_row_exact(const bf16 *src, const float2 *rope, const float *w, bool rotates,
                          bool first, int half_lanes, float eps, int *e) {
@@ -74,6 +79,7 @@ struct Prep {
     void *k_pages, *vt_pages;
     float *k_scale, *v_scale;
     int num_pages, k_blocks, v_blocks;
+    bool v_spread; /* a wave a group of V, or a page */
 };
 enum { ROW_Q, ROW_K, ROW_V };
 
@@ -245,10 +251,10 @@ template <int KIND, int TOK, bool E4M3> DEV void row_wave(const Prep &c, int hea
     }
 }
 
-/* A workgroup for page `unit` / Hkv of those that the new tokens touch */
-template <bool E4M3> DEV void v_page(const Prep &c, int unit) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int kh = unit % c.Hkv;
+/* V of groups g0 .. g1 - 1 of 16 positions of a page: of number `unit` / Hkv among
+ * those that the new tokens touch */
+template <bool E4M3> DEV void v_groups(const Prep &c, int unit, int g0, int g1) {
+    const int lane = threadIdx.x & 63, kh = unit % c.Hkv;
     pg_seq s;
     int i;
     const int b = find_item(
@@ -257,95 +263,98 @@ template <bool E4M3> DEV void v_page(const Prep &c, int unit) {
     if (b < 0)
         return;
     const int at = pg_new_lo(s) / PG + i;          /* the page's number in the sequence */
-    const int base = at * PG + wave * VTOK; /* the group's first position */
-    if (base + VTOK <= pg_new_lo(s) || base >= pg_new_hi(s))
-        return;
     const int page = c.page_table[(size_t)b * c.max_pages + at];
-    const int lo = max(pg_new_lo(s), base), hi = min(pg_new_hi(s), base + VTOK);
-    const bf16 *src = c.proj + c.Hq * 512 + c.Hkv * 256 + kh * 256 + 4 * lane;
-    bf16x4 v[VTOK];
-#pragma unroll
-    for (int t = 0; t < VTOK; t++) {
-        const int p = min(max(base + t, lo), hi - 1);
-        v[t] = *(const bf16x4 *)(src + (size_t)(s.q0 + p - s.p0) * c.ps);
-    }
     if (page < 0 || page >= c.num_pages)
         return;
-    const size_t head = (size_t)page * c.Hkv + kh;
-    const int col = base % PG;
-    const bool whole = hi - lo == VTOK;
-    if constexpr (E4M3) {
-        /* max of each token over the wave: lanes that meet exchange the halves
-         * they give up (16 -> 8 -> 4 -> 2 -> 1 tokens a lane), so lane l ends
-         * with token l >> 2 */
-        float m[VTOK];
+#pragma unroll 1
+    for (int group = g0; group < g1; group++) {
+        const int base = at * PG + group * VTOK; /* the group's first position */
+        if (base + VTOK <= pg_new_lo(s) || base >= pg_new_hi(s))
+            continue;
+        const int lo = max(pg_new_lo(s), base), hi = min(pg_new_hi(s), base + VTOK);
+        const bf16 *src = c.proj + c.Hq * 512 + c.Hkv * 256 + kh * 256 + 4 * lane;
+        bf16x4 v[VTOK];
 #pragma unroll
-        for (int t = 0; t < VTOK; t++)
-            m[t] = fmaxf(fmaxf(fabsf(bf2f(v[t][0])), fabsf(bf2f(v[t][1]))),
-                         fmaxf(fabsf(bf2f(v[t][2])), fabsf(bf2f(v[t][3]))));
-        auto meet = [](float p, float q, bool by32) {
-            const uint32_t u = __float_as_uint(p), v = __float_as_uint(q);
-            const auto a = by32 ? __builtin_amdgcn_permlane32_swap(u, v, false, false)
-                                : __builtin_amdgcn_permlane16_swap(u, v, false, false);
-            return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-        };
-#pragma unroll
-        for (int t = 0; t < 8; t++)
-            m[t] = meet(m[t], m[t + 8], true);
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-            m[t] = meet(m[t], m[t + 4], false);
-#pragma unroll
-        for (int t = 0; t < 2; t++) /* row_ror 8 */
-            m[t] = fmaxf(lane & 8 ? m[t + 2] : m[t], dpp<0x128>(lane & 8 ? m[t] : m[t + 2]));
-        /* row_half_mirror: lane ^ 7, in the other four as lane ^ 4 is */
-        m[0] = fmaxf(lane & 4 ? m[1] : m[0], dpp<0x141>(lane & 4 ? m[0] : m[1]));
-        m[0] = fmaxf(m[0], dpp<0x4e>(m[0])); /* quad_perm, lane ^ 2, lane ^ 1 */
-        m[0] = fmaxf(m[0], dpp<0xb1>(m[0]));
-        const int e = e4m3_exp(m[0]), tok = lane >> 2;
-        if ((lane & 3) == 0 && base + tok >= lo && base + tok < hi)
-            c.v_scale[head * PG + col + tok] = exp2_int(e);
-        float inv[VTOK];
-#pragma unroll
-        for (int t = 0; t < VTOK; t++)
-            inv[t] = exp2_int(-__builtin_amdgcn_readlane(e, 4 * t));
-        uint8_t *dst = (uint8_t *)c.vt_pages + head * PSLICE + (size_t)4 * lane * PG + col;
-#pragma unroll
-        for (int d = 0; d < 4; d++) {
-            u32x4 q;
-#pragma unroll
-            for (int w = 0; w < 4; w++)
-                q[w] = pack_e4m3(bf2f(v[4 * w][d]) * inv[4 * w],
-                                 bf2f(v[4 * w + 1][d]) * inv[4 * w + 1],
-                                 bf2f(v[4 * w + 2][d]) * inv[4 * w + 2],
-                                 bf2f(v[4 * w + 3][d]) * inv[4 * w + 3]);
-            if (whole) {
-                *(u32x4 *)(dst + d * PG) = q;
-            } else {
-#pragma unroll
-                for (int t = 0; t < VTOK; t++)
-                    if (base + t >= lo && base + t < hi)
-                        dst[d * PG + t] = (uint8_t)(q[t >> 2] >> (8 * (t & 3)));
-            }
+        for (int t = 0; t < VTOK; t++) {
+            const int p = min(max(base + t, lo), hi - 1);
+            v[t] = *(const bf16x4 *)(src + (size_t)(s.q0 + p - s.p0) * c.ps);
         }
-    } else {
-        bf16 *dst = (bf16 *)c.vt_pages + head * PSLICE + (size_t)4 * lane * PG + col;
+        const size_t head = (size_t)page * c.Hkv + kh;
+        const int col = base % PG;
+        const bool whole = hi - lo == VTOK;
+        if constexpr (E4M3) {
+            /* max of each token over the wave: lanes that meet exchange the halves
+             * they give up (16 -> 8 -> 4 -> 2 -> 1 tokens a lane), so lane l ends
+             * with token l >> 2 */
+            float m[VTOK];
 #pragma unroll
-        for (int d = 0; d < 4; d++) {
-            if (whole) {
+            for (int t = 0; t < VTOK; t++)
+                m[t] = fmaxf(fmaxf(fabsf(bf2f(v[t][0])), fabsf(bf2f(v[t][1]))),
+                             fmaxf(fabsf(bf2f(v[t][2])), fabsf(bf2f(v[t][3]))));
+            auto meet = [](float p, float q, bool by32) {
+                const uint32_t u = __float_as_uint(p), v = __float_as_uint(q);
+                const auto a = by32 ? __builtin_amdgcn_permlane32_swap(u, v, false, false)
+                                    : __builtin_amdgcn_permlane16_swap(u, v, false, false);
+                return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+            };
 #pragma unroll
-                for (int w = 0; w < 2; w++) {
-                    bf16x8 q;
+            for (int t = 0; t < 8; t++)
+                m[t] = meet(m[t], m[t + 8], true);
 #pragma unroll
-                    for (int t = 0; t < 8; t++)
-                        q[t] = v[8 * w + t][d];
-                    *(bf16x8 *)(dst + d * PG + 8 * w) = q;
+            for (int t = 0; t < 4; t++)
+                m[t] = meet(m[t], m[t + 4], false);
+#pragma unroll
+            for (int t = 0; t < 2; t++) /* row_ror 8 */
+                m[t] = fmaxf(lane & 8 ? m[t + 2] : m[t], dpp<0x128>(lane & 8 ? m[t] : m[t + 2]));
+            /* row_half_mirror: lane ^ 7, in the other four as lane ^ 4 is */
+            m[0] = fmaxf(lane & 4 ? m[1] : m[0], dpp<0x141>(lane & 4 ? m[0] : m[1]));
+            m[0] = fmaxf(m[0], dpp<0x4e>(m[0])); /* quad_perm, lane ^ 2, lane ^ 1 */
+            m[0] = fmaxf(m[0], dpp<0xb1>(m[0]));
+            const int e = e4m3_exp(m[0]), tok = lane >> 2;
+            if ((lane & 3) == 0 && base + tok >= lo && base + tok < hi)
+                c.v_scale[head * PG + col + tok] = exp2_int(e);
+            float inv[VTOK];
+#pragma unroll
+            for (int t = 0; t < VTOK; t++)
+                inv[t] = exp2_int(-__builtin_amdgcn_readlane(e, 4 * t));
+            uint8_t *dst = (uint8_t *)c.vt_pages + head * PSLICE + (size_t)4 * lane * PG + col;
+#pragma unroll
+            for (int d = 0; d < 4; d++) {
+                u32x4 q;
+#pragma unroll
+                for (int w = 0; w < 4; w++)
+                    q[w] = pack_e4m3(bf2f(v[4 * w][d]) * inv[4 * w],
+                                     bf2f(v[4 * w + 1][d]) * inv[4 * w + 1],
+                                     bf2f(v[4 * w + 2][d]) * inv[4 * w + 2],
+                                     bf2f(v[4 * w + 3][d]) * inv[4 * w + 3]);
+                if (whole) {
+                    *(u32x4 *)(dst + d * PG) = q;
+                } else {
+#pragma unroll
+                    for (int t = 0; t < VTOK; t++)
+                        if (base + t >= lo && base + t < hi)
+                            dst[d * PG + t] = (uint8_t)(q[t >> 2] >> (8 * (t & 3)));
                 }
-            } else {
+            }
+        } else {
+            bf16 *dst = (bf16 *)c.vt_pages + head * PSLICE + (size_t)4 * lane * PG + col;
 #pragma unroll
-                for (int t = 0; t < VTOK; t++)
-                    if (base + t >= lo && base + t < hi)
-                        dst[d * PG + t] = v[t][d];
+            for (int d = 0; d < 4; d++) {
+                if (whole) {
+#pragma unroll
+                    for (int w = 0; w < 2; w++) {
+                        bf16x8 q;
+#pragma unroll
+                        for (int t = 0; t < 8; t++)
+                            q[t] = v[8 * w + t][d];
+                        *(bf16x8 *)(dst + d * PG + 8 * w) = q;
+                    }
+                } else {
+#pragma unroll
+                    for (int t = 0; t < VTOK; t++)
+                        if (base + t >= lo && base + t < hi)
+                            dst[d * PG + t] = v[t][d];
+                }
             }
         }
     }
@@ -353,21 +362,24 @@ template <bool E4M3> DEV void v_page(const Prep &c, int unit) {
 
 template <int n> using is = std::integral_constant<int, n>;
 template <bool E4M3, bool V_ROWS>
-__global__ __launch_bounds__(256) void prep_paged_kernel(Prep c) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+__global__ __launch_bounds__(64) void prep_paged_kernel(Prep c) {
     int block = blockIdx.x;
     auto rows = [&](auto kind, auto tok, int heads) {
-        const int unit = block * 4 + wave, n0 = unit / heads * decltype(tok)::value;
+        const int n0 = block / heads * decltype(tok)::value;
         if (n0 < c.N)
-            row_wave<decltype(kind)::value, decltype(tok)::value, E4M3>(c, unit % heads, n0);
+            row_wave<decltype(kind)::value, decltype(tok)::value, E4M3>(c, block % heads, n0);
     };
-    /* The longest first: 8 x 700 e4m3 takes 17.6 us so, 19.3 with q's rows first (1024
-     * bf16, one round of workgroups, 10.6 and 9.8). */
+    /* The longest first (8 x 700 e4m3 1.7 us less than with q's rows first) */
     if (block < c.v_blocks) {
         if constexpr (V_ROWS)
             return rows(is<ROW_V>{}, is<PREP_TOK>{}, c.Hkv);
         else
-            return v_page<E4M3>(c, block);
+            {
+            /* a page's groups on one XCD: block b runs on b % 8 */
+            const int group = block / 8 % 4;
+            return c.v_spread ? v_groups<E4M3>(c, block / 32 * 8 + block % 8, group, group + 1)
+                              : v_groups<E4M3>(c, block, 0, 4);
+        }
     }
     block -= c.v_blocks;
     if (block < c.k_blocks)
@@ -491,11 +503,14 @@ extern "C" hipError_t k_attn_prep_paged(const bf16_t *proj, int proj_stride, con
     const bool v_rows = B > PREP_V_SEQS && N <= PREP_V_ROWS * (long long)B;
     const bool e4m3 = pages->type == CUJEV_KV_E4M3;
     auto row_blocks = [&](int tok, int heads) {
-        return CEIL_DIV((long long)CEIL_DIV(N, tok) * heads, 4);
+        return (long long)CEIL_DIV(N, tok) * heads;
     };
     const long long v_pages = N < N / PG + 2ll * B ? N : N / PG + 2ll * B;
+    const bool v_spread = v_pages * Hkv * 4 <= PREP_V_FEW || N >= PREP_V_WHOLE * (long long)B;
     const long long k_blocks = row_blocks(e4m3 ? PREP_TOK / 2 : PREP_TOK, Hkv);
-    const long long v_blocks = v_rows ? row_blocks(PREP_TOK, Hkv) : v_pages * Hkv;
+    const long long v_blocks = v_rows ? row_blocks(PREP_TOK, Hkv)
+                               : v_spread ? CEIL_DIV(v_pages * Hkv, 8) * 32
+                                          : v_pages * Hkv;
     const long long blocks = k_blocks + v_blocks + row_blocks(PREP_TOK, Hq);
     if (blocks > 0x7fffffff)
         return hipErrorInvalidValue;
@@ -503,9 +518,9 @@ extern "C" hipError_t k_attn_prep_paged(const bf16_t *proj, int proj_stride, con
                     seqs->kv_len, seqs->page_table, seqs->max_pages, B, N, Hq, Hkv, rot,
                     (const float2 *)rope_table, npos, eps, q_scale, (bf16 *)q_out, pages->k,
                     pages->vt, pages->k_scale, pages->v_scale, pages->num_pages, (int)k_blocks,
-                    (int)v_blocks};
+                    (int)v_blocks, v_spread};
 #define LAUNCH(T, V)                                                                              \
-    hipLaunchKernelGGL((prep_paged_kernel<T, V>), dim3((unsigned)blocks), dim3(256), 0, stream, c)
+    hipLaunchKernelGGL((prep_paged_kernel<T, V>), dim3((unsigned)blocks), dim3(64), 0, stream, c)
     if (e4m3 && v_rows)
         LAUNCH(true, true);
     else if (e4m3)
