@@ -226,12 +226,20 @@ class KvPages:
                            f"[pages, Hkv, {KV_PAGE}, 256]")
         n, Hkv = self.num_pages, self.Hkv = shape[0], shape[1]
         self.e4m3 = t is torch.float8_e4m3fn
-        _need("k", k, t, dev, (n, Hkv, KV_PAGE, 256))
-        _need("vt", vt, t, dev, (n, Hkv, 256, KV_PAGE))
+        if not (shape == (n, Hkv, KV_PAGE, 256) and k.is_contiguous() and vt is not None and
+                vt.dtype is t and vt.shape == (n, Hkv, 256, KV_PAGE) and vt.is_contiguous() and
+                vt.get_device() == dev):
+            _need("k", k, t, dev, (n, Hkv, KV_PAGE, 256))
+            _need("vt", vt, t, dev, (n, Hkv, 256, KV_PAGE))
         ks = vs = None
         if self.e4m3:
-            _need("k_scale", k_scale, torch.float32, dev, (n, Hkv, KV_PAGE))
-            _need("v_scale", v_scale, torch.float32, dev, (n, Hkv, KV_PAGE))
+            f32, of = torch.float32, (n, Hkv, KV_PAGE)
+            if not (k_scale is not None and v_scale is not None and k_scale.dtype is f32 and
+                    v_scale.dtype is f32 and k_scale.shape == of and v_scale.shape == of and
+                    k_scale.is_contiguous() and v_scale.is_contiguous() and
+                    k_scale.get_device() == dev and v_scale.get_device() == dev):
+                _need("k_scale", k_scale, f32, dev, of)
+                _need("v_scale", v_scale, f32, dev, of)
             ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
         elif k_scale is not None or v_scale is not None:
             raise OpsError("KvPages: bfloat16 pages have no scales")
@@ -253,7 +261,9 @@ def kv_pages(num_pages, Hkv, e4m3=False, device="cuda"):
 
 def _need(name, t, dtype, dev, shape):
     """A contiguous tensor of this type, device index (-1: CPU) and shape, or an
-    OpsError. Cheap: a call on a few tokens takes the device 5 us."""
+    OpsError. The paged operators ask the same of all their tensors in one
+    expression first and come here to name the one that is not: a call on a few
+    tokens takes the device 5 us, and a check by itself 0.35."""
     if t is None or t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or \
             t.get_device() != dev:
         got = "None" if t is None else f"{t.dtype} {tuple(t.shape)} on {t.device}" + (
@@ -263,9 +273,8 @@ def _need(name, t, dtype, dev, shape):
 
 def _need_ints(name, *values):
     """Sizes that a C int holds as they are (ctypes cuts larger ones)."""
-    for v in values:
-        if v >> 31:
-            raise OpsError(f"{name}: {v} is not a size from 0 to 2^31 - 1")
+    if any(v >> 31 for v in values):
+        raise OpsError(f"{name}: {values} are not all sizes from 0 to 2^31 - 1")
 
 
 def _paged_call(dev, name, *args):
@@ -287,9 +296,14 @@ def _paged_seqs(pages, page_table, kv_len, q_start=None):
     if len(shape) != 2:
         raise OpsError(f"page_table: need [B, max_pages], got {tuple(shape)}")
     B = shape[0]
-    _need("page_table", page_table, i32, dev, shape)
-    _need("kv_len", kv_len, i32, dev, (B,))
-    if q_start is not None:
+    if not (page_table.dtype is i32 and page_table.is_contiguous() and
+            page_table.get_device() == dev and kv_len is not None and kv_len.dtype is i32 and
+            kv_len.shape == (B,) and kv_len.is_contiguous() and kv_len.get_device() == dev):
+        _need("page_table", page_table, i32, dev, shape)
+        _need("kv_len", kv_len, i32, dev, (B,))
+    if q_start is not None and not (
+            q_start.dtype is i32 and q_start.shape == (B + 1,) and q_start.is_contiguous() and
+            q_start.get_device() == dev):
         _need("q_start", q_start, i32, dev, (B + 1,))
     return dev, B
 
@@ -307,11 +321,22 @@ def attn_prep_paged(proj, q_norm_w, k_norm_w, pos, q_start, kv_len, page_table, 
     if proj.dtype is not torch.bfloat16 or proj.get_device() != dev or \
             proj.stride(1) != 1 or proj.shape[1] < Hq * 512 + Hkv * 512:
         raise OpsError(f"proj: need bfloat16 rows of {Hq * 512 + Hkv * 512} values on device {dev}")
-    _need("q_norm_w", q_norm_w, torch.float32, dev, (256,))
-    _need("k_norm_w", k_norm_w, torch.float32, dev, (256,))
-    _need("pos", pos, torch.int32, dev, (N,))
-    _need("rope", rope, torch.float32, dev, (rope.shape[0], rot // 2, 2))
-    _need("q_out", q_out, torch.bfloat16, dev, (N, Hq, 256))
+    f32, angles = torch.float32, (rope.shape[0], rot // 2, 2)
+    if not (q_norm_w is not None and q_norm_w.dtype is f32 and q_norm_w.shape == (256,) and
+            q_norm_w.is_contiguous() and q_norm_w.get_device() == dev and
+            k_norm_w is not None and k_norm_w.dtype is f32 and k_norm_w.shape == (256,) and
+            k_norm_w.is_contiguous() and k_norm_w.get_device() == dev and
+            pos is not None and pos.dtype is torch.int32 and pos.shape == (N,) and
+            pos.is_contiguous() and pos.get_device() == dev and
+            rope.dtype is f32 and rope.shape == angles and rope.is_contiguous() and
+            rope.get_device() == dev and
+            q_out is not None and q_out.dtype is torch.bfloat16 and q_out.shape == (N, Hq, 256) and
+            q_out.is_contiguous() and q_out.get_device() == dev):
+        _need("q_norm_w", q_norm_w, f32, dev, (256,))
+        _need("k_norm_w", k_norm_w, f32, dev, (256,))
+        _need("pos", pos, torch.int32, dev, (N,))
+        _need("rope", rope, f32, dev, angles)
+        _need("q_out", q_out, torch.bfloat16, dev, (N, Hq, 256))
     _paged_call(dev, "cujev_op_attn_prep_paged", proj.data_ptr(), proj.stride(0),
                 q_norm_w.data_ptr(), k_norm_w.data_ptr(), pos.data_ptr(), q_start.data_ptr(),
                 kv_len.data_ptr(), page_table.data_ptr(), page_table.shape[1], B, N, Hq, Hkv, rot,
@@ -348,27 +373,34 @@ def attention_paged(q, gate, gate_tok_stride, gate_head_stride, pages, page_tabl
     that is 0)."""
     import torch
     dev, B = _paged_seqs(pages, page_table, kv_len, q_start)
-    _need_ints("attention_paged", max_q, max_kv, window, sinks, gate_tok_stride, gate_head_stride)
+    if (max_q | max_kv | window | sinks | gate_tok_stride | gate_head_stride) >> 31:
+        _need_ints("attention_paged", max_q, max_kv, window, sinks, gate_tok_stride,
+                   gate_head_stride)
     if q.dim() != 3:
         raise OpsError(f"q: need [N, Hq, 256], got {tuple(q.shape)}")
     N, Hq = q.shape[0], q.shape[1]
-    _need("q", q, torch.bfloat16, dev, (N, Hq, 256))
-    _need("out", out, torch.bfloat16, dev, (N, Hq * 256))
+    bf16 = torch.bfloat16
+    if not (q.dtype is bf16 and q.shape == (N, Hq, 256) and q.is_contiguous() and
+            q.get_device() == dev and out is not None and out.dtype is bf16 and
+            out.shape == (N, Hq * 256) and out.is_contiguous() and out.get_device() == dev):
+        _need("q", q, bf16, dev, (N, Hq, 256))
+        _need("out", out, bf16, dev, (N, Hq * 256))
     if gate is not None:
         last = (N - 1) * gate_tok_stride + (Hq - 1) * gate_head_stride + 256
-        if gate.dtype is not torch.bfloat16 or gate.get_device() != dev or gate_tok_stride < 0 or \
+        if gate.dtype is not bf16 or gate.get_device() != dev or gate_tok_stride < 0 or \
                 gate_head_stride < 0 or N > 0 and \
                 gate.untyped_storage().nbytes() < 2 * (gate.storage_offset() + last):
             raise OpsError(f"gate: need bfloat16 on device {dev}, with {N} rows and {Hq} heads at "
                            "these strides")
-    if ws is not None:
-        _need("ws", ws, torch.uint8, dev, (ws.numel(),))
+    size = 0 if ws is None else ws.numel()
+    if ws is not None and not (ws.dtype is torch.uint8 and ws.dim() == 1 and
+                               ws.is_contiguous() and ws.get_device() == dev):
+        _need("ws", ws, torch.uint8, dev, (size,))
     _paged_call(dev, "cujev_op_attention_paged", q.data_ptr(),
                 None if gate is None else gate.data_ptr(), gate_tok_stride, gate_head_stride,
                 *pages.args, q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(),
                 page_table.shape[1], B, N, max_q, max_kv, Hq, pages.Hkv, window, sinks,
-                out.data_ptr(), None if ws is None else ws.data_ptr(),
-                0 if ws is None else ws.numel())
+                out.data_ptr(), None if ws is None else ws.data_ptr(), size)
 
 
 def gdn_conv_prep(proj, conv_w, conv_in, conv_out, seg0_len, own_base, A_neg_exp, dt_bias,
