@@ -349,10 +349,17 @@ def kv_page_read(pages, page_table, kv_len, max_kv, k_cache, vt_cache):
     layout; stride at least kv_stride(max_kv)); the other columns stay."""
     import torch
     dev, B = _paged_seqs(pages, page_table, kv_len)
-    _need_ints("kv_page_read", max_kv)
-    stride = k_cache.shape[-2] if k_cache.dim() == 4 else 0
-    _need("k_cache", k_cache, torch.bfloat16, dev, (B, pages.Hkv, stride, 256))
-    _need("vt_cache", vt_cache, torch.bfloat16, dev, (B, pages.Hkv, 256, stride))
+    if max_kv >> 31:
+        _need_ints("kv_page_read", max_kv)
+    bf16, Hkv, shape = torch.bfloat16, pages.Hkv, k_cache.shape
+    stride = shape[2] if len(shape) == 4 else 0
+    if not (k_cache.dtype is bf16 and shape == (B, Hkv, stride, 256) and
+            k_cache.is_contiguous() and k_cache.get_device() == dev and
+            vt_cache is not None and vt_cache.dtype is bf16 and
+            vt_cache.shape == (B, Hkv, 256, stride) and vt_cache.is_contiguous() and
+            vt_cache.get_device() == dev):
+        _need("k_cache", k_cache, bf16, dev, (B, Hkv, stride, 256))
+        _need("vt_cache", vt_cache, bf16, dev, (B, Hkv, 256, stride))
     _paged_call(dev, "cujev_op_kv_page_read", *pages.args, page_table.data_ptr(),
                 page_table.shape[1], kv_len.data_ptr(), B, max_kv, pages.Hkv, k_cache.data_ptr(),
                 vt_cache.data_ptr(), stride)
