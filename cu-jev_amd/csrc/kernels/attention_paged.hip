@@ -90,6 +90,20 @@ DEV void settle(floatx16 (&o)[4]) {
 
 /* keys hi at most, and past lo or a sink (without branches) */
 DEV bool key_seen(int j, int hi, int lo, int sinks) { return (j <= hi) & ((j > lo) | (j < sinks)); }
+/* the same of keys j .. j + N - 1, a bit each (j >= 0; positions and windows are
+ * within PG_MOST and PG_MOST_KEYS, so that no difference leaves an int) */
+template <int N> DEV uint32_t keys_seen(int j, int hi, int lo, int sinks) {
+    auto below = [&](int x) { return (1u << min(max(x - j, 0), N)) - 1; }; /* keys < x */
+    return below(hi + 1) & (~below(lo + 1) | below(sinks));
+}
+/* x, or -inf where bit `bit` says hidden; all ones or zeros by it */
+template <int bit> DEV uint32_t spread_bit(uint32_t bits) {
+    return (uint32_t)((int)(bits << (31 - bit)) >> 31);
+}
+template <int bit> DEV float hide_by(uint32_t bits, float x) {
+    const uint32_t m = spread_bit<bit>(bits);
+    return __uint_as_float((__float_as_uint(x) & m) | (0xff800000u & ~m));
+}
 
 /* What the kernels and the merge share.
  *
@@ -797,11 +811,11 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
             return;
         const int kb = k0 + 32 * wj + (E4M3 ? 16 : 8) * h;
         const int top = there ? s.kv - 1 : -1;
-#pragma unroll
-        for (int r = 0; r < 16; r++)
-            x[r] = hide(key_seen(kb + (E4M3 ? r : 16 * (r >> 3) + (r & 7)), min(hi, top), lo,
-                                 c.sinks),
-                        x[r]);
+        const uint32_t bits = keys_seen<E4M3 ? 16 : 24>(kb, min(hi, top), lo, c.sinks);
+        unroll_for<16>([&](auto iv) {
+            constexpr int r = decltype(iv)::value;
+            x[r] = hide_by<E4M3 ? r : 16 * (r >> 3) + (r & 7)>(bits, x[r]);
+        });
         if constexpr (E4M3) /* a scale of no key of this call: any bits */
             vsc = __uint_as_float(
                 key_seen(kb + (lane & 15), top, pg_low(pmin, c.window), c.sinks)
@@ -905,19 +919,18 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
                 const int at = (n * 512 + (int)threadIdx.x) * 16, d = at / (L::T / PD);
                 const int piece = ((at >> 4) & (L::T / PD / 16 - 1)) ^ swz_v<E4M3>(d);
                 u32x4 w = lds_read16(lds, L::V + PAR * L::T + at);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    uint32_t keep = 0;
-#pragma unroll
-                    for (int f = 0; f < (E4M3 ? 4 : 2); f++) {
-                        const int j =
-                            k0 + (E4M3 ? 16 * piece + 4 * e + f : 8 * piece + 2 * e + f);
-                        const bool own =
-                            there && key_seen(j, s.kv - 1, pg_low(pmin, c.window), c.sinks);
-                        keep |= own ? (E4M3 ? 0xffu << (8 * f) : 0xffffu << (16 * f)) : 0u;
-                    }
-                    w[e] &= keep;
-                }
+                const uint32_t bits =
+                    there ? keys_seen<E4M3 ? 16 : 8>(k0 + (E4M3 ? 16 : 8) * piece, s.kv - 1,
+                                                     pg_low(pmin, c.window), c.sinks)
+                          : 0u;
+                unroll_for<4>([&](auto ie) {
+                    constexpr int e = decltype(ie)::value;
+                    if constexpr (E4M3) /* four bits to a byte each */
+                        w[e] &= ((bits >> (4 * e) & 15) * 0x204081u & 0x1010101u) * 0xffu;
+                    else
+                        w[e] &= (spread_bit<2 * e>(bits) & 0xffffu) |
+                                (spread_bit<2 * e + 1>(bits) & 0xffff0000u);
+                });
                 lds_write16(smem, L::V + PAR * L::T + at, w);
             }
             lds_barrier();
