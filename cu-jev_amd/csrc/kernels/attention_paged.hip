@@ -96,9 +96,14 @@ template <int N> DEV uint32_t keys_seen(int j, int hi, int lo, int sinks) {
     auto below = [&](int x) { return (1u << min(max(x - j, 0), N)) - 1; }; /* keys < x */
     return below(hi + 1) & (~below(lo + 1) | below(sinks));
 }
-/* x, or -inf where bit `bit` says hidden; all ones or zeros by it */
+/* Bit `bit` to all of a word; x, or -inf where it says hidden */
 template <int bit> DEV uint32_t spread_bit(uint32_t bits) {
     return (uint32_t)((int)(bits << (31 - bit)) >> 31);
+}
+/* four bits to a byte each, two to two bytes each */
+DEV uint32_t bytes_by(uint32_t bits) { return ((bits & 15) * 0x204081u & 0x1010101u) * 0xffu; }
+template <int bit> DEV uint32_t halves_by(uint32_t bits) {
+    return (spread_bit<bit>(bits) & 0xffffu) | (spread_bit<bit + 1>(bits) & 0xffff0000u);
 }
 template <int bit> DEV float hide_by(uint32_t bits, float x) {
     const uint32_t m = spread_bit<bit>(bits);
@@ -437,7 +442,7 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
              * are, meet p = 0 */
             u32x4 keep[E4M3 ? 1 : 2];
             bool foreign = false;
-            if (!there || k0 + PG - 1 > min(s.p0, s.kv - 1) || c.window > 0) { /* some key hidden */
+            if (!there || !pg_tile_whole(k0, s.p0, s.p0 + s.ql - 1, s.kv, c.window, c.sinks)) {
                 const int top = there ? s.kv - 1 : -1;
 #pragma unroll
                 for (int v = 0; v < 16; v++)
@@ -925,11 +930,10 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
                           : 0u;
                 unroll_for<4>([&](auto ie) {
                     constexpr int e = decltype(ie)::value;
-                    if constexpr (E4M3) /* four bits to a byte each */
-                        w[e] &= ((bits >> (4 * e) & 15) * 0x204081u & 0x1010101u) * 0xffu;
+                    if constexpr (E4M3)
+                        w[e] &= bytes_by(bits >> (4 * e));
                     else
-                        w[e] &= (spread_bit<2 * e>(bits) & 0xffffu) |
-                                (spread_bit<2 * e + 1>(bits) & 0xffff0000u);
+                        w[e] &= halves_by<2 * e>(bits);
                 });
                 lds_write16(smem, L::V + PAR * L::T + at, w);
             }
