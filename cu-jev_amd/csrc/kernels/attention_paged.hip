@@ -156,6 +156,13 @@ struct Where {
     int b, unit, parts, first, part;
     int begin, own, size; /* few rows: the unit on the line, tiles a piece */
 };
+/* many rows: w's unit, parts and first from its sequence, whose parts begin at `have` */
+DEV void set_part(const Call &c, Where &w, int target, int have, int share) {
+    const int whole = pg_short_units(w.s, c.G, c.window, w.own, share), at = target - have;
+    w.parts = at < whole ? 1 : pg_nshare(w.own, share);
+    w.unit = at < whole ? at : whole + (at - whole) / w.parts;
+    w.first = at < whole ? target : have + whole + (w.unit - whole) * w.parts;
+}
 /* J sequences a lane, 64 J a step: what all have, then where target lies */
 template <int RT_, int J> DEV Where locate_among(const Call &c, int target) {
     constexpr bool FEWR = RT_ == PG_FEW;
@@ -172,6 +179,9 @@ template <int RT_, int J> DEV Where locate_among(const Call &c, int target) {
             n[j] = units[j] ? pg_longest(s[j], c.G, RT_, c.window, c.sinks) : 0;
         }
     };
+    auto parts_of = [&](int j, int share) {
+        return units[j] ? pg_parts(s[j], c.G, c.window, n[j], share) : 0;
+    };
     if constexpr (J == 1) /* the only step */
         read(0);
     int size = PG_MOST;
@@ -183,7 +193,8 @@ template <int RT_, int J> DEV Where locate_among(const Call &c, int target) {
                 read(b0);
 #pragma unroll
             for (int j = 0; j < J; j++) {
-                T += (unsigned)units[j] * (unsigned)n[j];
+                T += FEWR || J > 1 ? (unsigned)units[j] * (unsigned)n[j]
+                                   : pg_all_tiles(s[j], c.G, c.window, n[j]) * (units[j] > 0);
                 U += units[j];
                 longest = max(longest, n[j]);
             }
@@ -195,7 +206,7 @@ template <int RT_, int J> DEV Where locate_among(const Call &c, int target) {
         } else if (pg_splits(c.plan, U)) {
             size = pg_share_first(c.plan, U, T, J > 1);
             if constexpr (J == 1)
-                while (last_lane(wave_scan(units[0] * pg_nshare(n[0], size))) > c.plan.goal)
+                while (last_lane(wave_scan(parts_of(0, size))) > c.plan.goal)
                     size = pg_share_next(size);
             longest = (int)fold_wave((float)longest, [](float p, float q) {
                 return fmaxf(p, q); /* below 2^24 tiles: exact */
@@ -213,7 +224,7 @@ template <int RT_, int J> DEV Where locate_among(const Call &c, int target) {
         int own[J], sum = 0;
 #pragma unroll
         for (int j = 0; j < J; j++)
-            sum += own[j] = units[j] * (FEWR ? n[j] : pg_nshare(n[j], size));
+            sum += own[j] = FEWR ? units[j] * n[j] : parts_of(j, size);
         const int to = before + wave_scan(sum);
         const uint64_t past = __ballot(to > item);
         if (past) {
@@ -236,9 +247,7 @@ template <int RT_, int J> DEV Where locate_among(const Call &c, int target) {
                 w.first = have / size;
                 w.parts = (have + w.own - 1) / size - w.first + 1;
             } else {
-                w.parts = pg_nshare(w.own, size);
-                w.unit = (target - have) / w.parts;
-                w.first = have + w.unit * w.parts;
+                set_part(c, w, target, have, size);
             }
             w.part = target - w.first;
             return w;
@@ -267,10 +276,17 @@ template <int RT_> DEV Where locate(const Call &c, int target) {
         w.parts = (n - 1) / w.size + 1;
     } else {
         int share = PG_MOST;
-        if (pg_splits(c.plan, units)) /* as many for each unit as there are */
-            share =
-                pg_share_last(pg_max((n - 1) / (c.plan.goal / units) + 1, PG_MANY_LEAST), n);
-        w.parts = pg_nshare(n, share);
+        if (pg_splits(c.plan, units)) {
+            share = pg_share_first(c.plan, units, pg_all_tiles(w.s, c.G, c.window, n), false);
+            while (pg_parts(w.s, c.G, c.window, n, share) > c.plan.goal)
+                share = pg_share_next(share);
+            share = pg_share_last(share, n);
+        }
+        w.own = n;
+        set_part(c, w, target, 0, share);
+        w.part = target - w.first;
+        w.b = w.unit < units ? 0 : -1;
+        return w;
     }
     w.unit = target / w.parts;
     w.first = w.unit * w.parts;

@@ -123,7 +123,8 @@ constexpr int pg_few_slot(int p0, int j) { return 2 * (p0 + j) + (j == 0); }
  * outnumber the workgroups that run at once. Try pg_share_first, then pg_share_next
  * of it until they fit; `sure` fits without trying. Where a share is then not
  * shorter by what a merge takes, some 6 tiles (10 us), all stay whole: 8 sequences'
- * 200 tokens on up to 1500 keys take 61 us so, 67 in 71 parts for 64 workgroups.
+ * 200 tokens on up to 1500 keys take 57 us so, 67 in 71 parts for 64 workgroups, and
+ * 32 x 8 on 1000 35 in shares of 8 tiles, 39 whole (16).
  * Shares have 8 tiles at least: 2 x 64 tokens on 2048 keys take 27 us, 37 with 16;
  * with 4 it is 25, and no less where there is more to do. */
 constexpr int PG_MANY_LEAST = 8, PG_MANY_MERGE = 6;
@@ -138,6 +139,30 @@ constexpr int pg_share_last(int share, int longest) {
     return share + PG_MANY_MERGE >= longest ? PG_MOST : share;
 }
 constexpr int pg_nshare(int tiles, int share) { return pg_max(pg_div_up(tiles, share), 1); }
+/* PG_MANY: a sequence's first units, those with no more tiles than a share, stay whole;
+ * the others are pg_nshare(longest, share) parts each: a new sequence's first rows
+ * have few, and leave workgroups to its last ones (1500 e4m3 keys 57 -> 50 us). */
+constexpr int pg_short_units(const pg_seq &s, int G, int window, int longest, int share) {
+    const int units = pg_units(s, G, PG_MANY);
+    if (longest <= share)
+        return units;
+    if (window > 0 || share >= PG_MOST / PG)
+        return 0;
+    const int rows = pg_min(PG * share - s.p0, s.ql); /* that see no more */
+    return rows <= 0 ? 0 : (int)pg_min((int)((long long)rows * G / PG_MANY), units);
+}
+constexpr int pg_parts(const pg_seq &s, int G, int window, int longest, int share) {
+    const int units = pg_units(s, G, PG_MANY);
+    const int whole = pg_short_units(s, G, window, longest, share);
+    return whole + (units - whole) * pg_nshare(longest, share);
+}
+/* about the tiles that its units have in all */
+constexpr unsigned pg_all_tiles(const pg_seq &s, int G, int window, int longest) {
+    const int units = pg_units(s, G, PG_MANY);
+    const int last = pg_min(s.p0 + (PG_MANY - 1) / G, s.kv - 1); /* of the first unit */
+    const int first = window > 0 ? longest : pg_min(pg_max(last, 0) / PG + 1, longest);
+    return (unsigned)units * (unsigned)(first + longest + 1) / 2;
+}
 /* First list entry of share i of n even ones */
 constexpr int pg_share_begin(int ntl, int i, int n) { return (int)((long long)ntl * i / n); }
 

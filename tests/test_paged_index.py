@@ -155,7 +155,7 @@ int main() {
             long long n = 0;
             for (int b = 0; b < B; b++) {
                 const int u = pg_units(seqs[b], G, p.rt);
-                n += u ? (long long)u * pg_nshare(pg_longest(seqs[b], G, p.rt, W, SS), share) : 0;
+                n += u ? pg_parts(seqs[b], G, W, pg_longest(seqs[b], G, p.rt, W, SS), share) : 0;
             }
             return n;
         };
@@ -165,11 +165,13 @@ int main() {
         if (pg_splits(p, (int)U) && U > 0) {
             const int sure = pg_share_first(p, (int)U, (unsigned)T, true);
             NEED(parts(sure) <= p.goal);
-            share = pg_share_first(p, (int)U, (unsigned)T, B > 64);
-            NEED(share <= sure);
-            if (B == 1)
-                share = pg_max((longest - 1) / (p.goal / (int)U) + 1, PG_MANY_LEAST);
-            else if (B <= 64)
+            unsigned all = 0;
+            for (int b = 0; b < B; b++)
+                if (pg_units(seqs[b], G, p.rt))
+                    all += pg_all_tiles(seqs[b], G, W, pg_longest(seqs[b], G, p.rt, W, SS));
+            NEED(all <= T + U);
+            share = pg_share_first(p, (int)U, B > 64 ? (unsigned)T : all, B > 64);
+            if (B <= 64)
                 for (int tries = 0; parts(share) > p.goal; tries++) {
                     NEED(tries < 100);
                     share = pg_share_next(share);
@@ -178,17 +180,24 @@ int main() {
         }
         bool split = false;
         for (int b = 0; b < B; b++) {
-            const int u = pg_units(seqs[b], G, p.rt), n = pg_nshare(pg_longest(seqs[b], G, p.rt, W, SS), share);
-            C += (long long)u * n;
-            split |= u > 0 && n > 1;
+            const int u = pg_units(seqs[b], G, p.rt), most = pg_longest(seqs[b], G, p.rt, W, SS);
+            const int whole = u ? pg_short_units(seqs[b], G, W, most, share) : 0;
+            NEED(whole >= 0 && whole <= u);
+            long long own = 0;
             for (int k = 0; k < u; k++) {
+                const int n = k < whole ? 1 : pg_nshare(most, share);
+                own += n;
+                split |= n > 1;
                 const int r0 = k * p.rt, rows = pg_min(seqs[b].ql * G - r0, p.rt);
                 NEED(rows > 0);
                 const pg_tiles t = pg_tile_list(seqs[b], r0 / G, (r0 + rows - 1) / G, W, SS);
+                NEED(k >= whole || share >= most || t.ntl <= share);
                 NEED(pg_share_begin(t.ntl, 0, n) == 0 && pg_share_begin(t.ntl, n, n) == t.ntl);
                 for (int i = 0; i < n && i < 70; i++)
                     NEED(pg_share_begin(t.ntl, i + 1, n) >= pg_share_begin(t.ntl, i, n));
             }
+            NEED(u == 0 || own == pg_parts(seqs[b], G, W, most, share));
+            C += own;
         }
         NEED(C <= p.shares && (!split || p.slots >= C));
     }
