@@ -622,6 +622,7 @@ def test_attention_of_hundreds_of_sequences(q):
     (4, [(0, 0)] * 15 + [(1, 9000)]),  # one sequence has all of the work of 16
     (16, [(1, 9000)]),
     (4, [(33, 17000)]),                # units of more than 16 shares
+    (4, [(1400, 1400), (60, 90)]),     # a new sequence: its first units stay whole
     (1, [(130, 2500), (1, 3)]),
 ])
 def test_attention_in_many_parts(Hq, lens, e4m3):
