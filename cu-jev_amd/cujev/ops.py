@@ -280,6 +280,8 @@ def _need_ints(name, *values):
 def _paged_call(dev, name, *args):
     """A call on the device of the pages, on that device's current stream."""
     import torch
+    if dev < 0:  # torch takes index -1 for the current GPU: host pointers would reach it
+        raise OpsError(f"{name}: the pages and tensors are in host memory, not on a GPU")
     fn = getattr(_lib or load(), name)
     if dev == torch.cuda.current_device():
         st = fn(*args, torch._C._cuda_getCurrentRawStream(dev))

@@ -134,3 +134,41 @@ def test_bindings_refuse_wrong_tensors():
                 dict(q_norm_w=w.bfloat16()), dict(k_norm_w=w[:128])]:
         with pytest.raises(ops.OpsError):
             ops.attn_prep_paged(**{**prep, **bad})
+
+
+def host_calls(e4m3):
+    """Calls of the three operators that are right but for the memory: all on the CPU."""
+    t = torch.float8_e4m3fn if e4m3 else torch.bfloat16
+    sc = [torch.ones(2, 1, 64) for _ in range(2 * e4m3)]
+    pages = ops.KvPages(torch.zeros(2, 1, 64, 256).to(t), torch.zeros(2, 1, 256, 64).to(t), *sc)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)
+    bf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)
+    q, w, seqs = bf(1, 4, 256), torch.ones(256), dict(kv_len=i32(1), page_table=i32(0)[None])
+    return {
+        PREP: lambda: ops.attn_prep_paged(
+            proj=bf(1, 2560), q_norm_w=w, k_norm_w=w, pos=i32(0), q_start=i32(0, 1), Hq=4, rot=64,
+            rope=torch.zeros(8, 32, 2), eps=1e-6, q_scale=0.1, q_out=q, pages=pages, **seqs),
+        READ: lambda: ops.kv_page_read(pages, max_kv=1, k_cache=bf(1, 1, 128, 256),
+                                       vt_cache=bf(1, 1, 256, 128), **seqs),
+        ATTN: lambda: ops.attention_paged(
+            q=q, gate=None, gate_tok_stride=0, gate_head_stride=0, pages=pages,
+            q_start=i32(0, 1), max_q=1, max_kv=1, out=bf(1, 1024), **seqs)}
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("name", [PREP, READ, ATTN])
+def test_bindings_refuse_tensors_in_host_memory(name, e4m3, monkeypatch):
+    """Device index -1 is the CPU's, and torch reads it as the current GPU's: such a
+    call would launch with host pointers. Nothing here can: the library is a stand-in."""
+    reached = []
+
+    class Library:
+        def __getattr__(self, symbol):
+            return lambda *args: reached.append(symbol) or 0
+
+    monkeypatch.setattr(ops, "_lib", Library())
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda dev: 0, raising=False)
+    with pytest.raises(ops.OpsError, match="host memory"):
+        host_calls(e4m3)[name]()
+    assert not reached
