@@ -1385,19 +1385,10 @@ __global__ __launch_bounds__(256) void merge_many_kernel(Call c) {
 } // namespace CUJEV_KNS
 using namespace CUJEV_KNS;
 
-/* o, l and mu of the slots' rows, then info */
-static size_t ws_bytes_of(const pg_plan &p, int Hkv) {
-    if (p.slots <= 0)
-        return 0;
-    return (size_t)p.slots * Hkv * p.rt * (PD + 2) * sizeof(float) +
-           (p.rt == FEW ? (size_t)p.units * sizeof(int2) : (size_t)p.slots * sizeof(int4));
-}
-
 extern "C" size_t cujev_attention_paged_ws_bytes(int N, int B, int max_q, int max_kv, int Hq,
                                                  int Hkv, int window, int sinks, int type) {
-    (void)type; /* the plan goes by key tiles */
-    const pg_plan p = pg_make_plan(N, B, max_q, max_kv, Hq / Hkv, Hkv, window, sinks);
-    return ws_bytes_of(p, Hkv);
+    (void)type, (void)window, (void)sinks; /* enough for either type and any window */
+    return pg_ws_most(N, B, max_q, max_kv, Hq / Hkv, Hkv);
 }
 
 extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int gate_tok_stride,
@@ -1413,7 +1404,7 @@ extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int
     if (p.shares < 0)
         return hipErrorInvalidValue;
     const size_t rows = (size_t)p.slots * Hkv * p.rt;
-    if (ws_bytes_of(p, Hkv) > ws_bytes)
+    if (pg_ws_bytes(p, Hkv) > ws_bytes)
         return hipErrorInvalidValue;
     if (window >= max_kv) /* no row's window ends before its first key */
         window = sinks = 0;

@@ -294,6 +294,8 @@ hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int gate_tok_s
                              const cujev_paged_seqs *seqs, int N, int max_q, int max_kv, int Hq,
                              int window, int sinks, bf16_t *out, void *ws, size_t ws_bytes,
                              hipStream_t stream);
+/* Enough for that call and every one of the same heads that is no larger in N, B, max_q
+ * and max_kv, of either type and any window. */
 size_t cujev_attention_paged_ws_bytes(int N, int B, int max_q, int max_kv, int Hq, int Hkv,
                                       int window, int sinks, int type);
 

@@ -402,8 +402,8 @@ EXPORT int cujev_op_attention_paged(const void *q, const void *gate, int gate_to
     if ((((uintptr_t)q | (uintptr_t)out) & 15) || ((uintptr_t)gate & 7) ||
         (gate && (gate_tok_stride % 4 || gate_head_stride % 4)))
         return fail(1, "attention_paged: q and out must be 16-byte, gate rows 8-byte aligned");
-    const size_t need = cujev_attention_paged_ws_bytes(N, B, max_q, max_kv, Hq, Hkv, window, sinks,
-                                                       kv_type);
+    const size_t need =
+        pg_ws_bytes(pg_make_plan(N, B, max_q, max_kv, Hq / Hkv, Hkv, window, sinks), Hkv);
     if (need > 0 && (!ws || ((uintptr_t)ws & 15) || ws_bytes < need))
         return fail(6, "attention_paged: needs a 16-byte aligned workspace of %zu bytes, got %zu",
                     need, ws ? ws_bytes : (size_t)0);

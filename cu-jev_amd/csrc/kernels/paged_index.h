@@ -5,6 +5,8 @@
 #ifndef CUJEV_PAGED_INDEX_H
 #define CUJEV_PAGED_INDEX_H
 
+#include <stddef.h>
+
 constexpr int PG = 64;   /* tokens a page, keys a tile */
 constexpr int VTOK = 16; /* positions of a V group of the prep */
 
@@ -166,6 +168,28 @@ constexpr unsigned pg_all_tiles(const pg_seq &s, int G, int window, int longest)
 /* First list entry of share i of n even ones */
 constexpr int pg_share_begin(int ntl, int i, int n) { return (int)((long long)ntl * i / n); }
 
+/* PG_FEW: waves of a kv-head. A wave a SIMD: 64 sequences of 1024 bf16 keys take 53 us
+ * so, 61 with two a SIMD, and half as many as SIMDs leave 24 of 5000 at 58 instead of
+ * 52. Few units: no more parts each than a merge takes in one go, 64 (one of 65536
+ * keys 42 us; 43 with 128 parts, 60 with 32). */
+constexpr int pg_few_goal(long long units, int Hkv) {
+    const int chip = pg_max(1024 / Hkv, 1);
+    return 64 * units < chip ? (int)(64 * units) : chip;
+}
+/* and pieces, at most, of a line of `units` units of up to `most` tiles: pieces of two
+ * tiles, or of one if there are no more than this of them */
+constexpr int pg_few_pieces(long long units, long long most, int goal) {
+    const long long line = units * most, two = (line + 1) / 2;
+    const long long one = units > PG_FEW_SHORT / 2 ? 2 * units : PG_FEW_SHORT;
+    const long long n = two > one ? two : line < one ? line : one;
+    return n < goal ? (int)n : goal;
+}
+constexpr int pg_many_goal(int Hkv) { return pg_max(256 / Hkv, 1); }
+/* Lists this long may be split among workgroups */
+constexpr bool pg_many_long(long long most) { return most > PG_MANY_LEAST + PG_MANY_MERGE; }
+/* Units times kv-heads, and shares times kv-heads, that a call may have */
+constexpr int PG_MOST_UNITS = 1 << 22;
+
 constexpr pg_plan pg_make_plan(int N, int B, int max_q, int max_kv, int G, int Hkv, int window,
                                int sinks) {
     pg_plan p{};
@@ -179,34 +203,24 @@ constexpr pg_plan pg_make_plan(int N, int B, int max_q, int max_kv, int G, int H
     const long long most = pg_max(pg_max_tiles(tok, max_kv, window, sinks), 1);
     long long units = B, shares = 0, slots = 0;
     if (p.rt == PG_FEW) {
-        /* A wave a SIMD: 64 sequences of 1024 bf16 keys take 53 us so, 61 with two
-         * a SIMD, and half as many as SIMDs leave 24 of 5000 at 58 instead of 52.
-         * Few units: no more parts each than a merge takes in one go, 64 (one of
-         * 65536 keys 42 us; 43 with 128 parts, 60 with 32). */
-        p.goal = pg_max(1024 / Hkv, 1);
-        p.goal = 64 * units < p.goal ? (int)(64 * units) : p.goal;
-        /* a line of at most units * most tiles, which are ints: pieces of two, or of
-         * one if there are no more than this of them */
-        const long long line = units * most, two = (line + 1) / 2;
-        const long long one = units > PG_FEW_SHORT / 2 ? 2 * units : PG_FEW_SHORT;
-        shares = two > one ? two : line < one ? line : one;
-        shares = line > 0x7fffffff ? PG_MOST : shares < p.goal ? shares : p.goal;
+        p.goal = pg_few_goal(units, Hkv);
+        shares = units * most > 0x7fffffff ? PG_MOST : pg_few_pieces(units, most, p.goal);
         slots = most > 1 ? 2 * shares : 0;
     } else {
         const long long by_rows = (long long)N * G / PG_MANY + B;
         const long long by_len = B * ((mq * G + PG_MANY - 1) / PG_MANY);
         units = by_rows < by_len ? by_rows : by_len;
         /* the rows that the caller brings fill the chip: whole units */
-        p.goal = pg_max(256 / Hkv, 1);
+        p.goal = pg_many_goal(Hkv);
         if ((long long)N * G / PG_MANY >= p.goal)
             p.goal = 0;
-        const bool split = p.goal > 0 && most > PG_MANY_LEAST + PG_MANY_MERGE;
+        const bool split = p.goal > 0 && pg_many_long(most);
         if (!split)
             p.goal = 0;
         shares = units > p.goal ? units : p.goal;
         slots = split ? p.goal : 0;
     }
-    if (units * Hkv > 1 << 22 || shares * Hkv > 1 << 22) {
+    if (units * Hkv > PG_MOST_UNITS || shares * Hkv > PG_MOST_UNITS) {
         p.shares = -1;
         return p;
     }
@@ -214,6 +228,34 @@ constexpr pg_plan pg_make_plan(int N, int B, int max_q, int max_kv, int G, int H
     p.shares = (int)shares;
     p.slots = (int)slots;
     return p;
+}
+
+/* ---- workspace -------------------------------------------------------------------
+ * o (256), l and mu of the slots' rows as floats, then info: {int, int} a unit, or 4
+ * ints a slot. */
+constexpr size_t pg_slot_bytes(int slots, int rt, int Hkv, int infos, int info_bytes) {
+    return slots <= 0 ? 0
+                      : (size_t)slots * Hkv * rt * (256 + 2) * 4 + (size_t)infos * info_bytes;
+}
+constexpr size_t pg_ws_bytes(const pg_plan &p, int Hkv) {
+    return p.rt == PG_FEW ? pg_slot_bytes(p.slots, p.rt, Hkv, p.units, 8)
+                          : pg_slot_bytes(p.slots, p.rt, Hkv, p.slots, 16);
+}
+/* The most that a call of these heads can need whose N, B, max_q and max_kv are these or
+ * less, whatever its window: a prompt's rows fill the chip and leave nothing to merge,
+ * and the steps after it, smaller calls, do. Slots rise with B and max_kv up to what
+ * the chip runs at once, so that it is about 34 MB at the very most. */
+constexpr size_t pg_ws_most(int N, int B, int max_q, int max_kv, int G, int Hkv) {
+    const long long mq = pg_min(max_q, N);
+    if (mq <= 0 || B <= 0)
+        return 0;
+    const int most = pg_div_up(pg_max(max_kv, 0), PG);
+    const int units = pg_min(B, PG_MOST_UNITS / Hkv);
+    const int pieces = pg_few_pieces(units, most, pg_few_goal(units, Hkv));
+    const size_t few = pg_slot_bytes(most > 1 ? 2 * pieces : 0, PG_FEW, Hkv, units, 8);
+    const int goal = mq * G > PG_FEW && pg_many_long(most) ? pg_many_goal(Hkv) : 0;
+    const size_t many = pg_slot_bytes(goal, PG_MANY, Hkv, goal, 16);
+    return few > many ? few : many;
 }
 
 /* Whether every row at positions pmin .. pmax sees all PG keys from k0 on */

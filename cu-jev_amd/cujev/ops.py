@@ -368,6 +368,8 @@ def kv_page_read(pages, page_table, kv_len, max_kv, k_cache, vt_cache):
 
 
 def attention_paged_ws_bytes(N, B, max_q, max_kv, Hq, Hkv, window=0, sinks=0, e4m3=False) -> int:
+    """Bytes that are enough for this call and for every smaller one of the same heads (N,
+    B, max_q and max_kv no larger), whatever its window and type."""
     _need_ints("attention_paged_ws_bytes", N, B, max_q, max_kv, Hq, Hkv, window, sinks)
     return int(load().cujev_ops_attention_paged_ws_bytes(N, B, max_q, max_kv, Hq, Hkv, window,
                                                          sinks, int(e4m3)))
@@ -378,8 +380,8 @@ def attention_paged(q, gate, gate_tok_stride, gate_head_stride, pages, page_tabl
     """Attention of the call's rows q [N, Hq, 256] over their sequences' pages,
     causal; with window > 0 over the last `window` positions and the first
     `sinks`. gate may be None. max_q and max_kv bound the sequences' new tokens
-    and keys; ws: uint8 device workspace of attention_paged_ws_bytes (None where
-    that is 0)."""
+    and keys; ws: uint8 device workspace of attention_paged_ws_bytes, of this call or
+    a larger one (None where that is 0)."""
     import torch
     dev, B = _paged_seqs(pages, page_table, kv_len, q_start)
     if (max_q | max_kv | window | sinks | gate_tok_stride | gate_head_stride) >> 31:

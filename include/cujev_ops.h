@@ -257,8 +257,12 @@ int cujev_op_kv_page_read(int kv_type, const void *k_pages, const void *vt_pages
  * keys that some row of the call sees have to be finite; other slots may hold
  * anything. Any Hq / Hkv up to 16, Hq up to 8192. No sequence has more than max_q new tokens
  * or max_kv keys (what is past them is not computed, or not seen). ws: device
- * workspace of cujev_ops_attention_paged_ws_bytes() for the same arguments
- * (0: none needed); calls that may overlap need one each. */
+ * workspace, 16-byte aligned, that need not be cleared; calls that may overlap
+ * need one each. cujev_ops_attention_paged_ws_bytes() is enough for the call of
+ * its arguments and for every smaller one (N, B, max_q and max_kv no larger, the
+ * same heads, either type, any window), so that one workspace of the largest
+ * call serves prompts and the steps after them. At most 34 MB and 8 bytes a
+ * sequence for up to 256 kv-heads; 0: no such call needs one. */
 int cujev_op_attention_paged(const void *q, const void *gate, int gate_tok_stride,
                              int gate_head_stride, int kv_type, const void *k_pages,
                              const void *vt_pages, const float *k_scale, const float *v_scale,

@@ -1,0 +1,77 @@
+"""GPU tests of the paged K/V cache's calls as a server makes them: one workspace
+for all, and lengths, strides and values at the ends of their ranges. Inputs,
+oracle and tolerances are test_gpu_paged.py's and paged_oracle.py's.
+"""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import paged_oracle as po  # noqa: E402
+import test_gpu_paged as gp  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+PAGE, D = po.PAGE, po.D
+
+
+def oracle(c, window=0, sinks=0, gate=True, there=None):
+    """(out, tolerance) of the case; `there`: per sequence the keys that are there."""
+    k, v = gp.values(c["pages"])
+    K, V, keys = [], [], []
+    for b, n in enumerate(c["kv_len"]):
+        at = [c["tab"][b][p // PAGE] for p in range(n)]
+        at, slot = torch.tensor(at, dtype=torch.long), torch.arange(n) % PAGE
+        K.append(k[at, :, slot].transpose(0, 1))
+        V.append(v[at, :, slot].transpose(0, 1))
+        keys.append(torch.ones(n, dtype=torch.bool) if there is None else there[b])
+    return po.attention(c["q"].double(), c["gate"].double() if gate else None, K, V, keys,
+                        c["qs"], c["kv_len"], window, sinks)
+
+
+def run(c, ws, window=0, sinks=0, gate=True, max_q=None, max_kv=None):
+    """attention_paged with this workspace, checked against nothing."""
+    o, N, Hq = gp.ops(), c["N"], c["Hq"]
+    g = c["gate"].cuda() if gate else None
+    out = torch.full((N, Hq * D), 7.0, dtype=torch.bfloat16, device="cuda")
+    o.attention_paged(c["q"].cuda(), g, Hq * D, D, c["pages"], gp.i32(c["tab"]), gp.i32(c["qs"]),
+                      gp.i32(c["kv_len"]), c["max_q"] if max_q is None else max_q,
+                      c["max_kv"] if max_kv is None else max_kv, out, window=window, sinks=sinks,
+                      ws=ws)
+    torch.cuda.synchronize()
+    return out.cpu().double().view(N, Hq, D)
+
+
+def check(got, ref, tol, rows):
+    assert torch.isfinite(got[:rows]).all()
+    over = (got - ref)[:rows].abs() - tol[:rows]
+    assert (over <= 0).all(), f"off by {over.max():.3g} over the bound, at {int(over.argmax())}"
+
+
+def test_one_workspace_serves_a_prompt_and_the_steps_after_it():
+    """Sized for a call of 2200 new tokens, whose rows fill the chip: chunks, single
+    tokens, windows and both types of pages go through it, full of NaN before each."""
+    Hq, Hkv = 16, 4
+    nb = gp.ops().attention_paged_ws_bytes(2200, 3, 2200, 2200, Hq, Hkv)
+    assert nb > 0
+    ws = torch.empty(nb, dtype=torch.uint8, device="cuda")
+    for i, (lens, window, sinks, e4m3) in enumerate([
+            ([(2200, 2200)], 0, 0, False), ([(40, 2200), (20, 900)], 0, 0, False),
+            ([(40, 2200), (20, 900)], 0, 0, True), ([(1, 2200), (1, 300), (1, 64)], 0, 0, True),
+            ([(1, 2200), (1, 300)], 1000, 4, False), ([(60, 2200)], 1500, 4, True)]):
+        print(f"case {lens} window={window} sinks={sinks} e4m3={e4m3}", flush=True)
+        c = gp.attention_case(201 + 3 * i, Hq, Hkv, e4m3, lens)
+        ws.view(torch.float32).fill_(math.nan)
+        got = run(c, ws, window, sinks)
+        if i == 0:  # every 100th row: the oracle goes row by row
+            k, v = gp.values(c["pages"])
+            at, slot = torch.tensor(c["tab"][0])[torch.arange(2200) // PAGE], torch.arange(2200) % PAGE
+            K, V = k[at, :, slot].transpose(0, 1), v[at, :, slot].transpose(0, 1)
+            for n in range(0, 2200, 100):
+                ref, tol = po.attention(c["q"][n:n + 1].double(), c["gate"][n:n + 1].double(),
+                                        [K[:, :n + 1]], [V[:, :n + 1]],
+                                        [torch.ones(n + 1, dtype=torch.bool)], [0, 1], [n + 1], 0,
+                                        0)
+                check(got[n:n + 1], ref, tol, 1)
+            continue
+        check(got, *oracle(c, window, sinks), c["qs"][-1])

@@ -172,3 +172,16 @@ def test_bindings_refuse_tensors_in_host_memory(name, e4m3, monkeypatch):
     with pytest.raises(ops.OpsError, match="host memory"):
         host_calls(e4m3)[name]()
     assert not reached
+
+
+def test_a_workspace_of_the_largest_call_serves_the_smaller_ones():
+    """A prompt of 4096 merges nothing, the chunks and single tokens after it do."""
+    size = lambda N, B, max_q, max_kv, **kw: ops.attention_paged_ws_bytes(N, B, max_q, max_kv, 16,
+                                                                         4, **kw)
+    most = size(4096, 64, 4096, 8192)
+    assert 0 < most < 35 << 20
+    for N, B, max_q in [(4096, 1, 4096), (512, 1, 512), (64, 64, 1), (1, 1, 1), (2047, 64, 1024),
+                        (2048, 64, 1024)]:
+        for kw in (dict(), dict(window=512, sinks=4), dict(e4m3=True)):
+            for max_kv in (100, 1000, 8192):
+                assert size(N, B, max_q, max_kv, **kw) <= most

@@ -224,3 +224,49 @@ def test_every_index_stays_inside(tmp_path):
                     "-I", str(KERNELS), str(src), "-o", str(exe)], check=True)
     run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
     assert run.returncode == 0, run.stdout + run.stderr
+
+
+WORKSPACE = r"""
+#include "paged_index.h"
+#include <cstdio>
+
+static int bad;
+#define NEED(c) do { if (!(c) && bad++ < 10) printf("line %d: %s\n", __LINE__, #c); } while (0)
+static unsigned rs = 777;
+static int rnd(int lo, int hi) { rs = rs * 1664525u + 1013904223u; return lo + (int)((rs >> 4) % (unsigned)(hi - lo + 1)); }
+static int upto(int most) { return rnd(0, 3) ? rnd(0, most) : rnd(0, 1) ? most : rnd(0, most < 40 ? most : 40); }
+
+int main() {
+    for (int it = 0; it < 400000; it++) {
+        const int G = rnd(1, 16), Hkv = it % 5 ? 1 << rnd(0, 4) : rnd(1, 300);
+        const int N = rnd(0, it % 3 ? 300 : 9000), B = rnd(0, it % 4 ? 70 : 3000);
+        const int mq = it % 2 ? rnd(0, 20) : rnd(0, 5000), mk = rnd(0, it % 3 ? 3000 : 70000);
+        const size_t most = pg_ws_most(N, B, mq, mk, G, Hkv);
+        const int n = upto(N), b = upto(B), q = upto(mq), k = upto(mk), w = rnd(0, 1) ? 0 : rnd(1, 4000);
+        const pg_plan p = pg_make_plan(n, b, q, k, G, Hkv, w, w ? rnd(0, 200) : 0);
+        if (p.shares < 0) continue; /* refused */
+        NEED(pg_ws_bytes(p, Hkv) <= most);
+        NEED(pg_ws_most(n, b, q, k, G, Hkv) <= most);
+        NEED(Hkv > 256 || most <= (34u << 20) + 8ull * B);
+    }
+    /* a prompt that needs none, and what follows it */
+    NEED(pg_ws_bytes(pg_make_plan(4096, 1, 4096, 8192, 4, 4, 0, 0), 4) == 0);
+    NEED(pg_ws_bytes(pg_make_plan(512, 1, 512, 8192, 4, 4, 0, 0), 4) > 0);
+    NEED(pg_ws_most(4096, 1, 4096, 8192, 4, 4) >= pg_ws_bytes(pg_make_plan(512, 1, 512, 8192, 4, 4, 0, 0), 4));
+    NEED(pg_ws_most(4096, 1, 4096, 8192, 4, 4) >= pg_ws_bytes(pg_make_plan(1, 1, 1, 8192, 4, 4, 0, 0), 4));
+    /* nothing to merge in one tile; the largest arguments */
+    NEED(pg_ws_most(16, 16, 1, 64, 4, 4) == 0 && pg_ws_most(0, 4, 4, 4096, 4, 4) == 0);
+    NEED(pg_ws_most(0x7fffffff, 0x7fffffff, 0x7fffffff, 0x7fffffff, 16, 1) < (80u << 20));
+    printf("bad %d\n", bad);
+    return bad != 0;
+}
+"""
+
+
+def test_one_workspace_is_enough_for_every_smaller_call(tmp_path):
+    src, exe = tmp_path / "ws.cpp", tmp_path / "ws"
+    src.write_text(WORKSPACE)
+    subprocess.run(["g++", "-O2", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover",
+                    "-I", str(KERNELS), str(src), "-o", str(exe)], check=True)
+    run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stdout + run.stderr
