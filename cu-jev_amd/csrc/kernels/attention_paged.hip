@@ -90,8 +90,8 @@ DEV void settle(floatx16 (&o)[4]) {
 
 /* keys hi at most, and past lo or a sink (without branches) */
 DEV bool key_seen(int j, int hi, int lo, int sinks) { return (j <= hi) & ((j > lo) | (j < sinks)); }
-/* the same of keys j .. j + N - 1, a bit each (j >= 0; positions and windows are
- * within PG_MOST and PG_MOST_KEYS, so that no difference leaves an int) */
+/* the same of keys j .. j + N - 1, a bit each (0 <= j <= PG_MOST_KEYS, hi >= -PG_MOST and
+ * lo >= -1, so that no difference leaves an int) */
 template <int N> DEV uint32_t keys_seen(int j, int hi, int lo, int sinks) {
     auto below = [&](int x) { return (1u << min(max(x - j, 0), N)) - 1; }; /* keys < x */
     return below(hi + 1) & (~below(lo + 1) | below(sinks));
@@ -126,6 +126,10 @@ struct Call {
     int num_pages;
     const int32_t *q_start, *kv_len, *page_table;
     int max_pages, B, N, max_q, max_kv, Hq, Hkv, G, window, sinks;
+    /* the same for lists of tiles and the plan: 0 where no window ends behind key 0 of
+     * the call's max_kv. A row past max_kv keys (of a longer sequence) has a mask
+     * all the same. */
+    int list_window, list_sinks;
     int rG; /* r / G = r * rG >> 16 for r < 4096 (an integer division is 30 instructions) */
     bf16 *out;
     float *po, *pl, *pmu;
@@ -158,7 +162,7 @@ struct Where {
 };
 /* many rows: w's unit, parts and first from its sequence, whose parts begin at `have` */
 DEV void set_part(const Call &c, Where &w, int target, int have, int share) {
-    const int whole = pg_short_units(w.s, c.G, c.window, w.own, share), at = target - have;
+    const int whole = pg_short_units(w.s, c.G, c.list_window, w.own, share), at = target - have;
     w.parts = at < whole ? 1 : pg_nshare(w.own, share);
     w.unit = at < whole ? at : whole + (at - whole) / w.parts;
     w.first = at < whole ? target : have + whole + (w.unit - whole) * w.parts;
@@ -176,11 +180,11 @@ template <int RT_, int J> DEV Where locate_among(const Call &c, int target) {
 #pragma unroll
         for (int j = 0; j < J; j++) {
             units[j] = b0 + J * lane + j < c.B ? pg_units(s[j], c.G, RT_) : 0;
-            n[j] = units[j] ? pg_longest(s[j], c.G, RT_, c.window, c.sinks) : 0;
+            n[j] = units[j] ? pg_longest(s[j], c.G, RT_, c.list_window, c.list_sinks) : 0;
         }
     };
     auto parts_of = [&](int j, int share) {
-        return units[j] ? pg_parts(s[j], c.G, c.window, n[j], share) : 0;
+        return units[j] ? pg_parts(s[j], c.G, c.list_window, n[j], share) : 0;
     };
     if constexpr (J == 1) /* the only step */
         read(0);
@@ -194,7 +198,7 @@ template <int RT_, int J> DEV Where locate_among(const Call &c, int target) {
 #pragma unroll
             for (int j = 0; j < J; j++) {
                 T += FEWR || J > 1 ? (unsigned)units[j] * (unsigned)n[j]
-                                   : pg_all_tiles(s[j], c.G, c.window, n[j]) * (units[j] > 0);
+                                   : pg_all_tiles(s[j], c.G, c.list_window, n[j]) * (units[j] > 0);
                 U += units[j];
                 longest = max(longest, n[j]);
             }
@@ -267,7 +271,7 @@ template <int RT_> DEV Where locate(const Call &c, int target) {
     w.b = -1, w.begin = 0;
     w.s = seq_of(c, 0);
     const int units = pg_units(w.s, c.G, RT_);
-    const int n = pg_longest(w.s, c.G, RT_, c.window, c.sinks);
+    const int n = pg_longest(w.s, c.G, RT_, c.list_window, c.list_sinks);
     if (units == 0)
         return w;
     if constexpr (FEWR) {
@@ -277,8 +281,8 @@ template <int RT_> DEV Where locate(const Call &c, int target) {
     } else {
         int share = PG_MOST;
         if (pg_splits(c.plan, units)) {
-            share = pg_share_first(c.plan, units, pg_all_tiles(w.s, c.G, c.window, n), false);
-            while (pg_parts(w.s, c.G, c.window, n, share) > c.plan.goal)
+            share = pg_share_first(c.plan, units, pg_all_tiles(w.s, c.G, c.list_window, n), false);
+            while (pg_parts(w.s, c.G, c.list_window, n, share) > c.plan.goal)
                 share = pg_share_next(share);
             share = pg_share_last(share, n);
         }
@@ -330,7 +334,7 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
         const int lane = lane_again(), m = lane & 15, g = lane >> 4;
         const pg_seq s = w.s;
         const int b = w.b, rows = min(s.ql * c.G, FEW);
-        const pg_tiles list = pg_tile_list(s, 0, s.ql - 1, c.window, c.sinks);
+        const pg_tiles list = pg_tile_list(s, 0, s.ql - 1, c.list_window, c.list_sinks);
         /* tiles [i0, i1) of the unit's; a unit without a key has one that is not there */
         const int cut = (w.first + w.part) * w.size - w.begin;
         const int i0 = max(cut, 0), i1 = min(min(cut + w.size, w.own), list.ntl);
@@ -588,7 +592,7 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
                 const int l = __ffsll((unsigned long long)any) - 1;
                 w.s = seq_at(t, l);
                 w.b = b0 + l;
-                w.own = pg_longest(w.s, c.G, FEW, c.window, c.sinks);
+                w.own = pg_longest(w.s, c.G, FEW, c.list_window, c.list_sinks);
                 w.parts = (w.begin + w.own - 1) / w.size - w.first + 1;
                 break;
             }
@@ -683,7 +687,7 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
     const int b = w.b, nshare = w.parts, share = w.part;
     const int r0 = w.unit * RT, nrows = min(s.ql * c.G - r0, RT);
     const int i0 = r0 / c.G, rest = r0 - i0 * c.G, i1 = i0 + ((rest + nrows - 1) * c.rG >> 16);
-    const pg_tiles list = pg_tile_list(s, i0, i1, c.window, c.sinks);
+    const pg_tiles list = pg_tile_list(s, i0, i1, c.list_window, c.list_sinks);
     const int tb = pg_share_begin(list.ntl, share, nshare);
     const int ntl = pg_share_begin(list.ntl, share + 1, nshare) - tb;
     const size_t slot = slot_of(c, kh, w.first + share);
@@ -1406,13 +1410,12 @@ extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int
     const size_t rows = (size_t)p.slots * Hkv * p.rt;
     if (pg_ws_bytes(p, Hkv) > ws_bytes)
         return hipErrorInvalidValue;
-    if (window >= max_kv) /* no row's window ends before its first key */
-        window = sinks = 0;
+    const bool all = window >= max_kv; /* keys of a row, but behind max_kv */
     const Call c = {(const bf16 *)q, (const bf16 *)gate, gate_tok_stride, gate_head_stride,
                     pages->k, pages->vt, pages->k_scale, pages->v_scale, pages->num_pages,
                     seqs->q_start, seqs->kv_len, seqs->page_table, seqs->max_pages, B, N,
                     max_q, max_kv, Hq, Hkv, G, window, sinks,
-                    pg_div_up(65536, G), (bf16 *)out,
+                    all ? 0 : window, all ? 0 : sinks, pg_div_up(65536, G), (bf16 *)out,
                     (float *)ws, (float *)ws + rows * PD, (float *)ws + rows * (PD + 1),
                     (int32_t *)((float *)ws + rows * (PD + 2)), p};
     const bool few = p.rt == FEW;

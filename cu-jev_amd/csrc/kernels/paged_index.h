@@ -258,19 +258,22 @@ constexpr size_t pg_ws_most(int N, int B, int max_q, int max_kv, int G, int Hkv)
     return few > many ? few : many;
 }
 
+/* The row at position p sees the keys j <= min(p, kv - 1) with j > pg_low or j <
+ * sinks; a key is some row's from pmin on where it is before kv and past
+ * pg_low(pmin) or a sink. -1 where the window reaches key 0, so that no position
+ * from -PG_MOST on and no window leaves an int. */
+constexpr int pg_low(int p, int window) {
+    return window > 0 ? pg_max(pg_max(p, -1) - window, -1) : -1;
+}
 /* Whether every row at positions pmin .. pmax sees all PG keys from k0 on */
 constexpr bool pg_tile_whole(int k0, int pmin, int pmax, int kv, int window, int sinks) {
     return k0 + PG - 1 <= pg_min(pmin, kv - 1) &&
-           (window <= 0 || k0 > pmax - window || k0 + PG <= sinks);
+           (k0 > pg_low(pmax, window) || k0 + PG <= sinks);
 }
 /* Whether keys of the tile are no key of the call (behind the last one, or
  * before every window and no sink): whatever is there may not reach a product. */
 constexpr bool pg_tile_foreign(int k0, int pmin, int kv, int window, int sinks) {
-    return k0 + PG > kv || (window > 0 && k0 <= pmin - window && k0 + PG > sinks);
+    return k0 + PG > kv || (k0 <= pg_low(pmin, window) && k0 + PG > sinks);
 }
-/* The row at position p sees the keys j <= min(p, kv - 1) with j > pg_low or j <
- * sinks; a key is some row's from pmin on where it is before kv and past
- * pg_low(pmin) or a sink. */
-constexpr int pg_low(int p, int window) { return window > 0 ? p - window : -1; }
 
 #endif

@@ -75,3 +75,19 @@ def test_one_workspace_serves_a_prompt_and_the_steps_after_it():
                 check(got[n:n + 1], ref, tol, 1)
             continue
         check(got, *oracle(c, window, sinks), c["qs"][-1])
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("lens", [[(1, 400), (3, 130), (1, 90)], [(50, 400), (20, 90)]])
+@pytest.mark.parametrize("window,sinks", [(128, 0), (128, 4), (150, 0), (200, 70), (1000, 4),
+                                          (2 ** 31 - 1, 2 ** 31 - 1)])
+def test_rows_past_max_kv_keep_their_window(window, sinks, lens, e4m3):
+    """Sequences of more than max_kv = 128 keys with a window of at least that: a row
+    sees the keys before max_kv that its window or the sinks hold, and no others."""
+    o = gp.ops()
+    c = gp.attention_case(231, 8, 2, e4m3, lens)
+    nb = o.attention_paged_ws_bytes(c["N"], len(lens), c["max_q"], 128, 8, 2)
+    ws = torch.empty(nb, dtype=torch.uint8, device="cuda") if nb else None
+    there = [torch.arange(kv) < 128 for _, kv in lens]
+    got = run(c, ws, window, sinks, max_kv=128)
+    check(got, *oracle(c, window, sinks, there=there), c["qs"][-1])

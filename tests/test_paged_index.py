@@ -270,3 +270,50 @@ def test_one_workspace_is_enough_for_every_smaller_call(tmp_path):
                     "-I", str(KERNELS), str(src), "-o", str(exe)], check=True)
     run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
     assert run.returncode == 0, run.stdout + run.stderr
+
+
+MASKS = r"""
+#include "paged_index.h"
+#include <cstdio>
+#include <initializer_list>
+
+static int bad;
+#define NEED(c) do { if (!(c) && bad++ < 10) printf("line %d: %s\n", __LINE__, #c); } while (0)
+
+int main() {
+    const int P[] = {-PG_MOST, -PG_MOST + 1, -64, -1, 0, 1, 63, 64, 129, 2000, PG_MOST_KEYS, 0x7ffffffe, 0x7fffffff};
+    const int W[] = {0, 1, 2, 64, 65, 128, 1999, 2001, PG_MOST_KEYS, PG_MOST, 0x7ffffffe, 0x7fffffff};
+    const int S[] = {0, 1, 64, 100, PG_MOST_KEYS, 0x7fffffff};
+    const int KV[] = {1, 63, 64, 128, 500, 2048, PG_MOST_KEYS};
+    for (int kv : KV) for (int w : W) for (int sinks : S) for (int p : P) for (int more : {0, 1, 40}) {
+        const long long q = p + (long long)more;
+        if (q > 0x7fffffff) continue;
+        for (int k0 = 0; k0 < kv && k0 < 2200; k0 += PG) {
+            bool whole = true, foreign = false;
+            for (int j = k0; j < k0 + PG; j++) {
+                /* the definition in 64 bits, of the rows at p and q and of any between */
+                auto sees = [&](long long r) { return j <= r && j < kv && (w == 0 || j > r - w || j < sinks); };
+                whole &= sees(p) && sees(q);
+                const bool own = j < kv && (w == 0 || j > (long long)p - w || j < sinks);
+                NEED(sees(p) == (j <= p && j < kv && (j > pg_low(p, w) || j < sinks)));
+                NEED(own == (j < kv && (j > pg_low(p, w) || j < sinks)) || p < 0);
+                foreign |= !own;
+            }
+            NEED(!pg_tile_whole(k0, p, (int)q, kv, w, sinks) || whole);
+            NEED(!foreign || pg_tile_foreign(k0, p, kv, w, sinks) || p < 0);
+        }
+    }
+    printf("bad %d\n", bad);
+    return bad != 0;
+}
+"""
+
+
+def test_masks_of_any_position_and_window(tmp_path):
+    """Rows of sequences longer than the call's max_kv keep their window, however far."""
+    src, exe = tmp_path / "masks.cpp", tmp_path / "masks"
+    src.write_text(MASKS)
+    subprocess.run(["g++", "-O2", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover",
+                    "-I", str(KERNELS), str(src), "-o", str(exe)], check=True)
+    run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stdout + run.stderr
