@@ -15,11 +15,11 @@ constexpr int pg_max(int a, int b) { return a > b ? a : b; }
 constexpr int pg_div_up(int a, int b) { return a / b + (a % b != 0); } /* a >= 0, b > 0 */
 
 /* Sequence b as one call sees it: rows q0 .. q0 + ql - 1, the first at position
- * p0 (negative where it has fewer keys than rows: those rows have no slot),
- * keys 0 .. kv - 1. Lengths outside the call's N rows, max_q and max_kv are
- * cut, so no value in q_start or kv_len leads out of a buffer. N and B are at most
- * PG_MOST, max_kv and windows PG_MOST_KEYS: sums and differences of two fit an
- * int, and the key tiles of fewer than 512 units 32 bits. */
+ * p0 (negative where it has fewer keys than rows: those rows have no slot), keys
+ * 0 .. kv - 1, where rows past max_q bring none. Lengths outside the call's N rows,
+ * max_q and max_kv are cut, so no value in q_start or kv_len leads out of a buffer.
+ * N and B are at most PG_MOST, max_kv PG_MOST_KEYS: sums and differences of two
+ * fit an int, and the key tiles of fewer than 512 units 32 bits. */
 constexpr int PG_MOST = 1 << 30, PG_MOST_KEYS = 1 << 28;
 struct pg_seq {
     int q0, ql, kv, p0;
@@ -30,7 +30,7 @@ constexpr pg_seq pg_clean_seq(int q0, int q1, int kv, int N, int max_q, int max_
     const int ql = pg_min(pg_max(q1, s.q0), N) - s.q0;
     s.p0 = pg_max(kv, 0) - ql;
     s.ql = pg_min(ql, max_q);
-    s.kv = pg_min(pg_max(kv, 0), max_kv);
+    s.kv = pg_min(pg_max(s.p0 + s.ql, 0), max_kv);
     return s;
 }
 

@@ -256,7 +256,8 @@ int cujev_op_kv_page_read(int kv_type, const void *k_pages, const void *vt_pages
  * first tokens of the sequence); a row that sees no key gives 0. K and V of
  * keys that some row of the call sees have to be finite; other slots may hold
  * anything. Any Hq / Hkv up to 16, Hq up to 8192. No sequence has more than max_q new tokens
- * or max_kv keys (what is past them is not computed, or not seen). ws: device
+ * or max_kv keys: rows past max_q are left as they were and their keys seen by
+ * none, and keys past max_kv are not seen. ws: device
  * workspace, 16-byte aligned, that need not be cleared; calls that may overlap
  * need one each. cujev_ops_attention_paged_ws_bytes() is enough for the call of
  * its arguments and for every smaller one (N, B, max_q and max_kv no larger, the

@@ -91,3 +91,29 @@ def test_rows_past_max_kv_keep_their_window(window, sinks, lens, e4m3):
     there = [torch.arange(kv) < 128 for _, kv in lens]
     got = run(c, ws, window, sinks, max_kv=128)
     check(got, *oracle(c, window, sinks, there=there), c["qs"][-1])
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("lens,max_q", [([(8, 300), (2, 90), (5, 64)], 3),
+                                        ([(60, 300), (20, 90), (70, 70)], 25)])
+def test_tokens_past_max_q_reach_no_row(lens, max_q, e4m3):
+    """Of a sequence of more than max_q new tokens the first max_q are computed, the
+    others' rows stay as they were, and their keys, NaN here, are none of the call's."""
+    o, nan = gp.ops(), math.nan
+    c = gp.attention_case(241, 8, 2, e4m3, lens)
+    ref, tol = oracle(c)
+    pages = c["pages"]
+    for b, (n, kv) in enumerate(lens):
+        for p in range(kv - n + min(n, max_q), kv):
+            page, slot = c["tab"][b][p // PAGE], p % PAGE
+            for t in (pages.k[page, :, slot], pages.vt[page, :, :, slot]):
+                t.view(torch.uint8).fill_(0x7f) if e4m3 else t.fill_(nan)
+            if e4m3:
+                pages.k_scale[page, :, slot], pages.v_scale[page, :, slot] = nan, nan
+    nb = o.attention_paged_ws_bytes(c["N"], len(lens), max_q, c["max_kv"], 8, 2)
+    ws = torch.empty(nb, dtype=torch.uint8, device="cuda") if nb else None
+    got = run(c, ws, max_q=max_q)
+    for b, (n, kv) in enumerate(lens):
+        q0, q1, q2 = c["qs"][b], c["qs"][b] + min(n, max_q), c["qs"][b + 1]
+        check(got[q0:q1], ref[q0:q1], tol[q0:q1], q1 - q0)
+        assert (got[q1:q2] == 7.0).all(), "a row past max_q was written"

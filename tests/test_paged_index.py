@@ -317,3 +317,38 @@ def test_masks_of_any_position_and_window(tmp_path):
                     "-I", str(KERNELS), str(src), "-o", str(exe)], check=True)
     run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
     assert run.returncode == 0, run.stdout + run.stderr
+
+
+LENGTHS = r"""
+#include "paged_index.h"
+#include <cstdio>
+#include <initializer_list>
+
+static int bad;
+#define NEED(c) do { if (!(c) && bad++ < 10) printf("line %d: %s\n", __LINE__, #c); } while (0)
+
+int main() {
+    for (int ql : {0, 1, 5, 64, 200}) for (int kv : {-7, 0, 1, 3, 64, 500, 0x7fffffff})
+        for (int mq : {0, 1, 3, 64, 1000}) for (int mk : {1, 64, 400, PG_MOST_KEYS}) {
+            const pg_seq s = pg_clean_seq(2, 2 + ql, kv, 1000, mq, mk);
+            const int keys = kv < 0 ? 0 : kv;
+            NEED(s.p0 == keys - ql && s.ql == (ql < mq ? ql : mq));
+            /* a key is one of the call's where some computed row can see it, or the
+             * sequence has no new token */
+            const long long last = (long long)s.p0 + s.ql - 1;
+            const long long want = last + 1 < 0 ? 0 : last + 1;
+            NEED(s.kv == (want < mk ? want : mk));
+        }
+    printf("bad %d\n", bad);
+    return bad != 0;
+}
+"""
+
+
+def test_keys_end_with_the_last_computed_row(tmp_path):
+    src, exe = tmp_path / "lens.cpp", tmp_path / "lens"
+    src.write_text(LENGTHS)
+    subprocess.run(["g++", "-O2", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover",
+                    "-I", str(KERNELS), str(src), "-o", str(exe)], check=True)
+    run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stdout + run.stderr
