@@ -401,7 +401,7 @@ __global__ __launch_bounds__(256) void page_read_kernel(
     int max_kv, int Hkv, bf16 *__restrict__ kc, bf16 *__restrict__ vtc, int stride) {
     const int j = blockIdx.x >> 1, b = blockIdx.z, kh = blockIdx.y, tid = threadIdx.x;
     const int page = page_table[(size_t)b * max_pages + j]; /* beside kv_len's load */
-    const int kv = min(kv_len[b], max_kv), left = kv - j * PG; /* tokens of this page */
+    const int kv = min(max(kv_len[b], 0), max_kv), left = kv - j * PG; /* tokens of this page */
     if (left <= 0)
         return;
     const bool ok = page >= 0 && page < num_pages;

@@ -117,3 +117,19 @@ def test_tokens_past_max_q_reach_no_row(lens, max_q, e4m3):
         q0, q1, q2 = c["qs"][b], c["qs"][b] + min(n, max_q), c["qs"][b + 1]
         check(got[q0:q1], ref[q0:q1], tol[q0:q1], q1 - q0)
         assert (got[q1:q2] == 7.0).all(), "a row past max_q was written"
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_read_of_negative_lengths_writes_nothing(e4m3):
+    """Down to the least int, whose distance to a page's first key is none."""
+    o = gp.ops()
+    pages = gp.pool(251, 5, 1, e4m3)
+    kv_len = [-2 ** 31, -1, -2 ** 31 + 100, 3, -64]
+    kc = torch.full((5, 1, 256, D), 5.0, dtype=torch.bfloat16, device="cuda")
+    vc = torch.full((5, 1, D, 256), 5.0, dtype=torch.bfloat16, device="cuda")
+    o.kv_page_read(pages, gp.i32([[0, 1, 2, 3]] * 5), gp.i32(kv_len), 190, kc, vc)
+    torch.cuda.synchronize()
+    k, v = gp.values(pages)
+    want_k, want_v = torch.full(kc.shape, 5.0).double(), torch.full(vc.shape, 5.0).double()
+    want_k[3, :, :3], want_v[3, :, :, :3] = k[0, :, :3], v[0, :, :3].transpose(1, 2)
+    assert torch.equal(kc.cpu().double(), want_k) and torch.equal(vc.cpu().double(), want_v)
