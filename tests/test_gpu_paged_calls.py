@@ -133,3 +133,58 @@ def test_read_of_negative_lengths_writes_nothing(e4m3):
     want_k, want_v = torch.full(kc.shape, 5.0).double(), torch.full(vc.shape, 5.0).double()
     want_k[3, :, :3], want_v[3, :, :, :3] = k[0, :, :3], v[0, :, :3].transpose(1, 2)
     assert torch.equal(kc.cpu().double(), want_k) and torch.equal(vc.cpu().double(), want_v)
+
+
+def uneven(seed, B, lo, hi, most):
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randint(lo, hi + 1, (B,), generator=g).tolist()
+    return [(n, n + int(torch.randint(0, most, (1,), generator=g))) for n in q]
+
+
+# (Hq, Hkv, [(new tokens, keys)]): V by groups with a wave a page, which takes more than
+# 1024 waves' worth of groups at fewer than 128 rows a sequence; by rows; a wave a group
+BY_PAGES = [(16, 4, uneven(261, 50, 5, 50, 250)), (8, 4, uneven(262, 64, 40, 64, 70)),
+            (4, 4, uneven(263, 40, 0, 90, 30)), (16, 8, uneven(264, 30, 17, 100, 500)),
+            (16, 4, [(5, 3), (0, 0), (40, 20)] + uneven(265, 60, 10, 40, 64))]
+BY_ROWS = [(8, 2, uneven(266, 80, 0, 3, 200))]
+BY_GROUPS = [(16, 4, uneven(267, 5, 1, 70, 200)), (4, 1, [(130, 131), (1, 64)])]
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("Hq,Hkv,lens", BY_PAGES)
+def test_prep_of_chunks_of_many_sequences(Hq, Hkv, lens, e4m3):
+    N, B = sum(n for n, _ in lens) + 3, len(lens)  # three rows behind the last
+    assert min(N, N // PAGE + 2 * B) * Hkv * 4 > 1024 and N < 128 * B and not (B > 64 and N <= 3 * B)
+    gp.test_prep_writes_pages(Hq, Hkv, e4m3, lens)
+
+
+@pytest.mark.parametrize("Hq,Hkv,lens", BY_PAGES + BY_ROWS + BY_GROUPS)
+def test_prep_leaves_the_scales_of_other_slots(Hq, Hkv, lens):
+    """Every byte of the pool that no new token has, scales among them, stays; a page id
+    outside the pool leaves all of its tokens' out."""
+    o = gp.ops()
+    q_lens, kv_len = [n for n, _ in lens], [k for _, k in lens]
+    qs, N = gp.starts(q_lens), sum(q_lens)
+    num_pages = sum(-(-k // PAGE) for k in kv_len) + 2
+    pages, tab = gp.pool(271, num_pages, Hkv, True), gp.table(272, kv_len, num_pages)
+    tab[0][0], tab[-1][-1] = -1, num_pages
+    for t in (pages.k, pages.vt, pages.k_scale, pages.v_scale):  # no value that prep writes
+        t.view(torch.uint8).fill_(0x7f)
+    g = torch.Generator().manual_seed(273)
+    proj = torch.randn(N, Hq * 512 + Hkv * 512, generator=g).bfloat16().cuda()
+    w = torch.ones(D, device="cuda")
+    q_out = torch.empty(N, Hq, D, dtype=torch.bfloat16, device="cuda")
+    o.attn_prep_paged(proj, w, w, gp.i32([0] * N), gp.i32(qs), gp.i32(kv_len), gp.i32(tab), Hq,
+                      gp.ROT, o.rope_table(1e7, gp.ROT, 4), gp.EPS, gp.Q_SCALE, q_out, pages)
+    torch.cuda.synchronize()
+    written = torch.zeros(num_pages, PAGE, dtype=torch.bool)
+    for b in range(len(kv_len)):
+        for _, _, page, slot in po.slots(qs, kv_len, tab, b, num_pages):
+            written[page, slot] = True
+    written = written[:, None, :].expand(-1, Hkv, -1)
+    same = lambda t, dim: (t.cpu().view(torch.uint8) == 0x7f).all(dim)
+    for name, t in (("k_scale", pages.k_scale), ("v_scale", pages.v_scale)):
+        kept = same(t.reshape(num_pages, Hkv, PAGE, 1), 3)
+        assert torch.equal(kept, ~written), name
+    assert torch.equal(same(pages.k, 3), ~written)
+    assert torch.equal(same(pages.vt, 2), ~written)
