@@ -323,6 +323,10 @@ def attn_prep_paged(proj, q_norm_w, k_norm_w, pos, q_start, kv_len, page_table, 
     if proj.dtype is not torch.bfloat16 or proj.get_device() != dev or \
             proj.stride(1) != 1 or proj.shape[1] < Hq * 512 + Hkv * 512:
         raise OpsError(f"proj: need bfloat16 rows of {Hq * 512 + Hkv * 512} values on device {dev}")
+    # the stride of a single row is no distance between rows: any value may stand there
+    stride = proj.stride(0) if N > 1 else Hq * 512 + Hkv * 512
+    if stride >> 31:
+        _need_ints("attn_prep_paged: the stride of proj's rows", stride)
     f32, angles = torch.float32, (rope.shape[0], rot // 2, 2)
     if not (q_norm_w is not None and q_norm_w.dtype is f32 and q_norm_w.shape == (256,) and
             q_norm_w.is_contiguous() and q_norm_w.get_device() == dev and
@@ -339,7 +343,7 @@ def attn_prep_paged(proj, q_norm_w, k_norm_w, pos, q_start, kv_len, page_table, 
         _need("pos", pos, torch.int32, dev, (N,))
         _need("rope", rope, f32, dev, angles)
         _need("q_out", q_out, torch.bfloat16, dev, (N, Hq, 256))
-    _paged_call(dev, "cujev_op_attn_prep_paged", proj.data_ptr(), proj.stride(0),
+    _paged_call(dev, "cujev_op_attn_prep_paged", proj.data_ptr(), stride,
                 q_norm_w.data_ptr(), k_norm_w.data_ptr(), pos.data_ptr(), q_start.data_ptr(),
                 kv_len.data_ptr(), page_table.data_ptr(), page_table.shape[1], B, N, Hq, Hkv, rot,
                 rope.data_ptr(), rope.shape[0], eps, q_scale, q_out.data_ptr(), *pages.args)

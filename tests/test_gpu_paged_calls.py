@@ -188,3 +188,26 @@ def test_prep_leaves_the_scales_of_other_slots(Hq, Hkv, lens):
         assert torch.equal(kept, ~written), name
     assert torch.equal(same(pages.k, 3), ~written)
     assert torch.equal(same(pages.vt, 2), ~written)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_prep_of_one_row_of_any_stride(e4m3):
+    """A single row's stride says nothing: a column turned over gives a row's bits."""
+    o = gp.ops()
+    Hq, Hkv = 4, 1
+    g = torch.Generator().manual_seed(281)
+    row = torch.randn(1, Hq * 512 + Hkv * 512, generator=g).bfloat16().cuda()
+    w, rope = torch.ones(D, device="cuda"), o.rope_table(1e7, gp.ROT, 4)
+    column = row.reshape(-1, 1).clone().t()
+    assert column.stride(0) == 1
+    got = []
+    for proj in (row, column, row.as_strided(row.shape, (2 ** 33, 1))):
+        pages = o.kv_pages(1, Hkv, e4m3)
+        q = torch.empty(1, Hq, D, dtype=torch.bfloat16, device="cuda")
+        o.attn_prep_paged(proj, w, w, gp.i32([3]), gp.i32([0, 1]), gp.i32([4]), gp.i32([[0]]), Hq,
+                          gp.ROT, rope, gp.EPS, gp.Q_SCALE, q, pages)
+        got.append((q, pages.k, pages.vt))
+    torch.cuda.synchronize()
+    assert got[0][0].any()
+    for other in got[1:]:
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got[0], other))

@@ -185,3 +185,17 @@ def test_a_workspace_of_the_largest_call_serves_the_smaller_ones():
         for kw in (dict(), dict(window=512, sinks=4), dict(e4m3=True)):
             for max_kv in (100, 1000, 8192):
                 assert size(N, B, max_q, max_kv, **kw) <= most
+
+
+def test_prep_refuses_strides_that_an_int_does_not_hold():
+    """ctypes cuts them: rows 2^32 + 2560 values apart would be read as 2560 apart. (The
+    memory is asked for and never touched.)"""
+    pages = ops.KvPages(torch.zeros(2, 1, 64, 256).bfloat16(), torch.zeros(2, 1, 256, 64).bfloat16())
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)
+    far = 2 ** 32 + 2560
+    proj = torch.empty(far + 2560, dtype=torch.bfloat16).as_strided((2, 2560), (far, 1))
+    w = torch.ones(256)
+    with pytest.raises(ops.OpsError, match="stride of proj"):
+        ops.attn_prep_paged(proj, w, w, i32(0, 1), i32(0, 2), i32(2), i32(0)[None], 4, 64,
+                            torch.zeros(8, 32, 2), 1e-6, 0.1,
+                            torch.zeros(2, 4, 256).bfloat16(), pages)
