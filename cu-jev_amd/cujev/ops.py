@@ -214,9 +214,13 @@ class KvPages:
     """A layer's page pool: k [pages, Hkv, 64, 256] and vt [pages, Hkv, 256, 64],
     both bf16, or both float8_e4m3fn with float32 scales k_scale, v_scale
     [pages, Hkv, 64] (powers of two). The tensors are the caller's; kv_pages()
-    makes new ones."""
+    makes new ones. They are checked once, here, and cannot be set to others."""
 
-    __slots__ = ("k", "vt", "k_scale", "v_scale", "num_pages", "Hkv", "e4m3", "device", "args")
+    __slots__ = ("_tensors", "num_pages", "Hkv", "e4m3", "device", "args")
+    k = property(lambda self: self._tensors[0])
+    vt = property(lambda self: self._tensors[1])
+    k_scale = property(lambda self: self._tensors[2])
+    v_scale = property(lambda self: self._tensors[3])
 
     def __init__(self, k, vt, k_scale=None, v_scale=None):
         import torch
@@ -243,7 +247,7 @@ class KvPages:
             ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
         elif k_scale is not None or v_scale is not None:
             raise OpsError("KvPages: bfloat16 pages have no scales")
-        self.k, self.vt, self.k_scale, self.v_scale, self.device = k, vt, k_scale, v_scale, dev
+        self._tensors, self.device = (k, vt, k_scale, v_scale), dev
         # kv_type, k, vt, k_scale, v_scale, num_pages of the C calls
         self.args = (1 if self.e4m3 else 0, k.data_ptr(), vt.data_ptr(), ks, vs, n)
 

@@ -199,3 +199,17 @@ def test_prep_refuses_strides_that_an_int_does_not_hold():
         ops.attn_prep_paged(proj, w, w, i32(0, 1), i32(0, 2), i32(2), i32(0)[None], 4, 64,
                             torch.zeros(8, 32, 2), 1e-6, 0.1,
                             torch.zeros(2, 4, 256).bfloat16(), pages)
+
+
+def test_a_pool_keeps_the_tensors_that_were_checked():
+    """The calls go by the addresses taken then: another tensor in a tensor's place would
+    be passed over, and the memory of the old one written to after it was freed."""
+    f8, sc = torch.float8_e4m3fn, torch.ones(2, 1, 64)
+    k, vt = torch.zeros(2, 1, 64, 256).to(f8), torch.zeros(2, 1, 256, 64).to(f8)
+    pages = ops.KvPages(k, vt, sc, sc.clone())
+    for name in ("k", "vt", "k_scale", "v_scale"):
+        with pytest.raises(AttributeError):
+            setattr(pages, name, getattr(pages, name).clone())
+    assert pages.k is k and pages.vt is vt and pages.k_scale is sc
+    assert pages.args == (1, k.data_ptr(), vt.data_ptr(), sc.data_ptr(),
+                          pages.v_scale.data_ptr(), 2)
