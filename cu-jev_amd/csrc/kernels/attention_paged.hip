@@ -1431,8 +1431,8 @@ extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int
         hipLaunchKernelGGL(attention_many_kernel<false>, grid, dim3(512), 0, stream, c);
     if (p.slots > 0) {
         const int rows = pg_min(max_q, N) * G;
-        const bool row = few && (long long)p.units * rows * Hkv <= 512;
-        const int groups = !few ? RT / 16 : row ? rows : pg_div_up(rows, 4);
+        const bool row = pg_merge_by_row(p, rows, Hkv);
+        const int groups = pg_merge_groups(p, rows, Hkv);
         const dim3 mgrid((unsigned)((few ? p.units : p.slots) * Hkv * groups));
         if (row)
             hipLaunchKernelGGL(merge_few_kernel<true>, mgrid, dim3(256), 0, stream, c, groups);

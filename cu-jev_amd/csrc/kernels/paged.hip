@@ -512,7 +512,7 @@ extern "C" hipError_t k_attn_prep_paged(const bf16_t *proj, int proj_stride, con
                                : v_spread ? CEIL_DIV(v_pages * Hkv, 8) * 32
                                           : v_pages * Hkv;
     const long long blocks = k_blocks + v_blocks + row_blocks(PREP_TOK, Hq);
-    if (blocks > 0x7fffffff)
+    if (blocks * 64 > PG_MOST_ITEMS)
         return hipErrorInvalidValue;
     const Prep c = {(const bf16 *)proj, proj_stride, q_norm_w, k_norm_w, pos, seqs->q_start,
                     seqs->kv_len, seqs->page_table, seqs->max_pages, B, N, Hq, Hkv, rot,

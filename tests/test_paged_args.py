@@ -213,3 +213,20 @@ def test_a_pool_keeps_the_tensors_that_were_checked():
     assert pages.k is k and pages.vt is vt and pages.k_scale is sc
     assert pages.args == (1, k.data_ptr(), vt.data_ptr(), sc.data_ptr(),
                           pages.v_scale.data_ptr(), 2)
+
+
+@pytest.mark.parametrize("big", [dict(N=1 << 26, B=1), dict(N=1 << 28, B=1 << 28),
+                                 dict(N=1 << 26, B=1, kv_type=0)], ids=str)
+def test_prep_refuses_more_work_items_than_a_launch_may_have(big):
+    """2^32 and more, in a grid that is still an int."""
+    st, msg = call(PREP, **big)
+    assert st == INVALID and "unsupported shape" in msg
+
+
+@pytest.mark.parametrize("big", [
+    dict(N=1 << 21, B=1 << 21, max_q=1),      # 2^22 units of both kv-heads: the merge's 2^32
+    dict(N=1 << 22, B=1 << 21, max_q=2)], ids=str)
+def test_attention_refuses_more_work_items_than_a_launch_may_have(big):
+    """Before the attention itself has run, not after it."""
+    st, msg = call(ATTN, **{**big, "ws": FAKE, "ws_bytes": 1 << 40})
+    assert st == INVALID and "unsupported shape" in msg

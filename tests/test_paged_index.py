@@ -352,3 +352,52 @@ def test_keys_end_with_the_last_computed_row(tmp_path):
                     "-I", str(KERNELS), str(src), "-o", str(exe)], check=True)
     run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
     assert run.returncode == 0, run.stdout + run.stderr
+
+
+LAUNCHES = r"""
+#include "paged_index.h"
+#include <cstdio>
+#include <initializer_list>
+
+static int bad;
+#define NEED(c) do { if (!(c) && bad++ < 10) printf("line %d: %s\n", __LINE__, #c); } while (0)
+static unsigned rs = 4242;
+static int rnd(int lo, int hi) { rs = rs * 1664525u + 1013904223u; return lo + (int)((rs >> 4) % (unsigned)(hi - lo + 1)); }
+
+int main() {
+    int largest = 0;
+    for (int it = 0; it < 300000; it++) {
+        const int G = rnd(1, 16), Hkv = rnd(0, 3) ? 1 << rnd(0, 9) : rnd(1, 8192 / G);
+        const int q = it % 2 ? rnd(1, 16) : rnd(1, 5000), k = 1 << rnd(0, 16);
+        const int B = rnd(0, 1) ? (1 << 22) / Hkv + rnd(-2, 2) : 1 << rnd(0, 24);
+        if (B < 1) continue;
+        const long long n = (long long)B * q;
+        const int N = n < PG_MOST ? (int)n : PG_MOST;
+        const pg_plan p = pg_make_plan(N, B, q, k, G, Hkv, 0, 0);
+        if (p.shares <= 0) continue;
+        const int per = p.rt == PG_MANY && 8 % Hkv == 0 ? 8 / Hkv : 1;
+        const long long grid = (long long)pg_div_up(p.shares, per) * per * Hkv;
+        NEED(grid * (p.rt == PG_FEW ? 64 : 512) <= PG_MOST_ITEMS);
+        if (p.slots <= 0) continue;
+        const int rows = pg_min(q, N) * G;
+        const int groups = pg_merge_groups(p, rows, Hkv);
+        const long long merge = (long long)(p.rt == PG_FEW ? p.units : p.slots) * Hkv * groups;
+        NEED(merge * 256 <= PG_MOST_ITEMS);
+        /* each row has a place in it */
+        NEED(p.rt == PG_FEW ? groups * (pg_merge_by_row(p, rows, Hkv) ? 1 : 4) >= rows : groups * 16 == 128);
+        largest += merge * 256 > PG_MOST_ITEMS - (1 << 20);
+    }
+    NEED(largest > 0); /* calls right below the bound were among them */
+    printf("bad %d\n", bad);
+    return bad != 0;
+}
+"""
+
+
+def test_launches_stay_within_their_bounds(tmp_path):
+    src, exe = tmp_path / "grid.cpp", tmp_path / "grid"
+    src.write_text(LAUNCHES)
+    subprocess.run(["g++", "-O2", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover",
+                    "-I", str(KERNELS), str(src), "-o", str(exe)], check=True)
+    run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stdout + run.stderr
