@@ -82,6 +82,9 @@ template <bool NOP> DEV void mfma_out(floatx16 &o, bf16x8 a, bf16x8 p) {
     else
         asm volatile(MFMA "%0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(p));
 }
+DEV void mfma_zero(floatx16 &o, bf16x8 none) { /* none: zeros */
+    asm volatile("s_nop 1\n\t" MFMA "%0, %1, %1, 0" : "=a"(o) : "v"(none));
+}
 #undef MFMA
 /* before O is read or written by anything but mfma_out, and after */
 DEV void settle(floatx16 (&o)[4]) {
@@ -627,6 +630,12 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
  * the first K, 5 on the epilogue (the gates' 32768 sigmoids are 2 of them). */
 constexpr int RT = PG_MANY;
 constexpr float SHIFT_RANGE = 64.f;
+/* With the reference 0, V far from 1 can lead p v out of fp32's range: p = 2^62 and V =
+ * 2^70, or 2^-62 and 2^-70. So where a row's l ends beyond 2^+-32 its O is looked at, and
+ * where that is above 2^96 or below 2^-64 the workgroup does its share once more with
+ * the range 0: the reference is then the maximum and p at most 1, as it is for few
+ * rows. V up to 2^80 so is safe with any scores and any number of keys. */
+constexpr float LOST_L = 0x1p32f, LOST_HIGH = 0x1p96f, LOST_LOW = 0x1p-64f;
 
 template <bool E4M3> struct Lay {
     static constexpr int T = PSLICE * (E4M3 ? 1 : 2); /* bytes of a K or V^T tile */
@@ -638,7 +647,8 @@ template <bool E4M3> struct Lay {
     static constexpr int Q0 = P, Q1 = E4M3 ? TILES : V + T, QEND = Q1 + RT / 2 * PD * 2;
     static constexpr int STAT = RT * PD * 4; /* l behind the staged O */
     static constexpr int ALL = TILES > QEND ? TILES : QEND;
-    static constexpr int BYTES = ALL > STAT + RT * 8 ? ALL : STAT + RT * 8;
+    static constexpr int AGAIN = STAT + RT * 8, END = AGAIN + 8 * 4; /* a flag a wave */
+    static constexpr int BYTES = ALL > END ? ALL : END;
 };
 static_assert(Lay<false>::BYTES <= 163840 && Lay<true>::BYTES <= 163840, "LDS of a CU");
 
@@ -659,10 +669,13 @@ template <bool E4M3> DEV int perm_row(int m) {
                 : (m & ~12) | ((m & 4) << 1) | ((m & 8) >> 1);
 }
 
-template <bool E4M3>
-__global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
+/* A workgroup's share, with a reference of 0 within the range; true: once more with none.
+ * The second time is the first one's code again, and nothing but the range may be kept
+ * for it: of 128 + 128 registers 124 + 128 are taken. */
+template <bool E4M3> DEV bool attend_many(const Call &c, unsigned char *smem, const float range) {
     typedef Lay<E4M3> L;
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[L::BYTES];
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid)); /* unknown: what goes by it is worked out each time */
     /* XCD-aware: where the kv-heads divide the 8 XCDs, an XCD's workgroups read
      * the same kv-head. The longest (last) tiles of a sequence start first. */
     int kh, at;
@@ -675,14 +688,14 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
         at = blockIdx.x / c.Hkv;
     }
     if (at >= c.plan.shares)
-        return;
+        return false;
     const int target = c.plan.shares - 1 - at;
     const Where w = locate<RT>(c, target);
-    if (kh == 0 && target < c.plan.slots && threadIdx.x == 0)
+    if (kh == 0 && target < c.plan.slots && tid == 0)
         ((int4 *)c.info)[target] =
             int4{w.b, w.unit, w.b >= 0 && w.part == 0 ? w.parts : 0, 0};
     if (w.b < 0)
-        return;
+        return false;
     const pg_seq s = w.s;
     const int b = w.b, nshare = w.parts, share = w.part;
     const int r0 = w.unit * RT, nrows = min(s.ql * c.G - r0, RT);
@@ -692,7 +705,7 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
     const int ntl = pg_share_begin(list.ntl, share + 1, nshare) - tb;
     const size_t slot = slot_of(c, kh, w.first + share);
 
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int wi = wave & 3, wj = wave >> 2, h = lane >> 5, col = lane & 31;
 
     /* page ids of the list, 64 entries in a lane each; the first ahead of Q's loads,
@@ -708,6 +721,8 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
         lo = pg_low(s.p0 + tok, c.window);
     }
     const int pmin = s.p0 + i0, pmax = s.p0 + i1;
+    int sinks = c.sinks;
+    asm volatile("" : "+s"(sinks)); /* kept: loaded again, each tile waited for it */
 
     /* ---- tile loads: memory -> LDS (buffer_load ... lds: lane l's 16 bytes land
      * at base + 16 l, so the swizzle is applied to the address). Load n of a wave is
@@ -739,10 +754,13 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
                                                  vvoff, at, 0, 0);
     };
     /* scales of tile t: wave 0 K's, wave 1 V's */
+    const float *scales = wave ? c.vs : c.ks;
+    if constexpr (E4M3)
+        asm volatile("" : "+s"(scales));
     auto issue_scales = [&](int page, int t) {
         if constexpr (E4M3) {
             if (wave < 2) {
-                const float *src = (wave ? c.vs : c.ks) + slice(page) * PG;
+                const float *src = scales + slice(page) * PG;
                 const int at = L::SC + (wave ? 512 + (t & 3) * 256 : (t & 1) * 256);
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(make_rsrc(src, 256),
                                                          (lds_ptr)(smem + at), 4, lane * 4, 0, 0,
@@ -798,10 +816,14 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
         return __builtin_amdgcn_readlane(ids, t & 63);
     };
 
-    floatx16 o[4];
+    floatx16 o[4]; /* zeros by MFMAs: constants were kept in 16 registers */
+    {
+        bf16x8 none = {};
+        asm volatile("" : "+v"(none));
 #pragma unroll
-    for (int d = 0; d < 4; d++)
-        o[d] = floatx16{};
+        for (int d = 0; d < 4; d++)
+            mfma_zero(o[d], none);
+    }
     /* of this lane's row: running maximum, l, the reference agreed on; of the
      * current tile: its p, their sum, the reference this wave wants */
     float mrun = -INFINITY, lrun = 0.f, mus = 0.f, mx = 0.f, ls = 0.f, mul = 0.f;
@@ -832,18 +854,18 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
     /* hides what the rows of tile t's scores do not see */
     auto mask = [&](floatx16 &x, int t, bool there) {
         const int k0 = pg_tile_page(list, tb + t) * PG;
-        if (there && pg_tile_whole(k0, pmin, pmax, s.kv, c.window, c.sinks))
+        if (there && pg_tile_whole(k0, pmin, pmax, s.kv, c.window, sinks))
             return;
         const int kb = k0 + 32 * wj + (E4M3 ? 16 : 8) * h;
         const int top = there ? s.kv - 1 : -1;
-        const uint32_t bits = keys_seen<E4M3 ? 16 : 24>(kb, min(hi, top), lo, c.sinks);
+        const uint32_t bits = keys_seen<E4M3 ? 16 : 24>(kb, min(hi, top), lo, sinks);
         unroll_for<16>([&](auto iv) {
             constexpr int r = decltype(iv)::value;
             x[r] = hide_by<E4M3 ? r : 16 * (r >> 3) + (r & 7)>(bits, x[r]);
         });
         if constexpr (E4M3) /* a scale of no key of this call: any bits */
             vsc = __uint_as_float(
-                key_seen(kb + (lane & 15), top, pg_low(pmin, c.window), c.sinks)
+                key_seen(kb + (lane & 15), top, pg_low(pmin, c.window), sinks)
                     ? __float_as_uint(vsc)
                     : 0u);
     };
@@ -868,9 +890,9 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
                                                          false, false);
         mrun = fmaxf(mrun, fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])));
         /* a row without a key yet leaves the choice to the other wave */
-        mul = mrun == -INFINITY                    ? -INFINITY
-              : fabsf(mrun - mus) > SHIFT_RANGE ? ceilf(mrun)
-                                                   : mus;
+        mul = mrun == -INFINITY           ? -INFINITY
+              : fabsf(mrun - mus) > range ? ceilf(mrun)
+                                          : mus;
         moved = __any(mul != 0.f);
     };
 
@@ -937,16 +959,16 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
         asm volatile("" ::: "memory");
 
         const int k0 = pg_tile_page(list, tb + i) * PG;
-        if (!there || pg_tile_foreign(k0, pmin, s.kv, c.window, c.sinks)) {
+        if (!there || pg_tile_foreign(k0, pmin, s.kv, c.window, sinks)) {
             /* values of no key of these rows meet p = 0: make them 0 */
 #pragma unroll 1
             for (int n = 0; n < L::T / 8192; n++) {
-                const int at = (n * 512 + (int)threadIdx.x) * 16, d = at / (L::T / PD);
+                const int at = (n * 512 + tid) * 16, d = at / (L::T / PD);
                 const int piece = ((at >> 4) & (L::T / PD / 16 - 1)) ^ swz_v<E4M3>(d);
                 u32x4 w = lds_read16(lds, L::V + PAR * L::T + at);
                 const uint32_t bits =
                     there ? keys_seen<E4M3 ? 16 : 8>(k0 + (E4M3 ? 16 : 8) * piece, s.kv - 1,
-                                                     pg_low(pmin, c.window), c.sinks)
+                                                     pg_low(pmin, c.window), sinks)
                           : 0u;
                 unroll_for<4>([&](auto ie) {
                     constexpr int e = decltype(ie)::value;
@@ -1185,6 +1207,25 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
     __syncthreads();
     const float l = stat[32 * wi + col] + stat[RT + 32 * wi + col];
     const float inv = !whole ? 1.f : l > 0.f ? 1.f / l : 0.f;
+    bool lost = false; /* see LOST_L */
+    const bool large = l > LOST_L, small = l < 1.f / LOST_L && l > 0.f;
+    if (__any(large || small)) {
+        uint32_t most = 0;
+#pragma unroll
+        for (int d = 0; d < 4; d++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) /* on the bits: O may be NaN */
+                most = max(most, __float_as_uint(o[d][r]) & 0x7fffffffu);
+            asm volatile("" : "+a"(o[d])); /* read again below, not kept */
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        lost = (large && most > __float_as_uint(LOST_HIGH)) ||
+               (small && most < __float_as_uint(LOST_LOW));
+    }
+    int *again = (int *)(smem + L::AGAIN);
+    const int any_lost = __any(lost);
+    if (lane == 0)
+        again[wave] = any_lost;
     if (!whole && wj == 0 && h == 0) {
         c.pl[slot * RT + 32 * wi + col] = l;
         c.pmu[slot * RT + 32 * wi + col] = mus;
@@ -1201,6 +1242,10 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
         __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
+    if (range > 0.f && __any(again[lane & 7])) {
+        __syncthreads(); /* the flags are read, LDS is free */
+        return true;
+    }
 #pragma unroll
     for (int half = 0; half < 2; half++) { /* no branch between the reads */
         floatx4 v[8];
@@ -1224,6 +1269,22 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
             if (t0 + t < nrows)
                 *(bf16x4 *)(c.out + of_row(oat, t) + 4 * lane) = res;
         }
+    }
+    return false;
+}
+template <bool E4M3>
+__global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[Lay<E4M3>::BYTES];
+    /* c by an address that is unknown each time: known, the arguments were kept, in more
+     * registers than there are */
+    auto *args =
+        (const __attribute__((address_space(4))) Call *)__builtin_amdgcn_kernarg_segment_ptr();
+    float range = SHIFT_RANGE;
+    for (;;) {
+        asm volatile("" : "+s"(args));
+        if (!attend_many<E4M3>(*(const Call *)args, smem, range))
+            break;
+        range = 0.f;
     }
 }
 

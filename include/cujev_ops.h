@@ -252,12 +252,15 @@ int cujev_op_kv_page_read(int kv_type, const void *k_pages, const void *vt_pages
 /* Attention of the call's rows over their sequences' pages. q bf16
  * [N][Hq][256], scaled by 256^-1/2 * log2 e; gate as for cujev_op_attention,
  * or NULL for none; out bf16 [N][Hq*256]. The row at position p sees keys j <=
- * p and, where window > 0, of those only j > p - window and j < sinks (the
+ * p and, where window > 0, of those only j > p - window or j < sinks (the
  * first tokens of the sequence); a row that sees no key gives 0. K and V of
  * keys that some row of the call sees have to be finite; other slots may hold
- * anything. Any Hq / Hkv up to 16, Hq up to 8192. No sequence has more than max_q new tokens
- * or max_kv keys: rows past max_q are left as they were and their keys seen by
- * none, and keys past max_kv are not seen. ws: device
+ * anything. V's magnitudes from 2^-64 to 2^80 count in full, whatever the scores;
+ * of smaller ones, and of those 2^-50 of the largest beside them, the result may
+ * be 0, of larger ones infinite. p is rounded to bf16 before its product with V,
+ * as in cujev_op_attention. Any Hq / Hkv up to 16, Hq up to 8192. No sequence has
+ * more than max_q new tokens or max_kv keys: rows past max_q are left as they
+ * were and their keys seen by none, and keys past max_kv are not seen. ws: device
  * workspace, 16-byte aligned, that need not be cleared; calls that may overlap
  * need one each. cujev_ops_attention_paged_ws_bytes() is enough for the call of
  * its arguments and for every smaller one (N, B, max_q and max_kv no larger, the

@@ -211,3 +211,48 @@ def test_prep_of_one_row_of_any_stride(e4m3):
     assert got[0][0].any()
     for other in got[1:]:
         assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got[0], other))
+
+
+SCORES = {
+    # the score of (row n of N, key j of kv), up to noise
+    "62": lambda n, N, j, kv: 62.0, "-62": lambda n, N, j, kv: -62.0,
+    "30": lambda n, N, j, kv: 30.0, "-30": lambda n, N, j, kv: -30.0,
+    "by row": lambda n, N, j, kv: -62.0 + 124.0 * n / max(N - 1, 1),
+    "rising": lambda n, N, j, kv: 62.0 * (2 * j / kv - 1), "far": lambda n, N, j, kv: 400.0,
+}
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("lens", [[(1, 300), (3, 64), (2, 1500)], [(40, 1500), (33, 90), (1, 70)]])
+@pytest.mark.parametrize("size", [80, 40, 0, -40, -64])
+@pytest.mark.parametrize("scores", list(SCORES))
+def test_values_of_any_magnitude_and_scores_together(scores, size, lens, e4m3):
+    """V of up to 2^80 and down to 2^-64 beside scores of up to 62 either way, where the
+    softmax's reference may stay 0 and p comes to 2^62 or 2^-62."""
+    o = gp.ops()
+    Hq, Hkv = 8, 2
+    c = gp.attention_case(291, Hq, Hkv, False, lens)
+    g = torch.Generator().manual_seed(292)
+    shape = c["pages"].k.shape
+    score, N = SCORES[scores], c["qs"][-1]
+    by_key = scores == "rising"
+    k = 1 + 0.05 * torch.randn(shape, generator=g)
+    if by_key:
+        for b, (_, kv) in enumerate(lens):
+            for j in range(kv):
+                k[c["tab"][b][j // PAGE], :, j % PAGE] *= score(0, N, j, kv) / 62
+    vt = (2 * torch.rand(c["pages"].vt.shape, generator=g) - 1) * 2.0 ** size
+    for n in range(N):
+        c["q"][n] = (62.0 if by_key else score(n, N, 0, 1)) / 256
+    if e4m3:
+        kq, ks = po.quantise(k.double(), 3)
+        vq, vs = po.quantise(vt.double(), 2)
+        f8 = lambda t: t.float().to(torch.float8_e4m3fn).cuda()
+        c["pages"] = o.KvPages(f8(kq), f8(vq), ks.float().cuda(), vs.float().cuda())
+    else:
+        c["pages"] = o.KvPages(k.bfloat16().cuda(), vt.bfloat16().cuda())
+    nb = o.attention_paged_ws_bytes(c["N"], len(lens), c["max_q"], c["max_kv"], Hq, Hkv)
+    got = run(c, torch.empty(nb, dtype=torch.uint8, device="cuda"))
+    ref, tol = oracle(c)
+    check(got, ref, tol, N)
+    assert (got[N:] == 7.0).all()
