@@ -256,3 +256,66 @@ def test_values_of_any_magnitude_and_scores_together(scores, size, lens, e4m3):
     ref, tol = oracle(c)
     check(got, ref, tol, N)
     assert (got[N:] == 7.0).all()
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (200, 4)])
+def test_single_tokens_beside_a_prompt(window, sinks, e4m3):
+    """A step of 63 sequences with one more's prompt in it: one call, of tiles of many
+    rows for all."""
+    g = torch.Generator().manual_seed(301)
+    lens = [(1, int(k)) for k in torch.randint(1, 1500, (63,), generator=g)]
+    lens.insert(20, (200, 900))
+    c = gp.attention_case(302, 8, 2, e4m3, lens)
+    gp.check_attention(c, window, sinks)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("lens", [[(3, 300), (2, 64)], [(40, 300), (33, 90)]])
+def test_rows_before_the_first_sequence_and_no_keys_at_all(lens, e4m3):
+    """q_start may begin behind row 0; with max_kv 0 no row sees a key; with max_q 0 no
+    row is one of the call's."""
+    o = gp.ops()
+    c = gp.attention_case(311, 8, 2, e4m3, lens)
+    ref, tol = oracle(c)
+    nb = o.attention_paged_ws_bytes(c["N"] + 5, 2, c["max_q"], c["max_kv"], 8, 2)
+    ws = torch.empty(nb, dtype=torch.uint8, device="cuda")
+    pad = lambda t: torch.cat([torch.full_like(t[:5], math.nan), t])
+    late = {**c, "q": pad(c["q"]), "gate": pad(c["gate"]), "N": c["N"] + 5,
+            "qs": [n + 5 for n in c["qs"]]}
+    got, rows = run(late, ws), c["qs"][-1]
+    assert (got[:5] == 7.0).all() and (got[5 + rows:] == 7.0).all()
+    check(got[5:], ref, tol, rows)
+    got = run(c, ws, max_kv=0)
+    assert (got[:rows] == 0.0).all() and (got[rows:] == 7.0).all()
+    assert (run(c, ws, max_q=0) == 7.0).all()
+    # prep: the same rows, K and V from row 5 on
+    Hq, Hkv, N = 8, 2, c["N"] + 5
+    g = torch.Generator().manual_seed(312)
+    proj = torch.randn(N, Hq * 512 + Hkv * 512, generator=g).bfloat16().cuda()
+    w, rope = torch.ones(D, device="cuda"), o.rope_table(1e7, gp.ROT, 4)
+    outs = []
+    for first, at in ((5, gp.i32(late["qs"])), (0, gp.i32(c["qs"]))):
+        pages = o.kv_pages(c["pages"].num_pages, Hkv, e4m3)
+        q = torch.full((N - 5 + first, Hq, D), 7.0, dtype=torch.bfloat16, device="cuda")
+        o.attn_prep_paged(proj[5 - first:], w, w, gp.i32([1] * (N - 5 + first)), at,
+                          gp.i32(c["kv_len"]), gp.i32(c["tab"]), Hq, gp.ROT, rope, gp.EPS,
+                          gp.Q_SCALE, q, pages)
+        outs.append((q[first:], pages.k, pages.vt))
+        assert (q[:first] == 7.0).all() and (q[first + rows:] == 7.0).all()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(*outs))
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("lens,bad", [([(3, 300), (2, 64)], [1]), ([(40, 1500), (33, 90)], [5, 50])])
+def test_a_row_of_nan_or_infinity_stays_a_row(lens, bad, e4m3):
+    """q that is not finite in a row (and a head) reaches no other."""
+    c = gp.attention_case(321, 8, 2, e4m3, lens)
+    ref, tol = oracle(c)
+    c["q"][bad[0], 3], c["q"][bad[-1], 5, 7] = math.nan, math.inf
+    nb = gp.ops().attention_paged_ws_bytes(c["N"], 2, c["max_q"], c["max_kv"], 8, 2)
+    got, rows = run(c, torch.empty(nb, dtype=torch.uint8, device="cuda")), c["qs"][-1]
+    for n, h in ((bad[0], 3), (bad[-1], 5)):
+        got[n, h], ref[n, h], tol[n, h] = 0.0, 0.0, 0.0
+    check(got, ref, tol, rows)
