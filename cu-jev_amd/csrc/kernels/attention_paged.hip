@@ -671,7 +671,7 @@ template <bool E4M3> DEV int perm_row(int m) {
 
 /* A workgroup's share, with a reference of 0 within the range; true: once more with none.
  * The second time is the first one's code again, and nothing but the range may be kept
- * for it: of 128 + 128 registers 124 + 128 are taken. */
+ * for it: all of the 128 + 128 registers are taken. */
 template <bool E4M3> DEV bool attend_many(const Call &c, unsigned char *smem, const float range) {
     typedef Lay<E4M3> L;
     int tid = threadIdx.x;
@@ -721,8 +721,6 @@ template <bool E4M3> DEV bool attend_many(const Call &c, unsigned char *smem, co
         lo = pg_low(s.p0 + tok, c.window);
     }
     const int pmin = s.p0 + i0, pmax = s.p0 + i1;
-    int sinks = c.sinks;
-    asm volatile("" : "+s"(sinks)); /* kept: loaded again, each tile waited for it */
 
     /* ---- tile loads: memory -> LDS (buffer_load ... lds: lane l's 16 bytes land
      * at base + 16 l, so the swizzle is applied to the address). Load n of a wave is
@@ -754,13 +752,10 @@ template <bool E4M3> DEV bool attend_many(const Call &c, unsigned char *smem, co
                                                  vvoff, at, 0, 0);
     };
     /* scales of tile t: wave 0 K's, wave 1 V's */
-    const float *scales = wave ? c.vs : c.ks;
-    if constexpr (E4M3)
-        asm volatile("" : "+s"(scales));
     auto issue_scales = [&](int page, int t) {
         if constexpr (E4M3) {
             if (wave < 2) {
-                const float *src = scales + slice(page) * PG;
+                const float *src = (wave ? c.vs : c.ks) + slice(page) * PG;
                 const int at = L::SC + (wave ? 512 + (t & 3) * 256 : (t & 1) * 256);
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(make_rsrc(src, 256),
                                                          (lds_ptr)(smem + at), 4, lane * 4, 0, 0,
@@ -854,18 +849,18 @@ template <bool E4M3> DEV bool attend_many(const Call &c, unsigned char *smem, co
     /* hides what the rows of tile t's scores do not see */
     auto mask = [&](floatx16 &x, int t, bool there) {
         const int k0 = pg_tile_page(list, tb + t) * PG;
-        if (there && pg_tile_whole(k0, pmin, pmax, s.kv, c.window, sinks))
+        if (there && pg_tile_whole(k0, pmin, pmax, s.kv, c.window, c.sinks))
             return;
         const int kb = k0 + 32 * wj + (E4M3 ? 16 : 8) * h;
         const int top = there ? s.kv - 1 : -1;
-        const uint32_t bits = keys_seen<E4M3 ? 16 : 24>(kb, min(hi, top), lo, sinks);
+        const uint32_t bits = keys_seen<E4M3 ? 16 : 24>(kb, min(hi, top), lo, c.sinks);
         unroll_for<16>([&](auto iv) {
             constexpr int r = decltype(iv)::value;
             x[r] = hide_by<E4M3 ? r : 16 * (r >> 3) + (r & 7)>(bits, x[r]);
         });
         if constexpr (E4M3) /* a scale of no key of this call: any bits */
             vsc = __uint_as_float(
-                key_seen(kb + (lane & 15), top, pg_low(pmin, c.window), sinks)
+                key_seen(kb + (lane & 15), top, pg_low(pmin, c.window), c.sinks)
                     ? __float_as_uint(vsc)
                     : 0u);
     };
@@ -959,7 +954,7 @@ template <bool E4M3> DEV bool attend_many(const Call &c, unsigned char *smem, co
         asm volatile("" ::: "memory");
 
         const int k0 = pg_tile_page(list, tb + i) * PG;
-        if (!there || pg_tile_foreign(k0, pmin, s.kv, c.window, sinks)) {
+        if (!there || pg_tile_foreign(k0, pmin, s.kv, c.window, c.sinks)) {
             /* values of no key of these rows meet p = 0: make them 0 */
 #pragma unroll 1
             for (int n = 0; n < L::T / 8192; n++) {
@@ -968,7 +963,7 @@ template <bool E4M3> DEV bool attend_many(const Call &c, unsigned char *smem, co
                 u32x4 w = lds_read16(lds, L::V + PAR * L::T + at);
                 const uint32_t bits =
                     there ? keys_seen<E4M3 ? 16 : 8>(k0 + (E4M3 ? 16 : 8) * piece, s.kv - 1,
-                                                     pg_low(pmin, c.window), sinks)
+                                                     pg_low(pmin, c.window), c.sinks)
                           : 0u;
                 unroll_for<4>([&](auto ie) {
                     constexpr int e = decltype(ie)::value;
@@ -1275,14 +1270,16 @@ template <bool E4M3> DEV bool attend_many(const Call &c, unsigned char *smem, co
 template <bool E4M3>
 __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
     __shared__ __attribute__((aligned(1024))) unsigned char smem[Lay<E4M3>::BYTES];
-    /* c by an address that is unknown each time: known, the arguments were kept, in more
-     * registers than there are */
+    /* c by an address that is unknown each time: known, the arguments were kept for the
+     * second time, in more registers than there are. A copy: through the address they
+     * were loaded where they are used, tile by tile (12 x 500 0.6 us more). */
     auto *args =
         (const __attribute__((address_space(4))) Call *)__builtin_amdgcn_kernarg_segment_ptr();
     float range = SHIFT_RANGE;
     for (;;) {
         asm volatile("" : "+s"(args));
-        if (!attend_many<E4M3>(*(const Call *)args, smem, range))
+        const Call a = *(const Call *)args;
+        if (!attend_many<E4M3>(a, smem, range))
             break;
         range = 0.f;
     }
