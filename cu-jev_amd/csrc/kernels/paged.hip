@@ -19,20 +19,20 @@ namespace {
  * are a wave's, or waves' on one XCD, whose L2 gathers their lines of V^T. With
  * V_ROWS V's tokens are row waves, too, and store single elements.
  *
- * 8 sequences of up to 700 tokens, e4m3: 15 us for 62 MB, 4.1 TB/s (25 with a page's
- * groups apart, reductions through LDS and rope loads by all lanes). 64 of one token:
- * 6.3 us, a chain of loads: arguments, lengths, page ids, stores. Four tokens a wave,
- * two of e4m3 keys: their rounding needs the registers. A wave a workgroup: 1024
- * tokens bf16 take 9.0 us so, 10.6 with four. */
+ * 8 sequences of up to 700 tokens, e4m3: 15.5 us a call (16.0 traced) for 62 MB, 4.0
+ * TB/s; reductions through LDS, rope loads by all lanes and a page's groups on other
+ * XCDs took 25. 64 of one token: 6.3 us, a chain of loads: arguments, lengths, page
+ * ids, stores; bf16 5.2. Four tokens a wave, two of e4m3 keys: their rounding needs
+ * the registers. A wave a workgroup: 1024 tokens bf16 take 8.6 us so, 10.6 with four. */
 constexpr int PREP_TOK = 4;
 /* V by rows as well, a token's 256 values as single elements, where there are many
  * sequences of a token or so each: 1024 x 1 e4m3 26 us, 38 by groups, each of which
  * has to find its sequence among all; 1024 x 3 bf16 63 and 84; but 256 x 4 20.0 and
  * 18.7, and 64 x 1 bf16 6.6 and 5.5. */
 constexpr int PREP_V_ROWS = 3, PREP_V_SEQS = 64;
-/* V by groups, a wave each where they are few or most of a page's are there (16 x 48
- * e4m3 9.5 us, 13.9 with a wave a page; 8 x 700 17.0 and 18.4), a wave a page
- * otherwise, which starts fewer that have nothing to do (64 x 48 22 and 27). */
+/* V by groups, a wave each where they are few or most of a page's are there (kernel of
+ * 16 x 48 e4m3 7.5 us, 11.2 with a wave a page; of 8 x 700 16.4 and 17.6), a wave a
+ * page otherwise, which starts fewer that have nothing to do (64 x 48 16.7 and 19.5). */
 constexpr int PREP_V_FEW = 1024, PREP_V_WHOLE = 128;
 /* A K row's lane in doubles, rounded to e4m3 once: the bytes, and the scale 2^*e */
 DEV uint32_t k_row_exact(const bf16 *src, const float2 *rope, const float *w, bool rotates,
@@ -371,10 +371,9 @@ __global__ __launch_bounds__(64) void prep_paged_kernel(Prep c) {
     };
     /* The longest first (8 x 700 e4m3 1.7 us less than with q's rows first) */
     if (block < c.v_blocks) {
-        if constexpr (V_ROWS)
+        if constexpr (V_ROWS) {
             return rows(is<ROW_V>{}, is<PREP_TOK>{}, c.Hkv);
-        else
-            {
+        } else {
             /* a page's groups on one XCD: block b runs on b % 8 */
             const int group = block / 8 % 4;
             return c.v_spread ? v_groups<E4M3>(c, block / 32 * 8 + block % 8, group, group + 1)
@@ -392,7 +391,7 @@ __global__ __launch_bounds__(64) void prep_paged_kernel(Prep c) {
  * One workgroup per (sequence, page, kv-head, K or V^T): 64 rows of 512 bytes
  * or 256 rows of 128 out, 16 values a thread and step. A page id outside the
  * pool reads as zeros; columns from kv_len on stay as they were. 8192 keys of 4
- * kv-heads from e4m3: 10.4 us for 50 MB, 4.8 TB/s. */
+ * kv-heads from e4m3: 10.4 us a call for 50 MB, 4.9 TB/s. */
 template <bool E4M3>
 __global__ __launch_bounds__(256) void page_read_kernel(
     const void *__restrict__ k_pages, const void *__restrict__ vt_pages,

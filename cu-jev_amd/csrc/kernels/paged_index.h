@@ -74,7 +74,9 @@ constexpr int pg_max_tiles(int tok, int max_kv, int window, int sinks) {
  * A unit is a tile of rt packed rows (token, q-head of the group) of a sequence and
  * kv-head. rt is PG_FEW where no sequence of the call has more rows than that (one
  * unit each; 16 are the columns of its MFMA), PG_MANY otherwise: 64 sequences' 16 rows
- * on 2560 e4m3 keys take 78 us as the former, 103 as the latter.
+ * on 2560 e4m3 keys take 78 us as the former, 103 as the latter. It is one for the
+ * call: single tokens beside a prompt are tiles of PG_MANY, too (64 on up to 4096 e4m3
+ * keys and a prompt of 512 127 us; 68 and 25 in two calls, one for each kind).
  *
  * PG_FEW: the units' key tiles, one after the other, are a line that pieces of equal
  * size cut, a wave's work each; what lies in one piece of one unit is a part.

@@ -6,7 +6,8 @@
  * (src/engine/forward.c:92-145). libcujev.so keeps exactly the 14 public
  * functions of include/cujev.h, so this separate library exposes the same
  * kernels one by one for kernel-level parity tests and benchmarks (the
- * reference has no kernel-level tests). Every entry point takes device
+ * reference has no kernel-level tests), and operators that the engine has no
+ * use for: the paged K/V cache. Every entry point takes device
  * pointers, plain sizes and a HIP stream (hipStream_t passed as void*; NULL is
  * the default stream), launches asynchronously and returns a cujev_status:
  * CUJEV_ERR_INVALID_ARGUMENT for shapes the kernels do not support,
@@ -216,9 +217,10 @@ int cujev_op_attention_noalloc(const void *q, const void *gate, int gate_tok_str
  *   page_table [B][max_pages]   position p is slot p % 64 of page
  *                     page_table[b][p / 64]
  * Sequences may share pages that a call only reads. A page that a call writes
- * belongs to one of its sequences: two sequences that write the same slot
- * leave either's values. Lengths are cut to N, max_pages * 64 (and max_q,
- * max_kv where given); a page id outside [0, num_pages) is a page that is not
+ * belongs to one of its sequences: of two sequences that write the same slot
+ * one's values may be left with the other's scale, or some of each. Lengths are
+ * cut to N, max_pages * 64 (and max_q, max_kv where given), where positions stay
+ * as kv_len has them; a page id outside [0, num_pages) is a page that is not
  * there: nothing is written to it, its keys are seen by no row, it reads as
  * zeros. These arrays are read on the device, so a captured graph can be
  * replayed with other lengths and tables within the same bounds. */
@@ -258,7 +260,10 @@ int cujev_op_kv_page_read(int kv_type, const void *k_pages, const void *vt_pages
  * anything. V's magnitudes from 2^-64 to 2^80 count in full, whatever the scores;
  * of smaller ones, and of those 2^-50 of the largest beside them, the result may
  * be 0, of larger ones infinite. p is rounded to bf16 before its product with V,
- * as in cujev_op_attention. Any Hq / Hkv up to 16, Hq up to 8192. No sequence has
+ * as in cujev_op_attention. max_q * Hq / Hkv <= 16 takes the form for few rows,
+ * more the one for many, for all sequences of the call: single tokens beside a
+ * prompt are faster in a call of their own, over their part of q_start, kv_len and
+ * page_table. Any Hq / Hkv up to 16, Hq up to 8192. No sequence has
  * more than max_q new tokens or max_kv keys: rows past max_q are left as they
  * were and their keys seen by none, and keys past max_kv are not seen. ws: device
  * workspace, 16-byte aligned, that need not be cleared; calls that may overlap

@@ -319,3 +319,28 @@ def test_a_row_of_nan_or_infinity_stays_a_row(lens, bad, e4m3):
     for n, h in ((bad[0], 3), (bad[-1], 5)):
         got[n, h], ref[n, h], tol[n, h] = 0.0, 0.0, 0.0
     check(got, ref, tol, rows)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_single_tokens_and_prompts_in_a_call_each(e4m3):
+    """One batch in two calls over parts of q_start, kv_len and page_table: each writes its
+    own sequences' rows, and both together the whole batch's."""
+    o = gp.ops()
+    n, lens = 5, [(1, 900), (1, 64), (1, 1), (0, 30), (1, 333), (60, 700), (90, 90), (0, 0)]
+    c = gp.attention_case(331, 8, 2, e4m3, lens)
+    nb = o.attention_paged_ws_bytes(c["N"], len(lens), c["max_q"], c["max_kv"], 8, 2)
+    ws = torch.empty(nb, dtype=torch.uint8, device="cuda")
+    q, gate = c["q"].cuda(), c["gate"].cuda()
+    tab, qs, kv = gp.i32(c["tab"]), gp.i32(c["qs"]), gp.i32(c["kv_len"])
+    out = torch.full((c["N"], 8 * D), 7.0, dtype=torch.bfloat16, device="cuda")
+    for seqs, starts, max_q in ((slice(0, n), slice(0, n + 1), 1),
+                                (slice(n, None), slice(n, None), c["max_q"])):
+        o.attention_paged(q, gate, 8 * D, D, c["pages"], tab[seqs], qs[starts], kv[seqs], max_q,
+                          c["max_kv"], out, ws=ws)
+        if max_q == 1:
+            torch.cuda.synchronize()
+            assert (out[c["qs"][n]:] == 7.0).all()
+    torch.cuda.synchronize()
+    got, rows = out.cpu().double().view(-1, 8, D), c["qs"][-1]
+    check(got, *oracle(c), rows)
+    assert (got[rows:] == 7.0).all()
