@@ -1498,7 +1498,7 @@ extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int
         const int rows = pg_min(max_q, N) * G;
         const bool row = pg_merge_by_row(p, rows, Hkv);
         const int groups = pg_merge_groups(p, rows, Hkv);
-        const dim3 mgrid((unsigned)((few ? p.units : p.slots) * Hkv * groups));
+        const dim3 mgrid((unsigned)(pg_merge_items(p, rows, Hkv) / 256));
         if (row)
             hipLaunchKernelGGL(merge_few_kernel<true>, mgrid, dim3(256), 0, stream, c, groups);
         else if (few)

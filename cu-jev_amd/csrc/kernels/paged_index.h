@@ -189,10 +189,20 @@ constexpr int pg_few_pieces(long long units, long long most, int goal) {
 constexpr int pg_many_goal(int Hkv) { return pg_max(256 / Hkv, 1); }
 /* Lists this long may be split among workgroups */
 constexpr bool pg_many_long(long long most) { return most > PG_MANY_LEAST + PG_MANY_MERGE; }
-/* Work-items that a launch may have, and units (and shares) times kv-heads of a call: the
- * merge of few rows has up to 4 workgroups of 256 for each */
+/* Work-items that a launch may have, and units (and shares) times kv-heads of a call */
 constexpr long long PG_MOST_ITEMS = 0xffffffffll;
-constexpr int PG_MOST_UNITS = (1 << 22) - 1;
+constexpr int PG_MOST_UNITS = 1 << 22;
+/* The merge: a workgroup a row of few rows after many keys, or a wave; 16 of many rows.
+ * Workgroups of a unit (few rows) or slot and kv-head. */
+constexpr bool pg_merge_by_row(const pg_plan &p, int rows, int Hkv) {
+    return p.rt == PG_FEW && (long long)p.units * rows * Hkv <= 512;
+}
+constexpr int pg_merge_groups(const pg_plan &p, int rows, int Hkv) {
+    return p.rt != PG_FEW ? PG_MANY / 16 : pg_merge_by_row(p, rows, Hkv) ? rows : pg_div_up(rows, 4);
+}
+constexpr long long pg_merge_items(const pg_plan &p, int rows, int Hkv) {
+    return 256ll * (p.rt == PG_FEW ? p.units : p.slots) * Hkv * pg_merge_groups(p, rows, Hkv);
+}
 
 constexpr pg_plan pg_make_plan(int N, int B, int max_q, int max_kv, int G, int Hkv, int window,
                                int sinks) {
@@ -231,16 +241,9 @@ constexpr pg_plan pg_make_plan(int N, int B, int max_q, int max_kv, int G, int H
     p.units = (int)units;
     p.shares = (int)shares;
     p.slots = (int)slots;
+    if (slots > 0 && pg_merge_items(p, (int)mq * G, Hkv) > PG_MOST_ITEMS)
+        p.shares = -1;
     return p;
-}
-
-/* The merge: a workgroup a row of few rows after many keys, or a wave; 16 of many rows.
- * Workgroups of a unit (few rows) or slot and kv-head. */
-constexpr bool pg_merge_by_row(const pg_plan &p, int rows, int Hkv) {
-    return p.rt == PG_FEW && (long long)p.units * rows * Hkv <= 512;
-}
-constexpr int pg_merge_groups(const pg_plan &p, int rows, int Hkv) {
-    return p.rt != PG_FEW ? PG_MANY / 16 : pg_merge_by_row(p, rows, Hkv) ? rows : pg_div_up(rows, 4);
 }
 
 /* ---- workspace -------------------------------------------------------------------

@@ -224,8 +224,8 @@ def test_prep_refuses_more_work_items_than_a_launch_may_have(big):
 
 
 @pytest.mark.parametrize("big", [
-    dict(N=1 << 21, B=1 << 21, max_q=1),      # 2^22 units of both kv-heads: the merge's 2^32
-    dict(N=1 << 22, B=1 << 21, max_q=2)], ids=str)
+    dict(N=1 << 23, B=1 << 21, max_q=4),  # 4 workgroups of 256 for each of 2^22 units
+    dict(N=1 << 23, B=(1 << 21) + 1, max_q=1)], ids=str)
 def test_attention_refuses_more_work_items_than_a_launch_may_have(big):
     """Before the attention itself has run, not after it."""
     st, msg = call(ATTN, **{**big, "ws": FAKE, "ws_bytes": 1 << 40})

@@ -382,12 +382,15 @@ int main() {
         const int rows = pg_min(q, N) * G;
         const int groups = pg_merge_groups(p, rows, Hkv);
         const long long merge = (long long)(p.rt == PG_FEW ? p.units : p.slots) * Hkv * groups;
-        NEED(merge * 256 <= PG_MOST_ITEMS);
+        NEED(merge * 256 <= PG_MOST_ITEMS && merge * 256 == pg_merge_items(p, rows, Hkv));
         /* each row has a place in it */
         NEED(p.rt == PG_FEW ? groups * (pg_merge_by_row(p, rows, Hkv) ? 1 : 4) >= rows : groups * 16 == 128);
         largest += merge * 256 > PG_MOST_ITEMS - (1 << 20);
     }
     NEED(largest > 0); /* calls right below the bound were among them */
+    /* as many units as there may be, where the merge has room for their rows */
+    NEED(pg_make_plan(1 << 20, 1 << 20, 1, 4096, 4, 4, 0, 0).shares > 0);
+    NEED(pg_make_plan(1 << 22, 1 << 20, 4, 4096, 4, 4, 0, 0).shares == -1);
     printf("bad %d\n", bad);
     return bad != 0;
 }
