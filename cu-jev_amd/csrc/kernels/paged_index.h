@@ -163,7 +163,8 @@ constexpr int pg_parts(const pg_seq &s, int G, int window, int longest, int shar
 /* about the tiles that its units have in all */
 constexpr unsigned pg_all_tiles(const pg_seq &s, int G, int window, int longest) {
     const int units = pg_units(s, G, PG_MANY);
-    const int last = pg_min(s.p0 + (PG_MANY - 1) / G, s.kv - 1); /* of the first unit */
+    /* last key of the first unit */
+    const int last = pg_min(pg_min(s.p0, s.kv) + (PG_MANY - 1) / G, s.kv - 1);
     const int first = window > 0 ? longest : pg_min(pg_max(last, 0) / PG + 1, longest);
     return (unsigned)units * (unsigned)(first + longest + 1) / 2;
 }
@@ -198,7 +199,9 @@ constexpr bool pg_merge_by_row(const pg_plan &p, int rows, int Hkv) {
     return p.rt == PG_FEW && (long long)p.units * rows * Hkv <= 512;
 }
 constexpr int pg_merge_groups(const pg_plan &p, int rows, int Hkv) {
-    return p.rt != PG_FEW ? PG_MANY / 16 : pg_merge_by_row(p, rows, Hkv) ? rows : pg_div_up(rows, 4);
+    if (p.rt != PG_FEW)
+        return PG_MANY / 16;
+    return pg_merge_by_row(p, rows, Hkv) ? rows : pg_div_up(rows, 4);
 }
 constexpr long long pg_merge_items(const pg_plan &p, int rows, int Hkv) {
     return 256ll * (p.rt == PG_FEW ? p.units : p.slots) * Hkv * pg_merge_groups(p, rows, Hkv);

@@ -338,6 +338,15 @@ int main() {
             const long long last = (long long)s.p0 + s.ql - 1;
             const long long want = last + 1 < 0 ? 0 : last + 1;
             NEED(s.kv == (want < mk ? want : mk));
+            /* the plan of such lengths: no sum leaves an int */
+            for (int G : {1, 4, 16}) for (int w : {0, 100}) {
+                if (s.ql == 0) continue;
+                const int n = pg_longest(s, G, PG_MANY, w, w ? 4 : 0);
+                const int units = pg_units(s, G, PG_MANY), all = (int)pg_all_tiles(s, G, w, n);
+                NEED(n >= 1 && all >= units && all <= units * n + units);
+                for (int share : {1, 8, 100, PG_MOST})
+                    NEED(pg_parts(s, G, w, n, share) >= units);
+            }
         }
     printf("bad %d\n", bad);
     return bad != 0;
