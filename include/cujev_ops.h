@@ -259,7 +259,7 @@ int cujev_op_kv_page_read(int kv_type, const void *k_pages, const void *vt_pages
  * keys that some row of the call sees have to be finite; other slots may hold
  * anything. V's magnitudes from 2^-64 to 2^80 count in full, whatever the scores;
  * of smaller ones, and of those 2^-50 of the largest beside them, the result may
- * be 0, of larger ones infinite. p is rounded to bf16 before its product with V,
+ * be 0, of larger ones infinite or NaN. p is rounded to bf16 before its product with V,
  * as in cujev_op_attention. max_q * Hq / Hkv <= 16 takes the form for few rows,
  * more the one for many, for all sequences of the call: single tokens beside a
  * prompt are faster in a call of their own, over their part of q_start, kv_len and
