@@ -100,7 +100,10 @@ template <int KIND, int TOK, bool E4M3> DEV void row_wave(const Prep &c, int hea
     for (int t = 0; t < TOK; t++)
         raw[t] = *(const bf16x4 *)(src + (size_t)min(n0 + t, N - 1) * c.ps);
     const float4 wl = *(const float4 *)(w + 4 * lane);
-    const int pos_lane = min(max(c.pos[min(n0 + (lane & (TOK - 1)), N - 1)], 0), c.npos - 1);
+    int pos_lane = min(max(c.pos[min(n0 + (lane & (TOK - 1)), N - 1)], 0), c.npos - 1);
+    /* read from all lanes below: sunk into the rotating lanes' branch it was worked out by
+     * those alone (rot 8: two, for four tokens) */
+    asm volatile("" : "+v"(pos_lane));
     /* The tokens' sequences, then (K) their slots, token t in lane t: one
      * chain of loads for all of them. at: the K row in the pool, -1: none */
     pg_seq s;
