@@ -25,26 +25,13 @@
 namespace CUJEV_KNS {
 namespace {
 
-typedef __attribute__((address_space(3))) void *lds_ptr;
 typedef __attribute__((address_space(3))) const unsigned char lds_u8;
 DEV u32x4 lds_read16(lds_u8 *base, uint32_t off) {
     return *(__attribute__((address_space(3))) const u32x4 *)(base + off);
 }
 DEV void lds_write16(unsigned char *base, uint32_t off, u32x4 v) { *(u32x4 *)(base + off) = v; }
 
-DEV __amdgpu_buffer_rsrc_t make_rsrc(const void *base, uint32_t bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, (int)bytes, 0x00020000);
-}
-DEV u32x4 buf_load16(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff) {
-    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, 0));
-}
 
-/* 8 e4m3 values (two dwords) times a power of two -> 8 bf16 */
-DEV bf16x8 widen(uint32_t a, uint32_t b, float scale) {
-    const bf16x2 p = unpack_e4m3<false>(a, scale), q = unpack_e4m3<true>(a, scale);
-    const bf16x2 r = unpack_e4m3<false>(b, scale), s = unpack_e4m3<true>(b, scale);
-    return bf16x8{p[0], p[1], q[0], q[1], r[0], r[1], s[0], s[1]};
-}
 /* x of lane i of this lane's 16 (DPP row broadcast) */
 template <int i> DEV float row_lane(float x) {
     return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(
@@ -139,6 +126,11 @@ struct Call {
      * all the same. */
     int list_window, list_sinks;
     int rG; /* r / G = r * rG >> 16 for r < 4096 (an integer division is 30 instructions) */
+    /* LSE and TREE calls: [N][words], bit j of row n: it sees its sequence's new token j;
+     * log2 of sum 2^(q.k), [N][Hq], -inf where there is none (NULL: not asked for) */
+    const uint64_t *tree;
+    int words;
+    float *lse;
     bf16 *out;
     float *po, *pl, *pmu;
     /* for the merge: few rows {first piece, parts} of each sequence, many rows
@@ -154,12 +146,41 @@ DEV int page_id(const Call &c, int b, const pg_tiles &t, int i) {
     return page >= 0 && page < c.num_pages ? page : -1;
 }
 
-/* The lane's number, worked out where it stands: kept, it may go to scratch memory */
-DEV int lane_again() {
-    int none = 0;
-    asm volatile("" : "+v"(none));
-    return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none));
+/* What a call asks for: causal rows; the same with lse; rows of a tree of drafted tokens.
+ * Kinds of their own, so that the first one's code stays what it is. */
+enum { CAUSAL, LSE, TREE };
+/* TREE: the keys k0 .. k0 + 63 that the row with these words sees by its tree, first key
+ * lowest: all before the sequence's first new token (at p0), then as the bits say */
+DEV uint64_t tree_keys(const uint64_t *row, int words, int k0, int p0) {
+    const int at = k0 - p0, i = at >> 6, sh = at & 63; /* i -1: the tile that p0 is in */
+    const uint64_t lo = i < 0 ? ~0ull : i < words ? row[i] : 0;
+    const uint64_t hi = i < -1 ? ~0ull : i + 1 < words ? row[i + 1] : 0;
+    return sh ? lo >> sh | hi << (64 - sh) : lo;
 }
+template <class F> DEV uint64_t each_half(uint64_t x, F f) {
+    return (uint64_t)f((uint32_t)(x >> 32)) << 32 | f((uint32_t)x);
+}
+/* or over the lanes of each row of 16; over the wave */
+template <int ctrl> DEV uint32_t or_dpp(uint32_t v) {
+    return v | (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xf, 0xf, true);
+}
+DEV uint32_t or_row(uint32_t v) { /* row_ror 8, 4, 2, 1 */
+    return or_dpp<0x121>(or_dpp<0x122>(or_dpp<0x124>(or_dpp<0x128>(v))));
+}
+DEV uint64_t or_row(uint64_t x) {
+    return each_half(x, [](uint32_t v) { return or_row(v); });
+}
+DEV uint64_t or_wave(uint64_t x) {
+    return or_row(each_half(x, [](uint32_t v) {
+        auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        const uint32_t u = a[0] | a[1];
+        a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        return (uint32_t)(a[0] | a[1]);
+    }));
+}
+/* log2 of l 2^mu; -inf for a row that has seen no key */
+DEV float lse_of(float l, float mu) { return l > 0.f ? mu + __builtin_amdgcn_logf(l) : -INFINITY; }
+
 /* The unit that share `target` of a kv-head belongs to (few rows: the one that piece
  * `target` begins in): its sequence (b -1: there is none), its number in it, its parts,
  * the first one's number (few rows: its piece's), which of them `target` is. */
@@ -331,7 +352,7 @@ DEV size_t slot_of(const Call &c, int kh, int at) { return (size_t)kh * c.plan.s
  * lengths, page ids, K, gates. */
 constexpr int FEW = PG_FEW;
 
-template <bool E4M3>
+template <bool E4M3, int KIND>
 __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
     constexpr uint32_t EB = E4M3 ? 1 : 2, SLICE = PSLICE * EB;
     __shared__ bf16x8 sq[8 * 64];
@@ -351,7 +372,8 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
 
         /* this lane's row (column of S^T and O^T) */
         const int row = min(m, rows - 1), tok = row * c.rG >> 16, head = kh * c.G + row - tok * c.G;
-        const int hi = min(s.p0 + tok, s.kv - 1), lo = pg_low(s.p0 + tok, c.window);
+        const int hi = KIND == TREE ? s.kv - 1 : min(s.p0 + tok, s.kv - 1);
+        const int lo = pg_low(s.p0 + tok, c.window);
         const int own_lo = pg_low(s.p0, c.window); /* of the first row: below, no row's key */
         bf16x8 *const qf = sq + lane;
         {
@@ -470,13 +492,35 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
              * are, meet p = 0 */
             u32x4 keep[E4M3 ? 1 : 2];
             bool foreign = false;
-            if (!there || !pg_tile_whole(k0, s.p0, s.p0 + s.ql - 1, s.kv, c.window, c.sinks)) {
+            uint32_t tbits = 0;
+            if (!there || !pg_tile_whole(k0, s.p0 - (KIND == TREE), s.p0 + s.ql - 1, s.kv, c.window,
+                                         c.sinks)) {
                 const int top = there ? s.kv - 1 : -1;
+                if constexpr (KIND == TREE) {
+                    /* bit v of the low half: this lane's row sees key key_of(v); of the
+                     * high half: some row does. Lane and row are worked out again: kept,
+                     * they went to scratch memory. */
+                    const int id = lane_again(), of = min(id & 15, rows - 1) * c.rG >> 16;
+                    uint64_t m64 =
+                        tree_keys(c.tree + (size_t)(s.q0 + of) * c.words, c.words, k0, s.p0);
+                    const int left = top + 1 - k0; /* keys of the tile, 64 at most count */
+                    m64 &= left >= PG ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
+                    m64 >>= (E4M3 ? 16 : 8) * (id >> 4);
+                    tbits = E4M3 ? (uint32_t)m64 & 0xffffu
+                                 : ((uint32_t)m64 & 0xffu) | ((uint32_t)(m64 >> 32) & 0xffu) << 8;
+                    tbits |= (uint32_t)or_row(tbits) << 16;
+                    unroll_for<16>([&](auto iv) {
+                        constexpr int v = decltype(iv)::value;
+                        x[v >> 2][v & 3] = hide_by<v>(tbits, x[v >> 2][v & 3]);
+                    });
+                } else {
 #pragma unroll
-                for (int v = 0; v < 16; v++)
-                    x[v >> 2][v & 3] =
-                        hide(key_seen(k0 + key_of(v), min(hi, top), lo, c.sinks), x[v >> 2][v & 3]);
-                foreign = !there || pg_tile_foreign(k0, s.p0, s.kv, c.window, c.sinks);
+                    for (int v = 0; v < 16; v++)
+                        x[v >> 2][v & 3] = hide(
+                            key_seen(k0 + key_of(v), min(hi, top), lo, c.sinks), x[v >> 2][v & 3]);
+                }
+                foreign = KIND == TREE || !there ||
+                          pg_tile_foreign(k0, s.p0, s.kv, c.window, c.sinks);
                 if (foreign) {
 #pragma unroll
                     for (int h = 0; h < (E4M3 ? 1 : 2); h++)
@@ -485,15 +529,21 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
                             uint32_t k = 0;
 #pragma unroll
                             for (int e = 0; e < (E4M3 ? 4 : 2); e++) {
-                                const int j = k0 + key_of(E4M3 ? 4 * d + e : 8 * h + 2 * d + e);
-                                k |= key_seen(j, top, own_lo, c.sinks)
+                                const int v = E4M3 ? 4 * d + e : 8 * h + 2 * d + e;
+                                const bool some =
+                                    KIND == TREE ? tbits >> (16 + v) & 1
+                                                 : key_seen(k0 + key_of(v), top, own_lo, c.sinks);
+                                k |= some
                                          ? (E4M3 ? 0xffu << (8 * e) : 0xffffu << (16 * e))
                                          : 0u;
                             }
                             keep[h][d] = k;
                         }
                     vsc = __uint_as_float(
-                        key_seen(k0 + keyg + m, top, own_lo, c.sinks) ? __float_as_uint(vsc) : 0u);
+                        (KIND == TREE ? tbits >> (16 + (lane_again() & 15)) & 1
+                                      : key_seen(k0 + keyg + m, top, own_lo, c.sinks))
+                            ? __float_as_uint(vsc)
+                            : 0u);
                 }
             }
             float mx = -INFINITY;
@@ -573,6 +623,10 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
         } else if (r < rows) {
             const float inv = lrun > 0.f ? 1.f / lrun : 0.f;
             const int tk = r * c.rG >> 16, n = s.q0 + tk, hd = kh * c.G + r - tk * c.G;
+            if constexpr (KIND != CAUSAL) {
+                if (c.lse && d0 == 0)
+                    c.lse[(size_t)n * c.Hq + hd] = lse_of(lrun, mrun);
+            }
             bf16x4 gv[16] = {};
             if (c.gate) {
                 const bf16 *gp = c.gate + (size_t)n * c.gts + (size_t)hd * c.ghs + d0;
@@ -679,7 +733,7 @@ template <bool E4M3> DEV int perm_row(int m) {
 /* A workgroup's share, with a reference of 0 within the range; true: once more with none.
  * The second time is the first one's code again, and nothing but the range may be kept
  * for it: all of the 128 + 128 registers are taken. */
-template <bool E4M3> DEV bool attend_many(const Call &c, unsigned char *smem, const float range) {
+template <bool E4M3, int KIND> DEV bool attend_many(const Call &c, unsigned char *smem, const float range) {
     typedef Lay<E4M3> L;
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid)); /* unknown: what goes by it is worked out each time */
@@ -707,7 +761,8 @@ template <bool E4M3> DEV bool attend_many(const Call &c, unsigned char *smem, co
     const int b = w.b, nshare = w.parts, share = w.part;
     const int r0 = w.unit * RT, nrows = min(s.ql * c.G - r0, RT);
     const int i0 = r0 / c.G, rest = r0 - i0 * c.G, i1 = i0 + ((rest + nrows - 1) * c.rG >> 16);
-    const pg_tiles list = pg_tile_list(s, i0, i1, c.list_window, c.list_sinks);
+    const pg_tiles list =
+        pg_tile_list(s, i0, KIND == TREE ? s.ql - 1 : i1, c.list_window, c.list_sinks);
     const int tb = pg_share_begin(list.ntl, share, nshare);
     const int ntl = pg_share_begin(list.ntl, share + 1, nshare) - tb;
     const size_t slot = slot_of(c, kh, w.first + share);
@@ -724,10 +779,19 @@ template <bool E4M3> DEV bool attend_many(const Call &c, unsigned char *smem, co
     int hi, lo; /* of this lane's row; rows past the last repeat it */
     {
         const int tok = i0 + ((rest + min(32 * wi + col, nrows - 1)) * c.rG >> 16);
-        hi = min(s.p0 + tok, s.kv - 1);
+        hi = KIND == TREE ? s.kv - 1 : min(s.p0 + tok, s.kv - 1);
         lo = pg_low(s.p0 + tok, c.window);
     }
-    const int pmin = s.p0 + i0, pmax = s.p0 + i1;
+    /* TREE: all rows see the keys up to pmin, no other order of theirs is known */
+    const int pmin = KIND == TREE ? s.p0 - 1 : s.p0 + i0, pmax = s.p0 + i1;
+    /* of keys k0 .. k0 + 63, those that the row of token i sees, and that any row does */
+    auto seen_by = [&](int k0, int i) {
+        return tree_keys(c.tree + (size_t)(s.q0 + i) * c.words, c.words, k0, s.p0);
+    };
+    auto seen_by_any = [&](int k0) { /* tokens i0 .. i1, up to 128 */
+        const int n = lane_again();
+        return or_wave(seen_by(k0, min(i0 + n, i1)) | seen_by(k0, min(i0 + 64 + n, i1)));
+    };
 
     /* ---- tile loads: memory -> LDS (buffer_load ... lds: lane l's 16 bytes land
      * at base + 16 l, so the swizzle is applied to the address). Load n of a wave is
@@ -860,16 +924,21 @@ template <bool E4M3> DEV bool attend_many(const Call &c, unsigned char *smem, co
             return;
         const int kb = k0 + 32 * wj + (E4M3 ? 16 : 8) * h;
         const int top = there ? s.kv - 1 : -1;
-        const uint32_t bits = keys_seen<E4M3 ? 16 : 24>(kb, min(hi, top), lo, c.sinks);
+        uint32_t bits = keys_seen<E4M3 ? 16 : 24>(kb, min(hi, top), lo, c.sinks);
+        if constexpr (KIND == TREE)
+            bits &= (uint32_t)(seen_by(k0, i0 + ((rest + min(32 * wi + col, nrows - 1)) * c.rG >>
+                                                 16)) >>
+                               (kb - k0));
         unroll_for<16>([&](auto iv) {
             constexpr int r = decltype(iv)::value;
             x[r] = hide_by<E4M3 ? r : 16 * (r >> 3) + (r & 7)>(bits, x[r]);
         });
-        if constexpr (E4M3) /* a scale of no key of this call: any bits */
-            vsc = __uint_as_float(
-                key_seen(kb + (lane & 15), top, pg_low(pmin, c.window), c.sinks)
-                    ? __float_as_uint(vsc)
-                    : 0u);
+        if constexpr (E4M3) { /* a scale of no key of this call: any bits */
+            bool some = key_seen(kb + (lane & 15), top, pg_low(pmin, c.window), c.sinks);
+            if constexpr (KIND == TREE)
+                some &= seen_by_any(k0) >> (kb - k0 + (lane & 15)) & 1;
+            vsc = __uint_as_float(some ? __float_as_uint(vsc) : 0u);
+        }
     };
     /* p of accumulators v, v + 1 into operand f */
     auto pair = [&](const floatx16 &x, bf16x8 &f, auto iv, float shift) {
@@ -961,8 +1030,12 @@ template <bool E4M3> DEV bool attend_many(const Call &c, unsigned char *smem, co
         asm volatile("" ::: "memory");
 
         const int k0 = pg_tile_page(list, tb + i) * PG;
-        if (!there || pg_tile_foreign(k0, pmin, s.kv, c.window, c.sinks)) {
+        if (!there || pg_tile_foreign(k0, pmin, s.kv, c.window, c.sinks) ||
+            (KIND == TREE && k0 + PG > s.p0)) {
             /* values of no key of these rows meet p = 0: make them 0 */
+            uint64_t any = ~0ull;
+            if constexpr (KIND == TREE)
+                any = seen_by_any(k0);
 #pragma unroll 1
             for (int n = 0; n < L::T / 8192; n++) {
                 const int at = (n * 512 + tid) * 16, d = at / (L::T / PD);
@@ -970,7 +1043,8 @@ template <bool E4M3> DEV bool attend_many(const Call &c, unsigned char *smem, co
                 u32x4 w = lds_read16(lds, L::V + PAR * L::T + at);
                 const uint32_t bits =
                     there ? keys_seen<E4M3 ? 16 : 8>(k0 + (E4M3 ? 16 : 8) * piece, s.kv - 1,
-                                                     pg_low(pmin, c.window), c.sinks)
+                                                     pg_low(pmin, c.window), c.sinks) &
+                                (uint32_t)(any >> ((E4M3 ? 16 : 8) * piece))
                           : 0u;
                 unroll_for<4>([&](auto ie) {
                     constexpr int e = decltype(ie)::value;
@@ -1224,6 +1298,13 @@ template <bool E4M3> DEV bool attend_many(const Call &c, unsigned char *smem, co
         lost = (large && most > __float_as_uint(LOST_HIGH)) ||
                (small && most < __float_as_uint(LOST_LOW));
     }
+    if constexpr (KIND != CAUSAL) {
+        if (whole && c.lse && wj == 0 && h == 0 && 32 * wi + col < nrows) {
+            const int r = rest + 32 * wi + col, after = r * c.rG >> 16;
+            c.lse[(size_t)(s.q0 + i0 + after) * c.Hq + kh * c.G + r - after * c.G] =
+                lse_of(l, mus);
+        }
+    }
     int *again = (int *)(smem + L::AGAIN);
     const int any_lost = __any(lost);
     if (lane == 0)
@@ -1274,7 +1355,7 @@ template <bool E4M3> DEV bool attend_many(const Call &c, unsigned char *smem, co
     }
     return false;
 }
-template <bool E4M3>
+template <bool E4M3, int KIND>
 __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
     __shared__ __attribute__((aligned(1024))) unsigned char smem[Lay<E4M3>::BYTES];
     /* c by an address that is unknown each time: known, the arguments were kept for the
@@ -1286,7 +1367,7 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
     for (;;) {
         asm volatile("" : "+s"(args));
         const Call a = *(const Call *)args;
-        if (!attend_many<E4M3>(a, smem, range))
+        if (!attend_many<E4M3, KIND>(a, smem, range))
             break;
         range = 0.f;
     }
@@ -1301,7 +1382,8 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
  * dims, o 64 parts at a time, 4 a load. That is for few rows after many keys (4 rows
  * of 64 parts: 5.4 us, and 8.8 a wave per row); the starts of many workgroups cost
  * more than it gains (1024 rows of 4 parts: 5.6 and 4.8, 4096 of them 22 and 8). */
-template <bool ROW> __global__ __launch_bounds__(256) void merge_few_kernel(Call c, int groups) {
+template <bool ROW, bool STATS>
+__global__ __launch_bounds__(256) void merge_few_kernel(Call c, int groups) {
     constexpr int STEP = ROW ? 64 : 16, PER = STEP / 16;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int group = blockIdx.x % groups, kh = blockIdx.x / groups % c.Hkv;
@@ -1366,12 +1448,14 @@ template <bool ROW> __global__ __launch_bounds__(256) void merge_few_kernel(Call
         res[e] = f2bf(acc[e] * inv * (c.gate ? sigmoid_f(bf2f(gv[e])) : 1.f));
     if (!ROW || lane < 16)
         *(bf16x4 *)(c.out + ((size_t)n * c.Hq + head) * PD + dim) = res;
+    if (STATS && c.lse && dim == 0 && (!ROW || lane < 16))
+        c.lse[(size_t)n * c.Hq + head] = lse_of(l, mu);
 }
 
 /* Of many rows: a wave 4 rows, all at once (one after the other took 11.2 us instead
  * of 9.6 for 16 sequences' 40 tokens in 2 or 3 parts). l and mu: lane 16 i + j has row
  * i's of part j, 16 parts in turn; o 4 parts at a time. */
-__global__ __launch_bounds__(256) void merge_many_kernel(Call c) {
+template <bool STATS> __global__ __launch_bounds__(256) void merge_many_kernel(Call c) {
     constexpr int R = 4, GROUPS = RT / (4 * R);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int group = blockIdx.x % GROUPS, kh = blockIdx.x / GROUPS % c.Hkv;
@@ -1447,6 +1531,8 @@ __global__ __launch_bounds__(256) void merge_many_kernel(Call c) {
             res[e] = f2bf(acc[i][e] * inv * (c.gate ? sigmoid_f(bf2f(gv[i][e])) : 1.f));
         if (t0 + i <= last)
             *(bf16x4 *)out[i] = res;
+        if (STATS && c.lse && lane == 0 && t0 + i <= last)
+            c.lse[(size_t)(out[i] - c.out) / PD] = lse_of(li, of(mu, 16 * i));
     }
 }
 
@@ -1463,7 +1549,8 @@ extern "C" size_t cujev_attention_paged_ws_bytes(int N, int B, int max_q, int ma
 extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int gate_tok_stride,
                                         int gate_head_stride, const cujev_kv_pages *pages,
                                         const cujev_paged_seqs *seqs, int N, int max_q, int max_kv,
-                                        int Hq, int window, int sinks, bf16_t *out, void *ws,
+                                        int Hq, int window, int sinks, const uint64_t *tree,
+                                        int tree_words, bf16_t *out, float *lse, void *ws,
                                         size_t ws_bytes, hipStream_t stream) {
     const int Hkv = pages->Hkv, B = seqs->B, G = Hq / Hkv;
     const bool e4m3 = pages->type == CUJEV_KV_E4M3;
@@ -1480,31 +1567,52 @@ extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int
                     pages->k, pages->vt, pages->k_scale, pages->v_scale, pages->num_pages,
                     seqs->q_start, seqs->kv_len, seqs->page_table, seqs->max_pages, B, N,
                     max_q, max_kv, Hq, Hkv, G, window, sinks,
-                    all ? 0 : window, all ? 0 : sinks, pg_div_up(65536, G), (bf16 *)out,
-                    (float *)ws, (float *)ws + rows * PD, (float *)ws + rows * (PD + 1),
-                    (int32_t *)((float *)ws + rows * (PD + 2)), p};
+                    all ? 0 : window, all ? 0 : sinks, pg_div_up(65536, G), tree, tree_words, lse,
+                    (bf16 *)out, (float *)ws, (float *)ws + rows * PD,
+                    (float *)ws + rows * (PD + 1), (int32_t *)((float *)ws + rows * (PD + 2)), p};
     const bool few = p.rt == FEW;
     const int per = !few && 8 % Hkv == 0 ? 8 / Hkv : 1;
     const dim3 grid((unsigned)(pg_div_up(p.shares, per) * per * Hkv)); /* all parts */
-    if (few && e4m3)
-        hipLaunchKernelGGL(attention_few_kernel<true>, grid, dim3(64), 0, stream, c);
-    else if (few)
-        hipLaunchKernelGGL(attention_few_kernel<false>, grid, dim3(64), 0, stream, c);
-    else if (e4m3)
-        hipLaunchKernelGGL(attention_many_kernel<true>, grid, dim3(512), 0, stream, c);
+    auto launch = [&](auto ie, auto ik) {
+        constexpr bool E = decltype(ie)::value;
+        constexpr int KIND = decltype(ik)::value;
+        if (few)
+            hipLaunchKernelGGL((attention_few_kernel<E, KIND>), grid, dim3(64), 0, stream, c);
+        else
+            hipLaunchKernelGGL((attention_many_kernel<E, KIND>), grid, dim3(512), 0, stream, c);
+    };
+    auto by_kind = [&](auto ie) {
+        if (tree)
+            launch(ie, template_int<TREE>{});
+        else if (lse)
+            launch(ie, template_int<LSE>{});
+        else
+            launch(ie, template_int<CAUSAL>{});
+    };
+    if (e4m3)
+        by_kind(std::true_type{});
     else
-        hipLaunchKernelGGL(attention_many_kernel<false>, grid, dim3(512), 0, stream, c);
+        by_kind(std::false_type{});
     if (p.slots > 0) {
         const int rows = pg_min(max_q, N) * G;
         const bool row = pg_merge_by_row(p, rows, Hkv);
         const int groups = pg_merge_groups(p, rows, Hkv);
         const dim3 mgrid((unsigned)(pg_merge_items(p, rows, Hkv) / 256));
-        if (row)
-            hipLaunchKernelGGL(merge_few_kernel<true>, mgrid, dim3(256), 0, stream, c, groups);
-        else if (few)
-            hipLaunchKernelGGL(merge_few_kernel<false>, mgrid, dim3(256), 0, stream, c, groups);
+        auto merge = [&](auto stats) {
+            constexpr bool S = decltype(stats)::value;
+            if (row)
+                hipLaunchKernelGGL((merge_few_kernel<true, S>), mgrid, dim3(256), 0, stream, c,
+                                   groups);
+            else if (few)
+                hipLaunchKernelGGL((merge_few_kernel<false, S>), mgrid, dim3(256), 0, stream, c,
+                                   groups);
+            else
+                hipLaunchKernelGGL((merge_many_kernel<S>), mgrid, dim3(256), 0, stream, c);
+        };
+        if (lse)
+            merge(std::true_type{});
         else
-            hipLaunchKernelGGL(merge_many_kernel, mgrid, dim3(256), 0, stream, c);
+            merge(std::false_type{});
     }
     return hipGetLastError();
 }

@@ -270,12 +270,13 @@ typedef struct cujev_paged_seqs {
 /* Whether the pool's pointers, alignment and type are usable. */
 int cujev_kv_pages_ok(const cujev_kv_pages *pages);
 
-/* k_attn_prep with K and V written into pages: rows, norms, RoPE (pos[n], cut
- * to the table's npos positions) and q_out as there, for any Hq / Hkv; rot 8,
- * 16, 32 or 64. Rows of no sequence are left alone. */
+/* k_attn_prep with K and V written into pages: rows, norms, RoPE and q_out as
+ * there, for any Hq / Hkv; rot 8, 16, 32 or 64. Positions have 1 to 4 axes: frequency
+ * i turns by pos[a * N + n] (cut to the table's npos positions), a = axis_of >> 2 i & 3
+ * (below axes). Rows of no sequence are left alone. */
 hipError_t k_attn_prep_paged(const bf16_t *proj, int proj_stride, const float *q_norm_w,
-                             const float *k_norm_w, const int32_t *pos,
-                             const cujev_paged_seqs *seqs, int N, int Hq, int rot,
+                             const float *k_norm_w, const int32_t *pos, int axes,
+                             uint64_t axis_of, const cujev_paged_seqs *seqs, int N, int Hq, int rot,
                              const float *rope_table, int npos, float eps, float q_scale,
                              bf16_t *q_out, const cujev_kv_pages *pages, hipStream_t stream);
 /* Columns [0, min(kv_len[b], max_kv)) of the caches k_cache [B][Hkv][stride][256]
@@ -288,16 +289,42 @@ hipError_t k_kv_page_read(const cujev_kv_pages *pages, const cujev_paged_seqs *s
  * sees keys j <= p with window == 0 or j > p - window or j < sinks;
  *   out[n, h*256 + d] = sigmoid(gate) * softmax2_j(q[n, h] . k_j) v_j
  * (gate NULL: no gate; no key: 0), q bf16 [N][Hq][256] scaled as for
- * k_attention. max_q and max_kv bound ql and kv_len. */
+ * k_attention. max_q and max_kv bound ql and kv_len. With tree (window 0) [N]
+ * [tree_words], row i of a sequence sees all keys before the new tokens and new token
+ * j where bit j % 64 of word j / 64 is set. lse [N][Hq], if not NULL: log2 of the
+ * sum over seen keys of 2^(q . k), -inf of none. */
 hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int gate_tok_stride,
                              int gate_head_stride, const cujev_kv_pages *pages,
                              const cujev_paged_seqs *seqs, int N, int max_q, int max_kv, int Hq,
-                             int window, int sinks, bf16_t *out, void *ws, size_t ws_bytes,
+                             int window, int sinks, const uint64_t *tree, int tree_words,
+                             bf16_t *out, float *lse, void *ws, size_t ws_bytes,
                              hipStream_t stream);
 /* Enough for that call and every one of the same heads that is no larger in N, B, max_q
  * and max_kv, of either type and any window. */
 size_t cujev_attention_paged_ws_bytes(int N, int B, int max_q, int max_kv, int Hq, int Hkv,
                                       int window, int sinks, int type);
+
+/* ---- eviction from the paged cache (evict.hip) --------------------------------
+ * weights[page][kv-head][slot] fp32, beside the pages. For each sequence with new
+ * tokens and each of its keys j: the sum over its rows n and the kv-head's q-heads h
+ * that see j (j <= the row's position) of 2^(q[n, h] . k_j - lse[n, h]), plus prev's
+ * value where prev is not NULL (it may be weights) and j is before the new tokens. */
+hipError_t k_kv_weights(const bf16_t *q, const float *lse, const cujev_kv_pages *pages,
+                        const cujev_paged_seqs *seqs, int N, int max_q, int max_kv, int Hq,
+                        const float *prev, float *weights, hipStream_t stream);
+/* keep[b][kv-head][0 .. n - 1], n = keep_len[b] = min(kv_len[b], budget): ascending, the
+ * positions of the first `sinks`, the last `recent` and the heaviest of the other keys
+ * (equal ones: the lowest; NaN the heaviest; of pages that are not there the lightest). */
+hipError_t k_kv_select(const float *weights, int num_pages, int Hkv, const cujev_paged_seqs *seqs,
+                       int max_kv, int budget, int sinks, int recent, int32_t *keep, int max_keep,
+                       int32_t *keep_len, hipStream_t stream);
+/* Position dst[b] + i (dst NULL: i), of to_table [B][to_pages] (NULL: in place), takes what
+ * position keep[b][kv-head or 0][i] has, i < keep_len[b]: K, V, scales and weights (NULL:
+ * none). In place keep ascends, no entry before the position that it goes to. */
+hipError_t k_kv_keep(const cujev_kv_pages *pages, float *weights, const cujev_paged_seqs *seqs,
+                     const int32_t *to_table, int to_pages, const int32_t *keep, int keep_heads,
+                     int max_keep, const int32_t *dst, const int32_t *keep_len,
+                     hipStream_t stream);
 
 /* ---- per-layer glue --------------------------------------------------------
  * x[N,H] fp32 residual = E[tokens] (bf16 table).  REF elementwise.cu:3-11. */

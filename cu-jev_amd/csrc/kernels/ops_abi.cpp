@@ -319,6 +319,44 @@ static int paged_heads_ok(int Hq, int Hkv) {
     return Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Hq / Hkv <= 16 && Hq <= 8192;
 }
 
+static int prep_paged(const char *what, const void *proj, int proj_stride, const float *q_norm_w,
+                                    const float *k_norm_w, const int32_t *pos, int axes, uint64_t axis_of,
+                                    const int32_t *q_start, const int32_t *kv_len,
+                                    const int32_t *page_table, int max_pages, int B, int N, int Hq,
+                                    int Hkv, int rot, const float *rope_table, int npos, float eps,
+                                    float q_scale, void *q_out, int kv_type, void *k_pages,
+                                    void *vt_pages, float *k_scale, float *v_scale, int num_pages,
+                                    void *stream) {
+    const cujev_kv_pages pages = {k_pages, vt_pages, k_scale, v_scale, num_pages, Hkv, kv_type};
+    const int st = paged_check(what, &pages, page_table, max_pages, kv_len, B);
+    if (st != 0)
+        return st;
+    if (N < 0 || N > PG_MOST || !paged_heads_ok(Hq, Hkv) ||
+        (rot != 8 && rot != 16 && rot != 32 && rot != 64) || npos <= 0)
+        return fail(1, "%s: unsupported shape N=%d Hq=%d Hkv=%d rot=%d npos=%d",
+                    what, N, Hq, Hkv, rot, npos);
+    if (axes < 1 || axes > 4)
+        return fail(1, "%s: positions have 1 to 4 axes, not %d", what, axes);
+    for (int i = 0; i < rot / 2; i++)
+        if ((int)(axis_of >> (2 * i) & 3) >= axes)
+            return fail(1, "%s: frequency %d turns by axis %d of %d", what, i,
+                        (int)(axis_of >> (2 * i) & 3), axes);
+    if (N > 0 && B > 0 &&
+        (!proj || !q_norm_w || !k_norm_w || !pos || !q_start || !rope_table || !q_out))
+        return fail(1, "%s: null argument", what);
+    if (proj_stride < Hq * 512 + Hkv * 512 || proj_stride % 4 || ((uintptr_t)proj & 7) ||
+        ((uintptr_t)q_out & 7))
+        return fail(1, "%s: rows must be 8-byte aligned and hold %d values", what,
+                    Hq * 512 + Hkv * 512);
+    if (((uintptr_t)q_norm_w | (uintptr_t)k_norm_w | (uintptr_t)rope_table) & 15)
+        return fail(1, "%s: weights and RoPE table must be 16-byte aligned", what);
+    const cujev_paged_seqs seqs = {q_start, kv_len, page_table, max_pages, B};
+    return launched(k_attn_prep_paged((const bf16_t *)proj, proj_stride, q_norm_w, k_norm_w, pos, axes,
+                                      axis_of, &seqs, N, Hq, rot, rope_table, npos, eps, q_scale,
+                                      (bf16_t *)q_out, &pages, (hipStream_t)stream),
+                    what);
+}
+
 EXPORT int cujev_op_attn_prep_paged(const void *proj, int proj_stride, const float *q_norm_w,
                                     const float *k_norm_w, const int32_t *pos,
                                     const int32_t *q_start, const int32_t *kv_len,
@@ -327,28 +365,24 @@ EXPORT int cujev_op_attn_prep_paged(const void *proj, int proj_stride, const flo
                                     float q_scale, void *q_out, int kv_type, void *k_pages,
                                     void *vt_pages, float *k_scale, float *v_scale, int num_pages,
                                     void *stream) {
-    const cujev_kv_pages pages = {k_pages, vt_pages, k_scale, v_scale, num_pages, Hkv, kv_type};
-    const int st = paged_check("attn_prep_paged", &pages, page_table, max_pages, kv_len, B);
-    if (st != 0)
-        return st;
-    if (N < 0 || N > PG_MOST || !paged_heads_ok(Hq, Hkv) ||
-        (rot != 8 && rot != 16 && rot != 32 && rot != 64) || npos <= 0)
-        return fail(1, "attn_prep_paged: unsupported shape N=%d Hq=%d Hkv=%d rot=%d npos=%d", N,
-                    Hq, Hkv, rot, npos);
-    if (N > 0 && B > 0 &&
-        (!proj || !q_norm_w || !k_norm_w || !pos || !q_start || !rope_table || !q_out))
-        return fail(1, "attn_prep_paged: null argument");
-    if (proj_stride < Hq * 512 + Hkv * 512 || proj_stride % 4 || ((uintptr_t)proj & 7) ||
-        ((uintptr_t)q_out & 7))
-        return fail(1, "attn_prep_paged: rows must be 8-byte aligned and hold %d values",
-                    Hq * 512 + Hkv * 512);
-    if (((uintptr_t)q_norm_w | (uintptr_t)k_norm_w | (uintptr_t)rope_table) & 15)
-        return fail(1, "attn_prep_paged: weights and RoPE table must be 16-byte aligned");
-    const cujev_paged_seqs seqs = {q_start, kv_len, page_table, max_pages, B};
-    return launched(k_attn_prep_paged((const bf16_t *)proj, proj_stride, q_norm_w, k_norm_w, pos,
-                                      &seqs, N, Hq, rot, rope_table, npos, eps, q_scale,
-                                      (bf16_t *)q_out, &pages, (hipStream_t)stream),
-                    "attn_prep_paged");
+    return prep_paged("attn_prep_paged", proj, proj_stride, q_norm_w, k_norm_w, pos, 1, 0, q_start,
+                      kv_len, page_table, max_pages, B, N, Hq, Hkv, rot, rope_table, npos, eps,
+                      q_scale, q_out, kv_type, k_pages, vt_pages, k_scale, v_scale, num_pages,
+                      stream);
+}
+
+EXPORT int cujev_op_attn_prep_paged_axes(const void *proj, int proj_stride, const float *q_norm_w,
+                                    const float *k_norm_w, const int32_t *pos, int axes, uint64_t axis_of,
+                                    const int32_t *q_start, const int32_t *kv_len,
+                                    const int32_t *page_table, int max_pages, int B, int N, int Hq,
+                                    int Hkv, int rot, const float *rope_table, int npos, float eps,
+                                    float q_scale, void *q_out, int kv_type, void *k_pages,
+                                    void *vt_pages, float *k_scale, float *v_scale, int num_pages,
+                                    void *stream) {
+    return prep_paged("attn_prep_paged_axes", proj, proj_stride, q_norm_w, k_norm_w, pos, axes, axis_of, q_start,
+                      kv_len, page_table, max_pages, B, N, Hq, Hkv, rot, rope_table, npos, eps,
+                      q_scale, q_out, kv_type, k_pages, vt_pages, k_scale, v_scale, num_pages,
+                      stream);
 }
 
 EXPORT int cujev_op_kv_page_read(int kv_type, const void *k_pages, const void *vt_pages,
@@ -375,6 +409,54 @@ EXPORT int cujev_op_kv_page_read(int kv_type, const void *k_pages, const void *v
                     "kv_page_read");
 }
 
+static int attend_paged(const char *what, const void *q, const void *gate, int gate_tok_stride,
+                                    int gate_head_stride, int kv_type, const void *k_pages,
+                                    const void *vt_pages, const float *k_scale,
+                                    const float *v_scale, int num_pages, const int32_t *q_start,
+                                    const int32_t *kv_len, const int32_t *page_table,
+                                    int max_pages, int B, int N, int max_q, int max_kv, int Hq,
+                                    int Hkv, int window, int sinks, const void *tree,
+                                    int tree_words, void *out, float *lse, void *ws,
+                                    size_t ws_bytes, void *stream) {
+    const cujev_kv_pages pages = {(void *)k_pages, (void *)vt_pages, (float *)k_scale,
+                                  (float *)v_scale, num_pages, Hkv, kv_type};
+    const int st = paged_check(what, &pages, page_table, max_pages, kv_len, B);
+    if (st != 0)
+        return st;
+    if (N < 0 || N > PG_MOST || max_q < 0 || max_kv < 0 || !paged_heads_ok(Hq, Hkv))
+        return fail(1, "%s: unsupported shape N=%d max_q=%d max_kv=%d Hq=%d Hkv=%d",
+                    what, N, max_q, max_kv, Hq, Hkv);
+    if (max_kv > max_pages * CUJEV_KV_PAGE)
+        return fail(1, "%s: max_kv=%d is not within the table's %d tokens", what, max_kv,
+                    max_pages * CUJEV_KV_PAGE);
+    if (window < 0 || sinks < 0 || (sinks > 0 && window == 0))
+        return fail(1, "%s: window=%d sinks=%d (sinks go with a window)", what, window,
+                    sinks);
+    if (N > 0 && B > 0 && (!q || !q_start || !out))
+        return fail(1, "%s: null argument", what);
+    if ((((uintptr_t)q | (uintptr_t)out) & 15) || ((uintptr_t)gate & 7) ||
+        (gate && (gate_tok_stride % 4 || gate_head_stride % 4)))
+        return fail(1, "%s: q and out must be 16-byte, gate rows 8-byte aligned", what);
+    if (((uintptr_t)tree & 7) || ((uintptr_t)lse & 3))
+        return fail(1, "%s: tree must be 8-byte, lse 4-byte aligned", what);
+    if (tree && (window || tree_words <= 0 || tree_words < pg_div_up(pg_min(max_q, N), 64)))
+        return fail(1, "%s: a tree of up to %d new tokens a sequence needs %d words a row and no "
+                       "window, got %d and window=%d",
+                    what, pg_min(max_q, N), pg_div_up(pg_min(max_q, N), 64), tree_words, window);
+    const size_t need =
+        pg_ws_bytes(pg_make_plan(N, B, max_q, max_kv, Hq / Hkv, Hkv, window, sinks), Hkv);
+    if (need > 0 && (!ws || ((uintptr_t)ws & 15) || ws_bytes < need))
+        return fail(6, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", what,
+                    need, ws ? ws_bytes : (size_t)0);
+    const cujev_paged_seqs seqs = {q_start, kv_len, page_table, max_pages, B};
+    return launched(k_attention_paged((const bf16_t *)q, (const bf16_t *)gate, gate_tok_stride,
+                                      gate_head_stride, &pages, &seqs, N, max_q, max_kv, Hq,
+                                      window, sinks, (const uint64_t *)tree, tree_words,
+                                      (bf16_t *)out, lse, ws, ws_bytes,
+                                      (hipStream_t)stream),
+                    what);
+}
+
 EXPORT int cujev_op_attention_paged(const void *q, const void *gate, int gate_tok_stride,
                                     int gate_head_stride, int kv_type, const void *k_pages,
                                     const void *vt_pages, const float *k_scale,
@@ -383,36 +465,42 @@ EXPORT int cujev_op_attention_paged(const void *q, const void *gate, int gate_to
                                     int max_pages, int B, int N, int max_q, int max_kv, int Hq,
                                     int Hkv, int window, int sinks, void *out, void *ws,
                                     size_t ws_bytes, void *stream) {
-    const cujev_kv_pages pages = {(void *)k_pages, (void *)vt_pages, (float *)k_scale,
-                                  (float *)v_scale, num_pages, Hkv, kv_type};
-    const int st = paged_check("attention_paged", &pages, page_table, max_pages, kv_len, B);
-    if (st != 0)
-        return st;
-    if (N < 0 || N > PG_MOST || max_q < 0 || max_kv < 0 || !paged_heads_ok(Hq, Hkv))
-        return fail(1, "attention_paged: unsupported shape N=%d max_q=%d max_kv=%d Hq=%d Hkv=%d",
-                    N, max_q, max_kv, Hq, Hkv);
-    if (max_kv > max_pages * CUJEV_KV_PAGE)
-        return fail(1, "attention_paged: max_kv=%d is not within the table's %d tokens", max_kv,
-                    max_pages * CUJEV_KV_PAGE);
-    if (window < 0 || sinks < 0 || (sinks > 0 && window == 0))
-        return fail(1, "attention_paged: window=%d sinks=%d (sinks go with a window)", window,
-                    sinks);
-    if (N > 0 && B > 0 && (!q || !q_start || !out))
-        return fail(1, "attention_paged: null argument");
-    if ((((uintptr_t)q | (uintptr_t)out) & 15) || ((uintptr_t)gate & 7) ||
-        (gate && (gate_tok_stride % 4 || gate_head_stride % 4)))
-        return fail(1, "attention_paged: q and out must be 16-byte, gate rows 8-byte aligned");
-    const size_t need =
-        pg_ws_bytes(pg_make_plan(N, B, max_q, max_kv, Hq / Hkv, Hkv, window, sinks), Hkv);
-    if (need > 0 && (!ws || ((uintptr_t)ws & 15) || ws_bytes < need))
-        return fail(6, "attention_paged: needs a 16-byte aligned workspace of %zu bytes, got %zu",
-                    need, ws ? ws_bytes : (size_t)0);
-    const cujev_paged_seqs seqs = {q_start, kv_len, page_table, max_pages, B};
-    return launched(k_attention_paged((const bf16_t *)q, (const bf16_t *)gate, gate_tok_stride,
-                                      gate_head_stride, &pages, &seqs, N, max_q, max_kv, Hq,
-                                      window, sinks, (bf16_t *)out, ws, ws_bytes,
-                                      (hipStream_t)stream),
-                    "attention_paged");
+    return attend_paged("attention_paged", q, gate, gate_tok_stride, gate_head_stride, kv_type,
+                        k_pages, vt_pages, k_scale, v_scale, num_pages, q_start, kv_len,
+                        page_table, max_pages, B, N, max_q, max_kv, Hq, Hkv, window, sinks,
+                        nullptr, 0, out, nullptr, ws, ws_bytes, stream);
+}
+
+EXPORT int cujev_op_attention_paged_lse(const void *q, const void *gate, int gate_tok_stride,
+                                    int gate_head_stride, int kv_type, const void *k_pages,
+                                    const void *vt_pages, const float *k_scale,
+                                    const float *v_scale, int num_pages, const int32_t *q_start,
+                                    const int32_t *kv_len, const int32_t *page_table,
+                                    int max_pages, int B, int N, int max_q, int max_kv, int Hq,
+                                    int Hkv, int window, int sinks, void *out, float *lse, void *ws,
+                                    size_t ws_bytes, void *stream) {
+    if (N > 0 && B > 0 && !lse)
+        return fail(1, "attention_paged_lse: null argument");
+    return attend_paged("attention_paged_lse", q, gate, gate_tok_stride, gate_head_stride, kv_type,
+                        k_pages, vt_pages, k_scale, v_scale, num_pages, q_start, kv_len,
+                        page_table, max_pages, B, N, max_q, max_kv, Hq, Hkv, window, sinks,
+                        nullptr, 0, out, lse, ws, ws_bytes, stream);
+}
+
+EXPORT int cujev_op_attention_paged_tree(const void *q, const void *gate, int gate_tok_stride,
+                                    int gate_head_stride, int kv_type, const void *k_pages,
+                                    const void *vt_pages, const float *k_scale,
+                                    const float *v_scale, int num_pages, const int32_t *q_start,
+                                    const int32_t *kv_len, const int32_t *page_table,
+                                    int max_pages, int B, int N, int max_q, int max_kv, int Hq,
+                                    int Hkv, const void *tree, int tree_words, void *out, float *lse, void *ws,
+                                    size_t ws_bytes, void *stream) {
+    if (N > 0 && B > 0 && !tree)
+        return fail(1, "attention_paged_tree: null argument");
+    return attend_paged("attention_paged_tree", q, gate, gate_tok_stride, gate_head_stride, kv_type,
+                        k_pages, vt_pages, k_scale, v_scale, num_pages, q_start, kv_len,
+                        page_table, max_pages, B, N, max_q, max_kv, Hq, Hkv, 0, 0, tree,
+                        tree_words, out, lse, ws, ws_bytes, stream);
 }
 
 EXPORT size_t cujev_ops_attention_paged_ws_bytes(int N, int B, int max_q, int max_kv, int Hq,
@@ -420,6 +508,82 @@ EXPORT size_t cujev_ops_attention_paged_ws_bytes(int N, int B, int max_q, int ma
     if (!paged_heads_ok(Hq, Hkv))
         return 0;
     return cujev_attention_paged_ws_bytes(N, B, max_q, max_kv, Hq, Hkv, window, sinks, kv_type);
+}
+
+EXPORT int cujev_op_kv_weights(const void *q, const float *lse, int kv_type, const void *k_pages,
+                               const float *k_scale, int num_pages, const int32_t *q_start,
+                               const int32_t *kv_len, const int32_t *page_table, int max_pages,
+                               int B, int N, int max_q, int max_kv, int Hq, int Hkv,
+                               const float *prev, float *weights, void *stream) {
+    /* V is not read: K stands in for it in the pool's check */
+    const cujev_kv_pages pages = {(void *)k_pages, (void *)k_pages, (float *)k_scale,
+                                  (float *)k_scale, num_pages, Hkv, kv_type};
+    const int st = paged_check("kv_weights", &pages, page_table, max_pages, kv_len, B);
+    if (st != 0)
+        return st;
+    if (N < 0 || N > PG_MOST || max_q < 0 || max_kv < 0 || !paged_heads_ok(Hq, Hkv))
+        return fail(1, "kv_weights: unsupported shape N=%d max_q=%d max_kv=%d Hq=%d Hkv=%d", N,
+                    max_q, max_kv, Hq, Hkv);
+    if (max_kv > max_pages * CUJEV_KV_PAGE)
+        return fail(1, "kv_weights: max_kv=%d is not within the table's %d tokens", max_kv,
+                    max_pages * CUJEV_KV_PAGE);
+    if (N > 0 && B > 0 && (!q || !lse || !q_start || !weights))
+        return fail(1, "kv_weights: null argument");
+    if (((uintptr_t)q & 15) || (((uintptr_t)lse | (uintptr_t)prev | (uintptr_t)weights) & 3))
+        return fail(1, "kv_weights: q must be 16-byte, lse and weights 4-byte aligned");
+    const cujev_paged_seqs seqs = {q_start, kv_len, page_table, max_pages, B};
+    return launched(k_kv_weights((const bf16_t *)q, lse, &pages, &seqs, N, max_q, max_kv, Hq, prev,
+                                 weights, (hipStream_t)stream),
+                    "kv_weights");
+}
+
+EXPORT int cujev_op_kv_select(const float *weights, int num_pages, int Hkv,
+                              const int32_t *page_table, int max_pages, const int32_t *kv_len,
+                              int B, int max_kv, int budget, int sinks, int recent, int32_t *keep,
+                              int max_keep, int32_t *keep_len, void *stream) {
+    if (num_pages <= 0 || Hkv <= 0 || B < 0 || B > PG_MOST || max_pages <= 0 ||
+        max_pages > PG_MOST_KEYS / CUJEV_KV_PAGE)
+        return fail(1, "kv_select: bad pool or page table (%d pages, %d kv-heads, B=%d, "
+                       "max_pages=%d)",
+                    num_pages, Hkv, B, max_pages);
+    if (max_kv < 0 || max_kv > max_pages * CUJEV_KV_PAGE)
+        return fail(1, "kv_select: max_kv=%d is not within the table's %d tokens", max_kv,
+                    max_pages * CUJEV_KV_PAGE);
+    if (budget < 0 || sinks < 0 || recent < 0 || (long long)sinks + recent > budget ||
+        max_keep < pg_min(budget, max_kv))
+        return fail(1, "kv_select: budget=%d has to hold sinks=%d and recent=%d, and keep rows of "
+                       "%d the budget",
+                    budget, sinks, recent, max_keep);
+    if (B > 0 && (!weights || !page_table || !kv_len || !keep || !keep_len))
+        return fail(1, "kv_select: null argument");
+    if (B > 0 && keep_len == kv_len) /* other kv-heads read kv_len while one writes */
+        return fail(1, "kv_select: keep_len must be another array than kv_len");
+    const cujev_paged_seqs seqs = {nullptr, kv_len, page_table, max_pages, B};
+    return launched(k_kv_select(weights, num_pages, Hkv, &seqs, max_kv, budget, sinks, recent,
+                                keep, max_keep, keep_len, (hipStream_t)stream),
+                    "kv_select");
+}
+
+EXPORT int cujev_op_kv_keep(int kv_type, void *k_pages, void *vt_pages, float *k_scale,
+                            float *v_scale, float *weights, int num_pages, int Hkv,
+                            const int32_t *page_table, int max_pages, const int32_t *to_table,
+                            int to_pages, int B, const int32_t *keep, int keep_heads, int max_keep,
+                            const int32_t *dst, const int32_t *keep_len, void *stream) {
+    const cujev_kv_pages pages = {k_pages, vt_pages, k_scale, v_scale, num_pages, Hkv, kv_type};
+    const int st = paged_check("kv_keep", &pages, page_table, max_pages, keep_len, B);
+    if (st != 0)
+        return st;
+    if (to_table && (to_pages <= 0 || to_pages > PG_MOST_KEYS / CUJEV_KV_PAGE))
+        return fail(1, "kv_keep: bad table to write to (to_pages=%d)", to_pages);
+    if (max_keep < 0 || max_keep > PG_MOST_KEYS || (keep_heads != 1 && keep_heads != Hkv))
+        return fail(1, "kv_keep: keep is [B][%d][%d], not of 1 or %d heads", keep_heads, max_keep,
+                    Hkv);
+    if (B > 0 && max_keep > 0 && !keep)
+        return fail(1, "kv_keep: null argument");
+    const cujev_paged_seqs seqs = {nullptr, keep_len, page_table, max_pages, B};
+    return launched(k_kv_keep(&pages, weights, &seqs, to_table, to_pages, keep, keep_heads,
+                              max_keep, dst, keep_len, (hipStream_t)stream),
+                    "kv_keep");
 }
 
 EXPORT int cujev_op_gdn_conv_prep(const void *proj, int proj_stride, const float *conv_w,

@@ -19,6 +19,20 @@ static_assert(PG == CUJEV_KV_PAGE, "one definition of a page");
 constexpr int PD = 256;                /* head dim */
 constexpr int PSLICE = PG * PD;        /* elements of one head's K or V^T in a page */
 
+typedef __attribute__((address_space(3))) void *lds_ptr;
+DEV __amdgpu_buffer_rsrc_t make_rsrc(const void *base, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, (int)bytes, 0x00020000);
+}
+DEV u32x4 buf_load16(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, 0));
+}
+/* The lane's number, worked out where it stands: kept, it may go to scratch memory */
+DEV int lane_again() {
+    int none = 0;
+    asm volatile("" : "+v"(none));
+    return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none));
+}
+
 DEV pg_seq load_seq(const int32_t *q_start, const int32_t *kv_len, int b, int N, int max_q,
                     int max_kv) {
     return pg_clean_seq(q_start[b], q_start[b + 1], kv_len[b], N, max_q, max_kv);
@@ -237,6 +251,12 @@ DEV float e4m3_of(uint32_t v, int i) {
 /* Two e4m3 bytes (of the low or high half) times 2^k, exact in bf16. */
 template <bool HIGH> DEV bf16x2 unpack_e4m3(uint32_t v, float scale) {
     return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v, scale, HIGH);
+}
+/* 8 e4m3 values (two dwords) times a power of two -> 8 bf16 */
+DEV bf16x8 widen(uint32_t a, uint32_t b, float scale) {
+    const bf16x2 p = unpack_e4m3<false>(a, scale), q = unpack_e4m3<true>(a, scale);
+    const bf16x2 r = unpack_e4m3<false>(b, scale), s = unpack_e4m3<true>(b, scale);
+    return bf16x8{p[0], p[1], q[0], q[1], r[0], r[1], s[0], s[1]};
 }
 
 } // namespace

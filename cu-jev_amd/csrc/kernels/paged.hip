@@ -34,9 +34,11 @@ constexpr int PREP_V_ROWS = 3, PREP_V_SEQS = 64;
  * 16 x 48 e4m3 7.5 us, 11.2 with a wave a page; of 8 x 700 16.4 and 17.6), a wave a
  * page otherwise, which starts fewer that have nothing to do (64 x 48 16.7 and 19.5). */
 constexpr int PREP_V_FEW = 1024, PREP_V_WHOLE = 128;
-/* A K row's lane in doubles, rounded to e4m3 once: the bytes, and the scale 2^*e */
-DEV uint32_t k_row_exact(const bf16 *src, const float2 *rope, const float *w, bool rotates,
-                         bool first, int half_lanes, float eps, int *e) {
+/* A K row's lane in doubles, rounded to e4m3 once: the bytes, and the scale 2^*e.
+ * rope(i): (cos, sin) of dim i of the lane's */
+template <class F>
+DEV uint32_t k_row_exact(const bf16 *src, F rope, const float *w, bool rotates, bool first,
+                         int half_lanes, float eps, int *e) {
     const bf16x4 raw = *(const bf16x4 *)src;
     double y[4], ss = 0., most = 0.;
 #pragma unroll
@@ -54,7 +56,7 @@ DEV uint32_t k_row_exact(const bf16 *src, const float2 *rope, const float *w, bo
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         y[i] *= rinv * w[i];
-        const float2 cs = rope[rotates ? i : 0];
+        const float2 cs = rope(rotates ? i : 0);
         const double o = __shfl_xor(y[i], half_lanes, 64) * cs.y;
         y[i] = rotates ? __builtin_fma(y[i], (double)cs.x, first ? -o : o) : y[i];
         most = fmax(most, fabs(y[i]));
@@ -73,7 +75,8 @@ struct Prep {
     const int32_t *pos, *q_start, *kv_len, *page_table;
     int max_pages, B, N, Hq, Hkv, rot;
     const float2 *rope;
-    int npos;
+    int npos, axes;
+    uint64_t axis_of; /* two bits a frequency */
     float eps, q_scale;
     bf16 *q_out;
     void *k_pages, *vt_pages;
@@ -83,8 +86,11 @@ struct Prep {
 };
 enum { ROW_Q, ROW_K, ROW_V };
 
-/* A wave for tokens n0 .. n0 + TOK - 1 of one head */
-template <int KIND, int TOK, bool E4M3> DEV void row_wave(const Prep &c, int head, int n0) {
+/* A wave for tokens n0 .. n0 + TOK - 1 of one head. AXES: pos has a row an axis, lane
+ * TOK a + t holds token t's on axis a, and each frequency picks its own: 4 loads of 8
+ * bytes a token and lane, scattered over up to 4 rows of the table. */
+template <int KIND, int TOK, bool E4M3, bool AXES>
+DEV void row_wave(const Prep &c, int head, int n0) {
     constexpr bool is_k = KIND == ROW_K;
     const int lane = threadIdx.x & 63, N = c.N, rot = c.rot;
     const float *w = is_k ? c.kw : c.qw;
@@ -100,10 +106,25 @@ template <int KIND, int TOK, bool E4M3> DEV void row_wave(const Prep &c, int hea
     for (int t = 0; t < TOK; t++)
         raw[t] = *(const bf16x4 *)(src + (size_t)min(n0 + t, N - 1) * c.ps);
     const float4 wl = *(const float4 *)(w + 4 * lane);
-    int pos_lane = min(max(c.pos[min(n0 + (lane & (TOK - 1)), N - 1)], 0), c.npos - 1);
+    const size_t pos_row = AXES ? (size_t)min(lane / TOK & 3, c.axes - 1) * N : 0;
+    int pos_lane = min(max(c.pos[pos_row + min(n0 + (lane & (TOK - 1)), N - 1)], 0), c.npos - 1);
     /* read from all lanes below: sunk into the rotating lanes' branch it was worked out by
      * those alone (rot 8: two, for four tokens) */
     asm volatile("" : "+v"(pos_lane));
+    /* (cos, sin) of token t for dim e of the lane's */
+    const uint32_t axis4 = (uint32_t)(c.axis_of >> (2 * fi0)); /* of the lane's four */
+    auto angle_row = [&](int t, int e) {
+        int p = __builtin_amdgcn_readlane(pos_lane, t);
+        if constexpr (AXES) {
+            const int a = axis4 >> (2 * e) & 3;
+#pragma unroll
+            for (int k = 1; k < 4; k++) {
+                const int pk = __builtin_amdgcn_readlane(pos_lane, TOK * k + t);
+                p = a == k ? pk : p;
+            }
+        }
+        return c.rope + (size_t)p * (rot / 2) + fi0;
+    };
     /* The tokens' sequences, then (K) their slots, token t in lane t: one
      * chain of loads for all of them. at: the K row in the pool, -1: none */
     pg_seq s;
@@ -112,10 +133,18 @@ template <int KIND, int TOK, bool E4M3> DEV void row_wave(const Prep &c, int hea
     if (rotates) { /* 16 lanes' loads or fewer: by all 64 they cost more than x's */
 #pragma unroll
         for (int t = 0; t < TOK; t++) {
-            const float4 *r = (const float4 *)(
-                c.rope + (size_t)__builtin_amdgcn_readlane(pos_lane, t) * (rot / 2) + fi0);
-            rc[t][0] = r[0];
-            rc[t][1] = r[1];
+            if constexpr (AXES) {
+                float2 r[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    r[e] = angle_row(t, e)[e];
+                rc[t][0] = float4{r[0].x, r[0].y, r[1].x, r[1].y};
+                rc[t][1] = float4{r[2].x, r[2].y, r[3].x, r[3].y};
+            } else {
+                const float4 *r = (const float4 *)angle_row(t, 0);
+                rc[t][0] = r[0];
+                rc[t][1] = r[1];
+            }
         }
     }
     if (n0 + lane >= N)
@@ -245,8 +274,7 @@ template <int KIND, int TOK, bool E4M3> DEV void row_wave(const Prep &c, int hea
         const long long row = row_of(t);
         int e;
         const uint32_t out = k_row_exact(
-            src + (size_t)(n0 + t) * c.ps,
-            c.rope + (size_t)__builtin_amdgcn_readlane(pos_lane, t) * (rot / 2) + fi0,
+            src + (size_t)(n0 + t) * c.ps, [&](int i) { return angle_row(t, i)[i]; },
             w + 4 * lane, rotates, first, half_lanes, c.eps, &e);
         ((uint32_t *)c.k_pages)[row * 64 + lane] = out;
         if (lane == 0)
@@ -364,13 +392,13 @@ template <bool E4M3> DEV void v_groups(const Prep &c, int unit, int g0, int g1) 
 }
 
 template <int n> using is = std::integral_constant<int, n>;
-template <bool E4M3, bool V_ROWS>
+template <bool E4M3, bool V_ROWS, bool AXES>
 __global__ __launch_bounds__(64) void prep_paged_kernel(Prep c) {
     int block = blockIdx.x;
     auto rows = [&](auto kind, auto tok, int heads) {
         const int n0 = block / heads * decltype(tok)::value;
         if (n0 < c.N)
-            row_wave<decltype(kind)::value, decltype(tok)::value, E4M3>(c, block % heads, n0);
+            row_wave<decltype(kind)::value, decltype(tok)::value, E4M3, AXES>(c, block % heads, n0);
     };
     /* The longest first (8 x 700 e4m3 1.7 us less than with q's rows first) */
     if (block < c.v_blocks) {
@@ -494,7 +522,8 @@ extern "C" int cujev_kv_pages_ok(const cujev_kv_pages *p) {
 }
 
 extern "C" hipError_t k_attn_prep_paged(const bf16_t *proj, int proj_stride, const float *q_norm_w,
-                                        const float *k_norm_w, const int32_t *pos,
+                                        const float *k_norm_w, const int32_t *pos, int axes,
+                                        uint64_t axis_of,
                                         const cujev_paged_seqs *seqs, int N, int Hq, int rot,
                                         const float *rope_table, int npos, float eps,
                                         float q_scale, bf16_t *q_out, const cujev_kv_pages *pages,
@@ -518,20 +547,30 @@ extern "C" hipError_t k_attn_prep_paged(const bf16_t *proj, int proj_stride, con
         return hipErrorInvalidValue;
     const Prep c = {(const bf16 *)proj, proj_stride, q_norm_w, k_norm_w, pos, seqs->q_start,
                     seqs->kv_len, seqs->page_table, seqs->max_pages, B, N, Hq, Hkv, rot,
-                    (const float2 *)rope_table, npos, eps, q_scale, (bf16 *)q_out, pages->k,
-                    pages->vt, pages->k_scale, pages->v_scale, pages->num_pages, (int)k_blocks,
+                    (const float2 *)rope_table, npos, axes, axis_of, eps, q_scale, (bf16 *)q_out,
+                    pages->k, pages->vt, pages->k_scale, pages->v_scale, pages->num_pages, (int)k_blocks,
                     (int)v_blocks, v_spread};
-#define LAUNCH(T, V)                                                                              \
-    hipLaunchKernelGGL((prep_paged_kernel<T, V>), dim3((unsigned)blocks), dim3(64), 0, stream, c)
-    if (e4m3 && v_rows)
-        LAUNCH(true, true);
-    else if (e4m3)
-        LAUNCH(true, false);
-    else if (v_rows)
-        LAUNCH(false, true);
+    auto launch = [&](auto t, auto v, auto a) {
+        hipLaunchKernelGGL(
+            (prep_paged_kernel<decltype(t)::value, decltype(v)::value, decltype(a)::value>),
+            dim3((unsigned)blocks), dim3(64), 0, stream, c);
+    };
+    auto by_axes = [&](auto t, auto v) {
+        if (axes > 1)
+            launch(t, v, std::true_type{});
+        else
+            launch(t, v, std::false_type{});
+    };
+    auto by_v = [&](auto t) {
+        if (v_rows)
+            by_axes(t, std::true_type{});
+        else
+            by_axes(t, std::false_type{});
+    };
+    if (e4m3)
+        by_v(std::true_type{});
     else
-        LAUNCH(false, false);
-#undef LAUNCH
+        by_v(std::false_type{});
     return hipGetLastError();
 }
 

@@ -53,6 +53,26 @@ _SIGS = {
     # max_pages, B, N, max_q, max_kv, Hq, Hkv, window, sinks, out, ws, ws_bytes, stream
     "cujev_op_attention_paged": [_P, _P, _I, _I, _I, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I,
                                  _I, _I, _I, _I, _I, _I, _P, _P, C.c_size_t, _P],
+    # as attn_prep_paged, with axes and axis_of after pos
+    "cujev_op_attn_prep_paged_axes": [_P, _I, _P, _P, _P, _I, C.c_uint64, _P, _P, _P, _I, _I, _I,
+                                      _I, _I, _I, _P, _I, _F, _F, _P, _I, _P, _P, _P, _P, _I, _P],
+    # as attention_paged, with lse after out
+    "cujev_op_attention_paged_lse": [_P, _P, _I, _I, _I, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I,
+                                     _I, _I, _I, _I, _I, _I, _I, _P, _P, _P, C.c_size_t, _P],
+    # as attention_paged_lse, with tree, tree_words for window, sinks
+    "cujev_op_attention_paged_tree": [_P, _P, _I, _I, _I, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I,
+                                      _I, _I, _I, _I, _I, _P, _I, _P, _P, _P, C.c_size_t, _P],
+    # q, lse, kv_type, k, k_scale, num_pages, q_start, kv_len, page_table, max_pages, B, N, max_q,
+    # max_kv, Hq, Hkv, prev, weights, stream
+    "cujev_op_kv_weights": [_P, _P, _I, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P,
+                            _P],
+    # weights, num_pages, Hkv, page_table, max_pages, kv_len, B, max_kv, budget, sinks, recent,
+    # keep, max_keep, keep_len, stream
+    "cujev_op_kv_select": [_P, _I, _I, _P, _I, _P, _I, _I, _I, _I, _I, _P, _I, _P, _P],
+    # kv_type, k, vt, k_scale, v_scale, weights, num_pages, Hkv, page_table, max_pages, to_table,
+    # to_pages, B, keep, keep_heads, max_keep, dst, keep_len, stream
+    "cujev_op_kv_keep": [_I, _P, _P, _P, _P, _P, _I, _I, _P, _I, _P, _I, _I, _P, _I, _I, _P, _P,
+                         _P],
     "cujev_op_gdn_conv_prep": [_P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _P, _P, _P, _P,
                                _P, _P],
     "cujev_op_gemm_small": [_P, _I, _P, _I, _I, _I, _I, _I, _P, _I, _P, _P],
@@ -314,11 +334,35 @@ def _paged_seqs(pages, page_table, kv_len, q_start=None):
     return dev, B
 
 
+class RopeAxes:
+    """Which axis of a token's position each of the rot / 2 rotary frequencies turns by:
+    axis_of[i] from 0 to 3. from_sections makes it of sections, a count of frequencies
+    for each axis: one after the other, or interleaved, in turn while an axis's section
+    lasts and the first axis after that (Qwen3.5's mrope_section of three axes)."""
+
+    __slots__ = ("axis_of", "axes", "packed")
+
+    def __init__(self, axis_of):
+        self.axis_of = tuple(int(a) for a in axis_of)
+        if not 1 <= len(self.axis_of) <= 32 or not all(0 <= a < 4 for a in self.axis_of):
+            raise OpsError(f"RopeAxes: need up to 32 axes from 0 to 3, got {self.axis_of}")
+        self.axes = max(self.axis_of) + 1
+        self.packed = sum(a << 2 * i for i, a in enumerate(self.axis_of))
+
+    @classmethod
+    def from_sections(cls, sections, interleaved=False):
+        n, k = sum(sections), len(sections)
+        if interleaved:
+            return cls(i % k if i < k * sections[i % k] else 0 for i in range(n))
+        return cls(a for a, count in enumerate(sections) for _ in range(count))
+
+
 def attn_prep_paged(proj, q_norm_w, k_norm_w, pos, q_start, kv_len, page_table, Hq, rot, rope,
-                    eps, q_scale, q_out, pages):
+                    eps, q_scale, q_out, pages, axes=None):
     """attn_prep with K and V written into the pages of each row's sequence:
     sequence b's new tokens are rows q_start[b] .. q_start[b + 1], the last of
-    its kv_len[b] keys. q_out [N, Hq, 256]; rope from rope_table."""
+    its kv_len[b] keys. q_out [N, Hq, 256]; rope from rope_table. With axes (a
+    RopeAxes of rot / 2 frequencies) pos is [axes.axes, N], a row an axis."""
     import torch
     dev, B = _paged_seqs(pages, page_table, kv_len, q_start)
     if proj.dim() != 2:
@@ -332,11 +376,17 @@ def attn_prep_paged(proj, q_norm_w, k_norm_w, pos, q_start, kv_len, page_table, 
     if stride >> 31:
         _need_ints("attn_prep_paged: the stride of proj's rows", stride)
     f32, angles = torch.float32, (rope.shape[0], rot // 2, 2)
+    places = (N,)
+    if axes is not None:
+        places = (axes.axes, N)
+        if len(axes.axis_of) * 2 != rot:
+            raise OpsError(f"axes: of {len(axes.axis_of)} frequencies, and rot {rot} has "
+                           f"{rot // 2}")
     if not (q_norm_w is not None and q_norm_w.dtype is f32 and q_norm_w.shape == (256,) and
             q_norm_w.is_contiguous() and q_norm_w.get_device() == dev and
             k_norm_w is not None and k_norm_w.dtype is f32 and k_norm_w.shape == (256,) and
             k_norm_w.is_contiguous() and k_norm_w.get_device() == dev and
-            pos is not None and pos.dtype is torch.int32 and pos.shape == (N,) and
+            pos is not None and pos.dtype is torch.int32 and pos.shape == places and
             pos.is_contiguous() and pos.get_device() == dev and
             rope.dtype is f32 and rope.shape == angles and rope.is_contiguous() and
             rope.get_device() == dev and
@@ -344,12 +394,14 @@ def attn_prep_paged(proj, q_norm_w, k_norm_w, pos, q_start, kv_len, page_table, 
             q_out.is_contiguous() and q_out.get_device() == dev):
         _need("q_norm_w", q_norm_w, f32, dev, (256,))
         _need("k_norm_w", k_norm_w, f32, dev, (256,))
-        _need("pos", pos, torch.int32, dev, (N,))
+        _need("pos", pos, torch.int32, dev, places)
         _need("rope", rope, f32, dev, angles)
         _need("q_out", q_out, torch.bfloat16, dev, (N, Hq, 256))
-    _paged_call(dev, "cujev_op_attn_prep_paged", proj.data_ptr(), stride,
-                q_norm_w.data_ptr(), k_norm_w.data_ptr(), pos.data_ptr(), q_start.data_ptr(),
-                kv_len.data_ptr(), page_table.data_ptr(), page_table.shape[1], B, N, Hq, Hkv, rot,
+    name, turned = "cujev_op_attn_prep_paged", ()
+    if axes is not None:
+        name, turned = "cujev_op_attn_prep_paged_axes", (axes.axes, axes.packed)
+    _paged_call(dev, name, proj.data_ptr(), stride, q_norm_w.data_ptr(), k_norm_w.data_ptr(),
+                pos.data_ptr(), *turned, q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(), page_table.shape[1], B, N, Hq, Hkv, rot,
                 rope.data_ptr(), rope.shape[0], eps, q_scale, q_out.data_ptr(), *pages.args)
 
 
@@ -384,12 +436,17 @@ def attention_paged_ws_bytes(N, B, max_q, max_kv, Hq, Hkv, window=0, sinks=0, e4
 
 
 def attention_paged(q, gate, gate_tok_stride, gate_head_stride, pages, page_table, q_start, kv_len,
-                    max_q, max_kv, out, window=0, sinks=0, ws=None):
+                    max_q, max_kv, out, window=0, sinks=0, ws=None, tree=None, lse=None):
     """Attention of the call's rows q [N, Hq, 256] over their sequences' pages,
     causal; with window > 0 over the last `window` positions and the first
     `sinks`. gate may be None. max_q and max_kv bound the sequences' new tokens
     and keys; ws: uint8 device workspace of attention_paged_ws_bytes, of this call or
-    a larger one (None where that is 0)."""
+    a larger one (None where that is 0).
+
+    tree int64 [N, words], words at least min(max_q, N) / 64 rounded up: the rows of a
+    sequence are drafted tokens that see all keys before them and, of each other, those
+    whose bits are set (row i's ancestors and its own: bit j % 64 of word j // 64 is new
+    token j); no window. lse float32 [N, Hq] gets the softmax's log2 of the sum of 2^(q.k)."""
     import torch
     dev, B = _paged_seqs(pages, page_table, kv_len, q_start)
     if (max_q | max_kv | window | sinks | gate_tok_stride | gate_head_stride) >> 31:
@@ -415,11 +472,122 @@ def attention_paged(q, gate, gate_tok_stride, gate_head_stride, pages, page_tabl
     if ws is not None and not (ws.dtype is torch.uint8 and ws.dim() == 1 and
                                ws.is_contiguous() and ws.get_device() == dev):
         _need("ws", ws, torch.uint8, dev, (size,))
-    _paged_call(dev, "cujev_op_attention_paged", q.data_ptr(),
+    name, seen, stats = "cujev_op_attention_paged", (window, sinks), ()
+    if lse is not None:
+        name, stats = "cujev_op_attention_paged_lse", (lse.data_ptr(),)
+        if not (lse.dtype is torch.float32 and lse.shape == (N, Hq) and lse.is_contiguous() and
+                lse.get_device() == dev):
+            _need("lse", lse, torch.float32, dev, (N, Hq))
+    if tree is not None:
+        name = "cujev_op_attention_paged_tree"
+        words = tree.shape[1] if tree.dim() == 2 else 0
+        if not (tree.dtype is torch.int64 and tree.shape == (N, words) and
+                tree.is_contiguous() and tree.get_device() == dev):
+            _need("tree", tree, torch.int64, dev, (N, words))
+        if window or sinks:
+            raise OpsError(f"attention_paged: window={window} sinks={sinks} do not go with a tree")
+        # no rows: an empty tensor has no address
+        seen, stats = (tree.data_ptr() or 8, words), stats or (None,)
+    _paged_call(dev, name, q.data_ptr(),
                 None if gate is None else gate.data_ptr(), gate_tok_stride, gate_head_stride,
                 *pages.args, q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(),
-                page_table.shape[1], B, N, max_q, max_kv, Hq, pages.Hkv, window, sinks,
-                out.data_ptr(), None if ws is None else ws.data_ptr(), size)
+                page_table.shape[1], B, N, max_q, max_kv, Hq, pages.Hkv, *seen,
+                out.data_ptr(), *stats, None if ws is None else ws.data_ptr(), size)
+
+
+def _weights_ok(name, w, pages):
+    import torch
+    shape = (pages.num_pages, pages.Hkv, KV_PAGE)
+    if not (w is not None and w.dtype is torch.float32 and w.shape == shape and
+            w.is_contiguous() and w.get_device() == pages.device):
+        _need(name, w, torch.float32, pages.device, shape)
+
+
+def kv_weights(q, lse, pages, page_table, q_start, kv_len, max_q, max_kv, weights, prev=None):
+    """weights [pages, Hkv, 64] (float32, beside the pages' keys) of every key of the
+    sequences that have new tokens: prev's, where given and the key is before the new
+    tokens, plus what the rows q [N, Hq, 256] of the call gave it, with the lse [N, Hq]
+    of their attention. prev may be weights itself, to add in place; None starts anew."""
+    import torch
+    dev, B = _paged_seqs(pages, page_table, kv_len, q_start)
+    if (max_q | max_kv) >> 31:
+        _need_ints("kv_weights", max_q, max_kv)
+    if q.dim() != 3:
+        raise OpsError(f"q: need [N, Hq, 256], got {tuple(q.shape)}")
+    N, Hq = q.shape[0], q.shape[1]
+    if not (q.dtype is torch.bfloat16 and q.shape == (N, Hq, 256) and q.is_contiguous() and
+            q.get_device() == dev and lse is not None and lse.dtype is torch.float32 and
+            lse.shape == (N, Hq) and lse.is_contiguous() and lse.get_device() == dev):
+        _need("q", q, torch.bfloat16, dev, (N, Hq, 256))
+        _need("lse", lse, torch.float32, dev, (N, Hq))
+    _weights_ok("weights", weights, pages)
+    if prev is not None and prev is not weights:
+        _weights_ok("prev", prev, pages)
+    kv_type, k, _, k_scale, _, num_pages = pages.args
+    _paged_call(dev, "cujev_op_kv_weights", q.data_ptr(), lse.data_ptr(), kv_type, k, k_scale,
+                num_pages, q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(),
+                page_table.shape[1], B, N, max_q, max_kv, Hq, pages.Hkv,
+                None if prev is None else prev.data_ptr(), weights.data_ptr())
+
+
+def kv_select(weights, page_table, kv_len, max_kv, budget, keep, keep_len, sinks=0, recent=0):
+    """The positions that each sequence and kv-head keeps, ascending, into keep [B, Hkv,
+    max_keep] and their number, min(kv_len, max_kv, budget), into keep_len [B] (int32, another
+    tensor than kv_len): the first `sinks`, the last `recent`, and of the others the heaviest by
+    weights [pages, Hkv, 64], the lowest position first among equals."""
+    import torch
+    dev, i32 = weights.get_device(), torch.int32
+    if weights.dim() != 3 or weights.shape[2] != KV_PAGE or weights.dtype is not torch.float32 or \
+            not weights.is_contiguous():
+        raise OpsError(f"weights: need contiguous float32 [pages, Hkv, {KV_PAGE}], got "
+                       f"{weights.dtype} {tuple(weights.shape)}")
+    if page_table.dim() != 2 or keep.dim() != 3:
+        raise OpsError(f"kv_select: need page_table [B, max_pages] and keep [B, Hkv, max_keep], got "
+                       f"{tuple(page_table.shape)} and {tuple(keep.shape)}")
+    if (max_kv | budget | sinks | recent) >> 31:
+        _need_ints("kv_select", max_kv, budget, sinks, recent)
+    B, Hkv, max_keep = page_table.shape[0], weights.shape[1], keep.shape[2]
+    for name, t, shape in (("page_table", page_table, page_table.shape), ("kv_len", kv_len, (B,)),
+                           ("keep", keep, (B, Hkv, max_keep)), ("keep_len", keep_len, (B,))):
+        if not (t.dtype is i32 and t.shape == shape and t.is_contiguous() and
+                t.get_device() == dev):
+            _need(name, t, i32, dev, tuple(shape))
+    _paged_call(dev, "cujev_op_kv_select", weights.data_ptr(), weights.shape[0], Hkv,
+                page_table.data_ptr(), page_table.shape[1], kv_len.data_ptr(), B, max_kv, budget,
+                sinks, recent, keep.data_ptr(), max_keep, keep_len.data_ptr())
+
+
+def kv_keep(pages, page_table, keep, keep_len, dst=None, to_table=None, weights=None):
+    """Position dst[b] + i (dst None: i) of sequence b takes K, V, scales and weight of its
+    position keep[b, h, i], i < keep_len[b]; keep [B, Hkv, n], or [B, 1, n] for all
+    kv-heads. In place, where keep has to ascend and be nowhere less than dst[b] + i; or,
+    with to_table [B, to_pages], into pages that page_table does not have."""
+    import torch
+    dev, B = _paged_seqs(pages, page_table, keep_len)
+    i32 = torch.int32
+    if keep.dim() != 3 or keep.shape[1] not in (1, pages.Hkv):
+        raise OpsError(f"keep: need [B, Hkv or 1, n], got {tuple(keep.shape)}")
+    if not (keep.dtype is i32 and keep.shape[0] == B and keep.is_contiguous() and
+            keep.get_device() == dev):
+        _need("keep", keep, i32, dev, (B, *keep.shape[1:]))
+    if dst is not None and not (dst.dtype is i32 and dst.shape == (B,) and dst.is_contiguous() and
+                                dst.get_device() == dev):
+        _need("dst", dst, i32, dev, (B,))
+    to_pages = 0
+    if to_table is not None:
+        to_pages = to_table.shape[1] if to_table.dim() == 2 else 0
+        if not (to_table.dtype is i32 and to_table.shape == (B, to_pages) and to_pages > 0 and
+                to_table.is_contiguous() and to_table.get_device() == dev):
+            _need("to_table", to_table, i32, dev, (B, max(to_pages, 1)))
+    if weights is not None:
+        _weights_ok("weights", weights, pages)
+    kv_type, k, vt, k_scale, v_scale, num_pages = pages.args
+    _paged_call(dev, "cujev_op_kv_keep", kv_type, k, vt, k_scale, v_scale,
+                None if weights is None else weights.data_ptr(), num_pages, pages.Hkv,
+                page_table.data_ptr(), page_table.shape[1],
+                None if to_table is None else to_table.data_ptr(), to_pages, B, keep.data_ptr(),
+                keep.shape[1], keep.shape[2], None if dst is None else dst.data_ptr(),
+                keep_len.data_ptr())
 
 
 def gdn_conv_prep(proj, conv_w, conv_in, conv_out, seg0_len, own_base, A_neg_exp, dt_bias,

@@ -240,6 +240,19 @@ int cujev_op_attn_prep_paged(const void *proj, int proj_stride, const float *q_n
                              void *k_pages, void *vt_pages, float *k_scale, float *v_scale,
                              int num_pages, void *stream);
 
+/* The same for rotary positions of several axes (time, height and width of a patch):
+ * pos is [axes][N], 1 to 4 axes, and frequency i, dims i and i + rot / 2, turns by axis
+ * axis_of >> 2 i & 3, less than axes. One axis gives the bits of the call above, and so
+ * do several with the same positions. */
+int cujev_op_attn_prep_paged_axes(const void *proj, int proj_stride, const float *q_norm_w,
+                                  const float *k_norm_w, const int32_t *pos, int axes,
+                                  uint64_t axis_of, const int32_t *q_start, const int32_t *kv_len,
+                                  const int32_t *page_table, int max_pages, int B, int N, int Hq,
+                                  int Hkv, int rot, const float *rope_table, int npos, float eps,
+                                  float q_scale, void *q_out, int kv_type, void *k_pages,
+                                  void *vt_pages, float *k_scale, float *v_scale, int num_pages,
+                                  void *stream);
+
 /* Reads sequences back: columns [0, min(kv_len[b], max_kv)) of k_cache
  * [B][Hkv][cache_stride][256] and vt_cache [B][Hkv][256][cache_stride], the
  * layout of a state's caches, cache_stride >= cujev_ops_kv_stride(max_kv);
@@ -281,6 +294,86 @@ int cujev_op_attention_paged(const void *q, const void *gate, int gate_tok_strid
                              void *ws, size_t ws_bytes, void *stream);
 size_t cujev_ops_attention_paged_ws_bytes(int N, int B, int max_q, int max_kv, int Hq, int Hkv,
                                           int window, int sinks, int kv_type);
+
+/* The same, and the softmax's statistics: lse fp32 [N][Hq], log2 of the sum over the
+ * row's keys of 2^(q.k), -inf for a row that sees none. out has the bits of the call
+ * above. */
+int cujev_op_attention_paged_lse(const void *q, const void *gate, int gate_tok_stride,
+                                 int gate_head_stride, int kv_type, const void *k_pages,
+                                 const void *vt_pages, const float *k_scale, const float *v_scale,
+                                 int num_pages, const int32_t *q_start, const int32_t *kv_len,
+                                 const int32_t *page_table, int max_pages, int B, int N, int max_q,
+                                 int max_kv, int Hq, int Hkv, int window, int sinks, void *out,
+                                 float *lse, void *ws, size_t ws_bytes, void *stream);
+
+/* Attention of drafted tokens that form a tree: a sequence's new tokens, written as
+ * any others are, see all keys before them and, of each other, what tree says.
+ * tree uint64 [N][tree_words], 8-byte aligned, tree_words at least min(max_q, N) / 64
+ * rounded up: row i of a sequence sees its new token j where bit j % 64 of word j / 64
+ * is set (its ancestors' and its own; any other bits are as good, later tokens' too).
+ * Bits of tokens that the sequence does not have are not read. K of any value, V of
+ * any value where no row of the call sees the key. lse as above, or NULL. No window;
+ * all else, the workspace too, as for cujev_op_attention_paged. */
+int cujev_op_attention_paged_tree(const void *q, const void *gate, int gate_tok_stride,
+                                  int gate_head_stride, int kv_type, const void *k_pages,
+                                  const void *vt_pages, const float *k_scale,
+                                  const float *v_scale, int num_pages, const int32_t *q_start,
+                                  const int32_t *kv_len, const int32_t *page_table, int max_pages,
+                                  int B, int N, int max_q, int max_kv, int Hq, int Hkv,
+                                  const void *tree, int tree_words, void *out, float *lse,
+                                  void *ws, size_t ws_bytes, void *stream);
+
+/* ---- eviction from the paged cache ----------------------------------------------
+ * No counterpart in the reference, whose caches only grow. Three calls on a stream,
+ * between steps: the weight that attention has given each key, the positions worth
+ * keeping, and their move to the front of the sequence; kv_len is then keep_len, and
+ * the pages past it are free. Keys keep their rotary positions, which are in K. A cache
+ * that was evicted from has a sequence's keys in order, but not at their positions:
+ * windows are of no use on it.
+ *
+ * Weights are fp32 [num_pages][Hkv][64], the caller's memory beside the pages: the
+ * weight of a key lies as its scales do. A page that a call writes weights or keys of
+ * belongs to one of its sequences. Page ids, lengths and positions that lie outside
+ * their arrays lead nowhere, as above. */
+
+/* Adds up attention weights: for every sequence that has new tokens (q_start, kv_len,
+ * max_q and max_kv as for the attention) and each of its keys j,
+ *   weights[j] = prev[j] + sum of 2^(q[n][h] . k_j - lse[n][h])
+ * over its rows n that see j, causally, and the q-heads h of the kv-head: with the
+ * attention's lse, what the softmax gave. prev counts for the keys before the new
+ * tokens, whose own weights start here; it may be weights itself, or NULL (all start
+ * here, as for a whole prompt). A row whose lse is -inf adds nothing. The sum's order
+ * depends on the call's sizes alone. Sequences without new tokens are left as they were. */
+int cujev_op_kv_weights(const void *q, const float *lse, int kv_type, const void *k_pages,
+                        const float *k_scale, int num_pages, const int32_t *q_start,
+                        const int32_t *kv_len, const int32_t *page_table, int max_pages, int B,
+                        int N, int max_q, int max_kv, int Hq, int Hkv, const float *prev,
+                        float *weights, void *stream);
+
+/* The positions to keep of each sequence and kv-head, ascending: keep int32 [B][Hkv]
+ * [max_keep] gets n = keep_len[b] = min(kv_len[b], max_kv, budget) of them, the rest of a
+ * row stays as it was. Where that is not all: the first `sinks`, the last `recent`
+ * (together at most budget), and of the others those of the largest weight, the lowest
+ * position first among equals (-0 equals 0; NaN counts as the largest; keys of a page
+ * that is not there as the least). keep_len is another array than kv_len. */
+int cujev_op_kv_select(const float *weights, int num_pages, int Hkv, const int32_t *page_table,
+                       int max_pages, const int32_t *kv_len, int B, int max_kv, int budget,
+                       int sinks, int recent, int32_t *keep, int max_keep, int32_t *keep_len,
+                       void *stream);
+
+/* Moves keys: position dst[b] + i of sequence b (dst NULL: position i) takes K, V, scales
+ * and weight (weights may be NULL) of position keep[b][h][i], i < keep_len[b] cut to
+ * max_keep, for kv-head h (keep_heads 1: one list for all kv-heads), so that a budget's
+ * keys or a draft's accepted path come to lie in a row. to_table NULL: in place; keep
+ * then ascends and keep[b][h][i] >= dst[b] + i (what other lists give is not defined,
+ * but stays within the sequence's pages). Otherwise to_table [B][to_pages] has pages
+ * that no page_table of the call has. An entry whose source or goal is no position of a
+ * page that is there moves nothing. */
+int cujev_op_kv_keep(int kv_type, void *k_pages, void *vt_pages, float *k_scale, float *v_scale,
+                     float *weights, int num_pages, int Hkv, const int32_t *page_table,
+                     int max_pages, const int32_t *to_table, int to_pages, int B,
+                     const int32_t *keep, int keep_heads, int max_keep, const int32_t *dst,
+                     const int32_t *keep_len, void *stream);
 
 /* Replaces reference src/kernels/kernels.h:214-215 (k_gdn_conv) and :221-223
  * (k_gdn_prep), fused. proj rows [q Hk*128 | k Hk*128 | v Hv*128 | z | b | a].
