@@ -25,10 +25,6 @@
 namespace CUJEV_KNS {
 namespace {
 
-typedef __attribute__((address_space(3))) const unsigned char lds_u8;
-DEV u32x4 lds_read16(lds_u8 *base, uint32_t off) {
-    return *(__attribute__((address_space(3))) const u32x4 *)(base + off);
-}
 DEV void lds_write16(unsigned char *base, uint32_t off, u32x4 v) { *(u32x4 *)(base + off) = v; }
 
 
@@ -36,13 +32,6 @@ DEV void lds_write16(unsigned char *base, uint32_t off, u32x4 v) { *(u32x4 *)(ba
 template <int i> DEV float row_lane(float x) {
     return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(
         0, (int)__float_as_uint(x), 0x150 + i, 0xf, 0xf, false));
-}
-template <int n> using template_int = std::integral_constant<int, n>;
-template <int n, typename F> DEV void unroll_for(F f) {
-    if constexpr (n > 0) {
-        unroll_for<n - 1>(f);
-        f(template_int<n - 1>{});
-    }
 }
 /* x, or -inf where the key is hidden. On the bits: hidden scores may be NaN. */
 DEV float hide(bool seen, float x) {
@@ -902,7 +891,6 @@ template <bool E4M3, int KIND> DEV bool attend_many(const Call &c, unsigned char
     auto kaddr = [&](int n, int buf) {
         return (E4M3 ? ka[n] : ka[n & 7] + (n >> 3) * 256) + buf * L::T;
     };
-    typedef __attribute__((address_space(3))) const float *lds_f32;
     auto kscale = [&](int buf) {
         return E4M3 ? *(lds_f32)(lds + L::SC + buf * 256 + (32 * wj + arow) * 4) : 1.f;
     };

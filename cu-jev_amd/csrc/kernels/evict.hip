@@ -11,11 +11,12 @@ namespace {
 /* ---- attention weights by key --------------------------------------------------
  *   w[j] = prev[j] + sum over the call's rows (n, h) that see key j of 2^(q.k_j - lse)
  * with the attention's own lse, so that one product with K gives p whole: no second
- * pass, and no sum that crosses workgroups. A workgroup holds KG pages of a kv-head's
- * K in registers, a wave 64 keys, as the A operand of v_mfma_f32_32x32x16_bf16, and
- * streams the packed rows (token, q-head) through LDS, 32 for each of its 8 / KG row
- * groups at a time. A lane then has p of one row and 32 keys and adds them up over
- * the rows; lanes and row groups are summed once, at the end, in a fixed order. */
+ * pass, and no sum that crosses workgroups. S^T = K Q^T on v_mfma_f32_32x32x16_bf16,
+ * keys on M: a lane has p of one row and 16 keys of each block of 32, and adds them up
+ * over the packed rows (token, q-head); lanes are summed once, at the end, in a fixed
+ * order. Two forms:
+ *   up to 128 rows  Q stays in LDS, a wave streams pages of K past it (weigh_few)
+ *   more            K stays in registers, Q streams through LDS (weigh_many) */
 struct Weigh {
     const bf16 *q;
     const float *lse;
@@ -23,193 +24,450 @@ struct Weigh {
     const float *ks;
     int num_pages;
     const int32_t *q_start, *kv_len, *page_table;
-    int max_pages, B, N, max_q, max_kv, Hq, Hkv, G, rG, blocks; /* of a sequence and head */
+    int max_pages, B, N, max_q, max_kv, Hq, Hkv, G, rG;
+    int blocks; /* workgroups of a sequence and kv-head (many rows: of each split) */
+    int splits; /* many rows: parts of a block's rows, each with a place in parts if over 1 */
     const float *prev;
-    float *w;
+    float *w, *parts; /* [splits][B][Hkv][blocks * 256] */
 };
+/* Rows of 512 bytes of Q by DMA into LDS, two a load; piece p of row r lies in slot
+ * p ^ (r & 15), so that 16 lanes' operands hit 16 bank groups. src: q of the token that
+ * row 0 minus `rest` is the first of; rows past `most` repeat it. */
+DEV void q_rows(const Weigh &c, __amdgpu_buffer_rsrc_t src, unsigned char *to, int first, int rest,
+                int most) {
+    const int id = lane_again(), at = first + (id >> 5); /* worked out each time, not kept */
+    const int row = rest + min(at, most), tok = row * c.rG >> 16;
+    const uint32_t off = (tok * c.Hq + row - tok * c.G) * PD * 2;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_ptr)(to + first * 512), 16,
+                                             off + (((id & 31) ^ (at & 15)) << 4), 0, 0, 0);
+}
+/* Where a lane finds its operand of step ks: the address of step 0's, in the buffer at
+ * `buf`, and the bits to flip. From the buffer's address each time: kept, 16 of them
+ * went to scratch memory. e4m3's steps take 16 dims of K in turn from a load's 16 bytes. */
+template <bool E4M3> DEV uint32_t q_lane(uint32_t buf, int row, int h) {
+    return buf + row * 512 + (((E4M3 ? 2 * h : h) ^ (row & 15)) << 4);
+}
+template <bool E4M3> constexpr uint32_t q_step(int ks) {
+    return (E4M3 ? 4 * (ks >> 1) + (ks & 1) : 2 * ks) << 4;
+}
+/* K of a page's keys, the first `keys` of them: what is past those reads as 0 */
+template <bool E4M3> DEV __amdgpu_buffer_rsrc_t k_rows(const Weigh &c, size_t slice, int keys) {
+    constexpr int ROW = PD * (E4M3 ? 1 : 2);
+    const int bytes = __builtin_amdgcn_readfirstlane(min(max(keys, 0), PG) * ROW);
+    return make_rsrc((const char *)c.k + slice * PG * ROW, bytes);
+}
+/* Sums over the 32 lanes of a half, of pairs a, b: in rows 0, 2 of 16 lanes a's, in 1, 3 b's */
+DEV float sum_rows(float a, float b) {
+    const auto s =
+        __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return fold_row(__uint_as_float(s[0]) + __uint_as_float(s[1]),
+                    [](float p, float q) { return p + q; });
+}
+/* key of accumulator v of a block, lane half h */
+DEV int key_at(int v, int h) { return 8 * (v >> 2) + 4 * h + (v & 3); }
 
-template <bool E4M3, int KG>
-__global__ __launch_bounds__(512, 2) void weigh_kernel(Weigh c) {
-    constexpr int RG = 8 / KG, STEP = 32 * RG;       /* rows a step */
-    constexpr int QB = STEP * PD * 2;                /* bytes of a step's Q */
-    constexpr int T = PSLICE * (E4M3 ? 1 : 2);       /* bytes of a K tile */
-    constexpr int QD = 3;                            /* Q operand reads ahead */
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * QB];
-    __shared__ float part[RG][KG][64];
+constexpr int WEIGH_FEW = 128; /* rows */
+/* A wave a page, up to this many: 64 sequences' token on 4096 bf16 keys 97 us, 5.5 TB/s,
+ * so, 113 with four pages a wave, the next on its way; 512 on 1024 188 and 196 with two */
+constexpr int WEIGH_WAVES = 1 << 20;
+
+/* Few rows: bound by K's bytes. Each of a workgroup's four waves takes a page of the
+ * sequence and kv-head, all 32 KiB of it on the way at once (and beyond WEIGH_WAVES every
+ * blocks * 4-th page), and works on it 32 keys at a time. RB blocks of 32 rows. */
+template <bool E4M3, int RB>
+__global__ __launch_bounds__(256, 2) void weigh_few_kernel(Weigh c) {
+    constexpr int ROW = PD * (E4M3 ? 1 : 2), NL = E4M3 ? 8 : 16; /* loads of 32 keys */
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[RB * 16384];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-    const int kg = wave % KG, rg = wave / KG, col = lane & 31, h = lane >> 5;
-    /* where the kv-heads divide the 8 XCDs, an XCD's workgroups read the same rows */
-    int kh, kb, b;
+    const int col = lane & 31, h = lane >> 5;
+    const int kh = blockIdx.x % c.Hkv, at = blockIdx.x / c.Hkv;
+    const int b = at / c.blocks, stride = c.blocks * 4;
+    int tile = (at % c.blocks) * 4 + wave;
+    const pg_seq s = load_seq(c.q_start, c.kv_len, b, c.N, c.max_q, c.max_kv);
+    const int tiles = pg_div_up(s.kv, PG);
+    if (s.ql <= 0 || (at % c.blocks) * 4 >= tiles)
+        return;
+    /* the page ids of 64 of the wave's tiles, one a lane */
+    int ids = -1, ids0 = tile;
+    auto page_of = [&](int t) {
+        if (t == ids0 || t - ids0 >= 64 * stride) {
+            ids0 = t;
+            const int mine = t + lane * stride;
+            ids = mine < tiles ? c.page_table[(size_t)b * c.max_pages + mine] : -1;
+            ids = ids < c.num_pages ? ids : -1;
+        }
+        return __builtin_amdgcn_readlane(ids, (t - ids0) / stride);
+    };
+    const int nrows = s.ql * c.G;
+    const __amdgpu_buffer_rsrc_t qsrc =
+        make_rsrc(c.q + ((size_t)s.q0 * c.Hq + kh * c.G) * PD, 0x7fffffff);
+#pragma unroll
+    for (int i = 0; i < RB * 4; i++)
+        q_rows(c, qsrc, smem, (i * 4 + wave) * 2, 0, nrows - 1);
+    /* this lane's rows: lse (+inf: none, or it sees nothing), and the last key each sees */
+    float lse[RB];
+    int last[RB];
+#pragma unroll
+    for (int r = 0; r < RB; r++) {
+        const int row = min(32 * r + col, nrows - 1), tok = row * c.rG >> 16;
+        const float x = c.lse[(size_t)(s.q0 + tok) * c.Hq + kh * c.G + row - tok * c.G];
+        lse[r] = 32 * r + col < nrows && x != -INFINITY ? x : INFINITY;
+        last[r] = s.p0 + tok;
+    }
+    u32x4 raw[2][NL];
+    float sc[2] = {1.f, 1.f};
+    auto load = [&](int half, int page, int t) { /* of tile t */
+        const size_t slice = (size_t)max(page, 0) * c.Hkv + kh;
+        const int keys = page < 0 ? 0 : s.kv - t * PG;
+        const __amdgpu_buffer_rsrc_t src = k_rows<E4M3>(c, slice, keys);
+#pragma unroll
+        for (int n = 0; n < NL; n++)
+            raw[half][n] = buf_load16(src, col * ROW + h * 16, half * 32 * ROW + n * 32);
+        if constexpr (E4M3) {
+            const float x = c.ks[slice * PG + 32 * half + col];
+            sc[half] = 32 * half + col < keys ? x : 1.f;
+        }
+    };
+    int page = page_of(tile);
+    load(0, page, tile);
+    load(1, page, tile);
+    /* Q is there (all waves' part of it) */
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    while (tile < tiles) {
+        const int next = tile + stride, next_page = next < tiles ? page_of(next) : -1;
+        unroll_for<2>([&](auto ih) {
+            constexpr int half = decltype(ih)::value;
+            const int key0 = tile * PG + 32 * half;
+            /* after the sums lane 16 r + v (v < 8) is left with accumulator v + 8 (r & 1) */
+            const int mine = key_at((lane & 7) + (lane >> 4 & 1) * 8, h);
+            const size_t to = ((size_t)max(page, 0) * c.Hkv + kh) * PG + 32 * half + mine;
+            const bool own = !(lane & 8) && page >= 0 && key0 + mine < s.kv;
+            const bool add = own && c.prev && key0 + mine < s.p0;
+            float before = 0.f;
+            if (add)
+                before = c.prev[to];
+            float sum[16] = {};
+#pragma unroll
+            for (int r = 0; r < RB; r++) {
+                if (32 * r >= nrows) /* uniform */
+                    break;
+                const uint32_t q0 = q_lane<E4M3>(r * 16384, col, h);
+                floatx16 x = {};
+#pragma unroll
+                for (int ks = 0; ks < 16; ks++) {
+                    const bf16x8 q = *(const bf16x8 *)(smem + (q0 ^ q_step<E4M3>(ks)));
+                    bf16x8 k;
+                    if constexpr (E4M3) {
+                        const u32x4 v = raw[half][ks >> 1];
+                        k = ks & 1 ? widen(v[2], v[3], sc[half]) : widen(v[0], v[1], sc[half]);
+                    } else {
+                        k = __builtin_bit_cast(bf16x8, raw[half][ks]);
+                    }
+                    x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q, x, 0, 0, 0);
+                }
+                if (key0 + 31 <= s.p0) { /* uniform: all rows see them all */
+#pragma unroll
+                    for (int v = 0; v < 16; v++)
+                        sum[v] += fast_exp2(x[v] - lse[r]);
+                } else {
+                    const int seen = last[r] - key0 - 4 * h;
+#pragma unroll
+                    for (int v = 0; v < 16; v++) {
+                        const float p = fast_exp2(x[v] - lse[r]);
+                        sum[v] += key_at(v, 0) <= seen ? p : 0.f;
+                    }
+                }
+            }
+            if (next < tiles)
+                load(half, next_page, next);
+            float all = 0.f;
+#pragma unroll
+            for (int v = 0; v < 8; v++) {
+                const float y = sum_rows(sum[v], sum[v + 8]);
+                all = (lane & 7) == v ? y : all;
+            }
+            if (own)
+                c.w[to] = all + before;
+        });
+        tile = next, page = next_page;
+    }
+}
+
+/* Many rows: bound by the matrix cores. A workgroup holds four pages of a kv-head's K in
+ * registers, a wave 64 keys as the A operands of v_mfma_f32_16x16x32_bf16, and streams
+ * packed rows through LDS, 16 for each of its two row groups a step: a Q operand feeds
+ * four products, and LDS holds four steps, of which three are on their way. Few blocks
+ * of keys share their rows out among several workgroups, whose sums weigh_sum_kernel
+ * adds up. */
+/* lse within it: 2^x and 2^-lse are taken apart, which loses weights below 2^-90 */
+constexpr float LSE_NEAR = 32.f;
+constexpr int WEIGH_KG = 4, WEIGH_AHEAD = 4, WEIGH_GROUPS = 1024, WEIGH_STEPS = 4;
+template <bool E4M3> DEV void weigh_many(const Weigh &c) {
+    constexpr int KG = WEIGH_KG, STEP = 32; /* rows a step, in two halves */
+    constexpr int QB = STEP * PD * 2;       /* bytes of a step's Q */
+    constexpr int NB = WEIGH_AHEAD;         /* steps that LDS holds */
+    constexpr int NL = QB / (KG * 1024);    /* a wave's loads of a step */
+    constexpr int ROW = PD * (E4M3 ? 1 : 2);
+    constexpr int QD = 3; /* Q operand reads ahead */
+    /* Q of NB steps, their lse, and at the end the sums: one array, since of several the
+     * compiler waits for all loads to any of them before it reads one */
+    constexpr int LSE = NB * QB;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[LSE + NB * STEP * 4];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int col = lane & 15, g = lane >> 4;
+    /* where the kv-heads divide the 8 XCDs, an XCD's workgroups read the same rows; the
+     * blocks of the most rows, a sequence's first, start first */
+    int kh, kb, b, split;
     {
-        const int per = 8 % c.Hkv == 0 ? 8 / c.Hkv : 1, all = pg_div_up(c.blocks, per) * per * c.Hkv;
+        const int per = 8 % c.Hkv == 0 ? 8 / c.Hkv : 1, items = c.blocks * c.splits;
+        const int all = pg_div_up(items, per) * per * c.Hkv;
         b = blockIdx.x / all;
-        const int at = blockIdx.x % all;
+        int at = blockIdx.x % all;
         if (8 % c.Hkv == 0) {
             kh = (at & 7) / per;
-            kb = (at >> 3) * per + (at & 7) % per;
+            at = (at >> 3) * per + (at & 7) % per;
         } else {
             kh = at % c.Hkv;
-            kb = at / c.Hkv;
+            at = at / c.Hkv;
         }
+        kb = at / c.splits;
+        split = at % c.splits;
     }
     const pg_seq s = load_seq(c.q_start, c.kv_len, b, c.N, c.max_q, c.max_kv);
     const int k0 = kb * KG * PG; /* the workgroup's first key */
-    if (s.ql <= 0 || k0 >= s.kv)
+    if (s.ql <= 0 || k0 >= s.kv || kb >= c.blocks)
         return;
-    const int key0 = k0 + kg * PG; /* the wave's */
+    const int key0 = k0 + wave * PG; /* the wave's */
     int page = -1;
     if (key0 < s.kv) {
-        page = c.page_table[(size_t)b * c.max_pages + key0 / PG];
+        page = __builtin_amdgcn_readfirstlane(c.page_table[(size_t)b * c.max_pages + key0 / PG]);
         page = page >= 0 && page < c.num_pages ? page : -1;
     }
     const size_t slice = (size_t)max(page, 0) * c.Hkv + kh;
 
-    /* rows: token t of the sequence sees key0 from position key0 on */
-    const int t_first = max(k0 - s.p0, 0), nrows = s.ql * c.G;
-    const int steps = pg_div_up(nrows - t_first * c.G, STEP);
-    /* Q of step n: 2 rows a load, piece p of row r in slot p ^ (r & 15) */
-    auto issue_q = [&](int n) {
-        const int r0 = t_first * c.G + n * STEP, i0 = r0 / c.G, rest = r0 - i0 * c.G;
-        const __amdgpu_buffer_rsrc_t src =
-            make_rsrc(c.q + ((size_t)(s.q0 + i0) * c.Hq + kh * c.G) * PD, 0x7fffffff);
-        const int id = lane_again(); /* addresses are worked out again, not kept */
+    /* Rows: the tokens from position k0 on, and all behind it; the last ones first, so that
+     * the workgroups of a kv-head, whatever their first, read the same ones at a time. A
+     * step has as many whole tokens as fit: where a lane's rows lie in its Q is the same
+     * in all steps. Past the last token Q and lse read as 0. */
+    const int t_first = max(k0 - s.p0, 0), toks = STEP / c.G;
+    const int all_steps = pg_div_up(s.ql - t_first, toks);
+    const int n0 = (int)((long long)all_steps * split / c.splits);
+    const int steps = (int)((long long)all_steps * (split + 1) / c.splits);
+    uint32_t qoff[NL], loff;
 #pragma unroll
-        for (int i = 0; i < 2 * RG; i++) {
-            const int at = (i * 8 + wave) * 2 + (id >> 5), row = rest + min(at, nrows - 1 - r0);
-            const int tok = row * c.rG >> 16;
-            const uint32_t off = (tok * c.Hq + row - tok * c.G) * PD * 2;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                src, (lds_ptr)(smem + (n & 1) * QB + (i * 8 + wave) * 1024), 16,
-                off + (((id & 31) ^ (at & 15)) << 4), 0, 0, 0);
-        }
-    };
-    /* this lane's row of step n: its lse (+inf where there is none, or it sees nothing), and
-     * the last key that it sees */
-    float lse;
-    int last;
-    auto row_of = [&](int n) {
-        const int r0 = t_first * c.G + n * STEP, i0 = r0 / c.G, rest = r0 - i0 * c.G;
-        const int at = 32 * rg + (lane_again() & 31), row = rest + min(at, nrows - 1 - r0);
-        const int tok = row * c.rG >> 16;
-        const float x = c.lse[(size_t)(s.q0 + i0 + tok) * c.Hq + kh * c.G + row - tok * c.G];
-        lse = r0 + at < nrows && x != -INFINITY ? x : INFINITY;
-        last = s.p0 + i0 + tok;
-    };
-    if (steps > 0)
-        issue_q(0);
-    bf16x8 kf[2][16];
-    {
-        const __amdgpu_buffer_rsrc_t src = make_rsrc((const char *)c.k + slice * T, T);
-        const uint32_t voff = col * (T / PG) + h * 16;
-        u32x4 raw[2][E4M3 ? 8 : 16];
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int n = 0; n < (E4M3 ? 8 : 16); n++)
-                raw[i][n] = buf_load16(src, voff, i * (T / 2) + n * 32);
-        float sc[2] = {1.f, 1.f};
-        if constexpr (E4M3) {
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-                sc[i] = c.ks[slice * PG + 32 * i + col];
-        }
-        if (page < 0 || key0 + PG > s.kv) { /* slots of no key may hold anything */
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const bool there = page >= 0 && key0 + 32 * i + col < s.kv;
-                sc[i] = there ? sc[i] : 1.f;
-#pragma unroll
-                for (int n = 0; n < (E4M3 ? 8 : 16); n++)
-                    raw[i][n] &= there ? ~0u : 0u;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int n = 0; n < (E4M3 ? 8 : 16); n++) {
-                const u32x4 v = raw[i][n];
-                if constexpr (E4M3) {
-                    kf[i][2 * n] = widen(v[0], v[1], sc[i]);
-                    kf[i][2 * n + 1] = widen(v[2], v[3], sc[i]);
-                } else {
-                    kf[i][n] = __builtin_bit_cast(bf16x8, v);
-                }
-            }
+    for (int i = 0; i < NL; i++) {
+        const int at = (i * KG + wave) * 2 + (lane >> 5), tok = at * c.rG >> 16;
+        qoff[i] = tok < toks ? (tok * c.Hq + at - tok * c.G) * PD * 2 +
+                                   (((lane & 31) ^ (at & 15)) << 4)
+                             : 0x7ffffff0u; /* no row: it reads as 0 */
     }
-    float sum[2][16] = {};
-    for (int n = 0; n < steps; n++) {
-        row_of(n);
-        /* step n's Q is there, and the other buffer read */
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    {
+        const int at = lane & (STEP - 1), tok = at * c.rG >> 16;
+        loff = (tok * c.Hq + at - tok * c.G) * 4;
+    }
+    /* from step `steps` on the first tokens again: what a wait counts stays the same */
+    auto first_tok = [&](int n) { return max(s.ql - (n + 1) * toks, t_first); };
+    auto issue = [&](int n) {
+        const int i0 = first_tok(n);
+        const size_t from = (size_t)(s.q0 + i0) * c.Hq + kh * c.G;
+        const size_t left = (size_t)(s.ql - i0) * c.Hq - kh * c.G;
+        const int bytes = (int)min(left * PD * 2, (size_t)0x7fffffff);
+        const __amdgpu_buffer_rsrc_t src =
+            make_rsrc(c.q + from * PD, __builtin_amdgcn_readfirstlane(bytes));
+#pragma unroll
+        for (int i = 0; i < NL; i++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                src, (lds_ptr)(smem + n % NB * QB + (i * KG + wave) * 1024), 16, qoff[i], 0, 0, 0);
+        if (wave == 0 && lane < STEP) {
+            const int lbytes = (int)min(left * 4, (size_t)0x7fffffff);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                make_rsrc(c.lse + from, __builtin_amdgcn_readfirstlane(lbytes)),
+                (lds_ptr)(smem + LSE + n % NB * (STEP * 4)), 4, loff, 0, 0, 0);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < NB - 1; i++)
+        issue(n0 + i);
+    bf16x8 kf[4][8];
+    {
+        const int keys = page < 0 ? 0 : s.kv - key0;
+        const __amdgpu_buffer_rsrc_t src = k_rows<E4M3>(c, slice, keys);
+        const uint32_t voff = col * ROW + g * 16;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if constexpr (E4M3) {
+                u32x4 raw[4];
+#pragma unroll
+                for (int n = 0; n < 4; n++)
+                    raw[n] = buf_load16(src, voff, i * 16 * ROW + n * 64);
+                const float x = c.ks[slice * PG + 16 * i + col];
+                const float sc = 16 * i + col < keys ? x : 1.f;
+#pragma unroll
+                for (int n = 0; n < 4; n++) {
+                    kf[i][2 * n] = widen(raw[n][0], raw[n][1], sc);
+                    kf[i][2 * n + 1] = widen(raw[n][2], raw[n][3], sc);
+                }
+            } else {
+#pragma unroll
+                for (int n = 0; n < 8; n++)
+                    kf[i][n] =
+                        __builtin_bit_cast(bf16x8, buf_load16(src, voff, i * 16 * ROW + n * 64));
+            }
+        }
+    }
+    float sum[4][4] = {};
+    floatx4 xa[4] = {}, xb[4] = {};
+    /* this lane's operand of row col of a step, the k-steps' bits flipped */
+    const uint32_t q_row = col * 512 + (((E4M3 ? 2 * g : g) ^ col) << 4);
+    bf16x8 ring[QD];
+    /* operand j of a step: k-step j % 8 of half j / 8 */
+    auto q_at = [&](uint32_t q0, int j) {
+        const int ks = j & 7;
+        const uint32_t bits = (E4M3 ? 8 * (ks >> 1) + (ks & 1) : 4 * ks) << 4;
+        return __builtin_bit_cast(
+            bf16x8, lds_read16((lds_u8 *)smem, (q0 ^ bits) + (j >> 3) * (16 * PD * 2)));
+    };
+    /* Products of a half of step n into x; beside(ks) goes between the k-steps */
+    auto products = [&](auto ih, uint32_t q0, floatx4 (&x)[4], auto beside) {
+        constexpr int half = decltype(ih)::value;
+        unroll_for<8>([&](auto iks) {
+            constexpr int ks = decltype(iks)::value, j = 8 * half + ks;
+            const bf16x8 q = ring[j % QD];
+            if constexpr (j + QD < 16)
+                ring[j % QD] = q_at(q0, j + QD);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                x[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i][ks], q,
+                                                               ks ? x[i] : floatx4{}, 0, 0, 0);
+            beside(iks);
+            __builtin_amdgcn_sched_barrier(0); /* no more operands at a time: registers */
+        });
+    };
+    int my_tok[2]; /* of this lane's row of each half */
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        my_tok[i] = 16 * i + col < toks * c.G ? (16 * i + col) * c.rG >> 16 : 0x7fffffff;
+    /* a half that is done: its lane's factor 2^-lse (0: no row) and lse, the last key that
+     * the row sees, from key0 + 4 g on; whether all is seen, every lse near, and every
+     * row counted but those that read as 0 */
+    struct Row {
+        float f, lse;
+        int seen;
+        bool plain;
+    };
+    auto row_of = [&](int n, int half) {
+        const float l = *(lds_f32)((lds_u8 *)smem + LSE + n % NB * (STEP * 4) + half * 64 + col * 4);
+        const int tok = my_tok[half];
+        const int i0 = first_tok(n); /* the last step's tokens end where the others began */
+        const bool there = tok < s.ql - n * toks - i0;
+        const bool near = __all(fabsf(l) <= LSE_NEAR), whole = s.p0 + i0 >= key0 + PG - 1;
+        Row r;
+        r.f = there ? fast_exp2(-l) : 0.f;
+        r.lse = there && l != -INFINITY ? l : INFINITY;
+        r.seen = whole ? PG : s.p0 + i0 + min(tok, STEP) - key0 - 4 * g;
+        r.plain = near && whole && (n + 1) * (long long)toks <= s.ql - t_first;
+        return r;
+    };
+    /* 2^x 2^-lse: a product added at once, no difference before. A row's x is at most its lse. */
+    auto add_plain = [&](const floatx4 (&x)[4], float f, int m) {
+        sum[m >> 2][m & 3] = __builtin_fmaf(fast_exp2(x[m >> 2][m & 3]), f, sum[m >> 2][m & 3]);
+    };
+    auto add = [&](const floatx4 (&x)[4], const Row &r) {
+#pragma unroll
+        for (int m = 0; m < 16; m++) {
+            const float p = fast_exp2(x[m >> 2][m & 3] - r.lse);
+            sum[m >> 2][m & 3] += 16 * (m >> 2) + (m & 3) <= r.seen ? p : 0.f;
+        }
+    };
+    /* a half's products into y, and beside them what x has of the half before */
+    auto turn = [&](auto ih, uint32_t q0, floatx4 (&y)[4], const floatx4 (&x)[4], const Row &r) {
+        if (r.plain) {
+            products(ih, q0, y, [&](auto iks) {
+                constexpr int ks = decltype(iks)::value;
+                add_plain(x, r.f, 2 * ks);
+                add_plain(x, r.f, 2 * ks + 1);
+            });
+        } else {
+            add(x, r);
+            products(ih, q0, y, [](auto) {});
+        }
+    };
+    Row before{0.f, INFINITY, 0, true}; /* ahead of the first half: nothing */
+    for (int n = n0; n < steps; n++) {
+        /* step n's Q is there, and that of n - 1 read: its place takes step n + NB - 1's */
+        if (wave == 0)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NB - 2) * (NL + 1)) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NB - 2) * NL) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (n + 1 < steps)
-            issue_q(n + 1);
-        /* this lane's row and half of piece 0; the others by their bits, worked out from
-         * the buffer's address each time: kept, 16 of them went to scratch memory */
-        const uint32_t at0 = (n & 1) * QB + (32 * rg + col) * 512 +
-                             (((E4M3 ? 2 * h : h) ^ (col & 15)) << 4);
-        auto q_at = [&](int ks) {
-            const uint32_t bits = (E4M3 ? 4 * (ks >> 1) + (ks & 1) : 2 * ks) << 4;
-            return *(const bf16x8 *)(smem + (at0 ^ bits));
-        };
-        floatx16 x[2] = {};
-        bf16x8 ring[QD];
+        const uint32_t q0 = n % NB * QB + q_row;
 #pragma unroll
-        for (int ks = 0; ks < QD; ks++)
-            ring[ks] = q_at(ks);
-#pragma unroll
-        for (int ks = 0; ks < 16; ks++) {
-            const bf16x8 qv = ring[ks % QD];
-            if (ks + QD < 16)
-                ring[ks % QD] = q_at(ks + QD);
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-                x[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i][ks], qv, x[i], 0, 0, 0);
-            __builtin_amdgcn_sched_barrier(0); /* no more operands at a time: registers */
-        }
-        /* accumulator v of block i is key key0 + 32 i + 8 (v >> 2) + 4 h + (v & 3) */
-        if (__all(last >= key0 + PG - 1)) {
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int v = 0; v < 16; v++)
-                    sum[i][v] += fast_exp2(x[i][v] - lse);
-        } else {
-            const int seen = last - key0 - 4 * h;
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int v = 0; v < 16; v++) {
-                    const float p = fast_exp2(x[i][v] - lse);
-                    sum[i][v] += 32 * i + 8 * (v >> 2) + (v & 3) <= seen ? p : 0.f;
-                }
-        }
+        for (int j = 0; j < QD; j++)
+            ring[j] = q_at(q0, j);
+        issue(n + NB - 1);
+        const Row r = row_of(n, 0);
+        turn(template_int<0>{}, q0, xa, xb, before);
+        before = row_of(n, 1);
+        turn(template_int<1>{}, q0, xb, xa, r);
     }
-    /* over the 32 rows' lanes: lane 16 r + v is left with block r & 1, half r >> 1, number v */
+    add(xb, before);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    /* over the 16 rows' lanes: lane 16 g + m is left with block m >> 2, number m & 3 */
     float mine = 0.f;
 #pragma unroll
-    for (int v = 0; v < 16; v++) {
-        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(sum[0][v]),
-                                                        __float_as_uint(sum[1][v]), false, false);
-        const float t = fold_row(__uint_as_float(a[0]) + __uint_as_float(a[1]),
-                                 [](float p, float q) { return p + q; });
-        mine = (lane & 15) == v ? t : mine;
+    for (int m = 0; m < 16; m++) {
+        const float y = fold_row(sum[m >> 2][m & 3], [](float p, float q) { return p + q; });
+        mine = col == m ? y : mine;
     }
-    const int v = lane & 15, key = 32 * (lane >> 4 & 1) + 8 * (v >> 2) + 4 * h + (v & 3);
-    part[rg][kg][key] = mine;
-    __syncthreads();
-    if (rg == 0 && page >= 0 && key0 + lane < s.kv) {
-        float all = part[0][kg][lane];
-#pragma unroll
-        for (int i = 1; i < RG; i++)
-            all += part[i][kg][lane];
-        const size_t to = slice * PG + lane;
-        if (c.prev && key0 + lane < s.p0)
-            all += c.prev[to];
-        c.w[to] = all;
+    /* and left with key l of the wave's in lane l */
+    mine = __shfl(mine, (lane >> 2 & 3) * 16 + (lane >> 4) * 4 + (lane & 3), 64);
+    {
+        if (c.splits > 1) {
+            c.parts[(((size_t)split * c.B + b) * c.Hkv + kh) * c.blocks * (KG * PG) + key0 +
+                    lane] = mine;
+        } else if (page >= 0 && key0 + lane < s.kv) {
+            const size_t to = slice * PG + lane;
+            if (c.prev && key0 + lane < s.p0)
+                mine += c.prev[to];
+            c.w[to] = mine;
+        }
     }
 }
+
+template <bool E4M3> __global__ __launch_bounds__(256, 2) void weigh_many_kernel(Weigh c) {
+    weigh_many<E4M3>(c);
+}
+
+/* The splits' sums of a key, in order: a thread a key */
+__global__ __launch_bounds__(256) void weigh_sum_kernel(Weigh c) {
+    const int kh = blockIdx.x % c.Hkv, at = blockIdx.x / c.Hkv;
+    const int b = at / c.blocks, key = at % c.blocks * 256 + threadIdx.x;
+    const pg_seq s = load_seq(c.q_start, c.kv_len, b, c.N, c.max_q, c.max_kv);
+    if (s.ql <= 0 || key >= s.kv)
+        return;
+    const int page = c.page_table[(size_t)b * c.max_pages + key / PG];
+    if (page < 0 || page >= c.num_pages)
+        return;
+    const size_t all = (size_t)c.B * c.Hkv * c.blocks * 256;
+    const float *from = c.parts + ((size_t)b * c.Hkv + kh) * c.blocks * 256 + key;
+    const size_t to = ((size_t)page * c.Hkv + kh) * PG + key % PG;
+    float x = c.prev && key < s.p0 ? c.prev[to] : 0.f;
+    float sum = 0.f;
+    for (int i = 0; i < c.splits; i += 8) { /* loads of 8 at a time */
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            v[j] = from[min(i + j, c.splits - 1) * all];
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            sum += i + j < c.splits ? v[j] : 0.f;
+    }
+    c.w[to] = x + sum;
+}
+static_assert(WEIGH_KG * PG == 256, "a thread a key of a block");
 
 /* ---- positions to keep ------------------------------------------------------------
  * A workgroup per sequence and kv-head. The weights' order is that of 32-bit integers
@@ -488,42 +746,78 @@ template <bool E4M3> __global__ __launch_bounds__(256) void keep_kernel(Keep c) 
 } // namespace CUJEV_KNS
 using namespace CUJEV_KNS;
 
+/* How many rows: splits of a block's, so that the chip has WEIGH_GROUPS workgroups of them
+ * (blocks of a prompt differ in rows: several each even out), of WEIGH_STEPS steps at
+ * least. */
+static int weigh_splits(long long units, int max_q, int G) {
+    const int steps = pg_div_up(max_q, 32 / G);
+    const long long n = pg_min((int)((WEIGH_GROUPS + units - 1) / units), steps / WEIGH_STEPS);
+    return n > 1 ? (int)n : 1;
+}
+extern "C" size_t cujev_kv_weights_ws_bytes(int N, int B, int max_q, int max_kv, int Hq, int Hkv) {
+    const long long mq = pg_min(max_q, N);
+    if (mq <= 0 || B <= 0 || max_kv <= 0 || mq * (Hq / Hkv) <= WEIGH_FEW)
+        return 0;
+    /* of fewer units than WEIGH_GROUPS, splits times units are below twice as many */
+    return (size_t)2 * WEIGH_GROUPS * 256 * sizeof(float);
+}
+
 extern "C" hipError_t k_kv_weights(const bf16_t *q, const float *lse, const cujev_kv_pages *pages,
                                    const cujev_paged_seqs *seqs, int N, int max_q, int max_kv,
-                                   int Hq, const float *prev, float *weights,
-                                   hipStream_t stream) {
+                                   int Hq, const float *prev, float *weights, void *ws,
+                                   size_t ws_bytes, hipStream_t stream) {
     const int Hkv = pages->Hkv, B = seqs->B, G = Hq / Hkv, tiles = pg_div_up(max_kv, PG);
-    if (N <= 0 || B <= 0 || max_q <= 0 || tiles <= 0)
+    const int mq = pg_min(max_q, N);
+    if (B <= 0 || mq <= 0 || tiles <= 0)
         return hipSuccess;
-    /* as many pages a workgroup as leave a workgroup for each CU */
-    int kg = 8;
-    while (kg > 2 && (long long)B * pg_div_up(tiles, kg) * Hkv < 256)
-        kg /= 2;
-    const int blocks = pg_div_up(tiles, kg), per = 8 % Hkv == 0 ? 8 / Hkv : 1;
-    const long long grid = (long long)pg_div_up(blocks, per) * per * Hkv * B;
-    if (grid * 512 > PG_MOST_ITEMS)
+    if ((long long)B * tiles > (1ll << 40) / Hkv) /* tables beyond any memory */
         return hipErrorInvalidValue;
-    const Weigh c = {(const bf16 *)q, lse, pages->k, pages->k_scale, pages->num_pages,
-                     seqs->q_start, seqs->kv_len, seqs->page_table, seqs->max_pages, B, N, max_q,
-                     max_kv, Hq, Hkv, G, pg_div_up(65536, G), blocks, prev, weights};
-#define LAUNCH(T, KG)                                                                             \
-    hipLaunchKernelGGL((weigh_kernel<T, KG>), dim3((unsigned)grid), dim3(512), 0, stream, c)
-    if (pages->type == CUJEV_KV_E4M3) {
-        if (kg == 8)
-            LAUNCH(true, 8);
-        else if (kg == 4)
-            LAUNCH(true, 4);
+    const bool e4m3 = pages->type == CUJEV_KV_E4M3;
+    const long long rows = (long long)mq * G;
+    Weigh c = {(const bf16 *)q, lse, pages->k, pages->k_scale, pages->num_pages,
+               seqs->q_start, seqs->kv_len, seqs->page_table, seqs->max_pages, B, N, max_q,
+               max_kv, Hq, Hkv, G, pg_div_up(65536, G), 0, 1, prev, weights, (float *)ws};
+    if (rows <= WEIGH_FEW) {
+        const long long all = (long long)B * tiles * Hkv;
+        const int pages_each = (int)((all + WEIGH_WAVES - 1) / WEIGH_WAVES);
+        c.blocks = pg_div_up(tiles, 4 * pages_each);
+        const long long grid = (long long)c.blocks * Hkv * B;
+        if (grid * 256 > PG_MOST_ITEMS)
+            return hipErrorInvalidValue;
+        const dim3 g((unsigned)grid), t(256);
+        auto launch = [&](auto ie) {
+            constexpr bool E = decltype(ie)::value;
+            if (rows <= 32)
+                hipLaunchKernelGGL((weigh_few_kernel<E, 1>), g, t, 0, stream, c);
+            else if (rows <= 64)
+                hipLaunchKernelGGL((weigh_few_kernel<E, 2>), g, t, 0, stream, c);
+            else
+                hipLaunchKernelGGL((weigh_few_kernel<E, 4>), g, t, 0, stream, c);
+        };
+        if (e4m3)
+            launch(std::true_type{});
         else
-            LAUNCH(true, 2);
-    } else {
-        if (kg == 8)
-            LAUNCH(false, 8);
-        else if (kg == 4)
-            LAUNCH(false, 4);
-        else
-            LAUNCH(false, 2);
+            launch(std::false_type{});
+        return hipGetLastError();
     }
-#undef LAUNCH
+    c.blocks = pg_div_up(tiles, WEIGH_KG);
+    const long long units = (long long)B * c.blocks * Hkv;
+    if (units * 256 > PG_MOST_ITEMS)
+        return hipErrorInvalidValue;
+    c.splits = units < WEIGH_GROUPS ? weigh_splits(units, mq, G) : 1;
+    if (c.splits > 1 && ws_bytes < (size_t)units * c.splits * 256 * sizeof(float))
+        return hipErrorInvalidValue;
+    const int per = 8 % Hkv == 0 ? 8 / Hkv : 1;
+    const long long grid = (long long)pg_div_up(c.blocks * c.splits, per) * per * Hkv * B;
+    if (grid * 256 > PG_MOST_ITEMS)
+        return hipErrorInvalidValue;
+    const dim3 g((unsigned)grid), t(256);
+    if (e4m3)
+        hipLaunchKernelGGL((weigh_many_kernel<true>), g, t, 0, stream, c);
+    else
+        hipLaunchKernelGGL((weigh_many_kernel<false>), g, t, 0, stream, c);
+    if (c.splits > 1)
+        hipLaunchKernelGGL(weigh_sum_kernel, dim3((unsigned)units), dim3(256), 0, stream, c);
     return hipGetLastError();
 }
 

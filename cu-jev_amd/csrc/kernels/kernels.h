@@ -311,7 +311,10 @@ size_t cujev_attention_paged_ws_bytes(int N, int B, int max_q, int max_kv, int H
  * value where prev is not NULL (it may be weights) and j is before the new tokens. */
 hipError_t k_kv_weights(const bf16_t *q, const float *lse, const cujev_kv_pages *pages,
                         const cujev_paged_seqs *seqs, int N, int max_q, int max_kv, int Hq,
-                        const float *prev, float *weights, hipStream_t stream);
+                        const float *prev, float *weights, void *ws, size_t ws_bytes,
+                        hipStream_t stream);
+/* Enough for that call and every one that is no larger. */
+size_t cujev_kv_weights_ws_bytes(int N, int B, int max_q, int max_kv, int Hq, int Hkv);
 /* keep[b][kv-head][0 .. n - 1], n = keep_len[b] = min(kv_len[b], budget): ascending, the
  * positions of the first `sinks`, the last `recent` and the heaviest of the other keys
  * (equal ones: the lowest; NaN the heaviest; of pages that are not there the lightest). */

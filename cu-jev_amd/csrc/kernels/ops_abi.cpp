@@ -514,7 +514,8 @@ EXPORT int cujev_op_kv_weights(const void *q, const float *lse, int kv_type, con
                                const float *k_scale, int num_pages, const int32_t *q_start,
                                const int32_t *kv_len, const int32_t *page_table, int max_pages,
                                int B, int N, int max_q, int max_kv, int Hq, int Hkv,
-                               const float *prev, float *weights, void *stream) {
+                               const float *prev, float *weights, void *ws, size_t ws_bytes,
+                               void *stream) {
     /* V is not read: K stands in for it in the pool's check */
     const cujev_kv_pages pages = {(void *)k_pages, (void *)k_pages, (float *)k_scale,
                                   (float *)k_scale, num_pages, Hkv, kv_type};
@@ -531,10 +532,20 @@ EXPORT int cujev_op_kv_weights(const void *q, const float *lse, int kv_type, con
         return fail(1, "kv_weights: null argument");
     if (((uintptr_t)q & 15) || (((uintptr_t)lse | (uintptr_t)prev | (uintptr_t)weights) & 3))
         return fail(1, "kv_weights: q must be 16-byte, lse and weights 4-byte aligned");
+    const size_t need = cujev_kv_weights_ws_bytes(N, B, max_q, max_kv, Hq, Hkv);
+    if (need > 0 && (!ws || ((uintptr_t)ws & 3) || ws_bytes < need))
+        return fail(6, "kv_weights: needs a 4-byte aligned workspace of %zu bytes, got %zu", need,
+                    ws ? ws_bytes : (size_t)0);
     const cujev_paged_seqs seqs = {q_start, kv_len, page_table, max_pages, B};
     return launched(k_kv_weights((const bf16_t *)q, lse, &pages, &seqs, N, max_q, max_kv, Hq, prev,
-                                 weights, (hipStream_t)stream),
+                                 weights, ws, ws_bytes, (hipStream_t)stream),
                     "kv_weights");
+}
+
+EXPORT size_t cujev_ops_kv_weights_ws_bytes(int N, int B, int max_q, int max_kv, int Hq, int Hkv) {
+    if (!paged_heads_ok(Hq, Hkv))
+        return 0;
+    return cujev_kv_weights_ws_bytes(N, B, max_q, max_kv, Hq, Hkv);
 }
 
 EXPORT int cujev_op_kv_select(const float *weights, int num_pages, int Hkv,

@@ -20,6 +20,11 @@ constexpr int PD = 256;                /* head dim */
 constexpr int PSLICE = PG * PD;        /* elements of one head's K or V^T in a page */
 
 typedef __attribute__((address_space(3))) void *lds_ptr;
+typedef __attribute__((address_space(3))) const unsigned char lds_u8;
+DEV u32x4 lds_read16(lds_u8 *base, uint32_t off) {
+    return *(__attribute__((address_space(3))) const u32x4 *)(base + off);
+}
+typedef __attribute__((address_space(3))) const float *lds_f32;
 DEV __amdgpu_buffer_rsrc_t make_rsrc(const void *base, uint32_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, (int)bytes, 0x00020000);
 }
@@ -31,6 +36,14 @@ DEV int lane_again() {
     int none = 0;
     asm volatile("" : "+v"(none));
     return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none));
+}
+
+template <int n> using template_int = std::integral_constant<int, n>;
+template <int n, typename F> DEV void unroll_for(F f) {
+    if constexpr (n > 0) {
+        unroll_for<n - 1>(f);
+        f(template_int<n - 1>{});
+    }
 }
 
 DEV pg_seq load_seq(const int32_t *q_start, const int32_t *kv_len, int b, int N, int max_q,

@@ -63,9 +63,9 @@ _SIGS = {
     "cujev_op_attention_paged_tree": [_P, _P, _I, _I, _I, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I,
                                       _I, _I, _I, _I, _I, _P, _I, _P, _P, _P, C.c_size_t, _P],
     # q, lse, kv_type, k, k_scale, num_pages, q_start, kv_len, page_table, max_pages, B, N, max_q,
-    # max_kv, Hq, Hkv, prev, weights, stream
+    # max_kv, Hq, Hkv, prev, weights, ws, ws_bytes, stream
     "cujev_op_kv_weights": [_P, _P, _I, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P,
-                            _P],
+                            _P, C.c_size_t, _P],
     # weights, num_pages, Hkv, page_table, max_pages, kv_len, B, max_kv, budget, sinks, recent,
     # keep, max_keep, keep_len, stream
     "cujev_op_kv_select": [_P, _I, _I, _P, _I, _P, _I, _I, _I, _I, _I, _P, _I, _P, _P],
@@ -115,6 +115,8 @@ def load():
     lib.cujev_ops_attention_ws_bytes.restype = C.c_size_t
     lib.cujev_ops_attention_paged_ws_bytes.argtypes = [_I] * 9
     lib.cujev_ops_attention_paged_ws_bytes.restype = C.c_size_t
+    lib.cujev_ops_kv_weights_ws_bytes.argtypes = [_I] * 6
+    lib.cujev_ops_kv_weights_ws_bytes.restype = C.c_size_t
     lib.cujev_ops_blaslt_version.argtypes = []
     lib.cujev_ops_blaslt_version.restype = _I
     lib.cujev_op_gemm_tune.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, _I, _I, _I, _I,
@@ -133,6 +135,7 @@ def exported_symbols():
     return ["cujev_ops_kv_stride", "cujev_ops_last_error", "cujev_ops_gdn_scratch_bytes",
             "cujev_ops_gemm_small_splits", "cujev_ops_gemm_plan", "cujev_ops_gemm_wide_plan",
             "cujev_ops_attention_ws_bytes", "cujev_ops_attention_paged_ws_bytes",
+            "cujev_ops_kv_weights_ws_bytes",
             "cujev_ops_blaslt_version", "cujev_op_gemm_tune", *_SIGS]
 
 
@@ -503,11 +506,20 @@ def _weights_ok(name, w, pages):
         _need(name, w, torch.float32, pages.device, shape)
 
 
-def kv_weights(q, lse, pages, page_table, q_start, kv_len, max_q, max_kv, weights, prev=None):
+def kv_weights_ws_bytes(N, B, max_q, max_kv, Hq, Hkv) -> int:
+    """Bytes that are enough for this kv_weights call and for every smaller one."""
+    _need_ints("kv_weights_ws_bytes", N, B, max_q, max_kv, Hq, Hkv)
+    return int(load().cujev_ops_kv_weights_ws_bytes(N, B, max_q, max_kv, Hq, Hkv))
+
+
+def kv_weights(q, lse, pages, page_table, q_start, kv_len, max_q, max_kv, weights, prev=None,
+               ws=None):
     """weights [pages, Hkv, 64] (float32, beside the pages' keys) of every key of the
     sequences that have new tokens: prev's, where given and the key is before the new
     tokens, plus what the rows q [N, Hq, 256] of the call gave it, with the lse [N, Hq]
-    of their attention. prev may be weights itself, to add in place; None starts anew."""
+    of their attention. prev may be weights itself, to add in place; None starts anew.
+    ws: uint8 device workspace of kv_weights_ws_bytes, of this call or a larger one; None
+    takes one from torch's allocator where the call needs any."""
     import torch
     dev, B = _paged_seqs(pages, page_table, kv_len, q_start)
     if (max_q | max_kv) >> 31:
@@ -523,11 +535,19 @@ def kv_weights(q, lse, pages, page_table, q_start, kv_len, max_q, max_kv, weight
     _weights_ok("weights", weights, pages)
     if prev is not None and prev is not weights:
         _weights_ok("prev", prev, pages)
+    if ws is None:
+        size = kv_weights_ws_bytes(N, B, max_q, max_kv, Hq, pages.Hkv) if dev >= 0 else 0
+        ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    size = 0 if ws is None else ws.numel()
+    if ws is not None and not (ws.dtype is torch.uint8 and ws.dim() == 1 and
+                               ws.is_contiguous() and ws.get_device() == dev):
+        _need("ws", ws, torch.uint8, dev, (size,))
     kv_type, k, _, k_scale, _, num_pages = pages.args
     _paged_call(dev, "cujev_op_kv_weights", q.data_ptr(), lse.data_ptr(), kv_type, k, k_scale,
                 num_pages, q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(),
                 page_table.shape[1], B, N, max_q, max_kv, Hq, pages.Hkv,
-                None if prev is None else prev.data_ptr(), weights.data_ptr())
+                None if prev is None else prev.data_ptr(), weights.data_ptr(),
+                None if ws is None else ws.data_ptr(), size)
 
 
 def kv_select(weights, page_table, kv_len, max_kv, budget, keep, keep_len, sinks=0, recent=0):

@@ -343,12 +343,16 @@ int cujev_op_attention_paged_tree(const void *q, const void *gate, int gate_tok_
  * attention's lse, what the softmax gave. prev counts for the keys before the new
  * tokens, whose own weights start here; it may be weights itself, or NULL (all start
  * here, as for a whole prompt). A row whose lse is -inf adds nothing. The sum's order
- * depends on the call's sizes alone. Sequences without new tokens are left as they were. */
+ * depends on the call's sizes alone. Sequences without new tokens are left as they were.
+ * ws: device workspace that need not be cleared, 4-byte aligned; calls that may overlap
+ * need one each. cujev_ops_kv_weights_ws_bytes() is enough for the call of its
+ * arguments and every smaller one: 2 MiB, or 0 where max_q (or N) * Hq / Hkv <= 128. */
 int cujev_op_kv_weights(const void *q, const float *lse, int kv_type, const void *k_pages,
                         const float *k_scale, int num_pages, const int32_t *q_start,
                         const int32_t *kv_len, const int32_t *page_table, int max_pages, int B,
                         int N, int max_q, int max_kv, int Hq, int Hkv, const float *prev,
-                        float *weights, void *stream);
+                        float *weights, void *ws, size_t ws_bytes, void *stream);
+size_t cujev_ops_kv_weights_ws_bytes(int N, int B, int max_q, int max_kv, int Hq, int Hkv);
 
 /* The positions to keep of each sequence and kv-head, ascending: keep int32 [B][Hkv]
  * [max_keep] gets n = keep_len[b] = min(kv_len[b], max_kv, budget) of them, the rest of a

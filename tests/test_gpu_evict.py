@@ -141,6 +141,15 @@ def test_weights_past_max_q_and_max_kv(lens, max_q, max_kv):
     check_weights(c, weigh(c, max_q=max_q, max_kv=max_kv), max_q=max_q, max_kv=max_kv)
 
 
+def test_weights_with_a_bound_far_past_the_keys():
+    """Tables of 2^20 columns, for which a wave takes more pages than one."""
+    c = fill(gp.attention_case(636, 8, 4, True, [(2, 700), (1, 130)]), 637)
+    want = weigh(c)
+    wide = [row + [-1] * ((1 << 20) - len(row)) for row in c["tab"]]
+    got = weigh({**c, "tab": wide}, max_kv=1 << 26)
+    assert torch.equal(got, want)
+
+
 def test_weights_repeat_bit_for_bit_on_any_stream():
     c = fill(gp.attention_case(641, 16, 4, True, [(300, 700), (33, 97), (1, 64)]), 642)
     first = weigh(c)

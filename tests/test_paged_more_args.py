@@ -30,7 +30,8 @@ BASE = {
                         tree=FAKE, tree_words=1), "out", lse=None),
     WEIGHTS: dict(q=FAKE, lse=FAKE, kv_type=1, k_pages=FAKE, k_scale=FAKE, num_pages=4,
                   q_start=FAKE, kv_len=FAKE, page_table=FAKE, max_pages=2, B=0, N=0, max_q=1,
-                  max_kv=128, Hq=8, Hkv=2, prev=None, weights=FAKE, stream=None),
+                  max_kv=128, Hq=8, Hkv=2, prev=None, weights=FAKE, ws=None, ws_bytes=0,
+                  stream=None),
     SELECT: dict(weights=FAKE, num_pages=4, Hkv=2, page_table=FAKE, max_pages=2, kv_len=FAKE, B=0,
                  max_kv=128, budget=64, sinks=4, recent=16, keep=FAKE, max_keep=64,
                  keep_len=FAKE + 64, stream=None),
@@ -113,6 +114,14 @@ def test_a_workspace_that_is_too_small_is_refused(name):
 def test_weights_refuse(bad):
     st, msg = call(WEIGHTS, **bad)
     assert st == INVALID and "kv_weights" in msg
+
+
+def test_weights_refuse_a_workspace_that_is_too_small():
+    need = ops.kv_weights_ws_bytes(1000, 1, 1000, 128, 8, 2)
+    assert need > 0 and ops.kv_weights_ws_bytes(1000, 1, 32, 128, 8, 2) == 0
+    for ws, size in ((None, 0), (FAKE, need - 1), (FAKE + 2, need)):
+        st, msg = call(WEIGHTS, N=1000, B=1, max_q=1000, ws=ws, ws_bytes=size)
+        assert st == CAPACITY and "workspace" in msg
 
 
 @pytest.mark.parametrize("bad", [
@@ -204,7 +213,7 @@ def test_bindings_refuse_wrong_tensors():
         WEIGHTS: [dict(lse=z(1, 3)), dict(lse=None), dict(q=z(1, 4, 256)), dict(q=z(4, 256)),
                   dict(weights=z(2, 1, 63)), dict(weights=z(1, 1, 64)), dict(weights=None),
                   dict(prev=z(2, 1, 64).double()), dict(max_kv=2 ** 32), dict(max_q=-1),
-                  dict(kv_len=i32(1, 1)), dict(q_start=i32(0))],
+                  dict(kv_len=i32(1, 1)), dict(q_start=i32(0)), dict(ws=z(8))],
         SELECT: [dict(weights=z(2, 1, 32)), dict(weights=z(2, 64)), dict(weights=z(2, 1, 64).double()),
                  dict(keep=i32(0)), dict(keep=z(1, 2, 1, dtype=torch.int32)),
                  dict(keep_len=i32(0, 0)), dict(kv_len=torch.tensor([1])), dict(page_table=i32(0)),
