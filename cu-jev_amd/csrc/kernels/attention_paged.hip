@@ -139,12 +139,21 @@ DEV int page_id(const Call &c, int b, const pg_tiles &t, int i) {
  * Kinds of their own, so that the first one's code stays what it is. */
 enum { CAUSAL, LSE, TREE };
 /* TREE: the keys k0 .. k0 + 63 that the row with these words sees by its tree, first key
- * lowest: all before the sequence's first new token (at p0), then as the bits say */
+ * lowest: all before the sequence's first new token (at p0), then as the bits say. Both
+ * words are loaded, whichever count: conditional loads came one after the other. */
 DEV uint64_t tree_keys(const uint64_t *row, int words, int k0, int p0) {
     const int at = k0 - p0, i = at >> 6, sh = at & 63; /* i -1: the tile that p0 is in */
-    const uint64_t lo = i < 0 ? ~0ull : i < words ? row[i] : 0;
-    const uint64_t hi = i < -1 ? ~0ull : i + 1 < words ? row[i + 1] : 0;
+    uint64_t lo = row[min(max(i, 0), words - 1)], hi = row[min(max(i + 1, 0), words - 1)];
+    lo = i < 0 ? ~0ull : i < words ? lo : 0;
+    hi = i < -1 ? ~0ull : i + 1 < words ? hi : 0;
     return sh ? lo >> sh | hi << (64 - sh) : lo;
+}
+/* the same of a sequence of up to 64 new tokens, from its row's first word */
+DEV uint64_t tree_keys(uint64_t word, int k0, int p0) {
+    const int at = k0 - p0;
+    return at <= -64 ? ~0ull
+           : at < 0  ? word << -at | ((1ull << -at) - 1)
+                     : at < 64 ? word >> at : 0;
 }
 template <class F> DEV uint64_t each_half(uint64_t x, F f) {
     return (uint64_t)f((uint32_t)(x >> 32)) << 32 | f((uint32_t)x);
@@ -187,7 +196,7 @@ DEV void set_part(const Call &c, Where &w, int target, int have, int share) {
 }
 /* J sequences a lane, 64 J a step: what all have, then where target lies */
 template <int RT_, int J> DEV Where locate_among(const Call &c, int target) {
-    constexpr bool FEWR = RT_ == PG_FEW;
+    constexpr bool FEWR = RT_ != PG_MANY;
     const int lane = threadIdx.x & 63;
     pg_seq s[J];
     int units[J], n[J];
@@ -279,7 +288,7 @@ template <int RT_, int J> DEV Where locate_among(const Call &c, int target) {
     return w;
 }
 template <int RT_> DEV Where locate(const Call &c, int target) {
-    constexpr bool FEWR = RT_ == PG_FEW;
+    constexpr bool FEWR = RT_ != PG_MANY;
     if (c.B > 64)
         return locate_among<RT_, 4>(c, target);
     if (c.B > 1)
@@ -490,8 +499,7 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
                      * high half: some row does. Lane and row are worked out again: kept,
                      * they went to scratch memory. */
                     const int id = lane_again(), of = min(id & 15, rows - 1) * c.rG >> 16;
-                    uint64_t m64 =
-                        tree_keys(c.tree + (size_t)(s.q0 + of) * c.words, c.words, k0, s.p0);
+                    uint64_t m64 = tree_keys(c.tree[(size_t)(s.q0 + of) * c.words], k0, s.p0);
                     const int left = top + 1 - k0; /* keys of the tile, 64 at most count */
                     m64 &= left >= PG ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
                     m64 >>= (E4M3 ? 16 : 8) * (id >> 4);
@@ -649,6 +657,446 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
             }
         }
     }
+}
+
+/* ---- a middling number of rows of a draft tree: units of up to 64 ----------------------
+ * Bound by the K/V bytes as few rows are, but O of 64 rows is four waves' registers. So the
+ * four waves of a workgroup, one a SIMD, share all the rows (RB blocks of 16): wave i
+ * scores the 16 keys i of a tile against them, and after P has gone through LDS takes
+ * dims 64 i .. + 63 of O^T. Each element of a tile is read (and e4m3 widened) once so: with
+ * the rows shared out, by every wave, 64 sequences' 16 tokens on 4096 e4m3 keys took
+ * 119 us. Tiles come to LDS by loads (buffer_load ... lds),
+ * K and V^T in rings of NB buffers each. Per tile three barriers: K of the tile is there
+ * and V^T of the one before read; the waves' maxima are known and K read; P is written and
+ * V^T there. Where a buffer is free its next tile goes out. The line of key tiles is cut
+ * and merged as for few rows. */
+template <bool E4M3, int RB, int RG> struct Mid {
+    static constexpr int T = PSLICE * (E4M3 ? 1 : 2); /* bytes of a K or V^T tile */
+    static constexpr int NB = E4M3 ? 4 : 2;
+    static constexpr int V = NB * T, SK = 2 * NB * T, SV = SK + NB * 256;
+    /* P, rows of 128 bytes; a float of each row and wave */
+    static constexpr int P = SK + (E4M3 ? 2 * NB * 256 : 0), STAT = P + RG * RB * 16 * 128;
+    static constexpr int BYTES = STAT + RG * RB * 16 * 16;
+};
+typedef const __attribute__((address_space(3))) floatx4 *lds_f32x4;
+
+/* The unit on the line that piece `target` begins in */
+DEV Where locate_mid(const Call &c, int target) {
+    const int lane = threadIdx.x & 63;
+    pg_seq s;
+    int n = 0, units = 0; /* of sequence b0 + lane */
+    auto read = [&](int b0) {
+        s = seq_of(c, min(b0 + lane, c.B - 1));
+        units = b0 + lane < c.B ? pg_units(s, c.G, PG_MID) : 0;
+        n = units ? pg_longest(s, c.G, PG_LINE, 0, 0) : 0;
+    };
+    int U = 0, T = 0;
+    for (int b0 = 0; b0 < c.B; b0 += 64) {
+        read(b0);
+        T += units * n;
+        U += units;
+    }
+    T = last_lane(wave_scan(T));
+    U = last_lane(wave_scan(U));
+    Where w;
+    w.b = -1;
+    w.size = pg_few_share(c.plan, U, (unsigned)T);
+    const int item = target * w.size;
+    int before = 0;
+    for (int b0 = 0; b0 < c.B; b0 += 64) {
+        if (c.B > 64)
+            read(b0);
+        const int own = units * n, to = before + wave_scan(own);
+        const uint64_t past = __ballot(to > item);
+        if (past) {
+            const int l = __ffsll((unsigned long long)past) - 1;
+            const int have = __builtin_amdgcn_readlane(to - own, l);
+            w.s = seq_at(s, l);
+            w.b = b0 + l;
+            w.own = __builtin_amdgcn_readlane(n, l);
+            w.unit = (item - have) / w.own;
+            w.begin = have + w.unit * w.own;
+            w.first = w.begin / w.size;
+            w.parts = (w.begin + w.own - 1) / w.size - w.first + 1;
+            w.part = target - w.first;
+            return w;
+        }
+        before = last_lane(to);
+    }
+    return w;
+}
+
+template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned char *smem) {
+    typedef Mid<E4M3, RB, RG> M;
+    constexpr int NW = 4 * RG, NB = M::NB, T = M::T, L = T / (NW * 1024); /* a wave's loads */
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int wq = wave & 3, rg = wave >> 2; /* keys or dims; rows */
+    const int m = lane & 15, g = lane >> 4, kh = blockIdx.x % c.Hkv;
+    lds_u8 *lds = (lds_u8 *)smem;
+    Where w = locate_mid(c, blockIdx.x / c.Hkv);
+    while (w.b >= 0) { /* the units that the piece lies in */
+        const pg_seq s = w.s;
+        /* rows r0 .. r0 + rows - 1: of tokens i_first on, the first from its head `rest` on */
+        const int b = w.b, r0 = w.unit * PG_MID, rows = min(s.ql * c.G - r0, 16 * RB * RG);
+        const int i_first = r0 / c.G, rest = r0 - i_first * c.G;
+        const pg_tiles list = pg_tile_list(s, 0, s.ql - 1, 0, 0);
+        const int cut = (w.first + w.part) * w.size - w.begin;
+        const int i0 = max(cut, 0), ntl = min(min(cut + w.size, w.own), list.ntl) - i0;
+        int ids = ntl > 0 ? page_id(c, b, list, min(i0 + lane, list.ntl - 1)) : -1, ids0 = 0;
+        auto page_of = [&](int t) { /* of tile t from i0 on; past the last, it again */
+            t = min(t, ntl - 1);
+            if (t - ids0 >= 64) {
+                ids0 = t;
+                ids = page_id(c, b, list, min(i0 + t + lane, list.ntl - 1));
+            }
+            return __builtin_amdgcn_readlane(ids, t - ids0);
+        };
+        /* this lane's rows */
+        auto row_of = [&](int rb) { return 16 * (rg * RB + rb) + m; };
+        auto after = [&](int rb) { /* tokens after i_first */
+            return (rest + min(row_of(rb), rows - 1)) * c.rG >> 16;
+        };
+        auto tok_of = [&](int rb) { return i_first + after(rb); };
+        auto head_of = [&](int rb) {
+            return kh * c.G + rest + min(row_of(rb), rows - 1) - after(rb) * c.G;
+        };
+        bf16x8 qf[RB][8];
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++) {
+            const bf16 *qp = c.q + ((size_t)(s.q0 + tok_of(rb)) * c.Hq + head_of(rb)) * PD;
+#pragma unroll
+            for (int ks = 0; ks < 8; ks++) /* dims as K's pieces below */
+                qf[rb][ks] = *(const bf16x8 *)(qp + (E4M3 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1)
+                                                          : 32 * ks + 8 * g));
+        }
+        /* the tree's words of this lane's rows, and of all the unit's tokens together: the first
+         * ones, all there are of up to 64 new tokens */
+        const int i_last = i_first + ((rest + rows - 1) * c.rG >> 16);
+        auto row_words = [&](int tok) { return c.tree + (size_t)(s.q0 + tok) * c.words; };
+        uint64_t word[RB], any_word = *row_words(min(i_first + lane, i_last));
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++)
+            word[rb] = *row_words(tok_of(rb));
+        /* Tiles: KiB j NW + wave of a tile is a wave's load j, 2 K rows or 8 V^T rows (e4m3
+         * 4 and 16). Pieces of 16 bytes are swizzled, in the address, so that 16 lanes'
+         * operands hit 16 bank groups: K's piece p of key k in slot p ^ (k & 15), V^T's of
+         * row d in p ^ (d / 2 & 7) (e4m3 d / 4 & 3), P's of row r in p ^ (r / 2 & 7). */
+        auto slice = [&](int page) { return (size_t)max(page, 0) * c.Hkv + kh; };
+        auto issue_k = [&](int t, int page) {
+            const __amdgpu_buffer_rsrc_t src = make_rsrc((const char *)c.k + slice(page) * T, T);
+#pragma unroll
+            for (int j = 0; j < L; j++) {
+                const int kib = j * NW + wave, key = E4M3 ? 4 * kib + g : 2 * kib + (lane >> 5);
+                const uint32_t off = E4M3 ? g * 256 + ((m ^ (key & 15)) << 4)
+                                          : (lane >> 5) * 512 + (((lane & 31) ^ (key & 15)) << 4);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    src, (lds_ptr)(smem + t % NB * T + kib * 1024), 16, off, kib * 1024, 0, 0);
+            }
+            if (E4M3 && wave < 2) /* both operands' scales: V's multiply p */
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    make_rsrc((wave ? c.vs : c.ks) + slice(page) * PG, 256),
+                    (lds_ptr)(smem + (wave ? M::SV : M::SK) + t % NB * 256), 4, lane * 4, 0, 0, 0);
+        };
+        auto issue_v = [&](int t, int page) {
+            const __amdgpu_buffer_rsrc_t src = make_rsrc((const char *)c.vt + slice(page) * T, T);
+#pragma unroll
+            for (int j = 0; j < L; j++) {
+                const int kib = j * NW + wave;
+                const int d = E4M3 ? 16 * kib + (lane >> 2) : 8 * kib + (lane >> 3);
+                const uint32_t off = E4M3 ? (lane >> 2) * 64 + (((lane & 3) ^ (d >> 2 & 3)) << 4)
+                                          : (lane >> 3) * 128 + (((lane & 7) ^ (d >> 1 & 7)) << 4);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    src, (lds_ptr)(smem + M::V + t % NB * T + kib * 1024), 16, off, kib * 1024, 0,
+                    0);
+            }
+        };
+        /* all but the newest `nk` of K's groups of loads and `nv` of V^T's are there, and all
+         * waves as far; what is issued past the last tile keeps the count */
+        auto meet = [&](auto nk, auto nv) {
+            constexpr int n = (decltype(nk)::value + decltype(nv)::value) * L;
+            if (E4M3 && wave < 2)
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(n + decltype(nk)::value)
+                             : "memory");
+            else
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(n) : "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        };
+        const uint32_t ka = (16 * wq + m) * (T / PG) + ((g ^ m) << 4);
+        const uint32_t va = M::V + (64 * wq + m) * (T / PD) +
+                            ((E4M3 ? g ^ (m >> 2) : g ^ (m >> 1)) << 4);
+        /* P of row m of a block: written 4 keys, 16 wq + 4 g on, read 8 at a time */
+        const uint32_t pw = M::P + (rg * RB * 16 + m) * 128 + (((2 * wq + (g >> 1)) ^ (m >> 1)) << 4) +
+                            (g & 1) * 8;
+        const uint32_t pr = M::P + (rg * RB * 16 + m) * 128;
+        const uint32_t stat = M::STAT + (rg * RB * 16 + m) * 16;
+
+        floatx4 o[RB][4]; /* dims 64 wq + 16 t + 4 g .. + 3 of row m of block rb */
+        float mrun[RB], lrun[RB];
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++) {
+            mrun[rb] = -INFINITY, lrun[rb] = 0.f;
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+                o[rb][t] = floatx4{};
+        }
+        int pg[NB + 1]; /* pages of tiles i .. i + NB */
+        if (ntl > 0) {
+#pragma unroll
+            for (int t = 0; t <= NB; t++)
+                pg[t] = page_of(t);
+#pragma unroll
+            for (int t = 0; t < NB; t++) { /* V^T of the last one: before the first scores */
+                issue_k(t, pg[t]);
+                if (t < NB - 1)
+                    issue_v(t, pg[t]);
+            }
+            /* Q is waited for here, where what was issued after it is known: in the loop the
+             * compiler would wait for tiles of the next round with it */
+#pragma unroll
+            for (int rb = 0; rb < RB; rb++) {
+                asm volatile("" : "+v"(word[rb]));
+#pragma unroll
+                for (int ks = 0; ks < 8; ks++)
+                    asm volatile("" : "+v"(qf[rb][ks]));
+            }
+            any_word = or_wave(any_word);
+        }
+        for (int i = 0; i < ntl; i++) {
+            const bool there = pg[0] >= 0;
+            const int k0 = pg_tile_page(list, i0 + i) * PG;
+            meet(template_int<NB - 1>{}, template_int<NB - 1>{});
+            issue_v(i + NB - 1, pg[NB - 1]);
+            floatx4 x[RB], vsc; /* vsc: e4m3, V's scales of the lane's keys */
+            const bool foreign =
+                !there || !pg_tile_whole(k0, s.p0 - 1, s.p0 + s.ql - 1, s.kv, 0, 0);
+            const int left = there ? s.kv - k0 : 0; /* keys of the tile, 64 at most count */
+            const uint64_t live = left >= PG ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
+            uint64_t any = ~0ull; /* keys that some row sees */
+            if (foreign)
+                any = live & (s.ql <= 64 ? tree_keys(any_word, k0, s.p0)
+                                         : or_wave(tree_keys(row_words(min(i_first + lane, i_last)),
+                                                             c.words, k0, s.p0)));
+            {
+                const uint32_t kbuf = i % NB * T + ka;
+                const float ksc =
+                    E4M3 ? *(lds_f32)(lds + M::SK + i % NB * 256 + (16 * wq + m) * 4) : 1.f;
+                if constexpr (E4M3)
+                    vsc = *(lds_f32x4)(lds + M::SV + i % NB * 256 + (16 * wq + 4 * g) * 4);
+#pragma unroll
+                for (int j = 0; j < (E4M3 ? 4 : 8); j++) {
+                    const u32x4 v = lds_read16(lds, (kbuf ^ ((j & 3) << 6)) + (j >> 2) * 256);
+#pragma unroll
+                    for (int rb = 0; rb < RB; rb++) {
+                        const floatx4 in = j ? x[rb] : floatx4{};
+                        if constexpr (E4M3) {
+                            x[rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                widen(v[0], v[1], ksc), qf[rb][2 * j], in, 0, 0, 0);
+                            x[rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                widen(v[2], v[3], ksc), qf[rb][2 * j + 1], x[rb], 0, 0, 0);
+                        } else {
+                            x[rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                __builtin_bit_cast(bf16x8, v), qf[rb][j], in, 0, 0, 0);
+                        }
+                    }
+                }
+                if (foreign) {
+                    if constexpr (E4M3) { /* scales of no key of the call: any bits */
+                        const uint32_t some = (uint32_t)(any >> (16 * wq + 4 * g));
+#pragma unroll
+                        for (int v = 0; v < 4; v++)
+                            vsc[v] = some >> v & 1 ? vsc[v] : 0.f;
+                    }
+#pragma unroll
+                    for (int rb = 0; rb < RB; rb++) {
+                        const uint64_t own =
+                            s.ql <= 64 ? tree_keys(word[rb], k0, s.p0)
+                                       : tree_keys(row_words(tok_of(rb)), c.words, k0, s.p0);
+                        const uint32_t bits = (uint32_t)((own & live) >> (16 * wq + 4 * g));
+                        unroll_for<4>([&](auto iv) {
+                            constexpr int v = decltype(iv)::value;
+                            x[rb][v] = hide_by<v>(bits, x[rb][v]);
+                        });
+                    }
+                }
+#pragma unroll
+                for (int rb = 0; rb < RB; rb++) {
+                    float mx = fmaxf(fmaxf(x[rb][0], x[rb][1]), fmaxf(x[rb][2], x[rb][3]));
+                    mx = fold_rows(mx, [](float a, float e) { return fmaxf(a, e); });
+                    if (g == 0)
+                        *(float *)(smem + stat + rb * 256 + wq * 4) = mx;
+                }
+            }
+            lds_barrier();
+            issue_k(i + NB, pg[NB]);
+            {
+#pragma unroll
+                for (int rb = 0; rb < RB; rb++) {
+                    const floatx4 all = *(lds_f32x4)(lds + stat + rb * 256);
+                    const float mnew = fmaxf(fmaxf(fmaxf(all[0], all[1]), fmaxf(all[2], all[3])),
+                                             mrun[rb]);
+                    const float ref = mnew == -INFINITY ? 0.f : mnew; /* no key yet: p = 0 */
+                    if (__any(mnew != mrun[rb])) {
+                        const float a = fast_exp2(mrun[rb] - ref);
+                        lrun[rb] *= a;
+#pragma unroll
+                        for (int t = 0; t < 4; t++)
+                            o[rb][t] *= a;
+                    }
+                    mrun[rb] = mnew;
+#pragma unroll
+                    for (int v = 0; v < 4; v++)
+                        x[rb][v] = fast_exp2(x[rb][v] - ref);
+                    lrun[rb] += (x[rb][0] + x[rb][1]) + (x[rb][2] + x[rb][3]);
+                    if constexpr (E4M3)
+                        x[rb] *= vsc;
+                    const bf16x4 p = {f2bf(x[rb][0]), f2bf(x[rb][1]), f2bf(x[rb][2]),
+                                      f2bf(x[rb][3])};
+                    *(bf16x4 *)(smem + pw + rb * 2048) = p;
+                }
+            }
+            meet(template_int<NB>{}, template_int<NB - 1>{});
+            {
+                const uint32_t vbuf = i % NB * T + va;
+                bf16x8 p[RB][2];
+#pragma unroll
+                for (int rb = 0; rb < RB; rb++)
+#pragma unroll
+                    for (int st = 0; st < 2; st++) /* keys 32 st + 8 g on (e4m3 16 g + 8 st) */
+                        p[rb][st] = __builtin_bit_cast(
+                            bf16x8, lds_read16(lds, pr + rb * 2048 +
+                                                        (((E4M3 ? 2 * g + st : 4 * st + g) ^
+                                                          (m >> 1))
+                                                         << 4)));
+                u32x4 keep[2]; /* bits to keep of V^T: of keys of the call */
+                if (foreign) {
+                    const uint32_t a = (uint32_t)(any >> ((E4M3 ? 16 : 8) * g));
+                    const uint32_t e = (uint32_t)(any >> 32 >> (8 * g));
+#pragma unroll
+                    for (int d = 0; d < 4; d++) {
+                        auto two = [&](uint32_t x2) {
+                            return ((x2 >> (2 * d) & 1) ? 0xffffu : 0u) |
+                                   ((x2 >> (2 * d + 1) & 1) ? 0xffff0000u : 0u);
+                        };
+                        keep[0][d] = E4M3 ? bytes_by(a >> (4 * d)) : two(a);
+                        keep[1][d] = two(e);
+                    }
+                }
+                auto products = [&](auto masked) {
+#pragma unroll
+                    for (int t = 0; t < 4; t++) {
+                        bf16x8 v[2];
+                        if constexpr (E4M3) {
+                            u32x4 raw = lds_read16(lds, vbuf + t * 1024);
+                            if constexpr (decltype(masked)::value)
+                                raw &= keep[0];
+                            v[0] = widen(raw[0], raw[1], 1.f), v[1] = widen(raw[2], raw[3], 1.f);
+                        } else {
+#pragma unroll
+                            for (int st = 0; st < 2; st++) {
+                                u32x4 raw = lds_read16(lds, (vbuf ^ (st << 6)) + t * 2048);
+                                if constexpr (decltype(masked)::value)
+                                    raw &= keep[st];
+                                v[st] = __builtin_bit_cast(bf16x8, raw);
+                            }
+                        }
+#pragma unroll
+                        for (int rb = 0; rb < RB; rb++)
+#pragma unroll
+                            for (int st = 0; st < 2; st++)
+                                o[rb][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                    v[st], p[rb][st], o[rb][t], 0, 0, 0);
+                    }
+                };
+                if (foreign)
+                    products(std::true_type{});
+                else
+                    products(std::false_type{});
+            }
+#pragma unroll
+            for (int t = 0; t < NB; t++)
+                pg[t] = pg[t + 1];
+            pg[NB] = page_of(i + 1 + NB);
+        }
+        /* nothing is on its way, and all have read */
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++) { /* l of a row from the four waves' keys */
+            const float l = fold_rows(lrun[rb], [](float a, float e) { return a + e; });
+            if (g == 0)
+                *(float *)(smem + stat + rb * 256 + wq * 4) = l;
+        }
+        lds_barrier();
+        if (w.part == 0 && kh == 0 && c.plan.slots > 0 && threadIdx.x == 0)
+            ((int2 *)c.info)[b * (c.plan.units / c.B) + w.unit] = int2{w.first, w.parts};
+        const size_t slot = slot_of(c, kh, pg_few_slot(w.first, w.part)) * c.plan.rt;
+        const int d0 = 64 * wq + 4 * g;
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++) {
+            const floatx4 all = *(lds_f32x4)(lds + stat + rb * 256);
+            const float l = (all[0] + all[1]) + (all[2] + all[3]);
+            const int r = row_of(rb);
+            if (r >= rows)
+                continue;
+            if (w.parts > 1) {
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+                    *(floatx4 *)(c.po + (slot + r) * PD + d0 + 16 * t) = o[rb][t];
+                if (d0 == 0) {
+                    c.pl[slot + r] = l;
+                    c.pmu[slot + r] = mrun[rb] == -INFINITY ? 0.f : mrun[rb];
+                }
+                continue;
+            }
+            const float inv = l > 0.f ? 1.f / l : 0.f;
+            const int n = s.q0 + tok_of(rb), head = head_of(rb);
+            if (c.lse && d0 == 0)
+                c.lse[(size_t)n * c.Hq + head] = lse_of(l, mrun[rb]);
+            bf16x4 gv[4] = {};
+            if (c.gate) {
+                const bf16 *gp = c.gate + (size_t)n * c.gts + (size_t)head * c.ghs + d0;
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+                    gv[t] = *(const bf16x4 *)(gp + 16 * t);
+            }
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                bf16x4 res;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    res[e] = f2bf(o[rb][t][e] * inv * (c.gate ? sigmoid_f(bf2f(gv[t][e])) : 1.f));
+                *(bf16x4 *)(c.out + ((size_t)n * c.Hq + head) * PD + d0 + 16 * t) = res;
+            }
+        }
+        /* on to the next unit, if the piece goes on after this one */
+        const bool more = cut + w.size > w.own;
+        w.begin += w.own, w.first = w.begin / w.size, w.part = 0;
+        if (more && w.unit + 1 < pg_units(s, c.G, PG_MID)) {
+            w.unit++;
+        } else {
+            w.unit = 0, w.b = -1;
+            for (int b0 = more ? b + 1 : c.B; b0 < c.B; b0 += 64) {
+                const pg_seq t = seq_of(c, min(b0 + lane, c.B - 1));
+                const uint64_t any = __ballot(b0 + lane < c.B && t.ql > 0);
+                if (any) {
+                    const int l = __ffsll((unsigned long long)any) - 1;
+                    w.s = seq_at(t, l);
+                    w.b = b0 + l;
+                    w.own = pg_longest(w.s, c.G, PG_LINE, 0, 0);
+                    break;
+                }
+            }
+        }
+        w.parts = (w.begin + w.own - 1) / w.size - w.first + 1;
+    }
+}
+template <bool E4M3, int RB, int RG>
+__global__ __launch_bounds__(256 * RG) void attention_mid_kernel(Call c) {
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[Mid<E4M3, RB, RG>::BYTES];
+    static_assert(sizeof(smem) <= 163840, "LDS of a CU");
+    attend_mid<E4M3, RB, RG>(c, smem);
 }
 
 /* ---- many rows: tiles of 128 packed rows -----------------------------------------
@@ -1370,21 +1818,24 @@ __global__ __launch_bounds__(512, 2) void attention_many_kernel(Call c) {
  * dims, o 64 parts at a time, 4 a load. That is for few rows after many keys (4 rows
  * of 64 parts: 5.4 us, and 8.8 a wave per row); the starts of many workgroups cost
  * more than it gains (1024 rows of 4 parts: 5.6 and 4.8, 4096 of them 22 and 8). */
-template <bool ROW, bool STATS>
+template <bool ROW, bool STATS, int RU = PG_FEW>
 __global__ __launch_bounds__(256) void merge_few_kernel(Call c, int groups) {
     constexpr int STEP = ROW ? 64 : 16, PER = STEP / 16;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int group = blockIdx.x % groups, kh = blockIdx.x / groups % c.Hkv;
-    const int b = blockIdx.x / groups / c.Hkv, r = ROW ? group : group * 4 + wave;
+    const int u = blockIdx.x / groups / c.Hkv, r = ROW ? group : group * 4 + wave;
+    /* RU rows a unit: of few rows a sequence is one */
+    const int per = RU == FEW ? 1 : c.plan.units / c.B, b = u / per, r0 = (u - b * per) * RU;
     const pg_seq s = seq_of(c, b);
-    const int2 info = ((const int2 *)c.info)[b]; /* of a sequence with rows */
-    if (r >= s.ql * c.G || info.y <= 1)
+    const int2 info = ((const int2 *)c.info)[u]; /* of a unit with rows */
+    if (r0 + r >= s.ql * c.G || info.y <= 1)
         return;
     const int first = info.x, parts = info.y;
     const size_t slot0 = slot_of(c, kh, 0);
-    auto at = [&](int j) { return (slot0 + pg_few_slot(first, j)) * FEW + r; };
+    auto at = [&](int j) { return (slot0 + pg_few_slot(first, j)) * RU + r; };
     const int dim = ROW ? 64 * wave + 4 * (lane & 15) : 4 * lane, own = ROW ? lane >> 4 : 0;
-    const int tok = r * c.rG >> 16, n = s.q0 + tok, head = kh * c.G + r - tok * c.G;
+    const int tok = RU == FEW ? r * c.rG >> 16 : (r0 + r) / c.G;
+    const int n = s.q0 + tok, head = kh * c.G + r0 + r - tok * c.G;
     bf16x4 gv = {};
     if (c.gate)
         gv = *(const bf16x4 *)(c.gate + (size_t)n * c.gts + (size_t)head * c.ghs + dim);
@@ -1534,6 +1985,53 @@ extern "C" size_t cujev_attention_paged_ws_bytes(int N, int B, int max_q, int ma
     return pg_ws_most(N, B, max_q, max_kv, Hq / Hkv, Hkv);
 }
 
+/* The workspace, from c.po on: o, l and mu of the plan's slots, then info */
+static void set_workspace(Call &c, int Hkv) {
+    const size_t rows = (size_t)c.plan.slots * Hkv * c.plan.rt;
+    c.pl = c.po + rows * PD, c.pmu = c.pl + rows, c.info = (int32_t *)(c.pmu + rows);
+}
+
+/* Draft trees of a middling number of rows */
+static hipError_t attend_middling(Call c, int Hkv, bool e4m3, size_t ws_bytes,
+                                  hipStream_t stream) {
+    const pg_plan p = c.plan = pg_make_mid_plan(c.N, c.B, c.max_q, c.max_kv, c.G, Hkv);
+    if (p.shares == 0)
+        return hipSuccess;
+    if (p.shares < 0 || pg_mid_ws_bytes(p, Hkv) > ws_bytes)
+        return hipErrorInvalidValue;
+    set_workspace(c, Hkv);
+    const dim3 grid((unsigned)(p.shares * Hkv));
+    auto attend = [&](auto ie, auto ig) {
+        constexpr int RG = decltype(ig)::value;
+        hipLaunchKernelGGL((attention_mid_kernel<decltype(ie)::value, 2, RG>), grid,
+                           dim3(256 * RG), 0, stream, c);
+    };
+    auto by_rows = [&](auto ie) {
+        if ((long long)pg_min(c.max_q, c.N) * c.G <= 32)
+            attend(ie, template_int<1>{});
+        else
+            attend(ie, template_int<2>{});
+    };
+    if (e4m3)
+        by_rows(std::true_type{});
+    else
+        by_rows(std::false_type{});
+    if (p.slots > 0) {
+        const bool row = pg_mid_by_row(p, Hkv);
+        const int groups = row ? PG_MID : PG_MID / 4;
+        const dim3 mgrid((unsigned)(pg_mid_merge_items(p, Hkv) / 256));
+        auto merge = [&](auto ir) {
+            hipLaunchKernelGGL((merge_few_kernel<decltype(ir)::value, true, PG_MID>), mgrid,
+                               dim3(256), 0, stream, c, groups);
+        };
+        if (row)
+            merge(std::true_type{});
+        else
+            merge(std::false_type{});
+    }
+    return hipGetLastError();
+}
+
 extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int gate_tok_stride,
                                         int gate_head_stride, const cujev_kv_pages *pages,
                                         const cujev_paged_seqs *seqs, int N, int max_q, int max_kv,
@@ -1542,22 +2040,21 @@ extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int
                                         size_t ws_bytes, hipStream_t stream) {
     const int Hkv = pages->Hkv, B = seqs->B, G = Hq / Hkv;
     const bool e4m3 = pages->type == CUJEV_KV_E4M3;
-    const pg_plan p = pg_make_plan(N, B, max_q, max_kv, G, Hkv, window, sinks);
+    const bool all = window >= max_kv; /* keys of a row, but behind max_kv */
+    Call c = {(const bf16 *)q, (const bf16 *)gate, gate_tok_stride, gate_head_stride,
+              pages->k, pages->vt, pages->k_scale, pages->v_scale, pages->num_pages,
+              seqs->q_start, seqs->kv_len, seqs->page_table, seqs->max_pages, B, N,
+              max_q, max_kv, Hq, Hkv, G, window, sinks,
+              all ? 0 : window, all ? 0 : sinks, pg_div_up(65536, G), tree, tree_words, lse,
+              (bf16 *)out, (float *)ws, nullptr, nullptr, nullptr, {}};
+    if (tree && pg_is_mid(N, B, max_q, max_kv, G, Hkv))
+        return attend_middling(c, Hkv, e4m3, ws_bytes, stream);
+    const pg_plan p = c.plan = pg_make_plan(N, B, max_q, max_kv, G, Hkv, window, sinks);
     if (p.shares == 0)
         return hipSuccess;
-    if (p.shares < 0)
+    if (p.shares < 0 || pg_ws_bytes(p, Hkv) > ws_bytes)
         return hipErrorInvalidValue;
-    const size_t rows = (size_t)p.slots * Hkv * p.rt;
-    if (pg_ws_bytes(p, Hkv) > ws_bytes)
-        return hipErrorInvalidValue;
-    const bool all = window >= max_kv; /* keys of a row, but behind max_kv */
-    const Call c = {(const bf16 *)q, (const bf16 *)gate, gate_tok_stride, gate_head_stride,
-                    pages->k, pages->vt, pages->k_scale, pages->v_scale, pages->num_pages,
-                    seqs->q_start, seqs->kv_len, seqs->page_table, seqs->max_pages, B, N,
-                    max_q, max_kv, Hq, Hkv, G, window, sinks,
-                    all ? 0 : window, all ? 0 : sinks, pg_div_up(65536, G), tree, tree_words, lse,
-                    (bf16 *)out, (float *)ws, (float *)ws + rows * PD,
-                    (float *)ws + rows * (PD + 1), (int32_t *)((float *)ws + rows * (PD + 2)), p};
+    set_workspace(c, Hkv);
     const bool few = p.rt == FEW;
     const int per = !few && 8 % Hkv == 0 ? 8 / Hkv : 1;
     const dim3 grid((unsigned)(pg_div_up(p.shares, per) * per * Hkv)); /* all parts */

@@ -443,8 +443,11 @@ static int attend_paged(const char *what, const void *q, const void *gate, int g
         return fail(1, "%s: a tree of up to %d new tokens a sequence needs %d words a row and no "
                        "window, got %d and window=%d",
                     what, pg_min(max_q, N), pg_div_up(pg_min(max_q, N), 64), tree_words, window);
+    const int G = Hq / Hkv;
     const size_t need =
-        pg_ws_bytes(pg_make_plan(N, B, max_q, max_kv, Hq / Hkv, Hkv, window, sinks), Hkv);
+        tree && pg_is_mid(N, B, max_q, max_kv, G, Hkv)
+            ? pg_mid_ws_bytes(pg_make_mid_plan(N, B, max_q, max_kv, G, Hkv), Hkv)
+            : pg_ws_bytes(pg_make_plan(N, B, max_q, max_kv, G, Hkv, window, sinks), Hkv);
     if (need > 0 && (!ws || ((uintptr_t)ws & 15) || ws_bytes < need))
         return fail(6, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", what,
                     need, ws ? ws_bytes : (size_t)0);

@@ -249,12 +249,62 @@ constexpr pg_plan pg_make_plan(int N, int B, int max_q, int max_kv, int G, int H
     return p;
 }
 
+/* ---- draft trees of a middling number of rows, or of few keys ------------------------
+ * A unit is PG_MID packed rows of a sequence and kv-head. The units' key tiles, unit after
+ * unit, are one line in pieces, as for few rows, a workgroup each: one a CU. */
+constexpr int PG_MID = 64, PG_LINE = 1 << 20; /* PG_LINE: "rows" of a unit of them all */
+constexpr int PG_MID_CHIP = 256; /* workgroups of all kv-heads: with two slots each 34 MB */
+constexpr long long pg_mid_units(int N, int B, int max_q, int G) {
+    return B * (((long long)pg_min(max_q, N) * G + PG_MID - 1) / PG_MID);
+}
+/* More rows than PG_MID go to tiles of PG_MANY, which read each key once for twice as
+ * many, unless there is little to do: up to this many tiles of PG_MID rows and kv-heads */
+constexpr long long PG_MID_LITTLE = 1024;
+constexpr bool pg_is_mid(int N, int B, int max_q, int max_kv, int G, int Hkv) {
+    const long long rows = (long long)pg_min(max_q, N) * G, units = pg_mid_units(N, B, max_q, G);
+    return rows > PG_FEW && Hkv <= PG_MID_CHIP &&
+           (rows <= PG_MID ||
+            (units <= PG_MID_LITTLE && units * pg_div_up(max_kv, PG) * Hkv <= PG_MID_LITTLE));
+}
+constexpr int pg_mid_goal(long long units, int Hkv) {
+    const int chip = PG_MID_CHIP / Hkv;
+    return 64 * units < chip ? (int)(64 * units) : chip;
+}
+/* The merge: a workgroup a row of few, or a wave */
+constexpr bool pg_mid_by_row(const pg_plan &p, int Hkv) {
+    return (long long)p.units * PG_MID * Hkv <= 512;
+}
+constexpr long long pg_mid_merge_items(const pg_plan &p, int Hkv) {
+    return 256ll * p.units * Hkv * (pg_mid_by_row(p, Hkv) ? PG_MID : PG_MID / 4);
+}
+constexpr pg_plan pg_make_mid_plan(int N, int B, int max_q, int max_kv, int G, int Hkv) {
+    pg_plan p{};
+    if (pg_min(max_q, N) <= 0 || B <= 0)
+        return p;
+    p.rt = PG_MID;
+    const long long most = pg_max(pg_div_up(max_kv, PG), 1), units = pg_mid_units(N, B, max_q, G);
+    if (units * Hkv > PG_MOST_UNITS) {
+        p.shares = -1;
+        return p;
+    }
+    p.goal = pg_mid_goal(units, Hkv);
+    p.units = (int)units;
+    p.shares = pg_few_pieces(units, most, p.goal);
+    p.slots = most > 1 ? 2 * p.shares : 0;
+    if (p.slots > 0 && pg_mid_merge_items(p, Hkv) > PG_MOST_ITEMS)
+        p.shares = -1;
+    return p;
+}
+
 /* ---- workspace -------------------------------------------------------------------
  * o (256), l and mu of the slots' rows as floats, then info: {int, int} a unit, or 4
  * ints a slot. */
 constexpr size_t pg_slot_bytes(int slots, int rt, int Hkv, int infos, int info_bytes) {
     return slots <= 0 ? 0
                       : (size_t)slots * Hkv * rt * (256 + 2) * 4 + (size_t)infos * info_bytes;
+}
+constexpr size_t pg_mid_ws_bytes(const pg_plan &p, int Hkv) {
+    return pg_slot_bytes(p.slots, p.rt, Hkv, p.units, 8);
 }
 constexpr size_t pg_ws_bytes(const pg_plan &p, int Hkv) {
     return p.rt == PG_FEW ? pg_slot_bytes(p.slots, p.rt, Hkv, p.units, 8)
@@ -274,7 +324,14 @@ constexpr size_t pg_ws_most(int N, int B, int max_q, int max_kv, int G, int Hkv)
     const size_t few = pg_slot_bytes(most > 1 ? 2 * pieces : 0, PG_FEW, Hkv, units, 8);
     const int goal = mq * G > PG_FEW && pg_many_long(most) ? pg_many_goal(Hkv) : 0;
     const size_t many = pg_slot_bytes(goal, PG_MANY, Hkv, goal, 16);
-    return few > many ? few : many;
+    size_t mid = 0;
+    if (mq * G > PG_FEW && most > 1 && Hkv <= PG_MID_CHIP) {
+        const long long all = pg_mid_units(N, units, max_q, G);
+        const int m = (int)(all < units ? all : units > PG_MID_LITTLE ? units
+                            : all < PG_MID_LITTLE ? all : PG_MID_LITTLE);
+        mid = pg_slot_bytes(2 * pg_few_pieces(m, most, pg_mid_goal(m, Hkv)), PG_MID, Hkv, m, 8);
+    }
+    return few > many ? (few > mid ? few : mid) : (many > mid ? many : mid);
 }
 
 /* The row at position p sees the keys j <= min(p, kv - 1) with j > pg_low or j <
