@@ -690,17 +690,15 @@ DEV Where locate_mid(const Call &c, int target) {
         units = b0 + lane < c.B ? pg_units(s, c.G, PG_MID) : 0;
         n = units ? pg_longest(s, c.G, PG_LINE, 0, 0) : 0;
     };
-    int U = 0, T = 0;
+    int T = 0;
     for (int b0 = 0; b0 < c.B; b0 += 64) {
         read(b0);
         T += units * n;
-        U += units;
     }
     T = last_lane(wave_scan(T));
-    U = last_lane(wave_scan(U));
     Where w;
     w.b = -1;
-    w.size = pg_few_share(c.plan, U, (unsigned)T);
+    w.size = pg_mid_share(c.plan, (unsigned)T);
     const int item = target * w.size;
     int before = 0;
     for (int b0 = 0; b0 < c.B; b0 += 64) {

@@ -473,7 +473,8 @@ static_assert(WEIGH_KG * PG == 256, "a thread a key of a block");
  * A workgroup per sequence and kv-head. The weights' order is that of 32-bit integers
  * (ordered()); the least one kept is found by its digits of 11, 11 and 10 bits from the
  * top, each by a histogram in LDS of what has the digits before. Then positions are
- * counted in order: heavier ones, and of its equals the first. */
+ * counted in order: heavier ones, and of its equals the first. A chain of loads, LDS and
+ * barriers: 1 x 8192 keys 13 us, 64 sequences of up to 4096, a workgroup a CU, 11. */
 constexpr int SEL_T = 1024;
 struct Select {
     const float *w;
@@ -514,10 +515,13 @@ DEV int block_scan(int v, int *scratch, int *total) {
     return before + to - v;
 }
 
-/* E weights a thread in registers, or E 0: read again each time */
+/* E tiles of SEL_T positions at a time, a thread's weights in registers: all there are, or
+ * read again for each pass over them */
 template <int E> __global__ __launch_bounds__(SEL_T) void select_kernel(Select c) {
-    __shared__ int hist[2048], scratch[SEL_T / 64], found[2];
-    const int tid = threadIdx.x, lane = tid & 63, kh = blockIdx.x % c.Hkv, b = blockIdx.x / c.Hkv;
+    constexpr int SPAN = E * SEL_T, WAVES = SEL_T / 64;
+    __shared__ int hist[2048], scratch[WAVES], found[3], counts[E * WAVES];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int kh = blockIdx.x % c.Hkv, b = blockIdx.x / c.Hkv;
     const int kv = min(max(c.kv_len[b], 0), c.max_kv), n = min(kv, c.budget);
     int32_t *keep = c.keep + (size_t)blockIdx.x * c.max_keep;
     if (kh == 0 && tid == 0)
@@ -529,46 +533,44 @@ template <int E> __global__ __launch_bounds__(SEL_T) void select_kernel(Select c
     }
     const int lo = c.sinks, hi = kv - c.recent; /* the positions to choose among */
     const int want = n - c.sinks - c.recent;
-    auto weight = [&](int j) -> uint32_t {
-        const int page = c.page_table[(size_t)b * c.max_pages + j / PG];
-        return page >= 0 && page < c.num_pages
-                   ? ordered(c.w[((size_t)page * c.Hkv + kh) * PG + j % PG])
-                   : 0u;
-    };
-    const int tiles = E ? E : pg_div_up(kv, SEL_T);
-    uint32_t u[E ? E : 1];
-    if constexpr (E > 0) {
+    uint32_t u[E];
+    auto load = [&](int from) {
+        int page[E];
 #pragma unroll
-        for (int e = 0; e < E; e++)
-            u[e] = e * SEL_T + tid < kv ? weight(e * SEL_T + tid) : 0u;
-    }
-    auto each = [&](auto f) { /* f(position, weight) of this thread's positions in order */
-        if constexpr (E > 0) {
+        for (int e = 0; e < E; e++) {
+            const int j = min(from + e * SEL_T + tid, kv - 1);
+            page[e] = c.page_table[(size_t)b * c.max_pages + j / PG];
+        }
 #pragma unroll
-            for (int e = 0; e < E; e++)
-                f(e * SEL_T + tid, u[e]);
-        } else {
-            for (int e = 0; e < tiles; e++) {
-                const int j = e * SEL_T + tid;
-                f(j, j < kv ? weight(j) : 0u);
-            }
+        for (int e = 0; e < E; e++) {
+            const int j = min(from + e * SEL_T + tid, kv - 1);
+            const bool there = page[e] >= 0 && page[e] < c.num_pages;
+            const float x = c.w[((size_t)(there ? page[e] : 0) * c.Hkv + kh) * PG + j % PG];
+            u[e] = there ? ordered(x) : 0u;
         }
     };
+    load(0);
+    const bool again = kv > SPAN;
     /* the least kept: digits `top` so far under `mask`; ties: how many of its equals */
     uint32_t top = 0, mask = 0;
     int ties = want;
-    if (want > 0) {
-        for (int shift = 21, bits = 11; shift >= 0; bits = shift == 10 ? 10 : 11, shift -= bits) {
-            for (int i = tid; i < 2048; i += SEL_T)
-                hist[i] = 0;
-            __syncthreads();
-            each([&](int j, uint32_t x) {
-                const bool in = j >= lo && j < hi && (x & mask) == top;
-                const int digit = x >> shift & ((1u << bits) - 1);
+    for (int pass = 0; want > 0 && pass < 3; pass++) {
+        const int bits = pass < 2 ? 11 : 10, shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        for (int i = tid; i < 2048; i += SEL_T)
+            hist[i] = 0;
+        __syncthreads();
+        for (int from = 0; from < kv; from += SPAN) {
+            if (again)
+                load(from);
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const int j = from + e * SEL_T + tid;
+                const bool in = j >= lo && j < hi && (u[e] & mask) == top;
+                const int digit = u[e] >> shift & ((1u << bits) - 1);
                 /* the first lane's digit by one add: many weights may be the same */
                 const uint64_t live = __ballot(in);
                 if (!live)
-                    return;
+                    continue;
                 const int l = __ffsll((unsigned long long)live) - 1;
                 const int d = __builtin_amdgcn_readlane(digit, l);
                 const uint64_t same = __ballot(in && digit == d);
@@ -576,39 +578,72 @@ template <int E> __global__ __launch_bounds__(SEL_T) void select_kernel(Select c
                     atomicAdd(&hist[d], __popcll(same));
                 if (in && digit != d)
                     atomicAdd(&hist[digit], 1);
-            });
-            __syncthreads();
-            /* from the top: two digits a thread */
-            const int d1 = 2047 - 2 * tid, c1 = hist[d1], c0 = hist[d1 - 1];
-            int all;
-            const int above = block_scan(c1 + c0, scratch, &all);
-            if (above < ties && above + c1 + c0 >= ties) {
-                const bool first = above + c1 >= ties;
-                found[0] = first ? d1 : d1 - 1;
-                found[1] = ties - above - (first ? 0 : c1);
             }
-            __syncthreads();
-            top |= (uint32_t)found[0] << shift;
-            mask |= ((1u << bits) - 1) << shift;
-            ties = found[1];
-            if (shift == 0)
-                break;
         }
-    }
-    /* in order: which are kept, and where they go */
-    int kept = 0, equal = 0;
-    each([&](int j, uint32_t x) {
-        const bool mid = j >= lo && j < hi && want > 0;
-        const bool eq = mid && x == top;
+        __syncthreads();
+        /* from the top: two digits a thread */
+        const int d1 = 2047 - 2 * tid, c1 = hist[d1], c0 = hist[d1 - 1];
         int all;
-        const int rank = equal + block_scan(eq, scratch, &all);
-        equal += all;
-        const bool yes = j < kv && (j < lo || j >= hi || (mid && x > top) || (eq && rank < ties));
-        const int at = kept + block_scan(yes, scratch, &all);
-        kept += all;
-        if (yes && at < n)
-            keep[at] = j;
-    });
+        const int above = block_scan(c1 + c0, scratch, &all);
+        if (above < ties && above + c1 + c0 >= ties) {
+            const bool first = above + c1 >= ties;
+            found[0] = first ? d1 : d1 - 1;
+            found[1] = ties - above - (first ? 0 : c1);
+            found[2] = first ? c1 : c0;
+        }
+        __syncthreads();
+        top |= (uint32_t)found[0] << shift;
+        mask |= ((1u << bits) - 1) << shift;
+        ties = found[1];
+        if (found[2] == ties) /* all with these digits are kept, whatever the rest are */
+            break;
+    }
+    /* In order, tile by tile and wave by wave: each wave's count of each tile to LDS, their
+     * sums up to each in its place, and a lane's own by the lanes below. First of the least
+     * kept one's equals, then of all that are kept. */
+    auto ranks = [&](auto flag, int before, int (&rank)[E]) {
+        uint64_t bal[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            bal[e] = __ballot(flag(e));
+            if (lane == 0)
+                counts[e * WAVES + wave] = __popcll(bal[e]);
+        }
+        __syncthreads();
+        const int own = tid < E * WAVES ? counts[tid] : 0;
+        int all;
+        const int to = block_scan(own, scratch, &all);
+        if (tid < E * WAVES)
+            counts[tid] = to;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            rank[e] = before + counts[e * WAVES + wave] +
+                      __builtin_amdgcn_mbcnt_hi((uint32_t)(bal[e] >> 32),
+                                                __builtin_amdgcn_mbcnt_lo((uint32_t)bal[e], 0));
+        __syncthreads(); /* the counts are read */
+        return before + all;
+    };
+    int kept = 0, equal = 0;
+    for (int from = 0; from < kv; from += SPAN) {
+        if (again)
+            load(from);
+        auto at = [&](int e) { return from + e * SEL_T + tid; };
+        auto mid = [&](int e) { return at(e) >= lo && at(e) < hi && want > 0; };
+        int rank[E];
+        equal = ranks([&](int e) { return mid(e) && (u[e] & mask) == top; }, equal, rank);
+        bool yes[E];
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            yes[e] = at(e) < kv && (at(e) < lo || at(e) >= hi ||
+                                    (mid(e) && ((u[e] & mask) > top || ((u[e] & mask) == top &&
+                                                                 rank[e] < ties))));
+        kept = ranks([&](int e) { return yes[e]; }, kept, rank);
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            if (yes[e] && rank[e] < n)
+                keep[rank[e]] = at(e);
+    }
 }
 
 /* ---- kept positions to the front -----------------------------------------------------
@@ -836,10 +871,10 @@ extern "C" hipError_t k_kv_select(const float *weights, int num_pages, int Hkv,
     hipLaunchKernelGGL((select_kernel<E>), dim3((unsigned)grid), dim3(SEL_T), 0, stream, c)
     if (max_kv <= 4 * SEL_T)
         LAUNCH(4);
-    else if (max_kv <= 16 * SEL_T)
-        LAUNCH(16);
+    else if (max_kv <= 8 * SEL_T)
+        LAUNCH(8);
     else
-        LAUNCH(0);
+        LAUNCH(16);
 #undef LAUNCH
     return hipGetLastError();
 }

@@ -270,6 +270,14 @@ constexpr int pg_mid_goal(long long units, int Hkv) {
     const int chip = PG_MID_CHIP / Hkv;
     return 64 * units < chip ? (int)(64 * units) : chip;
 }
+/* Pieces of a line of up to units * most tiles, at most; tiles a piece of one of T */
+constexpr int pg_mid_pieces(long long units, long long most, int goal) {
+    return units * most < goal ? (int)(units * most) : goal;
+}
+constexpr int pg_mid_share(const pg_plan &p, unsigned T) {
+    const unsigned n = (unsigned)p.goal;
+    return pg_max((int)(T / n + (T % n != 0)), 1);
+}
 /* The merge: a workgroup a row of few, or a wave */
 constexpr bool pg_mid_by_row(const pg_plan &p, int Hkv) {
     return (long long)p.units * PG_MID * Hkv <= 512;
@@ -289,7 +297,7 @@ constexpr pg_plan pg_make_mid_plan(int N, int B, int max_q, int max_kv, int G, i
     }
     p.goal = pg_mid_goal(units, Hkv);
     p.units = (int)units;
-    p.shares = pg_few_pieces(units, most, p.goal);
+    p.shares = pg_mid_pieces(units, most, p.goal);
     p.slots = most > 1 ? 2 * p.shares : 0;
     if (p.slots > 0 && pg_mid_merge_items(p, Hkv) > PG_MOST_ITEMS)
         p.shares = -1;
@@ -329,7 +337,7 @@ constexpr size_t pg_ws_most(int N, int B, int max_q, int max_kv, int G, int Hkv)
         const long long all = pg_mid_units(N, units, max_q, G);
         const int m = (int)(all < units ? all : units > PG_MID_LITTLE ? units
                             : all < PG_MID_LITTLE ? all : PG_MID_LITTLE);
-        mid = pg_slot_bytes(2 * pg_few_pieces(m, most, pg_mid_goal(m, Hkv)), PG_MID, Hkv, m, 8);
+        mid = pg_slot_bytes(2 * pg_mid_pieces(m, most, pg_mid_goal(m, Hkv)), PG_MID, Hkv, m, 8);
     }
     return few > many ? (few > mid ? few : mid) : (many > mid ? many : mid);
 }
