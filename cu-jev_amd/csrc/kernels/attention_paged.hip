@@ -346,8 +346,8 @@ DEV size_t slot_of(const Call &c, int kh, int at) { return (size_t)kh * c.plan.s
  * loads.
  *
  * 64 sequences' tokens on up to 4096 keys, e4m3: 63 us for 320 MB (5.1 TB/s), and 5
- * for the merge; bf16 114 for 628 (5.5), and 5. A call of one tile takes 7.5 us, a chain of loads: arguments,
- * lengths, page ids, K, gates. */
+ * for the merge; bf16 114 for 628 (5.5), and 5. A call of one tile takes 7.5 us, a
+ * chain of loads: arguments, lengths, page ids, K, gates. */
 constexpr int FEW = PG_FEW;
 
 template <bool E4M3, int KIND>
@@ -824,9 +824,8 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
         const uint32_t va = M::V + (64 * wq + m) * (T / PD) +
                             ((E4M3 ? g ^ (m >> 2) : g ^ (m >> 1)) << 4);
         /* P of row m of a block: written 4 keys, 16 wq + 4 g on, read 8 at a time */
-        const uint32_t pw = M::P + (rg * RB * 16 + m) * 128 + (((2 * wq + (g >> 1)) ^ (m >> 1)) << 4) +
-                            (g & 1) * 8;
         const uint32_t pr = M::P + (rg * RB * 16 + m) * 128;
+        const uint32_t pw = pr + (((2 * wq + (g >> 1)) ^ (m >> 1)) << 4) + (g & 1) * 8;
         const uint32_t stat = M::STAT + (rg * RB * 16 + m) * 16;
 
         floatx4 o[RB][4]; /* dims 64 wq + 16 t + 4 g .. + 3 of row m of block rb */
@@ -1122,8 +1121,9 @@ __global__ __launch_bounds__(256 * RG) void attention_mid_kernel(Call c) {
  *
  * 4096 tokens on 8192 keys: 363-371 us, 1.1 PFLOP/s, 80 % of the rate of a large
  * library product on the same card (1.41; bf16); e4m3 389-396, where the conversions
- * to bf16 fill the VALU beside the MFMAs. A workgroup spends 12 us outside its tiles: 3.5 on lengths, page ids and
- * the first K, 5 on the epilogue (the gates' 32768 sigmoids are 2 of them). */
+ * to bf16 fill the VALU beside the MFMAs. A workgroup spends 12 us outside its tiles:
+ * 3.5 on lengths, page ids and the first K, 5 on the epilogue (the gates' 32768
+ * sigmoids are 2 of them). */
 constexpr int RT = PG_MANY;
 constexpr float SHIFT_RANGE = 64.f;
 /* With the reference 0, V far from 1 can lead p v out of fp32's range: p = 2^62 and V =
@@ -1168,7 +1168,8 @@ template <bool E4M3> DEV int perm_row(int m) {
 /* A workgroup's share, with a reference of 0 within the range; true: once more with none.
  * The second time is the first one's code again, and nothing but the range may be kept
  * for it: all of the 128 + 128 registers are taken. */
-template <bool E4M3, int KIND> DEV bool attend_many(const Call &c, unsigned char *smem, const float range) {
+template <bool E4M3, int KIND>
+DEV bool attend_many(const Call &c, unsigned char *smem, const float range) {
     typedef Lay<E4M3> L;
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid)); /* unknown: what goes by it is worked out each time */

@@ -5,9 +5,6 @@
 
 namespace CUJEV_KNS {
 namespace {
-
-
-
 /* ---- attention weights by key --------------------------------------------------
  *   w[j] = prev[j] + sum over the call's rows (n, h) that see key j of 2^(q.k_j - lse)
  * with the attention's own lse, so that one product with K gives p whole: no second
@@ -267,13 +264,15 @@ template <bool E4M3> DEV void weigh_many(const Weigh &c) {
         const int at = lane & (STEP - 1), tok = at * c.rG >> 16;
         loff = (tok * c.Hq + at - tok * c.G) * 4;
     }
+    /* the most that a descriptor spans: below qoff of no row */
+    constexpr size_t SPAN = 0x7fff0000;
     /* from step `steps` on the first tokens again: what a wait counts stays the same */
     auto first_tok = [&](int n) { return max(s.ql - (n + 1) * toks, t_first); };
     auto issue = [&](int n) {
         const int i0 = first_tok(n);
         const size_t from = (size_t)(s.q0 + i0) * c.Hq + kh * c.G;
         const size_t left = (size_t)(s.ql - i0) * c.Hq - kh * c.G;
-        const int bytes = (int)min(left * PD * 2, (size_t)0x7fffffff);
+        const int bytes = (int)min(left * PD * 2, SPAN);
         const __amdgpu_buffer_rsrc_t src =
             make_rsrc(c.q + from * PD, __builtin_amdgcn_readfirstlane(bytes));
 #pragma unroll
@@ -281,7 +280,7 @@ template <bool E4M3> DEV void weigh_many(const Weigh &c) {
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 src, (lds_ptr)(smem + n % NB * QB + (i * KG + wave) * 1024), 16, qoff[i], 0, 0, 0);
         if (wave == 0 && lane < STEP) {
-            const int lbytes = (int)min(left * 4, (size_t)0x7fffffff);
+            const int lbytes = (int)min(left * 4, SPAN);
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 make_rsrc(c.lse + from, __builtin_amdgcn_readfirstlane(lbytes)),
                 (lds_ptr)(smem + LSE + n % NB * (STEP * 4)), 4, loff, 0, 0, 0);
@@ -358,7 +357,8 @@ template <bool E4M3> DEV void weigh_many(const Weigh &c) {
         bool plain;
     };
     auto row_of = [&](int n, int half) {
-        const float l = *(lds_f32)((lds_u8 *)smem + LSE + n % NB * (STEP * 4) + half * 64 + col * 4);
+        const float l =
+            *(lds_f32)((lds_u8 *)smem + LSE + n % NB * (STEP * 4) + half * 64 + col * 4);
         const int tok = my_tok[half];
         const int i0 = first_tok(n); /* the last step's tokens end where the others began */
         const bool there = tok < s.ql - n * toks - i0;
@@ -688,7 +688,8 @@ DEV Move move_of(const Keep &c, int b, int kh, int n, int dst0, int i) {
     return m;
 }
 DEV long long shfl(long long x, int l) {
-    return (long long)(uint32_t)__shfl((int)x, l, 64) | (long long)__shfl((int)(x >> 32), l, 64) << 32;
+    return (long long)(uint32_t)__shfl((int)x, l, 64) |
+           (long long)__shfl((int)(x >> 32), l, 64) << 32;
 }
 
 template <bool E4M3> __global__ __launch_bounds__(256) void keep_kernel(Keep c) {

@@ -320,13 +320,12 @@ static int paged_heads_ok(int Hq, int Hkv) {
 }
 
 static int prep_paged(const char *what, const void *proj, int proj_stride, const float *q_norm_w,
-                                    const float *k_norm_w, const int32_t *pos, int axes, uint64_t axis_of,
-                                    const int32_t *q_start, const int32_t *kv_len,
-                                    const int32_t *page_table, int max_pages, int B, int N, int Hq,
-                                    int Hkv, int rot, const float *rope_table, int npos, float eps,
-                                    float q_scale, void *q_out, int kv_type, void *k_pages,
-                                    void *vt_pages, float *k_scale, float *v_scale, int num_pages,
-                                    void *stream) {
+                      const float *k_norm_w, const int32_t *pos, int axes, uint64_t axis_of,
+                      const int32_t *q_start, const int32_t *kv_len, const int32_t *page_table,
+                      int max_pages, int B, int N, int Hq, int Hkv, int rot,
+                      const float *rope_table, int npos, float eps, float q_scale, void *q_out,
+                      int kv_type, void *k_pages, void *vt_pages, float *k_scale, float *v_scale,
+                      int num_pages, void *stream) {
     const cujev_kv_pages pages = {k_pages, vt_pages, k_scale, v_scale, num_pages, Hkv, kv_type};
     const int st = paged_check(what, &pages, page_table, max_pages, kv_len, B);
     if (st != 0)
@@ -351,9 +350,9 @@ static int prep_paged(const char *what, const void *proj, int proj_stride, const
     if (((uintptr_t)q_norm_w | (uintptr_t)k_norm_w | (uintptr_t)rope_table) & 15)
         return fail(1, "%s: weights and RoPE table must be 16-byte aligned", what);
     const cujev_paged_seqs seqs = {q_start, kv_len, page_table, max_pages, B};
-    return launched(k_attn_prep_paged((const bf16_t *)proj, proj_stride, q_norm_w, k_norm_w, pos, axes,
-                                      axis_of, &seqs, N, Hq, rot, rope_table, npos, eps, q_scale,
-                                      (bf16_t *)q_out, &pages, (hipStream_t)stream),
+    return launched(k_attn_prep_paged((const bf16_t *)proj, proj_stride, q_norm_w, k_norm_w, pos,
+                                      axes, axis_of, &seqs, N, Hq, rot, rope_table, npos, eps,
+                                      q_scale, (bf16_t *)q_out, &pages, (hipStream_t)stream),
                     what);
 }
 
@@ -372,17 +371,18 @@ EXPORT int cujev_op_attn_prep_paged(const void *proj, int proj_stride, const flo
 }
 
 EXPORT int cujev_op_attn_prep_paged_axes(const void *proj, int proj_stride, const float *q_norm_w,
-                                    const float *k_norm_w, const int32_t *pos, int axes, uint64_t axis_of,
-                                    const int32_t *q_start, const int32_t *kv_len,
-                                    const int32_t *page_table, int max_pages, int B, int N, int Hq,
-                                    int Hkv, int rot, const float *rope_table, int npos, float eps,
-                                    float q_scale, void *q_out, int kv_type, void *k_pages,
-                                    void *vt_pages, float *k_scale, float *v_scale, int num_pages,
-                                    void *stream) {
-    return prep_paged("attn_prep_paged_axes", proj, proj_stride, q_norm_w, k_norm_w, pos, axes, axis_of, q_start,
-                      kv_len, page_table, max_pages, B, N, Hq, Hkv, rot, rope_table, npos, eps,
-                      q_scale, q_out, kv_type, k_pages, vt_pages, k_scale, v_scale, num_pages,
-                      stream);
+                                         const float *k_norm_w, const int32_t *pos, int axes,
+                                         uint64_t axis_of, const int32_t *q_start,
+                                         const int32_t *kv_len, const int32_t *page_table,
+                                         int max_pages, int B, int N, int Hq, int Hkv, int rot,
+                                         const float *rope_table, int npos, float eps,
+                                         float q_scale, void *q_out, int kv_type, void *k_pages,
+                                         void *vt_pages, float *k_scale, float *v_scale,
+                                         int num_pages, void *stream) {
+    return prep_paged("attn_prep_paged_axes", proj, proj_stride, q_norm_w, k_norm_w, pos, axes,
+                      axis_of, q_start, kv_len, page_table, max_pages, B, N, Hq, Hkv, rot,
+                      rope_table, npos, eps, q_scale, q_out, kv_type, k_pages, vt_pages, k_scale,
+                      v_scale, num_pages, stream);
 }
 
 EXPORT int cujev_op_kv_page_read(int kv_type, const void *k_pages, const void *vt_pages,
@@ -410,14 +410,13 @@ EXPORT int cujev_op_kv_page_read(int kv_type, const void *k_pages, const void *v
 }
 
 static int attend_paged(const char *what, const void *q, const void *gate, int gate_tok_stride,
-                                    int gate_head_stride, int kv_type, const void *k_pages,
-                                    const void *vt_pages, const float *k_scale,
-                                    const float *v_scale, int num_pages, const int32_t *q_start,
-                                    const int32_t *kv_len, const int32_t *page_table,
-                                    int max_pages, int B, int N, int max_q, int max_kv, int Hq,
-                                    int Hkv, int window, int sinks, const void *tree,
-                                    int tree_words, void *out, float *lse, void *ws,
-                                    size_t ws_bytes, void *stream) {
+                        int gate_head_stride, int kv_type, const void *k_pages,
+                        const void *vt_pages, const float *k_scale, const float *v_scale,
+                        int num_pages, const int32_t *q_start, const int32_t *kv_len,
+                        const int32_t *page_table, int max_pages, int B, int N, int max_q,
+                        int max_kv, int Hq, int Hkv, int window, int sinks, const void *tree,
+                        int tree_words, void *out, float *lse, void *ws, size_t ws_bytes,
+                        void *stream) {
     const cujev_kv_pages pages = {(void *)k_pages, (void *)vt_pages, (float *)k_scale,
                                   (float *)v_scale, num_pages, Hkv, kv_type};
     const int st = paged_check(what, &pages, page_table, max_pages, kv_len, B);
@@ -464,10 +463,10 @@ EXPORT int cujev_op_attention_paged(const void *q, const void *gate, int gate_to
                                     int gate_head_stride, int kv_type, const void *k_pages,
                                     const void *vt_pages, const float *k_scale,
                                     const float *v_scale, int num_pages, const int32_t *q_start,
-                                    const int32_t *kv_len, const int32_t *page_table,
-                                    int max_pages, int B, int N, int max_q, int max_kv, int Hq,
-                                    int Hkv, int window, int sinks, void *out, void *ws,
-                                    size_t ws_bytes, void *stream) {
+                                    const int32_t *kv_len, const int32_t *page_table, int max_pages,
+                                    int B, int N, int max_q, int max_kv, int Hq, int Hkv,
+                                    int window, int sinks, void *out, void *ws, size_t ws_bytes,
+                                    void *stream) {
     return attend_paged("attention_paged", q, gate, gate_tok_stride, gate_head_stride, kv_type,
                         k_pages, vt_pages, k_scale, v_scale, num_pages, q_start, kv_len,
                         page_table, max_pages, B, N, max_q, max_kv, Hq, Hkv, window, sinks,
@@ -475,13 +474,13 @@ EXPORT int cujev_op_attention_paged(const void *q, const void *gate, int gate_to
 }
 
 EXPORT int cujev_op_attention_paged_lse(const void *q, const void *gate, int gate_tok_stride,
-                                    int gate_head_stride, int kv_type, const void *k_pages,
-                                    const void *vt_pages, const float *k_scale,
-                                    const float *v_scale, int num_pages, const int32_t *q_start,
-                                    const int32_t *kv_len, const int32_t *page_table,
-                                    int max_pages, int B, int N, int max_q, int max_kv, int Hq,
-                                    int Hkv, int window, int sinks, void *out, float *lse, void *ws,
-                                    size_t ws_bytes, void *stream) {
+                                        int gate_head_stride, int kv_type, const void *k_pages,
+                                        const void *vt_pages, const float *k_scale,
+                                        const float *v_scale, int num_pages, const int32_t *q_start,
+                                        const int32_t *kv_len, const int32_t *page_table,
+                                        int max_pages, int B, int N, int max_q, int max_kv, int Hq,
+                                        int Hkv, int window, int sinks, void *out, float *lse,
+                                        void *ws, size_t ws_bytes, void *stream) {
     if (N > 0 && B > 0 && !lse)
         return fail(1, "attention_paged_lse: null argument");
     return attend_paged("attention_paged_lse", q, gate, gate_tok_stride, gate_head_stride, kv_type,
@@ -491,13 +490,14 @@ EXPORT int cujev_op_attention_paged_lse(const void *q, const void *gate, int gat
 }
 
 EXPORT int cujev_op_attention_paged_tree(const void *q, const void *gate, int gate_tok_stride,
-                                    int gate_head_stride, int kv_type, const void *k_pages,
-                                    const void *vt_pages, const float *k_scale,
-                                    const float *v_scale, int num_pages, const int32_t *q_start,
-                                    const int32_t *kv_len, const int32_t *page_table,
-                                    int max_pages, int B, int N, int max_q, int max_kv, int Hq,
-                                    int Hkv, const void *tree, int tree_words, void *out, float *lse, void *ws,
-                                    size_t ws_bytes, void *stream) {
+                                         int gate_head_stride, int kv_type, const void *k_pages,
+                                         const void *vt_pages, const float *k_scale,
+                                         const float *v_scale, int num_pages,
+                                         const int32_t *q_start, const int32_t *kv_len,
+                                         const int32_t *page_table, int max_pages, int B, int N,
+                                         int max_q, int max_kv, int Hq, int Hkv, const void *tree,
+                                         int tree_words, void *out, float *lse, void *ws,
+                                         size_t ws_bytes, void *stream) {
     if (N > 0 && B > 0 && !tree)
         return fail(1, "attention_paged_tree: null argument");
     return attend_paged("attention_paged_tree", q, gate, gate_tok_stride, gate_head_stride, kv_type,
@@ -568,7 +568,7 @@ EXPORT int cujev_op_kv_select(const float *weights, int num_pages, int Hkv,
         return fail(1, "kv_select: budget=%d has to hold sinks=%d and recent=%d, and keep rows of "
                        "%d the budget",
                     budget, sinks, recent, max_keep);
-    if (B > 0 && (!weights || !page_table || !kv_len || !keep || !keep_len))
+    if (B > 0 && (!weights || !page_table || !kv_len || (!keep && max_keep > 0) || !keep_len))
         return fail(1, "kv_select: null argument");
     if (B > 0 && keep_len == kv_len) /* other kv-heads read kv_len while one writes */
         return fail(1, "kv_select: keep_len must be another array than kv_len");

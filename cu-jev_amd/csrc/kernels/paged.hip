@@ -548,8 +548,8 @@ extern "C" hipError_t k_attn_prep_paged(const bf16_t *proj, int proj_stride, con
     const Prep c = {(const bf16 *)proj, proj_stride, q_norm_w, k_norm_w, pos, seqs->q_start,
                     seqs->kv_len, seqs->page_table, seqs->max_pages, B, N, Hq, Hkv, rot,
                     (const float2 *)rope_table, npos, axes, axis_of, eps, q_scale, (bf16 *)q_out,
-                    pages->k, pages->vt, pages->k_scale, pages->v_scale, pages->num_pages, (int)k_blocks,
-                    (int)v_blocks, v_spread};
+                    pages->k, pages->vt, pages->k_scale, pages->v_scale, pages->num_pages,
+                    (int)k_blocks, (int)v_blocks, v_spread};
     auto launch = [&](auto t, auto v, auto a) {
         hipLaunchKernelGGL(
             (prep_paged_kernel<decltype(t)::value, decltype(v)::value, decltype(a)::value>),

@@ -263,6 +263,7 @@ constexpr long long PG_MID_LITTLE = 1024;
 constexpr bool pg_is_mid(int N, int B, int max_q, int max_kv, int G, int Hkv) {
     const long long rows = (long long)pg_min(max_q, N) * G, units = pg_mid_units(N, B, max_q, G);
     return rows > PG_FEW && Hkv <= PG_MID_CHIP &&
+           units * pg_div_up(max_kv, PG) <= PG_MOST && /* numbers on the line are ints */
            (rows <= PG_MID ||
             (units <= PG_MID_LITTLE && units * pg_div_up(max_kv, PG) * Hkv <= PG_MID_LITTLE));
 }

@@ -404,8 +404,9 @@ def attn_prep_paged(proj, q_norm_w, k_norm_w, pos, q_start, kv_len, page_table, 
     if axes is not None:
         name, turned = "cujev_op_attn_prep_paged_axes", (axes.axes, axes.packed)
     _paged_call(dev, name, proj.data_ptr(), stride, q_norm_w.data_ptr(), k_norm_w.data_ptr(),
-                pos.data_ptr(), *turned, q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(), page_table.shape[1], B, N, Hq, Hkv, rot,
-                rope.data_ptr(), rope.shape[0], eps, q_scale, q_out.data_ptr(), *pages.args)
+                pos.data_ptr(), *turned, q_start.data_ptr(), kv_len.data_ptr(),
+                page_table.data_ptr(), page_table.shape[1], B, N, Hq, Hkv, rot, rope.data_ptr(),
+                rope.shape[0], eps, q_scale, q_out.data_ptr(), *pages.args)
 
 
 def kv_page_read(pages, page_table, kv_len, max_kv, k_cache, vt_cache):
@@ -517,7 +518,7 @@ def kv_weights(q, lse, pages, page_table, q_start, kv_len, max_q, max_kv, weight
     """weights [pages, Hkv, 64] (float32, beside the pages' keys) of every key of the
     sequences that have new tokens: prev's, where given and the key is before the new
     tokens, plus what the rows q [N, Hq, 256] of the call gave it, with the lse [N, Hq]
-    of their attention. prev may be weights itself, to add in place; None starts anew.
+    of their attention, one without a window over the same keys. prev may be weights itself, to add in place; None starts anew.
     ws: uint8 device workspace of kv_weights_ws_bytes, of this call or a larger one; None
     takes one from torch's allocator where the call needs any."""
     import torch
@@ -562,8 +563,8 @@ def kv_select(weights, page_table, kv_len, max_kv, budget, keep, keep_len, sinks
         raise OpsError(f"weights: need contiguous float32 [pages, Hkv, {KV_PAGE}], got "
                        f"{weights.dtype} {tuple(weights.shape)}")
     if page_table.dim() != 2 or keep.dim() != 3:
-        raise OpsError(f"kv_select: need page_table [B, max_pages] and keep [B, Hkv, max_keep], got "
-                       f"{tuple(page_table.shape)} and {tuple(keep.shape)}")
+        raise OpsError("kv_select: need page_table [B, max_pages] and keep [B, Hkv, max_keep], "
+                       f"got {tuple(page_table.shape)} and {tuple(keep.shape)}")
     if (max_kv | budget | sinks | recent) >> 31:
         _need_ints("kv_select", max_kv, budget, sinks, recent)
     B, Hkv, max_keep = page_table.shape[0], weights.shape[1], keep.shape[2]
