@@ -660,28 +660,35 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
 }
 
 /* ---- a middling number of rows of a draft tree: units of up to 64 ----------------------
- * Bound by the K/V bytes as few rows are, but O of 64 rows is four waves' registers. So the
- * four waves of a workgroup, one a SIMD, share all the rows (RB blocks of 16): wave i
- * scores the 16 keys i of a tile against them, and after P has gone through LDS takes
- * dims 64 i .. + 63 of O^T. Each element of a tile is read (and e4m3 widened) once so: with
- * the rows shared out, by every wave, 64 sequences' 16 tokens on 4096 e4m3 keys took
- * 119 us. Tiles come to LDS by loads (buffer_load ... lds),
- * K and V^T in rings of NB buffers each. Per tile three barriers: K of the tile is there
- * and V^T of the one before read; the waves' maxima are known and K read; P is written and
- * V^T there. Where a buffer is free its next tile goes out. The line of key tiles is cut
- * and merged as for few rows. */
+ * Bound by the K/V bytes as few rows are, but O of 64 rows is four waves' registers. So four
+ * waves, one a SIMD, share RB blocks of 16 rows (RG such groups): wave i scores the 16 keys i
+ * of a tile against them, and after P has gone through LDS takes dims 64 i .. + 63 of O^T.
+ * Each element of a tile is read (and e4m3 widened) once a group so; with the rows shared
+ * out, once by every wave, 64 sequences' 16 tokens on up to 4096 e4m3 keys took 119 us.
+ * Tiles come to LDS by loads (buffer_load ... lds), K and V^T in rings of NB buffers each.
+ * One barrier a tile: between two, O^T of a tile and the scores of the next one are worked
+ * on side by side, and P of the next one is written. That needs the softmax's reference
+ * before the waves have compared their maxima: it stays what it was unless a score is more
+ * than MID_OVER above it (then the waves do compare, with two barriers more; each unit's
+ * first tile, and few others). The same with three barriers, scores before O^T: 64 sequences'
+ * 16 tokens on 4096 keys each 138 us e4m3 and 204 bf16, so 123 and 194 (5.5 TB/s).
+ * The line of key tiles is cut and merged as for few rows. */
 template <bool E4M3, int RB, int RG> struct Mid {
     static constexpr int T = PSLICE * (E4M3 ? 1 : 2); /* bytes of a K or V^T tile */
     static constexpr int NB = E4M3 ? 4 : 2;
     static constexpr int V = NB * T, SK = 2 * NB * T, SV = SK + NB * 256;
     /* P, rows of 128 bytes; a float of each row and wave */
-    static constexpr int P = SK + (E4M3 ? 2 * NB * 256 : 0), STAT = P + RG * RB * 16 * 128;
-    static constexpr int BYTES = STAT + RG * RB * 16 * 16;
+    static constexpr int P = SK + (E4M3 ? 2 * NB * 256 : 0), PB = RG * RB * 16 * 128;
+    static constexpr int STAT = P + 2 * PB, FLAG = STAT + RG * RB * 16 * 16, BYTES = FLAG + 16;
 };
 typedef const __attribute__((address_space(3))) floatx4 *lds_f32x4;
+typedef const __attribute__((address_space(3))) int *lds_i32;
+/* A tile moves the softmax's reference where a score is more than this above it: p is up to
+ * 2^8, far from fp32's and bf16's ends, and rounds as it does below 1 */
+constexpr float MID_OVER = 8.f;
 
 /* The unit on the line that piece `target` begins in */
-DEV Where locate_mid(const Call &c, int target) {
+DEV Where locate_mid(const Call &c, int target, int &over) {
     const int lane = threadIdx.x & 63;
     pg_seq s;
     int n = 0, units = 0; /* of sequence b0 + lane */
@@ -690,21 +697,23 @@ DEV Where locate_mid(const Call &c, int target) {
         units = b0 + lane < c.B ? pg_units(s, c.G, PG_MID) : 0;
         n = units ? pg_longest(s, c.G, PG_LINE, 0, 0) : 0;
     };
-    int T = 0;
+    int T = 0, U = 0;
     for (int b0 = 0; b0 < c.B; b0 += 64) {
         read(b0);
         T += units * n;
+        U += units;
     }
-    T = last_lane(wave_scan(T));
+    T = last_lane(wave_scan(T)), U = last_lane(wave_scan(U));
+    over = pg_mid_over(c.plan, (unsigned)T);
     Where w;
     w.b = -1;
-    w.size = pg_mid_share(c.plan, (unsigned)T);
+    w.size = pg_mid_share(c.plan, (unsigned)T + (unsigned)U * over);
     const int item = target * w.size;
     int before = 0;
     for (int b0 = 0; b0 < c.B; b0 += 64) {
         if (c.B > 64)
             read(b0);
-        const int own = units * n, to = before + wave_scan(own);
+        const int own = units * (n + over), to = before + wave_scan(own);
         const uint64_t past = __ballot(to > item);
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
@@ -712,8 +721,8 @@ DEV Where locate_mid(const Call &c, int target) {
             w.s = seq_at(s, l);
             w.b = b0 + l;
             w.own = __builtin_amdgcn_readlane(n, l);
-            w.unit = (item - have) / w.own;
-            w.begin = have + w.unit * w.own;
+            w.unit = (item - have) / (w.own + over);
+            w.begin = have + w.unit * (w.own + over) + over;
             w.first = w.begin / w.size;
             w.parts = (w.begin + w.own - 1) / w.size - w.first + 1;
             w.part = target - w.first;
@@ -731,7 +740,8 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
     const int wq = wave & 3, rg = wave >> 2; /* keys or dims; rows */
     const int m = lane & 15, g = lane >> 4, kh = blockIdx.x % c.Hkv;
     lds_u8 *lds = (lds_u8 *)smem;
-    Where w = locate_mid(c, blockIdx.x / c.Hkv);
+    int over;
+    Where w = locate_mid(c, blockIdx.x / c.Hkv, over);
     while (w.b >= 0) { /* the units that the piece lies in */
         const pg_seq s = w.s;
         /* rows r0 .. r0 + rows - 1: of tokens i_first on, the first from its head `rest` on */
@@ -837,19 +847,106 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
             for (int t = 0; t < 4; t++)
                 o[rb][t] = floatx4{};
         }
-        int pg[NB + 1]; /* pages of tiles i .. i + NB */
+        int pg[NB + 1] = {}; /* pages of tiles i .. i + NB */
+        if (threadIdx.x < 2)
+            *(int *)(smem + M::FLAG + threadIdx.x * 4) = 0;
+        floatx4 x[RB], vsc;      /* a tile's scores; e4m3: V's scales of the lane's keys */
+        float ladd[RB];          /* its sums of p */
+        bool foreign = false;    /* it has keys that not all rows see, */
+        uint64_t any = ~0ull;    /* and those that some row does */
+        /* What the scores of tile i need beside their products */
+        auto begin_scores = [&](int i, int page) {
+            const int k0 = pg_tile_page(list, i0 + i) * PG;
+            foreign = page < 0 || !pg_tile_whole(k0, s.p0 - 1, s.p0 + s.ql - 1, s.kv, 0, 0);
+            if constexpr (E4M3)
+                vsc = *(lds_f32x4)(lds + M::SV + i % NB * 256 + (16 * wq + 4 * g) * 4);
+        };
+        auto k_scale = [&](int i) {
+            return E4M3 ? *(lds_f32)(lds + M::SK + i % NB * 256 + (16 * wq + m) * 4) : 1.f;
+        };
+        auto scores = [&](int j, uint32_t kbuf, float ksc, floatx4 (&y)[RB]) { /* of step j */
+            const u32x4 v = lds_read16(lds, (kbuf ^ ((j & 3) << 6)) + (j >> 2) * 256);
+#pragma unroll
+            for (int rb = 0; rb < RB; rb++) {
+                const floatx4 in = j ? y[rb] : floatx4{};
+                if constexpr (E4M3) {
+                    y[rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(v[0], v[1], ksc),
+                                                                    qf[rb][2 * j], in, 0, 0, 0);
+                    y[rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        widen(v[2], v[3], ksc), qf[rb][2 * j + 1], y[rb], 0, 0, 0);
+                } else {
+                    y[rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        __builtin_bit_cast(bf16x8, v), qf[rb][j], in, 0, 0, 0);
+                }
+            }
+        };
+        auto flag_of = [&](int i) { /* i + 1 where the tile moves the reference */
+            return __builtin_amdgcn_readfirstlane(*(lds_i32)(lds + M::FLAG + (i & 1) * 4));
+        };
+        /* P of tile i from x, by the reference as it is */
+        auto write_p = [&](int i) {
+#pragma unroll
+            for (int rb = 0; rb < RB; rb++) {
+                const float ref = mrun[rb] == -INFINITY ? 0.f : mrun[rb]; /* no key yet: p = 0 */
+                floatx4 p;
+#pragma unroll
+                for (int v = 0; v < 4; v++)
+                    p[v] = fast_exp2(x[rb][v] - ref);
+                ladd[rb] = (p[0] + p[1]) + (p[2] + p[3]);
+                if constexpr (E4M3)
+                    p *= vsc;
+                *(bf16x4 *)(smem + pw + (i & 1) * M::PB + rb * 2048) =
+                    bf16x4{f2bf(p[0]), f2bf(p[1]), f2bf(p[2]), f2bf(p[3])};
+            }
+        };
+        auto end_scores = [&](int i, int page) {
+            const int k0 = pg_tile_page(list, i0 + i) * PG;
+            if (foreign) {
+                const int left = page >= 0 ? s.kv - k0 : 0; /* keys of the tile, 64 at most count */
+                const uint64_t live = left >= PG ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
+                any = live & (s.ql <= 64 ? tree_keys(any_word, k0, s.p0)
+                                         : or_wave(tree_keys(row_words(min(i_first + lane, i_last)),
+                                                             c.words, k0, s.p0)));
+                if constexpr (E4M3) { /* scales of no key of the call: any bits */
+                    const uint32_t some = (uint32_t)(any >> (16 * wq + 4 * g));
+#pragma unroll
+                    for (int v = 0; v < 4; v++)
+                        vsc[v] = some >> v & 1 ? vsc[v] : 0.f;
+                }
+#pragma unroll
+                for (int rb = 0; rb < RB; rb++) {
+                    const uint64_t own = s.ql <= 64
+                                             ? tree_keys(word[rb], k0, s.p0)
+                                             : tree_keys(row_words(tok_of(rb)), c.words, k0, s.p0);
+                    const uint32_t bits = (uint32_t)((own & live) >> (16 * wq + 4 * g));
+                    unroll_for<4>([&](auto iv) {
+                        constexpr int v = decltype(iv)::value;
+                        x[rb][v] = hide_by<v>(bits, x[rb][v]);
+                    });
+                }
+            }
+            bool over = false;
+#pragma unroll
+            for (int rb = 0; rb < RB; rb++)
+                over |= fmaxf(fmaxf(x[rb][0], x[rb][1]), fmaxf(x[rb][2], x[rb][3])) >
+                        mrun[rb] + MID_OVER;
+            if (__any(over) && lane == 0)
+                *(int *)(smem + M::FLAG + (i & 1) * 4) = i + 1;
+            write_p(i);
+        };
+        /* All of it in one branch: where Q's loads were waited for in another, the compiler
+         * waits for them in the loop again, and for tiles of the next rounds with them */
         if (ntl > 0) {
 #pragma unroll
             for (int t = 0; t <= NB; t++)
                 pg[t] = page_of(t);
+            issue_k(0, pg[0]);
 #pragma unroll
-            for (int t = 0; t < NB; t++) { /* V^T of the last one: before the first scores */
-                issue_k(t, pg[t]);
-                if (t < NB - 1)
-                    issue_v(t, pg[t]);
+            for (int t = 0; t < NB - 1; t++) {
+                issue_k(t + 1, pg[t + 1]);
+                issue_v(t, pg[t]);
             }
-            /* Q is waited for here, where what was issued after it is known: in the loop the
-             * compiler would wait for tiles of the next round with it */
+            /* Q is waited for here, where what was issued after it is known */
 #pragma unroll
             for (int rb = 0; rb < RB; rb++) {
                 asm volatile("" : "+v"(word[rb]));
@@ -858,130 +955,79 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
                     asm volatile("" : "+v"(qf[rb][ks]));
             }
             any_word = or_wave(any_word);
-        }
-        for (int i = 0; i < ntl; i++) {
-            const bool there = pg[0] >= 0;
-            const int k0 = pg_tile_page(list, i0 + i) * PG;
+            /* the first tile's scores */
             meet(template_int<NB - 1>{}, template_int<NB - 1>{});
-            issue_v(i + NB - 1, pg[NB - 1]);
-            floatx4 x[RB], vsc; /* vsc: e4m3, V's scales of the lane's keys */
-            const bool foreign =
-                !there || !pg_tile_whole(k0, s.p0 - 1, s.p0 + s.ql - 1, s.kv, 0, 0);
-            const int left = there ? s.kv - k0 : 0; /* keys of the tile, 64 at most count */
-            const uint64_t live = left >= PG ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
-            uint64_t any = ~0ull; /* keys that some row sees */
-            if (foreign)
-                any = live & (s.ql <= 64 ? tree_keys(any_word, k0, s.p0)
-                                         : or_wave(tree_keys(row_words(min(i_first + lane, i_last)),
-                                                             c.words, k0, s.p0)));
-            {
-                const uint32_t kbuf = i % NB * T + ka;
-                const float ksc =
-                    E4M3 ? *(lds_f32)(lds + M::SK + i % NB * 256 + (16 * wq + m) * 4) : 1.f;
-                if constexpr (E4M3)
-                    vsc = *(lds_f32x4)(lds + M::SV + i % NB * 256 + (16 * wq + 4 * g) * 4);
+            begin_scores(0, pg[0]);
+            const float ksc = k_scale(0);
 #pragma unroll
-                for (int j = 0; j < (E4M3 ? 4 : 8); j++) {
-                    const u32x4 v = lds_read16(lds, (kbuf ^ ((j & 3) << 6)) + (j >> 2) * 256);
+            for (int j = 0; j < (E4M3 ? 4 : 8); j++)
+                scores(j, ka, ksc, x);
+            end_scores(0, pg[0]);
+            for (int i = 0; i < ntl; i++) {
+                meet(template_int<NB - 2>{}, template_int<NB - 2>{});
+                issue_k(i + NB, pg[NB]);
+                issue_v(i + NB - 1, pg[NB - 1]);
+                if (flag_of(i) == i + 1) { /* uniform */
+                    /* the reference moves: to the maximum, and P is written again */
 #pragma unroll
                     for (int rb = 0; rb < RB; rb++) {
-                        const floatx4 in = j ? x[rb] : floatx4{};
-                        if constexpr (E4M3) {
-                            x[rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                widen(v[0], v[1], ksc), qf[rb][2 * j], in, 0, 0, 0);
-                            x[rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                widen(v[2], v[3], ksc), qf[rb][2 * j + 1], x[rb], 0, 0, 0);
-                        } else {
-                            x[rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                __builtin_bit_cast(bf16x8, v), qf[rb][j], in, 0, 0, 0);
-                        }
+                        float mx = fmaxf(fmaxf(x[rb][0], x[rb][1]), fmaxf(x[rb][2], x[rb][3]));
+                        mx = fold_rows(mx, [](float a, float e) { return fmaxf(a, e); });
+                        if (g == 0)
+                            *(float *)(smem + stat + rb * 256 + wq * 4) = mx;
                     }
-                }
-                if (foreign) {
-                    if constexpr (E4M3) { /* scales of no key of the call: any bits */
-                        const uint32_t some = (uint32_t)(any >> (16 * wq + 4 * g));
-#pragma unroll
-                        for (int v = 0; v < 4; v++)
-                            vsc[v] = some >> v & 1 ? vsc[v] : 0.f;
-                    }
+                    lds_barrier();
 #pragma unroll
                     for (int rb = 0; rb < RB; rb++) {
-                        const uint64_t own =
-                            s.ql <= 64 ? tree_keys(word[rb], k0, s.p0)
-                                       : tree_keys(row_words(tok_of(rb)), c.words, k0, s.p0);
-                        const uint32_t bits = (uint32_t)((own & live) >> (16 * wq + 4 * g));
-                        unroll_for<4>([&](auto iv) {
-                            constexpr int v = decltype(iv)::value;
-                            x[rb][v] = hide_by<v>(bits, x[rb][v]);
-                        });
-                    }
-                }
-#pragma unroll
-                for (int rb = 0; rb < RB; rb++) {
-                    float mx = fmaxf(fmaxf(x[rb][0], x[rb][1]), fmaxf(x[rb][2], x[rb][3]));
-                    mx = fold_rows(mx, [](float a, float e) { return fmaxf(a, e); });
-                    if (g == 0)
-                        *(float *)(smem + stat + rb * 256 + wq * 4) = mx;
-                }
-            }
-            lds_barrier();
-            issue_k(i + NB, pg[NB]);
-            {
-#pragma unroll
-                for (int rb = 0; rb < RB; rb++) {
-                    const floatx4 all = *(lds_f32x4)(lds + stat + rb * 256);
-                    const float mnew = fmaxf(fmaxf(fmaxf(all[0], all[1]), fmaxf(all[2], all[3])),
-                                             mrun[rb]);
-                    const float ref = mnew == -INFINITY ? 0.f : mnew; /* no key yet: p = 0 */
-                    if (__any(mnew != mrun[rb])) {
-                        const float a = fast_exp2(mrun[rb] - ref);
+                        const floatx4 all = *(lds_f32x4)(lds + stat + rb * 256);
+                        const float mnew = fmaxf(fmaxf(fmaxf(all[0], all[1]), fmaxf(all[2], all[3])),
+                                                 mrun[rb]);
+                        const float a = fast_exp2(mrun[rb] - (mnew == -INFINITY ? 0.f : mnew));
                         lrun[rb] *= a;
 #pragma unroll
                         for (int t = 0; t < 4; t++)
                             o[rb][t] *= a;
+                        mrun[rb] = mnew;
                     }
-                    mrun[rb] = mnew;
-#pragma unroll
-                    for (int v = 0; v < 4; v++)
-                        x[rb][v] = fast_exp2(x[rb][v] - ref);
-                    lrun[rb] += (x[rb][0] + x[rb][1]) + (x[rb][2] + x[rb][3]);
-                    if constexpr (E4M3)
-                        x[rb] *= vsc;
-                    const bf16x4 p = {f2bf(x[rb][0]), f2bf(x[rb][1]), f2bf(x[rb][2]),
-                                      f2bf(x[rb][3])};
-                    *(bf16x4 *)(smem + pw + rb * 2048) = p;
+                    write_p(i);
+                    lds_barrier();
                 }
-            }
-            meet(template_int<NB>{}, template_int<NB - 1>{});
-            {
-                const uint32_t vbuf = i % NB * T + va;
+#pragma unroll
+                for (int rb = 0; rb < RB; rb++)
+                    lrun[rb] += ladd[rb];
                 bf16x8 p[RB][2];
 #pragma unroll
                 for (int rb = 0; rb < RB; rb++)
 #pragma unroll
                     for (int st = 0; st < 2; st++) /* keys 32 st + 8 g on (e4m3 16 g + 8 st) */
                         p[rb][st] = __builtin_bit_cast(
-                            bf16x8, lds_read16(lds, pr + rb * 2048 +
-                                                        (((E4M3 ? 2 * g + st : 4 * st + g) ^
-                                                          (m >> 1))
-                                                         << 4)));
-                u32x4 keep[2]; /* bits to keep of V^T: of keys of the call */
-                if (foreign) {
-                    const uint32_t a = (uint32_t)(any >> ((E4M3 ? 16 : 8) * g));
-                    const uint32_t e = (uint32_t)(any >> 32 >> (8 * g));
-#pragma unroll
-                    for (int d = 0; d < 4; d++) {
-                        auto two = [&](uint32_t x2) {
-                            return ((x2 >> (2 * d) & 1) ? 0xffffu : 0u) |
-                                   ((x2 >> (2 * d + 1) & 1) ? 0xffff0000u : 0u);
-                        };
-                        keep[0][d] = E4M3 ? bytes_by(a >> (4 * d)) : two(a);
-                        keep[1][d] = two(e);
-                    }
-                }
+                            bf16x8,
+                            lds_read16(lds, pr + (i & 1) * M::PB + rb * 2048 +
+                                                (((E4M3 ? 2 * g + st : 4 * st + g) ^ (m >> 1)) << 4)));
+                /* O^T of tile i, dims 16 t on of the wave's, and scores of tile i + 1 between (past
+                 * the last of that one again, for nothing): neither waits for the other's */
+                const uint32_t vbuf = i % NB * T + va, kbuf = (i + 1) % NB * T + ka;
+                floatx4 y[RB];
+                const float ksc = k_scale(i + 1);
                 auto products = [&](auto masked) {
+                    u32x4 keep[2]; /* bits to keep of V^T: of keys of the call */
+                    if constexpr (decltype(masked)::value) {
+                        const uint32_t a = (uint32_t)(any >> ((E4M3 ? 16 : 8) * g));
+                        const uint32_t e = (uint32_t)(any >> 32 >> (8 * g));
+#pragma unroll
+                        for (int d = 0; d < 4; d++) {
+                            auto two = [&](uint32_t x2) {
+                                return ((x2 >> (2 * d) & 1) ? 0xffffu : 0u) |
+                                       ((x2 >> (2 * d + 1) & 1) ? 0xffff0000u : 0u);
+                            };
+                            keep[0][d] = E4M3 ? bytes_by(a >> (4 * d)) : two(a);
+                            keep[1][d] = two(e);
+                        }
+                    }
 #pragma unroll
                     for (int t = 0; t < 4; t++) {
+                        if constexpr (!E4M3)
+                            scores(2 * t, kbuf, ksc, y);
                         bf16x8 v[2];
                         if constexpr (E4M3) {
                             u32x4 raw = lds_read16(lds, vbuf + t * 1024);
@@ -997,6 +1043,7 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
                                 v[st] = __builtin_bit_cast(bf16x8, raw);
                             }
                         }
+                        scores(E4M3 ? t : 2 * t + 1, kbuf, ksc, y);
 #pragma unroll
                         for (int rb = 0; rb < RB; rb++)
 #pragma unroll
@@ -1009,11 +1056,18 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
                     products(std::true_type{});
                 else
                     products(std::false_type{});
-            }
 #pragma unroll
-            for (int t = 0; t < NB; t++)
-                pg[t] = pg[t + 1];
-            pg[NB] = page_of(i + 1 + NB);
+                for (int rb = 0; rb < RB; rb++)
+                    x[rb] = y[rb];
+                if (i + 1 < ntl) {
+                    begin_scores(i + 1, pg[1]);
+                    end_scores(i + 1, pg[1]);
+                }
+#pragma unroll
+                for (int t = 0; t < NB; t++)
+                    pg[t] = pg[t + 1];
+                pg[NB] = page_of(i + 1 + NB);
+            }
         }
         /* nothing is on its way, and all have read */
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -1068,8 +1122,8 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
             }
         }
         /* on to the next unit, if the piece goes on after this one */
-        const bool more = cut + w.size > w.own;
-        w.begin += w.own, w.first = w.begin / w.size, w.part = 0;
+        const bool more = cut + w.size > w.own + over;
+        w.begin += w.own + over, w.first = w.begin / w.size, w.part = 0;
         if (more && w.unit + 1 < pg_units(s, c.G, PG_MID)) {
             w.unit++;
         } else {

@@ -34,13 +34,15 @@ static void pieces(int B, int G, int Hkv, int most_q, int most_kv, int loose) {
     const pg_plan p = pg_make_mid_plan(N, B, max_q, max_kv, G, Hkv);
     NEED(p.shares >= 0 && p.rt == PG_MID && p.units % B == 0);
     NEED(pg_mid_ws_bytes(p, Hkv) <= pg_ws_most(N, B, max_q, max_kv, G, Hkv));
-    long long T = 0;
+    long long T = 0, U = 0;
     for (int b = 0, q0 = 0; b < B; q0 += ql[b++]) {
         seqs.push_back(pg_clean_seq(q0, q0 + ql[b], kv[b], N, max_q, max_kv));
         T += (long long)pg_units(seqs[b], G, PG_MID) * (ql[b] ? pg_longest(seqs[b], G, PG_LINE, 0, 0) : 0);
+        U += pg_units(seqs[b], G, PG_MID);
     }
-    const int size = pg_mid_share(p, (unsigned)T);
-    NEED(size >= 1 && (T + size - 1) / size <= p.shares); /* a workgroup for every piece */
+    const int over = pg_mid_over(p, (unsigned)T); /* what a unit counts for beside its tiles */
+    const int size = pg_mid_share(p, (unsigned)T + (unsigned)U * over);
+    NEED(size > over && (T + U * over + size - 1) / size <= p.shares); /* a workgroup for every piece */
     NEED((long long)p.shares * size < 0x7fffffff);
     std::set<int> slots, infos;
     long long begin = 0;
@@ -51,9 +53,14 @@ static void pieces(int B, int G, int Hkv, int most_q, int most_kv, int loose) {
         for (int u = 0; u < units; u++) {
             const int own = pg_longest(s, G, PG_LINE, 0, 0);
             NEED(own >= pg_tile_list(s, 0, s.ql - 1, 0, 0).ntl && own * PG <= pg_max(max_kv, 1) + PG);
+            begin += over;
             const int first = (int)(begin / size), parts = (int)((begin + own - 1) / size) - first + 1;
             int covered = 0;
             for (int j = 0; j < parts; j++) {
+                if (j > 0) /* what the piece's workgroup finds at the piece's start */
+                    NEED((long long)(first + j) * size >= begin);
+                else /* the start is in the unit, or the workgroup comes from one before */
+                    NEED((long long)first * size <= begin && ((long long)first * size >= begin - over || begin > over));
                 const int cut = (int)((first + (long long)j) * size - begin), i0 = pg_max(cut, 0);
                 const int ntl = pg_min(cut + size, own) - i0;
                 NEED(i0 == covered && ntl > 0);
@@ -70,7 +77,19 @@ static void pieces(int B, int G, int Hkv, int most_q, int most_kv, int loose) {
             begin += own;
         }
     }
-    NEED(begin == T);
+    NEED(begin == T + U * over);
+    /* a piece's start is in some unit, whose first tile is in the piece, or in one before */
+    begin = 0;
+    for (int b = 0; b < B; b++)
+        for (int u = 0; u < pg_units(seqs[b], G, PG_MID); u++) {
+            const int own = pg_longest(seqs[b], G, PG_LINE, 0, 0);
+            for (long long item = (begin + size - 1) / size * size; item < begin + over + own; item += size) {
+                const int target = (int)(item / size), first = (int)((begin + over) / size);
+                const int parts = (int)((begin + over + own - 1) / size) - first + 1;
+                NEED(first <= target && target - first < parts);
+            }
+            begin += over + own;
+        }
 }
 
 int main() {
@@ -87,7 +106,7 @@ int main() {
         if (p.shares < 0) continue; /* refused */
         const long long T = (long long)p.units * ((kv + PG - 1) / PG);
         NEED(T <= PG_MOST);
-        NEED((p.goal + 1ll) * pg_mid_share(p, (unsigned)T) < 0x7fffffff);
+        NEED((p.goal + 1ll) * pg_mid_share(p, (unsigned)(T + (long long)p.units * PG_MID_OVER)) < 0x7fffffff);
     }
     NEED(!pg_is_mid(1 << 22, 1 << 20, 4, PG_MOST_KEYS, 16, 1));
     /* one workspace for every smaller call */
