@@ -86,12 +86,13 @@ struct Prep {
 };
 enum { ROW_Q, ROW_K, ROW_V };
 
-/* A wave for tokens n0 .. n0 + TOK - 1 of one head. AXES: pos has a row an axis, lane
- * TOK a + t holds token t's on axis a, and each frequency picks its own: 4 loads of 8
- * bytes a token and lane, scattered over up to 4 rows of the table. */
+/* A wave for tokens n0 .. n0 + TOK - 1 of one head. AXES: pos has a row an axis, and each
+ * frequency picks its own: the wave's angles come to LDS, TOK / 2 loads of 8 bytes by all
+ * lanes. Loaded where they are used, 16 a rotating lane, 2 x 2500 bf16 took 40 us, so 33.5
+ * (without axes 33). */
 template <int KIND, int TOK, bool E4M3, bool AXES>
 DEV void row_wave(const Prep &c, int head, int n0) {
-    constexpr bool is_k = KIND == ROW_K;
+    constexpr bool is_k = KIND == ROW_K, BY_AXES = AXES && KIND != ROW_V;
     const int lane = threadIdx.x & 63, N = c.N, rot = c.rot;
     const float *w = is_k ? c.kw : c.qw;
     /* K's heads, then V's, follow q's and the gates' */
@@ -106,45 +107,49 @@ DEV void row_wave(const Prep &c, int head, int n0) {
     for (int t = 0; t < TOK; t++)
         raw[t] = *(const bf16x4 *)(src + (size_t)min(n0 + t, N - 1) * c.ps);
     const float4 wl = *(const float4 *)(w + 4 * lane);
-    const size_t pos_row = AXES ? (size_t)min(lane / TOK & 3, c.axes - 1) * N : 0;
-    int pos_lane = min(max(c.pos[pos_row + min(n0 + (lane & (TOK - 1)), N - 1)], 0), c.npos - 1);
-    /* read from all lanes below: sunk into the rotating lanes' branch it was worked out by
-     * those alone (rot 8: two, for four tokens) */
-    asm volatile("" : "+v"(pos_lane));
-    /* (cos, sin) of token t for dim e of the lane's */
-    const uint32_t axis4 = (uint32_t)(c.axis_of >> (2 * fi0)); /* of the lane's four */
-    auto angle_row = [&](int t, int e) {
-        int p = __builtin_amdgcn_readlane(pos_lane, t);
-        if constexpr (AXES) {
-            const int a = axis4 >> (2 * e) & 3;
+    /* AXES: angle i of the wave, frequency i % (rot / 2) of token i / (rot / 2), by lane i % 64 */
+    __shared__ __attribute__((aligned(16))) float2 angles[BY_AXES ? TOK * 32 : 1];
+    int pos_lane = 0, pos_of[BY_AXES ? TOK / 2 : 1];
+    if constexpr (BY_AXES) {
 #pragma unroll
-            for (int k = 1; k < 4; k++) {
-                const int pk = __builtin_amdgcn_readlane(pos_lane, TOK * k + t);
-                p = a == k ? pk : p;
-            }
+        for (int k = 0; k < TOK / 2; k++) {
+            const int tok = (64 * k + lane) * 2 / rot;
+            const int axis = c.axis_of >> 2 * (lane % (rot / 2)) & 3;
+            pos_of[k] = c.pos[(size_t)min(axis, c.axes - 1) * N + min(n0 + tok, N - 1)];
         }
-        return c.rope + (size_t)p * (rot / 2) + fi0;
+    } else {
+        pos_lane = min(max(c.pos[min(n0 + (lane & (TOK - 1)), N - 1)], 0), c.npos - 1);
+        /* read from all lanes below: sunk into the rotating lanes' branch it was worked out by
+         * those alone (rot 8: two, for four tokens) */
+        asm volatile("" : "+v"(pos_lane));
+    }
+    /* (cos, sin) of token t for the lane's four dims */
+    auto angle_row = [&](int t) {
+        if constexpr (BY_AXES)
+            return (const float2 *)angles + t * (rot / 2) + fi0;
+        else
+            return c.rope + (size_t)__builtin_amdgcn_readlane(pos_lane, t) * (rot / 2) + fi0;
     };
     /* The tokens' sequences, then (K) their slots, token t in lane t: one
      * chain of loads for all of them. at: the K row in the pool, -1: none */
     pg_seq s;
     int b = find_seqs<TOK>(c.q_start, c.kv_len, c.B, N, c.max_pages * PG, n0, &s);
+    if constexpr (BY_AXES) {
+#pragma unroll
+        for (int k = 0; k < TOK / 2; k++) {
+            const int i = 64 * k + lane, p = min(max(pos_of[k], 0), c.npos - 1);
+            if (i < TOK * rot / 2)
+                angles[i] = c.rope[(size_t)p * (rot / 2) + lane % (rot / 2)];
+        }
+        __syncthreads();
+    }
     float4 rc[TOK][2] = {};
     if (rotates) { /* 16 lanes' loads or fewer: by all 64 they cost more than x's */
 #pragma unroll
         for (int t = 0; t < TOK; t++) {
-            if constexpr (AXES) {
-                float2 r[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    r[e] = angle_row(t, e)[e];
-                rc[t][0] = float4{r[0].x, r[0].y, r[1].x, r[1].y};
-                rc[t][1] = float4{r[2].x, r[2].y, r[3].x, r[3].y};
-            } else {
-                const float4 *r = (const float4 *)angle_row(t, 0);
-                rc[t][0] = r[0];
-                rc[t][1] = r[1];
-            }
+            const float4 *r = (const float4 *)angle_row(t);
+            rc[t][0] = r[0];
+            rc[t][1] = r[1];
         }
     }
     if (n0 + lane >= N)
@@ -274,7 +279,7 @@ DEV void row_wave(const Prep &c, int head, int n0) {
         const long long row = row_of(t);
         int e;
         const uint32_t out = k_row_exact(
-            src + (size_t)(n0 + t) * c.ps, [&](int i) { return angle_row(t, i)[i]; },
+            src + (size_t)(n0 + t) * c.ps, [&](int i) { return angle_row(t)[i]; },
             w + 4 * lane, rotates, first, half_lanes, c.eps, &e);
         ((uint32_t *)c.k_pages)[row * 64 + lane] = out;
         if (lane == 0)
