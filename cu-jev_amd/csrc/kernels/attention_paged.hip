@@ -742,33 +742,104 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
     lds_u8 *lds = (lds_u8 *)smem;
     int over;
     Where w = locate_mid(c, blockIdx.x / c.Hkv, over);
-    while (w.b >= 0) { /* the units that the piece lies in */
-        const pg_seq s = w.s;
-        /* rows r0 .. r0 + rows - 1: of tokens i_first on, the first from its head `rest` on */
-        const int b = w.b, r0 = w.unit * PG_MID, rows = min(s.ql * c.G - r0, 16 * RB * RG);
-        const int i_first = r0 / c.G, rest = r0 - i_first * c.G;
-        const pg_tiles list = pg_tile_list(s, 0, s.ql - 1, 0, 0);
-        const int cut = (w.first + w.part) * w.size - w.begin;
-        const int i0 = max(cut, 0), ntl = min(min(cut + w.size, w.own), list.ntl) - i0;
-        int ids = ntl > 0 ? page_id(c, b, list, min(i0 + lane, list.ntl - 1)) : -1, ids0 = 0;
-        auto page_of = [&](int t) { /* of tile t from i0 on; past the last, it again */
-            t = min(t, ntl - 1);
-            if (t - ids0 >= 64) {
-                ids0 = t;
-                ids = page_id(c, b, list, min(i0 + t + lane, list.ntl - 1));
-            }
-            return __builtin_amdgcn_readlane(ids, t - ids0);
-        };
-        /* this lane's rows */
-        auto row_of = [&](int rb) { return 16 * (rg * RB + rb) + m; };
-        auto after = [&](int rb) { /* tokens after i_first */
-            return (rest + min(row_of(rb), rows - 1)) * c.rG >> 16;
-        };
-        auto tok_of = [&](int rb) { return i_first + after(rb); };
-        auto head_of = [&](int rb) {
-            return kh * c.G + rest + min(row_of(rb), rows - 1) - after(rb) * c.G;
-        };
-        bf16x8 qf[RB][8];
+    if (w.b < 0)
+        return;
+    /* A unit, or the part of it in the piece: rows r0 .. r0 + rows - 1 of tokens i_first .. i_last,
+     * the first from its head `rest` on; its tiles i0 .. i0 + ntl - 1 */
+    pg_seq s;
+    int b, rows, i_first, rest, i_last, cut, i0, ntl, ids, ids0;
+    auto id_at = [&](int i) {
+        const int page = c.page_table[(size_t)b * c.max_pages + min(i0 + i, (s.kv - 1) / PG)];
+        return page >= 0 && page < c.num_pages ? page : -1;
+    };
+    auto set_unit = [&] {
+        s = w.s, b = w.b;
+        const int r0 = w.unit * PG_MID;
+        rows = min(s.ql * c.G - r0, 16 * RB * RG);
+        i_first = r0 / c.G, rest = r0 - i_first * c.G;
+        i_last = i_first + ((rest + rows - 1) * c.rG >> 16);
+        cut = (w.first + w.part) * w.size - w.begin;
+        i0 = max(cut, 0);
+        ntl = min(min(cut + w.size, w.own), pg_tile_list(s, 0, s.ql - 1, 0, 0).ntl) - i0;
+        ids = ntl > 0 ? id_at(lane) : -1, ids0 = 0;
+    };
+    auto page_of = [&](int t) { /* of tile t from i0 on; past the last, it again */
+        t = max(min(t, ntl - 1), 0);
+        if (t - ids0 >= 64) {
+            ids0 = t;
+            ids = id_at(t + lane);
+        }
+        return __builtin_amdgcn_readlane(ids, t - ids0);
+    };
+    /* this lane's rows */
+    auto row_of = [&](int rb) { return 16 * (rg * RB + rb) + m; };
+    auto after = [&](int rb) { /* tokens after i_first */
+        return (rest + min(row_of(rb), rows - 1)) * c.rG >> 16;
+    };
+    auto tok_of = [&](int rb) { return i_first + after(rb); };
+    auto head_of = [&](int rb) {
+        return kh * c.G + rest + min(row_of(rb), rows - 1) - after(rb) * c.G;
+    };
+    auto row_words = [&](int tok) { return c.tree + (size_t)(s.q0 + tok) * c.words; };
+    bf16x8 qf[RB][8];
+    /* the tree's words of this lane's rows, and of all the unit's tokens together: the first
+     * ones, all there are of up to 64 new tokens */
+    uint64_t word[RB], any_word;
+    int pg[NB + 1]; /* pages of tiles i .. i + NB */
+    /* Tiles: KiB j NW + wave of a tile is a wave's load j, 2 K rows or 8 V^T rows (e4m3
+     * 4 and 16). Pieces of 16 bytes are swizzled, in the address, so that 16 lanes'
+     * operands hit 16 bank groups: K's piece p of key k in slot p ^ (k & 15), V^T's of
+     * row d in p ^ (d / 2 & 7) (e4m3 d / 4 & 3), P's of row r in p ^ (r / 2 & 7). */
+    auto slice = [&](int page) { return (size_t)max(page, 0) * c.Hkv + kh; };
+    auto issue_k = [&](int t, int page) {
+        const __amdgpu_buffer_rsrc_t src = make_rsrc((const char *)c.k + slice(page) * T, T);
+#pragma unroll
+        for (int j = 0; j < L; j++) {
+            const int kib = j * NW + wave, key = E4M3 ? 4 * kib + g : 2 * kib + (lane >> 5);
+            const uint32_t off = E4M3 ? g * 256 + ((m ^ (key & 15)) << 4)
+                                      : (lane >> 5) * 512 + (((lane & 31) ^ (key & 15)) << 4);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                src, (lds_ptr)(smem + t % NB * T + kib * 1024), 16, off, kib * 1024, 0, 0);
+        }
+        if (E4M3 && wave < 2) /* both operands' scales: V's multiply p */
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                make_rsrc((wave ? c.vs : c.ks) + slice(page) * PG, 256),
+                (lds_ptr)(smem + (wave ? M::SV : M::SK) + t % NB * 256), 4, lane * 4, 0, 0, 0);
+    };
+    auto issue_v = [&](int t, int page) {
+        const __amdgpu_buffer_rsrc_t src = make_rsrc((const char *)c.vt + slice(page) * T, T);
+#pragma unroll
+        for (int j = 0; j < L; j++) {
+            const int kib = j * NW + wave;
+            const int d = E4M3 ? 16 * kib + (lane >> 2) : 8 * kib + (lane >> 3);
+            const uint32_t off = E4M3 ? (lane >> 2) * 64 + (((lane & 3) ^ (d >> 2 & 3)) << 4)
+                                      : (lane >> 3) * 128 + (((lane & 7) ^ (d >> 1 & 7)) << 4);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                src, (lds_ptr)(smem + M::V + t % NB * T + kib * 1024), 16, off, kib * 1024, 0,
+                0);
+        }
+    };
+    /* all but the newest `nk` of K's groups of loads and `nv` of V^T's are there, and all
+     * waves as far; what is issued past the last tile keeps the count */
+    auto meet = [&](auto nk, auto nv) {
+        constexpr int n = (decltype(nk)::value + decltype(nv)::value) * L;
+        if (E4M3 && wave < 2)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(n + decltype(nk)::value)
+                         : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(n) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    const uint32_t ka = (16 * wq + m) * (T / PG) + ((g ^ m) << 4);
+    const uint32_t va = M::V + (64 * wq + m) * (T / PD) +
+                        ((E4M3 ? g ^ (m >> 2) : g ^ (m >> 1)) << 4);
+    /* P of row m of a block: written 4 keys, 16 wq + 4 g on, read 8 at a time */
+    const uint32_t pr = M::P + (rg * RB * 16 + m) * 128;
+    const uint32_t pw = pr + (((2 * wq + (g >> 1)) ^ (m >> 1)) << 4) + (g & 1) * 8;
+    const uint32_t stat = M::STAT + (rg * RB * 16 + m) * 16;
+    /* What a unit needs first, all of it on its way at once: Q, then tiles */
+    auto begin = [&] {
 #pragma unroll
         for (int rb = 0; rb < RB; rb++) {
             const bf16 *qp = c.q + ((size_t)(s.q0 + tok_of(rb)) * c.Hq + head_of(rb)) * PD;
@@ -776,68 +847,24 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
             for (int ks = 0; ks < 8; ks++) /* dims as K's pieces below */
                 qf[rb][ks] = *(const bf16x8 *)(qp + (E4M3 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1)
                                                           : 32 * ks + 8 * g));
-        }
-        /* the tree's words of this lane's rows, and of all the unit's tokens together: the first
-         * ones, all there are of up to 64 new tokens */
-        const int i_last = i_first + ((rest + rows - 1) * c.rG >> 16);
-        auto row_words = [&](int tok) { return c.tree + (size_t)(s.q0 + tok) * c.words; };
-        uint64_t word[RB], any_word = *row_words(min(i_first + lane, i_last));
-#pragma unroll
-        for (int rb = 0; rb < RB; rb++)
             word[rb] = *row_words(tok_of(rb));
-        /* Tiles: KiB j NW + wave of a tile is a wave's load j, 2 K rows or 8 V^T rows (e4m3
-         * 4 and 16). Pieces of 16 bytes are swizzled, in the address, so that 16 lanes'
-         * operands hit 16 bank groups: K's piece p of key k in slot p ^ (k & 15), V^T's of
-         * row d in p ^ (d / 2 & 7) (e4m3 d / 4 & 3), P's of row r in p ^ (r / 2 & 7). */
-        auto slice = [&](int page) { return (size_t)max(page, 0) * c.Hkv + kh; };
-        auto issue_k = [&](int t, int page) {
-            const __amdgpu_buffer_rsrc_t src = make_rsrc((const char *)c.k + slice(page) * T, T);
+        }
+        any_word = *row_words(min(i_first + lane, i_last));
 #pragma unroll
-            for (int j = 0; j < L; j++) {
-                const int kib = j * NW + wave, key = E4M3 ? 4 * kib + g : 2 * kib + (lane >> 5);
-                const uint32_t off = E4M3 ? g * 256 + ((m ^ (key & 15)) << 4)
-                                          : (lane >> 5) * 512 + (((lane & 31) ^ (key & 15)) << 4);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                    src, (lds_ptr)(smem + t % NB * T + kib * 1024), 16, off, kib * 1024, 0, 0);
-            }
-            if (E4M3 && wave < 2) /* both operands' scales: V's multiply p */
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                    make_rsrc((wave ? c.vs : c.ks) + slice(page) * PG, 256),
-                    (lds_ptr)(smem + (wave ? M::SV : M::SK) + t % NB * 256), 4, lane * 4, 0, 0, 0);
-        };
-        auto issue_v = [&](int t, int page) {
-            const __amdgpu_buffer_rsrc_t src = make_rsrc((const char *)c.vt + slice(page) * T, T);
+        for (int t = 0; t <= NB; t++)
+            pg[t] = page_of(t);
+        issue_k(0, pg[0]);
 #pragma unroll
-            for (int j = 0; j < L; j++) {
-                const int kib = j * NW + wave;
-                const int d = E4M3 ? 16 * kib + (lane >> 2) : 8 * kib + (lane >> 3);
-                const uint32_t off = E4M3 ? (lane >> 2) * 64 + (((lane & 3) ^ (d >> 2 & 3)) << 4)
-                                          : (lane >> 3) * 128 + (((lane & 7) ^ (d >> 1 & 7)) << 4);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                    src, (lds_ptr)(smem + M::V + t % NB * T + kib * 1024), 16, off, kib * 1024, 0,
-                    0);
-            }
-        };
-        /* all but the newest `nk` of K's groups of loads and `nv` of V^T's are there, and all
-         * waves as far; what is issued past the last tile keeps the count */
-        auto meet = [&](auto nk, auto nv) {
-            constexpr int n = (decltype(nk)::value + decltype(nv)::value) * L;
-            if (E4M3 && wave < 2)
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(n + decltype(nk)::value)
-                             : "memory");
-            else
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(n) : "memory");
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-        };
-        const uint32_t ka = (16 * wq + m) * (T / PG) + ((g ^ m) << 4);
-        const uint32_t va = M::V + (64 * wq + m) * (T / PD) +
-                            ((E4M3 ? g ^ (m >> 2) : g ^ (m >> 1)) << 4);
-        /* P of row m of a block: written 4 keys, 16 wq + 4 g on, read 8 at a time */
-        const uint32_t pr = M::P + (rg * RB * 16 + m) * 128;
-        const uint32_t pw = pr + (((2 * wq + (g >> 1)) ^ (m >> 1)) << 4) + (g & 1) * 8;
-        const uint32_t stat = M::STAT + (rg * RB * 16 + m) * 16;
-
+        for (int t = 0; t < NB - 1; t++) {
+            issue_k(t + 1, pg[t + 1]);
+            issue_v(t, pg[t]);
+        }
+        if (threadIdx.x < 2)
+            *(int *)(smem + M::FLAG + threadIdx.x * 4) = 0;
+    };
+    set_unit();
+    begin();
+    while (true) { /* the units that the piece lies in */
         floatx4 o[RB][4]; /* dims 64 wq + 16 t + 4 g .. + 3 of row m of block rb */
         float mrun[RB], lrun[RB];
 #pragma unroll
@@ -847,16 +874,13 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
             for (int t = 0; t < 4; t++)
                 o[rb][t] = floatx4{};
         }
-        int pg[NB + 1] = {}; /* pages of tiles i .. i + NB */
-        if (threadIdx.x < 2)
-            *(int *)(smem + M::FLAG + threadIdx.x * 4) = 0;
         floatx4 x[RB], vsc;      /* a tile's scores; e4m3: V's scales of the lane's keys */
         float ladd[RB];          /* its sums of p */
         bool foreign = false;    /* it has keys that not all rows see, */
         uint64_t any = ~0ull;    /* and those that some row does */
         /* What the scores of tile i need beside their products */
         auto begin_scores = [&](int i, int page) {
-            const int k0 = pg_tile_page(list, i0 + i) * PG;
+            const int k0 = (i0 + i) * PG;
             foreign = page < 0 || !pg_tile_whole(k0, s.p0 - 1, s.p0 + s.ql - 1, s.kv, 0, 0);
             if constexpr (E4M3)
                 vsc = *(lds_f32x4)(lds + M::SV + i % NB * 256 + (16 * wq + 4 * g) * 4);
@@ -900,7 +924,7 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
             }
         };
         auto end_scores = [&](int i, int page) {
-            const int k0 = pg_tile_page(list, i0 + i) * PG;
+            const int k0 = (i0 + i) * PG;
             if (foreign) {
                 const int left = page >= 0 ? s.kv - k0 : 0; /* keys of the tile, 64 at most count */
                 const uint64_t live = left >= PG ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
@@ -934,19 +958,9 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
                 *(int *)(smem + M::FLAG + (i & 1) * 4) = i + 1;
             write_p(i);
         };
-        /* All of it in one branch: where Q's loads were waited for in another, the compiler
-         * waits for them in the loop again, and for tiles of the next rounds with them */
         if (ntl > 0) {
-#pragma unroll
-            for (int t = 0; t <= NB; t++)
-                pg[t] = page_of(t);
-            issue_k(0, pg[0]);
-#pragma unroll
-            for (int t = 0; t < NB - 1; t++) {
-                issue_k(t + 1, pg[t + 1]);
-                issue_v(t, pg[t]);
-            }
-            /* Q is waited for here, where what was issued after it is known */
+            /* Q is waited for here, where what was issued after it is known: in the loop the
+             * compiler would wait for tiles of the next rounds with it */
 #pragma unroll
             for (int rb = 0; rb < RB; rb++) {
                 asm volatile("" : "+v"(word[rb]));
@@ -980,8 +994,8 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
 #pragma unroll
                     for (int rb = 0; rb < RB; rb++) {
                         const floatx4 all = *(lds_f32x4)(lds + stat + rb * 256);
-                        const float mnew = fmaxf(fmaxf(fmaxf(all[0], all[1]), fmaxf(all[2], all[3])),
-                                                 mrun[rb]);
+                        const float mnew =
+                            fmaxf(fmaxf(fmaxf(all[0], all[1]), fmaxf(all[2], all[3])), mrun[rb]);
                         const float a = fast_exp2(mrun[rb] - (mnew == -INFINITY ? 0.f : mnew));
                         lrun[rb] *= a;
 #pragma unroll
@@ -1001,9 +1015,10 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
 #pragma unroll
                     for (int st = 0; st < 2; st++) /* keys 32 st + 8 g on (e4m3 16 g + 8 st) */
                         p[rb][st] = __builtin_bit_cast(
-                            bf16x8,
-                            lds_read16(lds, pr + (i & 1) * M::PB + rb * 2048 +
-                                                (((E4M3 ? 2 * g + st : 4 * st + g) ^ (m >> 1)) << 4)));
+                            bf16x8, lds_read16(lds, pr + (i & 1) * M::PB + rb * 2048 +
+                                                        (((E4M3 ? 2 * g + st : 4 * st + g) ^
+                                                          (m >> 1))
+                                                         << 4)));
                 /* O^T of tile i, dims 16 t on of the wave's, and scores of tile i + 1 between (past
                  * the last of that one again, for nothing): neither waits for the other's */
                 const uint32_t vbuf = i % NB * T + va, kbuf = (i + 1) % NB * T + ka;
@@ -1069,10 +1084,47 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
                 pg[NB] = page_of(i + 1 + NB);
             }
         }
-        /* nothing is on its way, and all have read */
+        /* this unit's rows, and where they go */
+        const int parts = w.parts, old_rows = rows;
+        const size_t slot = slot_of(c, kh, pg_few_slot(w.first, w.part)) * c.plan.rt;
+        int n[RB], head[RB];
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++)
+            n[rb] = s.q0 + tok_of(rb), head[rb] = head_of(rb);
+        if (w.part == 0 && kh == 0 && c.plan.slots > 0 && threadIdx.x == 0)
+            ((int2 *)c.info)[b * (c.plan.units / c.B) + w.unit] = int2{w.first, w.parts};
+        /* on to the next unit, if the piece goes on after this one */
+        bool more = cut + w.size > w.own + over;
+        if (more) {
+            w.begin += w.own + over, w.first = w.begin / w.size, w.part = 0;
+            if (w.unit + 1 < pg_units(s, c.G, PG_MID)) {
+                w.unit++;
+            } else {
+                more = false;
+                for (int b0 = b + 1; b0 < c.B && !more; b0 += 64) {
+                    const pg_seq t = seq_of(c, min(b0 + lane, c.B - 1));
+                    const uint64_t some = __ballot(b0 + lane < c.B && t.ql > 0);
+                    if (some) {
+                        const int l = __ffsll((unsigned long long)some) - 1;
+                        w.s = seq_at(t, l);
+                        w.b = b0 + l;
+                        w.unit = 0;
+                        w.own = pg_longest(w.s, c.G, PG_LINE, 0, 0);
+                        more = true;
+                    }
+                }
+            }
+            w.parts = (w.begin + w.own - 1) / w.size - w.first + 1;
+        }
+        if (more)
+            set_unit();
+        /* nothing is on its way, and all have read: the next unit's Q and tiles go out ahead of
+         * what is left of this one */
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
+        if (more)
+            begin();
 #pragma unroll
         for (int rb = 0; rb < RB; rb++) { /* l of a row from the four waves' keys */
             const float l = fold_rows(lrun[rb], [](float a, float e) { return a + e; });
@@ -1080,18 +1132,15 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
                 *(float *)(smem + stat + rb * 256 + wq * 4) = l;
         }
         lds_barrier();
-        if (w.part == 0 && kh == 0 && c.plan.slots > 0 && threadIdx.x == 0)
-            ((int2 *)c.info)[b * (c.plan.units / c.B) + w.unit] = int2{w.first, w.parts};
-        const size_t slot = slot_of(c, kh, pg_few_slot(w.first, w.part)) * c.plan.rt;
         const int d0 = 64 * wq + 4 * g;
 #pragma unroll
         for (int rb = 0; rb < RB; rb++) {
             const floatx4 all = *(lds_f32x4)(lds + stat + rb * 256);
             const float l = (all[0] + all[1]) + (all[2] + all[3]);
             const int r = row_of(rb);
-            if (r >= rows)
+            if (r >= old_rows)
                 continue;
-            if (w.parts > 1) {
+            if (parts > 1) {
 #pragma unroll
                 for (int t = 0; t < 4; t++)
                     *(floatx4 *)(c.po + (slot + r) * PD + d0 + 16 * t) = o[rb][t];
@@ -1102,12 +1151,12 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
                 continue;
             }
             const float inv = l > 0.f ? 1.f / l : 0.f;
-            const int n = s.q0 + tok_of(rb), head = head_of(rb);
+            const size_t at = (size_t)n[rb] * c.Hq + head[rb];
             if (c.lse && d0 == 0)
-                c.lse[(size_t)n * c.Hq + head] = lse_of(l, mrun[rb]);
+                c.lse[at] = lse_of(l, mrun[rb]);
             bf16x4 gv[4] = {};
             if (c.gate) {
-                const bf16 *gp = c.gate + (size_t)n * c.gts + (size_t)head * c.ghs + d0;
+                const bf16 *gp = c.gate + (size_t)n[rb] * c.gts + (size_t)head[rb] * c.ghs + d0;
 #pragma unroll
                 for (int t = 0; t < 4; t++)
                     gv[t] = *(const bf16x4 *)(gp + 16 * t);
@@ -1118,29 +1167,11 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
 #pragma unroll
                 for (int e = 0; e < 4; e++)
                     res[e] = f2bf(o[rb][t][e] * inv * (c.gate ? sigmoid_f(bf2f(gv[t][e])) : 1.f));
-                *(bf16x4 *)(c.out + ((size_t)n * c.Hq + head) * PD + d0 + 16 * t) = res;
+                *(bf16x4 *)(c.out + at * PD + d0 + 16 * t) = res;
             }
         }
-        /* on to the next unit, if the piece goes on after this one */
-        const bool more = cut + w.size > w.own + over;
-        w.begin += w.own + over, w.first = w.begin / w.size, w.part = 0;
-        if (more && w.unit + 1 < pg_units(s, c.G, PG_MID)) {
-            w.unit++;
-        } else {
-            w.unit = 0, w.b = -1;
-            for (int b0 = more ? b + 1 : c.B; b0 < c.B; b0 += 64) {
-                const pg_seq t = seq_of(c, min(b0 + lane, c.B - 1));
-                const uint64_t any = __ballot(b0 + lane < c.B && t.ql > 0);
-                if (any) {
-                    const int l = __ffsll((unsigned long long)any) - 1;
-                    w.s = seq_at(t, l);
-                    w.b = b0 + l;
-                    w.own = pg_longest(w.s, c.G, PG_LINE, 0, 0);
-                    break;
-                }
-            }
-        }
-        w.parts = (w.begin + w.own - 1) / w.size - w.first + 1;
+        if (!more)
+            break;
     }
 }
 template <bool E4M3, int RB, int RG>
