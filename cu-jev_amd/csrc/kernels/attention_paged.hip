@@ -782,8 +782,8 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
     };
     auto row_words = [&](int tok) { return c.tree + (size_t)(s.q0 + tok) * c.words; };
     bf16x8 qf[RB][8];
-    /* the tree's words of this lane's rows, and of all the unit's tokens together: the first
-     * ones, all there are of up to 64 new tokens */
+    /* the tree's words of this lane's rows, and of all the unit's tokens together: of up to 64
+     * new tokens the first is all there is */
     uint64_t word[RB], any_word;
     int pg[NB + 1]; /* pages of tiles i .. i + NB */
     /* Tiles: KiB j NW + wave of a tile is a wave's load j, 2 K rows or 8 V^T rows (e4m3
@@ -928,9 +928,7 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
             if (foreign) {
                 const int left = page >= 0 ? s.kv - k0 : 0; /* keys of the tile, 64 at most count */
                 const uint64_t live = left >= PG ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
-                any = live & (s.ql <= 64 ? tree_keys(any_word, k0, s.p0)
-                                         : or_wave(tree_keys(row_words(min(i_first + lane, i_last)),
-                                                             c.words, k0, s.p0)));
+                any = live & tree_keys(any_word, k0, s.p0);
                 if constexpr (E4M3) { /* scales of no key of the call: any bits */
                     const uint32_t some = (uint32_t)(any >> (16 * wq + 4 * g));
 #pragma unroll
@@ -939,10 +937,8 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
                 }
 #pragma unroll
                 for (int rb = 0; rb < RB; rb++) {
-                    const uint64_t own = s.ql <= 64
-                                             ? tree_keys(word[rb], k0, s.p0)
-                                             : tree_keys(row_words(tok_of(rb)), c.words, k0, s.p0);
-                    const uint32_t bits = (uint32_t)((own & live) >> (16 * wq + 4 * g));
+                    const uint64_t own = live & tree_keys(word[rb], k0, s.p0);
+                    const uint32_t bits = (uint32_t)(own >> (16 * wq + 4 * g));
                     unroll_for<4>([&](auto iv) {
                         constexpr int v = decltype(iv)::value;
                         x[rb][v] = hide_by<v>(bits, x[rb][v]);

@@ -258,14 +258,18 @@ constexpr long long pg_mid_units(int N, int B, int max_q, int G) {
     return B * (((long long)pg_min(max_q, N) * G + PG_MID - 1) / PG_MID);
 }
 /* More rows than PG_MID go to tiles of PG_MANY, which read each key once for twice as
- * many, unless there is little to do: up to this many tiles of PG_MID rows and kv-heads */
-constexpr long long PG_MID_LITTLE = 1024;
+ * many, unless there is little to do: up to this many units, and tiles of theirs, of all
+ * kv-heads (16 / 4 heads, bf16: 26 tokens on 530 keys 18.5 us so and 25.8 as PG_MANY, 64 on
+ * 4096 26 and 31, 4 x 20 on 1024 23 and 28; but 64 on 8192 40 and 35, 16 x 20 on 256 25 and
+ * 19.5, and 128 on 2000 38 and 32, whose rows have more words of the tree than one) */
+constexpr int PG_MID_UNITS = 64, PG_MID_TILES = 1024;
 constexpr bool pg_is_mid(int N, int B, int max_q, int max_kv, int G, int Hkv) {
-    const long long rows = (long long)pg_min(max_q, N) * G, units = pg_mid_units(N, B, max_q, G);
-    return rows > PG_FEW && Hkv <= PG_MID_CHIP &&
-           units * pg_div_up(max_kv, PG) <= PG_MOST && /* numbers on the line are ints */
-           (rows <= PG_MID ||
-            (units <= PG_MID_LITTLE && units * pg_div_up(max_kv, PG) * Hkv <= PG_MID_LITTLE));
+    const long long mq = pg_min(max_q, N), units = pg_mid_units(N, B, max_q, G);
+    const int tiles = pg_div_up(max_kv, PG);
+    return mq * G > PG_FEW && mq <= 64 && Hkv <= PG_MID_CHIP &&
+           units * tiles <= PG_MOST && /* numbers on the line are ints */
+           (mq * G <= PG_MID ||
+            (units * Hkv <= PG_MID_UNITS && units * tiles * Hkv <= PG_MID_TILES));
 }
 constexpr int pg_mid_goal(long long units, int Hkv) {
     const int chip = PG_MID_CHIP / Hkv;
@@ -345,8 +349,8 @@ constexpr size_t pg_ws_most(int N, int B, int max_q, int max_kv, int G, int Hkv)
     size_t mid = 0;
     if (mq * G > PG_FEW && most > 1 && Hkv <= PG_MID_CHIP) {
         const long long all = pg_mid_units(N, units, max_q, G);
-        const int m = (int)(all < units ? all : units > PG_MID_LITTLE ? units
-                            : all < PG_MID_LITTLE ? all : PG_MID_LITTLE);
+        const int m = (int)(all < units ? all : units > PG_MID_UNITS ? units
+                            : all < PG_MID_UNITS ? all : PG_MID_UNITS);
         mid = pg_slot_bytes(2 * pg_mid_pieces(m, most, pg_mid_goal(m, Hkv)), PG_MID, Hkv, m, 8);
     }
     return few > many ? (few > mid ? few : mid) : (many > mid ? many : mid);
