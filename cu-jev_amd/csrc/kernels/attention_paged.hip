@@ -888,8 +888,10 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
         auto k_scale = [&](int i) {
             return E4M3 ? *(lds_f32)(lds + M::SK + i % NB * 256 + (16 * wq + m) * 4) : 1.f;
         };
-        auto scores = [&](int j, uint32_t kbuf, float ksc, floatx4 (&y)[RB]) { /* of step j */
-            const u32x4 v = lds_read16(lds, (kbuf ^ ((j & 3) << 6)) + (j >> 2) * 256);
+        auto k_at = [&](int j, uint32_t kbuf) {
+            return lds_read16(lds, (kbuf ^ ((j & 3) << 6)) + (j >> 2) * 256);
+        };
+        auto scores = [&](int j, u32x4 v, float ksc, floatx4 (&y)[RB]) { /* of step j */
 #pragma unroll
             for (int rb = 0; rb < RB; rb++) {
                 const floatx4 in = j ? y[rb] : floatx4{};
@@ -971,7 +973,7 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
             const float ksc = k_scale(0);
 #pragma unroll
             for (int j = 0; j < (E4M3 ? 4 : 8); j++)
-                scores(j, ka, ksc, x);
+                scores(j, k_at(j, ka), ksc, x);
             end_scores(0, pg[0]);
             for (int i = 0; i < ntl; i++) {
                 meet(template_int<NB - 2>{}, template_int<NB - 2>{});
@@ -1035,33 +1037,47 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
                             keep[1][d] = two(e);
                         }
                     }
+                    /* operands of a quarter are read while the one before is worked on */
+                    constexpr int KS = E4M3 ? 1 : 2;
+                    u32x4 kr[2][KS], vr[2][KS];
+                    auto read = [&](int t) {
 #pragma unroll
-                    for (int t = 0; t < 4; t++) {
-                        if constexpr (!E4M3)
-                            scores(2 * t, kbuf, ksc, y);
+                        for (int u = 0; u < KS; u++) {
+                            kr[t & 1][u] = k_at(KS * t + u, kbuf);
+                            vr[t & 1][u] = lds_read16(lds, (vbuf ^ (u << 6)) + t * (1024 * KS));
+                        }
+                    };
+                    read(0);
+                    unroll_for<4>([&](auto it) {
+                        constexpr int t = decltype(it)::value;
+                        if constexpr (t < 3)
+                            read(t + 1);
+                        __builtin_amdgcn_sched_barrier(0);
                         bf16x8 v[2];
                         if constexpr (E4M3) {
-                            u32x4 raw = lds_read16(lds, vbuf + t * 1024);
+                            u32x4 raw = vr[t & 1][0];
                             if constexpr (decltype(masked)::value)
                                 raw &= keep[0];
                             v[0] = widen(raw[0], raw[1], 1.f), v[1] = widen(raw[2], raw[3], 1.f);
                         } else {
 #pragma unroll
                             for (int st = 0; st < 2; st++) {
-                                u32x4 raw = lds_read16(lds, (vbuf ^ (st << 6)) + t * 2048);
+                                u32x4 raw = vr[t & 1][st];
                                 if constexpr (decltype(masked)::value)
                                     raw &= keep[st];
                                 v[st] = __builtin_bit_cast(bf16x8, raw);
                             }
                         }
-                        scores(E4M3 ? t : 2 * t + 1, kbuf, ksc, y);
+#pragma unroll
+                        for (int u = 0; u < KS; u++)
+                            scores(KS * t + u, kr[t & 1][u], ksc, y);
 #pragma unroll
                         for (int rb = 0; rb < RB; rb++)
 #pragma unroll
                             for (int st = 0; st < 2; st++)
                                 o[rb][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
                                     v[st], p[rb][st], o[rb][t], 0, 0, 0);
-                    }
+                    });
                 };
                 if (foreign)
                     products(std::true_type{});
