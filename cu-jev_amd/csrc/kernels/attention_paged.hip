@@ -671,7 +671,7 @@ __global__ __launch_bounds__(64, 2) void attention_few_kernel(Call c) {
  * before the waves have compared their maxima: it stays what it was unless a score is more
  * than MID_OVER above it (then the waves do compare, with two barriers more; each unit's
  * first tile, and few others). The same with three barriers, scores before O^T: 64 sequences'
- * 16 tokens on 4096 keys each 138 us e4m3 and 204 bf16, so 123 and 194 (5.5 TB/s).
+ * 16 tokens on 4096 keys each 138 us e4m3 and 204 bf16, so 118 and 193 (5.6 TB/s).
  * The line of key tiles is cut and merged as for few rows. */
 template <bool E4M3, int RB, int RG> struct Mid {
     static constexpr int T = PSLICE * (E4M3 ? 1 : 2); /* bytes of a K or V^T tile */
