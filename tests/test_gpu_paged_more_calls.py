@@ -113,3 +113,22 @@ def test_weights_of_a_draft_by_its_accepted_rows(e4m3):
         for h in range(16):
             want, tol, _ = eo.attend(a["q"][q0:q0 + ql, h].double(), K[h // 4], seen)
             assert ((a["lse"][q0:q0 + ql, h].double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("slope", [0.02, 0.05, 0.2, -0.2])
+@pytest.mark.parametrize("lens", [[(4, 700), (2, 64)], [(13, 700), (9, 64), (16, 300)],
+                                  [(40, 700), (33, 97)]])
+def test_trees_of_scores_that_rise_from_key_to_key(lens, slope, e4m3):
+    """By more or less a tile than moves the softmax's reference."""
+    c = gt.tree_case(431, 16, 4, e4m3, lens)
+    k = torch.zeros(c["pages"].k.shape)
+    for b, (_, kv) in enumerate(lens):
+        for p in range(kv):
+            k[c["tab"][b][p // PAGE], :, p % PAGE, 0] = slope * p
+    c["pages"].k.copy_(k.to(c["pages"].k.dtype))
+    if e4m3:
+        c["pages"].k_scale.fill_(1.0)
+    c["q"][..., 0] = 1.0
+    got, lse = gt.run(c, c["tree"])
+    gt.check(c, got, lse, gt.tree_seen(c))
