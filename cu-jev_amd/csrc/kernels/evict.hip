@@ -64,8 +64,9 @@ DEV float sum_rows(float a, float b) {
 DEV int key_at(int v, int h) { return 8 * (v >> 2) + 4 * h + (v & 3); }
 
 constexpr int WEIGH_FEW = 128; /* rows */
-/* A wave a page, up to this many: 64 sequences' token on 4096 bf16 keys 97 us, 5.5 TB/s,
- * so, 113 with four pages a wave, the next on its way; 512 on 1024 188 and 196 with two */
+/* A wave a page, up to this many: 64 sequences' token on 4096 bf16 keys 98 us, 5.5 TB/s,
+ * so, 106 with two pages a wave, the next on its way, 113 with four; e4m3 55 (4.9 TB/s), 62
+ * and 67; 512 on 1024 188 and 196 with two */
 constexpr int WEIGH_WAVES = 1 << 20;
 
 /* Few rows: bound by K's bytes. Each of a workgroup's four waves takes a page of the
@@ -197,7 +198,9 @@ __global__ __launch_bounds__(256, 2) void weigh_few_kernel(Weigh c) {
  * packed rows through LDS, 16 for each of its two row groups a step: a Q operand feeds
  * four products, and LDS holds four steps, of which three are on their way. Few blocks
  * of keys share their rows out among several workgroups, whose sums weigh_sum_kernel
- * adds up. */
+ * adds up. Half a step's products go beside the exponentials of the half before. 4096
+ * tokens on 8192 keys, 16 / 4 heads, bf16: 187 us with the sums' 4.5, 1.1 PFLOP/s, 84 %
+ * of a large library product's rate on the same card (1.31). */
 /* lse within it: 2^x and 2^-lse are taken apart, which loses weights below 2^-90 */
 constexpr float LSE_NEAR = 32.f;
 constexpr int WEIGH_KG = 4, WEIGH_AHEAD = 4, WEIGH_GROUPS = 1024, WEIGH_STEPS = 4;
@@ -651,7 +654,10 @@ template <int E> __global__ __launch_bounds__(SEL_T) void select_kernel(Select c
  * rows of dims, an element a slot, and scales and weights. In place a workgroup does its
  * lines or rows of a sequence and kv-head from the front to the back: positions ascend
  * and none is before the slot it goes to, so that all reads of a step are of slots that
- * no step before has written, and those of the step itself are done before its writes. */
+ * no step before has written, and those of the step itself are done before its writes.
+ * Bound by lines where few of a page are kept: 16 x 4096 keys to 1024, bf16, other pages, 33
+ * to 43 us for 135 MB that move, of V^T's 128-byte lines a quarter. In place one sequence of
+ * 8192 to 2048 takes 28, a chain of list, page ids, loads and stores a step. */
 constexpr int KEEP_STEP = 256; /* slots a step, 64 a wave (K) or each wave all (V^T) */
 constexpr int KEEP_VR = 8;     /* rows of V^T a wave */
 struct Keep {
