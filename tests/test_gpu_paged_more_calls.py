@@ -132,3 +132,58 @@ def test_trees_of_scores_that_rise_from_key_to_key(lens, slope, e4m3):
     c["q"][..., 0] = 1.0
     got, lse = gt.run(c, c["tree"])
     gt.check(c, got, lse, gt.tree_seen(c))
+
+
+def test_captured_weights_of_a_prompt_replay_with_other_lengths():
+    """Rows shared out among workgroups, the workspace from torch's allocator in the graph."""
+    o = gp.ops()
+    Hq, Hkv, num_pages, most = 8, 2, 24, 400
+    pages = gp.pool(441, num_pages, Hkv, False)
+    st = dict(q=torch.zeros(most, Hq, D, dtype=torch.bfloat16, device="cuda"),
+              lse=torch.zeros(most, Hq, device="cuda"), qs=gp.i32([0, 200, 400]),
+              kv=gp.i32([200, 300]), tab=gp.i32([list(range(12)), list(range(12, 24))]))
+    w = torch.rand(num_pages, Hkv, PAGE, device="cuda")
+    assert o.kv_weights_ws_bytes(most, 2, 300, 768, Hq, Hkv) > 0
+
+    def weigh():
+        o.kv_weights(st["q"], st["lse"], pages, st["tab"], st["qs"], st["kv"], 300, 768, w, prev=w)
+
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        weigh()
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        weigh()
+    g = torch.Generator().manual_seed(442)
+    for qs, lens in (([0, 200, 400], [200, 768]), ([0, 1, 290], [700, 289]),
+                     ([0, 300, 300], [768, 5]), ([0, 130, 400], [129, 500])):
+        st["q"].copy_((torch.randn(most, Hq, D, generator=g) * gp.Q_SCALE).bfloat16())
+        st["lse"].copy_(5 + torch.rand(most, Hq, generator=g))
+        st["qs"].copy_(torch.tensor(qs, dtype=torch.int32))
+        st["kv"].copy_(torch.tensor(lens, dtype=torch.int32))
+        st["tab"].copy_(torch.randperm(num_pages, generator=g).int().view(2, 12))
+        before = torch.rand(num_pages, Hkv, PAGE, generator=g)
+        w.copy_(before)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = w.clone()
+        w.copy_(before)
+        weigh()
+        torch.cuda.synchronize()
+        assert torch.equal(got, w)
+
+
+@pytest.mark.parametrize("lens", [[(3, 190)], [(13, 190)], [(70, 190)]])
+def test_trees_in_pages_past_32_bits_of_a_pool(lens):
+    """The bits of the same pages at the front of a small pool."""
+    o = gp.ops()
+    c = gt.tree_case(451, 16, 4, False, lens)
+    want, want_lse = gt.run(c, c["tree"])
+    num_pages, ids = 35000, [34999, 33000, 34000]  # 4.6 GB of K, 2^31 elements and more
+    k = torch.zeros(num_pages, 4, PAGE, D, dtype=torch.bfloat16, device="cuda")
+    vt = torch.zeros(num_pages, 4, D, PAGE, dtype=torch.bfloat16, device="cuda")
+    k[ids], vt[ids] = c["pages"].k[c["tab"][0][:3]], c["pages"].vt[c["tab"][0][:3]]
+    got, lse = gt.run({**c, "pages": o.KvPages(k, vt), "tab": [ids]}, c["tree"])
+    assert torch.equal(got, want) and torch.equal(lse, want_lse)
