@@ -477,7 +477,7 @@ static_assert(WEIGH_KG * PG == 256, "a thread a key of a block");
  * (ordered()); the least one kept is found by its digits of 11, 11 and 10 bits from the
  * top, each by a histogram in LDS of what has the digits before. Then positions are
  * counted in order: heavier ones, and of its equals the first. A chain of loads, LDS and
- * barriers: 1 x 8192 keys 13 us, 64 sequences of up to 4096, a workgroup a CU, 11. */
+ * barriers: 1 x 8192 keys 12 us, 64 sequences of up to 4096, a workgroup a CU, 11. */
 constexpr int SEL_T = 1024;
 struct Select {
     const float *w;
@@ -522,7 +522,9 @@ DEV int block_scan(int v, int *scratch, int *total) {
  * read again for each pass over them */
 template <int E> __global__ __launch_bounds__(SEL_T) void select_kernel(Select c) {
     constexpr int SPAN = E * SEL_T, WAVES = SEL_T / 64;
-    __shared__ int hist[2048], scratch[WAVES], found[3], counts[E * WAVES];
+    /* each pass's own: no barrier for their reuse */
+    __shared__ int hist[3][2048], sums[3][WAVES], found[3][3];
+    __shared__ int scratch[WAVES], counts[E * WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int kh = blockIdx.x % c.Hkv, b = blockIdx.x / c.Hkv;
     const int kv = min(max(c.kv_len[b], 0), c.max_kv), n = min(kv, c.budget);
@@ -536,6 +538,8 @@ template <int E> __global__ __launch_bounds__(SEL_T) void select_kernel(Select c
     }
     const int lo = c.sinks, hi = kv - c.recent; /* the positions to choose among */
     const int want = n - c.sinks - c.recent;
+    for (int i = tid; i < 2048; i += SEL_T)
+        hist[0][i] = hist[1][i] = hist[2][i] = 0;
     uint32_t u[E];
     auto load = [&](int from) {
         int page[E];
@@ -554,14 +558,14 @@ template <int E> __global__ __launch_bounds__(SEL_T) void select_kernel(Select c
     };
     load(0);
     const bool again = kv > SPAN;
-    /* the least kept: digits `top` so far under `mask`; ties: how many of its equals */
+    /* the least kept: digits `top` so far under `mask`; ties: how many of its equals, `every`
+     * one there is or not */
     uint32_t top = 0, mask = 0;
     int ties = want;
+    bool every = want == 0;
+    __syncthreads(); /* the histograms are clear */
     for (int pass = 0; want > 0 && pass < 3; pass++) {
         const int bits = pass < 2 ? 11 : 10, shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-        for (int i = tid; i < 2048; i += SEL_T)
-            hist[i] = 0;
-        __syncthreads();
         for (int from = 0; from < kv; from += SPAN) {
             if (again)
                 load(from);
@@ -578,27 +582,34 @@ template <int E> __global__ __launch_bounds__(SEL_T) void select_kernel(Select c
                 const int d = __builtin_amdgcn_readlane(digit, l);
                 const uint64_t same = __ballot(in && digit == d);
                 if (lane == l)
-                    atomicAdd(&hist[d], __popcll(same));
+                    atomicAdd(&hist[pass][d], __popcll(same));
                 if (in && digit != d)
-                    atomicAdd(&hist[digit], 1);
+                    atomicAdd(&hist[pass][digit], 1);
             }
         }
         __syncthreads();
         /* from the top: two digits a thread */
-        const int d1 = 2047 - 2 * tid, c1 = hist[d1], c0 = hist[d1 - 1];
-        int all;
-        const int above = block_scan(c1 + c0, scratch, &all);
+        const int d1 = 2047 - 2 * tid, c1 = hist[pass][d1], c0 = hist[pass][d1 - 1];
+        const int to = wave_scan(c1 + c0);
+        if (lane == 63)
+            sums[pass][wave] = to;
+        __syncthreads();
+        int above = to - c1 - c0;
+#pragma unroll
+        for (int i = 0; i < WAVES; i++)
+            above += i < wave ? sums[pass][i] : 0;
         if (above < ties && above + c1 + c0 >= ties) {
             const bool first = above + c1 >= ties;
-            found[0] = first ? d1 : d1 - 1;
-            found[1] = ties - above - (first ? 0 : c1);
-            found[2] = first ? c1 : c0;
+            found[pass][0] = first ? d1 : d1 - 1;
+            found[pass][1] = ties - above - (first ? 0 : c1);
+            found[pass][2] = first ? c1 : c0;
         }
         __syncthreads();
-        top |= (uint32_t)found[0] << shift;
+        top |= (uint32_t)found[pass][0] << shift;
         mask |= ((1u << bits) - 1) << shift;
-        ties = found[1];
-        if (found[2] == ties) /* all with these digits are kept, whatever the rest are */
+        ties = found[pass][1];
+        every = found[pass][2] == ties;
+        if (every) /* all with these digits are kept, whatever the rest are */
             break;
     }
     /* In order, tile by tile and wave by wave: each wave's count of each tile to LDS, their
@@ -633,14 +644,16 @@ template <int E> __global__ __launch_bounds__(SEL_T) void select_kernel(Select c
             load(from);
         auto at = [&](int e) { return from + e * SEL_T + tid; };
         auto mid = [&](int e) { return at(e) >= lo && at(e) < hi && want > 0; };
-        int rank[E];
-        equal = ranks([&](int e) { return mid(e) && (u[e] & mask) == top; }, equal, rank);
+        int rank[E] = {};
+        if (!every)
+            equal = ranks([&](int e) { return mid(e) && (u[e] & mask) == top; }, equal, rank);
         bool yes[E];
 #pragma unroll
         for (int e = 0; e < E; e++)
-            yes[e] = at(e) < kv && (at(e) < lo || at(e) >= hi ||
-                                    (mid(e) && ((u[e] & mask) > top || ((u[e] & mask) == top &&
-                                                                 rank[e] < ties))));
+            yes[e] = at(e) < kv &&
+                     (at(e) < lo || at(e) >= hi ||
+                      (mid(e) && ((u[e] & mask) > top ||
+                                  ((u[e] & mask) == top && (every || rank[e] < ties)))));
         kept = ranks([&](int e) { return yes[e]; }, kept, rank);
 #pragma unroll
         for (int e = 0; e < E; e++)
