@@ -201,8 +201,6 @@ __global__ __launch_bounds__(256, 2) void weigh_few_kernel(Weigh c) {
  * adds up. Half a step's products go beside the exponentials of the half before. 4096
  * tokens on 8192 keys, 16 / 4 heads, bf16: 187 us with the sums' 4.5, 1.1 PFLOP/s, 84 %
  * of a large library product's rate on the same card (1.31). */
-/* lse within it: 2^x and 2^-lse are taken apart, which loses weights below 2^-90 */
-constexpr float LSE_NEAR = 32.f;
 constexpr int WEIGH_KG = 4, WEIGH_AHEAD = 4, WEIGH_GROUPS = 1024, WEIGH_STEPS = 4;
 template <bool E4M3> DEV void weigh_many(const Weigh &c) {
     constexpr int KG = WEIGH_KG, STEP = 32; /* rows a step, in two halves */
@@ -255,17 +253,13 @@ template <bool E4M3> DEV void weigh_many(const Weigh &c) {
     const int all_steps = pg_div_up(s.ql - t_first, toks);
     const int n0 = (int)((long long)all_steps * split / c.splits);
     const int steps = (int)((long long)all_steps * (split + 1) / c.splits);
-    uint32_t qoff[NL], loff;
+    uint32_t qoff[NL];
 #pragma unroll
     for (int i = 0; i < NL; i++) {
         const int at = (i * KG + wave) * 2 + (lane >> 5), tok = at * c.rG >> 16;
         qoff[i] = tok < toks ? (tok * c.Hq + at - tok * c.G) * PD * 2 +
                                    (((lane & 31) ^ (at & 15)) << 4)
                              : 0x7ffffff0u; /* no row: it reads as 0 */
-    }
-    {
-        const int at = lane & (STEP - 1), tok = at * c.rG >> 16;
-        loff = (tok * c.Hq + at - tok * c.G) * 4;
     }
     /* the most that a descriptor spans: below qoff of no row */
     constexpr size_t SPAN = 0x7fff0000;
@@ -282,11 +276,13 @@ template <bool E4M3> DEV void weigh_many(const Weigh &c) {
         for (int i = 0; i < NL; i++)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 src, (lds_ptr)(smem + n % NB * QB + (i * KG + wave) * 1024), 16, qoff[i], 0, 0, 0);
-        if (wave == 0 && lane < STEP) {
-            const int lbytes = (int)min(left * 4, SPAN);
+        const int at = lane_again(); /* worked out each time, not kept: registers */
+        if (wave == 0 && at < STEP) {
+            const int lbytes = (int)min(left * 4, SPAN), tok = at * c.rG >> 16;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 make_rsrc(c.lse + from, __builtin_amdgcn_readfirstlane(lbytes)),
-                (lds_ptr)(smem + LSE + n % NB * (STEP * 4)), 4, loff, 0, 0, 0);
+                (lds_ptr)(smem + LSE + n % NB * (STEP * 4)), 4,
+                (tok * c.Hq + at - tok * c.G) * 4, 0, 0, 0);
         }
     };
 #pragma unroll
@@ -351,13 +347,12 @@ template <bool E4M3> DEV void weigh_many(const Weigh &c) {
 #pragma unroll
     for (int i = 0; i < 2; i++)
         my_tok[i] = 16 * i + col < toks * c.G ? (16 * i + col) * c.rG >> 16 : 0x7fffffff;
-    /* a half that is done: its lane's factor 2^-lse (0: no row) and lse, the last key that
-     * the row sees, from key0 + 4 g on; whether all is seen, every lse near, and every
-     * row counted but those that read as 0 */
+    /* a half that is done: its lane's lse (+inf: no row, or it sees nothing), the last key
+     * that the row sees, from key0 + 4 g on, and whether all rows see all the wave's keys */
     struct Row {
-        float f, lse;
+        float lse;
         int seen;
-        bool plain;
+        bool whole;
     };
     auto row_of = [&](int n, int half) {
         const float l =
@@ -365,17 +360,16 @@ template <bool E4M3> DEV void weigh_many(const Weigh &c) {
         const int tok = my_tok[half];
         const int i0 = first_tok(n); /* the last step's tokens end where the others began */
         const bool there = tok < s.ql - n * toks - i0;
-        const bool near = __all(fabsf(l) <= LSE_NEAR), whole = s.p0 + i0 >= key0 + PG - 1;
         Row r;
-        r.f = there ? fast_exp2(-l) : 0.f;
         r.lse = there && l != -INFINITY ? l : INFINITY;
-        r.seen = whole ? PG : s.p0 + i0 + min(tok, STEP) - key0 - 4 * g;
-        r.plain = near && whole && (n + 1) * (long long)toks <= s.ql - t_first;
+        r.whole = s.p0 + i0 >= key0 + PG - 1;
+        r.seen = r.whole ? PG : s.p0 + i0 + min(tok, STEP) - key0 - 4 * g;
         return r;
     };
-    /* 2^x 2^-lse: a product added at once, no difference before. A row's x is at most its lse. */
-    auto add_plain = [&](const floatx4 (&x)[4], float f, int m) {
-        sum[m >> 2][m & 3] = __builtin_fmaf(fast_exp2(x[m >> 2][m & 3]), f, sum[m >> 2][m & 3]);
+    /* The difference before the power: 2^x times 2^-lse would be a product added at once, but
+     * either may leave fp32's range where the weight does not */
+    auto add_whole = [&](const floatx4 (&x)[4], float lse, int m) {
+        sum[m >> 2][m & 3] += fast_exp2(x[m >> 2][m & 3] - lse);
     };
     auto add = [&](const floatx4 (&x)[4], const Row &r) {
 #pragma unroll
@@ -386,18 +380,18 @@ template <bool E4M3> DEV void weigh_many(const Weigh &c) {
     };
     /* a half's products into y, and beside them what x has of the half before */
     auto turn = [&](auto ih, uint32_t q0, floatx4 (&y)[4], const floatx4 (&x)[4], const Row &r) {
-        if (r.plain) {
+        if (r.whole) {
             products(ih, q0, y, [&](auto iks) {
                 constexpr int ks = decltype(iks)::value;
-                add_plain(x, r.f, 2 * ks);
-                add_plain(x, r.f, 2 * ks + 1);
+                add_whole(x, r.lse, 2 * ks);
+                add_whole(x, r.lse, 2 * ks + 1);
             });
         } else {
             add(x, r);
             products(ih, q0, y, [](auto) {});
         }
     };
-    Row before{0.f, INFINITY, 0, true}; /* ahead of the first half: nothing */
+    Row before{INFINITY, 0, true}; /* ahead of the first half: nothing */
     for (int n = n0; n < steps; n++) {
         /* step n's Q is there, and that of n - 1 read: its place takes step n + NB - 1's */
         if (wave == 0)
@@ -419,21 +413,22 @@ template <bool E4M3> DEV void weigh_many(const Weigh &c) {
     add(xb, before);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     /* over the 16 rows' lanes: lane 16 g + m is left with block m >> 2, number m & 3 */
+    const int id = lane_again();
     float mine = 0.f;
 #pragma unroll
     for (int m = 0; m < 16; m++) {
         const float y = fold_row(sum[m >> 2][m & 3], [](float p, float q) { return p + q; });
-        mine = col == m ? y : mine;
+        mine = (id & 15) == m ? y : mine;
     }
     /* and left with key l of the wave's in lane l */
-    mine = __shfl(mine, (lane >> 2 & 3) * 16 + (lane >> 4) * 4 + (lane & 3), 64);
+    mine = __shfl(mine, (id >> 2 & 3) * 16 + (id >> 4) * 4 + (id & 3), 64);
     {
         if (c.splits > 1) {
             c.parts[(((size_t)split * c.B + b) * c.Hkv + kh) * c.blocks * (KG * PG) + key0 +
-                    lane] = mine;
-        } else if (page >= 0 && key0 + lane < s.kv) {
-            const size_t to = slice * PG + lane;
-            if (c.prev && key0 + lane < s.p0)
+                    id] = mine;
+        } else if (page >= 0 && key0 + id < s.kv) {
+            const size_t to = slice * PG + id;
+            if (c.prev && key0 + id < s.p0)
                 mine += c.prev[to];
             c.w[to] = mine;
         }

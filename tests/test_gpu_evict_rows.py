@@ -1,5 +1,5 @@
-"""GPU tests of attention weights by key: up to 128 rows, waves of several pages; against
-the float64 form of evict_oracle.py."""
+"""GPU tests of attention weights by key: up to 128 rows, waves of several pages, weights
+at the ends of fp32; against the float64 form of evict_oracle.py."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -44,3 +44,26 @@ def test_weights_of_many_sequences_without_rows(Hkv, lens, B, e4m3):
                  w, prev=c["prev"].cuda())
     torch.cuda.synchronize()
     ge.check_weights(c, w.cpu())
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("lens", [[(200, 600)], [(16, 600)]])
+@pytest.mark.parametrize("most,lse", [(-26.0, None), (128.0, 31.0), (3.0, -31.0)])
+def test_weights_at_the_ends_of_fp32(lens, most, lse, e4m3):
+    """Weights of 2^-110, and of 2^97 by another lse than the rows' own: q.k alone is past
+    the ends of fp32's exponent."""
+    c = gp.attention_case(681, 8, 2, e4m3, lens)
+    k = torch.zeros(c["pages"].k.shape)
+    k[..., 0] = most
+    k[:, :, 5::16, 0] = -128.0
+    c["pages"].k.copy_(k.to(c["pages"].k.dtype))
+    if e4m3:
+        c["pages"].k_scale.fill_(1.0)
+    c["q"].zero_()
+    c["q"][..., 0] = 1.0
+    c = ge.fill(c, 682)
+    if lse is not None:
+        c["lse"].fill_(lse)
+    for name in ("prev", "w"):
+        c[name].zero_()
+    ge.check_weights(c, ge.weigh(c))
