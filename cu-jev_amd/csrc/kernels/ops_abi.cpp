@@ -319,6 +319,12 @@ static int paged_heads_ok(int Hq, int Hkv) {
     return Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Hq / Hkv <= 16 && Hq <= 8192;
 }
 
+/* Whether n values of 4 bytes at a and m of them at b have one in common */
+static bool overlap(const void *a, size_t n, const void *b, size_t m) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return a && b && x < y + m * 4 && y < x + n * 4;
+}
+
 static int prep_paged(const char *what, const void *proj, int proj_stride, const float *q_norm_w,
                       const float *k_norm_w, const int32_t *pos, int axes, uint64_t axis_of,
                       const int32_t *q_start, const int32_t *kv_len, const int32_t *page_table,
@@ -589,6 +595,10 @@ EXPORT int cujev_op_kv_keep(int kv_type, void *k_pages, void *vt_pages, float *k
         return st;
     if (to_table && (to_pages <= 0 || to_pages > PG_MOST_KEYS / CUJEV_KV_PAGE))
         return fail(1, "kv_keep: bad table to write to (to_pages=%d)", to_pages);
+    /* into other pages all steps run at once: a slot may be written before it is read */
+    if (overlap(to_table, (size_t)B * to_pages, page_table, (size_t)B * max_pages))
+        return fail(1, "kv_keep: to_table must be another array than page_table, of other pages "
+                       "(none: in place)");
     if (max_keep < 0 || max_keep > PG_MOST_KEYS || (keep_heads != 1 && keep_heads != Hkv))
         return fail(1, "kv_keep: keep is [B][%d][%d], not of 1 or %d heads", keep_heads, max_keep,
                     Hkv);

@@ -582,7 +582,7 @@ def kv_keep(pages, page_table, keep, keep_len, dst=None, to_table=None, weights=
     """Position dst[b] + i (dst None: i) of sequence b takes K, V, scales and weight of its
     position keep[b, h, i], i < keep_len[b]; keep [B, Hkv, n], or [B, 1, n] for all
     kv-heads. In place, where keep has to ascend and be nowhere less than dst[b] + i; or,
-    with to_table [B, to_pages], into pages that page_table does not have."""
+    with to_table [B, to_pages], another tensor, into pages that page_table does not have."""
     import torch
     dev, B = _paged_seqs(pages, page_table, keep_len)
     i32 = torch.int32

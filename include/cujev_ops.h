@@ -373,8 +373,9 @@ int cujev_op_kv_select(const float *weights, int num_pages, int Hkv, const int32
  * keys or a draft's accepted path come to lie in a row. to_table NULL: in place; keep
  * then ascends and keep[b][h][i] >= dst[b] + i (what other lists give is not defined,
  * but stays within the sequence's pages). Otherwise to_table [B][to_pages] has pages
- * that no page_table of the call has. An entry whose source or goal is no position of a
- * page that is there moves nothing. */
+ * that no page_table of the call has, and is another array (one that overlaps page_table is
+ * refused). An entry whose source or goal is no position of a page that is there moves
+ * nothing. */
 int cujev_op_kv_keep(int kv_type, void *k_pages, void *vt_pages, float *k_scale, float *v_scale,
                      float *weights, int num_pages, int Hkv, const int32_t *page_table,
                      int max_pages, const int32_t *to_table, int to_pages, int B,

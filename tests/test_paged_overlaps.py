@@ -1,0 +1,22 @@
+"""Arrays of a call that may not overlap, refused on the CPU by the host's checks before
+anything is launched. The base cases are test_paged_more_args.py's."""
+import pytest
+
+pytest.importorskip("torch")
+
+from test_paged_args import FAKE, INVALID  # noqa: E402
+from test_paged_more_args import KEEP, call  # noqa: E402
+
+
+@pytest.mark.parametrize("at", [0, 4, 28, -4, -20])
+def test_keep_refuses_a_goal_that_is_its_source(at):
+    """4 sequences of 2 pages to 3 each: in place is to_table NULL."""
+    bad = dict(B=4, to_table=FAKE + at, to_pages=3)
+    st, msg = call(KEEP, **bad)
+    assert st == INVALID and "to_table" in msg
+
+
+@pytest.mark.parametrize("at", [0, 32, -48])
+def test_keep_takes_tables_that_do_not_overlap(at):
+    """Nothing to keep: no launch. No sequence: no array."""
+    assert call(KEEP, B=4 if at else 0, to_table=FAKE + at, to_pages=3, max_keep=0)[0] == 0
