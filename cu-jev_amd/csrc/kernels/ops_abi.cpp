@@ -576,7 +576,7 @@ EXPORT int cujev_op_kv_select(const float *weights, int num_pages, int Hkv,
                     budget, sinks, recent, max_keep);
     if (B > 0 && (!weights || !page_table || !kv_len || (!keep && max_keep > 0) || !keep_len))
         return fail(1, "kv_select: null argument");
-    if (B > 0 && keep_len == kv_len) /* other kv-heads read kv_len while one writes */
+    if (overlap(keep_len, B, kv_len, B)) /* other kv-heads read kv_len while one writes */
         return fail(1, "kv_select: keep_len must be another array than kv_len");
     const cujev_paged_seqs seqs = {nullptr, kv_len, page_table, max_pages, B};
     return launched(k_kv_select(weights, num_pages, Hkv, &seqs, max_kv, budget, sinks, recent,

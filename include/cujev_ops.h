@@ -361,7 +361,8 @@ size_t cujev_ops_kv_weights_ws_bytes(int N, int B, int max_q, int max_kv, int Hq
  * row stays as it was. Where that is not all: the first `sinks`, the last `recent`
  * (together at most budget), and of the others those of the largest weight, the lowest
  * position first among equals (-0 equals 0; NaN counts as the largest; keys of a page
- * that is not there as the least). keep_len is another array than kv_len. */
+ * that is not there as the least). keep_len is another array than kv_len, and has no
+ * element of it. */
 int cujev_op_kv_select(const float *weights, int num_pages, int Hkv, const int32_t *page_table,
                        int max_pages, const int32_t *kv_len, int B, int max_kv, int budget,
                        int sinks, int recent, int32_t *keep, int max_keep, int32_t *keep_len,

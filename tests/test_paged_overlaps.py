@@ -5,7 +5,7 @@ import pytest
 pytest.importorskip("torch")
 
 from test_paged_args import FAKE, INVALID  # noqa: E402
-from test_paged_more_args import KEEP, call  # noqa: E402
+from test_paged_more_args import KEEP, SELECT, call  # noqa: E402
 
 
 @pytest.mark.parametrize("at", [0, 4, 28, -4, -20])
@@ -20,3 +20,10 @@ def test_keep_refuses_a_goal_that_is_its_source(at):
 def test_keep_takes_tables_that_do_not_overlap(at):
     """Nothing to keep: no launch. No sequence: no array."""
     assert call(KEEP, B=4 if at else 0, to_table=FAKE + at, to_pages=3, max_keep=0)[0] == 0
+
+
+@pytest.mark.parametrize("at", [4, -4, 28, -28])
+def test_select_refuses_lengths_that_it_writes_over(at):
+    """A kv-head writes what the others of its sequence, or of the next, still read."""
+    st, msg = call(SELECT, B=8, kv_len=FAKE, keep_len=FAKE + at)
+    assert st == INVALID and "keep_len" in msg
