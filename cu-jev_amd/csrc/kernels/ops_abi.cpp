@@ -541,6 +541,9 @@ EXPORT int cujev_op_kv_weights(const void *q, const float *lse, int kv_type, con
         return fail(1, "kv_weights: null argument");
     if (((uintptr_t)q & 15) || (((uintptr_t)lse | (uintptr_t)prev | (uintptr_t)weights) & 3))
         return fail(1, "kv_weights: q must be 16-byte, lse and weights 4-byte aligned");
+    const size_t slots = (size_t)num_pages * Hkv * CUJEV_KV_PAGE;
+    if (prev != weights && overlap(prev, slots, weights, slots)) /* written before it is read */
+        return fail(1, "kv_weights: prev must be weights itself or another array");
     const size_t need = cujev_kv_weights_ws_bytes(N, B, max_q, max_kv, Hq, Hkv);
     if (need > 0 && (!ws || ((uintptr_t)ws & 3) || ws_bytes < need))
         return fail(6, "kv_weights: needs a 4-byte aligned workspace of %zu bytes, got %zu", need,

@@ -341,10 +341,10 @@ int cujev_op_attention_paged_tree(const void *q, const void *gate, int gate_tok_
  *   weights[j] = prev[j] + sum of 2^(q[n][h] . k_j - lse[n][h])
  * over its rows n that see j, causally, and the q-heads h of the kv-head: with the lse of
  * their attention, a call without a window over the same keys, what the softmax gave (of a
- * draft, once its accepted tokens lie in a row: their rows of q and lse). prev counts for the keys before the new
- * tokens, whose own weights start here; it may be weights itself, or NULL (all start
- * here, as for a whole prompt). A row whose lse is -inf adds nothing. Keys of any value
- * where no row sees them. The sum's order
+ * draft, once its accepted tokens lie in a row: their rows of q and lse). prev counts for
+ * the keys before the new tokens, whose own weights start here; it may be weights itself,
+ * or NULL (all start here, as for a whole prompt), but not overlap it otherwise. A row
+ * whose lse is -inf adds nothing. Keys of any value where no row sees them. The sum's order
  * depends on the call's sizes alone. Sequences without new tokens are left as they were.
  * ws: device workspace that need not be cleared, 4-byte aligned; calls that may overlap
  * need one each. cujev_ops_kv_weights_ws_bytes() is enough for the call of its

@@ -5,7 +5,7 @@ import pytest
 pytest.importorskip("torch")
 
 from test_paged_args import FAKE, INVALID  # noqa: E402
-from test_paged_more_args import KEEP, SELECT, call  # noqa: E402
+from test_paged_more_args import KEEP, SELECT, WEIGHTS, call  # noqa: E402
 
 
 @pytest.mark.parametrize("at", [0, 4, 28, -4, -20])
@@ -27,3 +27,16 @@ def test_select_refuses_lengths_that_it_writes_over(at):
     """A kv-head writes what the others of its sequence, or of the next, still read."""
     st, msg = call(SELECT, B=8, kv_len=FAKE, keep_len=FAKE + at)
     assert st == INVALID and "keep_len" in msg
+
+
+@pytest.mark.parametrize("at", [4, -4, 256 * 8 - 4, 4 - 256 * 8])
+def test_weights_refuse_what_was_written_over_before_it_is_read(at):
+    """4 pages of 2 kv-heads: weights of one slot where prev has another's."""
+    st, msg = call(WEIGHTS, N=1, B=1, prev=FAKE + at)
+    assert st == INVALID and "prev" in msg
+
+
+def test_weights_take_prev_beside_them():
+    """No rows: no launch."""
+    for at in (0, 256 * 8, -256 * 8):
+        assert call(WEIGHTS, B=1, prev=FAKE + at)[0] == 0
