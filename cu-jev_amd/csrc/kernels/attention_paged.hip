@@ -2078,6 +2078,10 @@ using namespace CUJEV_KNS;
 extern "C" size_t cujev_attention_paged_ws_bytes(int N, int B, int max_q, int max_kv, int Hq,
                                                  int Hkv, int window, int sinks, int type) {
     (void)type, (void)window, (void)sinks; /* enough for either type and any window */
+    return pg_ws_causal(N, B, max_q, max_kv, Hq / Hkv, Hkv);
+}
+extern "C" size_t cujev_attention_paged_tree_ws_bytes(int N, int B, int max_q, int max_kv, int Hq,
+                                                      int Hkv) {
     return pg_ws_most(N, B, max_q, max_kv, Hq / Hkv, Hkv);
 }
 
@@ -2143,7 +2147,7 @@ extern "C" hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int
               max_q, max_kv, Hq, Hkv, G, window, sinks,
               all ? 0 : window, all ? 0 : sinks, pg_div_up(65536, G), tree, tree_words, lse,
               (bf16 *)out, (float *)ws, nullptr, nullptr, nullptr, {}};
-    if (tree && pg_is_mid(N, B, max_q, max_kv, G, Hkv))
+    if (tree && pg_takes_mid(N, B, max_q, max_kv, G, Hkv, ws_bytes))
         return attend_middling(c, Hkv, e4m3, ws_bytes, stream);
     const pg_plan p = c.plan = pg_make_plan(N, B, max_q, max_kv, G, Hkv, window, sinks);
     if (p.shares == 0)

@@ -299,10 +299,12 @@ hipError_t k_attention_paged(const bf16_t *q, const bf16_t *gate, int gate_tok_s
                              int window, int sinks, const uint64_t *tree, int tree_words,
                              bf16_t *out, float *lse, void *ws, size_t ws_bytes,
                              hipStream_t stream);
-/* Enough for that call and every one of the same heads that is no larger in N, B, max_q
- * and max_kv, of either type and any window. */
+/* Enough for that call without a tree and every one of the same heads that is no larger
+ * in N, B, max_q and max_kv, of either type and any window; and with trees at their
+ * fastest. (A tree's call takes a slower form where the workspace is enough for that.) */
 size_t cujev_attention_paged_ws_bytes(int N, int B, int max_q, int max_kv, int Hq, int Hkv,
                                       int window, int sinks, int type);
+size_t cujev_attention_paged_tree_ws_bytes(int N, int B, int max_q, int max_kv, int Hq, int Hkv);
 
 /* ---- eviction from the paged cache (evict.hip) --------------------------------
  * weights[page][kv-head][slot] fp32, beside the pages. For each sequence with new

@@ -449,13 +449,15 @@ static int attend_paged(const char *what, const void *q, const void *gate, int g
                        "window, got %d and window=%d",
                     what, pg_min(max_q, N), pg_div_up(pg_min(max_q, N), 64), tree_words, window);
     const int G = Hq / Hkv;
+    if (!ws)
+        ws_bytes = 0;
     const size_t need =
-        tree && pg_is_mid(N, B, max_q, max_kv, G, Hkv)
+        tree && pg_takes_mid(N, B, max_q, max_kv, G, Hkv, ws_bytes)
             ? pg_mid_ws_bytes(pg_make_mid_plan(N, B, max_q, max_kv, G, Hkv), Hkv)
             : pg_ws_bytes(pg_make_plan(N, B, max_q, max_kv, G, Hkv, window, sinks), Hkv);
-    if (need > 0 && (!ws || ((uintptr_t)ws & 15) || ws_bytes < need))
+    if (need > 0 && (((uintptr_t)ws & 15) || ws_bytes < need))
         return fail(6, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", what,
-                    need, ws ? ws_bytes : (size_t)0);
+                    need, ws_bytes);
     const cujev_paged_seqs seqs = {q_start, kv_len, page_table, max_pages, B};
     return launched(k_attention_paged((const bf16_t *)q, (const bf16_t *)gate, gate_tok_stride,
                                       gate_head_stride, &pages, &seqs, N, max_q, max_kv, Hq,
@@ -517,6 +519,13 @@ EXPORT size_t cujev_ops_attention_paged_ws_bytes(int N, int B, int max_q, int ma
     if (!paged_heads_ok(Hq, Hkv))
         return 0;
     return cujev_attention_paged_ws_bytes(N, B, max_q, max_kv, Hq, Hkv, window, sinks, kv_type);
+}
+
+EXPORT size_t cujev_ops_attention_paged_tree_ws_bytes(int N, int B, int max_q, int max_kv, int Hq,
+                                                      int Hkv) {
+    if (!paged_heads_ok(Hq, Hkv))
+        return 0;
+    return cujev_attention_paged_tree_ws_bytes(N, B, max_q, max_kv, Hq, Hkv);
 }
 
 EXPORT int cujev_op_kv_weights(const void *q, const float *lse, int kv_type, const void *k_pages,

@@ -332,11 +332,11 @@ constexpr size_t pg_ws_bytes(const pg_plan &p, int Hkv) {
     return p.rt == PG_FEW ? pg_slot_bytes(p.slots, p.rt, Hkv, p.units, 8)
                           : pg_slot_bytes(p.slots, p.rt, Hkv, p.slots, 16);
 }
-/* The most that a call of these heads can need whose N, B, max_q and max_kv are these or
- * less, whatever its window: a prompt's rows fill the chip and leave nothing to merge,
- * and the steps after it, smaller calls, do. Slots rise with B and max_kv up to what
- * the chip runs at once, so that it is about 34 MB at the very most. */
-constexpr size_t pg_ws_most(int N, int B, int max_q, int max_kv, int G, int Hkv) {
+/* The most that a call of these heads without a tree can need whose N, B, max_q and
+ * max_kv are these or less, whatever its window: a prompt's rows fill the chip and leave
+ * nothing to merge, and the steps after it, smaller calls, do. Slots rise with B and
+ * max_kv up to what the chip runs at once, so that it is about 34 MB at the very most. */
+constexpr size_t pg_ws_causal(int N, int B, int max_q, int max_kv, int G, int Hkv) {
     const long long mq = pg_min(max_q, N);
     if (mq <= 0 || B <= 0)
         return 0;
@@ -346,6 +346,18 @@ constexpr size_t pg_ws_most(int N, int B, int max_q, int max_kv, int G, int Hkv)
     const size_t few = pg_slot_bytes(most > 1 ? 2 * pieces : 0, PG_FEW, Hkv, units, 8);
     const int goal = mq * G > PG_FEW && pg_many_long(most) ? pg_many_goal(Hkv) : 0;
     const size_t many = pg_slot_bytes(goal, PG_MANY, Hkv, goal, 16);
+    return few > many ? few : many;
+}
+/* The same with draft trees among the calls. Their units of PG_MID rows, cut where
+ * other calls are whole, take more on short contexts (8 sequences' 8 tokens on 512 keys,
+ * 4 kv-heads, 34 MB for 4); with less they are tiles of PG_MANY. */
+constexpr size_t pg_ws_most(int N, int B, int max_q, int max_kv, int G, int Hkv) {
+    const long long mq = pg_min(max_q, N);
+    if (mq <= 0 || B <= 0)
+        return 0;
+    const size_t causal = pg_ws_causal(N, B, max_q, max_kv, G, Hkv);
+    const int most = pg_div_up(pg_max(max_kv, 0), PG);
+    const int units = pg_min(B, PG_MOST_UNITS / Hkv);
     size_t mid = 0;
     if (mq * G > PG_FEW && most > 1 && Hkv <= PG_MID_CHIP) {
         const long long all = pg_mid_units(N, units, max_q, G);
@@ -353,7 +365,13 @@ constexpr size_t pg_ws_most(int N, int B, int max_q, int max_kv, int G, int Hkv)
                             : all < PG_MID_UNITS ? all : PG_MID_UNITS);
         mid = pg_slot_bytes(2 * pg_mid_pieces(m, most, pg_mid_goal(m, Hkv)), PG_MID, Hkv, m, 8);
     }
-    return few > many ? (few > mid ? few : mid) : (many > mid ? many : mid);
+    return causal > mid ? causal : mid;
+}
+/* Whether a tree's call takes units of PG_MID rows: where that is the faster form, and the
+ * workspace has room for its parts (1 x 26 tokens on 530 keys 18 us so and 26 without) */
+constexpr bool pg_takes_mid(int N, int B, int max_q, int max_kv, int G, int Hkv, size_t ws) {
+    return pg_is_mid(N, B, max_q, max_kv, G, Hkv) &&
+           pg_mid_ws_bytes(pg_make_mid_plan(N, B, max_q, max_kv, G, Hkv), Hkv) <= ws;
 }
 
 /* The row at position p sees the keys j <= min(p, kv - 1) with j > pg_low or j <

@@ -115,6 +115,8 @@ def load():
     lib.cujev_ops_attention_ws_bytes.restype = C.c_size_t
     lib.cujev_ops_attention_paged_ws_bytes.argtypes = [_I] * 9
     lib.cujev_ops_attention_paged_ws_bytes.restype = C.c_size_t
+    lib.cujev_ops_attention_paged_tree_ws_bytes.argtypes = [_I] * 6
+    lib.cujev_ops_attention_paged_tree_ws_bytes.restype = C.c_size_t
     lib.cujev_ops_kv_weights_ws_bytes.argtypes = [_I] * 6
     lib.cujev_ops_kv_weights_ws_bytes.restype = C.c_size_t
     lib.cujev_ops_blaslt_version.argtypes = []
@@ -135,7 +137,7 @@ def exported_symbols():
     return ["cujev_ops_kv_stride", "cujev_ops_last_error", "cujev_ops_gdn_scratch_bytes",
             "cujev_ops_gemm_small_splits", "cujev_ops_gemm_plan", "cujev_ops_gemm_wide_plan",
             "cujev_ops_attention_ws_bytes", "cujev_ops_attention_paged_ws_bytes",
-            "cujev_ops_kv_weights_ws_bytes",
+            "cujev_ops_attention_paged_tree_ws_bytes", "cujev_ops_kv_weights_ws_bytes",
             "cujev_ops_blaslt_version", "cujev_op_gemm_tune", *_SIGS]
 
 
@@ -431,10 +433,14 @@ def kv_page_read(pages, page_table, kv_len, max_kv, k_cache, vt_cache):
                 vt_cache.data_ptr(), stride)
 
 
-def attention_paged_ws_bytes(N, B, max_q, max_kv, Hq, Hkv, window=0, sinks=0, e4m3=False) -> int:
+def attention_paged_ws_bytes(N, B, max_q, max_kv, Hq, Hkv, window=0, sinks=0, e4m3=False,
+                             tree=False) -> int:
     """Bytes that are enough for this call and for every smaller one of the same heads (N,
-    B, max_q and max_kv no larger), whatever its window and type."""
+    B, max_q and max_kv no larger), whatever its window and type; with tree, for those of
+    draft trees among them, which take more on short contexts."""
     _need_ints("attention_paged_ws_bytes", N, B, max_q, max_kv, Hq, Hkv, window, sinks)
+    if tree:
+        return int(load().cujev_ops_attention_paged_tree_ws_bytes(N, B, max_q, max_kv, Hq, Hkv))
     return int(load().cujev_ops_attention_paged_ws_bytes(N, B, max_q, max_kv, Hq, Hkv, window,
                                                          sinks, int(e4m3)))
 
@@ -450,7 +456,8 @@ def attention_paged(q, gate, gate_tok_stride, gate_head_stride, pages, page_tabl
     tree int64 [N, words], words at least min(max_q, N) / 64 rounded up: the rows of a
     sequence are drafted tokens that see all keys before them and, of each other, those
     whose bits are set (row i's ancestors and its own: bit j % 64 of word j // 64 is new
-    token j); no window. lse float32 [N, Hq] gets the softmax's log2 of the sum of 2^(q.k)."""
+    token j); no window. Where ws is less than a tree's workspace (tree=True), the call takes
+    one from torch's allocator. lse float32 [N, Hq] gets the softmax's log2 of the sum of 2^(q.k)."""
     import torch
     dev, B = _paged_seqs(pages, page_table, kv_len, q_start)
     if (max_q | max_kv | window | sinks | gate_tok_stride | gate_head_stride) >> 31:
@@ -490,6 +497,10 @@ def attention_paged(q, gate, gate_tok_stride, gate_head_stride, pages, page_tabl
             _need("tree", tree, torch.int64, dev, (N, words))
         if window or sinks:
             raise OpsError(f"attention_paged: window={window} sinks={sinks} do not go with a tree")
+        want = (_lib or load()).cujev_ops_attention_paged_tree_ws_bytes(
+            N, B, max_q, max_kv, Hq, pages.Hkv) if dev >= 0 else 0
+        if size < want:
+            ws, size = torch.empty(want, dtype=torch.uint8, device=q.device), want
         # no rows: an empty tensor has no address
         seen, stats = (tree.data_ptr() or 8, words), stats or (None,)
     _paged_call(dev, name, q.data_ptr(),

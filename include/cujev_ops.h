@@ -313,7 +313,10 @@ int cujev_op_attention_paged_lse(const void *q, const void *gate, int gate_tok_s
  * is set (its ancestors' and its own; any other bits are as good, later tokens' too).
  * Bits of tokens that the sequence does not have are not read. K of any value, V of
  * any value where no row of the call sees the key. lse as above, or NULL. No window;
- * all else, the workspace too, as for cujev_op_attention_paged. */
+ * all else as for cujev_op_attention_paged. Its workspace is enough for a tree, too; with
+ * that of cujev_ops_attention_paged_tree_ws_bytes() (as large a call's, and every smaller
+ * one's, with trees or without; at most 34 MB and 8 bytes a sequence) trees of 17 to 64
+ * rows max_q * Hq / Hkv, or on few keys, take a faster form. */
 int cujev_op_attention_paged_tree(const void *q, const void *gate, int gate_tok_stride,
                                   int gate_head_stride, int kv_type, const void *k_pages,
                                   const void *vt_pages, const float *k_scale,
@@ -322,6 +325,8 @@ int cujev_op_attention_paged_tree(const void *q, const void *gate, int gate_tok_
                                   int B, int N, int max_q, int max_kv, int Hq, int Hkv,
                                   const void *tree, int tree_words, void *out, float *lse,
                                   void *ws, size_t ws_bytes, void *stream);
+size_t cujev_ops_attention_paged_tree_ws_bytes(int N, int B, int max_q, int max_kv, int Hq,
+                                               int Hkv);
 
 /* ---- eviction from the paged cache ----------------------------------------------
  * No counterpart in the reference, whose caches only grow. Three calls on a stream,
