@@ -253,6 +253,13 @@ template <bool E4M3> DEV void weigh_many(const Weigh &c) {
     const int all_steps = pg_div_up(s.ql - t_first, toks);
     const int n0 = (int)((long long)all_steps * split / c.splits);
     const int steps = (int)((long long)all_steps * (split + 1) / c.splits);
+    auto part = [&](int k) { /* key0 + k's place among this split's sums */
+        return c.parts + (((size_t)split * c.B + b) * c.Hkv + kh) * c.blocks * (KG * PG) + key0 + k;
+    };
+    if (n0 == steps) { /* uniform: fewer steps than splits, and none is this one's */
+        *part(lane) = 0.f;
+        return;
+    }
     uint32_t qoff[NL];
 #pragma unroll
     for (int i = 0; i < NL; i++) {
@@ -424,8 +431,7 @@ template <bool E4M3> DEV void weigh_many(const Weigh &c) {
     mine = __shfl(mine, (id >> 2 & 3) * 16 + (id >> 4) * 4 + (id & 3), 64);
     {
         if (c.splits > 1) {
-            c.parts[(((size_t)split * c.B + b) * c.Hkv + kh) * c.blocks * (KG * PG) + key0 +
-                    id] = mine;
+            *part(id) = mine;
         } else if (page >= 0 && key0 + id < s.kv) {
             const size_t to = slice * PG + id;
             if (c.prev && key0 + id < s.p0)
