@@ -196,7 +196,7 @@ DEV void set_part(const Call &c, Where &w, int target, int have, int share) {
 }
 /* J sequences a lane, 64 J a step: what all have, then where target lies */
 template <int RT_, int J> DEV Where locate_among(const Call &c, int target) {
-    constexpr bool FEWR = RT_ != PG_MANY;
+    constexpr bool FEWR = RT_ == PG_FEW;
     const int lane = threadIdx.x & 63;
     pg_seq s[J];
     int units[J], n[J];
@@ -288,7 +288,7 @@ template <int RT_, int J> DEV Where locate_among(const Call &c, int target) {
     return w;
 }
 template <int RT_> DEV Where locate(const Call &c, int target) {
-    constexpr bool FEWR = RT_ != PG_MANY;
+    constexpr bool FEWR = RT_ == PG_FEW;
     if (c.B > 64)
         return locate_among<RT_, 4>(c, target);
     if (c.B > 1)
@@ -909,7 +909,9 @@ template <bool E4M3, int RB, int RG> DEV void attend_mid(const Call &c, unsigned
         auto flag_of = [&](int i) { /* i + 1 where the tile moves the reference */
             return __builtin_amdgcn_readfirstlane(*(lds_i32)(lds + M::FLAG + (i & 1) * 4));
         };
-        /* P of tile i from x, by the reference as it is */
+        /* P of tile i from x, by the reference as it is; rounded to bf16 for its product, as
+         * in the other forms (off by 2^-8 of a term at most): a second product, of what the
+         * rounding leaves, would add half to a tile's MFMAs, whose chain bounds it already */
         auto write_p = [&](int i) {
 #pragma unroll
             for (int rb = 0; rb < RB; rb++) {

@@ -199,8 +199,8 @@ __global__ __launch_bounds__(256, 2) void weigh_few_kernel(Weigh c) {
  * four products, and LDS holds four steps, of which three are on their way. Few blocks
  * of keys share their rows out among several workgroups, whose sums weigh_sum_kernel
  * adds up. Half a step's products go beside the exponentials of the half before. 4096
- * tokens on 8192 keys, 16 / 4 heads, bf16: 187 us with the sums' 4.5, 1.1 PFLOP/s, 84 %
- * of a large library product's rate on the same card (1.31). */
+ * tokens on 8192 keys, 16 / 4 heads, bf16, call after call: 202 us with the sums' 4.8,
+ * 1.02 PFLOP/s, 75 % of a large library product's rate in the same loop (1.37). */
 constexpr int WEIGH_KG = 4, WEIGH_AHEAD = 4, WEIGH_GROUPS = 1024, WEIGH_STEPS = 4;
 template <bool E4M3> DEV void weigh_many(const Weigh &c) {
     constexpr int KG = WEIGH_KG, STEP = 32; /* rows a step, in two halves */
@@ -478,7 +478,7 @@ static_assert(WEIGH_KG * PG == 256, "a thread a key of a block");
  * (ordered()); the least one kept is found by its digits of 11, 11 and 10 bits from the
  * top, each by a histogram in LDS of what has the digits before. Then positions are
  * counted in order: heavier ones, and of its equals the first. A chain of loads, LDS and
- * barriers: 1 x 8192 keys 12 us, 64 sequences of up to 4096, a workgroup a CU, 11. */
+ * barriers: 1 x 8192 keys 12 us, 64 sequences of up to 4096, a workgroup a CU, 9.5. */
 constexpr int SEL_T = 1024;
 struct Select {
     const float *w;
@@ -669,9 +669,10 @@ template <int E> __global__ __launch_bounds__(SEL_T) void select_kernel(Select c
  * lines or rows of a sequence and kv-head from the front to the back: positions ascend
  * and none is before the slot it goes to, so that all reads of a step are of slots that
  * no step before has written, and those of the step itself are done before its writes.
- * Bound by lines where few of a page are kept: 16 x 4096 keys to 1024, bf16, other pages, 33
- * to 43 us for 135 MB that move, of V^T's 128-byte lines a quarter. In place one sequence of
- * 8192 to 2048 takes 28, a chain of list, page ids, loads and stores a step. */
+ * Bound by lines where few of a page are kept: 16 sequences of up to 4096 keys (41972) to
+ * 1024 each, bf16, other pages, 43 us (the least of 20 33) for 187 MB, since all of V^T's
+ * lines of 128 bytes are read for a quarter or more of each. In place one sequence of 8192
+ * to 2048 takes 28, a chain of list, page ids, loads and stores a step. */
 constexpr int KEEP_STEP = 256; /* slots a step, 64 a wave (K) or each wave all (V^T) */
 constexpr int KEEP_VR = 8;     /* rows of V^T a wave */
 struct Keep {

@@ -457,7 +457,8 @@ def attention_paged(q, gate, gate_tok_stride, gate_head_stride, pages, page_tabl
     sequence are drafted tokens that see all keys before them and, of each other, those
     whose bits are set (row i's ancestors and its own: bit j % 64 of word j // 64 is new
     token j); no window. Where ws is less than a tree's workspace (tree=True), the call takes
-    one from torch's allocator. lse float32 [N, Hq] gets the softmax's log2 of the sum of 2^(q.k)."""
+    one from torch's allocator. lse float32 [N, Hq] gets the softmax's log2 of the sum of
+    2^(q.k)."""
     import torch
     dev, B = _paged_seqs(pages, page_table, kv_len, q_start)
     if (max_q | max_kv | window | sinks | gate_tok_stride | gate_head_stride) >> 31:
@@ -529,7 +530,8 @@ def kv_weights(q, lse, pages, page_table, q_start, kv_len, max_q, max_kv, weight
     """weights [pages, Hkv, 64] (float32, beside the pages' keys) of every key of the
     sequences that have new tokens: prev's, where given and the key is before the new
     tokens, plus what the rows q [N, Hq, 256] of the call gave it, with the lse [N, Hq]
-    of their attention, one without a window over the same keys. prev may be weights itself, to add in place; None starts anew.
+    of their attention, one without a window over the same keys. prev may be weights itself,
+    to add in place, but not overlap it otherwise; None starts anew.
     ws: uint8 device workspace of kv_weights_ws_bytes, of this call or a larger one; None
     takes one from torch's allocator where the call needs any."""
     import torch

@@ -393,8 +393,9 @@ int cujev_op_kv_keep(int kv_type, void *k_pages, void *vt_pages, float *k_scale,
  * Conv (width 4) + SiLU with taps before a segment taken from conv_in [C][3]
  * (NULL = zeros); own_base[n] = first token of n's segment. Outputs fp32
  * q, k [N][Hk][128] (l2-normalised, q * 128^-1/2), v [N][Hv][128], fp32
- * g, beta [N][Hv] (the scan keeps q, k, v at about 16 significant bits). conv_out (may be NULL) gets the last three pre-conv inputs
- * of tokens [0, seg0_len) as [C][3]. conv_w fp32 [C][4]. */
+ * g, beta [N][Hv] (the scan keeps q, k, v at about 16 significant bits). conv_out
+ * (may be NULL) gets the last three pre-conv inputs of tokens [0, seg0_len) as
+ * [C][3]. conv_w fp32 [C][4]. */
 int cujev_op_gdn_conv_prep(const void *proj, int proj_stride, const float *conv_w,
                            const float *conv_in, float *conv_out, int seg0_len,
                            const int32_t *own_base, const float *A_neg_exp,
